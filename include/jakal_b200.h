@@ -394,6 +394,95 @@ int jk_topk_reduce_backward_edges(const int64_t* indices, const void* state, con
 int jk_topk_to_dense(const float* w, const int64_t* indices, float* dense, int64_t rows, int64_t k,
                      int64_t n_cols, jk_stream_t stream);
 
+/* ---- training-step kernels --------------------------------------------------------
+ * The row and parameter operators around the propagation / transition operators in a training
+ * step: the apply step of a layer (sum = x + scale * delta, then a layer norm;
+ * progressive_b_example.py:71-99, 282-294), the loss over the query head's vocabulary and the
+ * clipping of the gradients. dtype codes JK_F32, JK_BF16, JK_F16; strides count elements from
+ * one row to the next (rows are contiguous inside); any alignment of a whole element. All
+ * arithmetic is f32 or wider; a result is rounded once, to its own type. Results do not depend
+ * on the order in which blocks run.
+ */
+
+/* Layer norm of sum = x + delta_scale * delta (delta NULL: of x):
+ *   mean = E[sum], rstd = 1 / sqrt(E[(sum - mean)^2] + eps), y = (sum - mean) * rstd * weight + bias
+ * x [rows, dim], delta [rows, dim] in dtype, weight / bias [dim] in param_dtype (NULL: 1 / 0);
+ * out: y and sum [rows, dim] contiguous in dtype (sum may be NULL; the statistics and y are of
+ * the unrounded sum), mean / rstd f32 [rows] (both or neither NULL). */
+int jk_layer_norm_forward(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride,
+                          float delta_scale, const void* weight, const void* bias, int param_dtype,
+                          int64_t rows, int64_t dim, int dtype, float eps, void* y, void* sum,
+                          float* mean, float* rstd, jk_stream_t stream);
+
+/* f32 elements of the workspace that jk_layer_norm_backward needs for its parameter gradients. */
+int64_t jk_layer_norm_backward_workspace(int64_t rows, int64_t dim);
+
+/* Backward of jk_layer_norm_forward. With n = (sum - mean) * rstd and u = grad_y * weight:
+ *   grad_x = rstd * (u - E[u] - n * E[u * n]) + grad_sum,  grad_delta = delta_scale * grad_x,
+ *   grad_weight = sum over rows of grad_y * n,             grad_bias = sum over rows of grad_y.
+ * grad_sum (NULL: 0) is the gradient that reaches sum from its other uses; grad_x, grad_delta
+ * [rows, dim] contiguous in dtype (grad_delta may be NULL); grad_weight and grad_bias [dim] in
+ * param_dtype (both or neither NULL), summed over fixed blocks of rows in a fixed order.
+ * workspace: jk_layer_norm_backward_workspace(rows, dim) floats, 16-byte aligned (may be NULL
+ * without parameter gradients). */
+int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* sum, int64_t sum_stride,
+                           const float* mean, const float* rstd, const void* weight, int param_dtype,
+                           const void* grad_sum, int64_t grad_sum_stride, float delta_scale, int64_t rows,
+                           int64_t dim, int dtype, void* grad_x, void* grad_delta, void* grad_weight,
+                           void* grad_bias, float* workspace, jk_stream_t stream);
+
+/* reduction codes of the cross entropy */
+#define JK_REDUCE_NONE 0
+#define JK_REDUCE_MEAN 1 /* over the rows whose target is not ignore_index */
+#define JK_REDUCE_SUM 2
+
+/* Bytes of the workspace of jk_cross_entropy_forward. */
+int64_t jk_cross_entropy_workspace(int64_t rows);
+
+/* Softmax cross entropy of logits [rows, vocab] (dtype) against targets int64 [rows]:
+ *   lse = log sum_j exp(z_j),  loss = lse - (1 - a) z_target - a E_j[z_j]   (a = label_smoothing)
+ * A row whose target is ignore_index is not read and has loss, lse and gradient 0; a target
+ * outside [0, vocab) gives its row a NaN loss and gradient (nothing is read there). Logits of
+ * -inf have probability 0; a row of nothing else has a NaN loss.
+ * out: losses f32 [rows] and lse f32 [rows] (each may be NULL), loss f32 scalar by `reduction`
+ * (NULL with JK_REDUCE_NONE; the mean over no row is NaN, the sum 0), and, when grad is not NULL
+ * (not with JK_REDUCE_NONE), grad [rows, vocab] in dtype, in the same pass over the logits:
+ *   grad = grad_scale * d loss / d logits = grad_scale * w * (softmax(z) - (1 - a) onehot - a / vocab)
+ * with w = 1 (sum) or 1 / number of rows that count (mean). grad may be the logits themselves.
+ * workspace: jk_cross_entropy_workspace(rows) bytes, 8-byte aligned. */
+int jk_cross_entropy_forward(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
+                             int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                             int reduction, float grad_scale, float* losses, float* lse, float* loss,
+                             void* grad, int64_t grad_stride, void* workspace, jk_stream_t stream);
+
+/* Gradient of the cross entropy from the lse that the forward pass kept:
+ *   grad = g * w * (exp(z - lse) - (1 - a) onehot - a / vocab)
+ * grad_loss: device f32, [rows] with JK_REDUCE_NONE (g per row, w = 1), else one value; grad
+ * [rows, vocab] in dtype (may be the logits); rows to ignore get zeros. */
+int jk_cross_entropy_backward(const float* grad_loss, const void* logits, int64_t logits_stride,
+                              const int64_t* targets, const float* lse, int64_t rows, int64_t vocab, int dtype,
+                              int64_t ignore_index, float label_smoothing, int reduction, void* grad,
+                              int64_t grad_stride, jk_stream_t stream);
+
+/* norm codes of jk_clip_grad_norm */
+#define JK_NORM_2 0
+#define JK_NORM_INF 1
+
+/* Bytes of the workspace of jk_clip_grad_norm. */
+int64_t jk_clip_grad_norm_workspace(void);
+
+/* Norm over all elements of `count` flat tensors, and their clipping:
+ *   total = sqrt(sum g^2) (JK_NORM_2; summed in f64, so squares neither overflow nor vanish) or
+ *           max |g| (JK_NORM_INF), NaN if any element is;
+ *   out_i = g_i * min(1, max_norm / (total + eps)).
+ * grads, outs, numels, dtypes, out_dtypes are HOST arrays of `count` entries that are read
+ * during the call; outs NULL: in place (then a coefficient of 1 writes nothing). clip 0: the norm
+ * alone (outs, max_norm, eps unused). total: device f32 scalar. workspace:
+ * jk_clip_grad_norm_workspace() bytes, 16-byte aligned. Tensors must not overlap. */
+int jk_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* numels, const int* dtypes,
+                      const int* out_dtypes, int64_t count, int norm_kind, int clip, float max_norm, float eps,
+                      float* total, void* workspace, jk_stream_t stream);
+
 /* Failure-path test entry (no reference counterpart): jk_propagation_window_forward
  * (softsign, no bias) with a producer warp that issues no load and no MMA, so every consumer
  * wait runs into its bound (about 2 s): the kernel sets the device error word, releases its

@@ -1,0 +1,105 @@
+// Element types, 16-byte packs and reductions of the row kernels (layer norm, cross entropy,
+// gradient clipping). Every kernel computes in f32 or wider and rounds a result once.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace jk {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// 16 bytes of T: kPack<T> elements.
+template <typename T>
+constexpr int kPack = 16 / static_cast<int>(sizeof(T));
+
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[4], float) {
+  f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);  // bf16 is the upper half of an f32
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[8], __half) {
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = __half22float2(h[i]);
+    f[2 * i] = p.x, f[2 * i + 1] = p.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[kPack<T>]) {
+  unpack(u, f, T());
+}
+
+__device__ __forceinline__ uint4 pack(const float (&f)[4], float) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], __nv_bfloat16) {
+  uint4 u;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  return u;
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], __half) {
+  uint4 u;
+  __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+  return u;
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&f)[kPack<T>]) {
+  return pack(f, T());
+}
+
+__device__ __forceinline__ float warp_sum32(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Programmatic dependent launch: a kernel launched with the attribute may begin while the one
+// before it in the stream still runs; grid_dependency_wait returns when that one has finished
+// and its writes are visible. Without the attribute both are no-ops.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Runs `body` with a type alias T for the dtype code.
+#define JK_WITH_TYPE(code, T, ...)                                       \
+  do {                                                                   \
+    if ((code) == JK_F32) {                                              \
+      using T = float;                                                   \
+      __VA_ARGS__;                                                       \
+    } else if ((code) == JK_BF16) {                                      \
+      using T = __nv_bfloat16;                                           \
+      __VA_ARGS__;                                                       \
+    } else {                                                             \
+      using T = __half;                                                  \
+      __VA_ARGS__;                                                       \
+    }                                                                    \
+  } while (0)
+
+inline bool float_dtype(int code) { return code == JK_F32 || code == JK_BF16 || code == JK_F16; }
+inline int64_t dtype_bytes(int code) { return code == JK_F32 ? 4 : 2; }
+
+}  // namespace jk

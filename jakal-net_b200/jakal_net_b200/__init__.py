@@ -42,6 +42,9 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import JakalB200Error, check, load
+from .training import (clip_grad_norm_, cross_entropy, cross_entropy_backward_cuda, cross_entropy_forward_cuda,
+                       cross_entropy_with_grad_cuda, grad_norm, layer_norm, layer_norm_backward_cuda,
+                       layer_norm_forward_cuda)
 
 __all__ = [
     "supported_ops",
@@ -58,6 +61,15 @@ __all__ = [
     "lowrank_project",
     "lowrank_project_pair",
     "topk_aggregate",
+    "layer_norm",
+    "layer_norm_forward_cuda",
+    "layer_norm_backward_cuda",
+    "cross_entropy",
+    "cross_entropy_forward_cuda",
+    "cross_entropy_backward_cuda",
+    "cross_entropy_with_grad_cuda",
+    "grad_norm",
+    "clip_grad_norm_",
     "JakalB200Error",
 ]
 

@@ -26,6 +26,9 @@ JK_ERR_ALIGNMENT = -8
 JK_F32, JK_BF16, JK_F16, JK_BF16X3 = 0, 1, 2, 3
 JK_SOFTSIGN, JK_SIGNED_ABS_SOFTMAX, JK_SIGNED_ENTMAX15, JK_SOFTMAX = 0, 1, 2, 3
 
+JK_REDUCE_NONE, JK_REDUCE_MEAN, JK_REDUCE_SUM = 0, 1, 2
+JK_NORM_2, JK_NORM_INF = 0, 1
+
 JK_HEADS_MAX, JK_HEADS_SMOOTHMAX, JK_HEADS_SIGNED_SMOOTHMAX = 0, 1, 2
 
 
@@ -114,6 +117,37 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i32, _i32, _p],                       # dtype, out_dtype, stream
     ),
     "jk_topk_to_dense": (_i32, [_p, _p, _p, _i64, _i64, _i64, _p]),
+    "jk_layer_norm_forward": (
+        _i32,
+        [_p, _i64, _p, _i64, _f32,              # x, x_stride, delta, delta_stride, delta_scale
+         _p, _p, _i32, _i64, _i64, _i32, _f32,  # weight, bias, param_dtype, rows, dim, dtype, eps
+         _p, _p, _p, _p, _p],                   # y, sum, mean, rstd, stream
+    ),
+    "jk_layer_norm_backward_workspace": (_i64, [_i64, _i64]),
+    "jk_layer_norm_backward": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _p, _p, _i32,  # grad_y, stride, sum, stride, mean, rstd, weight, param_dtype
+         _p, _i64, _f32, _i64, _i64, _i32,      # grad_sum, stride, delta_scale, rows, dim, dtype
+         _p, _p, _p, _p, _p, _p],               # grad_x, grad_delta, grad_weight, grad_bias, workspace, stream
+    ),
+    "jk_cross_entropy_workspace": (_i64, [_i64]),
+    "jk_cross_entropy_forward": (
+        _i32,
+        [_p, _i64, _p, _i64, _i64, _i32, _i64,  # logits, stride, targets, rows, vocab, dtype, ignore_index
+         _f32, _i32, _f32, _p, _p, _p,          # label_smoothing, reduction, grad_scale, losses, lse, loss
+         _p, _i64, _p, _p],                     # grad, grad_stride, workspace, stream
+    ),
+    "jk_cross_entropy_backward": (
+        _i32,
+        [_p, _p, _i64, _p, _p, _i64, _i64, _i32,  # grad_loss, logits, stride, targets, lse, rows, vocab, dtype
+         _i64, _f32, _i32, _p, _i64, _p],         # ignore_index, label_smoothing, reduction, grad, stride, stream
+    ),
+    "jk_clip_grad_norm_workspace": (_i64, []),
+    "jk_clip_grad_norm": (
+        _i32,
+        [_p, _p, _p, _p, _p, _i64, _i32, _i32,  # grads, outs, numels, dtypes, out_dtypes, count, norm_kind, clip
+         _f32, _f32, _p, _p, _p],               # max_norm, eps, total, workspace, stream
+    ),
     "jk_debug_window_stalled_producer": (
         _i32,
         [_p, _p, _i64, _i64, _i64, _i64, _i32,  # row_proj, col_proj, B, n_rows, n_cols, rp, proj_dtype

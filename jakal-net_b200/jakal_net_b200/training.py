@@ -1,0 +1,504 @@
+"""Training-step operators around the propagation / transition operators: the layer norm of an
+apply step, the loss over the query head's vocabulary, and the clipping of the gradients.
+
+A Jakal-Net training step applies every operator's delta to its layer as
+``LayerNorm(x + scale * delta)`` (progressive_b_example.py:71-99, 282-294), ends in a softmax
+cross entropy over the vocabulary and clips the global gradient norm before the optimizer.
+The functions come in two forms, as the other training operators of this package do:
+
+* ``*_cuda`` entry points over plain tensors (no autograd graph): ``layer_norm_forward_cuda``,
+  ``layer_norm_backward_cuda``, ``cross_entropy_forward_cuda``, ``cross_entropy_backward_cuda``,
+  ``cross_entropy_with_grad_cuda``, ``grad_norm``, ``clip_grad_norm_``;
+* ``layer_norm`` and ``cross_entropy``, which autograd differentiates through those.
+
+Inputs are CUDA tensors in f32, bf16 or f16, rows contiguous inside (other layouts are copied
+first); arithmetic and sums are f32 or wider whatever autocast says, and a result keeps its
+input's type. Everything runs on the current stream, allocates through torch and reads nothing
+back, so calls can be captured into a CUDA graph. Results are the same from run to run.
+"""
+from __future__ import annotations
+
+import array
+import math
+from typing import Iterable, Optional, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._lib import check, load
+
+__all__ = [
+    "layer_norm",
+    "layer_norm_forward_cuda",
+    "layer_norm_backward_cuda",
+    "cross_entropy",
+    "cross_entropy_forward_cuda",
+    "cross_entropy_backward_cuda",
+    "cross_entropy_with_grad_cuda",
+    "grad_norm",
+    "clip_grad_norm_",
+]
+
+_LIBRARY = load()
+_DTYPE_CODE = {torch.float32: _lib.JK_F32, torch.bfloat16: _lib.JK_BF16, torch.float16: _lib.JK_F16}
+_REDUCTION = {"none": _lib.JK_REDUCE_NONE, "mean": _lib.JK_REDUCE_MEAN, "sum": _lib.JK_REDUCE_SUM}
+
+
+# ----------------------------------------------------------------------------- helpers
+def _check_input(name: str, t: Tensor) -> int:
+    """The dtype code of a CUDA float tensor; anything else raises."""
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor in the b200_sm100a backend (got {t.device}).")
+    code = _DTYPE_CODE.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{name}: unsupported dtype {t.dtype}")
+    return code
+
+
+def _same(name: str, t: Tensor, like: Tensor, shape=None) -> None:
+    """t has like's device and dtype and the given shape (like's by default)."""
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
+    if t.dtype != like.dtype:
+        raise RuntimeError(f"{name} has dtype {t.dtype}, expected {like.dtype}")
+    if t.shape != (like.shape if shape is None else shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape if shape is None else shape)}")
+
+
+def _rows(t: Tensor) -> tuple[Tensor, int]:
+    """(t, elements from one row to the next), rows along the last dim: t itself where its rows
+    are contiguous inside and equally spaced (a slice of wider rows, an expanded row), else a
+    contiguous copy."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    t = t.detach()
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        try:
+            return t, t.view(-1, t.shape[-1]).stride(0)
+        except RuntimeError:  # leading dims that no single stride spans
+            pass
+    return t.contiguous(), t.shape[-1]
+
+
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _written(tensors: list[Tensor]) -> None:
+    """Tells autograd that the kernels wrote over these tensors (a value kept for a backward
+    pass is then seen to be stale)."""
+    if tensors and not tensors[0].is_inference():
+        torch.autograd.graph.increment_version(tensors)
+
+
+class _On:
+    """Makes `device` current for the block where it is not."""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self):
+        self.guard = None
+        if torch._C._cuda_getDevice() != self.device.index:
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _param(name: str, p: Optional[Tensor], x: Tensor, dim: int) -> Optional[Tensor]:
+    if p is None:
+        return None
+    _check_input(name, p)
+    if p.device != x.device:
+        raise RuntimeError(f"{name} is on {p.device}, expected {x.device}")
+    if p.shape != (dim,):
+        raise ValueError(f"{name} has shape {tuple(p.shape)}, expected {(dim,)}")
+    return p if p.is_contiguous() else p.detach().contiguous()
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+# ----------------------------------------------------------------------------- layer norm
+def layer_norm_forward_cuda(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+                            eps: float = 1e-5, delta: Optional[Tensor] = None, delta_scale: float = 1.0):
+    """Layer norm over the last dim of ``sum = x + delta_scale * delta`` (delta None: of x).
+
+    Returns (y, sum, mean, rstd): y and sum in x's dtype and shape (sum is x itself without a
+    delta), mean and rstd f32 of x's leading shape, for ``layer_norm_backward_cuda``. y is
+    normalised from the sum before it is rounded. delta has x's dtype and shape; weight and bias
+    are [dim], of one dtype, x's or another."""
+    code = _check_input("x", x)
+    if x.dim() == 0:
+        raise ValueError("x must have at least one dim")
+    dim = x.shape[-1]
+    if dim == 0:
+        raise ValueError("the normalised dim is empty")
+    weight, bias = _param("weight", weight, x, dim), _param("bias", bias, x, dim)
+    some = weight if weight is not None else bias
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError(f"weight and bias have different dtypes ({weight.dtype}, {bias.dtype})")
+    xr, x_stride = _rows(x)
+    dr, d_stride = None, 0
+    if delta is not None:
+        _same("delta", delta, x)
+        dr, d_stride = _rows(delta)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = x if delta is None else torch.empty_like(y)
+    stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean, rstd = stats.unbind(0)
+    with _On(x.device):
+        check(
+            _LIBRARY.jk_layer_norm_forward(
+                xr.data_ptr(), x_stride, _ptr(dr), d_stride, delta_scale, _ptr(weight), _ptr(bias),
+                code if some is None else _DTYPE_CODE[some.dtype], mean.numel(), dim, code, eps, y.data_ptr(),
+                None if delta is None else total.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(x.device)),
+            "jk_layer_norm_forward",
+        )
+    return y, total, mean, rstd
+
+
+def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Tensor, weight: Optional[Tensor] = None,
+                             grad_sum: Optional[Tensor] = None, delta_scale: float = 1.0, param_grads: bool = True):
+    """Backward of ``layer_norm_forward_cuda`` from the sum and statistics that it returned.
+
+    Returns (grad_x, grad_delta, grad_weight, grad_bias). grad_sum is the gradient that reaches
+    the sum from its other uses (the residual stream); grad_delta is grad_x itself when
+    delta_scale is 1. The parameter gradients have weight's dtype (the sum's without a weight);
+    param_grads=False returns None for them."""
+    code = _check_input("sum", sum)
+    if sum.dim() == 0 or sum.shape[-1] == 0:
+        raise ValueError("sum must have a last dim that is not empty")
+    dim = sum.shape[-1]
+    _same("grad_y", grad_y, sum)
+    weight = _param("weight", weight, sum, dim)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if not isinstance(t, Tensor) or t.dtype != torch.float32 or t.device != sum.device:
+            raise RuntimeError(f"{name} must be an f32 tensor on {sum.device}")
+        if t.shape != sum.shape[:-1]:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(sum.shape[:-1])}")
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    gy, gy_stride = _rows(grad_y)
+    hr, h_stride = _rows(sum)
+    gs, gs_stride = None, 0
+    if grad_sum is not None:
+        _same("grad_sum", grad_sum, sum)
+        gs, gs_stride = _rows(grad_sum)
+    rows = mean.numel()
+    grad_x = torch.empty(sum.shape, dtype=sum.dtype, device=sum.device)
+    grad_delta = grad_x if delta_scale == 1.0 else torch.empty_like(grad_x)
+    grad_weight = grad_bias = work = None
+    pcode = code if weight is None else _DTYPE_CODE[weight.dtype]
+    if param_grads:
+        ptype = sum.dtype if weight is None else weight.dtype
+        grad_weight, grad_bias = torch.empty((2, dim), dtype=ptype, device=sum.device).unbind(0)
+        work = torch.empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),), dtype=torch.float32,
+                           device=sum.device)
+    with _On(sum.device):
+        check(
+            _LIBRARY.jk_layer_norm_backward(
+                gy.data_ptr(), gy_stride, hr.data_ptr(), h_stride, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), pcode,
+                _ptr(gs), gs_stride, delta_scale, rows, dim, code, grad_x.data_ptr(),
+                None if grad_delta is grad_x else grad_delta.data_ptr(), _ptr(grad_weight), _ptr(grad_bias), _ptr(work),
+                _stream(sum.device)),
+            "jk_layer_norm_backward",
+        )
+    return grad_x, grad_delta, grad_weight, grad_bias
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, delta, delta_scale):
+        y, total, mean, rstd = layer_norm_forward_cuda(x, weight, bias, eps, delta, delta_scale)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(total, mean, rstd, weight)
+        ctx.delta_scale, ctx.has_delta = delta_scale, delta is not None
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return (y, total) if delta is not None else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y, grad_sum=None):
+        total, mean, rstd, weight = ctx.saved_tensors
+        need_x, need_w, need_b, _, need_delta, _ = ctx.needs_input_grad
+        if grad_y is None and grad_sum is None:
+            return (None,) * 6
+        if grad_y is None:  # only the residual stream was used: the norm's part is zero
+            grad_y = torch.zeros_like(total)
+        gx, gd, gw, gb = layer_norm_backward_cuda(grad_y, total, mean, rstd, weight, grad_sum, ctx.delta_scale,
+                                                  param_grads=need_w or need_b)
+        if need_b and gb.dtype != ctx.bias_dtype:  # no weight: the gradient came in the sum's dtype
+            gb = gb.to(ctx.bias_dtype)
+        return gx if need_x else None, gw if need_w else None, gb if need_b else None, None, gd if need_delta else None, None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
+               delta: Optional[Tensor] = None, delta_scale: float = 1.0):
+    """Differentiable layer norm of an apply step: y, or (y, sum) when a delta is given."""
+    return _LayerNorm.apply(x, weight, bias, float(eps), delta, float(delta_scale))
+
+
+# ----------------------------------------------------------------------------- cross entropy
+def _loss_inputs(logits: Tensor, targets: Tensor, reduction: str):
+    code = _check_input("logits", logits)
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError("logits must have a last dim (the vocabulary) that is not empty")
+    if not isinstance(targets, Tensor):
+        raise TypeError("targets must be a tensor")
+    if targets.device != logits.device:
+        raise RuntimeError(f"targets are on {targets.device}, expected {logits.device}")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"targets: unsupported dtype {targets.dtype} (int64 or int32)")
+    if targets.shape != logits.shape[:-1]:
+        raise ValueError(f"targets have shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
+    kind = _REDUCTION.get(reduction)
+    if kind is None:
+        raise ValueError(f"unknown reduction {reduction!r} (none, mean or sum)")
+    if targets.dtype != torch.int64 or not targets.is_contiguous():
+        targets = targets.to(torch.int64).contiguous()
+    lr, stride = _rows(logits)
+    return code, targets, kind, lr, stride
+
+
+def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, grad_scale, want_lse, grad, in_place=False):
+    code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
+    rows, dev = targets.numel(), logits.device
+    lse = losses = None
+    if want_lse:
+        lse = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    if kind == _lib.JK_REDUCE_NONE:
+        loss = losses = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    else:
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+    work = torch.empty((_LIBRARY.jk_cross_entropy_workspace(rows),), dtype=torch.uint8, device=dev)
+    if in_place:
+        grad_ptr, grad_stride = lr.data_ptr(), stride
+    else:
+        grad_ptr, grad_stride = _ptr(grad), logits.shape[-1]
+    with _On(dev):
+        check(
+            _LIBRARY.jk_cross_entropy_forward(
+                lr.data_ptr(), stride, targets.data_ptr(), rows, logits.shape[-1], code, ignore_index, label_smoothing,
+                kind, grad_scale, _ptr(losses), _ptr(lse), None if losses is not None else loss.data_ptr(), grad_ptr,
+                grad_stride, work.data_ptr(), _stream(dev)),
+            "jk_cross_entropy_forward",
+        )
+    return loss, lse
+
+
+def cross_entropy_forward_cuda(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
+                               reduction: str = "mean"):
+    """Softmax cross entropy of logits [..., vocab] against int64 (or int32) targets [...].
+
+    Returns (loss, lse): loss f32, a scalar for reduction "mean" (over the targets that are not
+    ignore_index) or "sum", of targets' shape for "none"; lse f32 of targets' shape, the rows'
+    log-sum-exp, which ``cross_entropy_backward_cuda`` takes. A row to ignore has loss and lse 0
+    and is not read. A target outside the vocabulary gives NaN."""
+    return _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, 1.0, True, None)
+
+
+def cross_entropy_with_grad_cuda(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
+                                 reduction: str = "mean", grad_scale: float = 1.0, in_place: bool = False):
+    """The loss ("mean" or "sum") and, in the same pass over the logits, their gradient.
+
+    Returns (loss, grad): grad = grad_scale * d loss / d logits in logits' dtype (grad_scale: a
+    loss scaler's factor), for ``logits.backward(grad)`` or a head's own backward. in_place
+    writes it over the logits, which must then have rows that are contiguous inside, equally
+    spaced and apart."""
+    if reduction == "none":
+        raise ValueError("a gradient needs a reduced loss (mean or sum)")
+    _check_input("logits", logits)
+    if in_place:
+        if logits.dim() == 0:
+            raise ValueError("logits must have a last dim (the vocabulary) that is not empty")
+        if torch.is_grad_enabled() and logits.requires_grad:
+            raise RuntimeError("in_place needs detached logits: autograd keeps their values")
+        lr, stride = _rows(logits)
+        if lr.data_ptr() != logits.data_ptr() or (logits.numel() > logits.shape[-1] and stride < logits.shape[-1]):
+            raise ValueError("in_place needs logits whose rows are contiguous inside, equally spaced and apart")
+        loss, _ = _cross_entropy(lr, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
+                                 False, None, in_place=True)
+        _written([logits])
+        return loss, logits
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    loss, _ = _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
+                             False, grad)
+    return loss, grad
+
+
+def cross_entropy_backward_cuda(grad_loss: Tensor, logits: Tensor, targets: Tensor, lse: Tensor, ignore_index: int = -100,
+                                label_smoothing: float = 0.0, reduction: str = "mean"):
+    """Gradient of ``cross_entropy_forward_cuda`` with respect to the logits, in their dtype,
+    from the lse that it returned and the loss's gradient (a scalar, or of targets' shape for
+    reduction "none")."""
+    code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
+    for name, t in (("lse", lse), ("grad_loss", grad_loss)):
+        if not isinstance(t, Tensor) or t.device != logits.device:
+            raise RuntimeError(f"{name} must be a tensor on {logits.device}")
+    if lse.dtype != torch.float32 or lse.shape != targets.shape:
+        raise ValueError(f"lse must be f32 of shape {tuple(targets.shape)}")
+    if grad_loss.shape != targets.shape if kind == _lib.JK_REDUCE_NONE else grad_loss.numel() != 1:
+        raise ValueError(f"grad_loss has shape {tuple(grad_loss.shape)}, which does not fit reduction {reduction!r}")
+    gl = grad_loss.detach().to(torch.float32).contiguous()
+    lse = lse.contiguous()
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    with _On(logits.device):
+        check(
+            _LIBRARY.jk_cross_entropy_backward(
+                gl.data_ptr(), lr.data_ptr(), stride, targets.data_ptr(), lse.data_ptr(), targets.numel(),
+                logits.shape[-1], code, int(ignore_index), float(label_smoothing), kind, grad.data_ptr(), logits.shape[-1],
+                _stream(logits.device)),
+            "jk_cross_entropy_backward",
+        )
+    return grad
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, ignore_index, label_smoothing, reduction):
+        loss, lse = cross_entropy_forward_cuda(logits, targets, ignore_index, label_smoothing, reduction)
+        ctx.save_for_backward(logits, targets, lse)
+        ctx.options = (ignore_index, label_smoothing, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, targets, lse = ctx.saved_tensors
+        return cross_entropy_backward_cuda(grad_loss, logits, targets, lse, *ctx.options), None, None, None, None
+
+
+def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
+                  reduction: str = "mean") -> Tensor:
+    """Differentiable softmax cross entropy (f32): ``cross_entropy_forward_cuda`` and, in the
+    backward pass, ``cross_entropy_backward_cuda``. A loop that owns its backward pass reads the
+    logits once less with ``cross_entropy_with_grad_cuda``."""
+    return _CrossEntropy.apply(logits, targets, int(ignore_index), float(label_smoothing), reduction)
+
+
+# ----------------------------------------------------------------------------- gradient norm
+_NORM = {2.0: _lib.JK_NORM_2, math.inf: _lib.JK_NORM_INF}
+
+
+def _flat(t: Tensor) -> bool:
+    """Whether t's elements fill one block of memory, in whatever order of its dims."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _gradients(grads) -> list[Tensor]:
+    tensors = [grads] if isinstance(grads, Tensor) else [g for g in grads if g is not None]
+    for i, g in enumerate(tensors):
+        _check_input(f"gradient {i}", g)
+        if g.device != tensors[0].device:
+            raise RuntimeError(f"gradient {i} is on {g.device}, expected {tensors[0].device}")
+    return tensors
+
+
+def _run_clip(tensors, outs, norm_type, clip, max_norm):
+    kind = _NORM.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"unsupported norm_type {norm_type} (2 or inf)")
+    dev = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
+    total = torch.empty((), dtype=torch.float32, device=dev)
+    work = torch.empty((_LIBRARY.jk_clip_grad_norm_workspace(),), dtype=torch.uint8, device=dev)
+    # a gradient that does not fill one block of memory is worked on in a contiguous copy
+    back = []
+    if clip:
+        for t in tensors if outs is None else outs:
+            if not t.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+                raise ValueError("a tensor to write has elements that share memory (an expanded tensor)")
+    src = list(tensors)
+    dst = None if outs is None else list(outs)
+    for i, g in enumerate(src):
+        flat = _flat(g)
+        if dst is None:
+            if not flat:
+                src[i] = g.detach().contiguous()
+                if clip:
+                    back.append((g, src[i]))
+        else:
+            o = dst[i]
+            if not flat or o.stride() != g.stride():
+                src[i] = g.detach().contiguous()
+                if not o.is_contiguous():
+                    dst[i] = torch.empty(o.shape, dtype=o.dtype, device=dev)
+                    back.append((o, dst[i]))
+    n = len(src)
+    ptrs = array.array("Q", [t.data_ptr() for t in src])
+    numels = array.array("q", [t.numel() for t in src])
+    codes = array.array("i", [_DTYPE_CODE[t.dtype] for t in src])
+    outs_at = codes_at = None
+    if dst is not None:
+        out_ptrs = array.array("Q", [t.data_ptr() for t in dst])
+        out_codes = array.array("i", [_DTYPE_CODE[t.dtype] for t in dst])
+        outs_at, codes_at = out_ptrs.buffer_info()[0], out_codes.buffer_info()[0]
+    if clip:
+        written = [p for p, m in zip(ptrs if dst is None else out_ptrs, numels) if m]
+        if len(set(written)) != len(written):
+            raise ValueError("a tensor is given twice: it would be scaled twice")
+    with _On(dev):
+        check(
+            _LIBRARY.jk_clip_grad_norm(ptrs.buffer_info()[0], outs_at, numels.buffer_info()[0], codes.buffer_info()[0],
+                                       codes_at, n, kind, int(clip), max_norm, 1e-6, total.data_ptr(), work.data_ptr(),
+                                       _stream(dev)),
+            "jk_clip_grad_norm",
+        )
+    if back:
+        with torch.no_grad():
+            for to, made in back:
+                to.copy_(made)
+    if clip:
+        _written(tensors if outs is None else outs)
+    return total
+
+
+def grad_norm(grads: Union[Tensor, Iterable[Optional[Tensor]]], norm_type: float = 2.0) -> Tensor:
+    """Norm (2 or inf) over all elements of the gradients together, an f32 scalar on their
+    device. The squares are summed in f64, so the norm is finite wherever it fits f32."""
+    return _run_clip(_gradients(grads), None, norm_type, False, 0.0)
+
+
+def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: float, norm_type: float = 2.0,
+                    out: Optional[Iterable[Tensor]] = None, error_if_nonfinite: bool = False) -> Tensor:
+    """Scales the gradients by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm that
+    they had (f32 scalar on their device, as ``grad_norm``).
+
+    grads: one tensor or several (None is skipped), in f32, bf16, f16 or a mix; scaled in place,
+    or into `out`, one tensor for each gradient, of its shape and any of the three dtypes (f32
+    master gradients of bf16 ones, say). Tensors must not overlap. A gradient that holds NaN
+    makes all of them NaN, one that holds an infinity makes the others 0, as the formula has it;
+    error_if_nonfinite raises instead, after reading the norm back, with the gradients scaled."""
+    tensors = _gradients(grads)
+    outs = None
+    if out is not None:
+        outs = [out] if isinstance(out, Tensor) else list(out)
+        if len(outs) != len(tensors):
+            raise ValueError(f"out has {len(outs)} tensors for {len(tensors)} gradients")
+        for i, (o, g) in enumerate(zip(outs, tensors)):
+            _check_input(f"out {i}", o)
+            if o.device != g.device:
+                raise RuntimeError(f"out {i} is on {o.device}, expected {g.device}")
+            if o.shape != g.shape:
+                raise ValueError(f"out {i} has shape {tuple(o.shape)}, expected {tuple(g.shape)}")
+    total = _run_clip(tensors, outs, norm_type, True, float(max_norm))
+    if error_if_nonfinite and not math.isfinite(total.item()):
+        raise RuntimeError(f"the norm of the gradients is {total.item()}")
+    return total
