@@ -389,12 +389,11 @@ def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100, lab
 
 # ----------------------------------------------------------------------------- gradient norm
 _NORM = {2.0: _lib.JK_NORM_2, math.inf: _lib.JK_NORM_INF}
+_CLIP_WORKSPACE = int(_LIBRARY.jk_clip_grad_norm_workspace())
 
 
 def _flat(t: Tensor) -> bool:
     """Whether t's elements fill one block of memory, in whatever order of its dims."""
-    if t.is_contiguous():
-        return True
     expected = 1
     for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
         if stride != expected:
@@ -403,13 +402,26 @@ def _flat(t: Tensor) -> bool:
     return True
 
 
-def _gradients(grads) -> list[Tensor]:
+def _gradients(grads, name: str) -> list[Tensor]:
     tensors = [grads] if isinstance(grads, Tensor) else [g for g in grads if g is not None]
-    for i, g in enumerate(tensors):
-        _check_input(f"gradient {i}", g)
-        if g.device != tensors[0].device:
-            raise RuntimeError(f"gradient {i} is on {g.device}, expected {tensors[0].device}")
+    if tensors:
+        # one look at all of them; what is wrong with which is only sought when something is
+        dev = tensors[0].device if isinstance(tensors[0], Tensor) else None
+        if not (all(isinstance(t, Tensor) for t in tensors) and {t.device for t in tensors} == {dev}
+                and dev.type == "cuda" and _DTYPE_CODE.keys() >= {t.dtype for t in tensors}):
+            for i, t in enumerate(tensors):
+                _check_input(f"{name} {i}", t)
+                if t.device != dev:
+                    raise RuntimeError(f"{name} {i} is on {t.device}, expected {dev}")
     return tensors
+
+
+def _addresses(tensors: list[Tensor]) -> array.array:
+    return array.array("Q", [t.data_ptr() for t in tensors])
+
+
+def _codes(tensors: list[Tensor]) -> array.array:
+    return array.array("i", [_DTYPE_CODE[t.dtype] for t in tensors])
 
 
 def _run_clip(tensors, outs, norm_type, clip, max_norm):
@@ -417,48 +429,32 @@ def _run_clip(tensors, outs, norm_type, clip, max_norm):
     if kind is None:
         raise ValueError(f"unsupported norm_type {norm_type} (2 or inf)")
     dev = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
-    total = torch.empty((), dtype=torch.float32, device=dev)
-    work = torch.empty((_LIBRARY.jk_clip_grad_norm_workspace(),), dtype=torch.uint8, device=dev)
-    # a gradient that does not fill one block of memory is worked on in a contiguous copy
-    back = []
-    if clip:
-        for t in tensors if outs is None else outs:
-            if not t.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
-                raise ValueError("a tensor to write has elements that share memory (an expanded tensor)")
-    src = list(tensors)
-    dst = None if outs is None else list(outs)
-    for i, g in enumerate(src):
-        flat = _flat(g)
-        if dst is None:
-            if not flat:
-                src[i] = g.detach().contiguous()
-                if clip:
-                    back.append((g, src[i]))
-        else:
-            o = dst[i]
-            if not flat or o.stride() != g.stride():
-                src[i] = g.detach().contiguous()
-                if not o.is_contiguous():
-                    dst[i] = torch.empty(o.shape, dtype=o.dtype, device=dev)
-                    back.append((o, dst[i]))
-    n = len(src)
-    ptrs = array.array("Q", [t.data_ptr() for t in src])
+    src, dst, back = tensors, outs, []
+    if not (all(t.is_contiguous() for t in tensors) and (outs is None or all(t.is_contiguous() for t in outs))):
+        if clip:
+            for t in tensors if outs is None else outs:
+                if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+                    raise ValueError("a tensor to write has elements that share memory (an expanded tensor)")
+        src, dst, back = _blocks(tensors, outs, clip)
+    ptrs, codes = _addresses(src), _codes(src)
     numels = array.array("q", [t.numel() for t in src])
-    codes = array.array("i", [_DTYPE_CODE[t.dtype] for t in src])
-    outs_at = codes_at = None
+    out_ptrs = out_codes = None
     if dst is not None:
-        out_ptrs = array.array("Q", [t.data_ptr() for t in dst])
-        out_codes = array.array("i", [_DTYPE_CODE[t.dtype] for t in dst])
-        outs_at, codes_at = out_ptrs.buffer_info()[0], out_codes.buffer_info()[0]
+        out_ptrs, out_codes = _addresses(dst), _codes(dst)
     if clip:
-        written = [p for p, m in zip(ptrs if dst is None else out_ptrs, numels) if m]
-        if len(set(written)) != len(written):
-            raise ValueError("a tensor is given twice: it would be scaled twice")
+        written = ptrs if dst is None else out_ptrs
+        if len(set(written)) != len(written):  # empty tensors may share an address
+            some = [p for p, n in zip(written, numels) if n]
+            if len(set(some)) != len(some):
+                raise ValueError("a tensor is given twice: it would be scaled twice")
+    total = torch.empty((), dtype=torch.float32, device=dev)
+    work = torch.empty((_CLIP_WORKSPACE,), dtype=torch.uint8, device=dev)
     with _On(dev):
         check(
-            _LIBRARY.jk_clip_grad_norm(ptrs.buffer_info()[0], outs_at, numels.buffer_info()[0], codes.buffer_info()[0],
-                                       codes_at, n, kind, int(clip), max_norm, 1e-6, total.data_ptr(), work.data_ptr(),
-                                       _stream(dev)),
+            _LIBRARY.jk_clip_grad_norm(ptrs.buffer_info()[0], None if dst is None else out_ptrs.buffer_info()[0],
+                                       numels.buffer_info()[0], codes.buffer_info()[0],
+                                       None if dst is None else out_codes.buffer_info()[0], len(src), kind, clip, max_norm,
+                                       1e-6, total.data_ptr(), work.data_ptr(), _stream(dev)),
             "jk_clip_grad_norm",
         )
     if back:
@@ -470,10 +466,31 @@ def _run_clip(tensors, outs, norm_type, clip, max_norm):
     return total
 
 
+def _blocks(tensors, outs, clip):
+    """(gradients, outs, copies to make after): a tensor that does not fill one block of memory is
+    worked on in a contiguous copy, and an out whose elements lie in another order than its
+    gradient's is written through one."""
+    src, back = list(tensors), []
+    dst = None if outs is None else list(outs)
+    for i, g in enumerate(src):
+        flat = _flat(g)
+        if dst is None:
+            if not flat:
+                src[i] = g.detach().contiguous()
+                if clip:
+                    back.append((g, src[i]))
+        elif not flat or dst[i].stride() != g.stride():
+            src[i] = g.detach().contiguous()
+            if not dst[i].is_contiguous():
+                back.append((dst[i], torch.empty(g.shape, dtype=dst[i].dtype, device=g.device)))
+                dst[i] = back[-1][1]
+    return src, dst, back
+
+
 def grad_norm(grads: Union[Tensor, Iterable[Optional[Tensor]]], norm_type: float = 2.0) -> Tensor:
     """Norm (2 or inf) over all elements of the gradients together, an f32 scalar on their
     device. The squares are summed in f64, so the norm is finite wherever it fits f32."""
-    return _run_clip(_gradients(grads), None, norm_type, False, 0.0)
+    return _run_clip(_gradients(grads, "gradient"), None, norm_type, 0, 0.0)
 
 
 def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: float, norm_type: float = 2.0,
@@ -486,19 +503,18 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: 
     master gradients of bf16 ones, say). Tensors must not overlap. A gradient that holds NaN
     makes all of them NaN, one that holds an infinity makes the others 0, as the formula has it;
     error_if_nonfinite raises instead, after reading the norm back, with the gradients scaled."""
-    tensors = _gradients(grads)
+    tensors = _gradients(grads, "gradient")
     outs = None
     if out is not None:
-        outs = [out] if isinstance(out, Tensor) else list(out)
+        outs = _gradients(out, "out")
         if len(outs) != len(tensors):
             raise ValueError(f"out has {len(outs)} tensors for {len(tensors)} gradients")
+        if outs and outs[0].device != tensors[0].device:
+            raise RuntimeError(f"out is on {outs[0].device}, expected {tensors[0].device}")
         for i, (o, g) in enumerate(zip(outs, tensors)):
-            _check_input(f"out {i}", o)
-            if o.device != g.device:
-                raise RuntimeError(f"out {i} is on {o.device}, expected {g.device}")
             if o.shape != g.shape:
                 raise ValueError(f"out {i} has shape {tuple(o.shape)}, expected {tuple(g.shape)}")
-    total = _run_clip(tensors, outs, norm_type, True, float(max_norm))
+    total = _run_clip(tensors, outs, norm_type, 1, float(max_norm))
     if error_if_nonfinite and not math.isfinite(total.item()):
         raise RuntimeError(f"the norm of the gradients is {total.item()}")
     return total
