@@ -7,21 +7,28 @@
 // tensors' addresses go into the kernels' parameters, so a call copies no table to the device
 // and can be captured into a graph.
 //
-// Bound: memory. A tensor is cut into chunks of 32 KB; a block takes a chunk at a time, each
-// thread four 16-byte loads at once. The second kernel takes the chunks from the last to the
-// first, as the last ones that the first kernel read are still in L2.
+// Bound: memory. A tensor is cut into chunks of 16 KB. In each block one warp finds the block's
+// chunks in the table and keeps kStages bulk copies in flight into a ring in shared memory
+// (two blocks per SM: 192 KB in flight), so that neither the search nor the sums stop the loads;
+// the other warps take a chunk out of the ring at a time. The second kernel takes the chunks from
+// the last to the first, as the last ones that the first kernel read are still in L2, and fills
+// its ring while the first one ends.
 #include "jk_host.h"
 #include "jk_rows.cuh"
+#include "jk_sm100.cuh"
 
 #include <type_traits>
 
 namespace jk {
 namespace clip {
 
-constexpr int kThreads = 512;
-constexpr int kPacks = 4;                                        // 16-byte packs of a thread's turn
-constexpr int64_t kChunkPacks = static_cast<int64_t>(kThreads) * kPacks;
-constexpr int kMaxBlocks = 148 * 2;
+constexpr int kWorkers = 256;             // threads that take chunks; one more warp loads them
+constexpr int kThreads = kWorkers + 32;
+constexpr int kPacks = 4;                 // 16-byte packs of a thread's turn
+constexpr int kChunkPacks = kWorkers * kPacks;
+constexpr int kStages = 6;
+constexpr int kBlocksPerSm = 2;
+constexpr int kMaxBlocks = 148 * kBlocksPerSm;
 constexpr int kSmall = 64, kLarge = 640;  // tensors of one launch: the parameters of a launch are copied, so few tensors take the small table
 constexpr int kMaxGroups = 64;            // launches of the first kernel whose partials fit the workspace
 
@@ -41,14 +48,16 @@ __device__ __forceinline__ double join(double a, double b, int kind) {
   return a != a || a > b ? a : b;  // NaN stays
 }
 
-__device__ __forceinline__ double block_join(double v, int kind, double* scratch) {
+// Over the workers (the loading warp takes no part).
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
+
+__device__ __forceinline__ double workers_join(double v, int kind, double* scratch) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o), kind);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = scratch[threadIdx.x & (kThreads / 32 - 1)];
-#pragma unroll
-  for (int o = kThreads / 64; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o), kind);
+  workers_sync();
+  v = scratch[0];
+  for (int i = 1; i < kWorkers / 32; ++i) v = join(v, scratch[i], kind);
   return v;
 }
 
@@ -62,28 +71,97 @@ __device__ __forceinline__ int find(const Table<N>& t, uint32_t chunk) {
   return lo;
 }
 
-// The part of a tensor that is one chunk: elements [head, head + packs * kPack) from a 16-byte
-// boundary on, `lead` elements before the first boundary (first chunk) and `trail` after the
-// last whole pack (last chunk).
-template <typename T>
+// One chunk, as the loading warp leaves it beside its data: elements [at, at + packs * kPack) of
+// a tensor, from a 16-byte boundary on, `lead` elements before the first boundary (first chunk)
+// and `trail` after the last whole pack (last chunk), which are read where they lie.
 struct Part {
-  const T* body;
-  int64_t at;  // body's first element in the tensor
-  int packs, lead, trail;
-
-  __device__ __forceinline__ Part(const void* base, int64_t numel, uint32_t chunk) {
-    const T* p = static_cast<const T*>(base);
-    int64_t head = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
-    if (head > numel) head = numel;
-    const int64_t all = (numel - head) / kPack<T>, from = chunk * kChunkPacks;
-    const int64_t left = all - from;
-    packs = static_cast<int>(left < kChunkPacks ? left : kChunkPacks);
-    at = head + from * kPack<T>;
-    body = p + at;
-    lead = chunk == 0 ? static_cast<int>(head) : 0;
-    trail = left <= kChunkPacks ? static_cast<int>(numel - head - all * kPack<T>) : 0;
-  }
+  const void* body;
+  void* out;  // the element of the output that corresponds to *body
+  int packs;
+  uint8_t type, out_type, lead, trail;
 };
+
+template <int N>
+__device__ __forceinline__ Part part_of(const Table<N>& t, uint32_t chunk) {
+  const int i = find(t, chunk);
+  Part p;
+  p.type = t.in_type[i], p.out_type = t.out_type[i];
+  const int size = p.type == JK_F32 ? 4 : 2, out_size = p.out_type == JK_F32 ? 4 : 2;
+  const char* in = static_cast<const char*>(t.in[i]);
+  const int64_t numel = t.numel[i];
+  int64_t head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / size;
+  if (head > numel) head = numel;
+  const uint32_t k = chunk - t.first[i];
+  const int per = 16 / size;
+  const int64_t all = (numel - head) / per, from = static_cast<int64_t>(k) * kChunkPacks, left = all - from;
+  p.packs = static_cast<int>(left < kChunkPacks ? left : kChunkPacks);
+  const int64_t at = head + from * per;
+  p.body = in + at * size;
+  p.out = static_cast<char*>(t.out[i]) + at * out_size;
+  p.lead = k == 0 ? static_cast<uint8_t>(head) : 0;
+  p.trail = left <= kChunkPacks ? static_cast<uint8_t>(numel - head - all * per) : 0;
+  return p;
+}
+
+struct Ring {
+  uint4 data[kStages][kChunkPacks];
+  Part part[kStages];
+  uint64_t full[kStages], empty[kStages];
+  double scratch[kWorkers / 32];
+  bool idle;
+};
+
+__device__ __forceinline__ void ring_init(Ring& ring) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], kWorkers / 32);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+}
+
+// The loading warp's one thread: chunks block, block + grid, ... (counted from the end when
+// `backwards`) into the ring. A stage whose workers do not come back in time ends the kernel with
+// an error, after the copies in flight have landed.
+template <int N>
+__device__ __forceinline__ void ring_load(const Table<N>& t, Ring& ring, bool backwards) {
+  const uint32_t chunks = t.first[t.count];
+  int n = 0;
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x, ++n) {
+    const int s = n % kStages;
+    if (n >= kStages && !mbar_wait(&ring.empty[s], (n / kStages - 1) & 1)) {
+      g_device_error = JK_ERR_DEVICE_TIMEOUT;
+      break;
+    }
+    const Part p = part_of(t, backwards ? chunks - 1 - c : c);
+    ring.part[s] = p;
+    mbar_arrive_expect_tx(&ring.full[s], p.packs * 16);
+    if (p.packs > 0) bulk_load(ring.data[s], p.body, p.packs * 16, &ring.full[s]);
+  }
+  for (int back = n < kStages ? n : kStages; back > 0; --back) {
+    const int k = n - back;
+    mbar_wait(&ring.full[k % kStages], (k / kStages) & 1);
+  }
+}
+
+// What a worker does with each chunk of its block.
+template <int N, typename F>
+__device__ __forceinline__ void ring_take(const Table<N>& t, Ring& ring, F&& take) {
+  const uint32_t chunks = t.first[t.count];
+  int n = 0;
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x, ++n) {
+    const int s = n % kStages;
+    if (!mbar_wait(&ring.full[s], (n / kStages) & 1)) {
+      g_device_error = JK_ERR_DEVICE_TIMEOUT;
+      return;
+    }
+    take(ring.part[s], ring.data[s]);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[s]);
+  }
+}
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -125,18 +203,18 @@ __device__ __forceinline__ double squares(const uint4 (&raw)[kPacks]) {
 }
 
 template <typename T>
-__device__ __forceinline__ double part_norm(const Part<T>& p, int kind, double acc) {
+__device__ __forceinline__ double part_norm(const Part& p, const uint4* data, int kind, double acc) {
   uint4 raw[kPacks];
-  const uint4* src = reinterpret_cast<const uint4*>(p.body);
 #pragma unroll
   for (int i = 0; i < kPacks; ++i) {
-    const int k = i * kThreads + threadIdx.x;
-    raw[i] = k < p.packs ? src[k] : make_uint4(0, 0, 0, 0);
+    const int k = i * kWorkers + threadIdx.x;
+    raw[i] = k < p.packs ? data[k] : make_uint4(0, 0, 0, 0);
   }
   float edge = 0.f;
   const int t = threadIdx.x;
-  if (t < p.lead) edge = to_f32(p.body[t - p.lead]);
-  if (t >= 32 && t < 32 + p.trail) edge = to_f32(p.body[static_cast<int64_t>(p.packs) * kPack<T> + t - 32]);
+  const T* body = static_cast<const T*>(p.body);
+  if (t < p.lead) edge = to_f32(body[t - p.lead]);
+  if (t >= 32 && t < 32 + p.trail) edge = to_f32(body[p.packs * kPack<T> + t - 32]);
   if (kind == JK_NORM_2) {
     acc += squares<T>(raw);
     if (edge != 0.f) acc += static_cast<double>(edge) * static_cast<double>(edge);
@@ -154,103 +232,116 @@ __device__ __forceinline__ double part_norm(const Part<T>& p, int kind, double a
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<N> t, int kind, double* partials) {
-  __shared__ double scratch[kThreads / 32];
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+    norm_kernel(const __grid_constant__ Table<N> t, int kind, double* partials) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  Ring& ring = *reinterpret_cast<Ring*>(memory);
+  ring_init(ring);
   double acc = 0.0;
-  const uint32_t chunks = t.first[t.count];
-  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int i = find(t, c);
-    const int type = t.in_type[i];
-    const uint32_t k = c - t.first[i];
-    JK_WITH_TYPE(type, T, acc = part_norm<T>(Part<T>(t.in[i], t.numel[i], k), kind, acc));
+  if (threadIdx.x < kWorkers) {
+    ring_take(t, ring, [&](const Part& p, const uint4* data) {
+      JK_WITH_TYPE(p.type, T, acc = part_norm<T>(p, data, kind, acc));
+    });
+    grid_dependency_launch();
+    acc = workers_join(acc, kind, ring.scratch);
+    if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  } else if (threadIdx.x == kWorkers) {
+    ring_load(t, ring, false);
   }
-  acc = block_join(acc, kind, scratch);
-  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
 // total over `n` partials, the same in every block.
 __device__ __forceinline__ float total_norm(const double* partials, int n, int kind, double* scratch) {
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += kThreads) v = join(v, partials[i], kind);
-  v = block_join(v, kind, scratch);
+  for (int i = threadIdx.x; i < n; i += kWorkers) v = join(v, partials[i], kind);
+  v = workers_join(v, kind, scratch);
   return static_cast<float>(kind == JK_NORM_2 ? sqrt(v) : v);
 }
 
-// B bytes of memory in registers.
-template <int B>
-struct Raw;
-template <>
-struct Raw<8> { using type = uint2; };
-template <>
-struct Raw<16> { using type = uint4; };
-
-// The unit of a thread's turn is what fills 16 bytes of the wider of the two types, so that
-// neighbouring threads read and write neighbouring addresses on both sides.
+// A turn's unit is what fills 16 bytes of the wider of the two types, so that neighbouring
+// threads read and write neighbouring addresses on both sides.
 template <typename T, typename O>
-__device__ __forceinline__ void part_scale(const Part<T>& p, O* out, float coef) {
+__device__ __forceinline__ void part_scale(const Part& p, const uint4* data, float coef) {
   constexpr int kUnit = sizeof(T) >= sizeof(O) ? kPack<T> : kPack<O>;  // elements
   constexpr int kTurns = kPacks * kPack<T> / kUnit;
-  using In = typename Raw<kUnit * sizeof(T)>::type;
-  using Out = typename Raw<kUnit * sizeof(O)>::type;
   const int units = p.packs * (kPack<T> / kUnit);
-  In raw[kTurns];
-  const In* src = reinterpret_cast<const In*>(p.body);
-#pragma unroll
-  for (int i = 0; i < kTurns; ++i) {
-    const int k = i * kThreads + threadIdx.x;
-    if (k < units) raw[i] = __ldcs(src + k);
-  }
+  const T* body = static_cast<const T*>(p.body);
+  O* out = static_cast<O*>(p.out);
   const int t = threadIdx.x;
-  O* dst = out + p.at;
-  if (t < p.lead) dst[t - p.lead] = from_f32<O>(to_f32(p.body[t - p.lead]) * coef);
+  if (t < p.lead) out[t - p.lead] = from_f32<O>(to_f32(body[t - p.lead]) * coef);
   if (t >= 32 && t < 32 + p.trail) {
-    const int64_t e = static_cast<int64_t>(p.packs) * kPack<T> + t - 32;
-    dst[e] = from_f32<O>(to_f32(p.body[e]) * coef);
+    const int e = p.packs * kPack<T> + t - 32;
+    out[e] = from_f32<O>(to_f32(body[e]) * coef);
   }
-  const bool vector = reinterpret_cast<uintptr_t>(dst) % sizeof(Out) == 0;
+  const bool vector = reinterpret_cast<uintptr_t>(out) % (kUnit * sizeof(O)) == 0;
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
-    const int k = i * kThreads + threadIdx.x;
+    const int k = i * kWorkers + t;
     if (k >= units) continue;
-    const T* in = reinterpret_cast<const T*>(&raw[i]);
-    Out wide;
-    O* f = reinterpret_cast<O*>(&wide);
+    float f[kUnit];
+    if constexpr (kUnit == kPack<T>) {
+      unpack<T>(data[k], f);
+    } else {  // half a pack
+      const uint2 h = reinterpret_cast<const uint2*>(data)[k];
+      float both[kPack<T>];
+      unpack<T>(make_uint4(h.x, h.y, 0, 0), both);
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) f[j] = from_f32<O>(to_f32(in[j]) * coef);
+      for (int j = 0; j < kUnit; ++j) f[j] = both[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) f[j] *= coef;
     if (vector) {
-      __stcs(reinterpret_cast<Out*>(dst) + k, wide);
+      if constexpr (kUnit == kPack<O>) {
+        __stcs(reinterpret_cast<uint4*>(out) + k, pack<O>(f));
+      } else {
+        float both[kPack<O>] = {};
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) both[j] = f[j];
+        const uint4 u = pack<O>(both);
+        __stcs(reinterpret_cast<uint2*>(out) + k, make_uint2(u.x, u.y));
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j) dst[static_cast<int64_t>(k) * kUnit + j] = f[j];
+      for (int j = 0; j < kUnit; ++j) out[k * kUnit + j] = from_f32<O>(f[j]);
     }
   }
 }
 
+// With outputs of their own, the ring fills before the norm is known. In place it does not: a
+// coefficient of 1 then leaves every gradient as it is, unread.
 template <int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     scale_kernel(const __grid_constant__ Table<N> t, int kind, const double* partials, int n, float max_norm, float eps,
-                 float* total) {
-  __shared__ double scratch[kThreads / 32];
-  const float norm = total_norm(partials, n, kind, scratch);
-  if (total != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *total = norm;
-  float coef = max_norm / (norm + eps);
-  coef = coef > 1.f ? 1.f : coef;  // a NaN stays
-  const uint32_t chunks = t.first[t.count];
-  for (uint32_t back = blockIdx.x; back < chunks; back += gridDim.x) {
-    const uint32_t c = chunks - 1 - back;
-    const int i = find(t, c);
-    if (coef == 1.f && t.in[i] == t.out[i]) continue;
-    const int type = t.in_type[i], out_type = t.out_type[i];
-    const uint32_t k = c - t.first[i];
-    JK_WITH_TYPE(type, T, {
-      const Part<T> part(t.in[i], t.numel[i], k);
-      JK_WITH_TYPE(out_type, O, part_scale<T, O>(part, static_cast<O*>(t.out[i]), coef));
+                 bool in_place, float* total) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  Ring& ring = *reinterpret_cast<Ring*>(memory);
+  ring_init(ring);
+  float coef = 0.f;
+  if (threadIdx.x < kWorkers) {
+    grid_dependency_wait();
+    const float norm = total_norm(partials, n, kind, ring.scratch);
+    coef = max_norm / (norm + eps);
+    coef = coef > 1.f ? 1.f : coef;  // a NaN stays
+    if (threadIdx.x == 0) {
+      ring.idle = coef == 1.f;
+      if (total != nullptr && blockIdx.x == 0) *total = norm;
+    }
+  }
+  if (in_place) {
+    __syncthreads();
+    if (ring.idle) return;
+  }
+  if (threadIdx.x < kWorkers) {
+    ring_take(t, ring, [&](const Part& p, const uint4* data) {
+      JK_WITH_TYPE(p.type, T, JK_WITH_TYPE(p.out_type, O, (part_scale<T, O>(p, data, coef))));
     });
+  } else if (threadIdx.x == kWorkers) {
+    ring_load(t, ring, true);
   }
 }
 
-__global__ void __launch_bounds__(kThreads) total_kernel(int kind, const double* partials, int n, float* total) {
-  __shared__ double scratch[kThreads / 32];
+__global__ void __launch_bounds__(kWorkers) total_kernel(int kind, const double* partials, int n, float* total) {
+  __shared__ double scratch[kWorkers / 32];
   const float norm = total_norm(partials, n, kind, scratch);
   if (threadIdx.x == 0) *total = norm;
 }
@@ -304,29 +395,42 @@ int blocks_for(const Table<N>& t) {
 template <int N>
 int launch(const Call& q, int kind, bool clip_on, float max_norm, float eps, float* total, double* partials,
            cudaStream_t s) {
+  // above 48 KB a kernel has to be told, once for each device; it costs less than the launch
+  if (cudaFuncSetAttribute(norm_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Ring)) != cudaSuccess ||
+      cudaFuncSetAttribute(scale_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Ring)) != cudaSuccess)
+    return launch_status();
   Table<N> t;
   int n = 0, groups = 0;
   for (int64_t at = 0; at < q.count;) {
     at = fill(t, q, at);
     if (t.count == 0) break;
     if (++groups > kMaxGroups) return JK_ERR_BAD_SHAPE;
-    norm_kernel<N><<<blocks_for(t), kThreads, 0, s>>>(t, kind, partials + n);
+    norm_kernel<N><<<blocks_for(t), kThreads, sizeof(Ring), s>>>(t, kind, partials + n);
     n += blocks_for(t);
   }
   if (!clip_on || n == 0) {
-    total_kernel<<<1, kThreads, 0, s>>>(kind, partials, n, total);
+    total_kernel<<<1, kWorkers, 0, s>>>(kind, partials, n, total);
     return launch_status();
   }
   for (int64_t at = 0, g = 0; at < q.count; ++g) {
     if (groups == 1) at = q.count;  // the table holds them all
     else at = fill(t, q, at);
     if (t.count == 0) break;
-    scale_kernel<N><<<blocks_for(t), kThreads, 0, s>>>(t, kind, partials, n, max_norm, eps, g == 0 ? total : nullptr);
+    const bool in_place = q.outs == nullptr;
+    // only the first of them follows the kernel whose partials it waits for
+    if (g == 0)
+      launch_dependent(scale_kernel<N>, blocks_for(t), kThreads, sizeof(Ring), s, t, kind, partials, n, max_norm, eps,
+                       in_place, total);
+    else
+      scale_kernel<N><<<blocks_for(t), kThreads, sizeof(Ring), s>>>(t, kind, partials, n, max_norm, eps, in_place, nullptr);
   }
   return launch_status();
 }
 
 }  // namespace clip
+
+JK_ERROR_READER(read_error_clip)
+
 }  // namespace jk
 
 extern "C" int64_t jk_clip_grad_norm_workspace(void) {

@@ -159,6 +159,9 @@ __global__ void __launch_bounds__(kThreads)
 inline int blocks_for(int64_t rows) { return static_cast<int>(rows < kMaxBlocks ? rows : kMaxBlocks); }
 
 }  // namespace loss
+
+JK_ERROR_READER(read_error_loss)
+
 }  // namespace jk
 
 extern "C" int64_t jk_cross_entropy_workspace(int64_t rows) {

@@ -78,6 +78,21 @@ __device__ __forceinline__ float warp_sum32(float v) {
   return v;
 }
 
+// Untiled bulk copy of global memory into this block's shared memory (both addresses 16-byte
+// aligned, a multiple of 16 bytes), counted on an mbarrier.
+__device__ __forceinline__ void bulk_load(void* dst_smem, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst_smem))),
+               "l"(src), "r"(bytes), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
+               : "memory");
+}
+// And back, as part of the thread's current bulk group.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src_smem, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(static_cast<uint32_t>(__cvta_generic_to_shared(src_smem))), "r"(bytes)
+               : "memory");
+}
+
 // Programmatic dependent launch: a kernel launched with the attribute may begin while the one
 // before it in the stream still runs; grid_dependency_wait returns when that one has finished
 // and its writes are visible. Without the attribute both are no-ops.
@@ -98,6 +113,24 @@ __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddep
       __VA_ARGS__;                                                       \
     }                                                                    \
   } while (0)
+
+// Launches a kernel that may begin before the one ahead of it in the stream has finished (it
+// calls grid_dependency_wait before it touches what that one writes).
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s,
+                             Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
 
 inline bool float_dtype(int code) { return code == JK_F32 || code == JK_BF16 || code == JK_F16; }
 inline int64_t dtype_bytes(int code) { return code == JK_F32 ? 4 : 2; }
