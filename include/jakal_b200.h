@@ -436,7 +436,7 @@ int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const void
 #define JK_REDUCE_MEAN 1 /* over the rows whose target is not ignore_index */
 #define JK_REDUCE_SUM 2
 
-/* Bytes of the workspace of jk_cross_entropy_forward. */
+/* Bytes of the workspace of jk_cross_entropy_forward and _backward. */
 int64_t jk_cross_entropy_workspace(int64_t rows);
 
 /* Softmax cross entropy of logits [rows, vocab] (dtype) against targets int64 [rows]:
@@ -458,11 +458,12 @@ int jk_cross_entropy_forward(const void* logits, int64_t logits_stride, const in
 /* Gradient of the cross entropy from the lse that the forward pass kept:
  *   grad = g * w * (exp(z - lse) - (1 - a) onehot - a / vocab)
  * grad_loss: device f32, [rows] with JK_REDUCE_NONE (g per row, w = 1), else one value; grad
- * [rows, vocab] in dtype (may be the logits); rows to ignore get zeros. */
+ * [rows, vocab] in dtype (may be the logits); rows to ignore get zeros. workspace:
+ * jk_cross_entropy_workspace(rows) bytes, 8-byte aligned. */
 int jk_cross_entropy_backward(const float* grad_loss, const void* logits, int64_t logits_stride,
                               const int64_t* targets, const float* lse, int64_t rows, int64_t vocab, int dtype,
                               int64_t ignore_index, float label_smoothing, int reduction, void* grad,
-                              int64_t grad_stride, jk_stream_t stream);
+                              int64_t grad_stride, void* workspace, jk_stream_t stream);
 
 /* norm codes of jk_clip_grad_norm */
 #define JK_NORM_2 0

@@ -395,10 +395,11 @@ int blocks_for(const Table<N>& t) {
 template <int N>
 int launch(const Call& q, int kind, bool clip_on, float max_norm, float eps, float* total, double* partials,
            cudaStream_t s) {
-  // above 48 KB a kernel has to be told, once for each device; it costs less than the launch
   if (cudaFuncSetAttribute(norm_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Ring)) != cudaSuccess ||
-      cudaFuncSetAttribute(scale_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Ring)) != cudaSuccess)
-    return launch_status();
+      cudaFuncSetAttribute(scale_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Ring)) != cudaSuccess) {
+    cudaGetLastError();
+    return JK_ERR_LAUNCH;
+  }
   Table<N> t;
   int n = 0, groups = 0;
   for (int64_t at = 0; at < q.count;) {

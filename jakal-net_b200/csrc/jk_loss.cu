@@ -4,18 +4,34 @@
 //   loss = lse - (1 - a) z_t - a E_j[z_j]
 //   grad_j = c (exp(z_j - lse) - (1 - a) [j = t] - a / V),  c = scale / number of rows that count
 //
-// With the maximum at hand, loss = log sum exp(z - m) + (1 - a) (m - z_t) + a E_j[m - z_j] and
+// With the maximum at hand, loss = log sum exp(z - m) + (1 - a) (m - z_t) + a (m - E_j[z_j]) and
 // softmax_j = exp(z_j - m) / sum: differences from m keep their digits where m is large, which
-// lse = m + log(sum), one f32 number, does not. exp(z - m) is taken of the difference: with z * log2(e) - m * log2(e) in one fma, logits of the
-// type's lowest value would overflow both products and meet as inf - inf.
+// lse = m + log(sum), one f32 number, does not. exp(z - m) is 2^(z log2(e) - r), one fma and the
+// hardware's exponential, with r = m log2(e) rounded once and carried along; where that product
+// would leave the type's range (logits of the order of its largest value), it is taken of z - m.
+//
+// Bound: memory, one read of the logits and one write of the gradient. Two forms:
+//   * warp_kernel, rows of up to 1024 logits: a warp has a row in its registers;
+//   * ring_kernel, longer rows: a cluster of blocks has a row, each block a slice of it in shared
+//     memory, brought there by bulk copies that run rows ahead of the arithmetic; the gradient is
+//     taken from the same copy, so the logits are read once however long the row is. Rows that
+//     eight blocks cannot hold go through stream_kernel, which reads them again.
 #include "jk_host.h"
 #include "jk_rows.cuh"
+#include "jk_sm100.cuh"
+
+#include <type_traits>
 
 namespace jk {
 namespace loss {
 
-constexpr int kThreads = 512;
-constexpr int kMaxBlocks = 148 * 4;
+enum Mode { kLoss, kBoth, kBackward, kLater };  // kLater: kBackward within the forward call
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int64_t kMaxVocab = int64_t(1) << 30;  // columns are counted in 32 bits
+constexpr int kMaxBlocks = 148 * 8;    // blocks that leave a partial
+constexpr int kCounts = 64;            // blocks of the counting kernel
+constexpr int64_t kCountRows = 4096;   // up to so many rows every block counts for itself
 
 // What a block leaves for the reduction over rows.
 struct Partial {
@@ -23,140 +39,1083 @@ struct Partial {
   long long rows;
 };
 
-// Sum of one value per thread, and the maximum of another, over the block (NaN is kept by the
-// sum; the maximum ignores it).
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
-  v = warp_sum32(v);
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < kThreads / 32; ++i) v += scratch[i];
-  __syncthreads();
-  return v;
-}
-
-__device__ __forceinline__ float block_max(float v, float* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = scratch[0];
-  for (int i = 1; i < kThreads / 32; ++i) v = fmaxf(v, scratch[i]);
-  __syncthreads();
-  return v;
-}
-
-// Rows that count, over all rows (every block counts for itself).
-__device__ __forceinline__ int count_rows(const int64_t* targets, int64_t rows, int64_t ignore_index, int* scratch) {
-  if (threadIdx.x == 0) *scratch = 0;
-  __syncthreads();
-  int n = 0;
-  for (int64_t r = threadIdx.x; r < rows; r += kThreads) n += targets[r] != ignore_index;
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) atomicAdd(scratch, n);
-  __syncthreads();
-  return *scratch;
-}
-
 template <typename T>
-__device__ __forceinline__ void write_grad(const T* z, T* grad, int64_t vocab, float base, float inv, float c,
-                                           int64_t target, float smoothing) {
-  const float share = smoothing / static_cast<float>(vocab), hit = 1.f - smoothing;
-  for (int64_t j = threadIdx.x; j < vocab; j += kThreads) {
-    float p = expf(to_f32(z[j]) - base) * inv - share;
-    if (j == target) p -= hit;
-    grad[j] = from_f32<T>(c * p);
-  }
+struct Args {
+  const T* logits;
+  int64_t stride;
+  const int64_t* targets;
+  int64_t rows, vocab, ignore_index;
+  float smoothing;
+  int reduction;
+  float scale;             // of the gradient (forward)
+  const float* grad_loss;  // backward
+  const float* lse_in;
+  float* losses;
+  float* lse_out;
+  T* grad;
+  int64_t grad_stride;
+  Partial* partials;
+  const int* counts;  // of kCounts blocks, or null: count here
+};
+
+// A product that is rounded by itself, whatever it is added to.
+__device__ __forceinline__ float product(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-// One block per row at a time; the row is read three times.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    forward_kernel(const T* logits, int64_t stride, const int64_t* targets, int64_t rows, int64_t vocab,
-                   int64_t ignore_index, float smoothing, int reduction, float grad_scale, float* losses, float* lse_out,
-                   T* grad, int64_t grad_stride, Partial* partials) {
-  __shared__ float scratch[kThreads / 32];
-  __shared__ int counted;
-  float c = grad_scale;
-  if (grad != nullptr && reduction == JK_REDUCE_MEAN)
-    c = grad_scale / static_cast<float>(count_rows(targets, rows, ignore_index, &counted));
-  Partial part{0.0, 0};
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t target = targets[r];
-    const T* z = logits + r * stride;
-    T* g = grad == nullptr ? nullptr : grad + r * grad_stride;
-    if (target == ignore_index) {
-      if (threadIdx.x == 0) {
-        if (losses != nullptr) losses[r] = 0.f;
-        if (lse_out != nullptr) lse_out[r] = 0.f;
-      }
-      if (g != nullptr)
-        for (int64_t j = threadIdx.x; j < vocab; j += kThreads) g[j] = from_f32<T>(0.f);
-      continue;
-    }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two f32 in a register pair: one instruction works on both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The largest of N packs, NaN aside; 16-bit types two at a time.
+template <typename T, int N>
+__device__ __forceinline__ float pack_max(const uint4 (&raw)[N]) {
+  if constexpr (sizeof(T) == 4) {
     float m = -INFINITY;
-    for (int64_t j = threadIdx.x; j < vocab; j += kThreads) m = fmaxf(m, to_f32(z[j]));
-    m = block_max(m, scratch);
-    float a = 0.f, all = 0.f;
-    for (int64_t j = threadIdx.x; j < vocab; j += kThreads) {
-      const float d = to_f32(z[j]) - m;
-      a += expf(d);
-      all -= d;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float f[4];
+      unpack<T>(raw[i], f);
+      m = fmaxf(m, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
     }
-    a = block_sum(a, scratch);
-    const float lse = m + logf(a);
-    const bool inside = target >= 0 && target < vocab;
-    float l = inside ? logf(a) + (1.f - smoothing) * (m - to_f32(z[target])) : NAN;
-    if (smoothing != 0.f) l += smoothing * (block_sum(all, scratch) / static_cast<float>(vocab));
-    __syncthreads();  // z[target] is read before an in-place gradient replaces it
-    if (threadIdx.x == 0) {
-      if (losses != nullptr) losses[r] = l;
-      if (lse_out != nullptr) lse_out[r] = lse;
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m = *reinterpret_cast<const T2*>(&raw[0].x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const T2* h = reinterpret_cast<const T2*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = __hmax2(m, h[j]);
     }
-    part.sum += l;
-    part.rows += 1;
-    if (g != nullptr) write_grad(z, g, vocab, m, 1.f / a, inside ? c : NAN, target, smoothing);
-    __syncthreads();
+    return fmaxf(to_f32(m.x), to_f32(m.y));
   }
-  if (threadIdx.x == 0) partials[blockIdx.x] = part;
 }
 
-// The blocks' partial sums, in their order.
-__global__ void reduce_kernel(const Partial* partials, int blocks, int reduction, float* loss) {
+// The reference of a sum of exponentials: exp(z - m) as 2^(z log2(e) - r).
+constexpr float kHuge = 1e38f;
+struct Base {
+  float m, r;
+  bool near;  // m log2(e) is finite
+
+  __device__ __forceinline__ explicit Base(float m_) : m(m_), r(product(m_, kLog2e)), near(fabsf(m_) < kHuge) {}
+  __device__ __forceinline__ float exp_near(float z) const { return exp2_approx(fmaf(z, kLog2e, -r)); }
+  __device__ __forceinline__ float exp_far(float z) const { return exp2_approx((z - m) * kLog2e); }
+  __device__ __forceinline__ float exp(float z) const { return near ? exp_near(z) : exp_far(z); }
+  // ln of what 2^-r is short of exp(-m)
+  __device__ __forceinline__ float rest() const { return near ? kLn2 * fmaf(-m, kLog2e, r) : 0.f; }
+};
+
+// Replaces N logits by their exponentials.
+template <int N>
+__device__ __forceinline__ void exponentials(float (&z)[N], const Base& b) {
+  if (b.near) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = b.exp_near(z[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = b.exp_far(z[i]);
+  }
+}
+
+// (m, s): a maximum and the sum of the exponentials on it; -inf and 0 for nothing.
+struct Sum {
+  float m, s;
+};
+
+// What a sum on maximum `from` is worth on a larger one. (Where only `from` is far, it is far
+// below, and both forms give 0.)
+__device__ __forceinline__ float factor_to(float from, float to) {
+  const Base b(to);
+  return b.near ? exp2_approx(product(from, kLog2e) - b.r) : b.exp_far(from);
+}
+
+__device__ __forceinline__ float warp_max32(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Over a warp: one maximum, one factor per lane, one sum. Every lane gets the same bits.
+__device__ __forceinline__ Sum warp_join(Sum v) {
+  const float m = warp_max32(v.m);
+  // a lane without a finite value has s = 0 or NaN, and neither needs a factor
+  return {m, warp_sum32(v.m == m ? v.s : v.s * factor_to(v.m, m))};
+}
+
+template <int N>
+__device__ __forceinline__ float top_of(const float (&z)[N]) {
+  float top = z[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+  return top;
+}
+
+// Adds N values to a thread's sum.
+template <int N>
+__device__ __forceinline__ void take(Sum& v, float (&z)[N]) {
+  const float top = top_of(z);
+  if (top > v.m) {
+    v.s *= factor_to(v.m, top);  // from -inf: 0
+    v.m = top;
+  }
+  exponentials(z, Base(v.m == -INFINITY ? 0.f : v.m));
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.s += z[i];
+}
+
+template <typename T, int N>
+__device__ __forceinline__ float pack_sum(const uint4 (&raw)[N]) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float f[kPack<T>];
+    unpack<T>(raw[i], f);
+#pragma unroll
+    for (int j = 0; j < kPack<T>; ++j) s += f[j];
+  }
+  return s;
+}
+
+// The same for N packs. All maxima first: 16 logits or more share one comparison and one factor.
+template <typename T, int N>
+__device__ __forceinline__ void take_packs(Sum& v, const uint4 (&raw)[N]) {
+  const float top = pack_max<T>(raw);
+  if (top > v.m) {
+    v.s *= factor_to(v.m, top);
+    v.m = top;
+  }
+  const Base b(v.m == -INFINITY ? 0.f : v.m);
+  if (b.near) {
+    const uint64_t l2e = pair(kLog2e, kLog2e), minus_r = pair(-b.r, -b.r);
+    uint64_t s = pair(v.s, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float f[kPack<T>];
+      unpack<T>(raw[i], f);
+#pragma unroll
+      for (int j = 0; j < kPack<T>; j += 2) {
+        const float2 x = unpair(fma2(pair(f[j], f[j + 1]), l2e, minus_r));
+        s = add2(s, pair(exp2_approx(x.x), exp2_approx(x.y)));
+      }
+    }
+    const float2 both = unpair(s);
+    v.s = both.x + both.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float f[kPack<T>];
+      unpack<T>(raw[i], f);
+#pragma unroll
+      for (int j = 0; j < kPack<T>; ++j) v.s += b.exp_far(f[j]);
+    }
+  }
+}
+
+// f = scale * exp(f - m) + other for a pack.
+template <typename T>
+__device__ __forceinline__ void gradient_pack(float (&f)[kPack<T>], const Base& b, float scale, float other) {
+  if (b.near) {
+    const uint64_t l2e = pair(kLog2e, kLog2e), minus_r = pair(-b.r, -b.r), by = pair(scale, scale), to = pair(other, other);
+#pragma unroll
+    for (int j = 0; j < kPack<T>; j += 2) {
+      const float2 x = unpair(fma2(pair(f[j], f[j + 1]), l2e, minus_r));
+      const float2 y = unpair(fma2(pair(exp2_approx(x.x), exp2_approx(x.y)), by, to));
+      f[j] = y.x, f[j + 1] = y.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPack<T>; ++j) f[j] = fmaf(b.exp_far(f[j]), scale, other);
+  }
+}
+
+// Rows that count, over all rows, by the block's threads [0, n).
+__device__ __forceinline__ int count_rows(const int64_t* targets, int64_t rows, int64_t ignore_index, int threads) {
+  int n = 0;
+  for (int64_t r = threadIdx.x; r < rows; r += threads) n += targets[r] != ignore_index;
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
+__global__ void __launch_bounds__(256) count_kernel(const int64_t* targets, int64_t rows, int64_t ignore_index, int* counts) {
+  __shared__ int part[8];
+  const int64_t per = (rows + gridDim.x - 1) / gridDim.x, from = per * blockIdx.x;
+  const int64_t n = rows - from < per ? rows - from : per;
+  const int mine = n > 0 ? count_rows(targets + from, n, ignore_index, 256) : 0;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int all = 0;
+    for (int i = 0; i < 8; ++i) all += part[i];
+    counts[blockIdx.x] = all;
+  }
+}
+
+// The factor of a row's gradient, without the row's own grad_loss, for all of the block's threads
+// [0, threads); `sync` is their barrier.
+template <typename T, typename Sync>
+__device__ __forceinline__ float gradient_factor(const Args<T>& a, bool forward, int threads, int* scratch, Sync&& sync) {
+  float c = forward ? a.scale : (a.reduction == JK_REDUCE_NONE ? 1.f : *a.grad_loss);
+  if (a.reduction != JK_REDUCE_MEAN) return c;
+  int n = 0;
+  if (a.counts != nullptr) {
+    for (int i = threadIdx.x & 31; i < kCounts; i += 32) n += a.counts[i];
+    n = __reduce_add_sync(0xffffffffu, n);
+  } else {
+    const int mine = count_rows(a.targets, a.rows, a.ignore_index, threads);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = mine;
+    sync();
+    for (int i = 0; i < threads / 32; ++i) n += scratch[i];
+  }
+  return c / static_cast<float>(n);
+}
+
+// A row's loss and log-sum from its sum, target logit and sum of logits.
+struct RowLoss {
+  float loss, lse;
+  __device__ __forceinline__ RowLoss(Sum v, float zt, float all, float smoothing, int64_t vocab) {
+    const float log_sum = logf(v.s) + Base(v.m).rest();  // ln sum exp(z - m)
+    loss = log_sum + (1.f - smoothing) * (v.m - zt);
+    if (smoothing != 0.f) loss += smoothing * (v.m - all / static_cast<float>(vocab));
+    lse = v.m + log_sum;
+  }
+};
+
+// ---------------------------------------------------------------- short rows
+// A warp per row, N turns of VEC neighbouring elements per lane.
+constexpr int kWarpThreads = 256;
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_row(float (&f)[VEC], const T* p) {
+  if constexpr (VEC == 1)
+    f[0] = to_f32(*p);
+  else
+    unpack<T>(*reinterpret_cast<const uint4*>(p), f);
+}
+
+template <typename T, int MODE, int VEC, int N>
+__global__ void __launch_bounds__(kWarpThreads) warp_kernel(const Args<T> a) {
+  __shared__ int scratch[kWarpThreads / 32];
+  __shared__ Partial parts[kWarpThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int vocab = static_cast<int>(a.vocab);
+  float factor = 0.f;
+  if (MODE != kLoss) factor = gradient_factor(a, MODE == kBoth, kWarpThreads, scratch, [] { __syncthreads(); });
+  const float share = a.smoothing / static_cast<float>(vocab), hit = 1.f - a.smoothing;
+  Partial part{0.0, 0};
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kWarpThreads / 32) + warp; r < a.rows;
+       r += static_cast<int64_t>(gridDim.x) * (kWarpThreads / 32)) {
+    const int64_t target = a.targets[r];
+    const T* z = a.logits + r * a.stride;
+    T* g = MODE == kLoss ? nullptr : a.grad + r * a.grad_stride;
+    const bool ignored = target == a.ignore_index;
+    const bool inside = target >= 0 && target < vocab;
+    float f[N][VEC];
+    if (!ignored) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * 32 + lane) * VEC;
+        if (c < vocab) {
+          load_row<T, VEC>(f[i], z + c);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) f[i][j] = -INFINITY;
+        }
+      }
+    }
+    float m = 0.f, scale = 0.f;
+    if (!ignored && MODE != kBackward) {
+      const float zt = inside ? to_f32(z[target]) : NAN;
+      Sum v{-INFINITY, 0.f};
+      float all = 0.f;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) top = fmaxf(top, f[i][j]);
+      v.m = top = warp_max32(top);
+      const Base base(top);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int c = (i * 32 + lane) * VEC + j;
+          if (a.smoothing != 0.f && c < vocab) all += f[i][j];
+          f[i][j] = base.exp(f[i][j]);
+          v.s += c < vocab ? f[i][j] : 0.f;
+        }
+      }
+      v.s = warp_sum32(v.s);
+      if (a.smoothing != 0.f) all = warp_sum32(all);
+      const RowLoss l(v, zt, all, a.smoothing, vocab);
+      if (lane == 0) {
+        if (a.losses != nullptr) a.losses[r] = l.loss;
+        if (a.lse_out != nullptr) a.lse_out[r] = l.lse;
+      }
+      part.sum += l.loss;
+      part.rows += 1;
+      scale = factor / v.s;
+      __syncwarp();  // z[target] is read before an in-place gradient replaces it
+    } else if (ignored && MODE != kBackward && lane == 0) {
+      if (a.losses != nullptr) a.losses[r] = 0.f;
+      if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
+    }
+    if (MODE == kLoss) continue;
+    float c0 = ignored ? 0.f : factor;
+    if (MODE == kBackward && !ignored) {
+      m = a.lse_in[r];
+      if (a.reduction == JK_REDUCE_NONE) c0 = a.grad_loss[r];
+      scale = c0 * expf(Base(m).rest());
+    }
+    if (!ignored && !inside) scale = c0 = NAN;
+    const Base from(m);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * 32 + lane) * VEC;
+      if (c >= vocab) continue;
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float e = ignored ? 0.f : MODE == kBackward ? from.exp(f[i][j]) : f[i][j];
+        o[j] = ignored ? 0.f : fmaf(e, scale, -(c + j == target ? hit + share : share) * c0);
+      }
+      if constexpr (VEC == 1)
+        g[c] = from_f32<T>(o[0]);
+      else
+        *reinterpret_cast<uint4*>(g + c) = pack<T>(o);
+    }
+  }
+  if (MODE == kBackward) return;
+  grid_dependency_launch();
+  if (lane == 0) parts[warp] = part;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kWarpThreads / 32; ++i) part.sum += parts[i].sum, part.rows += parts[i].rows;
+    a.partials[blockIdx.x] = part;
+  }
+}
+
+// ---------------------------------------------------------------- a row as 16-byte packs
+constexpr int kTurn = 4;  // packs that a thread takes at once
+
+// Where a row lies against 16-byte packs: pack k holds columns k * kPack - shift ..., the first
+// and the last one perhaps in part.
+template <typename T>
+struct Window {
+  const T* z;
+  int shift, packs;
+
+  __device__ __forceinline__ Window(const Args<T>& a, int64_t row) {
+    z = a.logits + row * a.stride;
+    shift = static_cast<int>(reinterpret_cast<uintptr_t>(z) & 15) / static_cast<int>(sizeof(T));
+    packs = (shift + static_cast<int>(a.vocab) + kPack<T> - 1) / kPack<T>;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ T minus_inf() {
+  return from_f32<T>(-INFINITY);
+}
+
+// ---------------------------------------------------------------- loss, and gradient from the lse
+// Warps on their own. The packs of all rows, in pieces of 32 x kTurn, are cut into equal runs, one
+// for each warp, so that no SM ends late; a lane has the next piece on its way while it works on
+// one. A row that more than one warp has part of leaves a record for each, and the reduction over
+// rows joins them.
+constexpr int kStreamThreads = 256;
+#ifndef JKV_SB
+#define JKV_SB 3
+#endif
+constexpr int kStreamBlocksPerSm = JKV_SB;
+constexpr int kMaxWarps = 148 * kStreamBlocksPerSm * (kStreamThreads / 32);
+constexpr int kPiece = 32 * kTurn;  // packs
+
+struct Record {
+  int64_t row;  // -1: none
+  float m, s, all;
+};
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
+    stream_kernel(const Args<T> a, int pieces, Record* records, int* come) {
+  __shared__ int scratch[kStreamThreads / 32];
+  constexpr int kP = kPack<T>;
+  const int lane = threadIdx.x & 31, vocab = static_cast<int>(a.vocab);
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kStreamThreads / 32);
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kStreamThreads / 32) + (threadIdx.x >> 5);
+  const int64_t all_items = a.rows * pieces;
+  int64_t item = all_items / warps * warp + min(warp, all_items % warps);
+  const int64_t end = item + all_items / warps + (warp < all_items % warps ? 1 : 0);
+  const float hit = 1.f - a.smoothing, share = a.smoothing / static_cast<float>(vocab);
+  float factor = 0.f;
+  if (MODE != kLoss) factor = gradient_factor(a, MODE == kLater, kStreamThreads, scratch, [] { __syncthreads(); });
+  if (MODE == kLoss && blockIdx.x == 0 && threadIdx.x == 0) *come = 0;  // for the reduction that follows
+
+  // the piece that is next, and what it needs beside its packs
+  int64_t row = item / pieces;
+  int piece = static_cast<int>(item - row * pieces);
+  const int64_t first_row = row;
+  int64_t targets_from = row, some_targets = 0;  // of 32 rows, a row per lane
+  if (item < end) some_targets = a.targets[min(row + lane, a.rows - 1)];
+  uint4 next[kTurn];
+  int64_t next_target = 0;
+  float next_zt = 0.f, next_lse = 0.f, next_grad = 0.f;
+  const auto load = [&] {
+    if (row - targets_from >= 32) {
+      targets_from = row;
+      some_targets = a.targets[min(row + lane, a.rows - 1)];
+    }
+    next_target = __shfl_sync(0xffffffffu, static_cast<long long>(some_targets), static_cast<int>(row - targets_from));
+    if (next_target == a.ignore_index) return;
+    const Window<T> w(a, row);
+    if (MODE == kLoss && piece == 0)
+      next_zt = next_target >= 0 && next_target < vocab ? to_f32(w.z[next_target]) : NAN;
+    if (MODE != kLoss) {
+      next_lse = a.lse_in[row];
+      if (a.reduction == JK_REDUCE_NONE) next_grad = a.grad_loss[row];
+    }
+#pragma unroll
+    for (int i = 0; i < kTurn; ++i) {
+      const int k = piece * kPiece + i * 32 + lane, c = k * kP - w.shift;
+      if (c >= 0 && c + kP <= vocab) {
+        next[i] = __ldcs(reinterpret_cast<const uint4*>(w.z + c));
+      } else {  // -inf where there is no column
+        T* e = reinterpret_cast<T*>(&next[i]);
+#pragma unroll
+        for (int j = 0; j < kP; ++j) e[j] = c + j >= 0 && c + j < vocab ? w.z[c + j] : minus_inf<T>();
+      }
+    }
+  };
+  if (item < end) load();
+
+  Sum v{-INFINITY, 0.f};
+  float all = 0.f, zt = 0.f;
+  bool from_start = false, recorded[2] = {false, false};
+  Partial part{0.0, 0};
+  while (item < end) {
+    uint4 raw[kTurn];
+#pragma unroll
+    for (int i = 0; i < kTurn; ++i) raw[i] = next[i];
+    const int64_t r = row, target = next_target;
+    const int at_piece = piece;
+    const float lse = next_lse, grad_loss = next_grad;
+    if (piece == 0) {
+      from_start = true;
+      zt = next_zt;
+    }
+    ++item;
+    if (++piece == pieces) {
+      piece = 0;
+      ++row;
+    }
+    if (item < end) load();
+    const bool ignored = target == a.ignore_index;
+    if (MODE == kLoss) {
+      const bool last = at_piece == pieces - 1;
+      if (!ignored) {
+        take_packs<T>(v, raw);
+        if (a.smoothing != 0.f) {
+          const Window<T> w(a, r);
+#pragma unroll
+          for (int i = 0; i < kTurn; ++i) {
+            const int c = (at_piece * kPiece + i * 32 + lane) * kP - w.shift;
+            float f[kP];
+            unpack<T>(raw[i], f);
+#pragma unroll
+            for (int j = 0; j < kP; ++j) all += c + j >= 0 && c + j < vocab ? f[j] : 0.f;
+          }
+        }
+        if (last || item == end) {
+          v = warp_join(v);
+          if (a.smoothing != 0.f) all = warp_sum32(all);
+          if (last && from_start) {
+            const RowLoss l(v, zt, all, a.smoothing, vocab);
+            if (lane == 0) {
+              if (a.losses != nullptr) a.losses[r] = l.loss;
+              if (a.lse_out != nullptr) a.lse_out[r] = l.lse;
+            }
+            part.sum += l.loss;
+            part.rows += 1;
+          } else {
+            const int slot = r == first_row ? 0 : 1;
+            recorded[slot] = true;
+            if (lane == 0) records[2 * warp + slot] = {r, v.m, v.s, all};
+          }
+          v = {-INFINITY, 0.f};
+          all = 0.f;
+        }
+      } else if (last && lane == 0) {
+        if (a.losses != nullptr) a.losses[r] = 0.f;
+        if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
+      }
+    } else {
+      const Window<T> w(a, r);
+      T* g = a.grad + r * a.grad_stride;
+      const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(w.z)) & 15) == 0;
+      const bool inside = target >= 0 && target < vocab;
+      const Base base(lse);
+      const float c0 = !inside ? NAN : a.reduction == JK_REDUCE_NONE ? grad_loss : factor;
+      const float scale = c0 * expf(base.rest()), other = -share * c0;
+#pragma unroll
+      for (int i = 0; i < kTurn; ++i) {
+        const int c = (at_piece * kPiece + i * 32 + lane) * kP - w.shift;
+        if (c >= vocab) continue;
+        float f[kP] = {};
+        if (!ignored) {
+          unpack<T>(raw[i], f);
+          gradient_pack<T>(f, base, scale, other);
+          if (inside && target >= c && target < c + kP) {
+#pragma unroll
+            for (int j = 0; j < kP; ++j) f[j] -= c + j == target ? hit * c0 : 0.f;
+          }
+        }
+        if (alike && c >= 0 && c + kP <= vocab) {
+          __stcs(reinterpret_cast<uint4*>(g + c), pack<T>(f));
+        } else {
+#pragma unroll
+          for (int j = 0; j < kP; ++j)
+            if (c + j >= 0 && c + j < vocab) g[c + j] = from_f32<T>(f[j]);
+        }
+      }
+    }
+    if (at_piece == pieces - 1) from_start = false;
+  }
+  if (MODE != kLoss) return;
+  grid_dependency_launch();
+  if (lane == 0) {
+    for (int i = 0; i < 2; ++i)
+      if (!recorded[i]) records[2 * warp + i].row = -1;
+    a.partials[warp] = part;
+  }
+}
+
+// ---------------------------------------------------------------- loss and gradient at once
+// A cluster of blocks has a row, each block a slice of it in shared memory. One warp of the block
+// has the next rows' slices copied there and finds out how they lie; the others (workers) take a
+// slice twice, for the sum and for the gradient.
+#ifndef JKV_W
+#define JKV_W 224
+#endif
+#ifndef JKV_P
+#define JKV_P 3
+#endif
+constexpr int kWorkers = JKV_W;
+constexpr int kRowBlocksPerSm = JKV_P;
+constexpr int kMaxStages = 6;
+constexpr int kMaxCluster = 8;
+
+// A slice, in positions from the first element of its first pack.
+struct Slice {
+  int64_t row;
+  const void* in;        // position 0 of the logits
+  void* out;             // and of the gradient
+  int whole, whole_end;  // packs that are whole and in shared memory
+  int end;               // pack 0 (whole = 1) and pack whole_end (< end) are the row's ends
+  int low, high;         // positions that have a column
+  int at, owner;         // position of the target, or -1, and which thread has its pack, if whole, or -1
+  bool ignored, inside;  // target
+  bool head_outside, tail_outside;  // an end's pack reaches outside the logits: it is not in shared memory
+};
+
+struct Shared {
+  uint64_t full[kMaxStages], empty[kMaxStages], joined[2];
+  Slice slice[kMaxStages];
+  float4 warp[2][kWorkers / 32];  // (m, s, target logit, sum of logits) of each warp
+  float4 peer[2][kMaxCluster];    // and of each block of the cluster
+  int counts[kWorkers / 32];
+};
+
+__device__ __forceinline__ uint32_t map_peer(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void store_peer(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void arrive_peer(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity) {
+  const long long start = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok != 0) return true;
+    if (clock64() - start > JK_WAIT_LIMIT_CYCLES) return false;
+  }
+}
+
+// No block of a cluster ends while another may still write to its shared memory.
+__device__ __forceinline__ void leave(int cluster) {
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The loading warp: slices of rows first, first + step, ... A wait that runs out is recorded, and no
+// later one is waited for: the kernel then ends soon, with an error that jk_device_status reports.
+template <typename T>
+__device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsigned char* memory, int stages, int slice_packs,
+                                            int rank, int cluster, int64_t first, int64_t step) {
+  constexpr int kP = kPack<T>;
+  const int lane = threadIdx.x & 31, vocab = static_cast<int>(a.vocab);
+  bool good = true;
+  int n = 0, stage = 0;
+  uint32_t turn = 0;
+  int64_t ahead = 0;
+  for (int64_t r = first; r < a.rows; r += step, ++n) {
+    if (n % 32 == 0 && r + lane * step < a.rows) ahead = a.targets[r + lane * step];  // of the next 32 rows
+    const int64_t target = __shfl_sync(0xffffffffu, static_cast<long long>(ahead), n % 32);
+    if (turn > 0 && good) good = mbar_wait(&sh.empty[stage], (turn - 1) & 1);
+    if (lane == 0) {
+      const Window<T> w(a, r);
+      const int per = (w.packs + cluster - 1) / cluster;
+      const int begin = min(per * rank, w.packs), end = min(begin + per, w.packs);
+      const int origin = begin * kP - w.shift;  // column of position 0
+      Slice s;
+      s.row = r;
+      s.in = w.z + origin;
+      s.out = a.grad + r * a.grad_stride + origin;
+      s.end = end - begin;
+      s.low = max(0, -origin);
+      s.high = min(s.end * kP, vocab - origin);
+      s.whole = s.low > 0 ? 1 : 0;
+      s.whole_end = s.end > s.whole && s.high < s.end * kP ? s.end - 1 : s.end;
+      s.head_outside = s.whole == 1 && w.z - w.shift < a.logits;
+      s.tail_outside = s.whole_end < s.end && w.z - w.shift + w.packs * kP > a.logits + (a.rows - 1) * a.stride + vocab;
+      // a row of one pack may leave the logits at both ends
+      if (s.whole == 1 && s.end == 1) s.head_outside |= w.z - w.shift + kP > a.logits + (a.rows - 1) * a.stride + vocab;
+      s.ignored = target == a.ignore_index;
+      s.inside = target >= 0 && target < vocab;
+      const int at = s.inside ? static_cast<int>(target) - origin : -1;
+      s.at = at >= s.low && at < s.high ? at : -1;
+      const int pack = s.at / kP;
+      s.owner = s.at >= 0 && pack >= s.whole && pack < s.whole_end ? (pack - s.whole) % kWorkers : -1;
+      sh.slice[stage] = s;
+      const int from = s.head_outside ? 1 : 0, to = s.tail_outside ? s.whole_end : s.end;
+      const uint32_t bytes = !s.ignored && to > from ? static_cast<uint32_t>(to - from) * 16 : 0;
+      mbar_arrive_expect_tx(&sh.full[stage], bytes);
+      if (bytes > 0)
+        bulk_load(memory + (static_cast<size_t>(stage) * slice_packs + from) * 16, static_cast<const T*>(s.in) + from * kP, bytes,
+                  &sh.full[stage]);
+    }
+    __syncwarp();
+    if (++stage == stages) stage = 0, ++turn;
+  }
+  // copies in flight land before the block's memory is given back
+  for (int i = 0; i < stages; ++i) {
+    const uint32_t loads = turn + (i < stage ? 1 : 0);
+    if (loads > 0 && good) good = mbar_wait(&sh.full[i], (loads - 1) & 1);
+  }
+  if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
+}
+
+template <typename T, bool CLUSTER, bool SMOOTH>
+__global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
+    rows_kernel(const Args<T> a, int stages, int slice_packs, int cluster_size) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ Shared sh;
+  constexpr int kP = kPack<T>, kWarps = kWorkers / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cluster = CLUSTER ? cluster_size : 1;
+  const int rank = CLUSTER ? blockIdx.x % cluster : 0;
+  const int64_t first = blockIdx.x / cluster, step = gridDim.x / cluster;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], kWarps);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.joined[i], cluster);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (CLUSTER) {  // no block reaches for another's barriers before they are set up
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (warp == kWarps) {
+    load_slices(a, sh, memory, stages, slice_packs, rank, cluster, first, step);
+    leave(cluster);
+    return;
+  }
+  const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); };
+  const float factor = gradient_factor(a, true, kWorkers, sh.counts, sync);
+  const float hit = 1.f - a.smoothing, share = SMOOTH ? a.smoothing / static_cast<float>(a.vocab) : 0.f;
+  bool good = true;
   double sum = 0.0;
-  long long n = 0;
-  for (int i = threadIdx.x; i < blocks; i += 32) {
-    sum += partials[i].sum;
-    n += partials[i].rows;
+  int counted = 0, stage = 0, joins = 0;
+  uint32_t turn = 0;
+  for (int64_t r = first; r < a.rows; r += step) {
+    if (good) good = mbar_wait(&sh.full[stage], turn & 1);
+    const Slice& sl = sh.slice[stage];
+    const uint4* packs = reinterpret_cast<const uint4*>(memory) + static_cast<size_t>(stage) * slice_packs;
+    const int whole = sl.whole, whole_end = sl.whole_end;
+    uint4* out = static_cast<uint4*>(sl.out);
+    // the row's ends, thread 0 and 1: pack and whether it has to be fetched from the logits
+    const int end_pack = threadIdx.x == 0 && whole > 0 ? 0 : threadIdx.x == 1 && whole_end < sl.end ? whole_end : -1;
+    const bool outside = threadIdx.x == 0 ? sl.head_outside : sl.tail_outside;
+    const auto element = [&](int pos, bool from_logits) {
+      return to_f32(from_logits ? static_cast<const T*>(sl.in)[pos] : reinterpret_cast<const T*>(packs)[pos]);
+    };
+    if (sl.ignored) {
+      for (int k = whole + threadIdx.x; k < whole_end; k += kWorkers) out[k] = make_uint4(0, 0, 0, 0);
+      if (end_pack >= 0)
+        for (int pos = max(end_pack * kP, sl.low); pos < min(end_pack * kP + kP, sl.high); ++pos)
+          static_cast<T*>(sl.out)[pos] = from_f32<T>(0.f);
+      if (threadIdx.x == 0 && rank == 0) {
+        if (a.losses != nullptr) a.losses[r] = 0.f;
+        if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
+      }
+    } else {
+      Sum v{-INFINITY, 0.f};
+      float all = 0.f, zt = 0.f;
+      int k = whole + threadIdx.x;
+      for (; k + (kTurn - 1) * kWorkers < whole_end; k += kTurn * kWorkers) {
+        uint4 raw[kTurn];
+#pragma unroll
+        for (int i = 0; i < kTurn; ++i) raw[i] = packs[k + i * kWorkers];
+        take_packs<T>(v, raw);
+        if (SMOOTH) all += pack_sum<T>(raw);
+      }
+      for (; k < whole_end; k += kWorkers) {
+        const uint4 raw[1] = {packs[k]};
+        take_packs<T>(v, raw);
+        if (SMOOTH) all += pack_sum<T>(raw);
+      }
+      if (end_pack >= 0) {
+        for (int pos = max(end_pack * kP, sl.low); pos < min(end_pack * kP + kP, sl.high); ++pos) {
+          float f[1] = {element(pos, outside)};
+          all += f[0];
+          take(v, f);
+        }
+      }
+      if (threadIdx.x == 0 && sl.at >= 0)
+        zt = element(sl.at, (sl.at < kP && sl.head_outside) || (sl.at >= whole_end * kP && sl.tail_outside));
+      v = warp_join(v);
+      if (SMOOTH) all = warp_sum32(all);
+      // of three rows that count, the warps of a block are never in the first and the third at once
+      if (lane == 0) sh.warp[joins & 1][warp] = make_float4(v.m, v.s, zt, all);
+      sync();
+      float4 q = lane < kWarps ? sh.warp[joins & 1][lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      v = warp_join({q.x, q.y});
+      if (SMOOTH) all = warp_sum32(q.w);
+      zt = q.z;  // of the first warp's first thread
+      if (CLUSTER) {  // neither are the blocks of a cluster, so a slot and a barrier are free again
+        zt = __shfl_sync(0xffffffffu, zt, 0);
+        if (threadIdx.x < cluster) {
+          store_peer(map_peer(&sh.peer[joins & 1][rank], threadIdx.x), make_float4(v.m, v.s, zt, all));
+          arrive_peer(map_peer(&sh.joined[joins & 1], threadIdx.x));
+        }
+        if (good) good = wait_cluster(&sh.joined[joins & 1], (joins >> 1) & 1);
+        q = lane < cluster ? sh.peer[joins & 1][lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        v = warp_join({q.x, q.y});
+        zt = warp_sum32(q.z);
+        if (SMOOTH) all = warp_sum32(q.w);
+      }
+      ++joins;
+      if (threadIdx.x == 0 && rank == 0) {
+        const RowLoss l(v, sl.inside ? zt : NAN, all, a.smoothing, a.vocab);
+        if (a.losses != nullptr) a.losses[r] = l.loss;
+        if (a.lse_out != nullptr) a.lse_out[r] = l.lse;
+        sum += l.loss;
+        ++counted;
+      }
+      const Base base(v.m);
+      const float c0 = sl.inside ? factor : NAN, scale = __fdividef(c0, v.s), other = -share * c0;
+      k = whole + threadIdx.x;
+      for (; k + (kTurn - 1) * kWorkers < whole_end; k += kTurn * kWorkers) {
+#pragma unroll
+        for (int i = 0; i < kTurn; ++i) {
+          float f[kP];
+          unpack<T>(packs[k + i * kWorkers], f);
+          gradient_pack<T>(f, base, scale, other);
+          out[k + i * kWorkers] = pack<T>(f);
+        }
+      }
+      for (; k < whole_end; k += kWorkers) {
+        float f[kP];
+        unpack<T>(packs[k], f);
+        gradient_pack<T>(f, base, scale, other);
+        out[k] = pack<T>(f);
+      }
+      if (threadIdx.x == sl.owner)  // after its pack
+        static_cast<T*>(sl.out)[sl.at] = from_f32<T>(fmaf(base.exp(element(sl.at, false)), scale, other) - hit * c0);
+      if (end_pack >= 0) {
+        for (int pos = max(end_pack * kP, sl.low); pos < min(end_pack * kP + kP, sl.high); ++pos)
+          static_cast<T*>(sl.out)[pos] =
+              from_f32<T>(fmaf(base.exp(element(pos, outside)), scale, other) - (pos == sl.at ? hit * c0 : 0.f));
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.empty[stage]);
+    if (++stage == stages) stage = 0, ++turn;
   }
+  if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
+  grid_dependency_launch();
+  if (threadIdx.x == 0) a.partials[blockIdx.x] = {sum, counted};
+  leave(cluster);
+}
+
+// ---------------------------------------------------------------- reduction over rows
+// The partial sums in their order, and the rows that warps have left in parts. The last block to
+// come adds up what the blocks have (the order of the sum does not depend on which that is).
+constexpr int kReduceBlocks = 32;
+
+struct Ticket {
+  Partial blocks[kReduceBlocks];
+  int come;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    reduce_kernel(const Args<T> a, int partials, const Record* records, int record_count, float* loss, Ticket* ticket) {
+  __shared__ Partial parts[8];
+  __shared__ bool last;
+  grid_dependency_wait();
+  const int at = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+  Partial p{0.0, 0};
+  for (int i = at; i < partials; i += step) {
+    p.sum += a.partials[i].sum;
+    p.rows += a.partials[i].rows;
+  }
+  for (int i = at; i < record_count; i += step) {
+    const Record head = records[i];
+    if (head.row < 0) continue;
+    // the records of a row follow one another, with one unused between two of them at most
+    const bool begun = (i >= 1 && records[i - 1].row == head.row) || (i >= 2 && records[i - 2].row == head.row);
+    if (begun) continue;
+    Sum v{head.m, head.s};
+    float all = head.all;
+    for (int j = i + 1, unused = 0; j < record_count && unused < 2; ++j) {
+      const Record q = records[j];
+      if (q.row < 0) {
+        ++unused;
+        continue;
+      }
+      if (q.row != head.row) break;
+      unused = 0;
+      const float m = fmaxf(v.m, q.m);
+      const float f = v.m == m ? 1.f : factor_to(v.m, m), g = q.m == m ? 1.f : factor_to(q.m, m);
+      v = {m, v.s * f + q.s * g};
+      all += q.all;
+    }
+    const int64_t target = a.targets[head.row];
+    const float zt = target >= 0 && target < a.vocab ? to_f32(a.logits[head.row * a.stride + target]) : NAN;
+    const RowLoss l(v, zt, all, a.smoothing, a.vocab);
+    if (a.losses != nullptr) a.losses[head.row] = l.loss;
+    if (a.lse_out != nullptr) a.lse_out[head.row] = l.lse;
+    p.sum += l.loss;
+    p.rows += 1;
+  }
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    n += __shfl_xor_sync(0xffffffffu, n, o);
+    p.sum += __shfl_xor_sync(0xffffffffu, p.sum, o);
+    p.rows += __shfl_xor_sync(0xffffffffu, p.rows, o);
   }
-  if (threadIdx.x == 0) *loss = static_cast<float>(reduction == JK_REDUCE_MEAN ? sum / static_cast<double>(n) : sum);
+  if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = p;
+  __syncthreads();
+  if (threadIdx.x != 0 || loss == nullptr) return;
+  for (int i = 1; i < 8; ++i) p.sum += parts[i].sum, p.rows += parts[i].rows;
+  if (gridDim.x > 1) {
+    ticket->blocks[blockIdx.x] = p;
+    __threadfence();
+    last = atomicAdd(&ticket->come, 1) == static_cast<int>(gridDim.x) - 1;
+    if (!last) return;
+    __threadfence();
+    p = {0.0, 0};
+    for (int i = 0; i < static_cast<int>(gridDim.x); ++i) {
+      const volatile Partial* q = &ticket->blocks[i];
+      p.sum += q->sum;
+      p.rows += q->rows;
+    }
+  }
+  *loss = static_cast<float>(a.reduction == JK_REDUCE_MEAN ? p.sum / static_cast<double>(p.rows) : p.sum);
+}
+
+// ---------------------------------------------------------------- launches
+// The caller's workspace. (With one record for each of a warp's runs' ends.)
+struct Workspace {
+  Partial partials[kMaxWarps > kMaxBlocks ? kMaxWarps : kMaxBlocks];
+  Record records[2 * kMaxWarps];
+  Ticket ticket;
+  int counts[kCounts];
+};
+
+constexpr int kWarpColumns = 1024;  // of the rows that a warp holds
+
+template <typename T, int MODE, int VEC>
+void launch_warps(const Args<T>& a, int blocks, cudaStream_t s) {
+  const int64_t turns = (a.vocab + 32 * VEC - 1) / (32 * VEC);
+  constexpr int kMost = kWarpColumns / 32 / VEC;
+  if constexpr (VEC == 1) {
+    if (turns <= 2) warp_kernel<T, MODE, VEC, 2><<<blocks, kWarpThreads, 0, s>>>(a);
+    else if (turns <= 8) warp_kernel<T, MODE, VEC, 8><<<blocks, kWarpThreads, 0, s>>>(a);
+    else warp_kernel<T, MODE, VEC, kMost><<<blocks, kWarpThreads, 0, s>>>(a);
+  } else {
+    if (turns <= 1) warp_kernel<T, MODE, VEC, 1><<<blocks, kWarpThreads, 0, s>>>(a);
+    else if (turns <= 2) warp_kernel<T, MODE, VEC, 2><<<blocks, kWarpThreads, 0, s>>>(a);
+    else warp_kernel<T, MODE, VEC, kMost><<<blocks, kWarpThreads, 0, s>>>(a);
+  }
+}
+
+// What the reduction over rows will find.
+struct Left {
+  int partials = 0, records = 0;
+};
+
+template <typename T, int MODE>
+Left launch_stream(const Args<T>& a, Workspace* ws, cudaStream_t s) {
+  const int packs = static_cast<int>((a.vocab + 2 * (kPack<T> - 1)) / kPack<T>);  // of a row, wherever it begins
+  const int pieces = (packs + kPiece - 1) / kPiece;
+  // a run of four pieces or more keeps the records of a row few
+  const int64_t want = (a.rows * pieces + 4 * (kStreamThreads / 32) - 1) / (4 * (kStreamThreads / 32));
+  const int blocks = static_cast<int>(want < 148 * kStreamBlocksPerSm ? want : 148 * kStreamBlocksPerSm);
+  stream_kernel<T, MODE><<<blocks, kStreamThreads, 0, s>>>(a, pieces, ws->records, &ws->ticket.come);
+  return {blocks * (kStreamThreads / 32), 2 * blocks * (kStreamThreads / 32)};
+}
+
+constexpr int64_t kRoom = 212 * 1024;  // of an SM's shared memory, for the slices of all its blocks
+constexpr int64_t kFewRows = 74;       // so few rows leave half of the SMs without a block
+
+template <typename T, bool CLUSTER, bool SMOOTH>
+bool launch_rows(const Args<T>& a, int64_t blocks, int stages, int slice_packs, int cluster, cudaStream_t s) {
+  auto kernel = rows_kernel<T, CLUSTER, SMOOTH>;
+  const size_t smem = static_cast<size_t>(stages) * slice_packs * 16;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return false;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kWorkers + 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, stages, slice_packs, cluster) == cudaSuccess;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    backward_kernel(const float* grad_loss, const T* logits, int64_t stride, const int64_t* targets, const float* lse,
-                    int64_t rows, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, T* grad,
-                    int64_t grad_stride) {
-  __shared__ int counted;
-  float w = 1.f;
-  if (reduction == JK_REDUCE_MEAN) w = 1.f / static_cast<float>(count_rows(targets, rows, ignore_index, &counted));
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t target = targets[r];
-    T* g = grad + r * grad_stride;
-    if (target == ignore_index) {
-      for (int64_t j = threadIdx.x; j < vocab; j += kThreads) g[j] = from_f32<T>(0.f);
-      continue;
-    }
-    const float c = target >= 0 && target < vocab ? w * grad_loss[reduction == JK_REDUCE_NONE ? r : 0] : NAN;
-    write_grad(logits + r * stride, g, vocab, lse[r], 1.f, c, target, smoothing);
+int launch_warp_rows(const Args<T>& a, int mode, cudaStream_t s) {
+  const bool aligned = a.vocab % kPack<T> == 0 && a.stride % kPack<T> == 0 && aligned16(a.logits) &&
+                       (mode == kLoss || (a.grad_stride % kPack<T> == 0 && aligned16(a.grad)));
+  const int64_t want = (a.rows + kWarpThreads / 32 - 1) / (kWarpThreads / 32);
+  const int blocks = static_cast<int>(want < kMaxBlocks ? want : kMaxBlocks);
+  if (mode == kLoss) {
+    if (aligned) launch_warps<T, kLoss, kPack<T>>(a, blocks, s); else launch_warps<T, kLoss, 1>(a, blocks, s);
+  } else if (mode == kBoth) {
+    if (aligned) launch_warps<T, kBoth, kPack<T>>(a, blocks, s); else launch_warps<T, kBoth, 1>(a, blocks, s);
+  } else {
+    if (aligned) launch_warps<T, kBackward, kPack<T>>(a, blocks, s); else launch_warps<T, kBackward, 1>(a, blocks, s);
   }
+  return blocks;
 }
 
-inline int blocks_for(int64_t rows) { return static_cast<int>(rows < kMaxBlocks ? rows : kMaxBlocks); }
+// Both at once, where rows_kernel can: slices of all blocks fit, twice (one that is worked on, one
+// that is on its way), and gradient and logits lie alike against 16 bytes. Returns the partials, or 0.
+template <typename T>
+int launch_both(const Args<T>& a, cudaStream_t s) {
+  const bool alike = (a.stride - a.grad_stride) % kPack<T> == 0 &&
+                     ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
+  const int64_t packs = (a.vocab + 2 * (kPack<T> - 1)) / kPack<T>;
+  if (!alike || 2 * 16 * packs > kRoom * kMaxCluster) return 0;
+  int cluster = 1;
+  while (cluster < kMaxCluster && (2 * 16 * ((packs + cluster - 1) / cluster) > kRoom || (a.rows * cluster <= kFewRows && packs >= 1024 * cluster)))
+    cluster *= 2;
+  const int slice = static_cast<int>((packs + cluster - 1) / cluster);
+  if (2 * 16ll * slice > kRoom) return 0;
+  int per_sm = kRowBlocksPerSm;
+  while (per_sm > 1 && 2 * 16ll * slice * per_sm > kRoom) --per_sm;
+  const int64_t fit = kRoom / per_sm / (16ll * slice);
+  const int stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
+  int64_t clusters = 148 * per_sm / cluster;
+  if (clusters > a.rows) clusters = a.rows;
+  const int64_t blocks = clusters * cluster;
+  const bool smooth = a.smoothing != 0.f;
+  bool done;
+  if (cluster > 1) done = smooth ? launch_rows<T, true, true>(a, blocks, stages, slice, cluster, s) : launch_rows<T, true, false>(a, blocks, stages, slice, cluster, s);
+  else done = smooth ? launch_rows<T, false, true>(a, blocks, stages, slice, cluster, s) : launch_rows<T, false, false>(a, blocks, stages, slice, cluster, s);
+  return done ? static_cast<int>(blocks) : -1;
+}
+
+// Where many rows have to be counted for the gradient's factor, a kernel of its own does it first.
+template <typename T>
+void count_apart(Args<T>& a, Workspace* ws, cudaStream_t s) {
+  if (a.reduction != JK_REDUCE_MEAN || a.rows <= kCountRows) return;
+  count_kernel<<<kCounts, 256, 0, s>>>(a.targets, a.rows, a.ignore_index, ws->counts);
+  a.counts = ws->counts;
+}
+
+template <typename T>
+int backward(Args<T> a, Workspace* ws, cudaStream_t s) {
+  count_apart(a, ws, s);
+  if (a.vocab <= kWarpColumns) launch_warp_rows(a, kBackward, s);
+  else launch_stream<T, kBackward>(a, ws, s);
+  return launch_status();
+}
+
+template <typename T>
+int forward(Args<T> a, float* loss, Workspace* ws, cudaStream_t s) {
+  Left left;
+  bool gradient_later = false;
+  a.partials = ws == nullptr ? nullptr : ws->partials;
+  if (a.rows > 0) {
+    if (a.grad != nullptr) count_apart(a, ws, s);
+    if (a.vocab <= kWarpColumns) {
+      left.partials = launch_warp_rows(a, a.grad != nullptr ? kBoth : kLoss, s);
+    } else {
+      if (a.grad != nullptr) left.partials = launch_both(a, s);
+      if (left.partials < 0) {
+        cudaGetLastError();
+        return JK_ERR_LAUNCH;
+      }
+      if (left.partials == 0) {
+        gradient_later = a.grad != nullptr;
+        if (gradient_later && a.lse_out == nullptr) a.lse_out = reinterpret_cast<float*>(ws + 1);
+        left = launch_stream<T, kLoss>(a, ws, s);
+      }
+    }
+  }
+  if (loss != nullptr || left.records > 0) {
+    launch_dependent(reduce_kernel<T>, left.records > 0 ? kReduceBlocks : 1, 256, 0, s, a, left.partials, ws == nullptr ? nullptr : ws->records, left.records, loss,
+                     ws == nullptr ? nullptr : &ws->ticket);
+  }
+  if (gradient_later) {
+    a.lse_in = a.lse_out;
+    launch_stream<T, kLater>(a, ws, s);
+  }
+  return launch_status();
+}
 
 }  // namespace loss
 
@@ -165,7 +1124,8 @@ JK_ERROR_READER(read_error_loss)
 }  // namespace jk
 
 extern "C" int64_t jk_cross_entropy_workspace(int64_t rows) {
-  return rows <= 0 ? 0 : jk::loss::blocks_for(rows) * static_cast<int64_t>(sizeof(jk::loss::Partial));
+  // and a log-sum of each row, for a gradient that is taken in a second pass
+  return rows <= 0 ? 0 : static_cast<int64_t>(sizeof(jk::loss::Workspace)) + (rows + 1) / 2 * 8;
 }
 
 extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
@@ -173,7 +1133,7 @@ extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_strid
                                         int reduction, float grad_scale, float* losses, float* lse, float* loss,
                                         void* grad, int64_t grad_stride, void* workspace, jk_stream_t stream) {
   using namespace jk;
-  if (rows < 0 || vocab <= 0 || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
+  if (rows < 0 || vocab <= 0 || vocab > loss::kMaxVocab || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
   if (!float_dtype(dtype)) return JK_ERR_BAD_DTYPE;
   if (reduction < JK_REDUCE_NONE || reduction > JK_REDUCE_SUM) return JK_ERR_UNSUPPORTED_KIND;
   if (!(label_smoothing >= 0.f && label_smoothing <= 1.f)) return JK_ERR_BAD_ARG;
@@ -183,38 +1143,36 @@ extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_strid
   if ((reinterpret_cast<uintptr_t>(workspace) & 7u) != 0) return JK_ERR_ALIGNMENT;
   int st = check_device();
   if (st != JK_OK) return st;
-  auto s = reinterpret_cast<cudaStream_t>(stream);
-  auto* partials = static_cast<loss::Partial*>(workspace);
-  const int blocks = rows == 0 ? 0 : loss::blocks_for(rows);
-  if (rows > 0) {
-    JK_WITH_TYPE(dtype, T, {
-      loss::forward_kernel<T><<<blocks, loss::kThreads, 0, s>>>(
-          static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index, label_smoothing, reduction,
-          grad_scale, losses, lse, static_cast<T*>(grad), grad_stride, partials);
-    });
-  }
-  if (loss != nullptr) loss::reduce_kernel<<<1, 32, 0, s>>>(partials, blocks, reduction, loss);
-  return launch_status();
+  JK_WITH_TYPE(dtype, T, {
+    const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
+                          label_smoothing, reduction, grad_scale, nullptr, nullptr, losses, lse,
+                          static_cast<T*>(grad), grad_stride, nullptr, nullptr};
+    st = loss::forward<T>(a, loss, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+  });
+  return st;
 }
 
 extern "C" int jk_cross_entropy_backward(const float* grad_loss, const void* logits, int64_t logits_stride,
                                          const int64_t* targets, const float* lse, int64_t rows, int64_t vocab, int dtype,
                                          int64_t ignore_index, float label_smoothing, int reduction, void* grad,
-                                         int64_t grad_stride, jk_stream_t stream) {
+                                         int64_t grad_stride, void* workspace, jk_stream_t stream) {
   using namespace jk;
-  if (rows < 0 || vocab <= 0 || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
+  if (rows < 0 || vocab <= 0 || vocab > loss::kMaxVocab || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
   if (!float_dtype(dtype)) return JK_ERR_BAD_DTYPE;
   if (reduction < JK_REDUCE_NONE || reduction > JK_REDUCE_SUM) return JK_ERR_UNSUPPORTED_KIND;
   if (!(label_smoothing >= 0.f && label_smoothing <= 1.f)) return JK_ERR_BAD_ARG;
   if (rows == 0) return JK_OK;
-  if (grad_loss == nullptr || logits == nullptr || targets == nullptr || lse == nullptr || grad == nullptr)
+  if (grad_loss == nullptr || logits == nullptr || targets == nullptr || lse == nullptr || grad == nullptr ||
+      workspace == nullptr)
     return JK_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 7u) != 0) return JK_ERR_ALIGNMENT;
   int st = check_device();
   if (st != JK_OK) return st;
   JK_WITH_TYPE(dtype, T, {
-    loss::backward_kernel<T><<<loss::blocks_for(rows), loss::kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-        grad_loss, static_cast<const T*>(logits), logits_stride, targets, lse, rows, vocab, ignore_index, label_smoothing,
-        reduction, static_cast<T*>(grad), grad_stride);
+    const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
+                          label_smoothing, reduction, 1.f, grad_loss, lse, nullptr, nullptr, static_cast<T*>(grad),
+                          grad_stride, nullptr, nullptr};
+    st = loss::backward<T>(a, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });
-  return launch_status();
+  return st;
 }

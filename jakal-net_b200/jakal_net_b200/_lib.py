@@ -140,7 +140,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "jk_cross_entropy_backward": (
         _i32,
         [_p, _p, _i64, _p, _p, _i64, _i64, _i32,  # grad_loss, logits, stride, targets, lse, rows, vocab, dtype
-         _i64, _f32, _i32, _p, _i64, _p],         # ignore_index, label_smoothing, reduction, grad, stride, stream
+         _i64, _f32, _i32, _p, _i64, _p, _p],     # ignore_index, label_smoothing, reduction, grad, stride, workspace, stream
     ),
     "jk_clip_grad_norm_workspace": (_i64, []),
     "jk_clip_grad_norm": (

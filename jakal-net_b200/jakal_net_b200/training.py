@@ -42,6 +42,7 @@ __all__ = [
 
 _LIBRARY = load()
 _DTYPE_CODE = {torch.float32: _lib.JK_F32, torch.bfloat16: _lib.JK_BF16, torch.float16: _lib.JK_F16}
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _REDUCTION = {"none": _lib.JK_REDUCE_NONE, "mean": _lib.JK_REDUCE_MEAN, "sum": _lib.JK_REDUCE_SUM}
 
 
@@ -85,10 +86,6 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
     return t.contiguous(), t.shape[-1]
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
 def _written(tensors: list[Tensor]) -> None:
     """Tells autograd that the kernels wrote over these tensors (a value kept for a backward
     pass is then seen to be stale)."""
@@ -96,23 +93,16 @@ def _written(tensors: list[Tensor]) -> None:
         torch.autograd.graph.increment_version(tensors)
 
 
-class _On:
-    """Makes `device` current for the block where it is not."""
-
-    __slots__ = ("device", "guard")
-
-    def __init__(self, device: torch.device):
-        self.device = device
-
-    def __enter__(self):
-        self.guard = None
-        if torch._C._cuda_getDevice() != self.device.index:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(fn, where: str, device: int, *args) -> None:
+    """fn(*args, stream) on the device's current stream, with the device current; raises on a
+    status that is not 0."""
+    if _current_device() == device:
+        status = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(device))
+    if status:
+        check(status, where)
 
 
 def _param(name: str, p: Optional[Tensor], x: Tensor, dim: int) -> Optional[Tensor]:
@@ -124,6 +114,11 @@ def _param(name: str, p: Optional[Tensor], x: Tensor, dim: int) -> Optional[Tens
     if p.shape != (dim,):
         raise ValueError(f"{name} has shape {tuple(p.shape)}, expected {(dim,)}")
     return p if p.is_contiguous() else p.detach().contiguous()
+
+
+def _empty_like(t: Tensor) -> Tensor:
+    """An uninitialised contiguous tensor of t's shape, dtype and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
@@ -154,18 +149,13 @@ def layer_norm_forward_cuda(x: Tensor, weight: Optional[Tensor] = None, bias: Op
     if delta is not None:
         _same("delta", delta, x)
         dr, d_stride = _rows(delta)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty_like(x)
     total = x if delta is None else torch.empty_like(y)
-    stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    with _On(x.device):
-        check(
-            _LIBRARY.jk_layer_norm_forward(
-                xr.data_ptr(), x_stride, _ptr(dr), d_stride, delta_scale, _ptr(weight), _ptr(bias),
-                code if some is None else _DTYPE_CODE[some.dtype], mean.numel(), dim, code, eps, y.data_ptr(),
-                None if delta is None else total.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(x.device)),
-            "jk_layer_norm_forward",
-        )
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _call(_LIBRARY.jk_layer_norm_forward, "jk_layer_norm_forward", x.get_device(), xr.data_ptr(), x_stride, _ptr(dr), d_stride,
+          delta_scale, _ptr(weight), _ptr(bias), code if some is None else _DTYPE_CODE[some.dtype], mean.numel(), dim, code,
+          eps, y.data_ptr(), None if delta is None else total.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, total, mean, rstd
 
 
@@ -196,24 +186,18 @@ def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Te
         _same("grad_sum", grad_sum, sum)
         gs, gs_stride = _rows(grad_sum)
     rows = mean.numel()
-    grad_x = torch.empty(sum.shape, dtype=sum.dtype, device=sum.device)
+    grad_x = _empty_like(sum)
     grad_delta = grad_x if delta_scale == 1.0 else torch.empty_like(grad_x)
     grad_weight = grad_bias = work = None
     pcode = code if weight is None else _DTYPE_CODE[weight.dtype]
     if param_grads:
-        ptype = sum.dtype if weight is None else weight.dtype
-        grad_weight, grad_bias = torch.empty((2, dim), dtype=ptype, device=sum.device).unbind(0)
-        work = torch.empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),), dtype=torch.float32,
-                           device=sum.device)
-    with _On(sum.device):
-        check(
-            _LIBRARY.jk_layer_norm_backward(
-                gy.data_ptr(), gy_stride, hr.data_ptr(), h_stride, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), pcode,
-                _ptr(gs), gs_stride, delta_scale, rows, dim, code, grad_x.data_ptr(),
-                None if grad_delta is grad_x else grad_delta.data_ptr(), _ptr(grad_weight), _ptr(grad_bias), _ptr(work),
-                _stream(sum.device)),
-            "jk_layer_norm_backward",
-        )
+        grad_weight = torch.empty_like(weight) if weight is not None else sum.new_empty((dim,))
+        grad_bias = torch.empty_like(grad_weight)
+        work = mean.new_empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),))
+    _call(_LIBRARY.jk_layer_norm_backward, "jk_layer_norm_backward", sum.get_device(), gy.data_ptr(), gy_stride, hr.data_ptr(),
+          h_stride, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), pcode, _ptr(gs), gs_stride, delta_scale, rows, dim, code,
+          grad_x.data_ptr(), None if grad_delta is grad_x else grad_delta.data_ptr(), _ptr(grad_weight), _ptr(grad_bias),
+          _ptr(work))
     return grad_x, grad_delta, grad_weight, grad_bias
 
 
@@ -271,29 +255,38 @@ def _loss_inputs(logits: Tensor, targets: Tensor, reduction: str):
     return code, targets, kind, lr, stride
 
 
+def _grad_like(logits: Tensor) -> Tensor:
+    """An uninitialised gradient whose rows lie as the logits' rows do, 16-byte blocks and padding
+    between rows included, where those are equally spaced and apart; else a contiguous one."""
+    shift = logits.data_ptr() % 16
+    if logits.is_contiguous() and not shift:
+        return torch.empty_like(logits)
+    rows, stride = _rows(logits)
+    if logits.numel() == 0 or rows.data_ptr() != logits.data_ptr() or stride < logits.shape[-1]:
+        return _empty_like(logits)
+    shift //= logits.element_size()
+    n = logits.numel() // logits.shape[-1]
+    return logits.new_empty((shift + n * stride,)).as_strided(logits.shape, logits.stride(), shift)
+
+
 def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, grad_scale, want_lse, grad, in_place=False):
     code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
-    rows, dev = targets.numel(), logits.device
+    rows = targets.numel()
     lse = losses = None
-    if want_lse:
-        lse = torch.empty(targets.shape, dtype=torch.float32, device=dev)
     if kind == _lib.JK_REDUCE_NONE:
-        loss = losses = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+        loss = losses = logits.new_empty(targets.shape, dtype=torch.float32)
     else:
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-    work = torch.empty((_LIBRARY.jk_cross_entropy_workspace(rows),), dtype=torch.uint8, device=dev)
+        loss = logits.new_empty((), dtype=torch.float32)
+    if want_lse:
+        lse = torch.empty_like(loss) if losses is not None else loss.new_empty(targets.shape)
+    work = loss.new_empty((_LIBRARY.jk_cross_entropy_workspace(rows) // 4,))
     if in_place:
         grad_ptr, grad_stride = lr.data_ptr(), stride
     else:
-        grad_ptr, grad_stride = _ptr(grad), logits.shape[-1]
-    with _On(dev):
-        check(
-            _LIBRARY.jk_cross_entropy_forward(
-                lr.data_ptr(), stride, targets.data_ptr(), rows, logits.shape[-1], code, ignore_index, label_smoothing,
-                kind, grad_scale, _ptr(losses), _ptr(lse), None if losses is not None else loss.data_ptr(), grad_ptr,
-                grad_stride, work.data_ptr(), _stream(dev)),
-            "jk_cross_entropy_forward",
-        )
+        grad_ptr, grad_stride = (None, 0) if grad is None else (grad.data_ptr(), _rows(grad)[1])
+    _call(_LIBRARY.jk_cross_entropy_forward, "jk_cross_entropy_forward", logits.get_device(), lr.data_ptr(), stride,
+          targets.data_ptr(), rows, logits.shape[-1], code, ignore_index, label_smoothing, kind, grad_scale, _ptr(losses),
+          _ptr(lse), None if losses is not None else loss.data_ptr(), grad_ptr, grad_stride, work.data_ptr())
     return loss, lse
 
 
@@ -312,8 +305,8 @@ def cross_entropy_with_grad_cuda(logits: Tensor, targets: Tensor, ignore_index: 
                                  reduction: str = "mean", grad_scale: float = 1.0, in_place: bool = False):
     """The loss ("mean" or "sum") and, in the same pass over the logits, their gradient.
 
-    Returns (loss, grad): grad = grad_scale * d loss / d logits in logits' dtype (grad_scale: a
-    loss scaler's factor), for ``logits.backward(grad)`` or a head's own backward. in_place
+    Returns (loss, grad): grad = grad_scale * d loss / d logits in logits' dtype, its rows spaced
+    as theirs (grad_scale: a loss scaler's factor), for ``logits.backward(grad)`` or a head's own backward. in_place
     writes it over the logits, which must then have rows that are contiguous inside, equally
     spaced and apart."""
     if reduction == "none":
@@ -331,7 +324,7 @@ def cross_entropy_with_grad_cuda(logits: Tensor, targets: Tensor, ignore_index: 
                                  False, None, in_place=True)
         _written([logits])
         return loss, logits
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = _grad_like(logits)
     loss, _ = _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
                              False, grad)
     return loss, grad
@@ -352,15 +345,11 @@ def cross_entropy_backward_cuda(grad_loss: Tensor, logits: Tensor, targets: Tens
         raise ValueError(f"grad_loss has shape {tuple(grad_loss.shape)}, which does not fit reduction {reduction!r}")
     gl = grad_loss.detach().to(torch.float32).contiguous()
     lse = lse.contiguous()
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    with _On(logits.device):
-        check(
-            _LIBRARY.jk_cross_entropy_backward(
-                gl.data_ptr(), lr.data_ptr(), stride, targets.data_ptr(), lse.data_ptr(), targets.numel(),
-                logits.shape[-1], code, int(ignore_index), float(label_smoothing), kind, grad.data_ptr(), logits.shape[-1],
-                _stream(logits.device)),
-            "jk_cross_entropy_backward",
-        )
+    grad = _grad_like(logits)
+    work = lse.new_empty((_LIBRARY.jk_cross_entropy_workspace(targets.numel()) // 4,))
+    _call(_LIBRARY.jk_cross_entropy_backward, "jk_cross_entropy_backward", logits.get_device(), gl.data_ptr(), lr.data_ptr(),
+          stride, targets.data_ptr(), lse.data_ptr(), targets.numel(), logits.shape[-1], code, int(ignore_index),
+          float(label_smoothing), kind, grad.data_ptr(), _rows(grad)[1], work.data_ptr())
     return grad
 
 
@@ -389,7 +378,7 @@ def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100, lab
 
 # ----------------------------------------------------------------------------- gradient norm
 _NORM = {2.0: _lib.JK_NORM_2, math.inf: _lib.JK_NORM_INF}
-_CLIP_WORKSPACE = int(_LIBRARY.jk_clip_grad_norm_workspace())
+_CLIP_WORKSPACE = int(_LIBRARY.jk_clip_grad_norm_workspace()) // 8  # f64 elements
 
 
 def _flat(t: Tensor) -> bool:
@@ -404,59 +393,58 @@ def _flat(t: Tensor) -> bool:
 
 def _gradients(grads, name: str) -> list[Tensor]:
     tensors = [grads] if isinstance(grads, Tensor) else [g for g in grads if g is not None]
-    if tensors:
-        # one look at all of them; what is wrong with which is only sought when something is
-        dev = tensors[0].device if isinstance(tensors[0], Tensor) else None
-        if not (all(isinstance(t, Tensor) for t in tensors) and {t.device for t in tensors} == {dev}
-                and dev.type == "cuda" and _DTYPE_CODE.keys() >= {t.dtype for t in tensors}):
-            for i, t in enumerate(tensors):
-                _check_input(f"{name} {i}", t)
-                if t.device != dev:
-                    raise RuntimeError(f"{name} {i} is on {t.device}, expected {dev}")
+    # one look at all of them (a model has hundreds); which one is wrong is sought only if one is
+    try:
+        fine = (len(set(map(Tensor.get_device, tensors))) <= 1 and all(map(Tensor.is_cuda.__get__, tensors))
+                and set(map(Tensor.dtype.__get__, tensors)) <= _DTYPE_CODE.keys())
+    except TypeError:  # not a tensor
+        fine = False
+    if not fine:
+        for i, t in enumerate(tensors):
+            _check_input(f"{name} {i}", t)
+            if t.device != tensors[0].device:
+                raise RuntimeError(f"{name} {i} is on {t.device}, expected {tensors[0].device}")
     return tensors
 
 
-def _addresses(tensors: list[Tensor]) -> array.array:
-    return array.array("Q", [t.data_ptr() for t in tensors])
-
-
-def _codes(tensors: list[Tensor]) -> array.array:
-    return array.array("i", [_DTYPE_CODE[t.dtype] for t in tensors])
+def _table(tensors: list[Tensor]) -> tuple[array.array, array.array]:
+    """The addresses and the dtype codes."""
+    types = list(map(Tensor.dtype.__get__, tensors))
+    codes = array.array("i", map(_DTYPE_CODE.__getitem__, types))
+    return array.array("Q", map(Tensor.data_ptr, tensors)), codes
 
 
 def _run_clip(tensors, outs, norm_type, clip, max_norm):
     kind = _NORM.get(float(norm_type))
     if kind is None:
         raise ValueError(f"unsupported norm_type {norm_type} (2 or inf)")
-    dev = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
-    src, dst, back = tensors, outs, []
-    if not (all(t.is_contiguous() for t in tensors) and (outs is None or all(t.is_contiguous() for t in outs))):
+    src, dst, back = tensors, outs, None
+    if not (all(map(Tensor.is_contiguous, tensors)) and (outs is None or all(map(Tensor.is_contiguous, outs)))):
         if clip:
             for t in tensors if outs is None else outs:
                 if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
                     raise ValueError("a tensor to write has elements that share memory (an expanded tensor)")
         src, dst, back = _blocks(tensors, outs, clip)
-    ptrs, codes = _addresses(src), _codes(src)
-    numels = array.array("q", [t.numel() for t in src])
-    out_ptrs = out_codes = None
-    if dst is not None:
-        out_ptrs, out_codes = _addresses(dst), _codes(dst)
+    ptrs, codes = _table(src)
+    numels = array.array("q", map(Tensor.numel, src))
+    out_ptrs, out_codes = (None, None) if dst is None else _table(dst)
     if clip:
         written = ptrs if dst is None else out_ptrs
         if len(set(written)) != len(written):  # empty tensors may share an address
             some = [p for p, n in zip(written, numels) if n]
             if len(set(some)) != len(some):
                 raise ValueError("a tensor is given twice: it would be scaled twice")
-    total = torch.empty((), dtype=torch.float32, device=dev)
-    work = torch.empty((_CLIP_WORKSPACE,), dtype=torch.uint8, device=dev)
-    with _On(dev):
-        check(
-            _LIBRARY.jk_clip_grad_norm(ptrs.buffer_info()[0], None if dst is None else out_ptrs.buffer_info()[0],
-                                       numels.buffer_info()[0], codes.buffer_info()[0],
-                                       None if dst is None else out_codes.buffer_info()[0], len(src), kind, clip, max_norm,
-                                       1e-6, total.data_ptr(), work.data_ptr(), _stream(dev)),
-            "jk_clip_grad_norm",
-        )
+    if tensors:
+        device = tensors[0].get_device()
+        work = tensors[0].new_empty((_CLIP_WORKSPACE,), dtype=torch.float64)
+    else:
+        device = _current_device()
+        work = torch.empty((_CLIP_WORKSPACE,), dtype=torch.float64, device=torch.device("cuda", device))
+    total = work.new_empty((), dtype=torch.float32)
+    _call(_LIBRARY.jk_clip_grad_norm, "jk_clip_grad_norm", device, ptrs.buffer_info()[0],
+          None if dst is None else out_ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0],
+          None if dst is None else out_codes.buffer_info()[0], len(src), kind, clip, max_norm, 1e-6, total.data_ptr(),
+          work.data_ptr())
     if back:
         with torch.no_grad():
             for to, made in back:
@@ -511,9 +499,9 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: 
             raise ValueError(f"out has {len(outs)} tensors for {len(tensors)} gradients")
         if outs and outs[0].device != tensors[0].device:
             raise RuntimeError(f"out is on {outs[0].device}, expected {tensors[0].device}")
-        for i, (o, g) in enumerate(zip(outs, tensors)):
-            if o.shape != g.shape:
-                raise ValueError(f"out {i} has shape {tuple(o.shape)}, expected {tuple(g.shape)}")
+        if list(map(Tensor.shape.__get__, outs)) != list(map(Tensor.shape.__get__, tensors)):
+            i = next(i for i, (o, g) in enumerate(zip(outs, tensors)) if o.shape != g.shape)
+            raise ValueError(f"out {i} has shape {tuple(outs[i].shape)}, expected {tuple(tensors[i].shape)}")
     total = _run_clip(tensors, outs, norm_type, 1, float(max_norm))
     if error_if_nonfinite and not math.isfinite(total.item()):
         raise RuntimeError(f"the norm of the gradients is {total.item()}")

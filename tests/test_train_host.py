@@ -42,7 +42,7 @@ def test_training_step_entry_points_check_their_arguments_before_the_device():
     assert fwd(p, 8, p, 2, 8, 0, -100, 1.5, 1, 1.0, None, None, p, None, 0, p, None) == -7
     assert fwd(p, 8, p, 2, 8, 0, -100, 0.0, 0, 1.0, p, None, None, p, 8, p, None) == -7
     assert fwd(p, 8, None, 2, 8, 0, -100, 0.0, 1, 1.0, None, None, p, None, 0, p, None) == -7
-    assert lib.jk_cross_entropy_backward(None, p, 8, p, p, 2, 8, 0, -100, 0.0, 1, p, 8, None) == -7
+    assert lib.jk_cross_entropy_backward(None, p, 8, p, p, 2, 8, 0, -100, 0.0, 1, p, 8, p, None) == -7
     one, n, f32 = (ctypes.c_uint64 * 1)(p), (ctypes.c_int64 * 1)(4), (ctypes.c_int * 1)(0)
     clip = lib.jk_clip_grad_norm
     assert clip(one, None, n, f32, None, 1, 5, 1, 1.0, 1e-6, p, p, None) == -3
