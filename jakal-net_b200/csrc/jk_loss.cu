@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
 // has the next rows' slices copied there and finds out how they lie; the others (workers) take a
 // slice twice, for the sum and for the gradient.
 #ifndef JKV_W
-#define JKV_W 224
+#define JKV_W 352
 #endif
 #ifndef JKV_P
 #define JKV_P 3
@@ -888,7 +888,16 @@ __global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
 // ---------------------------------------------------------------- reduction over rows
 // The partial sums in their order, and the rows that warps have left in parts. The last block to
 // come adds up what the blocks have (the order of the sum does not depend on which that is).
-constexpr int kReduceBlocks = 32;
+constexpr int kReduceBlocks = 32;  // a lane for each
+
+__device__ __forceinline__ Partial warp_add(Partial p) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    p.sum += __shfl_xor_sync(0xffffffffu, p.sum, o);
+    p.rows += __shfl_xor_sync(0xffffffffu, p.rows, o);
+  }
+  return p;
+}
 
 struct Ticket {
   Partial blocks[kReduceBlocks];
@@ -899,7 +908,6 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     reduce_kernel(const Args<T> a, int partials, const Record* records, int record_count, float* loss, Ticket* ticket) {
   __shared__ Partial parts[8];
-  __shared__ bool last;
   grid_dependency_wait();
   const int at = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
   Partial p{0.0, 0};
@@ -910,6 +918,8 @@ __global__ void __launch_bounds__(256)
   for (int i = at; i < record_count; i += step) {
     const Record head = records[i];
     if (head.row < 0) continue;
+    const int64_t target = a.targets[head.row];
+    const float zt = target >= 0 && target < a.vocab ? to_f32(a.logits[head.row * a.stride + target]) : NAN;
     // the records of a row follow one another, with one unused between two of them at most
     const bool begun = (i >= 1 && records[i - 1].row == head.row) || (i >= 2 && records[i - 2].row == head.row);
     if (begun) continue;
@@ -928,37 +938,32 @@ __global__ void __launch_bounds__(256)
       v = {m, v.s * f + q.s * g};
       all += q.all;
     }
-    const int64_t target = a.targets[head.row];
-    const float zt = target >= 0 && target < a.vocab ? to_f32(a.logits[head.row * a.stride + target]) : NAN;
     const RowLoss l(v, zt, all, a.smoothing, a.vocab);
     if (a.losses != nullptr) a.losses[head.row] = l.loss;
     if (a.lse_out != nullptr) a.lse_out[head.row] = l.lse;
     p.sum += l.loss;
     p.rows += 1;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    p.sum += __shfl_xor_sync(0xffffffffu, p.sum, o);
-    p.rows += __shfl_xor_sync(0xffffffffu, p.rows, o);
-  }
+  p = warp_add(p);
   if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = p;
   __syncthreads();
-  if (threadIdx.x != 0 || loss == nullptr) return;
-  for (int i = 1; i < 8; ++i) p.sum += parts[i].sum, p.rows += parts[i].rows;
+  if (threadIdx.x >= 32 || loss == nullptr) return;
+  p = warp_add(threadIdx.x < 8 ? parts[threadIdx.x] : Partial{0.0, 0});
   if (gridDim.x > 1) {
-    ticket->blocks[blockIdx.x] = p;
-    __threadfence();
-    last = atomicAdd(&ticket->come, 1) == static_cast<int>(gridDim.x) - 1;
-    if (!last) return;
-    __threadfence();
-    p = {0.0, 0};
-    for (int i = 0; i < static_cast<int>(gridDim.x); ++i) {
-      const volatile Partial* q = &ticket->blocks[i];
-      p.sum += q->sum;
-      p.rows += q->rows;
+    int order = 0;
+    if (threadIdx.x == 0) {
+      ticket->blocks[blockIdx.x] = p;
+      __threadfence();
+      order = atomicAdd(&ticket->come, 1);
     }
+    if (__shfl_sync(0xffffffffu, order, 0) != static_cast<int>(gridDim.x) - 1) return;
+    __threadfence();
+    const volatile Partial* q = &ticket->blocks[threadIdx.x];
+    p.sum = q->sum;
+    p.rows = q->rows;
+    p = warp_add(p);
   }
-  *loss = static_cast<float>(a.reduction == JK_REDUCE_MEAN ? p.sum / static_cast<double>(p.rows) : p.sum);
+  if (threadIdx.x == 0) *loss = static_cast<float>(a.reduction == JK_REDUCE_MEAN ? p.sum / static_cast<double>(p.rows) : p.sum);
 }
 
 // ---------------------------------------------------------------- launches

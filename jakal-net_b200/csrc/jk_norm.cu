@@ -7,116 +7,552 @@
 //
 // The variance is the mean of the squared distances from the mean (two sums over the row), not
 // E[sum^2] - mean^2, which cancels where the mean is large against the spread.
+//
+// Bound: memory, every row read once and written once. A row of up to 16384 elements stays in the
+// registers of the 8 to 1024 threads that share it (each has up to 16 elements, in 16-byte packs
+// where all rows allow it, else one by one); a thread keeps its columns for all rows it comes to, so
+// the parameters and, backward, the sums of their gradients stay in its registers too, and the next
+// row is on its way while one is worked on. Longer rows are read again for each sum.
 #include "jk_host.h"
 #include "jk_rows.cuh"
 
 namespace jk {
 namespace norm {
 
-constexpr int kThreads = 256;
-constexpr int kMaxBlocks = 148 * 4;
+constexpr int kMaxParts = 148 * 2;  // blocks that leave their share of the parameter gradients
 
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
+struct Forward {
+  const void *x, *delta;
+  int64_t x_stride, delta_stride;
+  float scale;
+  const void *weight, *bias;
+  int param_type;
+  int64_t rows;
+  int64_t dim;
+  float eps;
+  void *y, *sum;
+  float *mean, *rstd;
+};
+
+struct Backward {
+  const void *grad_y, *sum, *grad_sum;
+  int64_t grad_y_stride, sum_stride, grad_sum_stride;
+  const float *mean, *rstd;
+  const void* weight;
+  int param_type;
+  float scale;
+  int64_t rows;
+  int64_t dim;
+  void *grad_x, *grad_delta;
+  float* parts;  // [blocks][2][dim], or null
+};
+
+__device__ __forceinline__ float param_at(const void* p, int64_t c, int type, float none) {
+  if (p == nullptr) return none;
+  if (type == JK_F32) return static_cast<const float*>(p)[c];
+  if (type == JK_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[c]);
+  return to_f32(static_cast<const __half*>(p)[c]);
+}
+
+// VEC neighbouring elements as they lie in memory: a 16-byte pack, or one.
+template <typename T, int VEC>
+struct Raw {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void floats(float (&f)[VEC]) const { unpack<T>(v, f); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) { *reinterpret_cast<uint4*>(p) = pack<T>(f); }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void floats(float (&f)[1]) const { f[0] = to_f32(v); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
+};
+
+// Threads of a block, and rows that it has at a time, with `TPR` threads to a row.
+template <int TPR>
+constexpr int kBlock = TPR > 256 ? TPR : (TPR > 32 ? TPR : 256);
+template <int TPR>
+constexpr int kGroups = kBlock<TPR> / TPR;
+
+// Sums over the threads of a row, in all of them. With more than a warp to a row the row has the
+// whole block; `turn` alternates, so that one barrier does.
+template <int TPR, int COUNT>
+__device__ __forceinline__ void row_sums(float (&v)[COUNT], float (*scratch)[COUNT][32], int turn) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if constexpr (TPR > 32) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) scratch[turn][i][threadIdx.x >> 5] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      v[i] = lane < TPR / 32 ? scratch[turn][i][lane] : 0.f;
+#pragma unroll
+      for (int o = TPR / 64; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      if constexpr (TPR < 1024) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+    }
+  }
+}
+
+template <typename T, int VEC, int N, int TPR, bool DELTA>
+__global__ void __launch_bounds__(kBlock<TPR>) forward_kernel(const Forward a) {
+  __shared__ float scratch[2][1][32];
+  const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups<TPR>;
+  const T *x = static_cast<const T*>(a.x), *delta = static_cast<const T*>(a.delta);
+  float w[N][VEC], b[N][VEC];
+  Raw<T, VEC> next_x[N], next_d[DELTA ? N : 1];
+  const auto load = [&](int64_t r) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (c < dim) {
+        next_x[i].load(x + r * a.x_stride + c);
+        if (DELTA) next_d[DELTA ? i : 0].load(delta + r * a.delta_stride + c);
+      }
+    }
+  };
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups<TPR> + threadIdx.x / TPR;
+  if (r < a.rows) load(r);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int c = (i * TPR + thread) * VEC + j;
+      w[i][j] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
+      b[i][j] = c < dim ? param_at(a.bias, c, a.param_type, 0.f) : 0.f;
+    }
+  const float inv = 1.f / static_cast<float>(dim);
+  // all groups of a block take as many turns, as they may share a warp
+  for (int64_t base = r - threadIdx.x / TPR; base < a.rows; base += step, r += step) {
+    const bool here = r < a.rows;
+    float f[N][VEC], s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (here && c < dim) {
+        next_x[i].floats(f[i]);
+        if (DELTA) {
+          float d[VEC];
+          next_d[DELTA ? i : 0].floats(d);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) f[i][j] = fmaf(a.scale, d[j], f[i][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[0] += f[i][j];
+      }
+    }
+    if (r + step < a.rows) load(r + step);
+    row_sums<TPR, 1>(s, scratch, 0);
+    const float mu = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (here && c < dim) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float d = f[i][j] - mu;
+          s[0] = fmaf(d, d, s[0]);
+        }
+      }
+    }
+    row_sums<TPR, 1>(s, scratch, 1);
+    const float rs = rsqrtf(fmaf(s[0], inv, a.eps));
+    if (!here) continue;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (c < dim) {
+        float o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = fmaf((f[i][j] - mu) * rs, w[i][j], b[i][j]);
+        Raw<T, VEC>::store(static_cast<T*>(a.y) + r * dim + c, o);
+        if (a.sum != nullptr) Raw<T, VEC>::store(static_cast<T*>(a.sum) + r * dim + c, f[i]);
+      }
+    }
+    if (thread == 0 && a.mean != nullptr) {
+      a.mean[r] = mu;
+      a.rstd[r] = rs;
+    }
+  }
+}
+
+// The block's share of the parameter gradients: the groups' sums joined, in their order.
+template <int VEC, int N, int TPR>
+__device__ __forceinline__ void leave_parts(float (&dw)[N][VEC], float (&db)[N][VEC], int dim, float* parts, float* shared) {
+  const int thread = threadIdx.x % TPR;
+  float* mine = parts + static_cast<int64_t>(blockIdx.x) * 2 * dim;
+  if constexpr (TPR < 32) {  // the groups of a warp
+#pragma unroll
+    for (int o = 16; o >= TPR; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], o);
+          db[i][j] += __shfl_xor_sync(0xffffffffu, db[i][j], o);
+        }
+  }
+  constexpr int kShare = TPR <= 32 ? kBlock<TPR> / 32 : 1;  // warps that have the same columns
+  const bool speaks = TPR >= 32 || (threadIdx.x & 31) < TPR;
+  for (int g = 0; g < kShare; ++g) {
+    if (speaks && (kShare == 1 || static_cast<int>(threadIdx.x >> 5) == g)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int c = (i * TPR + thread) * VEC + j;
+          if (c < dim) {
+            if (kShare == 1) {
+              mine[c] = dw[i][j];
+              mine[dim + c] = db[i][j];
+            } else {
+              // an element's place: its turn, its place in the pack, its thread; neighbouring threads, neighbouring words
+              float* at = shared + ((i * VEC + j) * TPR + thread) * 2;
+              const float2 before = g == 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<float2*>(at);
+              const float2 now = make_float2(before.x + dw[i][j], before.y + db[i][j]);
+              if (g == kShare - 1) {
+                mine[c] = now.x;
+                mine[dim + c] = now.y;
+              } else {
+                *reinterpret_cast<float2*>(at) = now;
+              }
+            }
+          }
+        }
+    }
+    if (kShare > 1) __syncthreads();
+  }
+}
+
+template <typename T, int VEC, int N, int TPR, bool SUM, bool PARAMS>
+__global__ void __launch_bounds__(kBlock<TPR>) backward_kernel(const Backward a) {
+  __shared__ float scratch[2][2][32];
+  constexpr bool kShared = PARAMS && TPR <= 32;
+  __shared__ float shared[kShared ? N * VEC * TPR * 2 : 1];
+  const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups<TPR>;
+  const T *gy = static_cast<const T*>(a.grad_y), *h = static_cast<const T*>(a.sum), *gs = static_cast<const T*>(a.grad_sum);
+  float w[N][VEC], dw[N][VEC] = {}, db[N][VEC] = {};
+  Raw<T, VEC> next_y[N], next_h[N], next_s[SUM ? N : 1];
+  float next_mean = 0.f, next_rstd = 0.f;
+  const auto load = [&](int64_t r) {
+    next_mean = a.mean[r];
+    next_rstd = a.rstd[r];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (c < dim) {
+        next_y[i].load(gy + r * a.grad_y_stride + c);
+        next_h[i].load(h + r * a.sum_stride + c);
+        if (SUM) next_s[SUM ? i : 0].load(gs + r * a.grad_sum_stride + c);
+      }
+    }
+  };
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups<TPR> + threadIdx.x / TPR;
+  if (r < a.rows) load(r);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int c = (i * TPR + thread) * VEC + j;
+      w[i][j] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
+    }
+  const float inv = 1.f / static_cast<float>(dim);
+  int turn = 0;
+  for (int64_t base = r - threadIdx.x / TPR; base < a.rows; base += step, r += step, turn ^= 1) {
+    const bool here = r < a.rows;
+    Raw<T, VEC> y[N], hh[N], ss[SUM ? N : 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      y[i] = next_y[i], hh[i] = next_h[i];
+      if (SUM) ss[SUM ? i : 0] = next_s[SUM ? i : 0];
+    }
+    const float mu = next_mean, rs = next_rstd;
+    if (r + step < a.rows) load(r + step);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (here && c < dim) {
+        float g[VEC], n[VEC];
+        y[i].floats(g);
+        hh[i].floats(n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          n[j] = (n[j] - mu) * rs;
+          const float u = g[j] * w[i][j];
+          s[0] += u;
+          s[1] = fmaf(u, n[j], s[1]);
+          if (PARAMS) {
+            dw[i][j] = fmaf(g[j], n[j], dw[i][j]);
+            db[i][j] += g[j];
+          }
+        }
+      }
+    }
+    row_sums<TPR, 2>(s, scratch, turn);
+    if (!here) continue;
+    const float c0 = s[0] * inv, c1 = s[1] * inv;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + thread) * VEC;
+      if (c < dim) {
+        float g[VEC], n[VEC], o[VEC], q[VEC];
+        y[i].floats(g);
+        hh[i].floats(n);
+        if (SUM) ss[SUM ? i : 0].floats(q);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          n[j] = (n[j] - mu) * rs;
+          o[j] = fmaf(g[j], w[i][j], -fmaf(n[j], c1, c0));
+          o[j] = SUM ? fmaf(rs, o[j], q[j]) : rs * o[j];
+        }
+        Raw<T, VEC>::store(static_cast<T*>(a.grad_x) + r * dim + c, o);
+        if (a.grad_delta != nullptr) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) o[j] *= a.scale;
+          Raw<T, VEC>::store(static_cast<T*>(a.grad_delta) + r * dim + c, o);
+        }
+      }
+    }
+  }
+  if constexpr (PARAMS) {
+    grid_dependency_launch();
+    leave_parts<VEC, N, TPR>(dw, db, dim, a.parts, shared);
+  }
+}
+
+// ---------------------------------------------------------------- rows of any length
+constexpr int kLongThreads = 512;
+
+__device__ __forceinline__ float long_sum(float v, float* scratch) {
   v = warp_sum32(v);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < kThreads / 32; ++i) v += scratch[i];
-  __syncthreads();
-  return v;
+  return warp_sum32((threadIdx.x & 31) < kLongThreads / 32 ? scratch[threadIdx.x & 31] : 0.f);
 }
 
 template <typename T>
-__device__ __forceinline__ float sum_at(const T* x, const T* delta, float scale, int64_t c) {
-  const float v = to_f32(x[c]);
-  return delta == nullptr ? v : fmaf(scale, to_f32(delta[c]), v);
-}
-
-// One block per row, the row read three times.
-template <typename T, typename W>
-__global__ void __launch_bounds__(kThreads)
-    forward_kernel(const T* x, int64_t x_stride, const T* delta, int64_t delta_stride, float scale, const W* weight,
-                   const W* bias, int64_t rows, int64_t dim, float eps, T* y, T* sum, float* mean, float* rstd) {
-  __shared__ float scratch[kThreads / 32];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* xr = x + r * x_stride;
-    const T* dr = delta == nullptr ? nullptr : delta + r * delta_stride;
-    float a = 0.f;
-    for (int64_t c = threadIdx.x; c < dim; c += kThreads) a += sum_at(xr, dr, scale, c);
-    const float mu = block_sum(a, scratch) / static_cast<float>(dim);
-    a = 0.f;
-    for (int64_t c = threadIdx.x; c < dim; c += kThreads) {
-      const float d = sum_at(xr, dr, scale, c) - mu;
-      a = fmaf(d, d, a);
+__global__ void __launch_bounds__(kLongThreads) long_forward_kernel(const Forward a) {
+  __shared__ float scratch[kLongThreads / 32];
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+    const T* d = a.delta == nullptr ? nullptr : static_cast<const T*>(a.delta) + r * a.delta_stride;
+    const auto at = [&](int64_t c) { return d == nullptr ? to_f32(x[c]) : fmaf(a.scale, to_f32(d[c]), to_f32(x[c])); };
+    float s = 0.f;
+    for (int64_t c = threadIdx.x; c < a.dim; c += kLongThreads) s += at(c);
+    const float mu = long_sum(s, scratch) / static_cast<float>(a.dim);
+    s = 0.f;
+    for (int64_t c = threadIdx.x; c < a.dim; c += kLongThreads) {
+      const float v = at(c) - mu;
+      s = fmaf(v, v, s);
     }
-    const float rs = rsqrtf(block_sum(a, scratch) / static_cast<float>(dim) + eps);
-    for (int64_t c = threadIdx.x; c < dim; c += kThreads) {
-      const float h = sum_at(xr, dr, scale, c);
-      const float n = (h - mu) * rs;
-      const float w = weight == nullptr ? 1.f : to_f32(weight[c]), b = bias == nullptr ? 0.f : to_f32(bias[c]);
-      y[r * dim + c] = from_f32<T>(fmaf(n, w, b));
-      if (sum != nullptr) sum[r * dim + c] = from_f32<T>(h);
+    const float rs = rsqrtf(long_sum(s, scratch) / static_cast<float>(a.dim) + a.eps);
+    for (int64_t c = threadIdx.x; c < a.dim; c += kLongThreads) {
+      const float v = at(c);
+      static_cast<T*>(a.y)[r * a.dim + c] =
+          from_f32<T>(fmaf((v - mu) * rs, param_at(a.weight, c, a.param_type, 1.f), param_at(a.bias, c, a.param_type, 0.f)));
+      if (a.sum != nullptr) static_cast<T*>(a.sum)[r * a.dim + c] = from_f32<T>(v);
     }
-    if (threadIdx.x == 0 && mean != nullptr) {
-      mean[r] = mu;
-      rstd[r] = rs;
+    if (threadIdx.x == 0 && a.mean != nullptr) {
+      a.mean[r] = mu;
+      a.rstd[r] = rs;
     }
   }
 }
 
-// One block per row at a time; the block's share of the parameter gradients goes to its own
-// part of the workspace [blocks][2][dim], each column by one thread.
-template <typename T, typename W>
-__global__ void __launch_bounds__(kThreads)
-    backward_kernel(const T* grad_y, int64_t gy_stride, const T* sum, int64_t sum_stride, const float* mean,
-                    const float* rstd, const W* weight, const T* grad_sum, int64_t gs_stride, float scale, int64_t rows,
-                    int64_t dim, T* grad_x, T* grad_delta, float* workspace) {
-  __shared__ float scratch[kThreads / 32];
-  float* part = workspace == nullptr ? nullptr : workspace + static_cast<int64_t>(blockIdx.x) * 2 * dim;
-  if (part != nullptr)
-    for (int64_t c = threadIdx.x; c < dim; c += kThreads) part[c] = part[dim + c] = 0.f;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* gy = grad_y + r * gy_stride;
-    const T* h = sum + r * sum_stride;
-    const float mu = mean[r], rs = rstd[r];
-    float a = 0.f, b = 0.f;
-    for (int64_t c = threadIdx.x; c < dim; c += kThreads) {
-      const float g = to_f32(gy[c]), n = (to_f32(h[c]) - mu) * rs;
-      const float u = weight == nullptr ? g : g * to_f32(weight[c]);
-      a += u;
-      b = fmaf(u, n, b);
-      if (part != nullptr) {
-        part[c] = fmaf(g, n, part[c]);
-        part[dim + c] += g;
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) long_backward_kernel(const Backward a) {
+  __shared__ float scratch[kLongThreads / 32];
+  float* part = a.parts == nullptr ? nullptr : a.parts + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* gy = static_cast<const T*>(a.grad_y) + r * a.grad_y_stride;
+    const T* h = static_cast<const T*>(a.sum) + r * a.sum_stride;
+    const float mu = a.mean[r], rs = a.rstd[r];
+    float s0 = 0.f, s1 = 0.f;
+    for (int64_t c = threadIdx.x; c < a.dim; c += kLongThreads) {
+      const float g = to_f32(gy[c]), n = (to_f32(h[c]) - mu) * rs, u = g * param_at(a.weight, c, a.param_type, 1.f);
+      s0 += u;
+      s1 = fmaf(u, n, s1);
+      if (part != nullptr) {  // a column is always the same thread's
+        part[c] = r == blockIdx.x ? g * n : fmaf(g, n, part[c]);
+        part[a.dim + c] = r == blockIdx.x ? g : part[a.dim + c] + g;
       }
     }
-    a = block_sum(a, scratch) / static_cast<float>(dim);
-    b = block_sum(b, scratch) / static_cast<float>(dim);
-    for (int64_t c = threadIdx.x; c < dim; c += kThreads) {
-      const float g = to_f32(gy[c]), n = (to_f32(h[c]) - mu) * rs;
-      const float u = weight == nullptr ? g : g * to_f32(weight[c]);
-      float d = rs * (u - a - n * b);
-      if (grad_sum != nullptr) d += to_f32(grad_sum[r * gs_stride + c]);
-      grad_x[r * dim + c] = from_f32<T>(d);
-      if (grad_delta != nullptr) grad_delta[r * dim + c] = from_f32<T>(scale * d);
+    s0 = long_sum(s0, scratch) / static_cast<float>(a.dim);
+    s1 = long_sum(s1, scratch) / static_cast<float>(a.dim);
+    for (int64_t c = threadIdx.x; c < a.dim; c += kLongThreads) {
+      const float n = (to_f32(h[c]) - mu) * rs;
+      float d = rs * (to_f32(gy[c]) * param_at(a.weight, c, a.param_type, 1.f) - s0 - n * s1);
+      if (a.grad_sum != nullptr) d += to_f32(static_cast<const T*>(a.grad_sum)[r * a.grad_sum_stride + c]);
+      static_cast<T*>(a.grad_x)[r * a.dim + c] = from_f32<T>(d);
+      if (a.grad_delta != nullptr) static_cast<T*>(a.grad_delta)[r * a.dim + c] = from_f32<T>(a.scale * d);
     }
   }
 }
 
+// ---------------------------------------------------------------- parameter gradients
+// 32 columns to a block, 32 threads to a column; the blocks' shares are added in a fixed order.
 template <typename W>
-__global__ void __launch_bounds__(kThreads)
-    parameters_kernel(const float* workspace, int blocks, int64_t dim, W* grad_weight, W* grad_bias) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (c >= 2 * dim) return;
-  float a = 0.f;
-  for (int i = 0; i < blocks; ++i) a += workspace[static_cast<int64_t>(i) * 2 * dim + c];
-  if (c < dim)
-    grad_weight[c] = from_f32<W>(a);
+__global__ void __launch_bounds__(1024) parameters_kernel(const float* parts, int count, int64_t dim, W* grad_weight, W* grad_bias) {
+  __shared__ float sums[32][33];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
+  const int slice = threadIdx.x / 32;
+  grid_dependency_wait();
+  float s = 0.f;
+  if (c < 2 * dim)
+    for (int i = slice; i < count; i += 32) s += parts[static_cast<int64_t>(i) * 2 * dim + c];
+  sums[slice][threadIdx.x % 32] = s;
+  __syncthreads();
+  s = warp_sum32(sums[threadIdx.x % 32][slice]);  // thread (slice, lane) now has column `slice`
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + slice;
+  if (threadIdx.x % 32 != 0 || mine >= 2 * dim) return;
+  if (mine < dim)
+    grad_weight[mine] = from_f32<W>(s);
   else
-    grad_bias[c - dim] = from_f32<W>(a);
+    grad_bias[mine - dim] = from_f32<W>(s);
 }
 
-inline int blocks_for(int64_t rows) { return static_cast<int>(rows < kMaxBlocks ? rows : kMaxBlocks); }
+// ---------------------------------------------------------------- launches
+inline int64_t groups_to_blocks(int64_t rows, int groups, int64_t most) {
+  const int64_t want = (rows + groups - 1) / groups;
+  return want < most ? want : most;
+}
+
+// Blocks of a kernel that an SM holds, asked for once (the devices are alike).
+template <auto KERNEL>
+int blocks_per_sm(int threads) {
+  static const int per_sm = [threads] {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    return n;
+  }();
+  return per_sm;
+}
+
+template <auto KERNEL, int TPR>
+int run_forward(const Forward& a, cudaStream_t s) {
+  const int64_t blocks = groups_to_blocks(a.rows, kGroups<TPR>, 148ll * blocks_per_sm<KERNEL>(kBlock<TPR>));
+  KERNEL<<<static_cast<unsigned>(blocks), kBlock<TPR>, 0, s>>>(a);
+  return 0;
+}
+
+template <typename T, int VEC, int N, int TPR>
+int pick_forward(const Forward& a, cudaStream_t s) {
+  return a.delta != nullptr ? run_forward<forward_kernel<T, VEC, N, TPR, true>, TPR>(a, s)
+                            : run_forward<forward_kernel<T, VEC, N, TPR, false>, TPR>(a, s);
+}
+
+template <auto KERNEL, int TPR>
+int run_backward(const Backward& a, cudaStream_t s) {
+  int64_t most = 148ll * blocks_per_sm<KERNEL>(kBlock<TPR>);
+  if (a.parts != nullptr && most > kMaxParts) most = kMaxParts;
+  const int blocks = static_cast<int>(groups_to_blocks(a.rows, kGroups<TPR>, most));
+  KERNEL<<<blocks, kBlock<TPR>, 0, s>>>(a);
+  return blocks;
+}
+
+template <typename T, int VEC, int N, int TPR>
+int pick_backward(const Backward& a, cudaStream_t s) {
+  if (a.grad_sum != nullptr)
+    return a.parts != nullptr ? run_backward<backward_kernel<T, VEC, N, TPR, true, true>, TPR>(a, s)
+                              : run_backward<backward_kernel<T, VEC, N, TPR, true, false>, TPR>(a, s);
+  return a.parts != nullptr ? run_backward<backward_kernel<T, VEC, N, TPR, false, true>, TPR>(a, s)
+                            : run_backward<backward_kernel<T, VEC, N, TPR, false, false>, TPR>(a, s);
+}
+
+// The threads of a row and their turns: as few threads as hold it with 16 elements each (fewer where
+// a warp has room), a warp's or less while that does, so that no barrier is needed.
+#define JK_NORM_SHAPES(RUN)                                             \
+  if constexpr (VEC == 8) {                                             \
+    if (turns <= 8) return RUN(1, 8);                                   \
+    if (turns <= 16) return RUN(1, 16);                                 \
+    if (turns <= 32) return RUN(1, 32);                                 \
+    if (turns <= 64) return RUN(2, 32);                                 \
+    if (turns <= 256) return RUN(2, 128);                               \
+    if (turns <= 512) return RUN(2, 256);                               \
+    if (turns <= 1024) return RUN(2, 512);                              \
+    return RUN(2, 1024);                                                \
+  } else if constexpr (VEC == 4) {                                      \
+    if (turns <= 8) return RUN(1, 8);                                   \
+    if (turns <= 16) return RUN(1, 16);                                 \
+    if (turns <= 32) return RUN(1, 32);                                 \
+    if (turns <= 64) return RUN(2, 32);                                 \
+    if (turns <= 128) return RUN(4, 32);                                \
+    if (turns <= 512) return RUN(4, 128);                               \
+    if (turns <= 1024) return RUN(4, 256);                              \
+    if (turns <= 2048) return RUN(4, 512);                              \
+    return RUN(4, 1024);                                                \
+  } else {                                                              \
+    if (turns <= 32) return RUN(1, 32);                                 \
+    if (turns <= 128) return RUN(4, 32);                                \
+    if (turns <= 512) return RUN(16, 32);                               \
+    if (turns <= 2048) return RUN(16, 128);                             \
+    if (turns <= 4096) return RUN(16, 256);                             \
+    if (turns <= 8192) return RUN(16, 512);                             \
+    return RUN(16, 1024);                                               \
+  }
+
+constexpr int64_t kMaxDim = 16384;  // of the rows that stay in registers
+
+template <typename T, int VEC>
+int shape_forward(const Forward& a, cudaStream_t s) {
+  const int64_t turns = a.dim / VEC;
+#define JK_RUN(N, TPR) pick_forward<T, VEC, N, TPR>(a, s)
+  JK_NORM_SHAPES(JK_RUN)
+#undef JK_RUN
+}
+
+template <typename T, int VEC>
+int shape_backward(const Backward& a, cudaStream_t s) {
+  const int64_t turns = a.dim / VEC;
+#define JK_RUN(N, TPR) pick_backward<T, VEC, N, TPR>(a, s)
+  JK_NORM_SHAPES(JK_RUN)
+#undef JK_RUN
+}
+
+template <typename T>
+bool in_packs(const void* p, int64_t stride) {
+  return p == nullptr || (aligned16(p) && stride % kPack<T> == 0);
+}
+
+template <typename T>
+void forward(const Forward& a, cudaStream_t s) {
+  if (a.dim > kMaxDim) {
+    long_forward_kernel<T><<<static_cast<unsigned>(a.rows < 148 * 4 ? a.rows : 148 * 4), kLongThreads, 0, s>>>(a);
+  } else if (in_packs<T>(a.x, a.x_stride) && in_packs<T>(a.delta, a.delta_stride) && in_packs<T>(a.y, a.dim) &&
+             in_packs<T>(a.sum, a.dim)) {
+    shape_forward<T, kPack<T>>(a, s);
+  } else {
+    shape_forward<T, 1>(a, s);
+  }
+}
+
+// Returns the blocks that left a share of the parameter gradients.
+template <typename T>
+int backward(const Backward& a, cudaStream_t s) {
+  if (a.dim > kMaxDim) {
+    const int blocks = static_cast<int>(a.rows < kMaxParts ? a.rows : kMaxParts);
+    long_backward_kernel<T><<<blocks, kLongThreads, 0, s>>>(a);
+    return blocks;
+  }
+  if (in_packs<T>(a.grad_y, a.grad_y_stride) && in_packs<T>(a.sum, a.sum_stride) && in_packs<T>(a.grad_sum, a.grad_sum_stride) &&
+      in_packs<T>(a.grad_x, a.dim) && in_packs<T>(a.grad_delta, a.dim))
+    return shape_backward<T, kPack<T>>(a, s);
+  return shape_backward<T, 1>(a, s);
+}
 
 }  // namespace norm
 }  // namespace jk
@@ -132,18 +568,14 @@ extern "C" int jk_layer_norm_forward(const void* x, int64_t x_stride, const void
   if (x == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr)) return JK_ERR_BAD_ARG;
   int st = check_device();
   if (st != JK_OK) return st;
-  auto s = reinterpret_cast<cudaStream_t>(stream);
-  JK_WITH_TYPE(dtype, T, JK_WITH_TYPE(param_dtype, W, {
-    norm::forward_kernel<T, W><<<norm::blocks_for(rows), norm::kThreads, 0, s>>>(
-        static_cast<const T*>(x), x_stride, static_cast<const T*>(delta), delta_stride, delta_scale,
-        static_cast<const W*>(weight), static_cast<const W*>(bias), rows, dim, eps, static_cast<T*>(y),
-        static_cast<T*>(sum), mean, rstd);
-  }));
+  const norm::Forward a{x, delta, x_stride, delta_stride, delta_scale, weight, bias, param_dtype,
+                        rows, dim, eps, y, sum, mean, rstd};
+  JK_WITH_TYPE(dtype, T, norm::forward<T>(a, reinterpret_cast<cudaStream_t>(stream)));
   return launch_status();
 }
 
 extern "C" int64_t jk_layer_norm_backward_workspace(int64_t rows, int64_t dim) {
-  return rows <= 0 || dim <= 0 ? 0 : 2 * dim * jk::norm::blocks_for(rows);
+  return rows <= 0 || dim <= 0 ? 0 : 2 * dim * (rows < jk::norm::kMaxParts ? rows : jk::norm::kMaxParts);
 }
 
 extern "C" int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* sum, int64_t sum_stride,
@@ -163,20 +595,12 @@ extern "C" int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride,
   int st = check_device();
   if (st != JK_OK) return st;
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  const int blocks = rows == 0 ? 0 : norm::blocks_for(rows);
-  JK_WITH_TYPE(param_dtype, W, {
-    if (rows > 0) {
-      JK_WITH_TYPE(dtype, T, {
-        norm::backward_kernel<T, W><<<blocks, norm::kThreads, 0, s>>>(
-            static_cast<const T*>(grad_y), grad_y_stride, static_cast<const T*>(sum), sum_stride, mean, rstd,
-            static_cast<const W*>(weight), static_cast<const T*>(grad_sum), grad_sum_stride, delta_scale, rows, dim,
-            static_cast<T*>(grad_x), static_cast<T*>(grad_delta), params ? workspace : nullptr);
-      });
-    }
-    if (params)
-      norm::parameters_kernel<W><<<static_cast<unsigned>((2 * dim + norm::kThreads - 1) / norm::kThreads), norm::kThreads, 0,
-                                   s>>>(workspace, blocks, dim, static_cast<W*>(grad_weight),
-                                        static_cast<W*>(grad_bias));
-  });
+  const norm::Backward a{grad_y, sum, grad_sum, grad_y_stride, sum_stride, grad_sum_stride, mean, rstd, weight, param_dtype,
+                         delta_scale, rows, dim, grad_x, grad_delta, params ? workspace : nullptr};
+  int parts = 0;
+  if (rows > 0) JK_WITH_TYPE(dtype, T, parts = norm::backward<T>(a, s));
+  if (params)
+    JK_WITH_TYPE(param_dtype, W, launch_dependent(norm::parameters_kernel<W>, static_cast<unsigned>((2 * dim + 31) / 32), 1024, 0, s,
+                                                  workspace, parts, dim, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias)));
   return launch_status();
 }
