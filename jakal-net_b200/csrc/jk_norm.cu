@@ -9,12 +9,18 @@
 // E[sum^2] - mean^2, which cancels where the mean is large against the spread.
 //
 // Bound: memory, every row read once and written once. A row of up to 16384 elements stays in the
-// registers of the 8 to 1024 threads that share it (each has up to 16 elements, in 16-byte packs
-// where all rows allow it, else one by one); a thread keeps its columns for all rows it comes to, so
-// the parameters and, backward, the sums of their gradients stay in its registers too, and the next
-// row is on its way while one is worked on. Longer rows are read again for each sum.
+// registers of the 8 to 1024 threads that share it, each with up to 16 elements; a thread keeps its
+// columns for all rows it comes to, so the parameters and, backward, the sums of their gradients stay
+// in its registers too. Three forms:
+//   * forward_kernel, backward_kernel: rows that lie in 16-byte packs, a pack at a time, the next row
+//     on its way in registers while one is worked on;
+//   * staged_forward_kernel, staged_backward_kernel: rows that do not (an odd width, an odd offset).
+//     One warp has tiles of rows copied to shared memory as they lie, in 16-byte blocks, tiles ahead;
+//     the others take their elements from there one by one, whatever their alignment;
+//   * long_*: longer rows, read again for each sum.
 #include "jk_host.h"
 #include "jk_rows.cuh"
+#include "jk_sm100.cuh"
 
 namespace jk {
 namespace norm {
@@ -62,14 +68,6 @@ struct Raw {
   __device__ __forceinline__ void floats(float (&f)[VEC]) const { unpack<T>(v, f); }
   static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) { *reinterpret_cast<uint4*>(p) = pack<T>(f); }
 };
-template <typename T>
-struct Raw<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ void floats(float (&f)[1]) const { f[0] = to_f32(v); }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
-};
-
 // Threads of a block, and rows that it has at a time, with `TPR` threads to a row.
 template <int TPR>
 constexpr int kBlock = TPR > 256 ? TPR : (TPR > 32 ? TPR : 256);
@@ -78,7 +76,7 @@ constexpr int kGroups = kBlock<TPR> / TPR;
 
 // Sums over the threads of a row, in all of them. With more than a warp to a row the row has the
 // whole block; `turn` alternates, so that one barrier does.
-template <int TPR, int COUNT>
+template <int TPR, int COUNT, bool STAGED = false>
 __device__ __forceinline__ void row_sums(float (&v)[COUNT], float (*scratch)[COUNT][32], int turn) {
 #pragma unroll
   for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
@@ -89,7 +87,10 @@ __device__ __forceinline__ void row_sums(float (&v)[COUNT], float (*scratch)[COU
     if (lane == 0)
 #pragma unroll
       for (int i = 0; i < COUNT; ++i) scratch[turn][i][threadIdx.x >> 5] = v[i];
-    __syncthreads();
+    if constexpr (STAGED)
+      asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");  // not the loading warp
+    else
+      __syncthreads();
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       v[i] = lane < TPR / 32 ? scratch[turn][i][lane] : 0.f;
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) forward_kernel(const Forward a) {
 }
 
 // The block's share of the parameter gradients: the groups' sums joined, in their order.
-template <int VEC, int N, int TPR>
+template <int VEC, int N, int TPR, bool STAGED = false>
 __device__ __forceinline__ void leave_parts(float (&dw)[N][VEC], float (&db)[N][VEC], int dim, float* parts, float* shared) {
   const int thread = threadIdx.x % TPR;
   float* mine = parts + static_cast<int64_t>(blockIdx.x) * 2 * dim;
@@ -228,12 +229,17 @@ __device__ __forceinline__ void leave_parts(float (&dw)[N][VEC], float (&db)[N][
           }
         }
     }
-    if (kShare > 1) __syncthreads();
+    if constexpr (kShare > 1) {
+      if constexpr (STAGED)
+        asm volatile("bar.sync 1, %0;" ::"n"(kBlock<TPR>) : "memory");
+      else
+        __syncthreads();
+    }
   }
 }
 
 template <typename T, int VEC, int N, int TPR, bool SUM, bool PARAMS>
-__global__ void __launch_bounds__(kBlock<TPR>) backward_kernel(const Backward a) {
+__global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? 512 / kBlock<TPR> : 1) backward_kernel(const Backward a) {
   __shared__ float scratch[2][2][32];
   constexpr bool kShared = PARAMS && TPR <= 32;
   __shared__ float shared[kShared ? N * VEC * TPR * 2 : 1];
@@ -327,6 +333,263 @@ __global__ void __launch_bounds__(kBlock<TPR>) backward_kernel(const Backward a)
   if constexpr (PARAMS) {
     grid_dependency_launch();
     leave_parts<VEC, N, TPR>(dw, db, dim, a.parts, shared);
+  }
+}
+
+// ---------------------------------------------------------------- rows off 16-byte boundaries
+constexpr int kMaxFeeds = 5;
+constexpr int kMaxStages = 8;
+constexpr int kMaxTileRows = 128;
+
+// An input as the loading warp sees it: rows of bytes, `stride` apart. Rows without a gap are copied
+// as one piece, others one by one, each to a place `pitch` after the one before.
+struct Feed {
+  const char* p;
+  int64_t stride;
+  int row_bytes;
+  uint32_t offset;  // in a stage
+  int pitch;        // 0: one piece
+};
+
+struct Plan {
+  Feed feed[kMaxFeeds];
+  int feeds, tile_rows, stages;
+  uint32_t stage_bytes;
+};
+
+// Where row `i` of the tile that begins at row r0 lies in a stage.
+__device__ __forceinline__ const char* staged(const Feed& f, const unsigned char* stage, int64_t r0, int i) {
+  const uint32_t first = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(f.p) + r0 * f.stride) & 15u;
+  const uint32_t at = f.pitch == 0 ? first + i * f.row_bytes
+                                   : i * f.pitch + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(f.p) + (r0 + i) * f.stride) & 15u);
+  return reinterpret_cast<const char*>(stage) + f.offset + at;
+}
+
+// Bytes [from, to) of an input into shared memory at `dst` (which stands for the 16-byte block that
+// `from` lies in). Whole blocks by one bulk copy; where the first or the last block reaches outside
+// the input, its bytes one element's half or whole at a time, before the copies are announced.
+// Returns the bytes of the bulk copy.
+__device__ __forceinline__ uint32_t copy_piece(const Feed& f, int64_t rows, const char* from, const char* to, unsigned char* dst,
+                                               bool issue, uint64_t* bar) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(from), end = reinterpret_cast<uintptr_t>(to);
+  const uintptr_t low = begin & ~uintptr_t(15);
+  uintptr_t a = low, b = (end + 15) & ~uintptr_t(15);
+  if (a < reinterpret_cast<uintptr_t>(f.p)) a += 16;
+  if (b > reinterpret_cast<uintptr_t>(f.p) + (rows - 1) * f.stride + f.row_bytes) b -= 16;
+  if (b < a) b = a;  // nothing but ends
+  if (!issue) {
+    const uintptr_t head = a < end ? a : end, tail = b > head ? b : head;
+    for (uintptr_t p = begin; p < head; p += 2) *reinterpret_cast<uint16_t*>(dst + (p - low)) = *reinterpret_cast<const uint16_t*>(p);
+    for (uintptr_t p = tail; p < end; p += 2) *reinterpret_cast<uint16_t*>(dst + (p - low)) = *reinterpret_cast<const uint16_t*>(p);
+  } else if (b > a) {
+    bulk_load(dst + (a - low), reinterpret_cast<const void*>(a), static_cast<uint32_t>(b - a), bar);
+  }
+  return static_cast<uint32_t>(b - a);
+}
+
+struct Ring {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+};
+
+__device__ __forceinline__ void ring_init(Ring& ring, int stages, int workers) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], workers / 32);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+}
+
+// The loading warp: tiles block, block + grid, ... A wait that runs out is recorded, and no later one
+// is waited for: the kernel then ends soon, with an error that jk_device_status reports.
+__device__ __forceinline__ void load_tiles(const Plan& plan, Ring& ring, unsigned char* memory, int64_t rows) {
+  const int lane = threadIdx.x & 31;
+  bool good = true;
+  int stage = 0;
+  uint32_t turn = 0;
+  const int64_t tiles = (rows + plan.tile_rows - 1) / plan.tile_rows;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    if (turn > 0 && good) good = mbar_wait(&ring.empty[stage], (turn - 1) & 1);
+    const int64_t r0 = tile * plan.tile_rows;
+    const int n = static_cast<int>(rows - r0 < plan.tile_rows ? rows - r0 : plan.tile_rows);
+    unsigned char* base = memory + static_cast<size_t>(stage) * plan.stage_bytes;
+    uint32_t bytes = 0;
+    for (int issue = 0; issue < 2; ++issue) {
+      for (int k = 0; k < plan.feeds; ++k) {
+        const Feed& f = plan.feed[k];
+        if (f.pitch == 0) {
+          if (lane == k) {
+            const char* from = f.p + r0 * f.stride;
+            bytes += copy_piece(f, rows, from, from + static_cast<int64_t>(n) * f.row_bytes, base + f.offset, issue != 0, &ring.full[stage]);
+          }
+        } else {
+          for (int i = lane; i < n; i += 32) {
+            const char* from = f.p + (r0 + i) * f.stride;
+            bytes += copy_piece(f, rows, from, from + f.row_bytes, base + f.offset + i * f.pitch, issue != 0, &ring.full[stage]);
+          }
+        }
+      }
+      if (issue == 0) {
+        bytes = __reduce_add_sync(0xffffffffu, bytes);
+        if (lane == 0) mbar_arrive_expect_tx(&ring.full[stage], bytes);
+        __syncwarp();
+      }
+    }
+    if (++stage == plan.stages) stage = 0, ++turn;
+  }
+  // copies in flight land before the block's memory is given back
+  for (int i = 0; i < plan.stages; ++i) {
+    const uint32_t loads = turn + (i < stage ? 1 : 0);
+    if (loads > 0 && good) good = mbar_wait(&ring.full[i], (loads - 1) & 1);
+  }
+  if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
+}
+
+// `take(i, r, stage)` for the tiles' rows that this thread's group has: i in the tile, r in all.
+template <int TPR, typename F>
+__device__ __forceinline__ void take_tiles(const Plan& plan, Ring& ring, const unsigned char* memory, int64_t rows, F&& take) {
+  bool good = true;
+  int stage = 0;
+  uint32_t turn = 0;
+  const int64_t tiles = (rows + plan.tile_rows - 1) / plan.tile_rows;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    if (good) good = mbar_wait(&ring.full[stage], turn & 1);
+    const int64_t r0 = tile * plan.tile_rows;
+    const int n = static_cast<int>(rows - r0 < plan.tile_rows ? rows - r0 : plan.tile_rows);
+    const unsigned char* base = memory + static_cast<size_t>(stage) * plan.stage_bytes;
+    for (int i = threadIdx.x / TPR; i < n; i += kGroups<TPR>) take(i, r0, base);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[stage]);
+    if (++stage == plan.stages) stage = 0, ++turn;
+  }
+  if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
+}
+
+template <typename T, int N, int TPR, bool DELTA>
+__global__ void __launch_bounds__(kBlock<TPR> + 32) staged_forward_kernel(const Forward a, const __grid_constant__ Plan plan) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ Ring ring;
+  __shared__ float scratch[2][1][32];
+  ring_init(ring, plan.stages, kBlock<TPR>);
+  if (threadIdx.x >= kBlock<TPR>) {
+    load_tiles(plan, ring, memory, a.rows);
+    return;
+  }
+  const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
+  float w[N], b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = i * TPR + thread;
+    w[i] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
+    b[i] = c < dim ? param_at(a.bias, c, a.param_type, 0.f) : 0.f;
+  }
+  const float inv = 1.f / static_cast<float>(dim);
+  take_tiles<TPR>(plan, ring, memory, a.rows, [&](int row, int64_t r0, const unsigned char* stage) {
+    const T* x = reinterpret_cast<const T*>(staged(plan.feed[0], stage, r0, row));
+    const T* d = DELTA ? reinterpret_cast<const T*>(staged(plan.feed[1], stage, r0, row)) : nullptr;
+    float f[N], s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * TPR + thread;
+      f[i] = 0.f;
+      if (c < dim) {
+        f[i] = to_f32(x[c]);
+        if (DELTA) f[i] = fmaf(a.scale, to_f32(d[c]), f[i]);
+      }
+      s[0] += f[i];
+    }
+    row_sums<TPR, 1, true>(s, scratch, 0);
+    const float mu = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float v = i * TPR + thread < dim ? f[i] - mu : 0.f;
+      s[0] = fmaf(v, v, s[0]);
+    }
+    row_sums<TPR, 1, true>(s, scratch, 1);
+    const float rs = rsqrtf(fmaf(s[0], inv, a.eps));
+    const int64_t r = r0 + row;
+    T *y = static_cast<T*>(a.y) + r * dim, *sum = a.sum == nullptr ? nullptr : static_cast<T*>(a.sum) + r * dim;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * TPR + thread;
+      if (c < dim) {
+        y[c] = from_f32<T>(fmaf((f[i] - mu) * rs, w[i], b[i]));
+        if (sum != nullptr) sum[c] = from_f32<T>(f[i]);
+      }
+    }
+    if (thread == 0 && a.mean != nullptr) {
+      a.mean[r] = mu;
+      a.rstd[r] = rs;
+    }
+  });
+}
+
+template <typename T, int N, int TPR, bool SUM, bool PARAMS>
+__global__ void __launch_bounds__(kBlock<TPR> + 32) staged_backward_kernel(const Backward a, const __grid_constant__ Plan plan) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ Ring ring;
+  __shared__ float scratch[2][2][32];
+  constexpr bool kShared = PARAMS && TPR <= 32;
+  __shared__ float shared[kShared ? N * TPR * 2 : 1];
+  ring_init(ring, plan.stages, kBlock<TPR>);
+  if (threadIdx.x >= kBlock<TPR>) {
+    load_tiles(plan, ring, memory, a.rows);
+    return;
+  }
+  const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
+  float w[N], dw[N][1] = {}, db[N][1] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = i * TPR + thread;
+    w[i] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
+  }
+  const float inv = 1.f / static_cast<float>(dim);
+  int turn = 0;
+  take_tiles<TPR>(plan, ring, memory, a.rows, [&](int row, int64_t r0, const unsigned char* stage) {
+    const float mu = *reinterpret_cast<const float*>(staged(plan.feed[0], stage, r0, row));
+    const float rs = *reinterpret_cast<const float*>(staged(plan.feed[1], stage, r0, row));
+    const T* gy = reinterpret_cast<const T*>(staged(plan.feed[2], stage, r0, row));
+    const T* h = reinterpret_cast<const T*>(staged(plan.feed[3], stage, r0, row));
+    float g[N], n[N], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * TPR + thread;
+      g[i] = n[i] = 0.f;
+      if (c < dim) {
+        g[i] = to_f32(gy[c]);
+        n[i] = (to_f32(h[c]) - mu) * rs;
+      }
+      if (PARAMS) {
+        dw[i][0] = fmaf(g[i], n[i], dw[i][0]);
+        db[i][0] += g[i];
+      }
+      const float u = g[i] * w[i];
+      s[0] += u;
+      s[1] = fmaf(u, n[i], s[1]);
+    }
+    row_sums<TPR, 2, true>(s, scratch, turn);
+    turn ^= 1;
+    const float c0 = s[0] * inv, c1 = s[1] * inv;
+    const T* gs = SUM ? reinterpret_cast<const T*>(staged(plan.feed[4], stage, r0, row)) : nullptr;
+    const int64_t r = r0 + row;
+    T *gx = static_cast<T*>(a.grad_x) + r * dim, *gd = a.grad_delta == nullptr ? nullptr : static_cast<T*>(a.grad_delta) + r * dim;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * TPR + thread;
+      if (c < dim) {
+        float o = fmaf(g[i], w[i], -fmaf(n[i], c1, c0));
+        o = SUM ? fmaf(rs, o, to_f32(gs[c])) : rs * o;
+        gx[c] = from_f32<T>(o);
+        if (gd != nullptr) gd[c] = from_f32<T>(a.scale * o);
+      }
+    }
+  });
+  if constexpr (PARAMS) {
+    grid_dependency_launch();
+    leave_parts<1, N, TPR, true>(dw, db, dim, a.parts, shared);
   }
 }
 
@@ -473,6 +736,98 @@ int pick_backward(const Backward& a, cudaStream_t s) {
                             : run_backward<backward_kernel<T, VEC, N, TPR, false, false>, TPR>(a, s);
 }
 
+constexpr int kNoRoom = -1000;  // no status
+
+// A plan for rows off boundaries: tiles of some 8 KB, as many in flight as fill an SM's shared memory
+// with the blocks that it holds. False if two tiles of one row do not fit.
+struct Tiles {
+  int blocks_per_sm;
+  size_t smem;
+};
+inline bool plan_tiles(Plan& plan, int64_t rows, int groups, int want_blocks, Tiles& tiles) {
+  int64_t row = 0;
+  for (int k = 0; k < plan.feeds; ++k) row += plan.feed[k].row_bytes;
+  int64_t tile_rows = groups;
+  while (tile_rows * 2 <= kMaxTileRows && tile_rows * 2 * row <= 8192) tile_rows *= 2;
+  const int64_t least = (rows + 148 * want_blocks - 1) / (148 * want_blocks);  // rows of a block
+  while (tile_rows > groups && tile_rows > least) tile_rows /= 2;
+  plan.tile_rows = static_cast<int>(tile_rows);
+  uint32_t at = 0;
+  for (int k = 0; k < plan.feeds; ++k) {
+    Feed& f = plan.feed[k];
+    f.offset = at;
+    f.pitch = f.stride == f.row_bytes ? 0 : (f.row_bytes + 15 + 15) / 16 * 16;
+    at += f.pitch == 0 ? static_cast<uint32_t>((tile_rows * f.row_bytes + 15 + 15) / 16 * 16) : static_cast<uint32_t>(tile_rows * f.pitch);
+  }
+  plan.stage_bytes = at;
+  constexpr int64_t kRoom = 200 * 1024;
+  int blocks = want_blocks;
+  while (blocks > 1 && kRoom / blocks < 3 * static_cast<int64_t>(at)) --blocks;
+  const int64_t fit = kRoom / blocks / at;
+  if (fit < 2) return false;
+  plan.stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
+  tiles = {blocks, static_cast<size_t>(plan.stages) * at};
+  return true;
+}
+
+template <typename T>
+Feed feed_of(const void* p, int64_t stride, int64_t dim) {
+  return {static_cast<const char*>(p), stride * static_cast<int64_t>(sizeof(T)), static_cast<int>(dim * sizeof(T)), 0, 0};
+}
+
+template <auto KERNEL>
+bool allow(size_t smem) {
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess) return true;
+  cudaGetLastError();
+  return false;
+}
+
+template <auto KERNEL, typename T, int TPR>
+int run_staged_forward(const Forward& a, cudaStream_t s) {
+  Plan plan = {};
+  plan.feed[plan.feeds++] = feed_of<T>(a.x, a.x_stride, a.dim);
+  if (a.delta != nullptr) plan.feed[plan.feeds++] = feed_of<T>(a.delta, a.delta_stride, a.dim);
+  Tiles tiles;
+  if (!plan_tiles(plan, a.rows, kGroups<TPR>, blocks_per_sm<KERNEL>(kBlock<TPR> + 32), tiles)) return kNoRoom;
+  if (!allow<KERNEL>(tiles.smem)) return JK_ERR_LAUNCH;
+  const int64_t blocks = groups_to_blocks(a.rows, plan.tile_rows, 148ll * tiles.blocks_per_sm);
+  KERNEL<<<static_cast<unsigned>(blocks), kBlock<TPR> + 32, tiles.smem, s>>>(a, plan);
+  return 0;
+}
+
+template <auto KERNEL, typename T, int TPR>
+int run_staged_backward(const Backward& a, cudaStream_t s) {
+  Plan plan = {};
+  plan.feed[plan.feeds++] = feed_of<float>(a.mean, 1, 1);
+  plan.feed[plan.feeds++] = feed_of<float>(a.rstd, 1, 1);
+  plan.feed[plan.feeds++] = feed_of<T>(a.grad_y, a.grad_y_stride, a.dim);
+  plan.feed[plan.feeds++] = feed_of<T>(a.sum, a.sum_stride, a.dim);
+  if (a.grad_sum != nullptr) plan.feed[plan.feeds++] = feed_of<T>(a.grad_sum, a.grad_sum_stride, a.dim);
+  Tiles tiles;
+  if (!plan_tiles(plan, a.rows, kGroups<TPR>, blocks_per_sm<KERNEL>(kBlock<TPR> + 32), tiles)) return kNoRoom;
+  if (!allow<KERNEL>(tiles.smem)) return JK_ERR_LAUNCH;
+  int64_t most = 148ll * tiles.blocks_per_sm;
+  if (a.parts != nullptr && most > kMaxParts) most = kMaxParts;
+  const int blocks = static_cast<int>(groups_to_blocks(a.rows, plan.tile_rows, most));
+  KERNEL<<<blocks, kBlock<TPR> + 32, tiles.smem, s>>>(a, plan);
+  return blocks;
+}
+
+template <typename T, int N, int TPR>
+int pick_staged_forward(const Forward& a, cudaStream_t s) {
+  return a.delta != nullptr ? run_staged_forward<staged_forward_kernel<T, N, TPR, true>, T, TPR>(a, s)
+                            : run_staged_forward<staged_forward_kernel<T, N, TPR, false>, T, TPR>(a, s);
+}
+
+template <typename T, int N, int TPR>
+int pick_staged_backward(const Backward& a, cudaStream_t s) {
+  if (a.grad_sum != nullptr)
+    return a.parts != nullptr ? run_staged_backward<staged_backward_kernel<T, N, TPR, true, true>, T, TPR>(a, s)
+                              : run_staged_backward<staged_backward_kernel<T, N, TPR, true, false>, T, TPR>(a, s);
+  return a.parts != nullptr ? run_staged_backward<staged_backward_kernel<T, N, TPR, false, true>, T, TPR>(a, s)
+                            : run_staged_backward<staged_backward_kernel<T, N, TPR, false, false>, T, TPR>(a, s);
+}
+
 // The threads of a row and their turns: as few threads as hold it with 16 elements each (fewer where
 // a warp has room), a warp's or less while that does, so that no barrier is needed.
 #define JK_NORM_SHAPES(RUN)                                             \
@@ -497,20 +852,31 @@ int pick_backward(const Backward& a, cudaStream_t s) {
     return RUN(4, 1024);                                                \
   } else {                                                              \
     if (turns <= 32) return RUN(1, 32);                                 \
+    if (turns <= 64) return RUN(2, 32);                                 \
     if (turns <= 128) return RUN(4, 32);                                \
+    if (turns <= 256) return RUN(8, 32);                                \
     if (turns <= 512) return RUN(16, 32);                               \
-    if (turns <= 2048) return RUN(16, 128);                             \
-    if (turns <= 4096) return RUN(16, 256);                             \
-    if (turns <= 8192) return RUN(16, 512);                             \
-    return RUN(16, 1024);                                               \
+    if (turns <= 1024) return RUN(8, 128);                              \
+    if (turns <= 2048) return RUN(8, 256);                              \
+    if (turns <= 4096) return RUN(8, 512);                              \
+    return RUN(16, 512);                                                \
   }
 
-constexpr int64_t kMaxDim = 16384;  // of the rows that stay in registers
+constexpr int64_t kMaxDim = 16384, kMaxStagedDim = 8192;  // of the rows that stay in registers
 
 template <typename T, int VEC>
 int shape_forward(const Forward& a, cudaStream_t s) {
   const int64_t turns = a.dim / VEC;
 #define JK_RUN(N, TPR) pick_forward<T, VEC, N, TPR>(a, s)
+  JK_NORM_SHAPES(JK_RUN)
+#undef JK_RUN
+}
+
+template <typename T>
+int shape_staged_forward(const Forward& a, cudaStream_t s) {
+  constexpr int VEC = 1;
+  const int64_t turns = a.dim;
+#define JK_RUN(N, TPR) pick_staged_forward<T, N, TPR>(a, s)
   JK_NORM_SHAPES(JK_RUN)
 #undef JK_RUN
 }
@@ -524,37 +890,51 @@ int shape_backward(const Backward& a, cudaStream_t s) {
 }
 
 template <typename T>
+int shape_staged_backward(const Backward& a, cudaStream_t s) {
+  constexpr int VEC = 1;
+  const int64_t turns = a.dim;
+#define JK_RUN(N, TPR) pick_staged_backward<T, N, TPR>(a, s)
+  JK_NORM_SHAPES(JK_RUN)
+#undef JK_RUN
+}
+
+template <typename T>
 bool in_packs(const void* p, int64_t stride) {
   return p == nullptr || (aligned16(p) && stride % kPack<T> == 0);
 }
 
 template <typename T>
-void forward(const Forward& a, cudaStream_t s) {
-  if (a.dim > kMaxDim) {
-    long_forward_kernel<T><<<static_cast<unsigned>(a.rows < 148 * 4 ? a.rows : 148 * 4), kLongThreads, 0, s>>>(a);
-  } else if (in_packs<T>(a.x, a.x_stride) && in_packs<T>(a.delta, a.delta_stride) && in_packs<T>(a.y, a.dim) &&
-             in_packs<T>(a.sum, a.dim)) {
-    shape_forward<T, kPack<T>>(a, s);
-  } else {
-    shape_forward<T, 1>(a, s);
+int forward(const Forward& a, cudaStream_t s) {
+  if (a.dim <= kMaxDim && in_packs<T>(a.x, a.x_stride) && in_packs<T>(a.delta, a.delta_stride) && in_packs<T>(a.y, a.dim) &&
+      in_packs<T>(a.sum, a.dim))
+    return shape_forward<T, kPack<T>>(a, s);
+  if (a.dim <= kMaxStagedDim) {
+    const int done = shape_staged_forward<T>(a, s);
+    if (done != kNoRoom) return done;
   }
+  long_forward_kernel<T><<<static_cast<unsigned>(a.rows < 148 * 4 ? a.rows : 148 * 4), kLongThreads, 0, s>>>(a);
+  return 0;
 }
 
-// Returns the blocks that left a share of the parameter gradients.
+// Returns the blocks that left a share of the parameter gradients, or a status.
 template <typename T>
 int backward(const Backward& a, cudaStream_t s) {
-  if (a.dim > kMaxDim) {
-    const int blocks = static_cast<int>(a.rows < kMaxParts ? a.rows : kMaxParts);
-    long_backward_kernel<T><<<blocks, kLongThreads, 0, s>>>(a);
-    return blocks;
-  }
-  if (in_packs<T>(a.grad_y, a.grad_y_stride) && in_packs<T>(a.sum, a.sum_stride) && in_packs<T>(a.grad_sum, a.grad_sum_stride) &&
-      in_packs<T>(a.grad_x, a.dim) && in_packs<T>(a.grad_delta, a.dim))
+  if (a.dim <= kMaxDim && in_packs<T>(a.grad_y, a.grad_y_stride) && in_packs<T>(a.sum, a.sum_stride) &&
+      in_packs<T>(a.grad_sum, a.grad_sum_stride) && in_packs<T>(a.grad_x, a.dim) && in_packs<T>(a.grad_delta, a.dim))
     return shape_backward<T, kPack<T>>(a, s);
-  return shape_backward<T, 1>(a, s);
+  if (a.dim <= kMaxStagedDim) {
+    const int done = shape_staged_backward<T>(a, s);
+    if (done != kNoRoom) return done;
+  }
+  const int blocks = static_cast<int>(a.rows < kMaxParts ? a.rows : kMaxParts);
+  long_backward_kernel<T><<<blocks, kLongThreads, 0, s>>>(a);
+  return blocks;
 }
 
 }  // namespace norm
+
+JK_ERROR_READER(read_error_norm)
+
 }  // namespace jk
 
 extern "C" int jk_layer_norm_forward(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride,
@@ -570,8 +950,8 @@ extern "C" int jk_layer_norm_forward(const void* x, int64_t x_stride, const void
   if (st != JK_OK) return st;
   const norm::Forward a{x, delta, x_stride, delta_stride, delta_scale, weight, bias, param_dtype,
                         rows, dim, eps, y, sum, mean, rstd};
-  JK_WITH_TYPE(dtype, T, norm::forward<T>(a, reinterpret_cast<cudaStream_t>(stream)));
-  return launch_status();
+  JK_WITH_TYPE(dtype, T, st = norm::forward<T>(a, reinterpret_cast<cudaStream_t>(stream)));
+  return st < 0 ? st : launch_status();
 }
 
 extern "C" int64_t jk_layer_norm_backward_workspace(int64_t rows, int64_t dim) {
@@ -599,6 +979,7 @@ extern "C" int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride,
                          delta_scale, rows, dim, grad_x, grad_delta, params ? workspace : nullptr};
   int parts = 0;
   if (rows > 0) JK_WITH_TYPE(dtype, T, parts = norm::backward<T>(a, s));
+  if (parts < 0) return parts;
   if (params)
     JK_WITH_TYPE(param_dtype, W, launch_dependent(norm::parameters_kernel<W>, static_cast<unsigned>((2 * dim + 31) / 32), 1024, 0, s,
                                                   workspace, parts, dim, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias)));
