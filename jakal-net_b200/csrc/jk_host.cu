@@ -96,7 +96,7 @@ int jk_device_status(jk_stream_t stream, int* device_status) {
   }
   int (*readers[])(int*) = {jk::read_error_project,  jk::read_error_topk,     jk::read_error_topk_bf16,
                             jk::read_error_topk_f16, jk::read_error_topk_f32, jk::read_error_window,
-                            jk::read_error_clip,     jk::read_error_loss,     jk::read_error_norm};
+                            jk::read_error_clip,     jk::read_error_loss};
   int combined = JK_OK;
   for (auto read : readers) {
     int value = JK_OK;

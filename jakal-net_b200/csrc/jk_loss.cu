@@ -71,28 +71,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return r;
 }
 
-// Two f32 in a register pair: one instruction works on both.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // The largest of N packs, NaN aside; 16-bit types two at a time.
 template <typename T, int N>
 __device__ __forceinline__ float pack_max(const uint4 (&raw)[N]) {

@@ -9,23 +9,22 @@
 // E[sum^2] - mean^2, which cancels where the mean is large against the spread.
 //
 // Bound: memory, every row read once and written once. A row of up to 16384 elements stays in the
-// registers of the 8 to 1024 threads that share it, each with up to 16 elements; a thread keeps its
-// columns for all rows it comes to, so the parameters and, backward, the sums of their gradients stay
-// in its registers too. Three forms:
-//   * forward_kernel, backward_kernel: rows that lie in 16-byte packs, a pack at a time, the next row
-//     on its way in registers while one is worked on;
-//   * staged_forward_kernel, staged_backward_kernel: rows that do not (an odd width, an odd offset).
-//     One warp has tiles of rows copied to shared memory as they lie, in 16-byte blocks, tiles ahead;
-//     the others take their elements from there one by one, whatever their alignment;
-//   * long_*: longer rows, read again for each sum.
+// registers of the 8 to 1024 threads that share it, each with up to 16 elements, in 16-byte packs. A
+// thread keeps its columns for all rows it comes to, so the parameters and, backward, the sums of
+// their gradients stay in its registers too, and the next row is on its way while one is worked on.
+//
+// Rows of an odd width begin anywhere within a 16-byte block, but those a multiple of 8 (16-bit) or 4
+// rows apart begin alike: the rows of a group of threads are that far apart, so its packs lie on
+// 16-byte boundaries all the same (SHIFTED), whole but for a row's first and last. Where the tensors
+// lie differently from each other, elements are taken one by one. Longer rows are read again for
+// each sum.
 #include "jk_host.h"
 #include "jk_rows.cuh"
-#include "jk_sm100.cuh"
 
 namespace jk {
 namespace norm {
 
-constexpr int kMaxParts = 148 * 2;  // blocks that leave their share of the parameter gradients
+constexpr int kMaxParts = 148 * 4;  // blocks that leave their share of the parameter gradients
 
 struct Forward {
   const void *x, *delta;
@@ -65,18 +64,34 @@ template <typename T, int VEC>
 struct Raw {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ T* elements() { return reinterpret_cast<T*>(&v); }
   __device__ __forceinline__ void floats(float (&f)[VEC]) const { unpack<T>(v, f); }
   static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) { *reinterpret_cast<uint4*>(p) = pack<T>(f); }
 };
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void clear() { v = from_f32<T>(0.f); }
+  __device__ __forceinline__ T* elements() { return &v; }
+  __device__ __forceinline__ void floats(float (&f)[1]) const { f[0] = to_f32(v); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
+};
+
 // Threads of a block, and rows that it has at a time, with `TPR` threads to a row.
 template <int TPR>
 constexpr int kBlock = TPR > 256 ? TPR : (TPR > 32 ? TPR : 256);
 template <int TPR>
 constexpr int kGroups = kBlock<TPR> / TPR;
 
+// The least power of two from n on.
+template <int n>
+constexpr int kPowerOfTwo = n <= 1 ? 1 : 2 * kPowerOfTwo<(n + 1) / 2>;
+
 // Sums over the threads of a row, in all of them. With more than a warp to a row the row has the
 // whole block; `turn` alternates, so that one barrier does.
-template <int TPR, int COUNT, bool STAGED = false>
+template <int TPR, int COUNT>
 __device__ __forceinline__ void row_sums(float (&v)[COUNT], float (*scratch)[COUNT][32], int turn) {
 #pragma unroll
   for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
@@ -87,189 +102,328 @@ __device__ __forceinline__ void row_sums(float (&v)[COUNT], float (*scratch)[COU
     if (lane == 0)
 #pragma unroll
       for (int i = 0; i < COUNT; ++i) scratch[turn][i][threadIdx.x >> 5] = v[i];
-    if constexpr (STAGED)
-      asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");  // not the loading warp
-    else
-      __syncthreads();
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       v[i] = lane < TPR / 32 ? scratch[turn][i][lane] : 0.f;
 #pragma unroll
-      for (int o = TPR / 64; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      for (int o = kPowerOfTwo<TPR / 32> / 2; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
       if constexpr (TPR < 1024) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
     }
   }
 }
 
-template <typename T, int VEC, int N, int TPR, bool DELTA>
-__global__ void __launch_bounds__(kBlock<TPR>) forward_kernel(const Forward a) {
+// How far row r is from a 16-byte boundary, in elements, for the rows that a group of threads has.
+template <typename T, bool SHIFTED>
+__device__ __forceinline__ int shift_of(const T* p, int64_t r, int64_t stride) {
+  return SHIFTED ? static_cast<int>(reinterpret_cast<uintptr_t>(p + r * stride) & 15) / static_cast<int>(sizeof(T)) : 0;
+}
+
+// Which of a pack's columns from c on the row has, a bit for each.
+template <int VEC>
+__device__ __forceinline__ uint32_t columns_of(int c, int dim) {
+  const int from = min(max(-c, 0), VEC), to = min(max(dim - c, 0), VEC);
+  return ((1u << to) - 1u) & ~((1u << from) - 1u);
+}
+template <int VEC>
+constexpr uint32_t kWhole = (1u << VEC) - 1u;
+
+// A pack at p. Columns that the row does not have are read as they come (they are another row's), but
+// not past an end of the tensor (`first`, `last` row).
+template <typename T, int VEC, bool SHIFTED>
+__device__ __forceinline__ void load_pack(Raw<T, VEC>& raw, const T* p, uint32_t columns, bool first, bool last) {
+  if (SHIFTED && ((first && !(columns & 1u)) || (last && !(columns >> (VEC - 1))))) {
+    Raw<T, VEC> some;  // a rare case: in local memory, so that it takes no registers from the others
+    some.clear();
+#pragma unroll 1
+    for (int j = 0; j < VEC; ++j)
+      if ((columns >> j) & 1u) some.elements()[j] = p[j];
+    raw = some;
+  } else {
+    raw.load(p);
+  }
+}
+
+// Clears what a pack has of columns outside the row.
+template <int VEC, bool SHIFTED>
+__device__ __forceinline__ void clear_outside(float (&f)[VEC], uint32_t columns) {
+  if (SHIFTED && columns != kWhole<VEC>) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = (columns >> j) & 1u ? f[j] : 0.f;
+  }
+}
+
+// A pack's columns [0, m) or, `tail` false, its last m, in halves, quarters and one element: the pack
+// lies on a 16-byte boundary, and m is less than a pack.
+__device__ __forceinline__ void store_some(void* p, const uint4& u, int m, bool tail, int size) {
+  char* to = static_cast<char*>(p);
+  const int bytes = m * size;
+  if (bytes & 8) *reinterpret_cast<uint2*>(to + (tail ? 0 : 8)) = tail ? make_uint2(u.x, u.y) : make_uint2(u.z, u.w);
+  if (bytes & 4) {
+    const int at = tail ? bytes & 8 : 12 - (bytes & 8);
+    *reinterpret_cast<uint32_t*>(to + at) = tail ? (at == 0 ? u.x : u.z) : (at == 12 ? u.w : u.y);
+  }
+  if (bytes & 2) {
+    const int at = tail ? bytes - 2 : 16 - bytes;
+    const uint32_t low = at & 4 ? u.y : u.x, high = at & 4 ? u.w : u.z, word = at & 8 ? high : low;
+    *reinterpret_cast<uint16_t*>(to + at) = static_cast<uint16_t>(at & 2 ? word >> 16 : word);
+  }
+}
+
+template <typename T, int VEC, bool SHIFTED>
+__device__ __forceinline__ void store_pack(T* p, uint32_t columns, const float (&f)[VEC]) {
+  if (!SHIFTED || columns == kWhole<VEC>) {
+    Raw<T, VEC>::store(p, f);
+  } else if (columns & (1u | 1u << (VEC - 1))) {
+    uint4 u;
+    Raw<T, VEC>::store(reinterpret_cast<T*>(&u), f);
+    store_some(p, u, __popc(columns), columns & 1u, static_cast<int>(sizeof(T)));
+  } else {  // a row within a pack
+    Raw<T, VEC> some;
+    Raw<T, VEC>::store(some.elements(), f);
+#pragma unroll 1
+    for (int j = 0; j < VEC; ++j)
+      if ((columns >> j) & 1u) p[j] = some.elements()[j];
+  }
+}
+
+// (f - a) * b, element by element; two at a time where there are two.
+template <int VEC>
+__device__ __forceinline__ void centre(float (&f)[VEC], float a, float b) {
+  if constexpr (VEC == 1) {
+    f[0] = (f[0] - a) * b;
+  } else {
+    const uint64_t minus = pair(-a, -a), by = pair(b, b);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const float2 v = unpair(mul2(add2(pair(f[j], f[j + 1]), minus), by));
+      f[j] = v.x, f[j + 1] = v.y;
+    }
+  }
+}
+
+// a * b + c
+template <int VEC>
+__device__ __forceinline__ void multiply_add(float (&o)[VEC], const float (&a)[VEC], const float (&b)[VEC], const float (&c)[VEC]) {
+  if constexpr (VEC == 1) {
+    o[0] = fmaf(a[0], b[0], c[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const float2 v = unpair(fma2(pair(a[j], a[j + 1]), pair(b[j], b[j + 1]), pair(c[j], c[j + 1])));
+      o[j] = v.x, o[j + 1] = v.y;
+    }
+  }
+}
+
+// a * s + c, with one factor
+template <int VEC>
+__device__ __forceinline__ void scale_add(float (&o)[VEC], const float (&a)[VEC], float s, const float (&c)[VEC]) {
+  if constexpr (VEC == 1) {
+    o[0] = fmaf(a[0], s, c[0]);
+  } else {
+    const uint64_t by = pair(s, s);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const float2 v = unpair(fma2(pair(a[j], a[j + 1]), by, pair(c[j], c[j + 1])));
+      o[j] = v.x, o[j + 1] = v.y;
+    }
+  }
+}
+
+// A sum in two halves, and what is added to it: f, and a * b.
+struct Two {
+  uint64_t v;
+  __device__ __forceinline__ Two() : v(0) {}
+  template <int VEC>
+  __device__ __forceinline__ void add(const float (&f)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) v = add2(v, pair(f[j], VEC > 1 ? f[j + (VEC > 1)] : 0.f));
+  }
+  template <int VEC>
+  __device__ __forceinline__ void add(const float (&a)[VEC], const float (&b)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2)
+      v = fma2(pair(a[j], VEC > 1 ? a[j + (VEC > 1)] : 0.f), pair(b[j], VEC > 1 ? b[j + (VEC > 1)] : 0.f), v);
+  }
+  __device__ __forceinline__ float sum() const {
+    const float2 f = unpair(v);
+    return f.x + f.y;
+  }
+};
+
+template <typename T, int VEC, int N, int TPR, bool SHIFTED, bool DELTA>
+__global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? (N == 1 && TPR > 32 ? 768 : 512) / kBlock<TPR> : 1) forward_kernel(const Forward a) {
   __shared__ float scratch[2][1][32];
   const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups<TPR>;
-  const T *x = static_cast<const T*>(a.x), *delta = static_cast<const T*>(a.delta);
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups<TPR> + threadIdx.x / TPR;
+  const int first_column = thread * VEC - shift_of<T, SHIFTED>(static_cast<const T*>(a.x), r, a.x_stride);
+  constexpr int kNext = TPR * VEC;  // columns from one pack of a thread to its next
+  const T *x = static_cast<const T*>(a.x) + r * a.x_stride + first_column,
+          *delta = static_cast<const T*>(a.delta) + (DELTA ? r * a.delta_stride + first_column : 0);
+  const int64_t out = r * dim + first_column;
+  T *y = static_cast<T*>(a.y) + out, *sum = a.sum == nullptr ? nullptr : static_cast<T*>(a.sum) + out;
   float w[N][VEC], b[N][VEC];
+  uint32_t columns[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) columns[i] = columns_of<VEC>(first_column + i * kNext, dim);
   Raw<T, VEC> next_x[N], next_d[DELTA ? N : 1];
-  const auto load = [&](int64_t r) {
+  const auto load = [&](int64_t r) {  // row r, at x
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
-      if (c < dim) {
-        next_x[i].load(x + r * a.x_stride + c);
-        if (DELTA) next_d[DELTA ? i : 0].load(delta + r * a.delta_stride + c);
+      if (columns[i] != 0) {
+        load_pack<T, VEC, SHIFTED>(next_x[i], x + i * kNext, columns[i], r == 0, r == a.rows - 1);
+        if (DELTA) load_pack<T, VEC, SHIFTED>(next_d[DELTA ? i : 0], delta + i * kNext, columns[i], r == 0, r == a.rows - 1);
       }
     }
+    x += step * a.x_stride;
+    if (DELTA) delta += step * a.delta_stride;
   };
-  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups<TPR> + threadIdx.x / TPR;
   if (r < a.rows) load(r);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const int c = (i * TPR + thread) * VEC + j;
-      w[i][j] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
-      b[i][j] = c < dim ? param_at(a.bias, c, a.param_type, 0.f) : 0.f;
+      const bool has = (columns[i] >> j) & 1u;
+      w[i][j] = has ? param_at(a.weight, first_column + i * kNext + j, a.param_type, 1.f) : 0.f;
+      b[i][j] = has ? param_at(a.bias, first_column + i * kNext + j, a.param_type, 0.f) : 0.f;
     }
   const float inv = 1.f / static_cast<float>(dim);
   // all groups of a block take as many turns, as they may share a warp
   for (int64_t base = r - threadIdx.x / TPR; base < a.rows; base += step, r += step) {
     const bool here = r < a.rows;
-    float f[N][VEC], s[1] = {0.f};
+    float f[N][VEC], s[1];
+    Two total;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
-      if (here && c < dim) {
+      if (here && columns[i] != 0) {
         next_x[i].floats(f[i]);
         if (DELTA) {
           float d[VEC];
           next_d[DELTA ? i : 0].floats(d);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[i][j] = fmaf(a.scale, d[j], f[i][j]);
+          scale_add<VEC>(f[i], d, a.scale, f[i]);
         }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[0] += f[i][j];
+        clear_outside<VEC, SHIFTED>(f[i], columns[i]);
+        total.add(f[i]);
       }
     }
     if (r + step < a.rows) load(r + step);
+    s[0] = total.sum();
     row_sums<TPR, 1>(s, scratch, 0);
     const float mu = s[0] * inv;
-    s[0] = 0.f;
+    Two squares;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
-      if (here && c < dim) {
+      if (here && columns[i] != 0) {
+        float d[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = f[i][j] - mu;
-          s[0] = fmaf(d, d, s[0]);
-        }
+        for (int j = 0; j < VEC; ++j) d[j] = f[i][j];
+        centre<VEC>(d, mu, 1.f);
+        clear_outside<VEC, SHIFTED>(d, columns[i]);
+        squares.add(d, d);
       }
     }
+    s[0] = squares.sum();
     row_sums<TPR, 1>(s, scratch, 1);
     const float rs = rsqrtf(fmaf(s[0], inv, a.eps));
-    if (!here) continue;
+    if (here) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
-      if (c < dim) {
-        float o[VEC];
+      for (int i = 0; i < N; ++i) {
+        if (columns[i] != 0) {
+          float o[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = fmaf((f[i][j] - mu) * rs, w[i][j], b[i][j]);
-        Raw<T, VEC>::store(static_cast<T*>(a.y) + r * dim + c, o);
-        if (a.sum != nullptr) Raw<T, VEC>::store(static_cast<T*>(a.sum) + r * dim + c, f[i]);
+          for (int j = 0; j < VEC; ++j) o[j] = f[i][j];
+          centre<VEC>(o, mu, rs);
+          multiply_add<VEC>(o, o, w[i], b[i]);
+          store_pack<T, VEC, SHIFTED>(y + i * kNext, columns[i], o);
+          if (sum != nullptr) store_pack<T, VEC, SHIFTED>(sum + i * kNext, columns[i], f[i]);
+        }
+      }
+      if (thread == 0 && a.mean != nullptr) {
+        a.mean[r] = mu;
+        a.rstd[r] = rs;
       }
     }
-    if (thread == 0 && a.mean != nullptr) {
-      a.mean[r] = mu;
-      a.rstd[r] = rs;
-    }
+    y += step * dim;
+    if (sum != nullptr) sum += step * dim;
   }
 }
 
-// The block's share of the parameter gradients: the groups' sums joined, in their order.
-template <int VEC, int N, int TPR, bool STAGED = false>
-__device__ __forceinline__ void leave_parts(float (&dw)[N][VEC], float (&db)[N][VEC], int dim, float* parts, float* shared) {
-  const int thread = threadIdx.x % TPR;
+// Columns that a group of threads can have.
+template <int VEC, int N, int TPR>
+constexpr int kColumns = N * VEC * TPR;
+
+// The block's share of the parameter gradients: its groups' sums, which all have every column, joined
+// in their order.
+template <int VEC, int N, int TPR>
+__device__ __forceinline__ void leave_parts(const float (&dw)[N][VEC], const float (&db)[N][VEC], int first_column, int dim,
+                                            float* parts, float* shared) {
   float* mine = parts + static_cast<int64_t>(blockIdx.x) * 2 * dim;
-  if constexpr (TPR < 32) {  // the groups of a warp
+  // shared memory [group][2][kColumns], a column's place such that neighbouring threads write neighbouring words
+  const auto place = [&](int c) { return (c % VEC) * (kColumns<VEC, N, TPR> / VEC) + c / VEC; };
+  float* of_group = shared + threadIdx.x / TPR * (2 * kColumns<VEC, N, TPR>);
 #pragma unroll
-    for (int o = 16; o >= TPR; o >>= 1)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], o);
-          db[i][j] += __shfl_xor_sync(0xffffffffu, db[i][j], o);
+    for (int j = 0; j < VEC; ++j) {
+      const int c = i * TPR * VEC + first_column + j;
+      if (c >= 0 && c < dim) {
+        if constexpr (kGroups<TPR> == 1) {
+          mine[c] = dw[i][j];
+          mine[dim + c] = db[i][j];
+        } else {
+          of_group[place(c)] = dw[i][j];
+          of_group[kColumns<VEC, N, TPR> + place(c)] = db[i][j];
         }
-  }
-  constexpr int kShare = TPR <= 32 ? kBlock<TPR> / 32 : 1;  // warps that have the same columns
-  const bool speaks = TPR >= 32 || (threadIdx.x & 31) < TPR;
-  for (int g = 0; g < kShare; ++g) {
-    if (speaks && (kShare == 1 || static_cast<int>(threadIdx.x >> 5) == g)) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int c = (i * TPR + thread) * VEC + j;
-          if (c < dim) {
-            if (kShare == 1) {
-              mine[c] = dw[i][j];
-              mine[dim + c] = db[i][j];
-            } else {
-              // an element's place: its turn, its place in the pack, its thread; neighbouring threads, neighbouring words
-              float* at = shared + ((i * VEC + j) * TPR + thread) * 2;
-              const float2 before = g == 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<float2*>(at);
-              const float2 now = make_float2(before.x + dw[i][j], before.y + db[i][j]);
-              if (g == kShare - 1) {
-                mine[c] = now.x;
-                mine[dim + c] = now.y;
-              } else {
-                *reinterpret_cast<float2*>(at) = now;
-              }
-            }
-          }
-        }
+      }
     }
-    if constexpr (kShare > 1) {
-      if constexpr (STAGED)
-        asm volatile("bar.sync 1, %0;" ::"n"(kBlock<TPR>) : "memory");
-      else
-        __syncthreads();
+  if constexpr (kGroups<TPR> > 1) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * dim; c += kBlock<TPR>) {
+      const float* at = shared + (c < dim ? place(c) : kColumns<VEC, N, TPR> + place(c - dim));
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < kGroups<TPR>; ++g) s += at[g * 2 * kColumns<VEC, N, TPR>];
+      mine[c] = s;
     }
   }
 }
 
-template <typename T, int VEC, int N, int TPR, bool SUM, bool PARAMS>
+template <typename T, int VEC, int N, int TPR, bool SHIFTED, bool SUM, bool PARAMS>
 __global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? 512 / kBlock<TPR> : 1) backward_kernel(const Backward a) {
   __shared__ float scratch[2][2][32];
-  constexpr bool kShared = PARAMS && TPR <= 32;
-  __shared__ float shared[kShared ? N * VEC * TPR * 2 : 1];
+  __shared__ float shared[PARAMS && kGroups<TPR> > 1 ? kGroups<TPR> * 2 * kColumns<VEC, N, TPR> : 1];
   const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups<TPR>;
   const T *gy = static_cast<const T*>(a.grad_y), *h = static_cast<const T*>(a.sum), *gs = static_cast<const T*>(a.grad_sum);
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups<TPR> + threadIdx.x / TPR;
+  const int first_column = thread * VEC - shift_of<T, SHIFTED>(gy, r, a.grad_y_stride);
+  const auto columns = [&](int c) { return SHIFTED ? columns_of<VEC>(c, dim) : kWhole<VEC>; };
   float w[N][VEC], dw[N][VEC] = {}, db[N][VEC] = {};
   Raw<T, VEC> next_y[N], next_h[N], next_s[SUM ? N : 1];
   float next_mean = 0.f, next_rstd = 0.f;
   const auto load = [&](int64_t r) {
     next_mean = a.mean[r];
     next_rstd = a.rstd[r];
+    const bool first = r == 0, last = r == a.rows - 1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
+      const int c = i * TPR * VEC + first_column;
       if (c < dim) {
-        next_y[i].load(gy + r * a.grad_y_stride + c);
-        next_h[i].load(h + r * a.sum_stride + c);
-        if (SUM) next_s[SUM ? i : 0].load(gs + r * a.grad_sum_stride + c);
+        load_pack<T, VEC, SHIFTED>(next_y[i], gy + r * a.grad_y_stride + c, columns(c), first, last);
+        load_pack<T, VEC, SHIFTED>(next_h[i], h + r * a.sum_stride + c, columns(c), first, last);
+        if (SUM) load_pack<T, VEC, SHIFTED>(next_s[SUM ? i : 0], gs + r * a.grad_sum_stride + c, columns(c), first, last);
       }
     }
   };
-  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups<TPR> + threadIdx.x / TPR;
   if (r < a.rows) load(r);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const int c = (i * TPR + thread) * VEC + j;
-      w[i][j] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
+      const int c = i * TPR * VEC + first_column + j;
+      w[i][j] = c >= 0 && c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
     }
   const float inv = 1.f / static_cast<float>(dim);
   int turn = 0;
@@ -286,11 +440,13 @@ __global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? 512 / kBlock
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
+      const int c = i * TPR * VEC + first_column;
       if (here && c < dim) {
         float g[VEC], n[VEC];
         y[i].floats(g);
         hh[i].floats(n);
+        clear_outside<VEC, SHIFTED>(g, columns(c));
+        clear_outside<VEC, SHIFTED>(n, columns(c));  // another row's may be infinite
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           n[j] = (n[j] - mu) * rs;
@@ -309,7 +465,7 @@ __global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? 512 / kBlock
     const float c0 = s[0] * inv, c1 = s[1] * inv;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + thread) * VEC;
+      const int c = i * TPR * VEC + first_column;
       if (c < dim) {
         float g[VEC], n[VEC], o[VEC], q[VEC];
         y[i].floats(g);
@@ -321,275 +477,18 @@ __global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? 512 / kBlock
           o[j] = fmaf(g[j], w[i][j], -fmaf(n[j], c1, c0));
           o[j] = SUM ? fmaf(rs, o[j], q[j]) : rs * o[j];
         }
-        Raw<T, VEC>::store(static_cast<T*>(a.grad_x) + r * dim + c, o);
+        store_pack<T, VEC, SHIFTED>(static_cast<T*>(a.grad_x) + r * dim + c, columns(c), o);
         if (a.grad_delta != nullptr) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) o[j] *= a.scale;
-          Raw<T, VEC>::store(static_cast<T*>(a.grad_delta) + r * dim + c, o);
+          store_pack<T, VEC, SHIFTED>(static_cast<T*>(a.grad_delta) + r * dim + c, columns(c), o);
         }
       }
     }
   }
   if constexpr (PARAMS) {
     grid_dependency_launch();
-    leave_parts<VEC, N, TPR>(dw, db, dim, a.parts, shared);
-  }
-}
-
-// ---------------------------------------------------------------- rows off 16-byte boundaries
-constexpr int kMaxFeeds = 5;
-constexpr int kMaxStages = 8;
-constexpr int kMaxTileRows = 128;
-
-// An input as the loading warp sees it: rows of bytes, `stride` apart. Rows without a gap are copied
-// as one piece, others one by one, each to a place `pitch` after the one before.
-struct Feed {
-  const char* p;
-  int64_t stride;
-  int row_bytes;
-  uint32_t offset;  // in a stage
-  int pitch;        // 0: one piece
-};
-
-struct Plan {
-  Feed feed[kMaxFeeds];
-  int feeds, tile_rows, stages;
-  uint32_t stage_bytes;
-};
-
-// Where row `i` of the tile that begins at row r0 lies in a stage.
-__device__ __forceinline__ const char* staged(const Feed& f, const unsigned char* stage, int64_t r0, int i) {
-  const uint32_t first = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(f.p) + r0 * f.stride) & 15u;
-  const uint32_t at = f.pitch == 0 ? first + i * f.row_bytes
-                                   : i * f.pitch + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(f.p) + (r0 + i) * f.stride) & 15u);
-  return reinterpret_cast<const char*>(stage) + f.offset + at;
-}
-
-// Bytes [from, to) of an input into shared memory at `dst` (which stands for the 16-byte block that
-// `from` lies in). Whole blocks by one bulk copy; where the first or the last block reaches outside
-// the input, its bytes one element's half or whole at a time, before the copies are announced.
-// Returns the bytes of the bulk copy.
-__device__ __forceinline__ uint32_t copy_piece(const Feed& f, int64_t rows, const char* from, const char* to, unsigned char* dst,
-                                               bool issue, uint64_t* bar) {
-  const uintptr_t begin = reinterpret_cast<uintptr_t>(from), end = reinterpret_cast<uintptr_t>(to);
-  const uintptr_t low = begin & ~uintptr_t(15);
-  uintptr_t a = low, b = (end + 15) & ~uintptr_t(15);
-  if (a < reinterpret_cast<uintptr_t>(f.p)) a += 16;
-  if (b > reinterpret_cast<uintptr_t>(f.p) + (rows - 1) * f.stride + f.row_bytes) b -= 16;
-  if (b < a) b = a;  // nothing but ends
-  if (!issue) {
-    const uintptr_t head = a < end ? a : end, tail = b > head ? b : head;
-    for (uintptr_t p = begin; p < head; p += 2) *reinterpret_cast<uint16_t*>(dst + (p - low)) = *reinterpret_cast<const uint16_t*>(p);
-    for (uintptr_t p = tail; p < end; p += 2) *reinterpret_cast<uint16_t*>(dst + (p - low)) = *reinterpret_cast<const uint16_t*>(p);
-  } else if (b > a) {
-    bulk_load(dst + (a - low), reinterpret_cast<const void*>(a), static_cast<uint32_t>(b - a), bar);
-  }
-  return static_cast<uint32_t>(b - a);
-}
-
-struct Ring {
-  uint64_t full[kMaxStages], empty[kMaxStages];
-};
-
-__device__ __forceinline__ void ring_init(Ring& ring, int stages, int workers) {
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < stages; ++i) {
-      mbar_init(&ring.full[i], 1);
-      mbar_init(&ring.empty[i], workers / 32);
-    }
-    fence_barrier_init();
-  }
-  __syncthreads();
-}
-
-// The loading warp: tiles block, block + grid, ... A wait that runs out is recorded, and no later one
-// is waited for: the kernel then ends soon, with an error that jk_device_status reports.
-__device__ __forceinline__ void load_tiles(const Plan& plan, Ring& ring, unsigned char* memory, int64_t rows) {
-  const int lane = threadIdx.x & 31;
-  bool good = true;
-  int stage = 0;
-  uint32_t turn = 0;
-  const int64_t tiles = (rows + plan.tile_rows - 1) / plan.tile_rows;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    if (turn > 0 && good) good = mbar_wait(&ring.empty[stage], (turn - 1) & 1);
-    const int64_t r0 = tile * plan.tile_rows;
-    const int n = static_cast<int>(rows - r0 < plan.tile_rows ? rows - r0 : plan.tile_rows);
-    unsigned char* base = memory + static_cast<size_t>(stage) * plan.stage_bytes;
-    uint32_t bytes = 0;
-    for (int issue = 0; issue < 2; ++issue) {
-      for (int k = 0; k < plan.feeds; ++k) {
-        const Feed& f = plan.feed[k];
-        if (f.pitch == 0) {
-          if (lane == k) {
-            const char* from = f.p + r0 * f.stride;
-            bytes += copy_piece(f, rows, from, from + static_cast<int64_t>(n) * f.row_bytes, base + f.offset, issue != 0, &ring.full[stage]);
-          }
-        } else {
-          for (int i = lane; i < n; i += 32) {
-            const char* from = f.p + (r0 + i) * f.stride;
-            bytes += copy_piece(f, rows, from, from + f.row_bytes, base + f.offset + i * f.pitch, issue != 0, &ring.full[stage]);
-          }
-        }
-      }
-      if (issue == 0) {
-        bytes = __reduce_add_sync(0xffffffffu, bytes);
-        if (lane == 0) mbar_arrive_expect_tx(&ring.full[stage], bytes);
-        __syncwarp();
-      }
-    }
-    if (++stage == plan.stages) stage = 0, ++turn;
-  }
-  // copies in flight land before the block's memory is given back
-  for (int i = 0; i < plan.stages; ++i) {
-    const uint32_t loads = turn + (i < stage ? 1 : 0);
-    if (loads > 0 && good) good = mbar_wait(&ring.full[i], (loads - 1) & 1);
-  }
-  if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
-}
-
-// `take(i, r, stage)` for the tiles' rows that this thread's group has: i in the tile, r in all.
-template <int TPR, typename F>
-__device__ __forceinline__ void take_tiles(const Plan& plan, Ring& ring, const unsigned char* memory, int64_t rows, F&& take) {
-  bool good = true;
-  int stage = 0;
-  uint32_t turn = 0;
-  const int64_t tiles = (rows + plan.tile_rows - 1) / plan.tile_rows;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    if (good) good = mbar_wait(&ring.full[stage], turn & 1);
-    const int64_t r0 = tile * plan.tile_rows;
-    const int n = static_cast<int>(rows - r0 < plan.tile_rows ? rows - r0 : plan.tile_rows);
-    const unsigned char* base = memory + static_cast<size_t>(stage) * plan.stage_bytes;
-    for (int i = threadIdx.x / TPR; i < n; i += kGroups<TPR>) take(i, r0, base);
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[stage]);
-    if (++stage == plan.stages) stage = 0, ++turn;
-  }
-  if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
-}
-
-template <typename T, int N, int TPR, bool DELTA>
-__global__ void __launch_bounds__(kBlock<TPR> + 32) staged_forward_kernel(const Forward a, const __grid_constant__ Plan plan) {
-  extern __shared__ __align__(128) unsigned char memory[];
-  __shared__ Ring ring;
-  __shared__ float scratch[2][1][32];
-  ring_init(ring, plan.stages, kBlock<TPR>);
-  if (threadIdx.x >= kBlock<TPR>) {
-    load_tiles(plan, ring, memory, a.rows);
-    return;
-  }
-  const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
-  float w[N], b[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = i * TPR + thread;
-    w[i] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
-    b[i] = c < dim ? param_at(a.bias, c, a.param_type, 0.f) : 0.f;
-  }
-  const float inv = 1.f / static_cast<float>(dim);
-  take_tiles<TPR>(plan, ring, memory, a.rows, [&](int row, int64_t r0, const unsigned char* stage) {
-    const T* x = reinterpret_cast<const T*>(staged(plan.feed[0], stage, r0, row));
-    const T* d = DELTA ? reinterpret_cast<const T*>(staged(plan.feed[1], stage, r0, row)) : nullptr;
-    float f[N], s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * TPR + thread;
-      f[i] = 0.f;
-      if (c < dim) {
-        f[i] = to_f32(x[c]);
-        if (DELTA) f[i] = fmaf(a.scale, to_f32(d[c]), f[i]);
-      }
-      s[0] += f[i];
-    }
-    row_sums<TPR, 1, true>(s, scratch, 0);
-    const float mu = s[0] * inv;
-    s[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float v = i * TPR + thread < dim ? f[i] - mu : 0.f;
-      s[0] = fmaf(v, v, s[0]);
-    }
-    row_sums<TPR, 1, true>(s, scratch, 1);
-    const float rs = rsqrtf(fmaf(s[0], inv, a.eps));
-    const int64_t r = r0 + row;
-    T *y = static_cast<T*>(a.y) + r * dim, *sum = a.sum == nullptr ? nullptr : static_cast<T*>(a.sum) + r * dim;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * TPR + thread;
-      if (c < dim) {
-        y[c] = from_f32<T>(fmaf((f[i] - mu) * rs, w[i], b[i]));
-        if (sum != nullptr) sum[c] = from_f32<T>(f[i]);
-      }
-    }
-    if (thread == 0 && a.mean != nullptr) {
-      a.mean[r] = mu;
-      a.rstd[r] = rs;
-    }
-  });
-}
-
-template <typename T, int N, int TPR, bool SUM, bool PARAMS>
-__global__ void __launch_bounds__(kBlock<TPR> + 32) staged_backward_kernel(const Backward a, const __grid_constant__ Plan plan) {
-  extern __shared__ __align__(128) unsigned char memory[];
-  __shared__ Ring ring;
-  __shared__ float scratch[2][2][32];
-  constexpr bool kShared = PARAMS && TPR <= 32;
-  __shared__ float shared[kShared ? N * TPR * 2 : 1];
-  ring_init(ring, plan.stages, kBlock<TPR>);
-  if (threadIdx.x >= kBlock<TPR>) {
-    load_tiles(plan, ring, memory, a.rows);
-    return;
-  }
-  const int dim = static_cast<int>(a.dim), thread = threadIdx.x % TPR;
-  float w[N], dw[N][1] = {}, db[N][1] = {};
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = i * TPR + thread;
-    w[i] = c < dim ? param_at(a.weight, c, a.param_type, 1.f) : 0.f;
-  }
-  const float inv = 1.f / static_cast<float>(dim);
-  int turn = 0;
-  take_tiles<TPR>(plan, ring, memory, a.rows, [&](int row, int64_t r0, const unsigned char* stage) {
-    const float mu = *reinterpret_cast<const float*>(staged(plan.feed[0], stage, r0, row));
-    const float rs = *reinterpret_cast<const float*>(staged(plan.feed[1], stage, r0, row));
-    const T* gy = reinterpret_cast<const T*>(staged(plan.feed[2], stage, r0, row));
-    const T* h = reinterpret_cast<const T*>(staged(plan.feed[3], stage, r0, row));
-    float g[N], n[N], s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * TPR + thread;
-      g[i] = n[i] = 0.f;
-      if (c < dim) {
-        g[i] = to_f32(gy[c]);
-        n[i] = (to_f32(h[c]) - mu) * rs;
-      }
-      if (PARAMS) {
-        dw[i][0] = fmaf(g[i], n[i], dw[i][0]);
-        db[i][0] += g[i];
-      }
-      const float u = g[i] * w[i];
-      s[0] += u;
-      s[1] = fmaf(u, n[i], s[1]);
-    }
-    row_sums<TPR, 2, true>(s, scratch, turn);
-    turn ^= 1;
-    const float c0 = s[0] * inv, c1 = s[1] * inv;
-    const T* gs = SUM ? reinterpret_cast<const T*>(staged(plan.feed[4], stage, r0, row)) : nullptr;
-    const int64_t r = r0 + row;
-    T *gx = static_cast<T*>(a.grad_x) + r * dim, *gd = a.grad_delta == nullptr ? nullptr : static_cast<T*>(a.grad_delta) + r * dim;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * TPR + thread;
-      if (c < dim) {
-        float o = fmaf(g[i], w[i], -fmaf(n[i], c1, c0));
-        o = SUM ? fmaf(rs, o, to_f32(gs[c])) : rs * o;
-        gx[c] = from_f32<T>(o);
-        if (gd != nullptr) gd[c] = from_f32<T>(a.scale * o);
-      }
-    }
-  });
-  if constexpr (PARAMS) {
-    grid_dependency_launch();
-    leave_parts<1, N, TPR, true>(dw, db, dim, a.parts, shared);
+    leave_parts<VEC, N, TPR>(dw, db, first_column, dim, a.parts, shared);
   }
 }
 
@@ -705,139 +604,63 @@ int blocks_per_sm(int threads) {
   return per_sm;
 }
 
-template <auto KERNEL, int TPR>
+// Rows of one group are `step` apart; with SHIFTED they have to begin alike against 16-byte blocks, so
+// the step is a multiple of what a block has elements, or a group has one row only.
+template <int VEC, int TPR, bool SHIFTED>
+int64_t blocks_of(int64_t rows, int64_t most) {
+  const int64_t blocks = groups_to_blocks(rows, kGroups<TPR>, most);
+  if (!SHIFTED || blocks * kGroups<TPR> >= rows) return blocks;
+  constexpr int64_t kUnit = kGroups<TPR> % VEC == 0 ? 1 : VEC / kGroups<TPR>;  // groups: 1, or 8 and more
+  return blocks / kUnit * kUnit;
+}
+
+template <auto KERNEL, int VEC, int TPR, bool SHIFTED>
 int run_forward(const Forward& a, cudaStream_t s) {
-  const int64_t blocks = groups_to_blocks(a.rows, kGroups<TPR>, 148ll * blocks_per_sm<KERNEL>(kBlock<TPR>));
+  const int64_t blocks = blocks_of<VEC, TPR, SHIFTED>(a.rows, 148ll * blocks_per_sm<KERNEL>(kBlock<TPR>));
   KERNEL<<<static_cast<unsigned>(blocks), kBlock<TPR>, 0, s>>>(a);
   return 0;
 }
 
-template <typename T, int VEC, int N, int TPR>
+template <typename T, int VEC, bool SHIFTED, int N, int TPR>
 int pick_forward(const Forward& a, cudaStream_t s) {
-  return a.delta != nullptr ? run_forward<forward_kernel<T, VEC, N, TPR, true>, TPR>(a, s)
-                            : run_forward<forward_kernel<T, VEC, N, TPR, false>, TPR>(a, s);
+  return a.delta != nullptr ? run_forward<forward_kernel<T, VEC, N, TPR, SHIFTED, true>, VEC, TPR, SHIFTED>(a, s)
+                            : run_forward<forward_kernel<T, VEC, N, TPR, SHIFTED, false>, VEC, TPR, SHIFTED>(a, s);
 }
 
-template <auto KERNEL, int TPR>
+template <auto KERNEL, int VEC, int TPR, bool SHIFTED>
 int run_backward(const Backward& a, cudaStream_t s) {
   int64_t most = 148ll * blocks_per_sm<KERNEL>(kBlock<TPR>);
-  if (a.parts != nullptr && most > kMaxParts) most = kMaxParts;
-  const int blocks = static_cast<int>(groups_to_blocks(a.rows, kGroups<TPR>, most));
+  const int64_t parts = kBlock<TPR> <= 128 ? kMaxParts : kBlock<TPR> <= 256 ? kMaxParts / 4 * 3 : kMaxParts / 2;
+  if (a.parts != nullptr && most > parts) most = parts;
+  const int blocks = static_cast<int>(blocks_of<VEC, TPR, SHIFTED>(a.rows, most));
   KERNEL<<<blocks, kBlock<TPR>, 0, s>>>(a);
   return blocks;
 }
 
-template <typename T, int VEC, int N, int TPR>
+template <typename T, int VEC, bool SHIFTED, int N, int TPR>
 int pick_backward(const Backward& a, cudaStream_t s) {
   if (a.grad_sum != nullptr)
-    return a.parts != nullptr ? run_backward<backward_kernel<T, VEC, N, TPR, true, true>, TPR>(a, s)
-                              : run_backward<backward_kernel<T, VEC, N, TPR, true, false>, TPR>(a, s);
-  return a.parts != nullptr ? run_backward<backward_kernel<T, VEC, N, TPR, false, true>, TPR>(a, s)
-                            : run_backward<backward_kernel<T, VEC, N, TPR, false, false>, TPR>(a, s);
+    return a.parts != nullptr ? run_backward<backward_kernel<T, VEC, N, TPR, SHIFTED, true, true>, VEC, TPR, SHIFTED>(a, s)
+                              : run_backward<backward_kernel<T, VEC, N, TPR, SHIFTED, true, false>, VEC, TPR, SHIFTED>(a, s);
+  return a.parts != nullptr ? run_backward<backward_kernel<T, VEC, N, TPR, SHIFTED, false, true>, VEC, TPR, SHIFTED>(a, s)
+                            : run_backward<backward_kernel<T, VEC, N, TPR, SHIFTED, false, false>, VEC, TPR, SHIFTED>(a, s);
 }
 
-constexpr int kNoRoom = -1000;  // no status
-
-// A plan for rows off boundaries: tiles of some 8 KB, as many in flight as fill an SM's shared memory
-// with the blocks that it holds. False if two tiles of one row do not fit.
-struct Tiles {
-  int blocks_per_sm;
-  size_t smem;
-};
-inline bool plan_tiles(Plan& plan, int64_t rows, int groups, int want_blocks, Tiles& tiles) {
-  int64_t row = 0;
-  for (int k = 0; k < plan.feeds; ++k) row += plan.feed[k].row_bytes;
-  int64_t tile_rows = groups;
-  while (tile_rows * 2 <= kMaxTileRows && tile_rows * 2 * row <= 8192) tile_rows *= 2;
-  const int64_t least = (rows + 148 * want_blocks - 1) / (148 * want_blocks);  // rows of a block
-  while (tile_rows > groups && tile_rows > least) tile_rows /= 2;
-  plan.tile_rows = static_cast<int>(tile_rows);
-  uint32_t at = 0;
-  for (int k = 0; k < plan.feeds; ++k) {
-    Feed& f = plan.feed[k];
-    f.offset = at;
-    f.pitch = f.stride == f.row_bytes ? 0 : (f.row_bytes + 15 + 15) / 16 * 16;
-    at += f.pitch == 0 ? static_cast<uint32_t>((tile_rows * f.row_bytes + 15 + 15) / 16 * 16) : static_cast<uint32_t>(tile_rows * f.pitch);
-  }
-  plan.stage_bytes = at;
-  constexpr int64_t kRoom = 200 * 1024;
-  int blocks = want_blocks;
-  while (blocks > 1 && kRoom / blocks < 3 * static_cast<int64_t>(at)) --blocks;
-  const int64_t fit = kRoom / blocks / at;
-  if (fit < 2) return false;
-  plan.stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
-  tiles = {blocks, static_cast<size_t>(plan.stages) * at};
-  return true;
-}
-
-template <typename T>
-Feed feed_of(const void* p, int64_t stride, int64_t dim) {
-  return {static_cast<const char*>(p), stride * static_cast<int64_t>(sizeof(T)), static_cast<int>(dim * sizeof(T)), 0, 0};
-}
-
-template <auto KERNEL>
-bool allow(size_t smem) {
-  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess) return true;
-  cudaGetLastError();
-  return false;
-}
-
-template <auto KERNEL, typename T, int TPR>
-int run_staged_forward(const Forward& a, cudaStream_t s) {
-  Plan plan = {};
-  plan.feed[plan.feeds++] = feed_of<T>(a.x, a.x_stride, a.dim);
-  if (a.delta != nullptr) plan.feed[plan.feeds++] = feed_of<T>(a.delta, a.delta_stride, a.dim);
-  Tiles tiles;
-  if (!plan_tiles(plan, a.rows, kGroups<TPR>, blocks_per_sm<KERNEL>(kBlock<TPR> + 32), tiles)) return kNoRoom;
-  if (!allow<KERNEL>(tiles.smem)) return JK_ERR_LAUNCH;
-  const int64_t blocks = groups_to_blocks(a.rows, plan.tile_rows, 148ll * tiles.blocks_per_sm);
-  KERNEL<<<static_cast<unsigned>(blocks), kBlock<TPR> + 32, tiles.smem, s>>>(a, plan);
-  return 0;
-}
-
-template <auto KERNEL, typename T, int TPR>
-int run_staged_backward(const Backward& a, cudaStream_t s) {
-  Plan plan = {};
-  plan.feed[plan.feeds++] = feed_of<float>(a.mean, 1, 1);
-  plan.feed[plan.feeds++] = feed_of<float>(a.rstd, 1, 1);
-  plan.feed[plan.feeds++] = feed_of<T>(a.grad_y, a.grad_y_stride, a.dim);
-  plan.feed[plan.feeds++] = feed_of<T>(a.sum, a.sum_stride, a.dim);
-  if (a.grad_sum != nullptr) plan.feed[plan.feeds++] = feed_of<T>(a.grad_sum, a.grad_sum_stride, a.dim);
-  Tiles tiles;
-  if (!plan_tiles(plan, a.rows, kGroups<TPR>, blocks_per_sm<KERNEL>(kBlock<TPR> + 32), tiles)) return kNoRoom;
-  if (!allow<KERNEL>(tiles.smem)) return JK_ERR_LAUNCH;
-  int64_t most = 148ll * tiles.blocks_per_sm;
-  if (a.parts != nullptr && most > kMaxParts) most = kMaxParts;
-  const int blocks = static_cast<int>(groups_to_blocks(a.rows, plan.tile_rows, most));
-  KERNEL<<<blocks, kBlock<TPR> + 32, tiles.smem, s>>>(a, plan);
-  return blocks;
-}
-
-template <typename T, int N, int TPR>
-int pick_staged_forward(const Forward& a, cudaStream_t s) {
-  return a.delta != nullptr ? run_staged_forward<staged_forward_kernel<T, N, TPR, true>, T, TPR>(a, s)
-                            : run_staged_forward<staged_forward_kernel<T, N, TPR, false>, T, TPR>(a, s);
-}
-
-template <typename T, int N, int TPR>
-int pick_staged_backward(const Backward& a, cudaStream_t s) {
-  if (a.grad_sum != nullptr)
-    return a.parts != nullptr ? run_staged_backward<staged_backward_kernel<T, N, TPR, true, true>, T, TPR>(a, s)
-                              : run_staged_backward<staged_backward_kernel<T, N, TPR, true, false>, T, TPR>(a, s);
-  return a.parts != nullptr ? run_staged_backward<staged_backward_kernel<T, N, TPR, false, true>, T, TPR>(a, s)
-                            : run_staged_backward<staged_backward_kernel<T, N, TPR, false, false>, T, TPR>(a, s);
-}
-
-// The threads of a row and their turns: as few threads as hold it with 16 elements each (fewer where
-// a warp has room), a warp's or less while that does, so that no barrier is needed.
+// The threads of a row and their turns: a warp or less as long as 16 elements a thread do, so that no
+// barrier is needed; beyond, 8 to 16 elements of a 16-byte pack or two each, which leaves an SM 512
+// threads or more (f32 2047 wide, backward: 74 us with two packs, 111 with four; f16 5001 wide: 35 us
+// with one pack of 640 threads, 41 with two of 512).
 #define JK_NORM_SHAPES(RUN)                                             \
   if constexpr (VEC == 8) {                                             \
     if (turns <= 8) return RUN(1, 8);                                   \
     if (turns <= 16) return RUN(1, 16);                                 \
     if (turns <= 32) return RUN(1, 32);                                 \
     if (turns <= 64) return RUN(2, 32);                                 \
+    if (turns <= 128) return RUN(1, 128);                               \
     if (turns <= 256) return RUN(2, 128);                               \
     if (turns <= 512) return RUN(2, 256);                               \
+    if (turns <= 640) return RUN(1, 640);                               \
+    if (turns <= 768) return RUN(2, 384);                               \
     if (turns <= 1024) return RUN(2, 512);                              \
     return RUN(2, 1024);                                                \
   } else if constexpr (VEC == 4) {                                      \
@@ -846,95 +669,74 @@ int pick_staged_backward(const Backward& a, cudaStream_t s) {
     if (turns <= 32) return RUN(1, 32);                                 \
     if (turns <= 64) return RUN(2, 32);                                 \
     if (turns <= 128) return RUN(4, 32);                                \
-    if (turns <= 512) return RUN(4, 128);                               \
-    if (turns <= 1024) return RUN(4, 256);                              \
-    if (turns <= 2048) return RUN(4, 512);                              \
+    if (turns <= 256) return RUN(2, 128);                               \
+    if (turns <= 512) return RUN(2, 256);                               \
+    if (turns <= 768) return RUN(2, 384);                               \
+    if (turns <= 1024) return RUN(2, 512);                              \
+    if (turns <= 1536) return RUN(2, 768);                              \
+    if (turns <= 2048) return RUN(2, 1024);                             \
     return RUN(4, 1024);                                                \
   } else {                                                              \
-    if (turns <= 32) return RUN(1, 32);                                 \
-    if (turns <= 64) return RUN(2, 32);                                 \
     if (turns <= 128) return RUN(4, 32);                                \
-    if (turns <= 256) return RUN(8, 32);                                \
     if (turns <= 512) return RUN(16, 32);                               \
-    if (turns <= 1024) return RUN(8, 128);                              \
-    if (turns <= 2048) return RUN(8, 256);                              \
-    if (turns <= 4096) return RUN(8, 512);                              \
-    return RUN(16, 512);                                                \
+    if (turns <= 2048) return RUN(16, 128);                             \
+    if (turns <= 4096) return RUN(16, 256);                             \
+    if (turns <= 8192) return RUN(16, 512);                             \
+    return RUN(16, 1024);                                               \
   }
 
-constexpr int64_t kMaxDim = 16384, kMaxStagedDim = 8192;  // of the rows that stay in registers
+constexpr int64_t kMaxDim = 16384 - 8;  // of the rows that stay in registers, wherever they begin
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHIFTED>
 int shape_forward(const Forward& a, cudaStream_t s) {
-  const int64_t turns = a.dim / VEC;
-#define JK_RUN(N, TPR) pick_forward<T, VEC, N, TPR>(a, s)
+  const int64_t turns = (a.dim + (SHIFTED ? 2 : 1) * (VEC - 1)) / VEC;
+#define JK_RUN(N, TPR) pick_forward<T, VEC, SHIFTED, N, TPR>(a, s)
   JK_NORM_SHAPES(JK_RUN)
 #undef JK_RUN
 }
 
-template <typename T>
-int shape_staged_forward(const Forward& a, cudaStream_t s) {
-  constexpr int VEC = 1;
-  const int64_t turns = a.dim;
-#define JK_RUN(N, TPR) pick_staged_forward<T, N, TPR>(a, s)
-  JK_NORM_SHAPES(JK_RUN)
-#undef JK_RUN
-}
-
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHIFTED>
 int shape_backward(const Backward& a, cudaStream_t s) {
-  const int64_t turns = a.dim / VEC;
-#define JK_RUN(N, TPR) pick_backward<T, VEC, N, TPR>(a, s)
+  const int64_t turns = (a.dim + (SHIFTED ? 2 : 1) * (VEC - 1)) / VEC;
+#define JK_RUN(N, TPR) pick_backward<T, VEC, SHIFTED, N, TPR>(a, s)
   JK_NORM_SHAPES(JK_RUN)
 #undef JK_RUN
 }
 
+// Whether a tensor's rows begin where those of a contiguous one on a 16-byte boundary do.
 template <typename T>
-int shape_staged_backward(const Backward& a, cudaStream_t s) {
-  constexpr int VEC = 1;
-  const int64_t turns = a.dim;
-#define JK_RUN(N, TPR) pick_staged_backward<T, N, TPR>(a, s)
-  JK_NORM_SHAPES(JK_RUN)
-#undef JK_RUN
+bool lies_plain(const void* p, int64_t stride, int64_t dim) {
+  return p == nullptr || (aligned16(p) && (stride - dim) % kPack<T> == 0);
 }
 
 template <typename T>
-bool in_packs(const void* p, int64_t stride) {
-  return p == nullptr || (aligned16(p) && stride % kPack<T> == 0);
-}
-
-template <typename T>
-int forward(const Forward& a, cudaStream_t s) {
-  if (a.dim <= kMaxDim && in_packs<T>(a.x, a.x_stride) && in_packs<T>(a.delta, a.delta_stride) && in_packs<T>(a.y, a.dim) &&
-      in_packs<T>(a.sum, a.dim))
-    return shape_forward<T, kPack<T>>(a, s);
-  if (a.dim <= kMaxStagedDim) {
-    const int done = shape_staged_forward<T>(a, s);
-    if (done != kNoRoom) return done;
+void forward(const Forward& a, cudaStream_t s) {
+  if (a.dim > kMaxDim) {
+    long_forward_kernel<T><<<static_cast<unsigned>(a.rows < 148 * 4 ? a.rows : 148 * 4), kLongThreads, 0, s>>>(a);
+  } else if (lies_plain<T>(a.x, a.x_stride, a.dim) && lies_plain<T>(a.delta, a.delta_stride, a.dim) && aligned16(a.y) &&
+             aligned16(a.sum)) {
+    if (a.dim % kPack<T> == 0) shape_forward<T, kPack<T>, false>(a, s);
+    else shape_forward<T, kPack<T>, true>(a, s);
+  } else {
+    shape_forward<T, 1, false>(a, s);
   }
-  long_forward_kernel<T><<<static_cast<unsigned>(a.rows < 148 * 4 ? a.rows : 148 * 4), kLongThreads, 0, s>>>(a);
-  return 0;
 }
 
-// Returns the blocks that left a share of the parameter gradients, or a status.
+// Returns the blocks that left a share of the parameter gradients.
 template <typename T>
 int backward(const Backward& a, cudaStream_t s) {
-  if (a.dim <= kMaxDim && in_packs<T>(a.grad_y, a.grad_y_stride) && in_packs<T>(a.sum, a.sum_stride) &&
-      in_packs<T>(a.grad_sum, a.grad_sum_stride) && in_packs<T>(a.grad_x, a.dim) && in_packs<T>(a.grad_delta, a.dim))
-    return shape_backward<T, kPack<T>>(a, s);
-  if (a.dim <= kMaxStagedDim) {
-    const int done = shape_staged_backward<T>(a, s);
-    if (done != kNoRoom) return done;
+  if (a.dim > kMaxDim) {
+    const int blocks = static_cast<int>(a.rows < kMaxParts ? a.rows : kMaxParts);
+    long_backward_kernel<T><<<blocks, kLongThreads, 0, s>>>(a);
+    return blocks;
   }
-  const int blocks = static_cast<int>(a.rows < kMaxParts ? a.rows : kMaxParts);
-  long_backward_kernel<T><<<blocks, kLongThreads, 0, s>>>(a);
-  return blocks;
+  if (lies_plain<T>(a.grad_y, a.grad_y_stride, a.dim) && lies_plain<T>(a.sum, a.sum_stride, a.dim) &&
+      lies_plain<T>(a.grad_sum, a.grad_sum_stride, a.dim) && aligned16(a.grad_x) && aligned16(a.grad_delta))
+    return a.dim % kPack<T> == 0 ? shape_backward<T, kPack<T>, false>(a, s) : shape_backward<T, kPack<T>, true>(a, s);
+  return shape_backward<T, 1, false>(a, s);
 }
 
 }  // namespace norm
-
-JK_ERROR_READER(read_error_norm)
-
 }  // namespace jk
 
 extern "C" int jk_layer_norm_forward(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride,
@@ -950,8 +752,8 @@ extern "C" int jk_layer_norm_forward(const void* x, int64_t x_stride, const void
   if (st != JK_OK) return st;
   const norm::Forward a{x, delta, x_stride, delta_stride, delta_scale, weight, bias, param_dtype,
                         rows, dim, eps, y, sum, mean, rstd};
-  JK_WITH_TYPE(dtype, T, st = norm::forward<T>(a, reinterpret_cast<cudaStream_t>(stream)));
-  return st < 0 ? st : launch_status();
+  JK_WITH_TYPE(dtype, T, norm::forward<T>(a, reinterpret_cast<cudaStream_t>(stream)));
+  return launch_status();
 }
 
 extern "C" int64_t jk_layer_norm_backward_workspace(int64_t rows, int64_t dim) {
@@ -979,7 +781,6 @@ extern "C" int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride,
                          delta_scale, rows, dim, grad_x, grad_delta, params ? workspace : nullptr};
   int parts = 0;
   if (rows > 0) JK_WITH_TYPE(dtype, T, parts = norm::backward<T>(a, s));
-  if (parts < 0) return parts;
   if (params)
     JK_WITH_TYPE(param_dtype, W, launch_dependent(norm::parameters_kernel<W>, static_cast<unsigned>((2 * dim + 31) / 32), 1024, 0, s,
                                                   workspace, parts, dim, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias)));
