@@ -51,24 +51,24 @@ def _check_input(name: str, t: Tensor) -> int:
     """The dtype code of a CUDA float tensor; anything else raises."""
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor in the b200_sm100a backend (got {t.device}).")
     code = _DTYPE_CODE.get(t.dtype)
-    if code is None:
+    if code is None or not t.is_cuda:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor in the b200_sm100a backend (got {t.device}).")
         raise RuntimeError(f"{name}: unsupported dtype {t.dtype}")
     return code
 
 
-def _same(name: str, t: Tensor, like: Tensor, shape=None) -> None:
-    """t has like's device and dtype and the given shape (like's by default)."""
+def _same(name: str, t: Tensor, like: Tensor) -> None:
+    """t has like's device, dtype and shape."""
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
     if t.dtype != like.dtype:
         raise RuntimeError(f"{name} has dtype {t.dtype}, expected {like.dtype}")
-    if t.shape != (like.shape if shape is None else shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape if shape is None else shape)}")
+    if t.shape != like.shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
@@ -105,15 +105,14 @@ def _call(fn, where: str, device: int, *args) -> None:
         check(status, where)
 
 
-def _param(name: str, p: Optional[Tensor], x: Tensor, dim: int) -> Optional[Tensor]:
-    if p is None:
-        return None
-    _check_input(name, p)
-    if p.device != x.device:
-        raise RuntimeError(f"{name} is on {p.device}, expected {x.device}")
-    if p.shape != (dim,):
+def _param(name: str, p: Tensor, device: int, dim: int) -> tuple[Tensor, int]:
+    """(a contiguous [dim] parameter on the device, its dtype code)"""
+    code = _check_input(name, p)
+    if p.get_device() != device:
+        raise RuntimeError(f"{name} is on {p.device}, expected cuda:{device}")
+    if p.dim() != 1 or p.numel() != dim:
         raise ValueError(f"{name} has shape {tuple(p.shape)}, expected {(dim,)}")
-    return p if p.is_contiguous() else p.detach().contiguous()
+    return (p if p.is_contiguous() else p.detach().contiguous()), code
 
 
 def _empty_like(t: Tensor) -> Tensor:
@@ -140,22 +139,30 @@ def layer_norm_forward_cuda(x: Tensor, weight: Optional[Tensor] = None, bias: Op
     dim = x.shape[-1]
     if dim == 0:
         raise ValueError("the normalised dim is empty")
-    weight, bias = _param("weight", weight, x, dim), _param("bias", bias, x, dim)
-    some = weight if weight is not None else bias
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError(f"weight and bias have different dtypes ({weight.dtype}, {bias.dtype})")
+    device, pcode = x.get_device(), code
+    weight_at = bias_at = delta_at = sum_at = None
+    if weight is not None:
+        weight, pcode = _param("weight", weight, device, dim)
+        weight_at = weight.data_ptr()
+    if bias is not None:
+        bias, bcode = _param("bias", bias, device, dim)
+        bias_at = bias.data_ptr()
+        if weight is not None and bcode != pcode:
+            raise RuntimeError(f"weight and bias have different dtypes ({weight.dtype}, {bias.dtype})")
+        pcode = bcode
     xr, x_stride = _rows(x)
-    dr, d_stride = None, 0
+    y = _empty_like(x)
+    total, d_stride = x, 0
     if delta is not None:
         _same("delta", delta, x)
         dr, d_stride = _rows(delta)
-    y = _empty_like(x)
-    total = x if delta is None else torch.empty_like(y)
+        total = torch.empty_like(y)
+        delta_at, sum_at = dr.data_ptr(), total.data_ptr()
     mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    _call(_LIBRARY.jk_layer_norm_forward, "jk_layer_norm_forward", x.get_device(), xr.data_ptr(), x_stride, _ptr(dr), d_stride,
-          delta_scale, _ptr(weight), _ptr(bias), code if some is None else _DTYPE_CODE[some.dtype], mean.numel(), dim, code,
-          eps, y.data_ptr(), None if delta is None else total.data_ptr(), mean.data_ptr(), rstd.data_ptr())
+    _call(_LIBRARY.jk_layer_norm_forward, "jk_layer_norm_forward", device, xr.data_ptr(), x_stride, delta_at, d_stride,
+          delta_scale, weight_at, bias_at, pcode, mean.numel(), dim, code, eps, y.data_ptr(), sum_at, mean.data_ptr(),
+          rstd.data_ptr())
     return y, total, mean, rstd
 
 
@@ -172,32 +179,39 @@ def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Te
         raise ValueError("sum must have a last dim that is not empty")
     dim = sum.shape[-1]
     _same("grad_y", grad_y, sum)
-    weight = _param("weight", weight, sum, dim)
+    device, pcode = sum.get_device(), code
+    weight_at = gs_at = gd_at = gw_at = gb_at = work_at = None
+    if weight is not None:
+        weight, pcode = _param("weight", weight, device, dim)
+        weight_at = weight.data_ptr()
+    lead = sum.shape[:-1]
     for name, t in (("mean", mean), ("rstd", rstd)):
-        if not isinstance(t, Tensor) or t.dtype != torch.float32 or t.device != sum.device:
+        if not isinstance(t, Tensor) or t.dtype != torch.float32 or t.get_device() != device:
             raise RuntimeError(f"{name} must be an f32 tensor on {sum.device}")
-        if t.shape != sum.shape[:-1]:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(sum.shape[:-1])}")
+        if t.shape != lead:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(lead)}")
     mean, rstd = mean.contiguous(), rstd.contiguous()
     gy, gy_stride = _rows(grad_y)
     hr, h_stride = _rows(sum)
-    gs, gs_stride = None, 0
+    gs_stride = 0
     if grad_sum is not None:
         _same("grad_sum", grad_sum, sum)
         gs, gs_stride = _rows(grad_sum)
+        gs_at = gs.data_ptr()
     rows = mean.numel()
-    grad_x = _empty_like(sum)
-    grad_delta = grad_x if delta_scale == 1.0 else torch.empty_like(grad_x)
-    grad_weight = grad_bias = work = None
-    pcode = code if weight is None else _DTYPE_CODE[weight.dtype]
+    grad_x = grad_delta = _empty_like(sum)
+    if delta_scale != 1.0:
+        grad_delta = torch.empty_like(grad_x)
+        gd_at = grad_delta.data_ptr()
+    grad_weight = grad_bias = None
     if param_grads:
         grad_weight = torch.empty_like(weight) if weight is not None else sum.new_empty((dim,))
         grad_bias = torch.empty_like(grad_weight)
         work = mean.new_empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),))
-    _call(_LIBRARY.jk_layer_norm_backward, "jk_layer_norm_backward", sum.get_device(), gy.data_ptr(), gy_stride, hr.data_ptr(),
-          h_stride, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), pcode, _ptr(gs), gs_stride, delta_scale, rows, dim, code,
-          grad_x.data_ptr(), None if grad_delta is grad_x else grad_delta.data_ptr(), _ptr(grad_weight), _ptr(grad_bias),
-          _ptr(work))
+        gw_at, gb_at, work_at = grad_weight.data_ptr(), grad_bias.data_ptr(), work.data_ptr()
+    _call(_LIBRARY.jk_layer_norm_backward, "jk_layer_norm_backward", device, gy.data_ptr(), gy_stride, hr.data_ptr(), h_stride,
+          mean.data_ptr(), rstd.data_ptr(), weight_at, pcode, gs_at, gs_stride, delta_scale, rows, dim, code,
+          grad_x.data_ptr(), gd_at, gw_at, gb_at, work_at)
     return grad_x, grad_delta, grad_weight, grad_bias
 
 

@@ -125,6 +125,46 @@ def test_many_rows(jk, rows, vocab, dtype):
     within(back, want, e, "gradient from the lse")
 
 
+@pytest.mark.parametrize("vocab,dtype", [(1025, torch.float32), (20001, torch.bfloat16), (70003, torch.float16), (300001, torch.float32),
+                                         (500001, torch.bfloat16)])
+def test_gradient_rows_that_lie_otherwise(jk, vocab, dtype):
+    """An expanded row of an odd vocabulary has a gradient whose rows begin elsewhere against 16
+    bytes, and rows beyond a cluster's shared memory are read twice."""
+    logits, _ = data(1, vocab, dtype, 12, 0.0)
+    for z in (logits.expand(6, vocab), logits.repeat(3, 1)):
+        targets = torch.tensor([vocab - 1, IGNORE, 5, 0, 17, 2], device="cuda")[:z.shape[0]]
+        (loss, lse, grad), (e_loss, e_lse, e_grad), valid = exact(z, targets, 0.05)
+        want, e = stored(grad, e_grad + 2 * U * grad.abs(), 1.0 / int(valid.sum()), dtype)
+        got, g = jk.cross_entropy_with_grad_cuda(z, targets, IGNORE, 0.05)
+        within(got, loss.sum() / valid.sum(), e_loss[valid].mean() + 4 * U * loss.sum(), "mean")
+        # rows read twice have their gradient from the lse, which rounds once more
+        within(g, want, e + 2 * U * lse.abs().max() * want.abs(), "gradient")
+        got, got_lse = jk.cross_entropy_forward_cuda(z, targets, IGNORE, 0.05, "none")
+        within(got, loss, e_loss, "losses")
+        within(got_lse, lse, e_lse, "lse")
+        back = jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), z, targets, got_lse, IGNORE, 0.05)
+        within(back, want, e + 2 * U * lse.abs().max() * want.abs(), "gradient from the lse")
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 100000), (7, 30001), (150, 1025), (600, 2500), (1500, 8193)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_and_many_long_rows(jk, rows, vocab, dtype):
+    """Rows that a cluster of blocks shares, rows that several warps have parts of, and more rows
+    than blocks, with ignored rows among them."""
+    logits, targets = data(rows, vocab, dtype, 13, 0.4)
+    (loss, lse, grad), (e_loss, e_lse, e_grad), valid = exact(logits, targets)
+    n = int(valid.sum())
+    got, g = jk.cross_entropy_with_grad_cuda(logits, targets, grad_scale=float(n))
+    within(got, loss.sum() / n, e_loss[valid].mean() + 4 * U * loss.sum() / n, "mean")
+    want, e = stored(grad, e_grad + 2 * U * grad.abs(), 1.0, dtype)
+    within(g, want, e, "gradient")
+    got, got_lse = jk.cross_entropy_forward_cuda(logits, targets)
+    within(got, loss.sum() / n, e_loss[valid].mean() + 4 * U * loss.sum() / n, "mean alone")
+    within(got_lse, lse, e_lse, "lse")
+    back = jk.cross_entropy_backward_cuda(torch.full((), float(n), device="cuda"), logits, targets, got_lse)
+    within(back, want, e + 2 * U * lse.abs().max() * want.abs(), "gradient from the lse")
+
+
 @pytest.mark.parametrize("vocab", [72, 1000, 20000])
 def test_layouts(jk, vocab):
     """Slices of a padded vocabulary, rows off a 16-byte boundary, expanded rows and transposed

@@ -128,7 +128,10 @@ def test_forward_and_backward_match_the_formula(jk, rows, dim, dtype, params):
 
 
 @pytest.mark.parametrize("rows,dim,dtype", [(20000, 96, torch.bfloat16), (4096, 512, torch.float32), (9001, 130, torch.float16),
-                                            (1500, 3001, torch.bfloat16)])
+                                            (1500, 3001, torch.bfloat16), (30000, 37, torch.float16), (30001, 5, torch.bfloat16),
+                                            (40000, 3, torch.float32), (9000, 301, torch.float32), (4001, 1001, torch.bfloat16),
+                                            (20003, 90, torch.float16), (1203, 5999, torch.float16), (777, 6145, torch.float32),
+                                            (900, 16375, torch.bfloat16), (400, 16384, torch.float32)])
 def test_many_rows(jk, rows, dim, dtype):
     t = data(rows, dim, dtype, 5)
     y, total, mean, rstd = jk.layer_norm_forward_cuda(t["x"], t["weight"], t["bias"], EPS, t["delta"])
