@@ -56,6 +56,7 @@ struct Args {
   int64_t grad_stride;
   Partial* partials;
   const int* counts;  // of kCounts blocks, or null: count here
+  float* loss_now;    // not null where one block has all rows: it writes the reduced loss itself
 };
 
 // A product that is rounded by itself, whatever it is added to.
@@ -285,8 +286,10 @@ struct RowLoss {
 };
 
 // ---------------------------------------------------------------- short rows
-// A warp per row, N turns of VEC neighbouring elements per lane.
-constexpr int kWarpThreads = 256;
+// A warp per row, N turns of VEC neighbouring elements per lane. So few rows as kOneBlockRows are one
+// block's, which then needs no second kernel for their sum.
+constexpr int kWarpThreads = 256, kOneBlockThreads = 512;
+constexpr int64_t kOneBlockRows = 2 * kOneBlockThreads / 32;
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_row(float (&f)[VEC], const T* p) {
@@ -296,18 +299,18 @@ __device__ __forceinline__ void load_row(float (&f)[VEC], const T* p) {
     unpack<T>(*reinterpret_cast<const uint4*>(p), f);
 }
 
-template <typename T, int MODE, int VEC, int N>
-__global__ void __launch_bounds__(kWarpThreads) warp_kernel(const Args<T> a) {
-  __shared__ int scratch[kWarpThreads / 32];
-  __shared__ Partial parts[kWarpThreads / 32];
+template <typename T, int MODE, int VEC, int N, int THREADS>
+__global__ void __launch_bounds__(THREADS) warp_kernel(const Args<T> a) {
+  __shared__ int scratch[THREADS / 32];
+  __shared__ Partial parts[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int vocab = static_cast<int>(a.vocab);
   float factor = 0.f;
-  if (MODE != kLoss) factor = gradient_factor(a, MODE == kBoth, kWarpThreads, scratch, [] { __syncthreads(); });
+  if (MODE != kLoss) factor = gradient_factor(a, MODE == kBoth, THREADS, scratch, [] { __syncthreads(); });
   const float share = a.smoothing / static_cast<float>(vocab), hit = 1.f - a.smoothing;
   Partial part{0.0, 0};
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kWarpThreads / 32) + warp; r < a.rows;
-       r += static_cast<int64_t>(gridDim.x) * (kWarpThreads / 32)) {
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (THREADS / 32) + warp; r < a.rows;
+       r += static_cast<int64_t>(gridDim.x) * (THREADS / 32)) {
     const int64_t target = a.targets[r];
     const T* z = a.logits + r * a.stride;
     T* g = MODE == kLoss ? nullptr : a.grad + r * a.grad_stride;
@@ -393,13 +396,16 @@ __global__ void __launch_bounds__(kWarpThreads) warp_kernel(const Args<T> a) {
   if (lane == 0) parts[warp] = part;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < kWarpThreads / 32; ++i) part.sum += parts[i].sum, part.rows += parts[i].rows;
-    a.partials[blockIdx.x] = part;
+    for (int i = 1; i < THREADS / 32; ++i) part.sum += parts[i].sum, part.rows += parts[i].rows;
+    if (a.loss_now != nullptr)
+      *a.loss_now = static_cast<float>(a.reduction == JK_REDUCE_MEAN ? part.sum / static_cast<double>(part.rows) : part.sum);
+    else
+      a.partials[blockIdx.x] = part;
   }
 }
 
 // ---------------------------------------------------------------- a row as 16-byte packs
-constexpr int kTurn = 4;  // packs that a thread takes at once
+constexpr int kTurn = 6;  // packs that a thread takes at once
 
 // Where a row lies against 16-byte packs: pack k holds columns k * kPack - shift ..., the first
 // and the last one perhaps in part.
@@ -426,16 +432,25 @@ __device__ __forceinline__ T minus_inf() {
 // one. A row that more than one warp has part of leaves a record for each, and the reduction over
 // rows joins them.
 constexpr int kStreamThreads = 256;
-#ifndef JKV_SB
-#define JKV_SB 3
-#endif
-constexpr int kStreamBlocksPerSm = JKV_SB;
+// Loss of 4096 x 50001 bf16: 70 us with six packs and two blocks on an SM, 73 with four and three, 160
+// with two and six: what a piece costs apart from its packs is spread over more of them.
+constexpr int kStreamBlocksPerSm = 2;
 constexpr int kMaxWarps = 148 * kStreamBlocksPerSm * (kStreamThreads / 32);
 constexpr int kPiece = 32 * kTurn;  // packs
 
 struct Record {
   int64_t row;  // -1: none
   float m, s, all;
+};
+
+// A piece of a row.
+template <typename T>
+struct Item {
+  int64_t row, target;
+  const T* z;
+  int piece, shift;
+  float value, grad_loss;  // the target's logit (kLoss), or the row's lse
+  bool ignored, inside;
 };
 
 template <typename T, int MODE>
@@ -461,35 +476,54 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
   int64_t targets_from = row, some_targets = 0;  // of 32 rows, a row per lane
   if (item < end) some_targets = a.targets[min(row + lane, a.rows - 1)];
   uint4 next[kTurn];
-  int64_t next_target = 0;
-  float next_zt = 0.f, next_lse = 0.f, next_grad = 0.f;
-  const auto load = [&] {
+  Item<T> it{};
+  const auto enter_row = [&] {
     if (row - targets_from >= 32) {
       targets_from = row;
       some_targets = a.targets[min(row + lane, a.rows - 1)];
     }
-    next_target = __shfl_sync(0xffffffffu, static_cast<long long>(some_targets), static_cast<int>(row - targets_from));
-    if (next_target == a.ignore_index) return;
+    it.row = row;
+    it.target = __shfl_sync(0xffffffffu, static_cast<long long>(some_targets), static_cast<int>(row - targets_from));
+    it.ignored = it.target == a.ignore_index;
     const Window<T> w(a, row);
-    if (MODE == kLoss && piece == 0)
-      next_zt = next_target >= 0 && next_target < vocab ? to_f32(w.z[next_target]) : NAN;
+    it.z = w.z;
+    it.shift = w.shift;
+    it.inside = it.target >= 0 && it.target < vocab;
+    if (it.ignored) return;
+    if (MODE == kLoss && piece == 0) it.value = it.inside ? to_f32(w.z[it.target]) : NAN;
     if (MODE != kLoss) {
-      next_lse = a.lse_in[row];
-      if (a.reduction == JK_REDUCE_NONE) next_grad = a.grad_loss[row];
+      it.value = a.lse_in[row];
+      if (MODE == kBackward && a.reduction == JK_REDUCE_NONE) it.grad_loss = a.grad_loss[row];
     }
+  };
+  // whether all packs of a piece are whole
+  const auto interior = [&](const Item<T>& q) { return q.piece > 0 && (q.piece + 1) * kPiece * kP <= vocab + q.shift; };
+  const auto load = [&] {
+    it.piece = piece;
+    if (it.ignored) return;
+    const int c0 = (piece * kPiece + lane) * kP - it.shift;
+    if (interior(it)) {
+      const uint4* from = reinterpret_cast<const uint4*>(it.z + c0);
 #pragma unroll
-    for (int i = 0; i < kTurn; ++i) {
-      const int k = piece * kPiece + i * 32 + lane, c = k * kP - w.shift;
-      if (c >= 0 && c + kP <= vocab) {
-        next[i] = __ldcs(reinterpret_cast<const uint4*>(w.z + c));
-      } else {  // -inf where there is no column
-        T* e = reinterpret_cast<T*>(&next[i]);
+      for (int i = 0; i < kTurn; ++i) next[i] = __ldcs(from + i * 32);
+    } else {
 #pragma unroll
-        for (int j = 0; j < kP; ++j) e[j] = c + j >= 0 && c + j < vocab ? w.z[c + j] : minus_inf<T>();
+      for (int i = 0; i < kTurn; ++i) {
+        const int c = c0 + i * 32 * kP;
+        if (c >= 0 && c + kP <= vocab) {
+          next[i] = __ldcs(reinterpret_cast<const uint4*>(it.z + c));
+        } else {  // -inf where there is no column
+          T* e = reinterpret_cast<T*>(&next[i]);
+#pragma unroll
+          for (int j = 0; j < kP; ++j) e[j] = c + j >= 0 && c + j < vocab ? it.z[c + j] : minus_inf<T>();
+        }
       }
     }
   };
-  if (item < end) load();
+  if (item < end) {
+    enter_row();
+    load();
+  }
 
   Sum v{-INFINITY, 0.f};
   float all = 0.f, zt = 0.f;
@@ -499,33 +533,39 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
     uint4 raw[kTurn];
 #pragma unroll
     for (int i = 0; i < kTurn; ++i) raw[i] = next[i];
-    const int64_t r = row, target = next_target;
-    const int at_piece = piece;
-    const float lse = next_lse, grad_loss = next_grad;
-    if (piece == 0) {
+    const Item<T> q = it;
+    if (q.piece == 0) {
       from_start = true;
-      zt = next_zt;
+      zt = q.value;
     }
     ++item;
     if (++piece == pieces) {
       piece = 0;
       ++row;
     }
-    if (item < end) load();
-    const bool ignored = target == a.ignore_index;
+    if (item < end) {
+      if (piece == 0) enter_row();
+      load();
+    }
+    const int c0 = (q.piece * kPiece + lane) * kP - q.shift;
+    const bool last = q.piece == pieces - 1;
     if (MODE == kLoss) {
-      const bool last = at_piece == pieces - 1;
-      if (!ignored) {
+      if (!q.ignored) {
         take_packs<T>(v, raw);
         if (a.smoothing != 0.f) {
-          const Window<T> w(a, r);
+          if (interior(q)) {
+            all += pack_sum<T>(raw);
+          } else {
 #pragma unroll
-          for (int i = 0; i < kTurn; ++i) {
-            const int c = (at_piece * kPiece + i * 32 + lane) * kP - w.shift;
-            float f[kP];
-            unpack<T>(raw[i], f);
+            for (int i = 0; i < kTurn; ++i) {
+              float f[kP];
+              unpack<T>(raw[i], f);
 #pragma unroll
-            for (int j = 0; j < kP; ++j) all += c + j >= 0 && c + j < vocab ? f[j] : 0.f;
+              for (int j = 0; j < kP; ++j) {
+                const int c = c0 + i * 32 * kP + j;
+                all += c >= 0 && c < vocab ? f[j] : 0.f;
+              }
+            }
           }
         }
         if (last || item == end) {
@@ -534,45 +574,44 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
           if (last && from_start) {
             const RowLoss l(v, zt, all, a.smoothing, vocab);
             if (lane == 0) {
-              if (a.losses != nullptr) a.losses[r] = l.loss;
-              if (a.lse_out != nullptr) a.lse_out[r] = l.lse;
+              if (a.losses != nullptr) a.losses[q.row] = l.loss;
+              if (a.lse_out != nullptr) a.lse_out[q.row] = l.lse;
             }
             part.sum += l.loss;
             part.rows += 1;
           } else {
-            const int slot = r == first_row ? 0 : 1;
+            const int slot = q.row == first_row ? 0 : 1;
             recorded[slot] = true;
-            if (lane == 0) records[2 * warp + slot] = {r, v.m, v.s, all};
+            if (lane == 0) records[2 * warp + slot] = {q.row, v.m, v.s, all};
           }
           v = {-INFINITY, 0.f};
           all = 0.f;
         }
       } else if (last && lane == 0) {
-        if (a.losses != nullptr) a.losses[r] = 0.f;
-        if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
+        if (a.losses != nullptr) a.losses[q.row] = 0.f;
+        if (a.lse_out != nullptr) a.lse_out[q.row] = 0.f;
       }
     } else {
-      const Window<T> w(a, r);
-      T* g = a.grad + r * a.grad_stride;
-      const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(w.z)) & 15) == 0;
-      const bool inside = target >= 0 && target < vocab;
-      const Base base(lse);
-      const float c0 = !inside ? NAN : a.reduction == JK_REDUCE_NONE ? grad_loss : factor;
-      const float scale = c0 * expf(base.rest()), other = -share * c0;
+      T* g = a.grad + q.row * a.grad_stride;
+      const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(q.z)) & 15) == 0;
+      const Base base(q.value);
+      const float k0 = !q.inside ? NAN : MODE == kBackward && a.reduction == JK_REDUCE_NONE ? q.grad_loss : factor;
+      const float scale = k0 * expf(base.rest()), other = -share * k0;
+      const bool whole = alike && interior(q);
 #pragma unroll
       for (int i = 0; i < kTurn; ++i) {
-        const int c = (at_piece * kPiece + i * 32 + lane) * kP - w.shift;
-        if (c >= vocab) continue;
+        const int c = c0 + i * 32 * kP;
+        if (!whole && c >= vocab) continue;
         float f[kP] = {};
-        if (!ignored) {
+        if (!q.ignored) {
           unpack<T>(raw[i], f);
           gradient_pack<T>(f, base, scale, other);
-          if (inside && target >= c && target < c + kP) {
+          if (q.inside && static_cast<uint32_t>(static_cast<int>(q.target) - c) < static_cast<uint32_t>(kP)) {
 #pragma unroll
-            for (int j = 0; j < kP; ++j) f[j] -= c + j == target ? hit * c0 : 0.f;
+            for (int j = 0; j < kP; ++j) f[j] -= c + j == static_cast<int>(q.target) ? hit * k0 : 0.f;
           }
         }
-        if (alike && c >= 0 && c + kP <= vocab) {
+        if (whole || (alike && c >= 0 && c + kP <= vocab)) {
           __stcs(reinterpret_cast<uint4*>(g + c), pack<T>(f));
         } else {
 #pragma unroll
@@ -581,7 +620,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
         }
       }
     }
-    if (at_piece == pieces - 1) from_start = false;
+    if (last) from_start = false;
   }
   if (MODE != kLoss) return;
   grid_dependency_launch();
@@ -596,14 +635,10 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
 // A cluster of blocks has a row, each block a slice of it in shared memory. One warp of the block
 // has the next rows' slices copied there and finds out how they lie; the others (workers) take a
 // slice twice, for the sum and for the gradient.
-#ifndef JKV_W
-#define JKV_W 352
-#endif
-#ifndef JKV_P
-#define JKV_P 3
-#endif
-constexpr int kWorkers = JKV_W;
-constexpr int kRowBlocksPerSm = JKV_P;
+// 4096 x 16384 bf16: 56 us with 352 workers and three blocks on an SM, 60 with 224 and three, 72 with 96
+// and three, 67 with 224 and two.
+constexpr int kWorkers = 352;
+constexpr int kRowBlocksPerSm = 3;
 constexpr int kMaxStages = 6;
 constexpr int kMaxCluster = 8;
 
@@ -955,18 +990,18 @@ struct Workspace {
 
 constexpr int kWarpColumns = 1024;  // of the rows that a warp holds
 
-template <typename T, int MODE, int VEC>
+template <typename T, int MODE, int VEC, int THREADS>
 void launch_warps(const Args<T>& a, int blocks, cudaStream_t s) {
   const int64_t turns = (a.vocab + 32 * VEC - 1) / (32 * VEC);
   constexpr int kMost = kWarpColumns / 32 / VEC;
   if constexpr (VEC == 1) {
-    if (turns <= 2) warp_kernel<T, MODE, VEC, 2><<<blocks, kWarpThreads, 0, s>>>(a);
-    else if (turns <= 8) warp_kernel<T, MODE, VEC, 8><<<blocks, kWarpThreads, 0, s>>>(a);
-    else warp_kernel<T, MODE, VEC, kMost><<<blocks, kWarpThreads, 0, s>>>(a);
+    if (turns <= 2) warp_kernel<T, MODE, VEC, 2, THREADS><<<blocks, THREADS, 0, s>>>(a);
+    else if (turns <= 8) warp_kernel<T, MODE, VEC, 8, THREADS><<<blocks, THREADS, 0, s>>>(a);
+    else warp_kernel<T, MODE, VEC, kMost, THREADS><<<blocks, THREADS, 0, s>>>(a);
   } else {
-    if (turns <= 1) warp_kernel<T, MODE, VEC, 1><<<blocks, kWarpThreads, 0, s>>>(a);
-    else if (turns <= 2) warp_kernel<T, MODE, VEC, 2><<<blocks, kWarpThreads, 0, s>>>(a);
-    else warp_kernel<T, MODE, VEC, kMost><<<blocks, kWarpThreads, 0, s>>>(a);
+    if (turns <= 1) warp_kernel<T, MODE, VEC, 1, THREADS><<<blocks, THREADS, 0, s>>>(a);
+    else if (turns <= 2) warp_kernel<T, MODE, VEC, 2, THREADS><<<blocks, THREADS, 0, s>>>(a);
+    else warp_kernel<T, MODE, VEC, kMost, THREADS><<<blocks, THREADS, 0, s>>>(a);
   }
 }
 
@@ -1008,19 +1043,22 @@ bool launch_rows(const Args<T>& a, int64_t blocks, int stages, int slice_packs, 
   return cudaLaunchKernelEx(&cfg, kernel, a, stages, slice_packs, cluster) == cudaSuccess;
 }
 
-template <typename T>
-int launch_warp_rows(const Args<T>& a, int mode, cudaStream_t s) {
+// Returns the blocks that left a partial.
+template <typename T, int MODE>
+int launch_warp_rows(const Args<T>& a, cudaStream_t s) {
   const bool aligned = a.vocab % kPack<T> == 0 && a.stride % kPack<T> == 0 && aligned16(a.logits) &&
-                       (mode == kLoss || (a.grad_stride % kPack<T> == 0 && aligned16(a.grad)));
+                       (MODE == kLoss || (a.grad_stride % kPack<T> == 0 && aligned16(a.grad)));
+  if constexpr (MODE != kBackward) {
+    if (a.loss_now != nullptr) {
+      if (aligned) launch_warps<T, MODE, kPack<T>, kOneBlockThreads>(a, 1, s);
+      else launch_warps<T, MODE, 1, kOneBlockThreads>(a, 1, s);
+      return 0;
+    }
+  }
   const int64_t want = (a.rows + kWarpThreads / 32 - 1) / (kWarpThreads / 32);
   const int blocks = static_cast<int>(want < kMaxBlocks ? want : kMaxBlocks);
-  if (mode == kLoss) {
-    if (aligned) launch_warps<T, kLoss, kPack<T>>(a, blocks, s); else launch_warps<T, kLoss, 1>(a, blocks, s);
-  } else if (mode == kBoth) {
-    if (aligned) launch_warps<T, kBoth, kPack<T>>(a, blocks, s); else launch_warps<T, kBoth, 1>(a, blocks, s);
-  } else {
-    if (aligned) launch_warps<T, kBackward, kPack<T>>(a, blocks, s); else launch_warps<T, kBackward, 1>(a, blocks, s);
-  }
+  if (aligned) launch_warps<T, MODE, kPack<T>, kWarpThreads>(a, blocks, s);
+  else launch_warps<T, MODE, 1, kWarpThreads>(a, blocks, s);
   return blocks;
 }
 
@@ -1062,7 +1100,7 @@ void count_apart(Args<T>& a, Workspace* ws, cudaStream_t s) {
 template <typename T>
 int backward(Args<T> a, Workspace* ws, cudaStream_t s) {
   count_apart(a, ws, s);
-  if (a.vocab <= kWarpColumns) launch_warp_rows(a, kBackward, s);
+  if (a.vocab <= kWarpColumns) launch_warp_rows<T, kBackward>(a, s);
   else launch_stream<T, kBackward>(a, ws, s);
   return launch_status();
 }
@@ -1075,7 +1113,9 @@ int forward(Args<T> a, float* loss, Workspace* ws, cudaStream_t s) {
   if (a.rows > 0) {
     if (a.grad != nullptr) count_apart(a, ws, s);
     if (a.vocab <= kWarpColumns) {
-      left.partials = launch_warp_rows(a, a.grad != nullptr ? kBoth : kLoss, s);
+      if (a.rows <= kOneBlockRows) a.loss_now = loss;
+      left.partials = a.grad != nullptr ? launch_warp_rows<T, kBoth>(a, s) : launch_warp_rows<T, kLoss>(a, s);
+      if (a.loss_now != nullptr) loss = nullptr;
     } else {
       if (a.grad != nullptr) left.partials = launch_both(a, s);
       if (left.partials < 0) {
@@ -1129,7 +1169,7 @@ extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_strid
   JK_WITH_TYPE(dtype, T, {
     const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
                           label_smoothing, reduction, grad_scale, nullptr, nullptr, losses, lse,
-                          static_cast<T*>(grad), grad_stride, nullptr, nullptr};
+                          static_cast<T*>(grad), grad_stride, nullptr, nullptr, nullptr};
     st = loss::forward<T>(a, loss, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });
   return st;
@@ -1154,7 +1194,7 @@ extern "C" int jk_cross_entropy_backward(const float* grad_loss, const void* log
   JK_WITH_TYPE(dtype, T, {
     const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
                           label_smoothing, reduction, 1.f, grad_loss, lse, nullptr, nullptr, static_cast<T*>(grad),
-                          grad_stride, nullptr, nullptr};
+                          grad_stride, nullptr, nullptr, nullptr};
     st = loss::backward<T>(a, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });
   return st;

@@ -120,6 +120,14 @@ def _empty_like(t: Tensor) -> Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _empty(shape, dtype: torch.dtype, device: torch.device) -> Tensor:
+    """torch.empty, by its quickest way for no and for one dim."""
+    n = len(shape)
+    if n > 1:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty_strided(shape, (1,) * n, dtype=dtype, device=device)
+
+
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -158,7 +166,7 @@ def layer_norm_forward_cuda(x: Tensor, weight: Optional[Tensor] = None, bias: Op
         dr, d_stride = _rows(delta)
         total = torch.empty_like(y)
         delta_at, sum_at = dr.data_ptr(), total.data_ptr()
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    mean = _empty(x.shape[:-1], torch.float32, x.device)
     rstd = torch.empty_like(mean)
     _call(_LIBRARY.jk_layer_norm_forward, "jk_layer_norm_forward", device, xr.data_ptr(), x_stride, delta_at, d_stride,
           delta_scale, weight_at, bias_at, pcode, mean.numel(), dim, code, eps, y.data_ptr(), sum_at, mean.data_ptr(),
@@ -207,7 +215,7 @@ def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Te
     if param_grads:
         grad_weight = torch.empty_like(weight) if weight is not None else sum.new_empty((dim,))
         grad_bias = torch.empty_like(grad_weight)
-        work = mean.new_empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),))
+        work = _empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),), torch.float32, sum.device)
         gw_at, gb_at, work_at = grad_weight.data_ptr(), grad_bias.data_ptr(), work.data_ptr()
     _call(_LIBRARY.jk_layer_norm_backward, "jk_layer_norm_backward", device, gy.data_ptr(), gy_stride, hr.data_ptr(), h_stride,
           mean.data_ptr(), rstd.data_ptr(), weight_at, pcode, gs_at, gs_stride, delta_scale, rows, dim, code,
@@ -285,15 +293,15 @@ def _grad_like(logits: Tensor) -> Tensor:
 
 def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, grad_scale, want_lse, grad, in_place=False):
     code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
-    rows = targets.numel()
+    rows, device = targets.numel(), logits.device
     lse = losses = None
     if kind == _lib.JK_REDUCE_NONE:
-        loss = losses = logits.new_empty(targets.shape, dtype=torch.float32)
+        loss = losses = _empty(targets.shape, torch.float32, device)
     else:
-        loss = logits.new_empty((), dtype=torch.float32)
+        loss = _empty((), torch.float32, device)
     if want_lse:
-        lse = torch.empty_like(loss) if losses is not None else loss.new_empty(targets.shape)
-    work = loss.new_empty((_LIBRARY.jk_cross_entropy_workspace(rows) // 4,))
+        lse = torch.empty_like(loss) if losses is not None else _empty(targets.shape, torch.float32, device)
+    work = _empty((_LIBRARY.jk_cross_entropy_workspace(rows) // 4,), torch.float32, device)
     if in_place:
         grad_ptr, grad_stride = lr.data_ptr(), stride
     else:
@@ -360,7 +368,7 @@ def cross_entropy_backward_cuda(grad_loss: Tensor, logits: Tensor, targets: Tens
     gl = grad_loss.detach().to(torch.float32).contiguous()
     lse = lse.contiguous()
     grad = _grad_like(logits)
-    work = lse.new_empty((_LIBRARY.jk_cross_entropy_workspace(targets.numel()) // 4,))
+    work = _empty((_LIBRARY.jk_cross_entropy_workspace(targets.numel()) // 4,), torch.float32, logits.device)
     _call(_LIBRARY.jk_cross_entropy_backward, "jk_cross_entropy_backward", logits.get_device(), gl.data_ptr(), lr.data_ptr(),
           stride, targets.data_ptr(), lse.data_ptr(), targets.numel(), logits.shape[-1], code, int(ignore_index),
           float(label_smoothing), kind, grad.data_ptr(), _rows(grad)[1], work.data_ptr())
@@ -448,13 +456,10 @@ def _run_clip(tensors, outs, norm_type, clip, max_norm):
             some = [p for p, n in zip(written, numels) if n]
             if len(set(some)) != len(some):
                 raise ValueError("a tensor is given twice: it would be scaled twice")
-    if tensors:
-        device = tensors[0].get_device()
-        work = tensors[0].new_empty((_CLIP_WORKSPACE,), dtype=torch.float64)
-    else:
-        device = _current_device()
-        work = torch.empty((_CLIP_WORKSPACE,), dtype=torch.float64, device=torch.device("cuda", device))
-    total = work.new_empty((), dtype=torch.float32)
+    where = tensors[0].device if tensors else torch.device("cuda", _current_device())
+    device = where.index
+    work = _empty((_CLIP_WORKSPACE,), torch.float64, where)
+    total = _empty((), torch.float32, where)
     _call(_LIBRARY.jk_clip_grad_norm, "jk_clip_grad_norm", device, ptrs.buffer_info()[0],
           None if dst is None else out_ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0],
           None if dst is None else out_codes.buffer_info()[0], len(src), kind, clip, max_norm, 1e-6, total.data_ptr(),
