@@ -413,12 +413,14 @@ def _flat(t: Tensor) -> bool:
     return True
 
 
-def _gradients(grads, name: str) -> list[Tensor]:
+def _gradients(grads, name: str) -> tuple[list[Tensor], list[torch.dtype]]:
+    """The tensors, which are CUDA float tensors of one device, and their dtypes."""
     tensors = [grads] if isinstance(grads, Tensor) else [g for g in grads if g is not None]
     # one look at all of them (a model has hundreds); which one is wrong is sought only if one is
     try:
-        fine = (len(set(map(Tensor.get_device, tensors))) <= 1 and all(map(Tensor.is_cuda.__get__, tensors))
-                and set(map(Tensor.dtype.__get__, tensors)) <= _DTYPE_CODE.keys())
+        devices = set(map(Tensor.get_device, tensors))  # -1: not a CUDA tensor
+        types = list(map(Tensor.dtype.__get__, tensors))
+        fine = len(devices) <= 1 and -1 not in devices and set(types) <= _DTYPE_CODE.keys()
     except TypeError:  # not a tensor
         fine = False
     if not fine:
@@ -426,17 +428,20 @@ def _gradients(grads, name: str) -> list[Tensor]:
             _check_input(f"{name} {i}", t)
             if t.device != tensors[0].device:
                 raise RuntimeError(f"{name} {i} is on {t.device}, expected {tensors[0].device}")
-    return tensors
+    return tensors, types
 
 
-def _table(tensors: list[Tensor]) -> tuple[array.array, array.array]:
-    """The addresses and the dtype codes."""
-    types = list(map(Tensor.dtype.__get__, tensors))
-    codes = array.array("i", map(_DTYPE_CODE.__getitem__, types))
-    return array.array("Q", map(Tensor.data_ptr, tensors)), codes
+def _codes(types: list[torch.dtype]) -> array.array:
+    if types and types.count(types[0]) == len(types):
+        return array.array("i", [_DTYPE_CODE[types[0]]]) * len(types)
+    return array.array("i", map(_DTYPE_CODE.__getitem__, types))
 
 
-def _run_clip(tensors, outs, norm_type, clip, max_norm):
+def _addresses(tensors: list[Tensor]) -> array.array:
+    return array.array("Q", map(Tensor.data_ptr, tensors))
+
+
+def _run_clip(tensors, types, outs, out_types, norm_type, clip, max_norm):
     kind = _NORM.get(float(norm_type))
     if kind is None:
         raise ValueError(f"unsupported norm_type {norm_type} (2 or inf)")
@@ -447,9 +452,9 @@ def _run_clip(tensors, outs, norm_type, clip, max_norm):
                 if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
                     raise ValueError("a tensor to write has elements that share memory (an expanded tensor)")
         src, dst, back = _blocks(tensors, outs, clip)
-    ptrs, codes = _table(src)
+    ptrs, codes = _addresses(src), _codes(types)
     numels = array.array("q", map(Tensor.numel, src))
-    out_ptrs, out_codes = (None, None) if dst is None else _table(dst)
+    out_ptrs, out_codes = (None, None) if dst is None else (_addresses(dst), _codes(out_types))
     if clip:
         written = ptrs if dst is None else out_ptrs
         if len(set(written)) != len(written):  # empty tensors may share an address
@@ -497,7 +502,7 @@ def _blocks(tensors, outs, clip):
 def grad_norm(grads: Union[Tensor, Iterable[Optional[Tensor]]], norm_type: float = 2.0) -> Tensor:
     """Norm (2 or inf) over all elements of the gradients together, an f32 scalar on their
     device. The squares are summed in f64, so the norm is finite wherever it fits f32."""
-    return _run_clip(_gradients(grads, "gradient"), None, norm_type, 0, 0.0)
+    return _run_clip(*_gradients(grads, "gradient"), None, None, norm_type, 0, 0.0)
 
 
 def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: float, norm_type: float = 2.0,
@@ -510,18 +515,18 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: 
     master gradients of bf16 ones, say). Tensors must not overlap. A gradient that holds NaN
     makes all of them NaN, one that holds an infinity makes the others 0, as the formula has it;
     error_if_nonfinite raises instead, after reading the norm back, with the gradients scaled."""
-    tensors = _gradients(grads, "gradient")
-    outs = None
+    tensors, types = _gradients(grads, "gradient")
+    outs = out_types = None
     if out is not None:
-        outs = _gradients(out, "out")
+        outs, out_types = _gradients(out, "out")
         if len(outs) != len(tensors):
             raise ValueError(f"out has {len(outs)} tensors for {len(tensors)} gradients")
         if outs and outs[0].device != tensors[0].device:
             raise RuntimeError(f"out is on {outs[0].device}, expected {tensors[0].device}")
-        if list(map(Tensor.shape.__get__, outs)) != list(map(Tensor.shape.__get__, tensors)):
+        if not all(map(Tensor.is_same_size, outs, tensors)):
             i = next(i for i, (o, g) in enumerate(zip(outs, tensors)) if o.shape != g.shape)
             raise ValueError(f"out {i} has shape {tuple(outs[i].shape)}, expected {tuple(tensors[i].shape)}")
-    total = _run_clip(tensors, outs, norm_type, 1, float(max_norm))
+    total = _run_clip(tensors, types, outs, out_types, norm_type, 1, float(max_norm))
     if error_if_nonfinite and not math.isfinite(total.item()):
         raise RuntimeError(f"the norm of the gradients is {total.item()}")
     return total
