@@ -697,7 +697,11 @@ int pick_backward(const Backward& a, cudaStream_t s) {
     return RUN(16, 1024);                                               \
   }
 
-constexpr int64_t kMaxDim = 16384 - 8;  // of the rows that stay in registers, wherever they begin
+// Whether rows stay in registers: 16384 elements, with room for a start within a pack.
+template <typename T>
+bool in_registers(int64_t dim) {
+  return dim + (dim % kPack<T> != 0 ? kPack<T> : 0) <= 16384;
+}
 
 template <typename T, int VEC, bool SHIFTED>
 int shape_forward(const Forward& a, cudaStream_t s) {
@@ -723,7 +727,7 @@ bool lies_plain(const void* p, int64_t stride, int64_t dim) {
 
 template <typename T>
 void forward(const Forward& a, cudaStream_t s) {
-  if (a.dim > kMaxDim) {
+  if (!in_registers<T>(a.dim)) {
     long_forward_kernel<T><<<static_cast<unsigned>(a.rows < 148 * 4 ? a.rows : 148 * 4), kLongThreads, 0, s>>>(a);
   } else if (lies_plain<T>(a.x, a.x_stride, a.dim) && lies_plain<T>(a.delta, a.delta_stride, a.dim) && aligned16(a.y) &&
              aligned16(a.sum)) {
@@ -737,7 +741,7 @@ void forward(const Forward& a, cudaStream_t s) {
 // Returns the blocks that left a share of the parameter gradients.
 template <typename T>
 int backward(const Backward& a, cudaStream_t s) {
-  if (a.dim > kMaxDim) {
+  if (!in_registers<T>(a.dim)) {
     const int blocks = static_cast<int>(a.rows < kMaxParts ? a.rows : kMaxParts);
     long_backward_kernel<T><<<blocks, kLongThreads, 0, s>>>(a);
     return blocks;
