@@ -635,10 +635,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
 // A cluster of blocks has a row, each block a slice of it in shared memory. One warp of the block
 // has the next rows' slices copied there and finds out how they lie; the others (workers) take a
 // slice twice, for the sum and for the gradient.
-// 4096 x 16384 bf16: 56 us with 352 workers and three blocks on an SM, 60 with 224 and three, 72 with 96
-// and three, 67 with 224 and two.
-constexpr int kWorkers = 352;
-constexpr int kRowBlocksPerSm = 3;
+constexpr int kMaxWorkers = 480;
 constexpr int kMaxStages = 6;
 constexpr int kMaxCluster = 8;
 
@@ -658,9 +655,9 @@ struct Slice {
 struct Shared {
   uint64_t full[kMaxStages], empty[kMaxStages], joined[2];
   Slice slice[kMaxStages];
-  float4 warp[2][kWorkers / 32];  // (m, s, target logit, sum of logits) of each warp
+  float4 warp[2][kMaxWorkers / 32];  // (m, s, target logit, sum of logits) of each warp
   float4 peer[2][kMaxCluster];    // and of each block of the cluster
-  int counts[kWorkers / 32];
+  int counts[kMaxWorkers / 32];
 };
 
 __device__ __forceinline__ uint32_t map_peer(const void* p, int rank) {
@@ -697,7 +694,7 @@ __device__ __forceinline__ void leave(int cluster) {
 
 // The loading warp: slices of rows first, first + step, ... A wait that runs out is recorded, and no
 // later one is waited for: the kernel then ends soon, with an error that jk_device_status reports.
-template <typename T>
+template <typename T, int WORKERS>
 __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsigned char* memory, int stages, int slice_packs,
                                             int rank, int cluster, int64_t first, int64_t step) {
   constexpr int kP = kPack<T>;
@@ -733,7 +730,7 @@ __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsign
       const int at = s.inside ? static_cast<int>(target) - origin : -1;
       s.at = at >= s.low && at < s.high ? at : -1;
       const int pack = s.at / kP;
-      s.owner = s.at >= 0 && pack >= s.whole && pack < s.whole_end ? (pack - s.whole) % kWorkers : -1;
+      s.owner = s.at >= 0 && pack >= s.whole && pack < s.whole_end ? (pack - s.whole) % WORKERS : -1;
       sh.slice[stage] = s;
       const int from = s.head_outside ? 1 : 0, to = s.tail_outside ? s.whole_end : s.end;
       const uint32_t bytes = !s.ignored && to > from ? static_cast<uint32_t>(to - from) * 16 : 0;
@@ -753,12 +750,32 @@ __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsign
   if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
 }
 
-template <typename T, bool CLUSTER, bool SMOOTH>
-__global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
+// Adds packs k, k + WORKERS, ... (N of them, those before `end`) to a thread's sum.
+template <typename T, int WORKERS, bool SMOOTH, int N>
+__device__ __forceinline__ void sum_turn(Sum& v, float& all, const uint4* packs, int k, int end) {
+  const T low = minus_inf<T>();
+  uint32_t two;
+  if constexpr (sizeof(T) == 4) two = __float_as_uint(low);
+  else two = *reinterpret_cast<const uint16_t*>(&low) * 0x10001u;
+  uint4 raw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) raw[i] = k + i * WORKERS < end ? packs[k + i * WORKERS] : make_uint4(two, two, two, two);
+  take_packs<T>(v, raw);
+  if (SMOOTH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint4 one[1] = {raw[i]};
+      if (k + i * WORKERS < end) all += pack_sum<T>(one);
+    }
+  }
+}
+
+template <typename T, int WORKERS, int PER_SM, bool CLUSTER, bool SMOOTH>
+__global__ void __launch_bounds__(WORKERS + 32, PER_SM)
     rows_kernel(const Args<T> a, int stages, int slice_packs, int cluster_size) {
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ Shared sh;
-  constexpr int kP = kPack<T>, kWarps = kWorkers / 32;
+  constexpr int kP = kPack<T>, kWarps = WORKERS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cluster = CLUSTER ? cluster_size : 1;
   const int rank = CLUSTER ? blockIdx.x % cluster : 0;
@@ -776,12 +793,12 @@ __global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   if (warp == kWarps) {
-    load_slices(a, sh, memory, stages, slice_packs, rank, cluster, first, step);
+    load_slices<T, WORKERS>(a, sh, memory, stages, slice_packs, rank, cluster, first, step);
     leave(cluster);
     return;
   }
-  const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); };
-  const float factor = gradient_factor(a, true, kWorkers, sh.counts, sync);
+  const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); };
+  const float factor = gradient_factor(a, true, WORKERS, sh.counts, sync);
   const float hit = 1.f - a.smoothing, share = SMOOTH ? a.smoothing / static_cast<float>(a.vocab) : 0.f;
   bool good = true;
   double sum = 0.0;
@@ -793,17 +810,20 @@ __global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
     const uint4* packs = reinterpret_cast<const uint4*>(memory) + static_cast<size_t>(stage) * slice_packs;
     const int whole = sl.whole, whole_end = sl.whole_end;
     uint4* out = static_cast<uint4*>(sl.out);
-    // the row's ends, thread 0 and 1: pack and whether it has to be fetched from the logits
-    const int end_pack = threadIdx.x == 0 && whole > 0 ? 0 : threadIdx.x == 1 && whole_end < sl.end ? whole_end : -1;
-    const bool outside = threadIdx.x == 0 ? sl.head_outside : sl.tail_outside;
+    // the row's ends, an element to a thread: the first pack's for threads 0-7, the last one's for 8-15
+    const int in_pack = threadIdx.x & 7;
+    int end_at = -1;
+    if (threadIdx.x < 16 && in_pack < kP) {
+      if (threadIdx.x < 8 ? whole > 0 : whole_end < sl.end) end_at = (threadIdx.x < 8 ? 0 : whole_end * kP) + in_pack;
+      if (end_at < sl.low || end_at >= sl.high) end_at = -1;
+    }
+    const bool outside = threadIdx.x < 8 ? sl.head_outside : sl.tail_outside;
     const auto element = [&](int pos, bool from_logits) {
       return to_f32(from_logits ? static_cast<const T*>(sl.in)[pos] : reinterpret_cast<const T*>(packs)[pos]);
     };
     if (sl.ignored) {
-      for (int k = whole + threadIdx.x; k < whole_end; k += kWorkers) out[k] = make_uint4(0, 0, 0, 0);
-      if (end_pack >= 0)
-        for (int pos = max(end_pack * kP, sl.low); pos < min(end_pack * kP + kP, sl.high); ++pos)
-          static_cast<T*>(sl.out)[pos] = from_f32<T>(0.f);
+      for (int k = whole + threadIdx.x; k < whole_end; k += WORKERS) out[k] = make_uint4(0, 0, 0, 0);
+      if (end_at >= 0) static_cast<T*>(sl.out)[end_at] = from_f32<T>(0.f);
       if (threadIdx.x == 0 && rank == 0) {
         if (a.losses != nullptr) a.losses[r] = 0.f;
         if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
@@ -811,25 +831,14 @@ __global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
     } else {
       Sum v{-INFINITY, 0.f};
       float all = 0.f, zt = 0.f;
-      int k = whole + threadIdx.x;
-      for (; k + (kTurn - 1) * kWorkers < whole_end; k += kTurn * kWorkers) {
-        uint4 raw[kTurn];
-#pragma unroll
-        for (int i = 0; i < kTurn; ++i) raw[i] = packs[k + i * kWorkers];
-        take_packs<T>(v, raw);
-        if (SMOOTH) all += pack_sum<T>(raw);
-      }
-      for (; k < whole_end; k += kWorkers) {
-        const uint4 raw[1] = {packs[k]};
-        take_packs<T>(v, raw);
-        if (SMOOTH) all += pack_sum<T>(raw);
-      }
-      if (end_pack >= 0) {
-        for (int pos = max(end_pack * kP, sl.low); pos < min(end_pack * kP + kP, sl.high); ++pos) {
-          float f[1] = {element(pos, outside)};
-          all += f[0];
-          take(v, f);
-        }
+      // turns of kTurn packs while they are mostly full, then of two
+      int k = whole + threadIdx.x, left = (whole_end - whole + WORKERS - 1) / WORKERS;
+      for (; left > kTurn / 2; left -= kTurn, k += kTurn * WORKERS) sum_turn<T, WORKERS, SMOOTH, kTurn>(v, all, packs, k, whole_end);
+      for (; left > 0; left -= 2, k += 2 * WORKERS) sum_turn<T, WORKERS, SMOOTH, 2>(v, all, packs, k, whole_end);
+      if (end_at >= 0) {
+        float f[1] = {element(end_at, outside)};
+        all += f[0];
+        take(v, f);
       }
       if (threadIdx.x == 0 && sl.at >= 0)
         zt = element(sl.at, (sl.at < kP && sl.head_outside) || (sl.at >= whole_end * kP && sl.tail_outside));
@@ -864,29 +873,24 @@ __global__ void __launch_bounds__(kWorkers + 32, kRowBlocksPerSm)
       }
       const Base base(v.m);
       const float c0 = sl.inside ? factor : NAN, scale = __fdividef(c0, v.s), other = -share * c0;
-      k = whole + threadIdx.x;
-      for (; k + (kTurn - 1) * kWorkers < whole_end; k += kTurn * kWorkers) {
+      for (k = whole + threadIdx.x; k < whole_end; k += 3 * WORKERS) {
+        uint4 raw[3];
 #pragma unroll
-        for (int i = 0; i < kTurn; ++i) {
+        for (int i = 0; i < 3; ++i) raw[i] = packs[min(k + i * WORKERS, whole_end - 1)];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          if (k + i * WORKERS >= whole_end) continue;
           float f[kP];
-          unpack<T>(packs[k + i * kWorkers], f);
+          unpack<T>(raw[i], f);
           gradient_pack<T>(f, base, scale, other);
-          out[k + i * kWorkers] = pack<T>(f);
+          out[k + i * WORKERS] = pack<T>(f);
         }
-      }
-      for (; k < whole_end; k += kWorkers) {
-        float f[kP];
-        unpack<T>(packs[k], f);
-        gradient_pack<T>(f, base, scale, other);
-        out[k] = pack<T>(f);
       }
       if (threadIdx.x == sl.owner)  // after its pack
         static_cast<T*>(sl.out)[sl.at] = from_f32<T>(fmaf(base.exp(element(sl.at, false)), scale, other) - hit * c0);
-      if (end_pack >= 0) {
-        for (int pos = max(end_pack * kP, sl.low); pos < min(end_pack * kP + kP, sl.high); ++pos)
-          static_cast<T*>(sl.out)[pos] =
-              from_f32<T>(fmaf(base.exp(element(pos, outside)), scale, other) - (pos == sl.at ? hit * c0 : 0.f));
-      }
+      if (end_at >= 0)
+        static_cast<T*>(sl.out)[end_at] =
+            from_f32<T>(fmaf(base.exp(element(end_at, outside)), scale, other) - (end_at == sl.at ? hit * c0 : 0.f));
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.empty[stage]);
@@ -1024,14 +1028,14 @@ Left launch_stream(const Args<T>& a, Workspace* ws, cudaStream_t s) {
 constexpr int64_t kRoom = 212 * 1024;  // of an SM's shared memory, for the slices of all its blocks
 constexpr int64_t kFewRows = 74;       // so few rows leave half of the SMs without a block
 
-template <typename T, bool CLUSTER, bool SMOOTH>
+template <typename T, int WORKERS, int PER_SM, bool CLUSTER, bool SMOOTH>
 bool launch_rows(const Args<T>& a, int64_t blocks, int stages, int slice_packs, int cluster, cudaStream_t s) {
-  auto kernel = rows_kernel<T, CLUSTER, SMOOTH>;
+  auto kernel = rows_kernel<T, WORKERS, PER_SM, CLUSTER, SMOOTH>;
   const size_t smem = static_cast<size_t>(stages) * slice_packs * 16;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return false;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(kWorkers + 32);
+  cfg.blockDim = dim3(WORKERS + 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
@@ -1041,6 +1045,23 @@ bool launch_rows(const Args<T>& a, int64_t blocks, int stages, int slice_packs, 
   cfg.attrs = &attr;
   cfg.numAttrs = CLUSTER ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, a, stages, slice_packs, cluster) == cudaSuccess;
+}
+
+// Slices of this many packs, WORKERS threads and up to PER_SM blocks on an SM. Returns the blocks.
+template <typename T, int WORKERS, int PER_SM>
+int run_rows(const Args<T>& a, int slice, int cluster, cudaStream_t s) {
+  int per_sm = PER_SM;
+  while (per_sm > 1 && 2 * 16ll * slice * per_sm > kRoom) --per_sm;
+  const int64_t fit = kRoom / per_sm / (16ll * slice);
+  const int stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
+  int64_t clusters = 148 * per_sm / cluster;
+  if (clusters > a.rows) clusters = a.rows;
+  const int64_t blocks = clusters * cluster;
+  const bool smooth = a.smoothing != 0.f;
+  bool done;
+  if (cluster > 1) done = smooth ? launch_rows<T, WORKERS, PER_SM, true, true>(a, blocks, stages, slice, cluster, s) : launch_rows<T, WORKERS, PER_SM, true, false>(a, blocks, stages, slice, cluster, s);
+  else done = smooth ? launch_rows<T, WORKERS, PER_SM, false, true>(a, blocks, stages, slice, cluster, s) : launch_rows<T, WORKERS, PER_SM, false, false>(a, blocks, stages, slice, cluster, s);
+  return done ? static_cast<int>(blocks) : -1;
 }
 
 // Returns the blocks that left a partial.
@@ -1062,31 +1083,30 @@ int launch_warp_rows(const Args<T>& a, cudaStream_t s) {
   return blocks;
 }
 
-// Both at once, where rows_kernel can: slices of all blocks fit, twice (one that is worked on, one
-// that is on its way), and gradient and logits lie alike against 16 bytes. Returns the partials, or 0.
+// Both at once, where rows_kernel can: gradient and logits lie alike against 16 bytes, and two slices
+// (one that is worked on, one on its way) fit the block's shared memory. A row is one block's, but for
+// few rows, which a cluster of blocks shares; longer rows in greater number are read twice instead
+// (1500 x 60000 f32: 186 us, 236 with clusters of eight). Returns the partials, or 0.
 template <typename T>
 int launch_both(const Args<T>& a, cudaStream_t s) {
   const bool alike = (a.stride - a.grad_stride) % kPack<T> == 0 &&
                      ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
   const int64_t packs = (a.vocab + 2 * (kPack<T> - 1)) / kPack<T>;
-  if (!alike || 2 * 16 * packs > kRoom * kMaxCluster) return 0;
+  if (!alike || 2 * 16 * packs > kRoom * (a.rows <= kFewRows ? kMaxCluster : 1)) return 0;
   int cluster = 1;
-  while (cluster < kMaxCluster && (2 * 16 * ((packs + cluster - 1) / cluster) > kRoom || (a.rows * cluster <= kFewRows && packs >= 1024 * cluster)))
+  while (cluster < kMaxCluster && a.rows * cluster <= kFewRows &&
+         (2 * 16 * ((packs + cluster - 1) / cluster) > kRoom || packs >= 1024 * cluster))
     cluster *= 2;
   const int slice = static_cast<int>((packs + cluster - 1) / cluster);
   if (2 * 16ll * slice > kRoom) return 0;
-  int per_sm = kRowBlocksPerSm;
-  while (per_sm > 1 && 2 * 16ll * slice * per_sm > kRoom) --per_sm;
-  const int64_t fit = kRoom / per_sm / (16ll * slice);
-  const int stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
-  int64_t clusters = 148 * per_sm / cluster;
-  if (clusters > a.rows) clusters = a.rows;
-  const int64_t blocks = clusters * cluster;
-  const bool smooth = a.smoothing != 0.f;
-  bool done;
-  if (cluster > 1) done = smooth ? launch_rows<T, true, true>(a, blocks, stages, slice, cluster, s) : launch_rows<T, true, false>(a, blocks, stages, slice, cluster, s);
-  else done = smooth ? launch_rows<T, false, true>(a, blocks, stages, slice, cluster, s) : launch_rows<T, false, false>(a, blocks, stages, slice, cluster, s);
-  return done ? static_cast<int>(blocks) : -1;
+  // Threads by the slice's length: some eight packs each, so that what a row costs apart from its packs
+  // is spread over them, and as many blocks as an SM then holds. (4096 x 16384 bf16: 52.5 us with 256
+  // threads and three blocks, 57.8 with 128 and six, 66 with 480 and two; 16000 x 2500: 53 with 64 and
+  // eight, 69 with 128 and six, 105 with 256 and three.)
+  if (slice <= 600) return run_rows<T, 64, 8>(a, slice, cluster, s);
+  if (slice <= 1200) return run_rows<T, 128, 6>(a, slice, cluster, s);
+  if (slice <= 2400) return run_rows<T, 256, 3>(a, slice, cluster, s);
+  return run_rows<T, 480, 2>(a, slice, cluster, s);
 }
 
 // Where many rows have to be counted for the gradient's factor, a kernel of its own does it first.
