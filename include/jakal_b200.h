@@ -439,7 +439,7 @@ int jk_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const void
 /* Bytes of the workspace of jk_cross_entropy_forward and _backward. */
 int64_t jk_cross_entropy_workspace(int64_t rows);
 
-/* Softmax cross entropy of logits [rows, vocab] (dtype) against targets int64 [rows]:
+/* Softmax cross entropy of logits [rows, vocab] (dtype, vocab <= 2^30) against targets int64 [rows]:
  *   lse = log sum_j exp(z_j),  loss = lse - (1 - a) z_target - a E_j[z_j]   (a = label_smoothing)
  * A row whose target is ignore_index is not read and has loss, lse and gradient 0; a target
  * outside [0, vocab) gives its row a NaN loss and gradient (nothing is read there). Logits of

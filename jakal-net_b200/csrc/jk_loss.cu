@@ -10,12 +10,14 @@
 // hardware's exponential, with r = m log2(e) rounded once and carried along; where that product
 // would leave the type's range (logits of the order of its largest value), it is taken of z - m.
 //
-// Bound: memory, one read of the logits and one write of the gradient. Two forms:
+// Bound: memory, one read of the logits and one write of the gradient; for 16-bit logits with a
+// gradient the exponentials, two a logit, come near it. Three forms:
 //   * warp_kernel, rows of up to 1024 logits: a warp has a row in its registers;
-//   * ring_kernel, longer rows: a cluster of blocks has a row, each block a slice of it in shared
-//     memory, brought there by bulk copies that run rows ahead of the arithmetic; the gradient is
-//     taken from the same copy, so the logits are read once however long the row is. Rows that
-//     eight blocks cannot hold go through stream_kernel, which reads them again.
+//   * rows_kernel, loss and gradient of longer rows: a block has a row (of few rows, a cluster of
+//     blocks shares each) in shared memory, brought there by bulk copies that run rows ahead of the
+//     arithmetic, and takes the gradient from the same copy, so the logits are read once;
+//   * stream_kernel, the loss alone, or the gradient from the lse, and both one after the other where
+//     rows_kernel does not have the room: the packs of all rows in equal runs, one for each warp.
 #include "jk_host.h"
 #include "jk_rows.cuh"
 #include "jk_sm100.cuh"

@@ -113,12 +113,6 @@ __device__ __forceinline__ void bulk_load(void* dst_smem, const void* src, uint3
                "l"(src), "r"(bytes), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
                : "memory");
 }
-// And back, as part of the thread's current bulk group.
-__device__ __forceinline__ void bulk_store(void* dst, const void* src_smem, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
-               "r"(static_cast<uint32_t>(__cvta_generic_to_shared(src_smem))), "r"(bytes)
-               : "memory");
-}
 
 // Programmatic dependent launch: a kernel launched with the attribute may begin while the one
 // before it in the stream still runs; grid_dependency_wait returns when that one has finished

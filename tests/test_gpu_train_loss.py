@@ -306,8 +306,9 @@ def test_gradient_against_differences(jk):
     assert slack < 0.1 * along.abs() + 0.05, "the differences say nothing"
 
 
-def test_streams_and_graphs(jk):
-    logits, targets = data(64, 1000, torch.bfloat16, 4)
+@pytest.mark.parametrize("rows,vocab", [(64, 1000), (20, 600), (300, 5001), (2, 60000), (90, 150000)])
+def test_streams_and_graphs(jk, rows, vocab):
+    logits, targets = data(rows, vocab, torch.bfloat16, 4)
     want, want_grad = jk.cross_entropy_with_grad_cuda(logits, targets)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -318,8 +319,13 @@ def test_streams_and_graphs(jk):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         got, got_grad = jk.cross_entropy_with_grad_cuda(logits, targets)
+        alone, lse = jk.cross_entropy_forward_cuda(logits, targets)
+        back = jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), logits, targets, lse)
     graph.replay()
     assert torch.equal(got, want) and torch.equal(got_grad, want_grad)
+    want_alone, want_lse = jk.cross_entropy_forward_cuda(logits, targets)
+    assert torch.equal(alone, want_alone) and torch.equal(lse, want_lse)
+    assert torch.equal(back, jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), logits, targets, lse))
 
 
 def test_refusals(jk):
