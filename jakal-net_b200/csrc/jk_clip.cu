@@ -365,7 +365,8 @@ inline int64_t chunks_of(const Call& q, int64_t i) {
   return packs <= kChunkPacks ? 1 : (packs + kChunkPacks - 1) / kChunkPacks;
 }
 
-// Tensors [from, ...) into the table until it is full; returns the next tensor.
+// Tensors [from, ...) into the table until it is full; returns the next one that is not empty, or
+// `count`: another call for the rest would find something, and leaves a table that holds all as it is.
 template <int N>
 int64_t fill(Table<N>& t, const Call& q, int64_t from) {
   int n = 0;
@@ -384,6 +385,7 @@ int64_t fill(Table<N>& t, const Call& q, int64_t from) {
   }
   t.first[n] = chunk;
   t.count = n;
+  while (from < q.count && q.numels[from] == 0) ++from;
   return from;
 }
 

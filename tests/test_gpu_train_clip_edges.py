@@ -1,0 +1,45 @@
+"""Gradient clipping over lists with empty tensors in every place."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def jk():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    import jakal_net_b200
+
+    return jakal_net_b200
+
+
+@pytest.mark.parametrize("full,before,after", [(640, 0, 1), (640, 0, 100), (640, 3, 700), (640, 0, 0), (1280, 0, 1), (1280, 2, 650),
+                                               (641, 1, 1), (64, 0, 1), (64, 600, 1), (3, 0, 700), (0, 0, 700)])
+def test_empty_tensors_anywhere(jk, full, before, after):
+    """Empty shards among the gradients, as many full ones as a launch's table holds."""
+    def empties(n):
+        return [torch.empty(0, device="cuda") for _ in range(n)]
+
+    def some():
+        return [torch.full((i % 7 + 1,), 0.5, device="cuda") for i in range(full)]
+
+    count = sum(i % 7 + 1 for i in range(full))
+    norm = 0.5 * math.sqrt(count)
+    for norm_type, want in ((2.0, norm), (math.inf, 0.5 if full else 0.0)):
+        grads = some()
+        total = jk.clip_grad_norm_(empties(before) + grads + empties(after), 0.25 * want, norm_type)
+        assert abs(total.item() - want) <= 40 * U * want
+        assert all(((g - 0.125).abs() <= 0.125 * 64 * U + 1e-6).all() for g in grads)
+        grads, outs = some(), [torch.empty_like(g) for g in some()]
+        total = jk.clip_grad_norm_(empties(before) + grads + empties(after), 0.25 * want, norm_type,
+                                   out=empties(before) + outs + empties(after))
+        assert abs(total.item() - want) <= 40 * U * want
+        assert all(((g - 0.125).abs() <= 0.125 * 64 * U + 1e-6).all() for g in outs)
+        assert all((g == 0.5).all() for g in grads)
