@@ -7,8 +7,9 @@
 // With the maximum at hand, loss = log sum exp(z - m) + (1 - a) (m - z_t) + a (m - E_j[z_j]) and
 // softmax_j = exp(z_j - m) / sum: differences from m keep their digits where m is large, which
 // lse = m + log(sum), one f32 number, does not. exp(z - m) is 2^(z log2(e) - r), one fma and the
-// hardware's exponential, with r = m log2(e) rounded once and carried along; where that product
-// would leave the type's range (logits of the order of its largest value), it is taken of z - m.
+// hardware's exponential, with r = m log2(e) rounded once and carried along. What r is short of that
+// product is a factor of the whole sum, of up to 2^(half a unit in r's last place): beyond |m| = 2^23
+// it would be more than 2 (and out of range from 2^31 on), so there it is taken of z - m instead.
 //
 // Bound: memory, one read of the logits and one write of the gradient; for 16-bit logits with a
 // gradient the exponentials, two a logit, come near it. Three forms:
@@ -99,13 +100,13 @@ __device__ __forceinline__ float pack_max(const uint4 (&raw)[N]) {
   }
 }
 
-// The reference of a sum of exponentials: exp(z - m) as 2^(z log2(e) - r).
-constexpr float kHuge = 1e38f;
+// The reference of a sum of exponentials: exp(z - m) as 2^(z log2(e) - r) while r is good to one half.
+constexpr float kFar = 8388608.f;  // r < 2^24
 struct Base {
   float m, r;
-  bool near;  // m log2(e) is finite
+  bool near;
 
-  __device__ __forceinline__ explicit Base(float m_) : m(m_), r(product(m_, kLog2e)), near(fabsf(m_) < kHuge) {}
+  __device__ __forceinline__ explicit Base(float m_) : m(m_), r(product(m_, kLog2e)), near(fabsf(m_) < kFar) {}
   __device__ __forceinline__ float exp_near(float z) const { return exp2_approx(fmaf(z, kLog2e, -r)); }
   __device__ __forceinline__ float exp_far(float z) const { return exp2_approx((z - m) * kLog2e); }
   __device__ __forceinline__ float exp(float z) const { return near ? exp_near(z) : exp_far(z); }
@@ -130,11 +131,11 @@ struct Sum {
   float m, s;
 };
 
-// What a sum on maximum `from` is worth on a larger one. (Where only `from` is far, it is far
-// below, and both forms give 0.)
+// What a sum on maximum `from` is worth on a larger one: 2^-r counts for a near one, exp(-m) for a far one.
 __device__ __forceinline__ float factor_to(float from, float to) {
-  const Base b(to);
-  return b.near ? exp2_approx(product(from, kLog2e) - b.r) : b.exp_far(from);
+  const Base a(from), b(to);
+  if (a.near) return b.near ? exp2_approx(a.r - b.r) : b.exp_far(from) * expf(a.rest());
+  return b.exp(from);
 }
 
 __device__ __forceinline__ float warp_max32(float v) {
