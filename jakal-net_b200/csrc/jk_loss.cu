@@ -134,8 +134,8 @@ struct Sum {
 // What a sum on maximum `from` is worth on a larger one: 2^-r counts for a near one, exp(-m) for a far one.
 __device__ __forceinline__ float factor_to(float from, float to) {
   const Base a(from), b(to);
-  if (a.near) return b.near ? exp2_approx(a.r - b.r) : b.exp_far(from) * expf(a.rest());
-  return b.exp(from);
+  if (b.near) return exp2_approx(a.near ? a.r - b.r : fmaf(from, kLog2e, -b.r));
+  return exp2_approx(fmaf(from - to, kLog2e, a.near ? fmaf(-from, kLog2e, a.r) : 0.f));
 }
 
 __device__ __forceinline__ float warp_max32(float v) {
