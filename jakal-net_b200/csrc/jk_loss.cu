@@ -52,9 +52,9 @@ struct Args {
   int reduction;
   float scale;             // of the gradient (forward)
   const float* grad_loss;  // backward
-  const float* lse_in;
+  const float *lse_in, *low_in;  // low: what an lse in one f32 is short of the log-sum (null: 0)
   float* losses;
-  float* lse_out;
+  float *lse_out, *low_out;
   T* grad;
   int64_t grad_stride;
   Partial* partials;
@@ -277,16 +277,26 @@ __device__ __forceinline__ float gradient_factor(const Args<T>& a, bool forward,
   return c / static_cast<float>(n);
 }
 
-// A row's loss and log-sum from its sum, target logit and sum of logits.
+// A row's loss and log-sum (lse + low) from its sum, target logit and sum of logits.
 struct RowLoss {
-  float loss, lse;
+  float loss, lse, low;
   __device__ __forceinline__ RowLoss(Sum v, float zt, float all, float smoothing, int64_t vocab) {
     const float log_sum = logf(v.s) + Base(v.m).rest();  // ln sum exp(z - m)
     loss = log_sum + (1.f - smoothing) * (v.m - zt);
     if (smoothing != 0.f) loss += smoothing * (v.m - all / static_cast<float>(vocab));
     lse = v.m + log_sum;
+    const float t = lse - v.m;
+    low = (v.m - (lse - t)) + (log_sum - t);
   }
 };
+
+// Row r's results, of those that are asked for (LOW: of a loss alone, whose gradient may follow).
+template <bool LOW, typename T>
+__device__ __forceinline__ void leave_row(const Args<T>& a, int64_t r, float loss, float lse, float low) {
+  if (a.losses != nullptr) a.losses[r] = loss;
+  if (a.lse_out != nullptr) a.lse_out[r] = lse;
+  if (LOW && a.low_out != nullptr) a.low_out[r] = low;
+}
 
 // ---------------------------------------------------------------- short rows
 // A warp per row, N turns of VEC neighbouring elements per lane. So few rows as kOneBlockRows are one
@@ -357,24 +367,20 @@ __global__ void __launch_bounds__(THREADS) warp_kernel(const Args<T> a) {
       v.s = warp_sum32(v.s);
       if (a.smoothing != 0.f) all = warp_sum32(all);
       const RowLoss l(v, zt, all, a.smoothing, vocab);
-      if (lane == 0) {
-        if (a.losses != nullptr) a.losses[r] = l.loss;
-        if (a.lse_out != nullptr) a.lse_out[r] = l.lse;
-      }
+      if (lane == 0) leave_row<MODE == kLoss>(a, r, l.loss, l.lse, l.low);
       part.sum += l.loss;
       part.rows += 1;
       scale = factor / v.s;
       __syncwarp();  // z[target] is read before an in-place gradient replaces it
     } else if (ignored && MODE != kBackward && lane == 0) {
-      if (a.losses != nullptr) a.losses[r] = 0.f;
-      if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
+      leave_row<MODE == kLoss>(a, r, 0.f, 0.f, 0.f);
     }
     if (MODE == kLoss) continue;
     float c0 = ignored ? 0.f : factor;
     if (MODE == kBackward && !ignored) {
       m = a.lse_in[r];
       if (a.reduction == JK_REDUCE_NONE) c0 = a.grad_loss[r];
-      scale = c0 * expf(Base(m).rest());
+      scale = c0 * expf(Base(m).rest() - (a.low_in != nullptr ? a.low_in[r] : 0.f));
     }
     if (!ignored && !inside) scale = c0 = NAN;
     const Base from(m);
@@ -452,7 +458,7 @@ struct Item {
   int64_t row, target;
   const T* z;
   int piece, shift;
-  float value, grad_loss;  // the target's logit (kLoss), or the row's lse
+  float value, low, grad_loss;  // the target's logit (kLoss), or the row's lse
   bool ignored, inside;
 };
 
@@ -496,6 +502,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
     if (MODE == kLoss && piece == 0) it.value = it.inside ? to_f32(w.z[it.target]) : NAN;
     if (MODE != kLoss) {
       it.value = a.lse_in[row];
+      it.low = a.low_in != nullptr ? a.low_in[row] : 0.f;
       if (MODE == kBackward && a.reduction == JK_REDUCE_NONE) it.grad_loss = a.grad_loss[row];
     }
   };
@@ -576,10 +583,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
           if (a.smoothing != 0.f) all = warp_sum32(all);
           if (last && from_start) {
             const RowLoss l(v, zt, all, a.smoothing, vocab);
-            if (lane == 0) {
-              if (a.losses != nullptr) a.losses[q.row] = l.loss;
-              if (a.lse_out != nullptr) a.lse_out[q.row] = l.lse;
-            }
+            if (lane == 0) leave_row<true>(a, q.row, l.loss, l.lse, l.low);
             part.sum += l.loss;
             part.rows += 1;
           } else {
@@ -591,15 +595,14 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
           all = 0.f;
         }
       } else if (last && lane == 0) {
-        if (a.losses != nullptr) a.losses[q.row] = 0.f;
-        if (a.lse_out != nullptr) a.lse_out[q.row] = 0.f;
+        leave_row<true>(a, q.row, 0.f, 0.f, 0.f);
       }
     } else {
       T* g = a.grad + q.row * a.grad_stride;
       const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(q.z)) & 15) == 0;
       const Base base(q.value);
       const float k0 = !q.inside ? NAN : MODE == kBackward && a.reduction == JK_REDUCE_NONE ? q.grad_loss : factor;
-      const float scale = k0 * expf(base.rest()), other = -share * k0;
+      const float scale = k0 * expf(base.rest() - q.low), other = -share * k0;
       const bool whole = alike && interior(q);
 #pragma unroll
       for (int i = 0; i < kTurn; ++i) {
@@ -827,10 +830,7 @@ __global__ void __launch_bounds__(WORKERS + 32, PER_SM)
     if (sl.ignored) {
       for (int k = whole + threadIdx.x; k < whole_end; k += WORKERS) out[k] = make_uint4(0, 0, 0, 0);
       if (end_at >= 0) static_cast<T*>(sl.out)[end_at] = from_f32<T>(0.f);
-      if (threadIdx.x == 0 && rank == 0) {
-        if (a.losses != nullptr) a.losses[r] = 0.f;
-        if (a.lse_out != nullptr) a.lse_out[r] = 0.f;
-      }
+      if (threadIdx.x == 0 && rank == 0) leave_row<false>(a, r, 0.f, 0.f, 0.f);
     } else {
       Sum v{-INFINITY, 0.f};
       float all = 0.f, zt = 0.f;
@@ -869,8 +869,7 @@ __global__ void __launch_bounds__(WORKERS + 32, PER_SM)
       ++joins;
       if (threadIdx.x == 0 && rank == 0) {
         const RowLoss l(v, sl.inside ? zt : NAN, all, a.smoothing, a.vocab);
-        if (a.losses != nullptr) a.losses[r] = l.loss;
-        if (a.lse_out != nullptr) a.lse_out[r] = l.lse;
+        leave_row<false>(a, r, l.loss, l.lse, l.low);
         sum += l.loss;
         ++counted;
       }
@@ -959,8 +958,7 @@ __global__ void __launch_bounds__(256)
       all += q.all;
     }
     const RowLoss l(v, zt, all, a.smoothing, a.vocab);
-    if (a.losses != nullptr) a.losses[head.row] = l.loss;
-    if (a.lse_out != nullptr) a.lse_out[head.row] = l.lse;
+    leave_row<true>(a, head.row, l.loss, l.lse, l.low);
     p.sum += l.loss;
     p.rows += 1;
   }
@@ -1147,7 +1145,10 @@ int forward(Args<T> a, float* loss, Workspace* ws, cudaStream_t s) {
       }
       if (left.partials == 0) {
         gradient_later = a.grad != nullptr;
-        if (gradient_later && a.lse_out == nullptr) a.lse_out = reinterpret_cast<float*>(ws + 1);
+        if (gradient_later) {  // from the log-sum, kept in two parts: one f32 does not tell its neighbours apart far from 0
+          if (a.lse_out == nullptr) a.lse_out = reinterpret_cast<float*>(ws + 1);
+          a.low_out = reinterpret_cast<float*>(ws + 1) + a.rows;
+        }
         left = launch_stream<T, kLoss>(a, ws, s);
       }
     }
@@ -1158,6 +1159,7 @@ int forward(Args<T> a, float* loss, Workspace* ws, cudaStream_t s) {
   }
   if (gradient_later) {
     a.lse_in = a.lse_out;
+    a.low_in = a.low_out;
     launch_stream<T, kLater>(a, ws, s);
   }
   return launch_status();
@@ -1170,8 +1172,8 @@ JK_ERROR_READER(read_error_loss)
 }  // namespace jk
 
 extern "C" int64_t jk_cross_entropy_workspace(int64_t rows) {
-  // and a log-sum of each row, for a gradient that is taken in a second pass
-  return rows <= 0 ? 0 : static_cast<int64_t>(sizeof(jk::loss::Workspace)) + (rows + 1) / 2 * 8;
+  // and a log-sum of each row, in two parts, for a gradient that is taken in a second pass
+  return rows <= 0 ? 0 : static_cast<int64_t>(sizeof(jk::loss::Workspace)) + rows * 8;
 }
 
 extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
@@ -1191,7 +1193,7 @@ extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_strid
   if (st != JK_OK) return st;
   JK_WITH_TYPE(dtype, T, {
     const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
-                          label_smoothing, reduction, grad_scale, nullptr, nullptr, losses, lse,
+                          label_smoothing, reduction, grad_scale, nullptr, nullptr, nullptr, losses, lse, nullptr,
                           static_cast<T*>(grad), grad_stride, nullptr, nullptr, nullptr};
     st = loss::forward<T>(a, loss, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });
@@ -1216,7 +1218,7 @@ extern "C" int jk_cross_entropy_backward(const float* grad_loss, const void* log
   if (st != JK_OK) return st;
   JK_WITH_TYPE(dtype, T, {
     const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
-                          label_smoothing, reduction, 1.f, grad_loss, lse, nullptr, nullptr, static_cast<T*>(grad),
+                          label_smoothing, reduction, 1.f, grad_loss, lse, nullptr, nullptr, nullptr, nullptr, static_cast<T*>(grad),
                           grad_stride, nullptr, nullptr, nullptr};
     st = loss::backward<T>(a, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });

@@ -125,3 +125,17 @@ def test_maxima_on_both_sides_of_where_the_reference_changes(jk, vocab, sign):
     within(got, loss, e_loss, "losses")
     _, gr = jk.cross_entropy_with_grad_cuda(z, targets, reduction="sum")
     within(gr, *stored(grad, e_grad, torch.float32), "gradient in the same pass")
+
+
+@pytest.mark.parametrize("times,vocab,dtype", [(2, 40000, torch.float32), (2, 70001, torch.bfloat16)])
+def test_rows_read_twice_have_the_gradient_of_rows_read_once(jk, times, vocab, dtype):
+    z, targets = rows_of(times, vocab, dtype, 3)
+    (loss, grad), (e_loss, e_grad), (_, log_sum, _, p, _) = exact(z, targets)
+    # the softmax comes from the log-sum, kept to twice f32's digits: log sum's own rounding beside the sum's
+    e_grad = e_grad + p * 6 * U * (log_sum[:, None] + 1)
+    got, g = jk.cross_entropy_with_grad_cuda(z, targets, reduction="sum")
+    within(got, loss.sum(), e_loss.sum() + 4 * U * loss.sum(), "sum")
+    within(g, *stored(grad, e_grad, dtype), "gradient")
+    over = z.clone()
+    got_in, _ = jk.cross_entropy_with_grad_cuda(over, targets, reduction="sum", in_place=True)
+    assert torch.equal(got_in, got) and torch.equal(over, g)
