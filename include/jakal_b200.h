@@ -465,6 +465,20 @@ int jk_cross_entropy_backward(const float* grad_loss, const void* logits, int64_
                               int64_t ignore_index, float label_smoothing, int reduction, void* grad,
                               int64_t grad_stride, void* workspace, jk_stream_t stream);
 
+/* The same two with the log-sum kept in two f32, lse + lse_low (f32 [rows]; lse_low may be NULL, as 0):
+ * a gradient from one f32 is off by a factor of exp(half a unit in its last place), which matters for
+ * logits far from 0 (2^-11 at 1e4; at 1e8 neighbouring logits are not told apart). The forward form is
+ * the loss alone. */
+int jk_cross_entropy_forward_split(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
+                                   int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                                   int reduction, float* losses, float* lse, float* lse_low, float* loss,
+                                   void* workspace, jk_stream_t stream);
+int jk_cross_entropy_backward_split(const float* grad_loss, const void* logits, int64_t logits_stride,
+                                    const int64_t* targets, const float* lse, const float* lse_low, int64_t rows,
+                                    int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                                    int reduction, void* grad, int64_t grad_stride, void* workspace,
+                                    jk_stream_t stream);
+
 /* norm codes of jk_clip_grad_norm */
 #define JK_NORM_2 0
 #define JK_NORM_INF 1

@@ -1171,17 +1171,13 @@ JK_ERROR_READER(read_error_loss)
 
 }  // namespace jk
 
-extern "C" int64_t jk_cross_entropy_workspace(int64_t rows) {
-  // and a log-sum of each row, in two parts, for a gradient that is taken in a second pass
-  return rows <= 0 ? 0 : static_cast<int64_t>(sizeof(jk::loss::Workspace)) + rows * 8;
-}
+namespace jk {
+namespace loss {
 
-extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
-                                        int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
-                                        int reduction, float grad_scale, float* losses, float* lse, float* loss,
-                                        void* grad, int64_t grad_stride, void* workspace, jk_stream_t stream) {
-  using namespace jk;
-  if (rows < 0 || vocab <= 0 || vocab > loss::kMaxVocab || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
+int checked_forward(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows, int64_t vocab, int dtype,
+                    int64_t ignore_index, float label_smoothing, int reduction, float grad_scale, float* losses, float* lse,
+                    float* lse_low, float* loss, void* grad, int64_t grad_stride, void* workspace, jk_stream_t stream) {
+  if (rows < 0 || vocab <= 0 || vocab > kMaxVocab || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
   if (!float_dtype(dtype)) return JK_ERR_BAD_DTYPE;
   if (reduction < JK_REDUCE_NONE || reduction > JK_REDUCE_SUM) return JK_ERR_UNSUPPORTED_KIND;
   if (!(label_smoothing >= 0.f && label_smoothing <= 1.f)) return JK_ERR_BAD_ARG;
@@ -1192,20 +1188,18 @@ extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_strid
   int st = check_device();
   if (st != JK_OK) return st;
   JK_WITH_TYPE(dtype, T, {
-    const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
-                          label_smoothing, reduction, grad_scale, nullptr, nullptr, nullptr, losses, lse, nullptr,
-                          static_cast<T*>(grad), grad_stride, nullptr, nullptr, nullptr};
-    st = loss::forward<T>(a, loss, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+    const Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
+                    label_smoothing, reduction, grad_scale, nullptr, nullptr, nullptr, losses, lse, lse_low,
+                    static_cast<T*>(grad), grad_stride, nullptr, nullptr, nullptr};
+    st = forward<T>(a, loss, static_cast<Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });
   return st;
 }
 
-extern "C" int jk_cross_entropy_backward(const float* grad_loss, const void* logits, int64_t logits_stride,
-                                         const int64_t* targets, const float* lse, int64_t rows, int64_t vocab, int dtype,
-                                         int64_t ignore_index, float label_smoothing, int reduction, void* grad,
-                                         int64_t grad_stride, void* workspace, jk_stream_t stream) {
-  using namespace jk;
-  if (rows < 0 || vocab <= 0 || vocab > loss::kMaxVocab || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
+int checked_backward(const float* grad_loss, const void* logits, int64_t logits_stride, const int64_t* targets, const float* lse,
+                     const float* lse_low, int64_t rows, int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                     int reduction, void* grad, int64_t grad_stride, void* workspace, jk_stream_t stream) {
+  if (rows < 0 || vocab <= 0 || vocab > kMaxVocab || logits_stride < 0 || grad_stride < 0) return JK_ERR_BAD_SHAPE;
   if (!float_dtype(dtype)) return JK_ERR_BAD_DTYPE;
   if (reduction < JK_REDUCE_NONE || reduction > JK_REDUCE_SUM) return JK_ERR_UNSUPPORTED_KIND;
   if (!(label_smoothing >= 0.f && label_smoothing <= 1.f)) return JK_ERR_BAD_ARG;
@@ -1217,10 +1211,51 @@ extern "C" int jk_cross_entropy_backward(const float* grad_loss, const void* log
   int st = check_device();
   if (st != JK_OK) return st;
   JK_WITH_TYPE(dtype, T, {
-    const loss::Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
-                          label_smoothing, reduction, 1.f, grad_loss, lse, nullptr, nullptr, nullptr, nullptr, static_cast<T*>(grad),
-                          grad_stride, nullptr, nullptr, nullptr};
-    st = loss::backward<T>(a, static_cast<loss::Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+    const Args<T> a{static_cast<const T*>(logits), logits_stride, targets, rows, vocab, ignore_index,
+                    label_smoothing, reduction, 1.f, grad_loss, lse, lse_low, nullptr, nullptr, nullptr, static_cast<T*>(grad),
+                    grad_stride, nullptr, nullptr, nullptr};
+    st = backward<T>(a, static_cast<Workspace*>(workspace), reinterpret_cast<cudaStream_t>(stream));
   });
   return st;
+}
+
+}  // namespace loss
+}  // namespace jk
+
+extern "C" int64_t jk_cross_entropy_workspace(int64_t rows) {
+  // and a log-sum of each row, in two parts, for a gradient that is taken in a second pass
+  return rows <= 0 ? 0 : static_cast<int64_t>(sizeof(jk::loss::Workspace)) + rows * 8;
+}
+
+extern "C" int jk_cross_entropy_forward(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
+                                        int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                                        int reduction, float grad_scale, float* losses, float* lse, float* loss,
+                                        void* grad, int64_t grad_stride, void* workspace, jk_stream_t stream) {
+  return jk::loss::checked_forward(logits, logits_stride, targets, rows, vocab, dtype, ignore_index, label_smoothing, reduction,
+                                   grad_scale, losses, lse, nullptr, loss, grad, grad_stride, workspace, stream);
+}
+
+extern "C" int jk_cross_entropy_forward_split(const void* logits, int64_t logits_stride, const int64_t* targets, int64_t rows,
+                                              int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                                              int reduction, float* losses, float* lse, float* lse_low, float* loss,
+                                              void* workspace, jk_stream_t stream) {
+  return jk::loss::checked_forward(logits, logits_stride, targets, rows, vocab, dtype, ignore_index, label_smoothing, reduction,
+                                   1.f, losses, lse, lse_low, loss, nullptr, 0, workspace, stream);
+}
+
+extern "C" int jk_cross_entropy_backward(const float* grad_loss, const void* logits, int64_t logits_stride,
+                                         const int64_t* targets, const float* lse, int64_t rows, int64_t vocab, int dtype,
+                                         int64_t ignore_index, float label_smoothing, int reduction, void* grad,
+                                         int64_t grad_stride, void* workspace, jk_stream_t stream) {
+  return jk::loss::checked_backward(grad_loss, logits, logits_stride, targets, lse, nullptr, rows, vocab, dtype, ignore_index,
+                                    label_smoothing, reduction, grad, grad_stride, workspace, stream);
+}
+
+extern "C" int jk_cross_entropy_backward_split(const float* grad_loss, const void* logits, int64_t logits_stride,
+                                               const int64_t* targets, const float* lse, const float* lse_low, int64_t rows,
+                                               int64_t vocab, int dtype, int64_t ignore_index, float label_smoothing,
+                                               int reduction, void* grad, int64_t grad_stride, void* workspace,
+                                               jk_stream_t stream) {
+  return jk::loss::checked_backward(grad_loss, logits, logits_stride, targets, lse, lse_low, rows, vocab, dtype, ignore_index,
+                                    label_smoothing, reduction, grad, grad_stride, workspace, stream);
 }

@@ -142,6 +142,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _i64, _p, _p, _i64, _i64, _i32,  # grad_loss, logits, stride, targets, lse, rows, vocab, dtype
          _i64, _f32, _i32, _p, _i64, _p, _p],     # ignore_index, label_smoothing, reduction, grad, stride, workspace, stream
     ),
+    "jk_cross_entropy_forward_split": (
+        _i32,
+        [_p, _i64, _p, _i64, _i64, _i32, _i64,  # logits, stride, targets, rows, vocab, dtype, ignore_index
+         _f32, _i32, _p, _p, _p, _p, _p, _p],   # label_smoothing, reduction, losses, lse, lse_low, loss, workspace, stream
+    ),
+    "jk_cross_entropy_backward_split": (
+        _i32,
+        [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i32,  # grad_loss, logits, stride, targets, lse, lse_low, rows, vocab, dtype
+         _i64, _f32, _i32, _p, _i64, _p, _p],         # ignore_index, label_smoothing, reduction, grad, stride, workspace, stream
+    ),
     "jk_clip_grad_norm_workspace": (_i64, []),
     "jk_clip_grad_norm": (
         _i32,

@@ -312,6 +312,21 @@ def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, gr
     return loss, lse
 
 
+def _cross_entropy_split(logits, targets, ignore_index, label_smoothing, reduction):
+    """(loss, log-sums): the latter as two f32 each, [2, *targets.shape], whose sum they are."""
+    code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
+    rows, device = targets.numel(), logits.device
+    lse = torch.empty((2, *targets.shape), dtype=torch.float32, device=device)
+    each = kind == _lib.JK_REDUCE_NONE
+    loss = _empty(targets.shape if each else (), torch.float32, device)
+    work = _empty((_LIBRARY.jk_cross_entropy_workspace(rows) // 4,), torch.float32, device)
+    at = loss.data_ptr()
+    _call(_LIBRARY.jk_cross_entropy_forward_split, "jk_cross_entropy_forward_split", logits.get_device(), lr.data_ptr(), stride,
+          targets.data_ptr(), rows, logits.shape[-1], code, ignore_index, label_smoothing, kind, at if each else None,
+          lse.data_ptr(), lse.data_ptr() + 4 * rows, None if each else at, work.data_ptr())
+    return loss, lse
+
+
 def cross_entropy_forward_cuda(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
                                reduction: str = "mean"):
     """Softmax cross entropy of logits [..., vocab] against int64 (or int32) targets [...].
@@ -356,7 +371,12 @@ def cross_entropy_backward_cuda(grad_loss: Tensor, logits: Tensor, targets: Tens
                                 label_smoothing: float = 0.0, reduction: str = "mean"):
     """Gradient of ``cross_entropy_forward_cuda`` with respect to the logits, in their dtype,
     from the lse that it returned and the loss's gradient (a scalar, or of targets' shape for
-    reduction "none")."""
+    reduction "none"). One f32 lse leaves the softmax off by a factor of exp(half a unit in its
+    last place), 2^-11 for logits of the order of 1e4; the other forms do not go through it."""
+    return _cross_entropy_backward(grad_loss, logits, targets, lse, None, int(ignore_index), float(label_smoothing), reduction)
+
+
+def _cross_entropy_backward(grad_loss, logits, targets, lse, low, ignore_index, label_smoothing, reduction):
     code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
     for name, t in (("lse", lse), ("grad_loss", grad_loss)):
         if not isinstance(t, Tensor) or t.device != logits.device:
@@ -369,16 +389,16 @@ def cross_entropy_backward_cuda(grad_loss: Tensor, logits: Tensor, targets: Tens
     lse = lse.contiguous()
     grad = _grad_like(logits)
     work = _empty((_LIBRARY.jk_cross_entropy_workspace(targets.numel()) // 4,), torch.float32, logits.device)
-    _call(_LIBRARY.jk_cross_entropy_backward, "jk_cross_entropy_backward", logits.get_device(), gl.data_ptr(), lr.data_ptr(),
-          stride, targets.data_ptr(), lse.data_ptr(), targets.numel(), logits.shape[-1], code, int(ignore_index),
-          float(label_smoothing), kind, grad.data_ptr(), _rows(grad)[1], work.data_ptr())
+    _call(_LIBRARY.jk_cross_entropy_backward_split, "jk_cross_entropy_backward_split", logits.get_device(), gl.data_ptr(),
+          lr.data_ptr(), stride, targets.data_ptr(), lse.data_ptr(), _ptr(low), targets.numel(), logits.shape[-1], code,
+          ignore_index, label_smoothing, kind, grad.data_ptr(), _rows(grad)[1], work.data_ptr())
     return grad
 
 
 class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index, label_smoothing, reduction):
-        loss, lse = cross_entropy_forward_cuda(logits, targets, ignore_index, label_smoothing, reduction)
+        loss, lse = _cross_entropy_split(logits, targets, ignore_index, label_smoothing, reduction)
         ctx.save_for_backward(logits, targets, lse)
         ctx.options = (ignore_index, label_smoothing, reduction)
         return loss
@@ -387,14 +407,14 @@ class _CrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, targets, lse = ctx.saved_tensors
-        return cross_entropy_backward_cuda(grad_loss, logits, targets, lse, *ctx.options), None, None, None, None
+        return _cross_entropy_backward(grad_loss, logits, targets, lse[0], lse[1], *ctx.options), None, None, None, None
 
 
 def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
                   reduction: str = "mean") -> Tensor:
-    """Differentiable softmax cross entropy (f32): ``cross_entropy_forward_cuda`` and, in the
-    backward pass, ``cross_entropy_backward_cuda``. A loop that owns its backward pass reads the
-    logits once less with ``cross_entropy_with_grad_cuda``."""
+    """Differentiable softmax cross entropy (f32): the loss of ``cross_entropy_forward_cuda`` and, in
+    the backward pass, the gradient from the log-sum, which is kept in two f32. A loop that owns its
+    backward pass reads the logits once less with ``cross_entropy_with_grad_cuda``."""
     return _CrossEntropy.apply(logits, targets, int(ignore_index), float(label_smoothing), reduction)
 
 

@@ -139,3 +139,16 @@ def test_rows_read_twice_have_the_gradient_of_rows_read_once(jk, times, vocab, d
     over = z.clone()
     got_in, _ = jk.cross_entropy_with_grad_cuda(over, targets, reduction="sum", in_place=True)
     assert torch.equal(got_in, got) and torch.equal(over, g)
+
+
+@pytest.mark.parametrize("vocab", [40, 1001, 5000, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_autograd_at_any_magnitude(jk, vocab, dtype):
+    z, targets = rows_of(1, vocab, dtype, 5)
+    (loss, grad), (e_loss, e_grad), (_, log_sum, _, p, _) = exact(z, targets)
+    e_grad = e_grad + p * 6 * U * (log_sum[:, None] + 1)
+    leaf = z.clone().requires_grad_(True)
+    out = jk.cross_entropy(leaf, targets, reduction="none")
+    within(out.detach(), loss, e_loss, "losses")
+    out.sum().backward()
+    within(leaf.grad, *stored(grad, e_grad, dtype), "gradient")
