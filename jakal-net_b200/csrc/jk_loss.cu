@@ -4,12 +4,14 @@
 //   loss = lse - (1 - a) z_t - a E_j[z_j]
 //   grad_j = c (exp(z_j - lse) - (1 - a) [j = t] - a / V),  c = scale / number of rows that count
 //
-// With the maximum at hand, loss = log sum exp(z - m) + (1 - a) (m - z_t) + a (m - E_j[z_j]) and
+// With the maximum at hand, loss = log sum exp(z - m) + (1 - a) (m - z_t) + a E_j[m - z_j] and
 // softmax_j = exp(z_j - m) / sum: differences from m keep their digits where m is large, which
 // lse = m + log(sum), one f32 number, does not. exp(z - m) is 2^(z log2(e) - r), one fma and the
 // hardware's exponential, with r = m log2(e) rounded once and carried along. What r is short of that
 // product is a factor of the whole sum, of up to 2^(half a unit in r's last place): beyond |m| = 2^23
-// it would be more than 2 (and out of range from 2^31 on), so there it is taken of z - m instead.
+// it would be more than 2 (and out of range from 2^31 on), so there it is taken of z - m instead. The
+// mean distance from m comes from the same exponents (4096 x 16384 bf16 with gradient and smoothing:
+// 62 us, 104 when it took the logits once more; f32: 104 against 106).
 //
 // Bound: memory, one read of the logits and one write of the gradient; for 16-bit logits with a
 // gradient the exponentials, two a logit, come near it. Three forms:
@@ -110,8 +112,9 @@ struct Base {
   __device__ __forceinline__ float exp_near(float z) const { return exp2_approx(fmaf(z, kLog2e, -r)); }
   __device__ __forceinline__ float exp_far(float z) const { return exp2_approx((z - m) * kLog2e); }
   __device__ __forceinline__ float exp(float z) const { return near ? exp_near(z) : exp_far(z); }
-  // ln of what 2^-r is short of exp(-m)
-  __device__ __forceinline__ float rest() const { return near ? kLn2 * fmaf(-m, kLog2e, r) : 0.f; }
+  // What 2^-r is short of exp(-m), as a power of 2 (near only) and of e.
+  __device__ __forceinline__ float short_of() const { return fmaf(-m, kLog2e, r); }
+  __device__ __forceinline__ float rest() const { return near ? kLn2 * short_of() : 0.f; }
 };
 
 // Replaces N logits by their exponentials.
@@ -172,43 +175,71 @@ __device__ __forceinline__ void take(Sum& v, float (&z)[N]) {
   for (int i = 0; i < N; ++i) v.s += z[i];
 }
 
-template <typename T, int N>
-__device__ __forceinline__ float pack_sum(const uint4 (&raw)[N]) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float f[kPack<T>];
-    unpack<T>(raw[i], f);
-#pragma unroll
-    for (int j = 0; j < kPack<T>; ++j) s += f[j];
-  }
-  return s;
-}
+// The scale of a Gap, a power of two that is less than 1 / (2 vocab): the sum stays in f32's range.
+__device__ __forceinline__ float gap_scale(int vocab) { return __uint_as_float(static_cast<uint32_t>(94 + __clz(vocab)) << 23); }
 
-// The same for N packs. All maxima first: 16 logits or more share one comparison and one factor.
-template <typename T, int N>
-__device__ __forceinline__ void take_packs(Sum& v, const uint4 (&raw)[N]) {
+// For label smoothing: the sum of (z - m) * scale over n logits, m being their maximum so far. All terms
+// have one sign, so the sum keeps its digits wherever m is, which a sum of logits would not.
+struct Gap {
+  float sum;
+  int n;
+
+  // m has grown
+  __device__ __forceinline__ void move(float from, float to, float scale) {
+    if (n > 0 && from != to) sum = fmaf(static_cast<float>(n), fmaf(from, scale, -to * scale), sum);
+  }
+  __device__ __forceinline__ void add(float z, float m, float scale) {
+    sum += fmaf(z, scale, m == -INFINITY ? 0.f : -m * scale);  // where all are -inf, so is the sum
+    ++n;
+  }
+  // Over a warp whose lanes had maxima `from`.
+  __device__ __forceinline__ void join(float from, float to, float scale) {
+    move(from, to, scale);
+    sum = warp_sum32(sum);
+    n = __reduce_add_sync(0xffffffffu, n);
+  }
+};
+
+// Adds N packs to a thread's sum and, with GAP, the first `whole` of them to its gap (the others are
+// all -inf); again(i) is pack i once more. All maxima first: 16 logits or more share one comparison
+// and one factor.
+template <typename T, bool GAP, int N, typename Again>
+__device__ __forceinline__ void take_packs(Sum& v, const uint4 (&raw)[N], Gap& gap, float scale, int whole, Again&& again) {
   const float top = pack_max<T>(raw);
   if (top > v.m) {
     v.s *= factor_to(v.m, top);
+    if (GAP) gap.move(v.m, top, scale);
     v.m = top;
   }
-  const Base b(v.m == -INFINITY ? 0.f : v.m);
+  const float m = v.m == -INFINITY ? 0.f : v.m;
+  const Base b(m);
+  float g = -INFINITY;  // of the gap, in powers of 2: the exponents are at hand
   if (b.near) {
     const uint64_t l2e = pair(kLog2e, kLog2e), minus_r = pair(-b.r, -b.r);
-    uint64_t s = pair(v.s, 0.f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
+    uint64_t s = pair(v.s, 0.f), x_sum = 0;
+    const auto take_pack = [&](const uint4& u) {
       float f[kPack<T>];
-      unpack<T>(raw[i], f);
+      unpack<T>(u, f);
 #pragma unroll
       for (int j = 0; j < kPack<T>; j += 2) {
-        const float2 x = unpair(fma2(pair(f[j], f[j + 1]), l2e, minus_r));
+        const uint64_t x2 = fma2(pair(f[j], f[j + 1]), l2e, minus_r);
+        const float2 x = unpair(x2);
         s = add2(s, pair(exp2_approx(x.x), exp2_approx(x.y)));
+        if (GAP) x_sum = add2(x_sum, x2);
       }
+    };
+    if (!GAP || whole == N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) take_pack(raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < whole) take_pack(raw[i]);
     }
-    const float2 both = unpair(s);
+    float2 both = unpair(s);
     v.s = both.x + both.y;
+    both = unpair(x_sum);
+    if (GAP) g = fmaf(static_cast<float>(whole * kPack<T>), b.short_of(), both.x + both.y);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -216,6 +247,21 @@ __device__ __forceinline__ void take_packs(Sum& v, const uint4 (&raw)[N]) {
       unpack<T>(raw[i], f);
 #pragma unroll
       for (int j = 0; j < kPack<T>; ++j) v.s += b.exp_far(f[j]);
+    }
+  }
+  if (GAP) {
+    gap.n += whole * kPack<T>;
+    if (g > -1e38f) {
+      gap.sum = fmaf(g, kLn2 * scale, gap.sum);
+    } else {  // the exponents have left f32's range, or are not at hand
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i >= whole) continue;
+        float f[kPack<T>];
+        unpack<T>(again(i), f);
+#pragma unroll
+        for (int j = 0; j < kPack<T>; ++j) gap.sum += fmaf(f[j], scale, -m * scale);
+      }
     }
   }
 }
@@ -277,13 +323,13 @@ __device__ __forceinline__ float gradient_factor(const Args<T>& a, bool forward,
   return c / static_cast<float>(n);
 }
 
-// A row's loss and log-sum (lse + low) from its sum, target logit and sum of logits.
+// A row's loss and log-sum (lse + low) from its sum, target logit and Gap's sum.
 struct RowLoss {
   float loss, lse, low;
-  __device__ __forceinline__ RowLoss(Sum v, float zt, float all, float smoothing, int64_t vocab) {
+  __device__ __forceinline__ RowLoss(Sum v, float zt, float gap, float smoothing, int vocab) {
     const float log_sum = logf(v.s) + Base(v.m).rest();  // ln sum exp(z - m)
     loss = log_sum + (1.f - smoothing) * (v.m - zt);
-    if (smoothing != 0.f) loss += smoothing * (v.m - all / static_cast<float>(vocab));
+    if (smoothing != 0.f) loss -= smoothing * gap / (gap_scale(vocab) * static_cast<float>(vocab));
     lse = v.m + log_sum;
     const float t = lse - v.m;
     low = (v.m - (lse - t)) + (log_sum - t);
@@ -346,7 +392,6 @@ __global__ void __launch_bounds__(THREADS) warp_kernel(const Args<T> a) {
     if (!ignored && MODE != kBackward) {
       const float zt = inside ? to_f32(z[target]) : NAN;
       Sum v{-INFINITY, 0.f};
-      float all = 0.f;
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -354,19 +399,30 @@ __global__ void __launch_bounds__(THREADS) warp_kernel(const Args<T> a) {
         for (int j = 0; j < VEC; ++j) top = fmaxf(top, f[i][j]);
       v.m = top = warp_max32(top);
       const Base base(top);
+      float gap = 0.f;  // of the exponents, then of the logits
 #pragma unroll
       for (int i = 0; i < N; ++i) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const int c = (i * 32 + lane) * VEC + j;
-          if (a.smoothing != 0.f && c < vocab) all += f[i][j];
+          const bool has = (i * 32 + lane) * VEC + j < vocab;
+          if (a.smoothing != 0.f) gap += has ? fmaf(f[i][j], kLog2e, -base.r) : 0.f;
           f[i][j] = base.exp(f[i][j]);
-          v.s += c < vocab ? f[i][j] : 0.f;
+          v.s += has ? f[i][j] : 0.f;
         }
       }
       v.s = warp_sum32(v.s);
-      if (a.smoothing != 0.f) all = warp_sum32(all);
-      const RowLoss l(v, zt, all, a.smoothing, vocab);
+      if (a.smoothing != 0.f) {
+        const float by = gap_scale(vocab);
+        gap = fmaf(static_cast<float>(vocab), base.short_of(), warp_sum32(gap));
+        if (base.near && gap > -1e38f) {
+          gap *= kLn2 * by;
+        } else {  // the exponents have left f32's range
+          gap = 0.f;
+          for (int c = lane; c < vocab; c += 32) gap += fmaf(to_f32(z[c]), by, -top * by);
+          gap = warp_sum32(gap);
+        }
+      }
+      const RowLoss l(v, zt, gap, a.smoothing, vocab);
       if (lane == 0) leave_row<MODE == kLoss>(a, r, l.loss, l.lse, l.low);
       part.sum += l.loss;
       part.rows += 1;
@@ -449,7 +505,8 @@ constexpr int kPiece = 32 * kTurn;  // packs
 
 struct Record {
   int64_t row;  // -1: none
-  float m, s, all;
+  float m, s, gap;
+  int n;  // logits in it, if smoothing asks
 };
 
 // A piece of a row.
@@ -462,7 +519,7 @@ struct Item {
   bool ignored, inside;
 };
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool SMOOTH>
 __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
     stream_kernel(const Args<T> a, int pieces, Record* records, int* come) {
   __shared__ int scratch[kStreamThreads / 32];
@@ -536,7 +593,9 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
   }
 
   Sum v{-INFINITY, 0.f};
-  float all = 0.f, zt = 0.f;
+  Gap gap{0.f, 0};
+  const float gap_by = gap_scale(vocab);
+  float zt = 0.f;
   bool from_start = false, recorded[2] = {false, false};
   Partial part{0.0, 0};
   while (item < end) {
@@ -561,38 +620,42 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocksPerSm)
     const bool last = q.piece == pieces - 1;
     if (MODE == kLoss) {
       if (!q.ignored) {
-        take_packs<T>(v, raw);
-        if (a.smoothing != 0.f) {
-          if (interior(q)) {
-            all += pack_sum<T>(raw);
-          } else {
+        const bool whole = interior(q);
+        const float before = v.m;
+        if (SMOOTH && whole) {
+          take_packs<T, true>(v, raw, gap, gap_by, kTurn, [&](int i) { return raw[i]; });
+        } else {
+          take_packs<T, false>(v, raw, gap, 0.f, 0, [&](int i) { return raw[i]; });
+        }
+        if (SMOOTH && !whole) {
+          gap.move(before, v.m, gap_by);
 #pragma unroll
-            for (int i = 0; i < kTurn; ++i) {
-              float f[kP];
-              unpack<T>(raw[i], f);
+          for (int i = 0; i < kTurn; ++i) {
+            float f[kP];
+            unpack<T>(raw[i], f);
 #pragma unroll
-              for (int j = 0; j < kP; ++j) {
-                const int c = c0 + i * 32 * kP + j;
-                all += c >= 0 && c < vocab ? f[j] : 0.f;
-              }
+            for (int j = 0; j < kP; ++j) {
+              const int c = c0 + i * 32 * kP + j;
+              if (c >= 0 && c < vocab) gap.add(f[j], v.m, gap_by);
             }
           }
         }
         if (last || item == end) {
+          const float mine = v.m;
           v = warp_join(v);
-          if (a.smoothing != 0.f) all = warp_sum32(all);
+          if (SMOOTH) gap.join(mine, v.m, gap_by);
           if (last && from_start) {
-            const RowLoss l(v, zt, all, a.smoothing, vocab);
+            const RowLoss l(v, zt, gap.sum, a.smoothing, vocab);
             if (lane == 0) leave_row<true>(a, q.row, l.loss, l.lse, l.low);
             part.sum += l.loss;
             part.rows += 1;
           } else {
             const int slot = q.row == first_row ? 0 : 1;
             recorded[slot] = true;
-            if (lane == 0) records[2 * warp + slot] = {q.row, v.m, v.s, all};
+            if (lane == 0) records[2 * warp + slot] = {q.row, v.m, v.s, gap.sum, gap.n};
           }
           v = {-INFINITY, 0.f};
-          all = 0.f;
+          gap = {0.f, 0};
         }
       } else if (last && lane == 0) {
         leave_row<true>(a, q.row, 0.f, 0.f, 0.f);
@@ -661,7 +724,7 @@ struct Slice {
 struct Shared {
   uint64_t full[kMaxStages], empty[kMaxStages], joined[2];
   Slice slice[kMaxStages];
-  float4 warp[2][kMaxWorkers / 32];  // (m, s, target logit, sum of logits) of each warp
+  float4 warp[2][kMaxWorkers / 32];  // (m, s, target logit, gap) of each warp
   float4 peer[2][kMaxCluster];    // and of each block of the cluster
   int counts[kMaxWorkers / 32];
 };
@@ -673,6 +736,9 @@ __device__ __forceinline__ uint32_t map_peer(const void* p, int rank) {
 }
 __device__ __forceinline__ void store_peer(uint32_t addr, float4 v) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void store_peer(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void arrive_peer(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -758,7 +824,7 @@ __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsign
 
 // Adds packs k, k + WORKERS, ... (N of them, those before `end`) to a thread's sum.
 template <typename T, int WORKERS, bool SMOOTH, int N>
-__device__ __forceinline__ void sum_turn(Sum& v, float& all, const uint4* packs, int k, int end) {
+__device__ __forceinline__ void sum_turn(Sum& v, Gap& gap, float gap_by, const uint4* packs, int k, int end) {
   const T low = minus_inf<T>();
   uint32_t two;
   if constexpr (sizeof(T) == 4) two = __float_as_uint(low);
@@ -766,14 +832,9 @@ __device__ __forceinline__ void sum_turn(Sum& v, float& all, const uint4* packs,
   uint4 raw[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) raw[i] = k + i * WORKERS < end ? packs[k + i * WORKERS] : make_uint4(two, two, two, two);
-  take_packs<T>(v, raw);
-  if (SMOOTH) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint4 one[1] = {raw[i]};
-      if (k + i * WORKERS < end) all += pack_sum<T>(one);
-    }
-  }
+  const int left = end - k;  // packs of this thread lie WORKERS apart
+  take_packs<T, SMOOTH>(v, raw, gap, gap_by, left <= 0 ? 0 : min((left + WORKERS - 1) / WORKERS, N),
+                        [&](int i) { return packs[k + i * WORKERS]; });
 }
 
 template <typename T, int WORKERS, int PER_SM, bool CLUSTER, bool SMOOTH>
@@ -781,6 +842,7 @@ __global__ void __launch_bounds__(WORKERS + 32, PER_SM)
     rows_kernel(const Args<T> a, int stages, int slice_packs, int cluster_size) {
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ Shared sh;
+  __shared__ int gap_counts[SMOOTH ? 2 : 1][kMaxWorkers / 32 + kMaxCluster];  // of the gaps in sh.warp and sh.peer
   constexpr int kP = kPack<T>, kWarps = WORKERS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cluster = CLUSTER ? cluster_size : 1;
@@ -806,6 +868,7 @@ __global__ void __launch_bounds__(WORKERS + 32, PER_SM)
   const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); };
   const float factor = gradient_factor(a, true, WORKERS, sh.counts, sync);
   const float hit = 1.f - a.smoothing, share = SMOOTH ? a.smoothing / static_cast<float>(a.vocab) : 0.f;
+  const float gap_by = SMOOTH ? gap_scale(static_cast<int>(a.vocab)) : 0.f;
   bool good = true;
   double sum = 0.0;
   int counted = 0, stage = 0, joins = 0;
@@ -833,42 +896,58 @@ __global__ void __launch_bounds__(WORKERS + 32, PER_SM)
       if (threadIdx.x == 0 && rank == 0) leave_row<false>(a, r, 0.f, 0.f, 0.f);
     } else {
       Sum v{-INFINITY, 0.f};
-      float all = 0.f, zt = 0.f;
+      Gap gap{0.f, 0};
+      float zt = 0.f;
       // turns of kTurn packs while they are mostly full, then of two
       int k = whole + threadIdx.x, left = (whole_end - whole + WORKERS - 1) / WORKERS;
-      for (; left > kTurn / 2; left -= kTurn, k += kTurn * WORKERS) sum_turn<T, WORKERS, SMOOTH, kTurn>(v, all, packs, k, whole_end);
-      for (; left > 0; left -= 2, k += 2 * WORKERS) sum_turn<T, WORKERS, SMOOTH, 2>(v, all, packs, k, whole_end);
+      for (; left > kTurn / 2; left -= kTurn, k += kTurn * WORKERS) sum_turn<T, WORKERS, SMOOTH, kTurn>(v, gap, gap_by, packs, k, whole_end);
+      for (; left > 0; left -= 2, k += 2 * WORKERS) sum_turn<T, WORKERS, SMOOTH, 2>(v, gap, gap_by, packs, k, whole_end);
       if (end_at >= 0) {
-        float f[1] = {element(end_at, outside)};
-        all += f[0];
+        const float z = element(end_at, outside), before = v.m;
+        float f[1] = {z};
         take(v, f);
+        if (SMOOTH) {
+          gap.move(before, v.m, gap_by);
+          gap.add(z, v.m, gap_by);
+        }
       }
       if (threadIdx.x == 0 && sl.at >= 0)
         zt = element(sl.at, (sl.at < kP && sl.head_outside) || (sl.at >= whole_end * kP && sl.tail_outside));
+      const float mine = v.m;
       v = warp_join(v);
-      if (SMOOTH) all = warp_sum32(all);
+      if (SMOOTH) gap.join(mine, v.m, gap_by);
       // of three rows that count, the warps of a block are never in the first and the third at once
-      if (lane == 0) sh.warp[joins & 1][warp] = make_float4(v.m, v.s, zt, all);
+      if (lane == 0) {
+        sh.warp[joins & 1][warp] = make_float4(v.m, v.s, zt, gap.sum);
+        if (SMOOTH) gap_counts[joins & 1][warp] = gap.n;
+      }
       sync();
       float4 q = lane < kWarps ? sh.warp[joins & 1][lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
       v = warp_join({q.x, q.y});
-      if (SMOOTH) all = warp_sum32(q.w);
+      if (SMOOTH) {
+        gap = {q.w, lane < kWarps ? gap_counts[joins & 1][lane] : 0};
+        gap.join(q.x, v.m, gap_by);
+      }
       zt = q.z;  // of the first warp's first thread
       if (CLUSTER) {  // neither are the blocks of a cluster, so a slot and a barrier are free again
         zt = __shfl_sync(0xffffffffu, zt, 0);
         if (threadIdx.x < cluster) {
-          store_peer(map_peer(&sh.peer[joins & 1][rank], threadIdx.x), make_float4(v.m, v.s, zt, all));
+          store_peer(map_peer(&sh.peer[joins & 1][rank], threadIdx.x), make_float4(v.m, v.s, zt, gap.sum));
+          if (SMOOTH) store_peer(map_peer(&gap_counts[joins & 1][kMaxWorkers / 32 + rank], threadIdx.x), gap.n);
           arrive_peer(map_peer(&sh.joined[joins & 1], threadIdx.x));
         }
         if (good) good = wait_cluster(&sh.joined[joins & 1], (joins >> 1) & 1);
         q = lane < cluster ? sh.peer[joins & 1][lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
         v = warp_join({q.x, q.y});
         zt = warp_sum32(q.z);
-        if (SMOOTH) all = warp_sum32(q.w);
+        if (SMOOTH) {
+          gap = {q.w, lane < cluster ? gap_counts[joins & 1][kMaxWorkers / 32 + lane] : 0};
+          gap.join(q.x, v.m, gap_by);
+        }
       }
       ++joins;
       if (threadIdx.x == 0 && rank == 0) {
-        const RowLoss l(v, sl.inside ? zt : NAN, all, a.smoothing, a.vocab);
+        const RowLoss l(v, sl.inside ? zt : NAN, gap.sum, a.smoothing, static_cast<int>(a.vocab));
         leave_row<false>(a, r, l.loss, l.lse, l.low);
         sum += l.loss;
         ++counted;
@@ -943,7 +1022,8 @@ __global__ void __launch_bounds__(256)
     const bool begun = (i >= 1 && records[i - 1].row == head.row) || (i >= 2 && records[i - 2].row == head.row);
     if (begun) continue;
     Sum v{head.m, head.s};
-    float all = head.all;
+    Gap gap{head.gap, head.n};
+    const float gap_by = gap_scale(static_cast<int>(a.vocab));
     for (int j = i + 1, unused = 0; j < record_count && unused < 2; ++j) {
       const Record q = records[j];
       if (q.row < 0) {
@@ -954,10 +1034,14 @@ __global__ void __launch_bounds__(256)
       unused = 0;
       const float m = fmaxf(v.m, q.m);
       const float f = v.m == m ? 1.f : factor_to(v.m, m), g = q.m == m ? 1.f : factor_to(q.m, m);
+      Gap other{q.gap, q.n};
+      gap.move(v.m, m, gap_by);
+      other.move(q.m, m, gap_by);
+      gap.sum += other.sum;
+      gap.n += other.n;
       v = {m, v.s * f + q.s * g};
-      all += q.all;
     }
-    const RowLoss l(v, zt, all, a.smoothing, a.vocab);
+    const RowLoss l(v, zt, gap.sum, a.smoothing, static_cast<int>(a.vocab));
     leave_row<true>(a, head.row, l.loss, l.lse, l.low);
     p.sum += l.loss;
     p.rows += 1;
@@ -1022,7 +1106,10 @@ Left launch_stream(const Args<T>& a, Workspace* ws, cudaStream_t s) {
   // a run of four pieces or more keeps the records of a row few
   const int64_t want = (a.rows * pieces + 4 * (kStreamThreads / 32) - 1) / (4 * (kStreamThreads / 32));
   const int blocks = static_cast<int>(want < 148 * kStreamBlocksPerSm ? want : 148 * kStreamBlocksPerSm);
-  stream_kernel<T, MODE><<<blocks, kStreamThreads, 0, s>>>(a, pieces, ws->records, &ws->ticket.come);
+  if (MODE == kLoss && a.smoothing != 0.f)
+    stream_kernel<T, MODE, MODE == kLoss><<<blocks, kStreamThreads, 0, s>>>(a, pieces, ws->records, &ws->ticket.come);
+  else
+    stream_kernel<T, MODE, false><<<blocks, kStreamThreads, 0, s>>>(a, pieces, ws->records, &ws->ticket.come);
   return {blocks * (kStreamThreads / 32), 2 * blocks * (kStreamThreads / 32)};
 }
 

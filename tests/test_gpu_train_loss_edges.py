@@ -7,6 +7,8 @@ log-sum by the sum's relative error; the result type rounds once (2^-8 bf16). No
 depends on the magnitude of the logits themselves."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -152,3 +154,31 @@ def test_autograd_at_any_magnitude(jk, vocab, dtype):
     within(out.detach(), loss, e_loss, "losses")
     out.sum().backward()
     within(leaf.grad, *stored(grad, e_grad, dtype), "gradient")
+
+
+@pytest.mark.parametrize("times,vocab", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_label_smoothing_at_any_magnitude(jk, times, vocab, dtype):
+    """The mean of the logits enters the loss as the mean of their distances from the maximum."""
+    z, targets = rows_of(times, vocab, dtype, vocab + 2)
+    lowest = torch.finfo(dtype).min
+    z[0] = lowest                     # a row masked as a whole
+    z[1, : vocab // 2] = lowest       # half of a row masked: a finite loss in f32's range
+    (loss, grad), (e_loss, e_grad), _ = exact(z, targets, 0.1)
+    got, _ = jk.cross_entropy_forward_cuda(z, targets, label_smoothing=0.1, reduction="none")
+    within(got, loss, e_loss, "losses")
+    got, g = jk.cross_entropy_with_grad_cuda(z[2:], targets[2:], label_smoothing=0.1, reduction="sum")
+    within(got, loss[2:].sum(), e_loss[2:].sum() + 4 * U * loss[2:].sum(), "sum")
+    within(g, *stored(grad[2:], e_grad[2:], dtype), "gradient in the same pass")
+
+
+@pytest.mark.parametrize("vocab", [40, 1000, 5000])
+def test_smoothing_over_logits_of_minus_infinity(jk, vocab):
+    z = torch.randn(3, vocab, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    z[0, vocab // 2] = -math.inf
+    z[1, 0] = -math.inf
+    targets = torch.tensor([1, 1, 1], device="cuda")
+    got, _ = jk.cross_entropy_forward_cuda(z, targets, label_smoothing=0.1, reduction="none")
+    assert got[0] == math.inf and got[1] == math.inf and got[2].isfinite()
+    got, g = jk.cross_entropy_with_grad_cuda(z, targets, label_smoothing=0.1, reduction="sum")
+    assert got == math.inf and g.isfinite().all()
