@@ -443,7 +443,7 @@ int64_t jk_cross_entropy_workspace(int64_t rows);
  *   lse = log sum_j exp(z_j),  loss = lse - (1 - a) z_target - a E_j[z_j]   (a = label_smoothing)
  * A row whose target is ignore_index is not read and has loss, lse and gradient 0; a target
  * outside [0, vocab) gives its row a NaN loss and gradient (nothing is read there). Logits of
- * -inf have probability 0; a row of nothing else has a NaN loss.
+ * -inf have probability 0; a row of nothing else has a NaN loss and gradient and an lse of -inf.
  * out: losses f32 [rows] and lse f32 [rows] (each may be NULL), loss f32 scalar by `reduction`
  * (NULL with JK_REDUCE_NONE; the mean over no row is NaN, the sum 0), and, when grad is not NULL
  * (not with JK_REDUCE_NONE), grad [rows, vocab] in dtype, in the same pass over the logits:

@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(THREADS) warp_kernel(const Args<T> a) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) top = fmaxf(top, f[i][j]);
       v.m = top = warp_max32(top);
-      const Base base(top);
+      const Base base(top == -INFINITY ? 0.f : top);  // the sum of nothing but exp(-inf) is 0, its log -inf
       float gap = 0.f;  // of the exponents, then of the logits
 #pragma unroll
       for (int i = 0; i < N; ++i) {

@@ -182,3 +182,19 @@ def test_smoothing_over_logits_of_minus_infinity(jk, vocab):
     assert got[0] == math.inf and got[1] == math.inf and got[2].isfinite()
     got, g = jk.cross_entropy_with_grad_cuda(z, targets, label_smoothing=0.1, reduction="sum")
     assert got == math.inf and g.isfinite().all()
+
+
+@pytest.mark.parametrize("vocab", [40, 1000, 1001, 5000, 60000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_of_nothing_but_minus_infinity(jk, vocab, dtype):
+    """log sum exp of nothing is -inf in every form; the loss and the gradient are NaN."""
+    z = torch.randn(5, vocab, device="cuda").to(dtype)
+    z[2] = -math.inf
+    targets = torch.arange(5, device="cuda")
+    loss, lse = jk.cross_entropy_forward_cuda(z, targets, reduction="none")
+    assert lse[2] == -math.inf and loss[2].isnan()
+    assert lse[[0, 1, 3, 4]].isfinite().all() and loss[[0, 1, 3, 4]].isfinite().all()
+    _, g = jk.cross_entropy_with_grad_cuda(z, targets, reduction="sum")
+    back = jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), z, targets, lse, reduction="sum")
+    for got in (g, back):
+        assert got[2].isnan().all() and got[[0, 1, 3, 4]].isfinite().all()
