@@ -277,13 +277,13 @@ def _loss_inputs(logits: Tensor, targets: Tensor, reduction: str):
     return code, targets, kind, lr, stride
 
 
-def _grad_like(logits: Tensor) -> Tensor:
+def _grad_like(logits: Tensor, rows: Tensor, stride: int) -> Tensor:
     """An uninitialised gradient whose rows lie as the logits' rows do, 16-byte blocks and padding
-    between rows included, where those are equally spaced and apart; else a contiguous one."""
+    between rows included, where those are equally spaced and apart; else a contiguous one.
+    (rows, stride): the logits as ``_rows`` has them."""
     shift = logits.data_ptr() % 16
     if logits.is_contiguous() and not shift:
         return torch.empty_like(logits)
-    rows, stride = _rows(logits)
     if logits.numel() == 0 or rows.data_ptr() != logits.data_ptr() or stride < logits.shape[-1]:
         return _empty_like(logits)
     shift //= logits.element_size()
@@ -291,10 +291,13 @@ def _grad_like(logits: Tensor) -> Tensor:
     return logits.new_empty((shift + n * stride,)).as_strided(logits.shape, logits.stride(), shift)
 
 
-def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, grad_scale, want_lse, grad, in_place=False):
+def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, grad_scale, want_lse=False, want_grad=False,
+                   in_place=False):
+    """(loss, lse, gradient), the latter two None where they are not asked for; in_place: the gradient
+    goes over the logits."""
     code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
     rows, device = targets.numel(), logits.device
-    lse = losses = None
+    lse = losses = grad = None
     if kind == _lib.JK_REDUCE_NONE:
         loss = losses = _empty(targets.shape, torch.float32, device)
     else:
@@ -302,14 +305,16 @@ def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, gr
     if want_lse:
         lse = torch.empty_like(loss) if losses is not None else _empty(targets.shape, torch.float32, device)
     work = _empty((_LIBRARY.jk_cross_entropy_workspace(rows) // 4,), torch.float32, device)
+    grad_ptr, grad_stride = None, 0
     if in_place:
         grad_ptr, grad_stride = lr.data_ptr(), stride
-    else:
-        grad_ptr, grad_stride = (None, 0) if grad is None else (grad.data_ptr(), _rows(grad)[1])
+    elif want_grad:
+        grad = _grad_like(logits, lr, stride)
+        grad_ptr, grad_stride = grad.data_ptr(), _rows(grad)[1]
     _call(_LIBRARY.jk_cross_entropy_forward, "jk_cross_entropy_forward", logits.get_device(), lr.data_ptr(), stride,
           targets.data_ptr(), rows, logits.shape[-1], code, ignore_index, label_smoothing, kind, grad_scale, _ptr(losses),
           _ptr(lse), None if losses is not None else loss.data_ptr(), grad_ptr, grad_stride, work.data_ptr())
-    return loss, lse
+    return loss, lse, grad
 
 
 def _cross_entropy_split(logits, targets, ignore_index, label_smoothing, reduction):
@@ -335,7 +340,7 @@ def cross_entropy_forward_cuda(logits: Tensor, targets: Tensor, ignore_index: in
     ignore_index) or "sum", of targets' shape for "none"; lse f32 of targets' shape, the rows'
     log-sum-exp, which ``cross_entropy_backward_cuda`` takes. A row to ignore has loss and lse 0
     and is not read. A target outside the vocabulary gives NaN."""
-    return _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, 1.0, True, None)
+    return _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, 1.0, want_lse=True)[:2]
 
 
 def cross_entropy_with_grad_cuda(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
@@ -357,13 +362,12 @@ def cross_entropy_with_grad_cuda(logits: Tensor, targets: Tensor, ignore_index: 
         lr, stride = _rows(logits)
         if lr.data_ptr() != logits.data_ptr() or (logits.numel() > logits.shape[-1] and stride < logits.shape[-1]):
             raise ValueError("in_place needs logits whose rows are contiguous inside, equally spaced and apart")
-        loss, _ = _cross_entropy(lr, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
-                                 False, None, in_place=True)
+        loss, _, _ = _cross_entropy(lr, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
+                                    in_place=True)
         _written([logits])
         return loss, logits
-    grad = _grad_like(logits)
-    loss, _ = _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
-                             False, grad)
+    loss, _, grad = _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, float(grad_scale),
+                                   want_grad=True)
     return loss, grad
 
 
@@ -387,7 +391,7 @@ def _cross_entropy_backward(grad_loss, logits, targets, lse, low, ignore_index, 
         raise ValueError(f"grad_loss has shape {tuple(grad_loss.shape)}, which does not fit reduction {reduction!r}")
     gl = grad_loss.detach().to(torch.float32).contiguous()
     lse = lse.contiguous()
-    grad = _grad_like(logits)
+    grad = _grad_like(logits, lr, stride)
     work = _empty((_LIBRARY.jk_cross_entropy_workspace(targets.numel()) // 4,), torch.float32, logits.device)
     _call(_LIBRARY.jk_cross_entropy_backward_split, "jk_cross_entropy_backward_split", logits.get_device(), gl.data_ptr(),
           lr.data_ptr(), stride, targets.data_ptr(), lse.data_ptr(), _ptr(low), targets.numel(), logits.shape[-1], code,

@@ -198,3 +198,16 @@ def test_rows_of_nothing_but_minus_infinity(jk, vocab, dtype):
     back = jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), z, targets, lse, reduction="sum")
     for got in (g, back):
         assert got[2].isnan().all() and got[[0, 1, 3, 4]].isfinite().all()
+
+
+def test_logits_that_need_a_copy_are_copied_once(jk):
+    z = torch.randn(4096, 600, device="cuda").t()  # 600 rows of 4096, columns apart
+    targets = torch.zeros(600, dtype=torch.int64, device="cuda")
+    size = z.numel() * 4
+    for call in (lambda: jk.cross_entropy_with_grad_cuda(z, targets, reduction="sum"),
+                 lambda: jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), z, targets, torch.zeros(600, device="cuda"))):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
+        call()
+        made = torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before
+        assert made < 2.5 * size  # the copy and the gradient
