@@ -377,15 +377,16 @@ def cross_entropy_backward_cuda(grad_loss: Tensor, logits: Tensor, targets: Tens
     from the lse that it returned and the loss's gradient (a scalar, or of targets' shape for
     reduction "none"). One f32 lse leaves the softmax off by a factor of exp(half a unit in its
     last place), 2^-11 for logits of the order of 1e4; the other forms do not go through it."""
-    return _cross_entropy_backward(grad_loss, logits, targets, lse, None, int(ignore_index), float(label_smoothing), reduction)
+    return _cross_entropy_backward(grad_loss, logits, targets, lse, int(ignore_index), float(label_smoothing), reduction)
 
 
-def _cross_entropy_backward(grad_loss, logits, targets, lse, low, ignore_index, label_smoothing, reduction):
+def _cross_entropy_backward(grad_loss, logits, targets, lse, ignore_index, label_smoothing, reduction, split=False):
+    """split: lse is what ``_cross_entropy_split`` returned."""
     code, targets, kind, lr, stride = _loss_inputs(logits, targets, reduction)
     for name, t in (("lse", lse), ("grad_loss", grad_loss)):
         if not isinstance(t, Tensor) or t.device != logits.device:
             raise RuntimeError(f"{name} must be a tensor on {logits.device}")
-    if lse.dtype != torch.float32 or lse.shape != targets.shape:
+    if not split and (lse.dtype != torch.float32 or lse.shape != targets.shape):
         raise ValueError(f"lse must be f32 of shape {tuple(targets.shape)}")
     if grad_loss.shape != targets.shape if kind == _lib.JK_REDUCE_NONE else grad_loss.numel() != 1:
         raise ValueError(f"grad_loss has shape {tuple(grad_loss.shape)}, which does not fit reduction {reduction!r}")
@@ -394,8 +395,8 @@ def _cross_entropy_backward(grad_loss, logits, targets, lse, low, ignore_index, 
     grad = _grad_like(logits, lr, stride)
     work = _empty((_LIBRARY.jk_cross_entropy_workspace(targets.numel()) // 4,), torch.float32, logits.device)
     _call(_LIBRARY.jk_cross_entropy_backward_split, "jk_cross_entropy_backward_split", logits.get_device(), gl.data_ptr(),
-          lr.data_ptr(), stride, targets.data_ptr(), lse.data_ptr(), _ptr(low), targets.numel(), logits.shape[-1], code,
-          ignore_index, label_smoothing, kind, grad.data_ptr(), _rows(grad)[1], work.data_ptr())
+          lr.data_ptr(), stride, targets.data_ptr(), lse.data_ptr(), lse.data_ptr() + 4 * targets.numel() if split else None,
+          targets.numel(), logits.shape[-1], code, ignore_index, label_smoothing, kind, grad.data_ptr(), _rows(grad)[1], work.data_ptr())
     return grad
 
 
@@ -411,7 +412,7 @@ class _CrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, targets, lse = ctx.saved_tensors
-        return _cross_entropy_backward(grad_loss, logits, targets, lse[0], lse[1], *ctx.options), None, None, None, None
+        return _cross_entropy_backward(grad_loss, logits, targets, lse, *ctx.options, split=True), None, None, None, None
 
 
 def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
