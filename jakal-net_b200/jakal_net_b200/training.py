@@ -278,17 +278,24 @@ def _loss_inputs(logits: Tensor, targets: Tensor, reduction: str):
 
 
 def _grad_like(logits: Tensor, rows: Tensor, stride: int) -> Tensor:
-    """An uninitialised gradient whose rows lie as the logits' rows do, 16-byte blocks and padding
-    between rows included, where those are equally spaced and apart; else a contiguous one.
+    """An uninitialised gradient whose rows lie against 16-byte blocks as the logits' rows do, where
+    those are equally spaced and apart; else a contiguous one. Rows are spaced as the logits' are while
+    the padding between them is an eighth of a row at most (a padded vocabulary), else (one position
+    of each sequence, a slice of the vocabulary) as closely as that allows.
     (rows, stride): the logits as ``_rows`` has them."""
     shift = logits.data_ptr() % 16
     if logits.is_contiguous() and not shift:
         return torch.empty_like(logits)
-    if logits.numel() == 0 or rows.data_ptr() != logits.data_ptr() or stride < logits.shape[-1]:
+    vocab = logits.shape[-1]
+    if logits.numel() == 0 or rows.data_ptr() != logits.data_ptr() or stride < vocab:
         return _empty_like(logits)
-    shift //= logits.element_size()
-    n = logits.numel() // logits.shape[-1]
-    return logits.new_empty((shift + n * stride,)).as_strided(logits.shape, logits.stride(), shift)
+    size = logits.element_size()
+    shift //= size
+    n = logits.numel() // vocab
+    if stride - vocab <= vocab // 8:
+        return logits.new_empty((shift + n * stride,)).as_strided(logits.shape, logits.stride(), shift)
+    stride = vocab + (stride - vocab) % (16 // size)
+    return logits.new_empty((shift + n * stride,)).as_strided((n, vocab), (stride, 1), shift).view(logits.shape)
 
 
 def _cross_entropy(logits, targets, ignore_index, label_smoothing, reduction, grad_scale, want_lse=False, want_grad=False,
@@ -347,10 +354,10 @@ def cross_entropy_with_grad_cuda(logits: Tensor, targets: Tensor, ignore_index: 
                                  reduction: str = "mean", grad_scale: float = 1.0, in_place: bool = False):
     """The loss ("mean" or "sum") and, in the same pass over the logits, their gradient.
 
-    Returns (loss, grad): grad = grad_scale * d loss / d logits in logits' dtype, its rows spaced
-    as theirs (grad_scale: a loss scaler's factor), for ``logits.backward(grad)`` or a head's own backward. in_place
-    writes it over the logits, which must then have rows that are contiguous inside, equally
-    spaced and apart."""
+    Returns (loss, grad): grad = grad_scale * d loss / d logits in logits' dtype (grad_scale: a loss
+    scaler's factor), for ``logits.backward(grad)`` or a head's own backward; its rows are spaced as
+    theirs where the padding is up to an eighth of a row. in_place writes it over the logits, which must
+    then have rows that are contiguous inside, equally spaced and apart."""
     if reduction == "none":
         raise ValueError("a gradient needs a reduced loss (mean or sum)")
     _check_input("logits", logits)

@@ -200,6 +200,30 @@ def test_rows_of_nothing_but_minus_infinity(jk, vocab, dtype):
         assert got[2].isnan().all() and got[[0, 1, 3, 4]].isfinite().all()
 
 
+def test_gradient_of_a_slice_takes_no_more_memory_than_it_needs(jk):
+    wide = torch.randn(4, 50, 1003, device="cuda").to(torch.bfloat16)
+    targets = torch.randint(0, 1003, (4,), device="cuda")
+    last = wide[:, -1]
+    _, g = jk.cross_entropy_with_grad_cuda(last, targets)
+    assert g.untyped_storage().nbytes() <= 2 * (4 * (1003 + 8) + 8)
+    _, want = jk.cross_entropy_with_grad_cuda(last.contiguous(), targets)
+    assert torch.equal(g, want)
+    _, lse = jk.cross_entropy_forward_cuda(last, targets)
+    back = jk.cross_entropy_backward_cuda(torch.ones((), device="cuda"), last, targets, lse)
+    assert back.untyped_storage().nbytes() <= 2 * (4 * (1003 + 8) + 8)
+    # three dims, an odd start and a vocabulary's slice of many
+    part = torch.randn(3, 5, 40000, device="cuda")[..., 7:307]
+    targets = torch.randint(0, 300, (3, 5), device="cuda")
+    _, g = jk.cross_entropy_with_grad_cuda(part, targets, reduction="sum")
+    assert g.shape == part.shape and g.untyped_storage().nbytes() <= 4 * (15 * (300 + 4) + 4)
+    _, want = jk.cross_entropy_with_grad_cuda(part.contiguous(), targets, reduction="sum")
+    assert torch.allclose(g, want, rtol=2 * (300 / 32 + 64) * U, atol=4 * U)  # other lanes, another order of the sum
+    # a padded vocabulary keeps its rows' spacing
+    padded = torch.randn(6, 1024, device="cuda")[:, :1000]
+    _, g = jk.cross_entropy_with_grad_cuda(padded, torch.zeros(6, dtype=torch.int64, device="cuda"))
+    assert g.stride() == padded.stride()
+
+
 def test_logits_that_need_a_copy_are_copied_once(jk):
     z = torch.randn(4096, 600, device="cuda").t()  # 600 rows of 4096, columns apart
     targets = torch.zeros(600, dtype=torch.int64, device="cuda")
