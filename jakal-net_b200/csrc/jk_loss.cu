@@ -764,8 +764,9 @@ __device__ __forceinline__ void leave(int cluster) {
   if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// The loading warp: slices of rows first, first + step, ... A wait that runs out is recorded, and no
-// later one is waited for: the kernel then ends soon, with an error that jk_device_status reports.
+// The loading warp: slices of rows first, first + step, ... A wait that runs out is recorded and ends the
+// loading, after the copies in flight have landed; the workers wait no more after one that runs out of
+// theirs. The kernel then ends soon, with an error that jk_device_status reports.
 template <typename T, int WORKERS>
 __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsigned char* memory, int stages, int slice_packs,
                                             int rank, int cluster, int64_t first, int64_t step) {
@@ -778,7 +779,10 @@ __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsign
   for (int64_t r = first; r < a.rows; r += step, ++n) {
     if (n % 32 == 0 && r + lane * step < a.rows) ahead = a.targets[r + lane * step];  // of the next 32 rows
     const int64_t target = __shfl_sync(0xffffffffu, static_cast<long long>(ahead), n % 32);
-    if (turn > 0 && good) good = mbar_wait(&sh.empty[stage], (turn - 1) & 1);
+    if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], (turn - 1) & 1))) {
+      good = false;
+      break;
+    }
     if (lane == 0) {
       const Window<T> w(a, r);
       const int per = (w.packs + cluster - 1) / cluster;
@@ -817,7 +821,7 @@ __device__ __forceinline__ void load_slices(const Args<T>& a, Shared& sh, unsign
   // copies in flight land before the block's memory is given back
   for (int i = 0; i < stages; ++i) {
     const uint32_t loads = turn + (i < stage ? 1 : 0);
-    if (loads > 0 && good) good = mbar_wait(&sh.full[i], (loads - 1) & 1);
+    if (loads > 0 && !mbar_wait(&sh.full[i], (loads - 1) & 1)) good = false;
   }
   if (!good) g_device_error = JK_ERR_DEVICE_TIMEOUT;
 }
