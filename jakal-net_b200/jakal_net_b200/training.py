@@ -473,6 +473,13 @@ def _addresses(tensors: list[Tensor]) -> array.array:
     return array.array("Q", map(Tensor.data_ptr, tensors))
 
 
+def _refuse_twice(addresses: array.array, tensors: list[Tensor]) -> None:
+    if len(set(addresses)) != len(addresses):  # empty tensors may share an address
+        some = [p for p, t in zip(addresses, tensors) if t.numel()]
+        if len(set(some)) != len(some):
+            raise ValueError("a tensor is given twice: it would be scaled twice")
+
+
 def _run_clip(tensors, types, outs, out_types, norm_type, clip, max_norm):
     kind = _NORM.get(float(norm_type))
     if kind is None:
@@ -480,19 +487,17 @@ def _run_clip(tensors, types, outs, out_types, norm_type, clip, max_norm):
     src, dst, back = tensors, outs, None
     if not (all(map(Tensor.is_contiguous, tensors)) and (outs is None or all(map(Tensor.is_contiguous, outs)))):
         if clip:
-            for t in tensors if outs is None else outs:
+            written = tensors if outs is None else outs
+            for t in written:
                 if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
                     raise ValueError("a tensor to write has elements that share memory (an expanded tensor)")
+            _refuse_twice(_addresses(written), written)
         src, dst, back = _blocks(tensors, outs, clip)
     ptrs, codes = _addresses(src), _codes(types)
     numels = array.array("q", map(Tensor.numel, src))
     out_ptrs, out_codes = (None, None) if dst is None else (_addresses(dst), _codes(out_types))
-    if clip:
-        written = ptrs if dst is None else out_ptrs
-        if len(set(written)) != len(written):  # empty tensors may share an address
-            some = [p for p, n in zip(written, numels) if n]
-            if len(set(some)) != len(some):
-                raise ValueError("a tensor is given twice: it would be scaled twice")
+    if clip and back is None:
+        _refuse_twice(ptrs if dst is None else out_ptrs, tensors)
     where = tensors[0].device if tensors else torch.device("cuda", _current_device())
     device = where.index
     work = _empty((_CLIP_WORKSPACE,), torch.float64, where)

@@ -1,4 +1,4 @@
-"""Gradient clipping over lists with empty tensors in every place."""
+"""Gradient clipping over lists with empty tensors in every place, and a tensor that is given twice."""
 from __future__ import annotations
 
 import math
@@ -43,3 +43,19 @@ def test_empty_tensors_anywhere(jk, full, before, after):
         assert abs(total.item() - want) <= 40 * U * want
         assert all(((g - 0.125).abs() <= 0.125 * 64 * U + 1e-6).all() for g in outs)
         assert all((g == 0.5).all() for g in grads)
+
+
+def test_a_tensor_given_twice_is_refused_in_every_layout(jk):
+    base = torch.ones(8, 6, device="cuda")
+    for v in (base, base.t(), base[:, ::2], base[2:, 1:4]):
+        into = torch.empty_like(v)
+        with pytest.raises(ValueError, match="twice"):
+            jk.clip_grad_norm_([v, v], 1.0)
+        with pytest.raises(ValueError, match="twice"):
+            jk.clip_grad_norm_([v, v.clone()], 1.0, out=[base[:, ::2], base[:, ::2]] if v.shape == (8, 3) else [into, into])
+        assert (base == 1).all()
+    # two halves of one tensor, and a tensor that is only read twice, are no mistake
+    total = jk.clip_grad_norm_([base[:, ::2], base[:, 1::2]], 1.0)
+    assert abs(total.item() - math.sqrt(48)) <= 40 * U * 7
+    v = torch.ones(9, device="cuda")[::2]
+    assert abs(jk.clip_grad_norm_([v, v], 1.0, out=[torch.empty(5, device="cuda"), torch.empty(5, device="cuda")]).item() - math.sqrt(10)) < 1e-5
