@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import array
 import math
+import operator
 from typing import Iterable, Optional, Union
 
 import torch
@@ -432,6 +433,7 @@ def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100, lab
 
 # ----------------------------------------------------------------------------- gradient norm
 _NORM = {2.0: _lib.JK_NORM_2, math.inf: _lib.JK_NORM_INF}
+_requires_grad = operator.attrgetter("requires_grad")
 _CLIP_WORKSPACE = int(_LIBRARY.jk_clip_grad_norm_workspace()) // 8  # f64 elements
 
 
@@ -445,13 +447,22 @@ def _flat(t: Tensor) -> bool:
     return True
 
 
-def _gradients(grads, name: str) -> tuple[list[Tensor], list[torch.dtype]]:
-    """The tensors, which are CUDA float tensors of one device, and their dtypes."""
-    tensors = [grads] if isinstance(grads, Tensor) else [g for g in grads if g is not None]
+def _gradients(grads, name: str, only_gradients: bool = False) -> tuple[list[Tensor], list[torch.dtype]]:
+    """The tensors, which are CUDA float tensors of one device, and their dtypes. only_gradients:
+    parameters, and other leaves that autograd would refuse to change, are refused; a model's
+    parameters, given in their gradients' place, would be scaled."""
+    tensors = [grads] if isinstance(grads, Tensor) else list(grads)
+    kinds = set(map(type, tensors))
+    if type(None) in kinds:
+        tensors = [g for g in tensors if g is not None]
+        kinds.remove(type(None))
+    if only_gradients and (kinds != {Tensor} or any(map(_requires_grad, tensors))):
+        if any(isinstance(t, torch.nn.Parameter) or (isinstance(t, Tensor) and t.requires_grad and t.is_leaf) for t in tensors):
+            raise TypeError("clip_grad_norm_ takes gradients, not parameters: [p.grad for p in parameters]")
     # one look at all of them (a model has hundreds); which one is wrong is sought only if one is
     try:
         devices = set(map(Tensor.get_device, tensors))  # -1: not a CUDA tensor
-        types = list(map(Tensor.dtype.__get__, tensors))
+        types = [t.dtype for t in tensors]
         fine = len(devices) <= 1 and -1 not in devices and set(types) <= _DTYPE_CODE.keys()
     except TypeError:  # not a tensor
         fine = False
@@ -547,15 +558,15 @@ def clip_grad_norm_(grads: Union[Tensor, Iterable[Optional[Tensor]]], max_norm: 
     """Scales the gradients by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm that
     they had (f32 scalar on their device, as ``grad_norm``).
 
-    grads: one tensor or several (None is skipped), in f32, bf16, f16 or a mix; scaled in place,
-    or into `out`, one tensor for each gradient, of its shape and any of the three dtypes (f32
+    grads: one gradient or several (None is skipped; parameters are refused: they would be scaled
+    themselves), in f32, bf16, f16 or a mix; scaled in place, or into `out`, one tensor for each gradient, of its shape and any of the three dtypes (f32
     master gradients of bf16 ones, say). Tensors must not overlap. A gradient that holds NaN
     makes all of them NaN, one that holds an infinity makes the others 0, as the formula has it;
     error_if_nonfinite raises instead, after reading the norm back, with the gradients scaled."""
-    tensors, types = _gradients(grads, "gradient")
+    tensors, types = _gradients(grads, "gradient", only_gradients=True)
     outs = out_types = None
     if out is not None:
-        outs, out_types = _gradients(out, "out")
+        outs, out_types = _gradients(out, "out", only_gradients=True)
         if len(outs) != len(tensors):
             raise ValueError(f"out has {len(outs)} tensors for {len(tensors)} gradients")
         if outs and outs[0].device != tensors[0].device:

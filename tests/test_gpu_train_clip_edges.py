@@ -1,4 +1,4 @@
-"""Gradient clipping over lists with empty tensors in every place, and a tensor that is given twice."""
+"""Gradient clipping over lists with empty tensors in every place, and what it refuses."""
 from __future__ import annotations
 
 import math
@@ -59,3 +59,25 @@ def test_a_tensor_given_twice_is_refused_in_every_layout(jk):
     assert abs(total.item() - math.sqrt(48)) <= 40 * U * 7
     v = torch.ones(9, device="cuda")[::2]
     assert abs(jk.clip_grad_norm_([v, v], 1.0, out=[torch.empty(5, device="cuda"), torch.empty(5, device="cuda")]).item() - math.sqrt(10)) < 1e-5
+
+
+def test_parameters_are_refused(jk):
+    """The function takes gradients: a model's parameters, given instead, would be scaled."""
+    model = torch.nn.Linear(5, 3).cuda()
+    keep = [p.detach().clone() for p in model.parameters()]
+    frozen = torch.nn.Parameter(torch.ones(3, device="cuda"), requires_grad=False)
+    leaf = torch.ones(3, device="cuda", requires_grad=True)
+    grads = [torch.ones_like(p) for p in keep]
+    for call in (lambda: jk.clip_grad_norm_(model.parameters(), 0.1), lambda: jk.clip_grad_norm_(model.weight, 0.1),
+                 lambda: jk.clip_grad_norm_([grads[0], model.bias], 0.1), lambda: jk.clip_grad_norm_([frozen], 0.1),
+                 lambda: jk.clip_grad_norm_([leaf], 0.1), lambda: jk.clip_grad_norm_(grads, 0.1, out=list(model.parameters()))):
+        with pytest.raises(TypeError, match="gradients"):
+            call()
+    assert all(torch.equal(p, k) for p, k in zip(model.parameters(), keep))
+    assert (frozen == 1).all() and (leaf == 1).all() and all((g == 1).all() for g in grads)
+    # a gradient that is itself differentiable is a gradient
+    x = torch.ones(3, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    assert abs(jk.clip_grad_norm_([g], 1.0).item() - math.sqrt(27)) < 1e-5
+    # the norm alone changes nothing, and may be a model's own
+    assert jk.grad_norm(model.parameters()).isfinite()

@@ -1,8 +1,11 @@
 """CPU-side tests of the training-step operators: argument checks of the entry points with the
-log-sum in two parts."""
+log-sum in two parts, and what clipping refuses before it looks at devices."""
 from __future__ import annotations
 
 import ctypes
+
+import pytest
+import torch
 
 
 def test_split_log_sum_entry_points_check_their_arguments_before_the_device():
@@ -21,3 +24,19 @@ def test_split_log_sum_entry_points_check_their_arguments_before_the_device():
     assert back(None, p, 8, p, p, p, 2, 8, 0, -100, 0.0, 1, p, 8, p, None) == -7
     assert back(p, p, 8, p, None, p, 2, 8, 0, -100, 0.0, 1, p, 8, p, None) == -7
     assert back(p, p, 8, p, p, p, 2, 8, 3, -100, 0.0, 1, p, 8, p, None) == -2
+
+
+def test_clipping_refuses_parameters_before_it_looks_at_devices():
+    import jakal_net_b200 as jk
+
+    model = torch.nn.Linear(3, 2)
+    grads = [torch.ones_like(p) for p in model.parameters()]
+    for call in (lambda: jk.clip_grad_norm_(model.parameters(), 1.0), lambda: jk.clip_grad_norm_(model.weight, 1.0),
+                 lambda: jk.clip_grad_norm_([torch.ones(2, requires_grad=True)], 1.0),
+                 lambda: jk.clip_grad_norm_([torch.nn.Parameter(torch.ones(2), requires_grad=False)], 1.0)):
+        with pytest.raises(TypeError, match="gradients"):
+            call()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        jk.clip_grad_norm_(grads, 1.0)
+    with pytest.raises(TypeError):
+        jk.clip_grad_norm_([1.0], 1.0)
