@@ -176,13 +176,14 @@ def layer_norm_forward_cuda(x: Tensor, weight: Optional[Tensor] = None, bias: Op
 
 
 def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Tensor, weight: Optional[Tensor] = None,
-                             grad_sum: Optional[Tensor] = None, delta_scale: float = 1.0, param_grads: bool = True):
+                             grad_sum: Optional[Tensor] = None, delta_scale: float = 1.0, param_grads: bool = True,
+                             param_dtype: Optional[torch.dtype] = None):
     """Backward of ``layer_norm_forward_cuda`` from the sum and statistics that it returned.
 
     Returns (grad_x, grad_delta, grad_weight, grad_bias). grad_sum is the gradient that reaches
     the sum from its other uses (the residual stream); grad_delta is grad_x itself when
-    delta_scale is 1. The parameter gradients have weight's dtype (the sum's without a weight);
-    param_grads=False returns None for them."""
+    delta_scale is 1. The parameter gradients have weight's dtype, without a weight param_dtype
+    (None: the sum's); param_grads=False returns None for them."""
     code = _check_input("sum", sum)
     if sum.dim() == 0 or sum.shape[-1] == 0:
         raise ValueError("sum must have a last dim that is not empty")
@@ -193,6 +194,12 @@ def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Te
     if weight is not None:
         weight, pcode = _param("weight", weight, device, dim)
         weight_at = weight.data_ptr()
+        if param_dtype not in (None, weight.dtype):
+            raise RuntimeError(f"param_dtype {param_dtype} is not the weight's dtype {weight.dtype}")
+    elif param_dtype is not None:
+        pcode = _DTYPE_CODE.get(param_dtype)
+        if pcode is None:
+            raise RuntimeError(f"param_dtype: unsupported dtype {param_dtype}")
     lead = sum.shape[:-1]
     for name, t in (("mean", mean), ("rstd", rstd)):
         if not isinstance(t, Tensor) or t.dtype != torch.float32 or t.get_device() != device:
@@ -214,7 +221,7 @@ def layer_norm_backward_cuda(grad_y: Tensor, sum: Tensor, mean: Tensor, rstd: Te
         gd_at = grad_delta.data_ptr()
     grad_weight = grad_bias = None
     if param_grads:
-        grad_weight = torch.empty_like(weight) if weight is not None else sum.new_empty((dim,))
+        grad_weight = torch.empty_like(weight) if weight is not None else sum.new_empty((dim,), dtype=param_dtype)
         grad_bias = torch.empty_like(grad_weight)
         work = _empty((_LIBRARY.jk_layer_norm_backward_workspace(rows, dim),), torch.float32, sum.device)
         gw_at, gb_at, work_at = grad_weight.data_ptr(), grad_bias.data_ptr(), work.data_ptr()
@@ -244,9 +251,7 @@ class _LayerNorm(torch.autograd.Function):
         if grad_y is None:  # only the residual stream was used: the norm's part is zero
             grad_y = torch.zeros_like(total)
         gx, gd, gw, gb = layer_norm_backward_cuda(grad_y, total, mean, rstd, weight, grad_sum, ctx.delta_scale,
-                                                  param_grads=need_w or need_b)
-        if need_b and gb.dtype != ctx.bias_dtype:  # no weight: the gradient came in the sum's dtype
-            gb = gb.to(ctx.bias_dtype)
+                                                  need_w or need_b, ctx.bias_dtype if weight is None else None)
         return gx if need_x else None, gw if need_w else None, gb if need_b else None, None, gd if need_delta else None, None
 
 
