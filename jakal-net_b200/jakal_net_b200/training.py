@@ -89,8 +89,8 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
 
 def _written(tensors: list[Tensor]) -> None:
     """Tells autograd that the kernels wrote over these tensors (a value kept for a backward
-    pass is then seen to be stale)."""
-    if tensors and not tensors[0].is_inference():
+    pass is then seen to be stale); inference tensors, which have no version, may be among them."""
+    if tensors:
         torch.autograd.graph.increment_version(tensors)
 
 

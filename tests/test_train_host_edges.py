@@ -1,5 +1,6 @@
 """CPU-side tests of the training-step operators: argument checks of the entry points with the
-log-sum in two parts, and what clipping refuses before it looks at devices."""
+log-sum in two parts, what clipping refuses before it looks at devices, and the versions of
+tensors that kernels wrote over."""
 from __future__ import annotations
 
 import ctypes
@@ -40,3 +41,18 @@ def test_clipping_refuses_parameters_before_it_looks_at_devices():
         jk.clip_grad_norm_(grads, 1.0)
     with pytest.raises(TypeError):
         jk.clip_grad_norm_([1.0], 1.0)
+
+
+def test_every_written_tensor_has_a_new_version():
+    """Whatever tensors are with it: an inference tensor in front does not hide the others."""
+    from jakal_net_b200 import training
+
+    plain, other = torch.ones(2), torch.ones(2)
+    with torch.inference_mode():
+        inference = torch.ones(2)
+    for tensors in ([plain, other], [inference, plain, other], [plain, inference, other]):
+        before = plain._version, other._version
+        training._written(tensors)
+        assert plain._version > before[0] and other._version > before[1]
+    training._written([inference])
+    training._written([])
