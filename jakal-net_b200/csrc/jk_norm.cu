@@ -719,10 +719,12 @@ int shape_backward(const Backward& a, cudaStream_t s) {
 #undef JK_RUN
 }
 
-// Whether a tensor's rows begin where those of a contiguous one on a 16-byte boundary do.
+// Whether a tensor's rows can be taken in packs: they begin where those of a contiguous one on a 16-byte
+// boundary do and, where packs hold parts of two rows, only the first and the last row's packs reach past
+// the tensor (an earlier row's would where the rows after it are no longer than what it reaches).
 template <typename T>
 bool lies_plain(const void* p, int64_t stride, int64_t dim) {
-  return p == nullptr || (aligned16(p) && (stride - dim) % kPack<T> == 0);
+  return p == nullptr || (aligned16(p) && (stride - dim) % kPack<T> == 0 && (dim % kPack<T> == 0 || stride >= kPack<T> - 1));
 }
 
 template <typename T>

@@ -1,5 +1,7 @@
-"""Layer norm with a bias and no weight."""
+"""Layer norm: a bias without a weight, and rows of a few columns among other data."""
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -43,3 +45,37 @@ def test_refusals_of_a_parameter_dtype(jk):
         jk.layer_norm_backward_cuda(y, x, mean, rstd, param_dtype=torch.float64)
     with pytest.raises(RuntimeError, match="dtype"):
         jk.layer_norm_backward_cuda(y, x, mean, rstd, torch.ones(8, device="cuda"), param_dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [1, 2, 3, 5, 7, 9, 11])
+def test_few_columns_between_other_data(jk, dtype, dim):
+    """Rows shorter than a 16-byte block, whose neighbours and surroundings are NaN where they are not
+    rows of the tensor."""
+    for rows in (1, 2, 3, 7, 8, 9, 300):
+        for stride in (dim, dim + 8, dim + 3):
+            g = torch.Generator(device="cuda").manual_seed(rows + dim)
+            made = []
+            for _ in range(2):
+                flat = torch.full((16 + rows * stride + 16,), math.nan, device="cuda", dtype=dtype)
+                view = flat[16:].as_strided((rows, dim), (stride, 1), 16)
+                view.copy_(torch.randn(rows, dim, generator=g, device="cuda"))
+                made.append(view)
+            x, grad = made
+            y, _, mean, rstd = jk.layer_norm_forward_cuda(x)
+            h = x.double()
+            m = h.mean(-1, keepdim=True)
+            r = ((h - m).square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+            n = (h - m) * r
+            # the differences from the mean err by a few u of the largest value, and r by as much relative to the spread
+            e = 16 * U * h.abs().amax(-1, keepdim=True) * r * (1 + n.abs()) + 8 * U
+            assert ((y.double() - n).abs() <= e + ROUND[dtype] * 1.01 * n.abs() + 2.0 ** -24).all()
+            gx, _, gw, gb = jk.layer_norm_backward_cuda(grad, x, mean, rstd)
+            k = (h - mean.double()[:, None]) * rstd.double()[:, None]
+            dy, s = grad.double(), rstd.double()[:, None]
+            dx = s * (dy - dy.mean(-1, keepdim=True) - k * (dy * k).mean(-1, keepdim=True))
+            size = s * (dy.abs() + dy.abs().mean(-1, keepdim=True) + k.abs() * (dy * k).abs().mean(-1, keepdim=True))
+            assert ((gx.double() - dx).abs() <= 40 * U * size + ROUND[dtype] * 1.01 * dx.abs() + 2.0 ** -24).all()
+            depth = rows / 32 + 664
+            assert ((gw.double() - (dy * k).sum(0)).abs() <= depth * U * (dy * k).abs().sum(0) + ROUND[dtype] * 1.01 * (dy * k).sum(0).abs() + 2.0 ** -24).all()
+            assert ((gb.double() - dy.sum(0)).abs() <= depth * U * dy.abs().sum(0) + ROUND[dtype] * 1.01 * dy.sum(0).abs() + 2.0 ** -24).all()
