@@ -660,8 +660,12 @@ int pick_backward(const Backward& a, cudaStream_t s) {
 
 // The threads of a row and their turns: a warp or less as long as 16 elements a thread do, so that no
 // barrier is needed; beyond, 8 to 16 elements of a 16-byte pack or two each, which leaves an SM 512
-// threads or more (f32 2047 wide, backward: 74 us with two packs, 111 with four; f16 5001 wide: 35 us
-// with one pack of 640 threads, 41 with two of 512).
+// threads or more. Four packs to fewer threads are no better (us a call, forward and backward; f32,
+// 8192 x 2048: 25.5 and 42.1 with two, 23.5 and 43.6 with four; 8192 x 2047: 59.9 and 63.9, either way).
+// Rows of 4097 to 5113 16-bit elements that begin anywhere take one pack of 640 threads (3000 x 4501
+// f16: 29.2 and 39.5, 31.2 and 41.6 with two of 384), those that begin on a 16-byte boundary two
+// (3000 x 4608 f16: 23.0 and 30.7, 23.0 and 31.7 with one of 640); above, one pack is slower for both
+// (3000 x 6001 f16: 31.2 and 47.7 with two, 32.8 and 48.2 with one of 768).
 #define JK_NORM_SHAPES(RUN)                                             \
   if constexpr (VEC == 8) {                                             \
     if (turns <= 8) return RUN(1, 8);                                   \
@@ -671,7 +675,9 @@ int pick_backward(const Backward& a, cudaStream_t s) {
     if (turns <= 128) return RUN(1, 128);                               \
     if (turns <= 256) return RUN(2, 128);                               \
     if (turns <= 512) return RUN(2, 256);                               \
-    if (turns <= 640) return RUN(1, 640);                               \
+    if constexpr (SHIFTED) {                                            \
+      if (turns <= 640) return RUN(1, 640);                             \
+    }                                                                   \
     if (turns <= 768) return RUN(2, 384);                               \
     if (turns <= 1024) return RUN(2, 512);                              \
     return RUN(2, 1024);                                                \
