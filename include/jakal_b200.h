@@ -487,7 +487,8 @@ int jk_cross_entropy_backward_split(const float* grad_loss, const void* logits, 
 int64_t jk_clip_grad_norm_workspace(void);
 
 /* Norm over all elements of `count` flat tensors, and their clipping:
- *   total = sqrt(sum g^2) (JK_NORM_2; summed in f64, so squares neither overflow nor vanish) or
+ *   total = sqrt(sum g^2) (JK_NORM_2; squares are added in f32 by up to 32, in f64 where that would
+ *           leave f32's range, and their sums in f64, so they neither overflow nor vanish) or
  *           max |g| (JK_NORM_INF), NaN if any element is;
  *   out_i = g_i * min(1, max_norm / (total + eps)).
  * grads, outs, numels, dtypes, out_dtypes are HOST arrays of `count` entries that are read

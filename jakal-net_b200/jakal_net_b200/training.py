@@ -352,7 +352,10 @@ def cross_entropy_forward_cuda(logits: Tensor, targets: Tensor, ignore_index: in
     Returns (loss, lse): loss f32, a scalar for reduction "mean" (over the targets that are not
     ignore_index) or "sum", of targets' shape for "none"; lse f32 of targets' shape, the rows'
     log-sum-exp, which ``cross_entropy_backward_cuda`` takes. A row to ignore has loss and lse 0
-    and is not read. A target outside the vocabulary gives NaN."""
+    and is not read. A target outside the vocabulary gives NaN.
+
+    Logits whose rows no single stride spans (logits[:, :-1] of a batch) are copied first: to leave a
+    position out, give it the target ignore_index."""
     return _cross_entropy(logits, targets, int(ignore_index), float(label_smoothing), reduction, 1.0, want_lse=True)[:2]
 
 
@@ -554,7 +557,8 @@ def _blocks(tensors, outs, clip):
 
 def grad_norm(grads: Union[Tensor, Iterable[Optional[Tensor]]], norm_type: float = 2.0) -> Tensor:
     """Norm (2 or inf) over all elements of the gradients together, an f32 scalar on their
-    device. The squares are summed in f64, so the norm is finite wherever it fits f32."""
+    device. Squares are added in f32 by up to 32 (in f64 where that would leave f32's range) and their
+    sums in f64, so the norm is good to a few units of f32 and finite wherever it fits f32."""
     return _run_clip(*_gradients(grads, "gradient"), None, None, norm_type, 0, 0.0)
 
 
