@@ -457,11 +457,12 @@ __global__ void __launch_bounds__(kBlock<TPR>, kBlock<TPR> <= 512 ? 512 / kBlock
         float g[VEC], n[VEC];
         y[i].floats(g);
         hh[i].floats(n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) n[j] = (n[j] - mu) * rs;
         clear_outside<VEC, SHIFTED>(g, columns(c));
-        clear_outside<VEC, SHIFTED>(n, columns(c));  // another row's may be infinite
+        clear_outside<VEC, SHIFTED>(n, columns(c));  // another row's may be infinite, or be so against this row's mean
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          n[j] = (n[j] - mu) * rs;
           const float u = g[j] * w[i][j];
           s[0] += u;
           s[1] = fmaf(u, n[j], s[1]);

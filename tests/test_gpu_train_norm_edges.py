@@ -1,4 +1,4 @@
-"""Layer norm: a bias without a weight, and rows of a few columns among other data."""
+"""Layer norm: a bias without a weight, rows of a few columns among other data, rows of one large value."""
 from __future__ import annotations
 
 import math
@@ -79,3 +79,22 @@ def test_few_columns_between_other_data(jk, dtype, dim):
             depth = rows / 32 + 664
             assert ((gw.double() - (dy * k).sum(0)).abs() <= depth * U * (dy * k).abs().sum(0) + ROUND[dtype] * 1.01 * (dy * k).sum(0).abs() + 2.0 ** -24).all()
             assert ((gb.double() - dy.sum(0)).abs() <= depth * U * dy.abs().sum(0) + ROUND[dtype] * 1.01 * dy.sum(0).abs() + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dim", [5, 8, 9, 30])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_one_large_value(jk, dtype, dim):
+    """A constant row is normalised to 0, whatever its value: distances from the mean count, and only
+    of the row's own columns."""
+    value = 1e37
+    x = torch.full((9, dim), value, device="cuda").to(dtype)
+    x[4] = -x[4]
+    mean, rstd = x[:, 0].float(), torch.full((9,), 1e5 ** 0.5, device="cuda")
+    grad = torch.randn(9, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    gx, _, gw, gb = jk.layer_norm_backward_cuda(grad, x, mean, rstd)
+    dy = grad.double()
+    want = rstd.double()[:, None] * (dy - dy.mean(-1, keepdim=True))
+    size = rstd.double()[:, None] * (dy.abs() + dy.abs().mean(-1, keepdim=True))
+    assert ((gx.double() - want).abs() <= 40 * U * size + ROUND[dtype] * 1.01 * want.abs()).all()
+    assert not gw.any()
+    assert ((gb.double() - dy.sum(0)).abs() <= 700 * U * dy.abs().sum(0) + ROUND[dtype] * 1.01 * dy.sum(0).abs()).all()
