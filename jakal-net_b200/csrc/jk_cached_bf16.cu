@@ -1,0 +1,10 @@
+// Propagation over a paged cache, bf16 (a unit of its own, so that the types compile in parallel).
+#include "jk_cached.cuh"
+
+namespace jk {
+namespace cached {
+
+int launch_bf16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__nv_bfloat16>(a, s, units, stream); }
+
+}  // namespace cached
+}  // namespace jk

@@ -72,6 +72,27 @@ __device__ __forceinline__ uint4 pack(const float (&f)[kPack<T>]) {
   return pack(f, T());
 }
 
+// The 16 bytes at p, a = p mod 16: from the one or two aligned blocks that hold them
+// (so no byte of a block is read that has none of the 16).
+__device__ __forceinline__ uint4 load16(const void* p, uint32_t a) {
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) - a);
+  const uint4 lo = q[0];
+  if (a == 0) return lo;
+  const uint4 hi = q[1];
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (a & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (a & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const uint32_t bits = (a & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
+}
+
 __device__ __forceinline__ float warp_sum32(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

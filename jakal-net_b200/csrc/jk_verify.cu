@@ -1,0 +1,284 @@
+// Verification of drafted tokens from given random numbers (jk_verify_draft).
+//
+// Token i of a sequence, drawn from the draft's q_i, is accepted while u_i q_i(x_i) < p_i(x_i). With
+// the first place a that is not, the new token is drawn from r = max(p_a - q_a, 0), which makes the
+// sequence one of the target's: it is the least j at which the running sum of r passes u r's total.
+// Where all are accepted r is the target's next distribution.
+//
+// A comparison of a product or of a running sum decides a token, so both are in f64: products of two
+// f32 are exact there, and a running sum is off by less than 2^-50 of the total, where f32 would give
+// another token in one of some thousand draws over a vocabulary of 100,000.
+//
+// Of the draft's and the target's rows only place a's are read, once: a cluster of blocks per
+// sequence adds them up by warps, each a run of 16-byte packs; the run that holds the draw is cut
+// into runs again, one for each warp of its block, until one warp finds the token (the second look
+// at a run comes from L2). Bound: memory for a batch, the latency of these steps for a few sequences.
+#include <cooperative_groups.h>
+
+#include "jk_host.h"
+#include "jk_rows.cuh"
+
+namespace jk {
+namespace verify {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kSms = 148;
+
+struct Args {
+  const void *target, *draft;
+  int64_t target_b, target_t, draft_b, draft_t;
+  const int64_t* tokens;
+  const float* uniform;
+  const int32_t* counts;
+  int32_t drafted, vocab;
+  int64_t* out;
+  int32_t* accepted;
+};
+
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// NaN and negative values count as 0.
+__device__ __forceinline__ float mass(float v) { return v > 0.0f ? v : 0.0f; }
+
+// One place's r: packs of E entries on the 16-byte blocks of the target's row.
+template <typename T>
+struct Rest {
+  static constexpr int E = kPack<T>;
+  const T *p, *q;   // q null: 0 throughout
+  int32_t without;  // this entry is 0 (the token that a certain draft had), -1: none
+  int32_t vocab, head, packs;
+  uint32_t apart;   // bytes by which the draft's packs begin inside a 16-byte block
+
+  __device__ __forceinline__ Rest(const T* p_, const T* q_, int32_t without_, int32_t vocab_)
+      : p(p_), q(q_), without(without_), vocab(vocab_) {
+    head = static_cast<int32_t>((reinterpret_cast<uintptr_t>(p_) & 15) / sizeof(T));
+    packs = (head + vocab + E - 1) / E;
+    apart = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q_) - reinterpret_cast<uintptr_t>(p_)) & 15u;
+  }
+
+  // Entries [E k - head, E k - head + E); those outside the row are 0.
+  __device__ __forceinline__ void load(int32_t k, double (&r)[E]) const {
+    const int32_t j = k * E - head;
+    float a[E], b[E];
+    if (j >= 0 && j + E <= vocab) {
+      unpack<T>(*reinterpret_cast<const uint4*>(p + j), a);
+      if (q == nullptr) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) b[e] = 0.0f;
+      } else {
+        unpack<T>(load16(q + j, apart), b);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool in = j + e >= 0 && j + e < vocab;
+        a[e] = in ? to_f32(p[j + e]) : 0.0f;
+        b[e] = in && q != nullptr ? to_f32(q[j + e]) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = mass(a[e]), y = mass(b[e]);
+      r[e] = x > y && j + e != without ? static_cast<double>(x) - static_cast<double>(y) : 0.0;
+    }
+  }
+
+  // Over packs [from, to), a warp.
+  __device__ __forceinline__ double sum(int32_t from, int32_t to) const {
+    double s = 0.0;
+#pragma unroll 4
+    for (int32_t k = from + (threadIdx.x & 31); k < to; k += 32) {
+      double r[E];
+      load(k, r);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += r[e];
+    }
+    return warp_sum64(s);
+  }
+};
+
+// The part (of n, their sums given) that holds `draw` when the parts are laid one after the other
+// from `before`: the first whose end passes it, else (the sums' rounding) the last that is not empty;
+// -1: all are empty. before: receives where that part begins.
+__device__ __forceinline__ int part_of(const double* sums, int n, double draw, double& before) {
+  int best = -1;
+  double at = before, begin = before;
+  for (int i = 0; i < n; ++i) {
+    if (sums[i] > 0.0) {
+      best = i, begin = at;
+      if (at + sums[i] > draw) break;
+    }
+    at += sums[i];
+  }
+  before = begin;
+  return best;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const Args g) {
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  __shared__ double sums[kWarps];
+  __shared__ double totals[kMaxCluster];
+  __shared__ int32_t first, token;
+  cluster.barrier_arrive();  // before another block writes here, this one has begun
+  const int rank = cluster.block_rank(), size = cluster.num_blocks();
+  const int64_t b = blockIdx.x / size;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int32_t n = g.counts == nullptr ? g.drafted : g.counts[b];
+  n = n < 0 ? 0 : n > g.drafted ? g.drafted : n;
+  const T* target = static_cast<const T*>(g.target) + b * g.target_b;
+  const T* draft = g.draft == nullptr ? nullptr : static_cast<const T*>(g.draft) + b * g.draft_b;
+  const int64_t* tokens = g.tokens + b * g.drafted;
+  const float* uniform = g.uniform + b * (g.drafted + 1);
+  if (tid == 0) first = n;
+  __syncthreads();
+  for (int32_t i = tid; i < n; i += kThreads) {
+    const int64_t x = tokens[i];
+    bool ok = false;
+    if (x >= 0 && x < g.vocab) {
+      const float q = draft == nullptr ? 1.0f : mass(to_f32(draft[i * g.draft_t + x]));
+      ok = static_cast<double>(uniform[i]) * static_cast<double>(q) < static_cast<double>(mass(to_f32(target[i * g.target_t + x])));
+    }
+    if (!ok) atomicMin(&first, i);
+  }
+  __syncthreads();
+  const int32_t a = first;
+  const bool rejected = a < n;
+  const int64_t x = rejected ? tokens[a] : -1;
+  Rest<T> rest(target + a * g.target_t, rejected && draft != nullptr ? draft + a * g.draft_t : nullptr,
+               rejected && draft == nullptr && x >= 0 && x < g.vocab ? static_cast<int32_t>(x) : -1, g.vocab);
+  const double u = static_cast<double>(uniform[g.drafted]);
+  // this block's run of packs, and each warp's of it
+  const int32_t mine = (rest.packs + size - 1) / size;
+  int32_t from = rank * mine < rest.packs ? rank * mine : rest.packs;
+  int32_t to = from + mine < rest.packs ? from + mine : rest.packs;
+  double total = 0.0;
+  for (int turn = 0; turn < 2; ++turn) {
+    const int32_t each = (to - from + kWarps - 1) / kWarps;
+    const int32_t low = from + warp * each < to ? from + warp * each : to;
+    const double s = rest.sum(low, low + each < to ? low + each : to);
+    if (lane == 0) sums[warp] = s;
+    __syncthreads();
+    if (turn == 0) cluster.barrier_wait();
+    if (tid < size) {
+      double all = 0.0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) all += sums[w];
+      *cluster.map_shared_rank(&totals[rank], tid) = all;
+    }
+    cluster.sync();
+    total = 0.0;
+    for (int i = 0; i < size; ++i) total += totals[i];
+    // without mass (the target is nowhere above the draft): the target itself
+    if (total > 0.0 || !rejected || turn == 1) break;
+    rest.q = nullptr, rest.without = -1;
+    cluster.sync();  // the totals have been read
+  }
+  double draw = u * total, before = 0.0;
+  const int owner = part_of(totals, size, draw, before);
+  if (owner == rank) {
+    // the run that holds the draw, cut into the warps' runs until it is a few packs
+    double begin = before;
+    while (true) {
+      const int32_t each = (to - from + kWarps - 1) / kWarps;
+      const int w = part_of(sums, kWarps, draw, begin);
+      from = from + w * each < to ? from + w * each : to;  // w >= 0: the run has mass
+      to = from + each < to ? from + each : to;
+      if (to - from <= 64) break;
+      __syncthreads();  // the sums have been read
+      const int32_t next = (to - from + kWarps - 1) / kWarps;
+      const int32_t low = from + warp * next < to ? from + warp * next : to;
+      const double s = rest.sum(low, low + next < to ? low + next : to);
+      if (lane == 0) sums[warp] = s;
+      __syncthreads();
+    }
+    if (warp == 0) {
+      int32_t found = -1, last = -1;
+      for (int32_t k0 = from; k0 < to && found < 0; k0 += 32) {
+        double r[Rest<T>::E] = {};
+        if (k0 + lane < to) rest.load(k0 + lane, r);
+        double own = 0.0;
+#pragma unroll
+        for (int e = 0; e < Rest<T>::E; ++e) own += r[e];
+        double upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += up;
+        }
+        const double all = __shfl_sync(0xffffffffu, upto, 31);
+        double at = begin + (upto - own);
+        int32_t here = -1, positive = -1;
+#pragma unroll
+        for (int e = 0; e < Rest<T>::E; ++e) {
+          at += r[e];
+          if (r[e] > 0.0) {
+            positive = (k0 + lane) * Rest<T>::E - rest.head + e;
+            if (here < 0 && at > draw) here = positive;
+          }
+        }
+        const unsigned hits = __ballot_sync(0xffffffffu, here >= 0), some = __ballot_sync(0xffffffffu, positive >= 0);
+        if (hits != 0) found = __shfl_sync(0xffffffffu, here, __ffs(hits) - 1);
+        if (some != 0) last = __shfl_sync(0xffffffffu, positive, 31 - __clz(some));
+        begin += all;
+      }
+      if (lane == 0) token = found >= 0 ? found : last;
+    }
+  } else if (tid == 0) {
+    token = -1;
+  }
+  __syncthreads();
+  if (owner == rank || (owner < 0 && rank == 0)) {
+    int64_t* out = g.out + b * (g.drafted + 1);
+    for (int32_t i = tid; i <= g.drafted; i += kThreads) out[i] = i < a ? tokens[i] : i == a ? token : -1;
+    if (tid == 0) g.accepted[b] = a;
+  }
+}
+
+template <typename T>
+int launch(const Args& g, int64_t batch, cudaStream_t s) {
+  // Blocks of a sequence: as many as leave each SM two blocks at most, none for less than 2048
+  // entries. (One sequence of 131072 entries in f32: see the figures below.)
+  int size = 1;
+  while (size < kMaxCluster && batch * size * 2 <= 2 * kSms && g.vocab / (size * 2) >= 2048) size *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(batch * size));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(size);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, verify_kernel<T>, g);
+  return launch_status();
+}
+
+}  // namespace verify
+}  // namespace jk
+
+extern "C" int jk_verify_draft(const void* target, int64_t target_stride_b, int64_t target_stride_t, const void* draft,
+                               int64_t draft_stride_b, int64_t draft_stride_t, const int64_t* tokens, const float* uniform,
+                               const int32_t* counts, int64_t batch, int64_t drafted, int64_t vocab, int dtype, int64_t* out_tokens,
+                               int32_t* accepted, jk_stream_t stream) {
+  using namespace jk;
+  using namespace jk::verify;
+  if (batch < 0 || drafted < 0 || vocab < 1 || batch > (1 << 24) || drafted > (1 << 30) || vocab > (1 << 30)) return JK_ERR_BAD_SHAPE;
+  if (!float_dtype(dtype)) return JK_ERR_BAD_DTYPE;
+  if (batch > 0 && (target == nullptr || uniform == nullptr || out_tokens == nullptr || accepted == nullptr)) return JK_ERR_BAD_ARG;
+  if (batch > 0 && drafted > 0 && tokens == nullptr) return JK_ERR_BAD_ARG;
+  if (int st = check_device()) return st;
+  if (batch == 0) return JK_OK;
+  const Args g{target,  draft,  target_stride_b, target_stride_t, draft_stride_b, draft_stride_t, tokens,
+               uniform, counts, static_cast<int32_t>(drafted), static_cast<int32_t>(vocab), out_tokens, accepted};
+  auto s = reinterpret_cast<cudaStream_t>(stream);
+  JK_WITH_TYPE(dtype, T, return launch<T>(g, batch, s));
+}

@@ -42,6 +42,8 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import JakalB200Error, check, load
+from .generation import (cache_compact_, cache_copy_, cache_fork_, cache_release_, cache_reserve_, cache_write_,
+                         cached_propagation, verify_draft)
 from .training import (clip_grad_norm_, cross_entropy, cross_entropy_backward_cuda, cross_entropy_forward_cuda,
                        cross_entropy_with_grad_cuda, grad_norm, layer_norm, layer_norm_backward_cuda,
                        layer_norm_forward_cuda)
@@ -70,6 +72,14 @@ __all__ = [
     "cross_entropy_with_grad_cuda",
     "grad_norm",
     "clip_grad_norm_",
+    "cached_propagation",
+    "cache_reserve_",
+    "cache_write_",
+    "cache_fork_",
+    "cache_release_",
+    "cache_compact_",
+    "cache_copy_",
+    "verify_draft",
     "JakalB200Error",
 ]
 

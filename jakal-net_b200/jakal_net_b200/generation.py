@@ -1,0 +1,444 @@
+"""Generation-step operators: what a model that produces one node (token) after another needs beside
+the propagation / transition operators, which compute whole layers.
+
+* ``cached_propagation``: the window / dense propagation of the newest nodes of every sequence over
+  the nodes that a paged cache holds;
+* ``cache_reserve_``, ``cache_write_``: room for new nodes, and their rows;
+  ``cache_fork_``, ``cache_release_``: sequences that branch, end or are cut back;
+  ``cache_compact_``, ``cache_copy_``: pages moved together, pages copied;
+* ``verify_draft``: drafted tokens held against the target's probabilities.
+
+A cache is made of plain tensors, which the caller owns:
+
+* pools ``[pages, kv_heads, page_size, width]`` (keys: the source projections; values) and
+  ``[pages, kv_heads, page_size]`` (states), as many sets as there are layers;
+* ``table`` int32 ``[batch, columns]``: the page that holds a sequence's nodes
+  ``[c * page_size, (c + 1) * page_size)``, -1 where there is none;
+* ``lengths`` int32 ``[batch]``; ``refs`` int32 ``[pages]``: how many table entries name a page (0: free).
+
+An empty cache has a table of -1 and zeros. All of it stays on the device: nothing is read back, so
+a step (``cache_reserve_``, for every layer ``cache_write_`` and ``cached_propagation``, then
+``verify_draft`` and ``cache_release_``) can be captured into a CUDA graph. Everything runs on the
+current stream; calls on one cache have to be ordered. Results are the same from run to run.
+The operators have no backward pass and refuse inputs that ask for one.
+"""
+from __future__ import annotations
+
+import array
+import ctypes
+from typing import Optional, Sequence, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .training import _call, _check_input, _empty, _ptr, _written
+
+__all__ = [
+    "cached_propagation",
+    "cache_reserve_",
+    "cache_write_",
+    "cache_fork_",
+    "cache_release_",
+    "cache_compact_",
+    "cache_copy_",
+    "verify_draft",
+]
+
+_LIBRARY = _lib.load()
+_COMPRESS = {
+    "softmax": _lib.JK_SOFTMAX,
+    "softsign": _lib.JK_SOFTSIGN,
+    "signed_abs_softmax": _lib.JK_SIGNED_ABS_SOFTMAX,
+}
+_MAX_WRITE = 64  # pairs of one jk_cache_write
+
+
+# ----------------------------------------------------------------------------- checks
+def _ints(name: str, t: Tensor, shape: Optional[tuple], device: int) -> None:
+    """t is an int32 tensor on the device, of the shape (None: of one dim), contiguous."""
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor in the b200_sm100a backend (got {t.device}).")
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected cuda:{device}")
+    if t.dtype != torch.int32:
+        raise RuntimeError(f"{name}: unsupported dtype {t.dtype} (int32)")
+    if t.dim() != 1 if shape is None else t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {'one dim' if shape is None else shape}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _table(table: Tensor) -> tuple[int, int, int, int]:
+    """(device, batch, columns, elements from one row to the next)"""
+    if not isinstance(table, Tensor):
+        raise TypeError("table must be a tensor")
+    if not table.is_cuda:
+        raise RuntimeError(f"table must be a CUDA tensor in the b200_sm100a backend (got {table.device}).")
+    if table.dtype != torch.int32:
+        raise RuntimeError(f"table: unsupported dtype {table.dtype} (int32)")
+    if table.dim() != 2:
+        raise ValueError(f"table has shape {tuple(table.shape)}, expected [batch, columns]")
+    batch, columns = table.shape
+    row, step = table.stride()
+    if (columns > 1 and step != 1) or (batch > 1 and row < columns):
+        raise ValueError("table must have rows that are contiguous inside and apart")
+    return table.get_device(), batch, columns, max(row, columns)
+
+
+def _no_grad(**tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} requires grad: the generation-step operators have no backward pass (use torch.no_grad())")
+
+
+def _one_block(shape, strides) -> bool:
+    """Whether these dims fill one block of memory, in whatever order."""
+    expected = 1
+    for stride, size in sorted((s, n) for n, s in zip(shape, strides) if n != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+class _Pools:
+    """A call's pools as jk_pools_t; `arrays` keeps what it points to alive."""
+
+    def __init__(self, pools: Union[Tensor, Sequence[Tensor]], pages: int, device: int):
+        tensors = [pools] if isinstance(pools, Tensor) else list(pools)
+        data, sizes, strides = array.array("Q"), array.array("q"), array.array("q")
+        for i, p in enumerate(tensors):
+            if not isinstance(p, Tensor):
+                raise TypeError(f"pool {i} must be a tensor")
+            if p.get_device() != device:
+                raise RuntimeError(f"pool {i} is on {p.device}, expected cuda:{device}")
+            shape, stride, size = p.shape, p.stride(), p.element_size()
+            if not shape or shape[0] != pages:
+                raise ValueError(f"pool {i} has shape {tuple(shape)}, expected {pages} pages in its first dim")
+            block = 1
+            for n in shape[1:]:
+                block *= n
+            if not (p.is_contiguous() or _one_block(shape[1:], stride[1:])) or (pages > 1 and stride[0] < block):
+                raise ValueError(f"pool {i}: a page must be one block of memory, apart from the other pages")
+            data.append(p.data_ptr())
+            sizes.append(block * size)
+            strides.append(max(stride[0], block) * size)
+        if len(set(data)) != len(data) and any(p.numel() for p in tensors):
+            raise ValueError("a pool is given twice")
+        self.tensors, self.arrays = tensors, (data, sizes, strides)
+        self.struct = _lib.JkPools(data.buffer_info()[0], sizes.buffer_info()[0], strides.buffer_info()[0], len(tensors))
+
+    def pointer(self):
+        return ctypes.addressof(self.struct)
+
+
+def _page_size(page_size: int) -> int:
+    page_size = int(page_size)
+    if page_size < 1:
+        raise ValueError(f"page_size is {page_size}")
+    return page_size
+
+
+# ----------------------------------------------------------------------------- propagation
+def _cache_pages(name: str, t: Tensor, query: Tensor, dims: int) -> None:
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.get_device() != query.get_device():
+        raise RuntimeError(f"{name} is on {t.device}, expected {query.device}")
+    if t.dtype != query.dtype:
+        raise RuntimeError(f"{name} has dtype {t.dtype}, expected {query.dtype}")
+    if t.dim() != dims:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {dims} dims")
+    if dims == 4 and t.shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError(f"{name} must be contiguous in its last dim")
+
+
+def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, table: Tensor, lengths: Tensor,
+                       state_pages: Optional[Tensor] = None, counts: Optional[Tensor] = None, window: Optional[int] = None,
+                       compress: str = "softmax", scale: float = 1.0, score_bias: float = 0.0):
+    """Propagation of every sequence's newest nodes over the nodes of a paged cache, which they are
+    among: what ``propagation_window`` (window None: ``propagation_dense``, causal) gives for those
+    nodes, without the others.
+
+    query [batch, new, heads, rank], the target projections; key_pages [pages, kv_heads, page_size,
+    rank], the source projections; value_pages [.., dim]; state_pages [pages, kv_heads, page_size] or
+    None; all f32, bf16 or f16. heads is a multiple of kv_heads, and each head of the cache is read by
+    as many in a row. counts int32 [batch]: how many of the `new` nodes a sequence has (None: all); they
+    are its last ones, the first of them in query's first rows. Node at place p sees the places
+    [p - window, p]; with s = scale * q . k + score_bias,
+
+        value = sum_j w_j v_j,   state = sum_j w_j state_j,   w = compress(s)
+
+    compress: "softmax", "softsign" (s / (1 + |s|)) or "signed_abs_softmax" (sign(s) softmax(|s|)).
+
+    Returns value [batch, new, heads, dim], or (state [batch, new, heads], value), in query's dtype.
+    Nodes that see nothing (an empty sequence, pages that are missing) and rows past counts are zeros.
+    Places that are not seen have no part in a result, whatever they hold. rank <= 256, dim <= 512, new <= 64."""
+    code = _check_input("query", query)
+    if query.dim() != 4:
+        raise ValueError(f"query has shape {tuple(query.shape)}, expected [batch, new, heads, rank]")
+    kind = _COMPRESS.get(compress)
+    if kind is None:
+        raise ValueError(f"unknown compress {compress!r} (softmax, softsign or signed_abs_softmax)")
+    _cache_pages("key_pages", key_pages, query, 4)
+    _cache_pages("value_pages", value_pages, query, 4)
+    _no_grad(query=query, key_pages=key_pages, value_pages=value_pages, state_pages=state_pages)
+    batch, new, heads, rank = query.shape
+    pages, kv_heads, page_size, dim = value_pages.shape
+    if key_pages.shape != (pages, kv_heads, page_size, rank):
+        raise ValueError(f"key_pages has shape {tuple(key_pages.shape)}, expected {(pages, kv_heads, page_size, rank)}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} heads cannot share {kv_heads} heads of the cache")
+    if page_size < 1 or not 1 <= rank <= 256 or not 1 <= dim <= 512 or new > 64:
+        raise ValueError(f"page_size {page_size}, rank {rank}, dim {dim} or {new} new nodes outside the supported range "
+                         "(rank <= 256, dim <= 512, new <= 64)")
+    device, rows, columns, table_stride = _table(table)
+    if rows != batch or device != query.get_device():
+        raise ValueError(f"table has {rows} rows on {table.device}, expected {batch} on {query.device}")
+    _ints("lengths", lengths, (batch,), device)
+    if counts is not None:
+        _ints("counts", counts, (batch,), device)
+    if window is not None and window < 0:
+        raise ValueError(f"window is {window}")
+    state_at, state_strides, state = None, (0, 0, 0), None
+    if state_pages is not None:
+        _cache_pages("state_pages", state_pages, query, 3)
+        if state_pages.shape != (pages, kv_heads, page_size):
+            raise ValueError(f"state_pages has shape {tuple(state_pages.shape)}, expected {(pages, kv_heads, page_size)}")
+        state = torch.empty((batch, new, heads), dtype=query.dtype, device=query.device)
+        state_at, state_strides = state_pages.data_ptr(), state_pages.stride()
+    if rank > 1 and query.stride(3) != 1:
+        query = query.contiguous()
+    value = torch.empty((batch, new, heads, dim), dtype=query.dtype, device=query.device)
+    work = _empty((_LIBRARY.jk_cached_propagation_workspace(batch, new, heads, kv_heads, dim, page_size, columns, code) // 4,),
+                  torch.float32, query.device)
+    _call(_LIBRARY.jk_cached_propagation, "jk_cached_propagation", device, query.data_ptr(), *query.stride()[:3],
+          key_pages.data_ptr(), *key_pages.stride()[:3], value_pages.data_ptr(), *value_pages.stride()[:3], state_at, *state_strides,
+          table.data_ptr(), table_stride, lengths.data_ptr(), _ptr(counts), batch, new, heads, kv_heads, rank, dim, pages, page_size,
+          columns, code, -1 if window is None else min(int(window), 0x7fffffff), kind, float(scale), float(score_bias), value.data_ptr(),
+          _ptr(state), work.data_ptr())
+    return value if state is None else (state, value)
+
+
+# ----------------------------------------------------------------------------- pages
+def cache_reserve_(pools: Union[Tensor, Sequence[Tensor]], table: Tensor, lengths: Tensor, refs: Tensor, counts: Tensor,
+                   page_size: int) -> Tensor:
+    """Makes room for counts[b] more nodes in every sequence, in the order of the sequences: free
+    pages, lowest first, enter the table, and lengths grow. A sequence that grows inside a page that
+    others hold too first gets a copy of it in every pool (all pools whose pages the table names: keys,
+    values and states of every layer).
+
+    counts int32 [batch]. Returns added int32 [batch]: counts[b], or 0 for a sequence that is left
+    as it is because its count is negative, its row of the table is too short, or the pages ran out (from
+    the first sequence that could not be served on, none that needs a page is). Give `added` to
+    ``cache_write_`` and ``cached_propagation`` as their counts."""
+    device, batch, columns, stride = _table(table)
+    _ints("lengths", lengths, (batch,), device)
+    _ints("refs", refs, None, device)
+    _ints("counts", counts, (batch,), device)
+    page_size = _page_size(page_size)
+    pages = refs.numel()
+    named = _Pools(pools, pages, device)
+    added = torch.empty_like(counts)
+    work = _empty((_LIBRARY.jk_cache_reserve_workspace(batch, pages) // 8,), torch.int64, table.device)
+    _call(_LIBRARY.jk_cache_reserve, "jk_cache_reserve", device, named.pointer(), table.data_ptr(), stride, lengths.data_ptr(),
+          refs.data_ptr(), counts.data_ptr(), batch, columns, pages, page_size, added.data_ptr(), work.data_ptr())
+    _written([table, lengths, refs, *named.tensors])
+    return added
+
+
+def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Sequence[Tensor]], table: Tensor, lengths: Tensor,
+                 counts: Optional[Tensor] = None) -> None:
+    """Writes the rows of every sequence's newest nodes into their places.
+
+    pages: one tensor [pages, kv_heads, page_size, width] or [pages, kv_heads, page_size], or several
+    (a layer's keys, values and states); rows: for each [batch, new, kv_heads, width] or [batch, new,
+    kv_heads] of its dtype. Node t of the counts[b] (None: `new`) that a sequence has goes to place
+    lengths[b] - counts[b] + t; places without a page are left out."""
+    pages = [pages] if isinstance(pages, Tensor) else list(pages)
+    rows = [rows] if isinstance(rows, Tensor) else list(rows)
+    device, batch, columns, stride = _table(table)
+    _ints("lengths", lengths, (batch,), device)
+    if counts is not None:
+        _ints("counts", counts, (batch,), device)
+    if len(pages) != len(rows) or not pages:
+        raise ValueError(f"{len(rows)} tensors of rows for {len(pages)} of pages")
+    count = new = heads = page_size = None
+    at, from_ = array.array("Q"), array.array("Q")
+    page_strides, row_strides, widths, sizes = (array.array("q") for _ in range(4))
+    kept = []  # copies of rows, until the launch
+    for i, (p, r) in enumerate(zip(pages, rows)):
+        if not isinstance(p, Tensor) or not isinstance(r, Tensor):
+            raise TypeError(f"pages {i} and rows {i} must be tensors")
+        if p.get_device() != device or r.get_device() != device:
+            raise RuntimeError(f"pages {i} and rows {i} are on {p.device} and {r.device}, expected cuda:{device}")
+        if p.dtype != r.dtype:
+            raise RuntimeError(f"rows {i} has dtype {r.dtype}, expected {p.dtype}")
+        if p.dim() not in (3, 4) or r.dim() != p.dim():
+            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(p.shape)} and {tuple(r.shape)}")
+        if i == 0:
+            (count, heads, page_size), new = p.shape[:3], r.shape[1]
+        if p.shape[:3] != (count, heads, page_size) or r.shape != (batch, new, heads, *p.shape[3:]):
+            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(p.shape)} and {tuple(r.shape)}, which do not fit "
+                             f"{batch} sequences, {new} nodes, {heads} heads and {count} pages of {page_size}")
+        _no_grad(pages=p, rows=r)
+        width = p.shape[3] if p.dim() == 4 else 1
+        page_stride = p.stride()
+        if p.dim() == 4 and width > 1 and page_stride[3] != 1:
+            raise ValueError(f"pages {i} must be contiguous in their last dim")
+        if not (p.is_contiguous() or _one_block(p.shape[1:], page_stride[1:])) or (count > 1 and page_stride[0] < heads * page_size * width):
+            raise ValueError(f"pages {i}: a page must be one block of memory, apart from the other pages")
+        if r.dim() == 4 and width > 1 and r.stride(3) != 1:
+            r = r.contiguous()
+            kept.append(r)
+        at.append(p.data_ptr())
+        from_.append(r.data_ptr())
+        page_strides.extend(page_stride[:3])
+        row_strides.extend(r.stride()[:3])
+        widths.append(width)
+        sizes.append(p.element_size())
+    if not page_size:
+        raise ValueError("page_size is 0")
+    for i in range(0, len(pages), _MAX_WRITE):
+        n = min(_MAX_WRITE, len(pages) - i)
+        _call(_LIBRARY.jk_cache_write, "jk_cache_write", device, at.buffer_info()[0] + 8 * i, page_strides.buffer_info()[0] + 24 * i,
+              from_.buffer_info()[0] + 8 * i, row_strides.buffer_info()[0] + 24 * i, widths.buffer_info()[0] + 8 * i,
+              sizes.buffer_info()[0] + 8 * i, n, table.data_ptr(), stride, lengths.data_ptr(), _ptr(counts), batch, new, heads, count,
+              page_size, columns)
+    _written(pages)
+
+
+def cache_fork_(table: Tensor, lengths: Tensor, refs: Tensor, parents: Tensor, children: Tensor) -> Tensor:
+    """Sequence children[i] becomes a copy of sequence parents[i] as that was before the call, and
+    shares its pages (``cache_reserve_`` copies the last one once either grows in it).
+
+    parents, children int32 [n]: rows of the table. Returns done bool [n]: False, and nothing
+    happens, where a number is outside the batch, the child is not empty (length 0; release it
+    first), or an earlier i names the same child."""
+    device, batch, columns, stride = _table(table)
+    _ints("lengths", lengths, (batch,), device)
+    _ints("refs", refs, None, device)
+    _ints("parents", parents, None, device)
+    _ints("children", children, parents.shape, device)
+    forks = parents.numel()
+    done = torch.empty_like(parents, dtype=torch.bool)
+    work = _empty((_LIBRARY.jk_cache_fork_workspace(batch, forks) // 4,), torch.int32, table.device)
+    _call(_LIBRARY.jk_cache_fork, "jk_cache_fork", device, table.data_ptr(), stride, lengths.data_ptr(), refs.data_ptr(), parents.data_ptr(),
+          children.data_ptr(), forks, batch, columns, refs.numel(), done.data_ptr(), work.data_ptr())
+    _written([table, lengths, refs])
+    return done
+
+
+def cache_release_(table: Tensor, lengths: Tensor, refs: Tensor, new_lengths: Tensor, page_size: int) -> None:
+    """Cuts every sequence back to new_lengths[b] nodes (int32; 0: it ends; one that is longer than the
+    sequence leaves it as it is) and gives up the pages that it no longer needs; those that nobody
+    holds any more are free."""
+    device, batch, columns, stride = _table(table)
+    _ints("lengths", lengths, (batch,), device)
+    _ints("refs", refs, None, device)
+    _ints("new_lengths", new_lengths, (batch,), device)
+    _call(_LIBRARY.jk_cache_release, "jk_cache_release", device, table.data_ptr(), stride, lengths.data_ptr(), refs.data_ptr(),
+          new_lengths.data_ptr(), batch, columns, refs.numel(), _page_size(page_size))
+    _written([table, lengths, refs])
+
+
+def cache_compact_(pools: Union[Tensor, Sequence[Tensor]], table: Tensor, refs: Tensor) -> Tensor:
+    """Moves the pages in use to the front of every pool: with `live` of them, the i-th in use past the
+    first `live` goes to the i-th free one among those. table and refs follow.
+
+    Returns live (int32 scalar on the device): pages [live, ...) are free. What they hold stays as it
+    is until it is written anew, so a step in flight that reads by a copy of the old table is not
+    disturbed. Every table that names the pools' pages has to go into one call."""
+    device, batch, columns, stride = _table(table)
+    _ints("refs", refs, None, device)
+    pages = refs.numel()
+    named = _Pools(pools, pages, device)
+    live = _empty((), torch.int32, table.device)
+    work = _empty((_LIBRARY.jk_cache_compact_workspace(pages) // 4,), torch.int32, table.device)
+    _call(_LIBRARY.jk_cache_compact, "jk_cache_compact", device, named.pointer(), table.data_ptr(), stride, refs.data_ptr(), batch, columns,
+          pages, live.data_ptr(), work.data_ptr())
+    _written([table, refs, *named.tensors])
+    return live
+
+
+def cache_copy_(pools: Union[Tensor, Sequence[Tensor]], src: Tensor, dst: Tensor) -> None:
+    """pool[dst[i]] = pool[src[i]] in every pool, for int32 src and dst [n]. Pairs with a number that
+    is not a page are left out. A page may be read by several pairs; one that is written may be neither
+    read nor written by another pair (its contents would depend on which runs first)."""
+    tensors = [pools] if isinstance(pools, Tensor) else list(pools)
+    if not tensors:
+        raise ValueError("no pools")
+    if not isinstance(tensors[0], Tensor):
+        raise TypeError("pool 0 must be a tensor")
+    if not tensors[0].is_cuda:
+        raise RuntimeError(f"pool 0 must be a CUDA tensor in the b200_sm100a backend (got {tensors[0].device}).")
+    device = tensors[0].get_device()
+    _ints("src", src, None, device)
+    _ints("dst", dst, src.shape, device)
+    pages = tensors[0].shape[0] if tensors[0].dim() else 0
+    named = _Pools(tensors, pages, device)
+    _call(_LIBRARY.jk_cache_copy, "jk_cache_copy", device, named.pointer(), src.data_ptr(), dst.data_ptr(), src.numel(), pages)
+    _written(tensors)
+
+
+# ----------------------------------------------------------------------------- drafted tokens
+def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, uniform: Tensor, counts: Optional[Tensor] = None):
+    """Holds drafted tokens against the target's probabilities, so that what is kept is distributed
+    as the target's own tokens are.
+
+    target [batch, drafted + 1, vocab] and draft [batch, drafted, vocab]: probabilities (f32, bf16 or
+    f16) of the token at each place, draft None: the draft is certain of its tokens; tokens int64 (or
+    int32) [batch, drafted], drawn from the draft; uniform f32 [batch, drafted + 1] random numbers in
+    [0, 1), one to accept each token and the last to draw the new one; counts int32 [batch]: how
+    many tokens a sequence has (None: all).
+
+    Token i is accepted while uniform[i] * draft[i, token] < target[i, token]. At the first place a
+    that is not accepted the new token is drawn from max(target[a] - draft[a], 0) (where that is 0
+    throughout, from target[a]), after the last from target[counts]: the least whose running sum passes
+    uniform[drafted] of the total, in f64. NaN and negative values count as 0.
+
+    Returns (out int64 [batch, drafted + 1]: the accepted tokens, the new one, -1 behind it (and in its
+    place where there is nothing to draw from); accepted int32 [batch]: a)."""
+    code = _check_input("target", target)
+    if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
+        raise ValueError(f"target has shape {tuple(target.shape)}, expected [batch, drafted + 1, vocab]")
+    batch, drafted, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    device = target.get_device()
+    if draft is not None:
+        if not isinstance(draft, Tensor):
+            raise TypeError("draft must be a tensor")
+        if draft.get_device() != device:
+            raise RuntimeError(f"draft is on {draft.device}, expected {target.device}")
+        if draft.dtype != target.dtype:
+            raise RuntimeError(f"draft has dtype {draft.dtype}, expected {target.dtype}")
+        if draft.shape != (batch, drafted, vocab):
+            raise ValueError(f"draft has shape {tuple(draft.shape)}, expected {(batch, drafted, vocab)}")
+        if draft.stride(2) != 1 and vocab > 1:
+            draft = draft.detach().contiguous()
+    for name, t, shape, dtypes in (("tokens", tokens, (batch, drafted), (torch.int64, torch.int32)),
+                                   ("uniform", uniform, (batch, drafted + 1), (torch.float32,))):
+        if not isinstance(t, Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if t.get_device() != device:
+            raise RuntimeError(f"{name} is on {t.device}, expected {target.device}")
+        if t.dtype not in dtypes:
+            raise RuntimeError(f"{name}: unsupported dtype {t.dtype} ({' or '.join(str(d) for d in dtypes)})")
+        if t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if counts is not None:
+        _ints("counts", counts, (batch,), device)
+    if target.stride(2) != 1 and vocab > 1:
+        target = target.detach().contiguous()
+    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    uniform = uniform.detach().contiguous()
+    out = torch.empty((batch, drafted + 1), dtype=torch.int64, device=target.device)
+    accepted = _empty((batch,), torch.int32, target.device)
+    draft_strides = (0, 0) if draft is None else draft.stride()[:2]
+    _call(_LIBRARY.jk_verify_draft, "jk_verify_draft", device, target.data_ptr(), *target.stride()[:2], _ptr(draft), *draft_strides,
+          tokens.data_ptr(), uniform.data_ptr(), _ptr(counts), batch, drafted, vocab, code, out.data_ptr(), accepted.data_ptr())
+    return out, accepted
