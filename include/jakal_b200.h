@@ -513,9 +513,41 @@ int jk_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t
  * go on one stream, or are ordered by events. Strides count elements unless they say bytes.
  */
 
-/* Bytes of the workspace of jk_cached_propagation. */
+/* The cache of a call. refs may be NULL where it is not named below. */
+typedef struct jk_cache {
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* lengths;
+  int32_t* refs;
+  int64_t batch, columns, pages, page_size;
+} jk_cache_t;
+
+/* Nodes to propagate: query [batch, new_nodes, heads, rank]; keys, values, states [pages, kv_heads,
+ * page_size, rank | dim | -], last dim contiguous, strides of the dims before it (query: sequence, node,
+ * head; else page, head, place) in elements; states NULL: none, then out_state is NULL. All in
+ * dtype, any alignment of an element. out_value [batch, new_nodes, heads, dim] and out_state
+ * [batch, new_nodes, heads] contiguous in dtype. workspace: jk_cached_propagation_workspace(...) bytes,
+ * 16-byte aligned. */
+typedef struct jk_nodes {
+  const void* query;
+  int64_t query_stride[3];
+  const void* keys;
+  int64_t key_stride[3];
+  const void* values;
+  int64_t value_stride[3];
+  const void* states;
+  int64_t state_stride[3];
+  const int32_t* counts;
+  int64_t new_nodes, heads, kv_heads, rank, dim, dtype, window, compress;
+  void* out_value;
+  void* out_state;
+  void* workspace;
+} jk_nodes_t;
+
+/* Bytes of the workspace of jk_cached_propagation (0: none is needed). */
 int64_t jk_cached_propagation_workspace(int64_t batch, int64_t new_nodes, int64_t heads, int64_t kv_heads,
-                                        int64_t dim, int64_t page_size, int64_t columns, int dtype);
+                                        int64_t rank, int64_t dim, int64_t page_size, int64_t columns,
+                                        int64_t window, int dtype);
 
 /* Propagation of the last n = counts[b] (NULL: new_nodes; clamped to [0, new_nodes]) nodes of every
  * sequence over the nodes before them and themselves. Node t of the n is at place
@@ -525,21 +557,11 @@ int64_t jk_cached_propagation_workspace(int64_t batch, int64_t new_nodes, int64_
  *   out_value[b, t, h] = sum_j w_j values[j],  out_state[b, t, h] = sum_j w_j states[j]
  * with compress JK_SOFTMAX, JK_SOFTSIGN or JK_SIGNED_ABS_SOFTMAX. A node that sees none, and nodes
  * t >= n, have zeros; a softmax over scores that are all -inf is NaN. What places that are not
- * seen hold (NaN, infinities) has no part in a result.
- * query [batch, new_nodes, heads, rank], keys, values, states (NULL: none; then out_state is NULL) in
- * dtype, last dim contiguous, any alignment of an element; outputs contiguous in dtype.
- * rank <= 256, dim <= 512, new_nodes <= 64, heads a multiple of kv_heads. Sums are f32; 16-bit weights
- * go into the value product as two planes (16 significant bits and more). workspace:
- * jk_cached_propagation_workspace(...) bytes, 16-byte aligned. */
-int jk_cached_propagation(const void* query, int64_t query_stride_b, int64_t query_stride_t, int64_t query_stride_h,
-                          const void* keys, int64_t key_stride_p, int64_t key_stride_h, int64_t key_stride_n,
-                          const void* values, int64_t value_stride_p, int64_t value_stride_h, int64_t value_stride_n,
-                          const void* states, int64_t state_stride_p, int64_t state_stride_h, int64_t state_stride_n,
-                          const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* counts,
-                          int64_t batch, int64_t new_nodes, int64_t heads, int64_t kv_heads, int64_t rank,
-                          int64_t dim, int64_t pages, int64_t page_size, int64_t columns, int dtype,
-                          int64_t window, int compress, float scale, float score_bias, void* out_value,
-                          void* out_state, void* workspace, jk_stream_t stream);
+ * seen hold (NaN, infinities) has no part in a result. Sums are f32; 16-bit weights go into the value
+ * product as two planes (16 significant bits and more).
+ * rank <= 256, dim <= 512, new_nodes <= 64, heads a multiple of kv_heads. */
+int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* nodes, float scale, float score_bias,
+                          jk_stream_t stream);
 
 /* Pools of a call: HOST arrays of `count` entries (at most 512), read during the call: the pools'
  * addresses, the bytes of a page and the bytes from one page to the next. */
@@ -559,21 +581,27 @@ int64_t jk_cache_reserve_workspace(int64_t batch, int64_t pages);
  * in every pool and gives up its reference. added[b] (int32 [batch]) is counts[b], or 0 where the
  * sequence is left as it is: a negative count, more nodes than the table's row has room for, or
  * pages that ran out (from the first sequence that could not be served on, none that needs a page
- * is). workspace: jk_cache_reserve_workspace(...) bytes, 16-byte aligned. */
-int jk_cache_reserve(const jk_pools_t* pools, int32_t* table, int64_t table_stride, int32_t* lengths,
-                     int32_t* refs, const int32_t* counts, int64_t batch, int64_t columns, int64_t pages,
-                     int64_t page_size, int32_t* added, void* workspace, jk_stream_t stream);
+ * is). Needs refs. workspace: jk_cache_reserve_workspace(...) bytes, 16-byte aligned. */
+int jk_cache_reserve(const jk_pools_t* pools, const jk_cache_t* cache, const int32_t* counts, int32_t* added,
+                     void* workspace, jk_stream_t stream);
 
-/* Writes rows[i] [batch, new_nodes, heads, width] into pages[i] [pages, heads, page_size, width]
- * for `count` (at most 64) pairs: node t < n = counts[b] (NULL: new_nodes; clamped to [0, new_nodes]) of
- * sequence b goes to place lengths[b] - n + t, if the table has a page for it. HOST arrays: addresses; strides,
- * three a tensor (page, head, node; batch, node, head), elements; widths; element sizes in bytes
- * (1, 2, 4, 8). Rows are contiguous inside. */
-int jk_cache_write(void* const* pages_data, const int64_t* pages_strides, const void* const* rows_data,
-                   const int64_t* rows_strides, const int64_t* widths, const int64_t* element_bytes, int64_t count,
-                   const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* counts,
-                   int64_t batch, int64_t new_nodes, int64_t heads, int64_t pages, int64_t page_size,
-                   int64_t columns, jk_stream_t stream);
+/* Rows to write, rows[i] [batch, new_nodes, heads, width] into pages[i] [pages, heads, page_size, width]
+ * for `count` (at most 64) pairs. HOST arrays: addresses; strides, three a tensor (page, head, place;
+ * sequence, node, head) in elements; widths; element sizes in bytes (1, 2, 4, 8). Rows are contiguous
+ * inside. */
+typedef struct jk_rows {
+  void* const* pages_data;
+  const int64_t* pages_strides;
+  const void* const* rows_data;
+  const int64_t* rows_strides;
+  const int64_t* widths;
+  const int64_t* element_bytes;
+  int64_t count, new_nodes, heads;
+} jk_rows_t;
+
+/* Node t < n = counts[b] (NULL: new_nodes; clamped to [0, new_nodes]) of sequence b goes to place
+ * lengths[b] - n + t, if the table has a page for it. */
+int jk_cache_write(const jk_rows_t* rows, const jk_cache_t* cache, const int32_t* counts, jk_stream_t stream);
 
 /* Bytes of the workspace of jk_cache_fork. */
 int64_t jk_cache_fork_workspace(int64_t batch, int64_t forks);
@@ -581,26 +609,24 @@ int64_t jk_cache_fork_workspace(int64_t batch, int64_t forks);
 /* Sequence children[i] becomes a copy of sequence parents[i] as that was when the call began; its
  * pages are shared (one more reference each). done[i] (bytes, 0 or 1) is 0, and nothing happens,
  * where a number is outside the batch, the child is not empty (length 0), or an earlier i names the
- * same child. workspace: jk_cache_fork_workspace(...) bytes, 16-byte aligned. */
-int jk_cache_fork(int32_t* table, int64_t table_stride, int32_t* lengths, int32_t* refs, const int32_t* parents,
-                  const int32_t* children, int64_t forks, int64_t batch, int64_t columns, int64_t pages,
+ * same child. Needs refs. workspace: jk_cache_fork_workspace(...) bytes, 16-byte aligned. */
+int jk_cache_fork(const jk_cache_t* cache, const int32_t* parents, const int32_t* children, int64_t forks,
                   uint8_t* done, void* workspace, jk_stream_t stream);
 
 /* Sequences are cut to new_lengths[b] nodes (clamped to [0, lengths[b]]): table entries past the last
- * page that is still needed give up their references and become -1. new_lengths may be lengths. */
-int jk_cache_release(int32_t* table, int64_t table_stride, int32_t* lengths, int32_t* refs,
-                     const int32_t* new_lengths, int64_t batch, int64_t columns, int64_t pages,
-                     int64_t page_size, jk_stream_t stream);
+ * page that is still needed give up their references and become -1. new_lengths may be lengths.
+ * Needs refs. */
+int jk_cache_release(const jk_cache_t* cache, const int32_t* new_lengths, jk_stream_t stream);
 
 /* Bytes of the workspace of jk_cache_compact. */
 int64_t jk_cache_compact_workspace(int64_t pages);
 
 /* Moves the pages in use (refs > 0) to the front: with live of them, the i-th in use at or past `live`
  * goes to the i-th free one before it, in every pool; table and refs follow, live (device int32)
- * receives their number. The pages that were moved from keep their contents. workspace:
- * jk_cache_compact_workspace(pages) bytes, 16-byte aligned. */
-int jk_cache_compact(const jk_pools_t* pools, int32_t* table, int64_t table_stride, int32_t* refs, int64_t batch,
-                     int64_t columns, int64_t pages, int32_t* live, void* workspace, jk_stream_t stream);
+ * receives their number. The pages that were moved from keep their contents. Needs refs (lengths may
+ * be NULL). workspace: jk_cache_compact_workspace(pages) bytes, 16-byte aligned. */
+int jk_cache_compact(const jk_pools_t* pools, const jk_cache_t* cache, int32_t* live, void* workspace,
+                     jk_stream_t stream);
 
 /* pool[dst[i]] = pool[src[i]] in every pool, for int32 src, dst [n]; pairs with a number outside
  * [0, pages) are left out. A page may be read by several pairs; one that a pair writes may be neither
@@ -608,22 +634,33 @@ int jk_cache_compact(const jk_pools_t* pools, int32_t* table, int64_t table_stri
 int jk_cache_copy(const jk_pools_t* pools, const int32_t* src, const int32_t* dst, int64_t n, int64_t pages,
                   jk_stream_t stream);
 
+/* Drafted tokens: target [batch, drafted + 1, vocab] and draft [batch, drafted, vocab] (NULL: the draft is
+ * certain of its tokens) in dtype, rows contiguous, strides of the first two dims in elements; tokens
+ * int64 [batch, drafted], uniform f32 [batch, drafted + 1], contiguous; counts int32 [batch] or NULL.
+ * out_tokens int64 [batch, drafted + 1], accepted int32 [batch]. */
+typedef struct jk_draft {
+  const void* target;
+  int64_t target_stride[2];
+  const void* draft;
+  int64_t draft_stride[2];
+  const int64_t* tokens;
+  const float* uniform;
+  const int32_t* counts;
+  int64_t batch, drafted, vocab, dtype;
+  int64_t* out_tokens;
+  int32_t* accepted;
+} jk_draft_t;
+
 /* Verification of drafted tokens. Sequence b has n = counts[b] (NULL: drafted; clamped to [0, drafted])
  * drafted tokens x_i, drawn from draft[b, i, :], and the target's probabilities target[b, i, :] for
- * i <= n. Token i is accepted while uniform[b, i] * draft[b, i, x_i] < target[b, i, x_i] (exact);
- * with the first a that is not (a = n: all are), out_tokens[b, a] is the least j with
+ * i <= n. Token i is accepted while uniform[b, i] * draft[b, i, x_i] < target[b, i, x_i] (exact; draft
+ * NULL: probability 1); with the first a that is not (a = n: all are), out_tokens[b, a] is the least j with
  *   sum_{j' <= j} r_j' > uniform[b, drafted] * sum r,
  * r = max(target[b, a] - draft[b, a], 0) for a < n (target[b, a] where that is 0 throughout), target[b, n]
- * for a = n, in f64. draft NULL: the draft is certain of its tokens (probability 1). NaN and negative
- * values count as 0; a token outside the vocabulary is not accepted; where r has no positive entry
- * out_tokens[b, a] is -1.
- * target [batch, drafted + 1, vocab], draft [batch, drafted, vocab] in dtype, rows contiguous; tokens
- * int64 [batch, drafted], uniform f32 [batch, drafted + 1], contiguous. out_tokens int64 [batch, drafted + 1]: the
- * accepted tokens, the new one, -1 behind it; accepted int32 [batch]: a. vocab <= 2^30. */
-int jk_verify_draft(const void* target, int64_t target_stride_b, int64_t target_stride_t, const void* draft,
-                    int64_t draft_stride_b, int64_t draft_stride_t, const int64_t* tokens, const float* uniform,
-                    const int32_t* counts, int64_t batch, int64_t drafted, int64_t vocab, int dtype,
-                    int64_t* out_tokens, int32_t* accepted, jk_stream_t stream);
+ * for a = n, in f64. NaN and negative values count as 0; a token outside the vocabulary is not
+ * accepted; where r has no positive entry out_tokens[b, a] is -1. Before it stand the accepted tokens,
+ * behind it -1; accepted[b] is a. vocab <= 2^30. */
+int jk_verify_draft(const jk_draft_t* draft, jk_stream_t stream);
 
 /* Failure-path test entry (no reference counterpart): jk_propagation_window_forward
  * (softsign, no bias) with a producer warp that issues no load and no MMA, so every consumer

@@ -448,13 +448,18 @@ inline int check_pools(const jk_pools_t* q, int64_t pages) {
   return JK_OK;
 }
 
-inline int check_table(const int32_t* table, int64_t stride, int64_t batch, int64_t columns, int64_t pages) {
-  if (batch < 0 || columns < 0 || pages < 0 || batch > 0x7fffffff || columns > 0x7fffffff || pages > 0x7fffffff || stride < 0)
+inline int check_cache(const jk_cache_t* c) {
+  if (c == nullptr) return JK_ERR_BAD_ARG;
+  constexpr int64_t most = 0x7fffffff;
+  if (c->batch < 0 || c->columns < 0 || c->pages < 0 || c->batch > most || c->columns > most || c->pages > most || c->table_stride < 0 ||
+      c->page_size < 1 || c->page_size > most)
     return JK_ERR_BAD_SHAPE;
-  if (batch > 1 && stride < columns) return JK_ERR_BAD_SHAPE;  // rows would overlap
-  if (batch > 0 && columns > 0 && table == nullptr) return JK_ERR_BAD_ARG;
+  if (c->batch > 1 && c->table_stride < c->columns) return JK_ERR_BAD_SHAPE;  // rows would overlap
+  if (c->batch > 0 && c->columns > 0 && c->table == nullptr) return JK_ERR_BAD_ARG;
   return JK_OK;
 }
+
+inline Table table_of(const jk_cache_t* c) { return Table{c->table, c->table_stride, c->batch, c->columns, c->pages}; }
 
 inline unsigned copy_grid(int64_t pairs, uint32_t per) {
   const int64_t warps = pairs > (int64_t(1) << 30) / (per + 1) ? int64_t(1) << 30 : pairs * per;
@@ -494,16 +499,15 @@ int64_t jk_cache_reserve_workspace(int64_t batch, int64_t pages) {
   return jk::cache::round16(batch * 8) + 2 * jk::cache::round16(batch * 4) + jk::cache::round16(batch * 8) + jk::cache::round16(pages * 4);
 }
 
-int jk_cache_reserve(const jk_pools_t* pools, int32_t* table, int64_t table_stride, int32_t* lengths, int32_t* refs,
-                     const int32_t* counts, int64_t batch, int64_t columns, int64_t pages, int64_t page_size, int32_t* added,
-                     void* workspace, jk_stream_t stream) {
+int jk_cache_reserve(const jk_pools_t* pools, const jk_cache_t* cache, const int32_t* counts, int32_t* added, void* workspace,
+                     jk_stream_t stream) {
   using namespace jk;
   using namespace jk::cache;
+  if (int st = check_cache(cache)) return st;
+  const int64_t batch = cache->batch, pages = cache->pages;
   if (int st = check_pools(pools, pages)) return st;
-  if (int st = check_table(table, table_stride, batch, columns, pages)) return st;
-  if (page_size < 1 || page_size > 0x7fffffff) return JK_ERR_BAD_SHAPE;
-  if (batch > 0 && (lengths == nullptr || counts == nullptr || added == nullptr || workspace == nullptr)) return JK_ERR_BAD_ARG;
-  if (pages > 0 && refs == nullptr) return JK_ERR_BAD_ARG;
+  if (batch > 0 && (cache->lengths == nullptr || counts == nullptr || added == nullptr || workspace == nullptr)) return JK_ERR_BAD_ARG;
+  if (pages > 0 && cache->refs == nullptr) return JK_ERR_BAD_ARG;
   if (!aligned16(workspace)) return JK_ERR_ALIGNMENT;
   if (int st = check_device()) return st;
   if (batch == 0) return JK_OK;
@@ -515,42 +519,40 @@ int jk_cache_reserve(const jk_pools_t* pools, int32_t* table, int64_t table_stri
   w.pairs = reinterpret_cast<int32_t*>(p), p += round16(batch * 8);
   w.free = reinterpret_cast<int32_t*>(p);
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  reserve_kernel<<<1, kOne, 0, s>>>(Table{table, table_stride, batch, columns, pages}, lengths, refs, counts, page_size, added, w);
+  reserve_kernel<<<1, kOne, 0, s>>>(table_of(cache), cache->lengths, cache->refs, counts, cache->page_size, added, w);
   if (int st = launch_status()) return st;
   if (pools->count == 0) return JK_OK;
   const Pairs pairs{w.pairs, w.pairs + 1, 2, batch, nullptr};
   return pools->count <= kSmall ? launch_copy<kSmall>(*pools, pairs, batch, pages, s) : launch_copy<kLarge>(*pools, pairs, batch, pages, s);
 }
 
-int jk_cache_write(void* const* pages_data, const int64_t* pages_strides, const void* const* rows_data, const int64_t* rows_strides,
-                   const int64_t* widths, const int64_t* element_bytes, int64_t count, const int32_t* table, int64_t table_stride,
-                   const int32_t* lengths, const int32_t* counts, int64_t batch, int64_t new_nodes, int64_t heads, int64_t pages,
-                   int64_t page_size, int64_t columns, jk_stream_t stream) {
+int jk_cache_write(const jk_rows_t* q, const jk_cache_t* cache, const int32_t* counts, jk_stream_t stream) {
   using namespace jk;
   using namespace jk::cache;
+  if (q == nullptr) return JK_ERR_BAD_ARG;
+  const int64_t count = q->count, new_nodes = q->new_nodes, heads = q->heads;
   if (count < 0 || count > kMaxWrite) return JK_ERR_BAD_SHAPE;
-  if (int st = check_table(table, table_stride, batch, columns, pages)) return st;
-  if (page_size < 1 || page_size > 0x7fffffff || new_nodes < 0 || heads < 0) return JK_ERR_BAD_SHAPE;
-  if (count > 0 && (pages_data == nullptr || pages_strides == nullptr || rows_data == nullptr || rows_strides == nullptr ||
-                    widths == nullptr || element_bytes == nullptr))
+  if (int st = check_cache(cache)) return st;
+  if (new_nodes < 0 || heads < 0 || new_nodes > 0x7fffffff || heads > 0x7fffffff) return JK_ERR_BAD_SHAPE;
+  if (count > 0 && (q->pages_data == nullptr || q->pages_strides == nullptr || q->rows_data == nullptr || q->rows_strides == nullptr ||
+                    q->widths == nullptr || q->element_bytes == nullptr))
     return JK_ERR_BAD_ARG;
-  if (new_nodes > 0x7fffffff || heads > 0x7fffffff) return JK_ERR_BAD_SHAPE;
-  const int64_t nodes = batch * new_nodes;  // below 2^62
+  const int64_t nodes = cache->batch * new_nodes;  // below 2^62
   if (nodes > 0 && heads > 0x7fffffff / nodes) return JK_ERR_BAD_SHAPE;
-  const int64_t rows = nodes * heads;
+  const int64_t rows = nodes * heads, pages = cache->pages;
   Write w;
   int most = 0;
   for (int64_t i = 0; i < count; ++i) {
-    const int64_t size = element_bytes[i];
+    const int64_t size = q->element_bytes[i];
     if (size != 1 && size != 2 && size != 4 && size != 8) return JK_ERR_BAD_DTYPE;
-    if (widths[i] < 0 || widths[i] > 0x7fffffff) return JK_ERR_BAD_SHAPE;
-    if (rows > 0 && widths[i] > 0 && (rows_data[i] == nullptr || (pages > 0 && pages_data[i] == nullptr))) return JK_ERR_BAD_ARG;
-    w.pages[i] = static_cast<char*>(pages_data[i]);
-    w.rows[i] = static_cast<const char*>(rows_data[i]);
-    w.bytes[i] = widths[i] * size;
+    if (q->widths[i] < 0 || q->widths[i] > 0x7fffffff) return JK_ERR_BAD_SHAPE;
+    if (rows > 0 && q->widths[i] > 0 && (q->rows_data[i] == nullptr || (pages > 0 && q->pages_data[i] == nullptr))) return JK_ERR_BAD_ARG;
+    w.pages[i] = static_cast<char*>(q->pages_data[i]);
+    w.rows[i] = static_cast<const char*>(q->rows_data[i]);
+    w.bytes[i] = q->widths[i] * size;
     for (int j = 0; j < 3; ++j) {
-      w.page_stride[i][j] = pages_strides[3 * i + j] * size;
-      w.row_stride[i][j] = rows_strides[3 * i + j] * size;
+      w.page_stride[i][j] = q->pages_strides[3 * i + j] * size;
+      w.row_stride[i][j] = q->rows_strides[3 * i + j] * size;
     }
     w.unit[i] = static_cast<uint8_t>(size);
     // as many lanes as a row has blocks (one more where it begins inside a block), a power of 2
@@ -560,14 +562,14 @@ int jk_cache_write(void* const* pages_data, const int64_t* pages_strides, const 
     w.lanes_log2[i] = static_cast<uint8_t>(log2);
     if (log2 > most) most = log2;
   }
-  if (rows > 0 && lengths == nullptr) return JK_ERR_BAD_ARG;
+  if (rows > 0 && cache->lengths == nullptr) return JK_ERR_BAD_ARG;
   if (int st = check_device()) return st;
-  if (rows == 0 || count == 0 || pages == 0 || columns == 0) return JK_OK;
+  if (rows == 0 || count == 0 || pages == 0 || cache->columns == 0) return JK_OK;
   const int64_t grid = ((rows << most) + kThreads - 1) / kThreads;
   if (grid > 0x7fffffff) return JK_ERR_BAD_SHAPE;
   write_kernel<<<dim3(static_cast<unsigned>(grid), static_cast<unsigned>(count)), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      w, table, table_stride, lengths, counts, static_cast<uint32_t>(rows), static_cast<uint32_t>(new_nodes), static_cast<uint32_t>(heads), pages,
-      static_cast<uint32_t>(page_size), columns);
+      w, cache->table, cache->table_stride, cache->lengths, counts, static_cast<uint32_t>(rows), static_cast<uint32_t>(new_nodes),
+      static_cast<uint32_t>(heads), pages, static_cast<uint32_t>(cache->page_size), cache->columns);
   return launch_status();
 }
 
@@ -576,18 +578,20 @@ int64_t jk_cache_fork_workspace(int64_t batch, int64_t forks) {
   return jk::cache::round16(batch * 4) + jk::cache::round16(forks * 4);
 }
 
-int jk_cache_fork(int32_t* table, int64_t table_stride, int32_t* lengths, int32_t* refs, const int32_t* parents, const int32_t* children,
-                  int64_t forks, int64_t batch, int64_t columns, int64_t pages, uint8_t* done, void* workspace, jk_stream_t stream) {
+int jk_cache_fork(const jk_cache_t* cache, const int32_t* parents, const int32_t* children, int64_t forks, uint8_t* done, void* workspace,
+                  jk_stream_t stream) {
   using namespace jk;
   using namespace jk::cache;
-  if (int st = check_table(table, table_stride, batch, columns, pages)) return st;
+  if (int st = check_cache(cache)) return st;
+  const int64_t batch = cache->batch, columns = cache->columns;
   if (forks < 0 || forks > 0x7ffffffe) return JK_ERR_BAD_SHAPE;
   if (forks > 0 && (parents == nullptr || children == nullptr || done == nullptr || workspace == nullptr)) return JK_ERR_BAD_ARG;
-  if ((batch > 0 && lengths == nullptr) || (pages > 0 && refs == nullptr)) return JK_ERR_BAD_ARG;
+  if ((batch > 0 && cache->lengths == nullptr) || (cache->pages > 0 && cache->refs == nullptr)) return JK_ERR_BAD_ARG;
   if (!aligned16(workspace)) return JK_ERR_ALIGNMENT;
   if (int st = check_device()) return st;
   if (forks == 0) return JK_OK;
-  const Table t{table, table_stride, batch, columns, pages};
+  const Table t = table_of(cache);
+  int32_t *lengths = cache->lengths, *refs = cache->refs;
   auto* taken = static_cast<int32_t*>(workspace);
   auto* copied = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + round16(batch * 4));
   auto s = reinterpret_cast<cudaStream_t>(stream);
@@ -600,18 +604,17 @@ int jk_cache_fork(int32_t* table, int64_t table_stride, int32_t* lengths, int32_
   return launch_status();
 }
 
-int jk_cache_release(int32_t* table, int64_t table_stride, int32_t* lengths, int32_t* refs, const int32_t* new_lengths, int64_t batch,
-                     int64_t columns, int64_t pages, int64_t page_size, jk_stream_t stream) {
+int jk_cache_release(const jk_cache_t* cache, const int32_t* new_lengths, jk_stream_t stream) {
   using namespace jk;
   using namespace jk::cache;
-  if (int st = check_table(table, table_stride, batch, columns, pages)) return st;
-  if (page_size < 1 || page_size > 0x7fffffff) return JK_ERR_BAD_SHAPE;
-  if (batch > 0 && (lengths == nullptr || new_lengths == nullptr)) return JK_ERR_BAD_ARG;
-  if (pages > 0 && refs == nullptr) return JK_ERR_BAD_ARG;
+  if (int st = check_cache(cache)) return st;
+  const int64_t batch = cache->batch;
+  if (batch > 0 && (cache->lengths == nullptr || new_lengths == nullptr)) return JK_ERR_BAD_ARG;
+  if (cache->pages > 0 && cache->refs == nullptr) return JK_ERR_BAD_ARG;
   if (int st = check_device()) return st;
   if (batch == 0) return JK_OK;
   release_kernel<<<static_cast<unsigned>(batch < kMaxBlocks ? batch : kMaxBlocks), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      Table{table, table_stride, batch, columns, pages}, lengths, refs, new_lengths, page_size);
+      table_of(cache), cache->lengths, cache->refs, new_lengths, cache->page_size);
   return launch_status();
 }
 
@@ -620,13 +623,13 @@ int64_t jk_cache_compact_workspace(int64_t pages) {
   return 16 + 3 * jk::cache::round16(pages * 4);
 }
 
-int jk_cache_compact(const jk_pools_t* pools, int32_t* table, int64_t table_stride, int32_t* refs, int64_t batch, int64_t columns,
-                     int64_t pages, int32_t* live, void* workspace, jk_stream_t stream) {
+int jk_cache_compact(const jk_pools_t* pools, const jk_cache_t* cache, int32_t* live, void* workspace, jk_stream_t stream) {
   using namespace jk;
   using namespace jk::cache;
+  if (int st = check_cache(cache)) return st;
+  const int64_t pages = cache->pages;
   if (int st = check_pools(pools, pages)) return st;
-  if (int st = check_table(table, table_stride, batch, columns, pages)) return st;
-  if (live == nullptr || workspace == nullptr || (pages > 0 && refs == nullptr)) return JK_ERR_BAD_ARG;
+  if (live == nullptr || workspace == nullptr || (pages > 0 && cache->refs == nullptr)) return JK_ERR_BAD_ARG;
   if (!aligned16(workspace)) return JK_ERR_ALIGNMENT;
   if (int st = check_device()) return st;
   char* p = static_cast<char*>(workspace);
@@ -636,9 +639,9 @@ int jk_cache_compact(const jk_pools_t* pools, int32_t* table, int64_t table_stri
   w.to = reinterpret_cast<int32_t*>(p), p += round16(pages * 4);
   w.map = reinterpret_cast<int32_t*>(p);
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  compact_kernel<<<1, kOne, 0, s>>>(refs, pages, live, w);
+  compact_kernel<<<1, kOne, 0, s>>>(cache->refs, pages, live, w);
   if (int st = launch_status()) return st;
-  const Table t{table, table_stride, batch, columns, pages};
+  const Table t = table_of(cache);
   return pools->count <= kSmall ? launch_move<kSmall>(*pools, t, live, w, s) : launch_move<kLarge>(*pools, t, live, w, s);
 }
 

@@ -12,8 +12,9 @@
 //     from what they leave: reference, sum and unnormalised values. Few tiles a unit: a block each, and
 //     no second kernel.
 //   * A warp has every fourth 16 places of the run to itself: its own ring of shared memory fed by
-//     asynchronous copies, its own running maximum and sums, no barrier between warps until the run's
-//     end, where the four are joined in shared memory.
+//     asynchronous copies, its own reference and sums, no barrier between warps until the run's end,
+//     where the four are joined in shared memory. Its turn is short of instructions, as few warps fit an
+//     SM beside their rings: 16 places that all rows see, of one page, need no masks and one address.
 // 16-bit types: both products are warp matrix instructions with the places (scores) and the value's
 // columns (sums) as their 16 rows, and the unit's rows as their 8 columns, of which one node of one head
 // fills one: S^T = K Q^T, O^T = V^T W^T. W^T leaves the first product with places across the wrong
@@ -21,7 +22,8 @@
 // high + low, so their rounding (2^-16 and less) is far below that of the result.
 // f32: the same walk with fused multiply-adds, which keep f32's rounding.
 // Exponentials are base 2 on a reference that is itself rounded, so partial sums with different
-// references join without a rounding of their own.
+// references join without a rounding of their own. The reference follows the maximum only once that is
+// 8 (a factor of 256) above it: a vote a turn, in place of a maximum over the warp.
 //
 // What is not seen has no part in a result, whatever it holds: places past the last node and places
 // without a page arrive as zeros, and a tile of which rows see different parts (the newest nodes of a
@@ -30,6 +32,7 @@
 
 #include "jk_host.h"
 #include "jk_rows.cuh"
+#include "jk_sm100.cuh"
 
 #include <type_traits>
 
@@ -41,10 +44,12 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kKeys = 16;               // places of a warp's turn
 constexpr int kTile = kWarps * kKeys;   // places of a block's turn
 constexpr int kSms = 148;
+constexpr int kMaxPerSm = 3;            // blocks of an SM
 constexpr int kMaxBatch = 1024;         // sequences of a launch
 constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
 constexpr int kUnitTiles = 8;           // units of at most so many tiles get a block each
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.0f;          // by which a score may pass its row's reference, in units of log 2
 
 struct Args {
   const char *query, *keys, *values, *states;  // states null: none
@@ -61,9 +66,10 @@ struct Args {
   int32_t blocks, row_blocks, rows;       // blocks of the grid; row blocks of a unit's rows, and rows of one
   int32_t key_chunk, value_chunk;         // bytes of one asynchronous copy (16, 8, 4), 0: element by element
   int32_t key_row, value_row;             // elements of a row in shared memory
-  int32_t stages, stage_bytes, ring_bytes;
+  int32_t key_cols;                       // of a key's row read: rank rounded up to the product's steps
+  int32_t stages, stage_bytes;
+  bool blocks16;                          // rows of keys and values are in 16-byte blocks
   int32_t part_row;                       // floats of a row that a block leaves: dim rounded up to 4, reference, sum, state
-  int64_t* plan;                          // [batch + 2]: tiles of a block, tiles before each sequence
   float* parts;                           // [blocks][2][rows][part_row]
   bool split;
 };
@@ -155,41 +161,34 @@ __device__ __forceinline__ void copy_wait(int pending) {
 
 // ---- compressors
 
-// A score (the bare product) as the compressor takes it: z, whose maximum is the reference (log2 units).
-__device__ __forceinline__ float level(int compress, float dot, float scale, float bias) {
-  if (compress == JK_SOFTMAX) return dot * scale;  // scale has log2(e) in it
-  return fabsf(fmaf(dot, scale, bias)) * kLog2e;
-}
-// Its weight before normalisation, on reference `ref` (unused by softsign).
-__device__ __forceinline__ float weight(int compress, float dot, float scale, float bias, float ref) {
-  if (compress == JK_SOFTMAX) return exp2f(fmaf(dot, scale, -ref));
-  const float s = fmaf(dot, scale, bias);
-  if (compress == JK_SOFTSIGN) return s / (1.0f + fabsf(s));
-  return exp2f(fmaf(fabsf(s), kLog2e, -ref));  // the sign is put on after the sum
-}
-__device__ __forceinline__ float signed_weight(int compress, float dot, float scale, float bias, float w) {
-  if (compress != JK_SIGNED_ABS_SOFTMAX) return w;
-  const float s = fmaf(dot, scale, bias);
-  return s > 0.0f ? w : s < 0.0f ? -w : s == 0.0f ? 0.0f : s;  // NaN stays
+__device__ __forceinline__ float power2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// What one warp has of a tile: shared memory of one stage, then the walk's own words.
-struct Stage {
-  char* keys;
-  char* values;
-  float* states;   // [kKeys]
-  uint32_t* seen;  // bit i: place i of the tile is in the cache
-};
-
-struct Layout {
-  char* base;
-  int32_t key_bytes, value_bytes, stage_bytes;
-  __device__ __forceinline__ Stage at(int i) const {
-    char* p = base + i * stage_bytes;
-    char* words = p + key_bytes + value_bytes;
-    return Stage{p, p + key_bytes, reinterpret_cast<float*>(words), reinterpret_cast<uint32_t*>(words + 4 * kKeys)};
-  }
-};
+// What a product becomes: for the softmax nothing yet (its scale has log2(e) in it), else the score.
+template <int COMPRESS>
+__device__ __forceinline__ float score_of(float dot, float scale, float bias) {
+  return COMPRESS == JK_SOFTMAX ? dot : fmaf(dot, scale, bias);
+}
+// Its level, which is held against the reference (units of log 2).
+template <int COMPRESS>
+__device__ __forceinline__ float level_of(float s, float scale) {
+  return COMPRESS == JK_SOFTMAX ? s * scale : fabsf(s) * kLog2e;
+}
+// Its part of the sum, on the reference (softsign: the weight itself).
+template <int COMPRESS>
+__device__ __forceinline__ float mass_of(float s, float scale, float ref) {
+  if (COMPRESS == JK_SOFTSIGN) return s / (1.0f + fabsf(s));
+  return power2(COMPRESS == JK_SOFTMAX ? fmaf(s, scale, -ref) : fmaf(fabsf(s), kLog2e, -ref));
+}
+// Its weight.
+template <int COMPRESS>
+__device__ __forceinline__ float weight_of(float s, float mass) {
+  if (COMPRESS != JK_SIGNED_ABS_SOFTMAX) return mass;
+  return s == 0.0f ? 0.0f : copysignf(mass, s);
+}
 
 template <typename T, int BYTES>
 __device__ __forceinline__ void load_chunks(char* dst, int32_t dst_row, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
@@ -223,22 +222,42 @@ __device__ __forceinline__ void load_rows(char* dst, int32_t dst_row, const char
 
 // ---- the kernel
 
+// A turn on its way: which of its places are in the cache and count, and the state of this lane's (lane % 16).
+struct Turn {
+  uint32_t there;
+  float state;
+};
+
 // ROWS: rows of a unit that a block takes (a multiple of 8 for 16-bit types); DIM: columns of the value at most.
-template <typename T, int ROWS, int DIM>
-__global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant__ Args a) {
+// BULK: rows of keys and values are in 16-byte blocks, so each lane copies one row by one instruction (lanes 0-15 the keys,
+// the others the values). Else rows are copied in pieces of the size that their alignment allows.
+template <typename T, int ROWS, int DIM, int COMPRESS, bool BULK>
+__global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) cached_kernel(const __grid_constant__ Args a) {
   constexpr bool kWide = std::is_same_v<T, float>;
   constexpr int NT = kWide ? 1 : ROWS / 8;             // 8-row tiles of the matrix instructions
   constexpr int MT = kWide ? 1 : DIM / 16;             // 16-column tiles of the value
-  constexpr int CT = kWide ? DIM / 32 : 1;             // f32: columns of a lane
-  constexpr int OWN = kWide ? ROWS : 2 * NT;           // rows whose reference and sum a thread keeps
+  constexpr int CP = kWide ? DIM / 64 : 1;             // f32: pairs of columns of a lane, 64 columns apart
+  // rows whose reference and sum a thread keeps (f32: half of them, lanes 16.. the other half)
+  constexpr int OWN = kWide ? (ROWS + 1) / 2 : 2 * NT;
+  constexpr int SIZE = sizeof(T);
   extern __shared__ __align__(16) char memory[];
   __shared__ int64_t before[kMaxBatch + 1];
   __shared__ int64_t scan[kWarps];
   __shared__ float ref_s[kWarps][ROWS], sum_s[kWarps][ROWS], state_s[kWarps][ROWS];
+  __shared__ uint64_t landed[kWarps][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t issued = 0, taken = 0;  // BULK: this warp's turns that copied something, of all units
+  bool late = false;               // a wait gave up
+  if (BULK && lane == 0) {
+    mbar_init(&landed[warp][0], 1);
+    mbar_init(&landed[warp][1], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
 
-  // tiles before each sequence
-  {
+  int64_t chunk = 1, at = 0, until = 1;
+  if (a.split) {
+    // tiles before each sequence
     int64_t carry = 0;
     if (tid == 0) before[0] = 0;
     for (int32_t base = 0; base < a.batch; base += kThreads) {
@@ -261,31 +280,20 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
       if (b < a.batch) before[b + 1] = v + add;
     }
     __syncthreads();
-  }
-  grid_dependency_launch();
-  const int64_t total = before[a.batch];
-  int64_t chunk, at, until;
-  int32_t unit = 0;
-  if (a.split) {
-    chunk = (total + a.blocks - 1) / a.blocks;
-    at = chunk * blockIdx.x < total ? chunk * blockIdx.x : total;
-    until = at + chunk < total ? at + chunk : total;
-    if (blockIdx.x == 0) {
-      if (tid == 0) a.plan[0] = chunk;
-      for (int32_t b = tid; b <= a.batch; b += kThreads) a.plan[1 + b] = before[b];
-    }
-  } else {
-    unit = blockIdx.x;
-    chunk = 1, at = 0, until = 1;
+    grid_dependency_launch();
+    chunk = (carry + a.blocks - 1) / a.blocks;
+    at = chunk * blockIdx.x < carry ? chunk * blockIdx.x : carry;
+    until = at + chunk < carry ? at + chunk : carry;
   }
 
-  // shared memory: queries, the f32 weights of a tile, then the rings
+  // shared memory: queries, the weights of a tile that is added up row by row, then the rings
   const int query_row = a.key_row;
   T* query = reinterpret_cast<T*>(memory);
   constexpr int kWeightRow = kWide ? kKeys : kKeys + 1;
-  float* weights = reinterpret_cast<float*>(memory + ((ROWS * query_row * sizeof(T) + 15) & ~size_t(15))) + warp * (ROWS * kWeightRow);
-  char* rings = memory + ((ROWS * query_row * sizeof(T) + 15) & ~size_t(15)) + ((kWarps * ROWS * kWeightRow * 4 + 15) & ~15);
-  const Layout ring{rings + warp * a.stages * a.stage_bytes, kKeys * a.key_row * int(sizeof(T)), kKeys * a.value_row * int(sizeof(T)), a.stage_bytes};
+  float* weights = reinterpret_cast<float*>(memory + ((ROWS * query_row * SIZE + 15) & ~15)) + warp * (ROWS * kWeightRow);
+  char* rings = memory + ((ROWS * query_row * SIZE + 15) & ~15) + ((kWarps * ROWS * kWeightRow * 4 + 15) & ~15);
+  const int key_bytes = kKeys * a.key_row * SIZE;
+  char* const ring = rings + warp * a.stages * a.stage_bytes;
   float* joined = reinterpret_cast<float*>(rings);  // [kWarps][ROWS][DIM + 4], once the rings are drained
 
   while (at < until) {
@@ -294,14 +302,14 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
     int64_t unit_begin = 0;
     if (a.split) {
       int32_t low = 0, high = a.batch - 1;
-      while (low < high) {  // the last sequence that begins at or before `at`, and is not empty
+      while (low < high) {  // the sequence that tile `at` is of: the first that ends after it
         const int32_t mid = (low + high) >> 1;
         if (before[mid + 1] > at) high = mid;
         else low = mid + 1;
       }
       b = low;
     } else {
-      b = unit / (a.kv_heads * a.row_blocks);
+      b = blockIdx.x / (a.kv_heads * a.row_blocks);
     }
     const Span span = span_of(a, b);
     unit_tiles = tiles_of(span);
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
       const int64_t left = until - at;
       tiles = unit_tiles - tile < left ? unit_tiles - tile : static_cast<int32_t>(left);
     } else {
-      inner = unit - b * (a.kv_heads * a.row_blocks);
+      inner = blockIdx.x - b * (a.kv_heads * a.row_blocks);
       tiles = unit_tiles;
     }
     const int32_t kv = inner / a.row_blocks, row0 = (inner - kv * a.row_blocks) * ROWS;
@@ -327,106 +335,146 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
     const int64_t far = int64_t(span.first) + t_last - a.window;
     const int32_t all_low = a.window < 0 || far < span.low ? span.low : far < span.end ? static_cast<int32_t>(far) : span.end;
 
-    // ---- queries
-    for (int i = tid; i < ROWS * query_row; i += kThreads) {
-      const int r = i / query_row, c = i - r * query_row;
-      float v = 0.0f;
-      if (r < rows && c < a.rank) {
-        const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
-        if (t < span.n)
-          v = to_f32(reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2])[c]);
+    // ---- loads
+    const char* keys = a.keys + kv * a.key_stride[1];
+    const char* values = a.values + kv * a.value_stride[1];
+    const char* states = a.states == nullptr ? nullptr : a.states + kv * a.state_stride[1];
+    const int32_t* table = a.table + b * a.table_stride;
+    const int32_t key0 = span.low + tile * kTile + warp * kKeys;
+    // the page and offset of this lane's place, turn after turn
+    const uint32_t first_place = static_cast<uint32_t>(key0) + (lane & 15);
+    uint32_t column = first_place / a.page_size, offset = first_place - column * a.page_size;
+    const uint32_t column_step = kTile / a.page_size, offset_step = kTile - column_step * a.page_size;
+    struct Place {
+      int32_t page;  // -1: none
+      uint32_t offset;
+    };
+    auto next_place = [&](int32_t i) {
+      Place p{-1, offset};
+      // (64 bits: the turn after the last may lie past 2^31)
+      if (i < tiles && int64_t(key0) + int64_t(i) * kTile + (lane & 15) < span.end) {
+        const int32_t page = table[column];
+        if (static_cast<uint32_t>(page) < static_cast<uint64_t>(a.pages)) p.page = page;
       }
-      query[i] = from_f32<T>(v);
+      column += column_step;
+      offset += offset_step;
+      if (offset >= a.page_size) offset -= a.page_size, ++column;
+      return p;
+    };
+    auto issue = [&](int32_t i, Place p) {
+      Turn made{0, 0.0f};
+      if (i < tiles && !late) {
+        const int place = lane & 15;
+        const bool mine = p.page >= 0;
+        made.there = __ballot_sync(0xffffffffu, mine) & 0xffffu;
+        if (BULK) {
+          if (made.there != 0) {
+            char* stage = ring + (issued & 1) * a.stage_bytes;
+            uint64_t* bar = &landed[warp][issued & 1];
+            ++issued;
+            const int key_row = a.rank * SIZE, value_row = a.dim * SIZE;
+            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(made.there) * (key_row + value_row));
+            char* to = lane < 16 ? stage + place * a.key_row * SIZE : stage + key_bytes + place * a.value_row * SIZE;
+            if (mine) {
+              const char* from = lane < 16 ? keys + p.page * a.key_stride[0] + p.offset * a.key_stride[2]
+                                           : values + p.page * a.value_stride[0] + p.offset * a.value_stride[2];
+              bulk_load(to, from, lane < 16 ? key_row : value_row, bar);
+            } else if (lane >= 16) {  // a weight of 0 is no help against a value of NaN
+              for (int c = 0; c < value_row; c += 16) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+            }
+          }
+        } else {
+          char* stage = ring + (a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
+          const int64_t page = mine ? p.page : 0, off = mine ? p.offset : 0;
+          load_rows<T>(stage, a.key_row * SIZE, keys, page * a.key_stride[0] + off * a.key_stride[2], made.there, a.rank * SIZE, a.key_chunk, lane);
+          load_rows<T>(stage + key_bytes, a.value_row * SIZE, values, page * a.value_stride[0] + off * a.value_stride[2], made.there, a.dim * SIZE,
+                       a.value_chunk, lane);
+        }
+        if (states != nullptr && mine)
+          made.state = to_f32(*reinterpret_cast<const T*>(states + p.page * a.state_stride[0] + p.offset * a.state_stride[2]));
+      }
+      if (!BULK) copy_commit();
+      return made;
+    };
+    const int lead = BULK ? 1 : a.stages - 1;  // turns on their way while one is worked on
+    Place todo = next_place(0);
+    Turn turn{0, 0.0f};
+    if (lead) {
+      const Place after = next_place(1);
+      turn = issue(0, todo);
+      todo = after;
     }
-    // pads of the rings' rows: 0, and not written again before the rings are used to join
-    for (int i = lane; i < a.stages * kKeys; i += 32) {
-      const Stage s = ring.at(i / kKeys);
-      T* k = reinterpret_cast<T*>(s.keys) + (i % kKeys) * a.key_row;
-      T* v = reinterpret_cast<T*>(s.values) + (i % kKeys) * a.value_row;
-      for (int c = a.rank; c < a.key_row; ++c) k[c] = from_f32<T>(0.0f);
-      for (int c = a.dim; c < a.value_row; ++c) v[c] = from_f32<T>(0.0f);
+
+    // ---- queries, and the keys' columns that no copy fills: 0
+    for (int r = warp; r < ROWS; r += kWarps) {
+      const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
+      const bool counts = r < rows && t < span.n;
+      const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
+      for (int c = lane; c < a.key_cols; c += 32) query[r * query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
     }
-    __syncthreads();
+    if (a.key_cols > a.rank) {
+      for (int i = lane; i < a.stages * kKeys; i += 32) {
+        T* k = reinterpret_cast<T*>(ring + i / kKeys * a.stage_bytes) + i % kKeys * a.key_row;
+        for (int c = a.rank; c < a.key_cols; ++c) k[c] = from_f32<T>(0.0f);
+      }
+    }
 
     // ---- this thread's rows: the places they see, [row_low, row_end)
+    const int own_row = kWide && ROWS > 1 && lane >= 16 ? OWN : 0;
     int32_t row_low[OWN], row_end[OWN];
     float ref[OWN], sum[OWN], state[OWN];
     bool any[OWN];
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      const int r = kWide ? i : (i >> 1) * 8 + 2 * (lane & 3) + (i & 1);
+      const int r = kWide ? own_row + i : (i >> 1) * 8 + 2 * (lane & 3) + (i & 1);
       const int t = (row0 + r) / a.group;
       const bool counts = r < rows && t < span.n;
       const int32_t place = span.first + t;
       row_end[i] = !counts ? 0 : place + 1 < span.end ? place + 1 : span.end;
       row_low[i] = a.window < 0 || place < a.window ? 0 : place - a.window;
-      ref[i] = a.compress == JK_SOFTSIGN ? 0.0f : -INFINITY;
+      ref[i] = COMPRESS == JK_SOFTSIGN ? 0.0f : -INFINITY;
       sum[i] = state[i] = 0.0f;
       any[i] = false;
     }
-    float out[kWide ? ROWS : MT][kWide ? CT : NT * 4];
+    float out[MT][NT * 4];
+    uint64_t pairs[kWide ? ROWS : 1][CP];  // f32's sums
 #pragma unroll
-    for (int i = 0; i < (kWide ? ROWS : MT); ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < (kWide ? CT : NT * 4); ++j) out[i][j] = 0.0f;
+      for (int j = 0; j < NT * 4; ++j) out[i][j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < (kWide ? ROWS : 1); ++i)
+#pragma unroll
+      for (int j = 0; j < CP; ++j) pairs[i][j] = 0;
+    __syncthreads();
 
-    const char* keys = a.keys + kv * a.key_stride[1];
-    const char* values = a.values + kv * a.value_stride[1];
-    const char* states = a.states == nullptr ? nullptr : a.states + kv * a.state_stride[1];
-    const int32_t key0 = span.low + tile * kTile + warp * kKeys;
-
-    // the page of this lane's place (lanes 16.. as lanes 0..) of turn i, -1: none
-    auto page_of = [&](int32_t i) -> int32_t {
-      const int64_t j = int64_t(key0) + int64_t(i) * kTile + (lane & 15);
-      if (i >= tiles || j >= span.end) return -1;
-      const int32_t page = a.table[b * a.table_stride + static_cast<uint32_t>(j) / a.page_size];
-      return static_cast<uint32_t>(page) < static_cast<uint64_t>(a.pages) ? page : -1;
-    };
-    float state_next = 0.0f;  // of the turn that was issued last
-    auto issue = [&](int32_t i, int32_t page) {
-      if (i < tiles) {
-        const Stage s = ring.at(i % a.stages);
-        const uint32_t j = static_cast<uint32_t>(key0 + i * kTile + (lane & 15));
-        const uint32_t off = page < 0 ? 0 : j % a.page_size;
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-        const int64_t p = page < 0 ? 0 : page;
-        load_rows<T>(s.keys, a.key_row * int(sizeof(T)), keys, p * a.key_stride[0] + off * a.key_stride[2], there, a.rank * int(sizeof(T)), a.key_chunk, lane);
-        load_rows<T>(s.values, a.value_row * int(sizeof(T)), values, p * a.value_stride[0] + off * a.value_stride[2], there, a.dim * int(sizeof(T)),
-                     a.value_chunk, lane);
-        if (lane == 0) *s.seen = there;
-        if (states != nullptr && lane < kKeys)
-          state_next = page < 0 ? 0.0f : to_f32(*reinterpret_cast<const T*>(states + p * a.state_stride[0] + off * a.state_stride[2]));
-      }
-      copy_commit();
-    };
-    auto put_state = [&](int32_t i) {  // of turn i, read when it was issued
-      if (states != nullptr && i >= 0 && i < tiles && lane < kKeys) ring.at(i % a.stages).states[lane] = state_next;
-    };
-
-    int32_t page = page_of(0);
-    for (int i = 0; i < a.stages - 1; ++i) {
-      const int32_t next = page_of(i + 1);
-      issue(i, page);
-      put_state(i);
-      page = next;
-    }
     for (int32_t i = 0; i < tiles; ++i) {
       __syncwarp();  // the stage to fill has been read by all lanes
-      const int32_t ahead = i + a.stages - 1;
-      if (a.stages > 1 && i > 0) put_state(ahead - 1);
-      const int32_t next = page_of(ahead + 1);
-      issue(ahead, page);
-      if (a.stages == 1) put_state(ahead);
-      page = next;
-      copy_wait(a.stages - 1);
-      __syncwarp();
-      const Stage s = ring.at(i % a.stages);
-      const uint32_t there = *s.seen;
-      const int32_t k0 = key0 + i * kTile;
+      const Place after = next_place(i + lead + 1);
+      const Turn made = issue(i + lead, todo);
+      const Turn now = lead ? turn : made;
+      turn = made;
+      todo = after;
+      const uint32_t there = now.there;
+      if (!BULK) copy_wait(lead);
       if (there == 0) continue;
+      const char* stage = ring + (BULK ? taken & 1 : a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
+      if (BULK) {
+        if (!late && !mbar_wait(&landed[warp][taken & 1], (taken >> 1) & 1)) {
+          late = true;
+          g_device_error = JK_ERR_DEVICE_TIMEOUT;
+        }
+        late = __any_sync(0xffffffffu, late);
+        ++taken;
+      }
+      __syncwarp();
+      const T* const stage_keys = reinterpret_cast<const T*>(stage);
+      const T* const stage_values = reinterpret_cast<const T*>(stage + key_bytes);
+      const int32_t k0 = key0 + i * kTile;
       // rows see different parts of it
-      const int32_t tile_end = k0 + kKeys < span.end ? k0 + kKeys : span.end;
-      const bool mixed = tile_end > all_end || k0 < all_low;
+      const bool mixed = (k0 + kKeys < span.end ? k0 + kKeys : span.end) > all_end || k0 < all_low;
+      const bool full = there == 0xffffu && !mixed;
 
       if constexpr (!kWide) {
         float c[NT][4], c2[NT][4];
@@ -434,112 +482,120 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[n][e] = c2[n][e] = 0.0f;
-        // K: matrices (places 0-7 | 8-15) x (columns 0-7 | 8-15)
-        const uint32_t k_at = shared_at(reinterpret_cast<T*>(s.keys) + (lane & 15) * a.key_row + (lane >> 4) * 8);
-        const uint32_t q_at = shared_at(query + (lane & 7) * query_row + ((lane >> 3) & 1) * 8);
-        const int steps = (a.rank + 15) / 16;
-        for (int k = 0; k < steps; k += 2) {
-          uint32_t ka[4], kb[4];
-          ldmatrix4(ka, k_at + k * 32);
-          const bool more = k + 1 < steps;
-          if (more) ldmatrix4(kb, k_at + (k + 1) * 32);
+        {
+          // K: matrices (places 0-7 | 8-15) x (columns 0-7 | 8-15); Q: rows 0-7 x four times 8 columns; two steps at a time
+          uint32_t k_at = shared_at(stage_keys + (lane & 15) * a.key_row + (lane >> 4) * 8);
+          uint32_t q_at = shared_at(query + (lane & 7) * query_row + (lane >> 3) * 8);
+#pragma unroll 2
+          for (int k = 0; k < a.key_cols; k += 32) {
+            uint32_t ka[4], kb[4];
+            ldmatrix4(ka, k_at);
+            ldmatrix4(kb, k_at + 32);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t b0, b1;
-            ldmatrix2(b0, b1, q_at + n * 8 * query_row * 2 + k * 32);
-            mma<T>(c[n], ka, b0, b1);
-            if (more) {
-              ldmatrix2(b0, b1, q_at + n * 8 * query_row * 2 + (k + 1) * 32);
-              mma<T>(c2[n], kb, b0, b1);
+            for (int n = 0; n < NT; ++n) {
+              uint32_t q[4];
+              ldmatrix4(q, q_at + n * 16 * query_row);
+              mma<T>(c[n], ka, q[0], q[1]);
+              mma<T>(c2[n], kb, q[2], q[3]);
             }
+            k_at += 64;
+            q_at += 64;
           }
         }
         // c[n][e]: place (lane / 4) + 8 (e / 2), row 8 n + 2 (lane % 4) + e % 2
         const int place = lane >> 2;
-        const float st0 = states == nullptr ? 0.0f : s.states[place], st1 = states == nullptr ? 0.0f : s.states[place + 8];
-        uint32_t high[NT][2], low[NT][2];
-        bool moved = false;
-        float factor[OWN];
+        float st[2] = {0.0f, 0.0f};
+        if (states != nullptr) {
+          st[0] = __shfl_sync(0xffffffffu, now.state, place);
+          st[1] = __shfl_sync(0xffffffffu, now.state, place + 8);
+        }
+        // weights in c; FULL: every row sees every place
+        auto weigh = [&](auto whole) {
+          constexpr bool FULL = decltype(whole)::value;
+          bool sees[NT][4];
+          bool higher = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[4];
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i2 = 2 * n + e;
-            const float d0 = c[n][e] + c2[n][e], d1 = c[n][e + 2] + c2[n][e + 2];
-            const int32_t j0 = k0 + place, j1 = j0 + 8;
-            const bool v0 = ((there >> place) & 1) && j0 < row_end[i2] && j0 >= row_low[i2];
-            const bool v1 = ((there >> (place + 8)) & 1) && j1 < row_end[i2] && j1 >= row_low[i2];
-            any[i2] |= v0 || v1;
-            factor[i2] = 1.0f;
-            float r = 0.0f;
-            if (a.compress != JK_SOFTSIGN) {
-              float top = v0 ? level(a.compress, d0, a.scale, a.bias) : -INFINITY;
-              if (v1) top = fmaxf(top, level(a.compress, d1, a.scale, a.bias));
+            for (int e = 0; e < 4; ++e) {
+              const int i2 = 2 * n + (e & 1), p = place + 8 * (e >> 1);
+              c[n][e] = score_of<COMPRESS>(c[n][e] + c2[n][e], a.scale, a.bias);
+              sees[n][e] = FULL || (((there >> p) & 1) && k0 + p < row_end[i2] && k0 + p >= row_low[i2]);
+              any[i2] |= sees[n][e];
+              if (COMPRESS != JK_SOFTSIGN) higher |= sees[n][e] && level_of<COMPRESS>(c[n][e], a.scale) > ref[i2] + kSlack;
+            }
+          if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
+#pragma unroll
+            for (int i2 = 0; i2 < OWN; ++i2) {
+              const int n = i2 >> 1, e = i2 & 1;
+              float top = sees[n][e] ? level_of<COMPRESS>(c[n][e], a.scale) : -INFINITY;
+              if (sees[n][e + 2]) top = fmaxf(top, level_of<COMPRESS>(c[n][e + 2], a.scale));
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               top = fmaxf(top, ref[i2]);
-              r = top == -INFINITY ? 0.0f : top;
-              if (top != ref[i2]) {
-                factor[i2] = exp2f(ref[i2] - r);
-                ref[i2] = top;
-                moved = true;
-              }
-            }
-            const float w0 = v0 ? weight(a.compress, d0, a.scale, a.bias, r) : 0.0f;
-            const float w1 = v1 ? weight(a.compress, d1, a.scale, a.bias, r) : 0.0f;
-            sum[i2] = fmaf(sum[i2], factor[i2], w0 + w1);
-            w[e] = v0 ? signed_weight(a.compress, d0, a.scale, a.bias, w0) : 0.0f;
-            w[e + 2] = v1 ? signed_weight(a.compress, d1, a.scale, a.bias, w1) : 0.0f;
-            if (states != nullptr) {
-              float x = state[i2] * factor[i2];
-              if (v0) x = fmaf(w[e], st0, x);
-              if (v1) x = fmaf(w[e + 2], st1, x);
-              state[i2] = x;
+              const float factor = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
+              ref[i2] = top;
+              sum[i2] *= factor;
+              state[i2] *= factor;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) out[m][4 * n + e] *= factor, out[m][4 * n + e + 2] *= factor;
             }
           }
-          if (mixed) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) weights[(8 * n + 2 * (lane & 3) + (e & 1)) * kWeightRow + place + 8 * (e >> 1)] = w[e];
-          } else {
-            using P = Two<T>;
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i2 = 2 * n + (e & 1);
+              float w = mass_of<COMPRESS>(c[n][e], a.scale, COMPRESS == JK_SOFTSIGN || ref[i2] == -INFINITY ? 0.0f : ref[i2]);
+              if (!FULL && !sees[n][e]) w = 0.0f;
+              if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
+              w = weight_of<COMPRESS>(c[n][e], w);
+              if (!FULL && !sees[n][e]) w = 0.0f;
+              if (states != nullptr && sees[n][e]) state[i2] = fmaf(w, st[e >> 1], state[i2]);
+              c[n][e] = w;
+            }
+        };
+        if (full) weigh(std::true_type());
+        else weigh(std::false_type());
+        if (!mixed) {
+          uint32_t high[NT][2], low[NT][2];
+          using P = Two<T>;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const typename P::type hi = P::of(w[2 * h], w[2 * h + 1]);
+              const typename P::type hi = P::of(c[n][2 * h], c[n][2 * h + 1]);
               const float2 f = P::back(hi);
-              const typename P::type lo = P::of(w[2 * h] - f.x, w[2 * h + 1] - f.y);
+              const typename P::type lo = P::of(c[n][2 * h] - f.x, c[n][2 * h + 1] - f.y);
               high[n][h] = transpose8(*reinterpret_cast<const uint32_t*>(&hi));
               low[n][h] = transpose8(*reinterpret_cast<const uint32_t*>(&lo));
             }
-          }
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) out[m][4 * n + e] *= factor[2 * n + (e & 1)];
-        }
-        if (!mixed) {
           // V^T: matrices (columns 0-7 | 8-15) x (places 0-7 | 8-15), read transposed
-          const uint32_t v_at = shared_at(reinterpret_cast<T*>(s.values) + ((lane & 7) + ((lane >> 4) & 1) * 8) * a.value_row + ((lane >> 3) & 1) * 8);
+          const uint32_t v_at = shared_at(stage_values + ((lane & 7) + ((lane >> 4) & 1) * 8) * a.value_row + ((lane >> 3) & 1) * 8);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            if (m * 16 < a.dim) {
-              uint32_t va[4];
-              ldmatrix4_trans(va, v_at + m * 32);
+          for (int m4 = 0; m4 < MT; m4 += 4) {
+            if (m4 * 16 < a.dim) {  // (columns past the value's are read and added up for nothing)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                float(&o)[4] = *reinterpret_cast<float(*)[4]>(&out[m][4 * n]);
-                mma<T>(o, va, high[n][0], high[n][1]);
-                mma<T>(o, va, low[n][0], low[n][1]);
+              for (int m = m4; m < m4 + 4; ++m) {
+                uint32_t va[4];
+                ldmatrix4_trans(va, v_at + m * 32);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  float(&o)[4] = *reinterpret_cast<float(*)[4]>(&out[m][4 * n]);
+                  mma<T>(o, va, high[n][0], high[n][1]);
+                  mma<T>(o, va, low[n][0], low[n][1]);
+                }
               }
             }
           }
         } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) weights[(8 * n + 2 * (lane & 3) + (e & 1)) * kWeightRow + place + 8 * (e >> 1)] = c[n][e];
           __syncwarp();
-          const T* v = reinterpret_cast<const T*>(s.values);
+          const T* v = stage_values + place;
+#pragma unroll 1
           for (int k = 0; k < kKeys; ++k) {
             if (!((there >> k) & 1)) continue;
 #pragma unroll
@@ -551,100 +607,128 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                   if (m * 16 < a.dim) {
-                    out[m][4 * n + e] = fmaf(w, to_f32(v[k * a.value_row + m * 16 + place]), out[m][4 * n + e]);
-                    out[m][4 * n + e + 2] = fmaf(w, to_f32(v[k * a.value_row + m * 16 + place + 8]), out[m][4 * n + e + 2]);
+                    out[m][4 * n + e] = fmaf(w, to_f32(v[k * a.value_row + m * 16]), out[m][4 * n + e]);
+                    out[m][4 * n + e + 2] = fmaf(w, to_f32(v[k * a.value_row + m * 16 + 8]), out[m][4 * n + e + 2]);
                   }
                 }
               }
           }
         }
       } else {
-        // f32: a lane has half a place's columns, lanes 16.. the second half
+        // f32: a lane has half of a place's columns, lanes 16.. the other half
         const int place = lane & 15;
-        const int half = a.key_row / 2 / 4 * 4;  // key_row is a multiple of 4; the two halves need not be equal
-        const int begin = lane < 16 ? 0 : half, end = lane < 16 ? half : a.key_row - 4;
-        const float* k = reinterpret_cast<const float*>(s.keys) + place * a.key_row;
-        const float* q = reinterpret_cast<const float*>(query);
-        float dot[ROWS];
+        const int half = a.key_cols / 2;
+        const float* k = stage_keys + place * a.key_row + (lane < 16 ? 0 : half);
+        const float* q = reinterpret_cast<const float*>(query) + (lane < 16 ? 0 : half);
+        uint64_t dots[ROWS];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) dot[r] = 0.0f;
-        for (int x = begin; x < end; x += 4) {
-          const float4 kv4 = *reinterpret_cast<const float4*>(k + x);
+        for (int r = 0; r < ROWS; ++r) dots[r] = 0;
+#pragma unroll 2
+        for (int x = 0; x < half; x += 4) {
+          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(k + x);
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
-            if (r < rows) {
-              const float4 q4 = *reinterpret_cast<const float4*>(q + r * query_row + x);
-              dot[r] = fmaf(kv4.x, q4.x, fmaf(kv4.y, q4.y, fmaf(kv4.z, q4.z, fmaf(kv4.w, q4.w, dot[r]))));
-            }
+            const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(q + r * query_row + x);
+            dots[r] = fma2(k4.y, q4.y, fma2(k4.x, q4.x, dots[r]));
           }
         }
-        const int32_t j = k0 + place;
-        const float st = states == nullptr ? 0.0f : s.states[place];
+        float score[OWN];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-          if (r < rows) {
-            const float d = dot[r] + __shfl_xor_sync(0xffffffffu, dot[r], 16);
-            const bool v = ((there >> place) & 1) && j < row_end[r] && j >= row_low[r];
-            any[r] |= v;
-            float factor = 1.0f, base = 0.0f;
-            if (a.compress != JK_SOFTSIGN) {
-              float top = v ? level(a.compress, d, a.scale, a.bias) : -INFINITY;
-#pragma unroll
-              for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              top = fmaxf(top, ref[r]);
-              base = top == -INFINITY ? 0.0f : top;
-              if (top != ref[r]) {
-                factor = exp2f(ref[r] - base);
-                ref[r] = top;
-#pragma unroll
-                for (int x = 0; x < CT; ++x) out[r][x] *= factor;
-              }
-            }
-            float w = v ? weight(a.compress, d, a.scale, a.bias, base) : 0.0f;
-            sum[r] = fmaf(sum[r], factor, lane < 16 ? w : 0.0f);
-            w = v ? signed_weight(a.compress, d, a.scale, a.bias, w) : 0.0f;
-            if (states != nullptr) {
-              state[r] *= factor;
-              if (v && lane < 16) state[r] = fmaf(w, st, state[r]);
-            }
-            if (lane < 16) weights[r * kWeightRow + place] = w;
+        for (int i2 = 0; i2 < OWN; ++i2) {
+          float2 v = unpair(dots[i2]);
+          const float first = v.x + v.y;
+          if (ROWS == 1) {
+            score[i2] = first + __shfl_xor_sync(0xffffffffu, first, 16);
+          } else {  // each half of the warp gives the other half the sums of its rows
+            v = unpair(dots[i2 + ROWS - OWN]);
+            const float second = v.x + v.y;
+            score[i2] = (lane < 16 ? first : second) + __shfl_xor_sync(0xffffffffu, lane < 16 ? second : first, 16);
           }
+          score[i2] = score_of<COMPRESS>(score[i2], a.scale, a.bias);
+        }
+        bool sees[OWN];
+        bool higher = false;
+#pragma unroll
+        for (int i2 = 0; i2 < OWN; ++i2) {
+          sees[i2] = full || (((there >> place) & 1) && k0 + place < row_end[i2] && k0 + place >= row_low[i2]);
+          any[i2] |= sees[i2];
+          if (COMPRESS != JK_SOFTSIGN) higher |= sees[i2] && level_of<COMPRESS>(score[i2], a.scale) > ref[i2] + kSlack;
+        }
+        if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
+          float factor[OWN];
+#pragma unroll
+          for (int i2 = 0; i2 < OWN; ++i2) {
+            float top = sees[i2] ? level_of<COMPRESS>(score[i2], a.scale) : -INFINITY;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, ref[i2]);
+            factor[i2] = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
+            ref[i2] = top;
+            sum[i2] *= factor[i2];
+            state[i2] *= factor[i2];
+          }
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const float f = __shfl_sync(0xffffffffu, factor[r % OWN], r < OWN ? 0 : 16);
+#pragma unroll
+            for (int y = 0; y < CP; ++y) pairs[r][y] = mul2(pairs[r][y], pair(f, f));
+          }
+        }
+#pragma unroll
+        for (int i2 = 0; i2 < OWN; ++i2) {
+          float w = mass_of<COMPRESS>(score[i2], a.scale, COMPRESS == JK_SOFTSIGN || ref[i2] == -INFINITY ? 0.0f : ref[i2]);
+          w = sees[i2] ? w : 0.0f;
+          if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
+          w = sees[i2] ? weight_of<COMPRESS>(score[i2], w) : 0.0f;
+          if (states != nullptr && sees[i2]) state[i2] = fmaf(w, now.state, state[i2]);
+          weights[(own_row + i2) * kWeightRow + place] = w;
         }
         __syncwarp();
-        const float* v = reinterpret_cast<const float*>(s.values);
+        const float* v = stage_values + 2 * lane;
+        constexpr int AT_ONCE = DIM == 512 ? 2 : 4;  // places whose values are in registers together
 #pragma unroll 1
-        for (int k4 = 0; k4 < kKeys; k4 += 4) {
-          float x[4][CT];
+        for (int k4 = 0; k4 < kKeys; k4 += AT_ONCE) {
+          uint64_t x[AT_ONCE][CP];
 #pragma unroll
-          for (int k1 = 0; k1 < 4; ++k1)
+          for (int k1 = 0; k1 < AT_ONCE; ++k1)
 #pragma unroll
-            for (int y = 0; y < CT; ++y) x[k1][y] = lane + 32 * y < a.dim ? v[(k4 + k1) * a.value_row + lane + 32 * y] : 0.0f;
+            for (int y = 0; y < CP; ++y) x[k1][y] = *reinterpret_cast<const uint64_t*>(v + (k4 + k1) * a.value_row + 64 * y);
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
-            if (r < rows) {
+            float w[AT_ONCE];
+            if constexpr (AT_ONCE == 4) {
               const float4 w4 = *reinterpret_cast<const float4*>(weights + r * kWeightRow + k4);
-              const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+              w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
+            } else {
+              const float2 w2 = *reinterpret_cast<const float2*>(weights + r * kWeightRow + k4);
+              w[0] = w2.x, w[1] = w2.y;
+            }
+            int from = 0, to = kKeys;
+            if (mixed) {
+              from = __shfl_sync(0xffffffffu, row_low[r % OWN], r < OWN ? 0 : 16) - k0;
+              to = __shfl_sync(0xffffffffu, row_end[r % OWN], r < OWN ? 0 : 16) - k0;
+            }
 #pragma unroll
-              for (int k1 = 0; k1 < 4; ++k1) {
-                const int32_t jj = k0 + k4 + k1;
-                if (!mixed || (jj >= row_low[r] && jj < row_end[r])) {
+            for (int k1 = 0; k1 < AT_ONCE; ++k1) {
+              if (k4 + k1 >= from && k4 + k1 < to) {
 #pragma unroll
-                  for (int y = 0; y < CT; ++y) out[r][y] = fmaf(w[k1], x[k1][y], out[r][y]);
-                }
+                for (int y = 0; y < CP; ++y) pairs[r][y] = fma2(x[k1][y], pair(w[k1], w[k1]), pairs[r][y]);
               }
             }
           }
         }
       }
     }
-    copy_wait(0);
+    if (!BULK) copy_wait(0);
+    // what gave up waiting still lets its copies land
+    for (uint32_t q = issued < 2 ? 0 : issued - 2; BULK && late && q != issued; ++q) mbar_wait(&landed[warp][q & 1], (q >> 1) & 1);
 
     // ---- the warps' sums, then the block's
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       bool seen = any[i];
 #pragma unroll
-      for (int o = kWide ? 1 : 4; o < 32; o <<= 1) {
+      for (int o = kWide ? 1 : 4; o < (kWide ? 16 : 32); o <<= 1) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
         state[i] += __shfl_xor_sync(0xffffffffu, state[i], o);
         seen |= __shfl_xor_sync(0xffffffffu, int(seen), o) != 0;
@@ -672,14 +756,13 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
             }
         }
     } else {
-      if (lane == 0) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) ref_s[warp][r] = ref[r], sum_s[warp][r] = sum[r], state_s[warp][r] = state[r];
-      }
+      for (int i = 0; i < OWN; ++i)
+        if ((lane & 15) == 0) ref_s[warp][own_row + i] = ref[i], sum_s[warp][own_row + i] = sum[i], state_s[warp][own_row + i] = state[i];
 #pragma unroll
       for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-        for (int y = 0; y < CT; ++y) joined[(warp * ROWS + r) * kJoinRow + lane + 32 * y] = out[r][y];
+        for (int y = 0; y < CP; ++y) *reinterpret_cast<uint64_t*>(joined + (warp * ROWS + r) * kJoinRow + 2 * lane + 64 * y) = pairs[r][y];
     }
     __syncthreads();
     const bool whole = tiles == unit_tiles;
@@ -696,11 +779,11 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const bool none = top != -INFINITY && ref_s[w][r] == -INFINITY;  // a warp that saw nothing, or only -inf
-        f[w] = top == -INFINITY ? 1.0f : exp2f(ref_s[w][r] - top);
+        f[w] = top == -INFINITY ? 1.0f : power2(ref_s[w][r] - top);
         if (!none) all = fmaf(sum_s[w][r], f[w], all), st = fmaf(state_s[w][r], f[w], st);
       }
       float norm = 1.0f;
-      if (whole && a.compress != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
+      if (whole && COMPRESS != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
       const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
       const int64_t row = (int64_t(b) * a.new_nodes + t) * a.heads + kv * a.group + g;
       const bool zero = whole && (t >= span.n || (top == -INFINITY && norm == 0.0f));
@@ -720,98 +803,111 @@ __global__ void __launch_bounds__(kThreads) cached_kernel(const __grid_constant_
         }
       }
     }
+    if (BULK) fence_proxy_async_smem();
     __syncthreads();  // before the next unit's queries, and before the rings are filled again
     if (a.split) at += tiles;
     else at = until;
   }
 }
 
-// Joins the parts of a unit's row that several blocks left; a unit without tiles has zeros.
+// Joins the parts of a unit's row that several blocks left, 128 columns a block; a unit without tiles has zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
-  __shared__ float factor[2 * kSms];
-  __shared__ float scratch[8][4];
+  __shared__ int64_t counted[8][2];
+  __shared__ float words_s[8][3];
   __shared__ __align__(16) float columns[8][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int32_t unit_rows = a.group * a.new_nodes;
-  const int64_t unit = blockIdx.x / unit_rows;  // sequence and head of the cache
+  const int32_t unit_rows = a.group * a.new_nodes, slices = (a.dim + 127) / 128;
+  const int64_t at = blockIdx.x / slices;
+  const int32_t d0 = (blockIdx.x - static_cast<uint32_t>(at * slices)) * 128;
+  const int64_t unit = at / unit_rows;  // sequence and head of the cache
   const int32_t b = static_cast<int32_t>(unit / a.kv_heads), kv = static_cast<int32_t>(unit - int64_t(b) * a.kv_heads);
-  const int32_t row_of = blockIdx.x - static_cast<uint32_t>(unit * unit_rows);
+  const int32_t row_of = static_cast<int32_t>(at - unit * unit_rows);
   const int32_t t = row_of / a.group, g = row_of - t * a.group;
   const int64_t row = (int64_t(b) * a.new_nodes + t) * a.heads + kv * a.group + g;
+  // the blocks' runs, as the first kernel has them (while it runs)
   const Span span = span_of(a, b);
   const int32_t tiles = tiles_of(span);
-  T* out = reinterpret_cast<T*>(a.out_value) + row * a.dim;
-  grid_dependency_wait();
-  if (tiles == 0) {
-    for (int d = tid; d < a.dim; d += 256) out[d] = from_f32<T>(0.0f);
-    if (tid == 0 && a.out_state != nullptr) reinterpret_cast<T*>(a.out_state)[row] = from_f32<T>(0.0f);
-    return;
-  }
-  const int64_t chunk = a.plan[0];
-  const int32_t row_block = row_of / a.rows, r = row_of - row_block * a.rows;
-  const int64_t begin = a.plan[1 + b] + (int64_t(kv) * a.row_blocks + row_block) * tiles;
-  const int32_t first = static_cast<int32_t>(begin / chunk), last = static_cast<int32_t>((begin + tiles - 1) / chunk);
-  if (first == last) return;  // one block had all of it
-  const int32_t n = last - first + 1;
-  // part i: of block first + i; only the first block's can be one that began there
-  auto part_at = [&](int32_t i) {
-    const int64_t block = first + i;
-    return a.parts + ((block * 2 + (begin < chunk * block ? 0 : 1)) * a.rows + r) * a.part_row;
-  };
-  const int32_t words = a.part_row - 4;
-  float top = -INFINITY;
-  for (int32_t i = tid; i < n; i += 256) top = fmaxf(top, part_at(i)[words]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) scratch[warp][0] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, scratch[w][0]);
-  float all = 0.0f, st = 0.0f;
-  for (int32_t i = tid; i < n; i += 256) {
-    const float* p = part_at(i) + words;
-    const float ref = p[0];
-    const float f = top == -INFINITY ? 1.0f : exp2f(ref - top);
-    factor[i] = f;
-    if (top == -INFINITY || ref != -INFINITY) all = fmaf(p[1], f, all), st = fmaf(p[2], f, st);
+  int64_t mine = 0, all_tiles = 0;
+  for (int32_t i = tid; i < a.batch; i += 256) {
+    const int64_t n = int64_t(tiles_of(span_of(a, i))) * a.kv_heads * a.row_blocks;
+    all_tiles += n;
+    if (i < b) mine += n;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    st += __shfl_xor_sync(0xffffffffu, st, o);
+    mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    all_tiles += __shfl_xor_sync(0xffffffffu, all_tiles, o);
   }
-  if (lane == 0) scratch[warp][1] = all, scratch[warp][2] = st;
+  if (lane == 0) counted[warp][0] = mine, counted[warp][1] = all_tiles;
   __syncthreads();
+  mine = all_tiles = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mine += counted[w][0], all_tiles += counted[w][1];
+  T* out = reinterpret_cast<T*>(a.out_value) + row * a.dim + d0;
+  const bool first_slice = tid == 0 && d0 == 0 && a.out_state != nullptr;
+  if (tiles == 0) {
+    if (tid < 128 && d0 + tid < a.dim) out[tid] = from_f32<T>(0.0f);
+    if (first_slice) reinterpret_cast<T*>(a.out_state)[row] = from_f32<T>(0.0f);
+    grid_dependency_wait();
+    return;
+  }
+  const int64_t chunk = (all_tiles + a.blocks - 1) / a.blocks;
+  const int32_t row_block = row_of / a.rows, r = row_of - row_block * a.rows;
+  const int64_t begin = mine + (int64_t(kv) * a.row_blocks + row_block) * tiles;
+  const int32_t first = static_cast<int32_t>(begin / chunk), last = static_cast<int32_t>((begin + tiles - 1) / chunk);
+  grid_dependency_wait();
+  if (first == last) return;  // one block had all of it
+  // a warp has every eighth part, a lane four columns
+  const int32_t words = a.part_row - 4;
+  const bool has = d0 + 4 * lane < words;
+  float top = -INFINITY, all = 0.0f, st = 0.0f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int32_t block = first + warp; block <= last; block += 4 * 8) {
+    float4 v[4], w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (block + 8 * i <= last) {
+        // only in the first block it can be a part that began there
+        const float* p = a.parts + (((int64_t(block) + 8 * i) * 2 + (begin < chunk * (block + 8 * i) ? 0 : 1)) * a.rows + r) * a.part_row;
+        w[i] = *reinterpret_cast<const float4*>(p + words);
+        if (has) v[i] = *reinterpret_cast<const float4*>(p + d0 + 4 * lane);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float higher = fmaxf(top, w[i].x);
+      const bool none = higher == -INFINITY;
+      const float f = none ? 1.0f : power2(top - higher), h = none ? 1.0f : power2(w[i].x - higher);
+      // a part of scores of -inf alone has a NaN for its sum, which counts only where there is nothing else
+      const float s0 = !none && top == -INFINITY ? 0.0f : all * f, s1 = !none && w[i].x == -INFINITY ? 0.0f : w[i].y * h;
+      all = s0 + s1;
+      st = fmaf(w[i].z, h, st * f);
+      x.x = fmaf(v[i].x, h, x.x * f), x.y = fmaf(v[i].y, h, x.y * f), x.z = fmaf(v[i].z, h, x.z * f), x.w = fmaf(v[i].w, h, x.w * f);
+      top = higher;
+    }
+  }
+  if (lane == 0) words_s[warp][0] = top, words_s[warp][1] = all, words_s[warp][2] = st;
+  *reinterpret_cast<float4*>(&columns[warp][4 * lane]) = x;
+  __syncthreads();
+  top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, words_s[w][0]);
+  float y = 0.0f;
   all = st = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) all += scratch[w][1], st += scratch[w][2];
+  for (int w = 0; w < 8; ++w) {
+    const float ref = words_s[w][0], f = top == -INFINITY ? 1.0f : power2(ref - top);
+    if (top == -INFINITY || ref != -INFINITY) all = fmaf(words_s[w][1], f, all), st = fmaf(words_s[w][2], f, st);
+    if (tid < 128) y = fmaf(columns[w][tid], f, y);
+  }
   float norm = 1.0f;
   if (a.compress != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
   const bool zero = t >= span.n || (top == -INFINITY && norm == 0.0f);
-  if (tid == 0 && a.out_state != nullptr) reinterpret_cast<T*>(a.out_state)[row] = from_f32<T>(zero ? 0.0f : st * norm);
-  // a warp has every eighth part, a lane four columns
-  for (int32_t d0 = 0; d0 < a.dim; d0 += 128) {
-    const int32_t d = d0 + 4 * lane;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < words) {
-#pragma unroll 4
-      for (int32_t i = warp; i < n; i += 8) {
-        const float4 v = *reinterpret_cast<const float4*>(part_at(i) + d);
-        const float f = factor[i];
-        x.x = fmaf(f, v.x, x.x), x.y = fmaf(f, v.y, x.y), x.z = fmaf(f, v.z, x.z), x.w = fmaf(f, v.w, x.w);
-      }
-    }
-    *reinterpret_cast<float4*>(&columns[warp][4 * lane]) = x;
-    __syncthreads();
-    if (tid < 128 && d0 + tid < a.dim) {
-      float y = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) y += columns[w][tid];
-      out[d0 + tid] = from_f32<T>(zero ? 0.0f : y * norm);
-    }
-    __syncthreads();
-  }
+  if (tid < 128 && d0 + tid < a.dim) out[tid] = from_f32<T>(zero ? 0.0f : y * norm);
+  if (first_slice) reinterpret_cast<T*>(a.out_state)[row] = from_f32<T>(zero ? 0.0f : st * norm);
 }
 
 // ---- host
@@ -819,69 +915,99 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 struct Shape {
   int rows, dim;     // template arguments
   int row_blocks;
+  int key_cols, key_row, value_row;
   size_t shared;
   int stages, stage_bytes, per_sm;
 };
 
 // Rows of a block and its shared memory, from sizes alone (the workspace's size depends on them).
-inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype) {
+inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, bool blocks16) {
   Shape s;
   const bool wide = dtype == JK_F32;
   const int size = wide ? 4 : 2;
-  s.dim = dim <= 128 ? 128 : dim <= 256 ? 256 : 512;
-  // 128 registers of sums a thread at most
-  if (wide) s.rows = unit_rows == 1 ? 1 : 8;
-  else s.rows = unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
+  s.dim = dim <= 64 && !wide ? 64 : dim <= 128 ? 128 : dim <= 256 ? 256 : 512;
+  // 128 registers of sums a thread at most (f32: 64, as it keeps a tile's values too); rows that are copied in smaller
+  // pieces take what time that takes, so they have one size of a block
+  if (wide) s.rows = !blocks16 ? 4 : unit_rows == 1 ? 1 : unit_rows <= 4 || s.dim == 512 ? 4 : 8;
+  else s.rows = !blocks16 || unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
   s.row_blocks = static_cast<int>((unit_rows + s.rows - 1) / s.rows);
-  const int64_t key_row = wide ? (rank + 7) / 8 * 8 + 4 : (rank + 15) / 16 * 16 + 8;
-  const int64_t value_row = wide ? (dim + 3) / 4 * 4 : (dim + 15) / 16 * 16 + 8;
-  s.stage_bytes = static_cast<int>(kKeys * (key_row + value_row) * size + 4 * kKeys + 16);
-  const size_t fixed = ((s.rows * key_row * size + 15) & ~15) + ((kWarps * s.rows * (wide ? kKeys : kKeys + 1) * 4 + 15) & ~15);
+  // columns in the products' steps (two of 16, or two halves of 4), and rows an odd number of 16-byte blocks apart, so that
+  // eight of them lie in different banks
+  s.key_cols = static_cast<int>(wide ? (rank + 7) / 8 * 8 : (rank + 31) / 32 * 32);
+  s.key_row = s.key_cols + 16 / size;
+  s.value_row = static_cast<int>(wide ? (dim + 3) / 4 * 4 : (dim + 15) / 16 * 16 + 8);
+  s.stage_bytes = kKeys * (s.key_row + s.value_row) * size;
+  const size_t fixed = ((s.rows * s.key_row * size + 15) & ~15) + ((kWarps * s.rows * (wide ? kKeys : kKeys + 1) * 4 + 15) & ~15);
   const size_t join = size_t(kWarps) * s.rows * (s.dim + 4) * 4;
   auto bytes = [&](int stages) {
     const size_t rings = size_t(kWarps) * stages * s.stage_bytes;
-    return fixed + (rings > join ? rings : join);
+    // (the last row is read up to DIM columns)
+    return fixed + (rings + s.dim * size > join ? rings + s.dim * size : join);
   };
-  // two blocks of an SM with three stages each, else one with as many (up to three) as fit
-  const size_t half = 102 * 1024, whole = 212 * 1024;
-  s.stages = 3, s.per_sm = 2;
-  if (bytes(3) > half) {
-    if (bytes(2) <= half) s.stages = 2;
-    else {
-      s.per_sm = 1;
-      while (s.stages > 1 && bytes(s.stages) > whole) --s.stages;
-    }
-  }
+  // Two stages a warp, in as many blocks as an SM holds (three at most: registers); where not even one block has room for
+  // them, one stage. (32 sequences of 10240 f16 nodes, rank and dim 128: see the figures above.)
+  const size_t sm = 227 * 1024, fixed_block = 10 * 1024 + 512;
+  s.stages = bytes(2) + fixed_block <= sm ? 2 : 1;
+  s.per_sm = static_cast<int>(sm / (bytes(s.stages) + fixed_block));
+  const int most = s.rows * s.dim <= 1024 ? kMaxPerSm : 2;
+  if (s.per_sm > most) s.per_sm = most;
   s.shared = bytes(s.stages);
   return s;
 }
 
-template <typename T, int ROWS, int DIM>
-int launch_one(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(cached_kernel<T, ROWS, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(s.shared)) != cudaSuccess) {
+template <typename T, int ROWS, int DIM, int COMPRESS, bool BULK>
+int launch_kernel(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
+  if (cudaFuncSetAttribute(cached_kernel<T, ROWS, DIM, COMPRESS, BULK>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(s.shared)) != cudaSuccess) {
     cudaGetLastError();
     return JK_ERR_LAUNCH;
   }
-  cached_kernel<T, ROWS, DIM><<<static_cast<unsigned>(a.split ? a.blocks : units), kThreads, s.shared, stream>>>(a);
+  cached_kernel<T, ROWS, DIM, COMPRESS, BULK><<<static_cast<unsigned>(a.split ? a.blocks : units), kThreads, s.shared, stream>>>(a);
   if (int st = launch_status()) return st;
   if (!a.split) return JK_OK;
-  launch_dependent(join_kernel<T>, static_cast<unsigned>(int64_t(a.batch) * a.kv_heads * a.group * a.new_nodes), 256, 0, stream, a);
+  launch_dependent(join_kernel<T>, static_cast<unsigned>(int64_t(a.batch) * a.heads * a.new_nodes * ((a.dim + 127) / 128)), 256, 0, stream, a);
   return launch_status();
 }
 
-// One launch, for at most kMaxBatch sequences; defined for each type in a unit of its own.
+template <typename T, int ROWS, int DIM, bool BULK = true>
+int launch_one(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
+  if (a.compress == JK_SOFTMAX) return launch_kernel<T, ROWS, DIM, JK_SOFTMAX, BULK>(a, s, units, stream);
+  if (a.compress == JK_SOFTSIGN) return launch_kernel<T, ROWS, DIM, JK_SOFTSIGN, BULK>(a, s, units, stream);
+  return launch_kernel<T, ROWS, DIM, JK_SIGNED_ABS_SOFTMAX, BULK>(a, s, units, stream);
+}
+
+// One launch, for at most kMaxBatch sequences; instantiated for each type in a unit of its own.
 template <typename T>
 int launch(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
   if constexpr (std::is_same_v<T, float>) {
+    if (!a.blocks16) {
+      if (s.dim == 128) return launch_one<T, 4, 128, false>(a, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 4, 256, false>(a, s, units, stream);
+      return launch_one<T, 4, 512, false>(a, s, units, stream);
+    }
     if (s.rows == 1) {
       if (s.dim == 128) return launch_one<T, 1, 128>(a, s, units, stream);
       if (s.dim == 256) return launch_one<T, 1, 256>(a, s, units, stream);
       return launch_one<T, 1, 512>(a, s, units, stream);
     }
+    if (s.rows == 4) {
+      if (s.dim == 128) return launch_one<T, 4, 128>(a, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 4, 256>(a, s, units, stream);
+      return launch_one<T, 4, 512>(a, s, units, stream);
+    }
     if (s.dim == 128) return launch_one<T, 8, 128>(a, s, units, stream);
-    if (s.dim == 256) return launch_one<T, 8, 256>(a, s, units, stream);
-    return launch_one<T, 8, 512>(a, s, units, stream);
+    return launch_one<T, 8, 256>(a, s, units, stream);
   } else {
+    if (!a.blocks16) {
+      if (s.dim == 64) return launch_one<T, 8, 64, false>(a, s, units, stream);
+      if (s.dim == 128) return launch_one<T, 8, 128, false>(a, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 8, 256, false>(a, s, units, stream);
+      return launch_one<T, 8, 512, false>(a, s, units, stream);
+    }
+    if (s.dim == 64) {
+      if (s.rows == 8) return launch_one<T, 8, 64>(a, s, units, stream);
+      if (s.rows == 16) return launch_one<T, 16, 64>(a, s, units, stream);
+      return launch_one<T, 32, 64>(a, s, units, stream);
+    }
     if (s.dim == 128) {
       if (s.rows == 8) return launch_one<T, 8, 128>(a, s, units, stream);
       if (s.rows == 16) return launch_one<T, 16, 128>(a, s, units, stream);

@@ -7,4 +7,7 @@ namespace cached {
 int launch_bf16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__nv_bfloat16>(a, s, units, stream); }
 
 }  // namespace cached
+
+JK_ERROR_READER(read_error_cached_bf16)
+
 }  // namespace jk

@@ -7,4 +7,7 @@ namespace cached {
 int launch_f16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__half>(a, s, units, stream); }
 
 }  // namespace cached
+
+JK_ERROR_READER(read_error_cached_f16)
+
 }  // namespace jk

@@ -7,4 +7,7 @@ namespace cached {
 int launch_f32(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<float>(a, s, units, stream); }
 
 }  // namespace cached
+
+JK_ERROR_READER(read_error_cached_f32)
+
 }  // namespace jk

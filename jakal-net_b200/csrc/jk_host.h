@@ -30,7 +30,7 @@ static __device__ int g_device_error = 0;
   }
 
 // Readers of the units that launch kernels with bounded waits (jk_project.cu, jk_topk.cu and
-// its per-value-type units jk_topk_vt_*.cu, jk_window.cu, jk_clip.cu, jk_loss.cu).
+// its per-value-type units jk_topk_vt_*.cu, jk_window.cu, jk_clip.cu, jk_loss.cu, jk_cached_*.cu).
 int read_error_project(int* value);
 int read_error_topk(int* value);
 int read_error_topk_bf16(int* value);
@@ -39,6 +39,9 @@ int read_error_topk_f32(int* value);
 int read_error_window(int* value);
 int read_error_clip(int* value);
 int read_error_loss(int* value);
+int read_error_cached_f32(int* value);
+int read_error_cached_bf16(int* value);
+int read_error_cached_f16(int* value);
 
 // Returns JK_OK when the current device is sm_100 (cached per device ordinal).
 int check_device();

@@ -265,20 +265,20 @@ int launch(const Args& g, int64_t batch, cudaStream_t s) {
 }  // namespace verify
 }  // namespace jk
 
-extern "C" int jk_verify_draft(const void* target, int64_t target_stride_b, int64_t target_stride_t, const void* draft,
-                               int64_t draft_stride_b, int64_t draft_stride_t, const int64_t* tokens, const float* uniform,
-                               const int32_t* counts, int64_t batch, int64_t drafted, int64_t vocab, int dtype, int64_t* out_tokens,
-                               int32_t* accepted, jk_stream_t stream) {
+extern "C" int jk_verify_draft(const jk_draft_t* q, jk_stream_t stream) {
   using namespace jk;
   using namespace jk::verify;
+  if (q == nullptr) return JK_ERR_BAD_ARG;
+  const int64_t batch = q->batch, drafted = q->drafted, vocab = q->vocab;
   if (batch < 0 || drafted < 0 || vocab < 1 || batch > (1 << 24) || drafted > (1 << 30) || vocab > (1 << 30)) return JK_ERR_BAD_SHAPE;
-  if (!float_dtype(dtype)) return JK_ERR_BAD_DTYPE;
-  if (batch > 0 && (target == nullptr || uniform == nullptr || out_tokens == nullptr || accepted == nullptr)) return JK_ERR_BAD_ARG;
-  if (batch > 0 && drafted > 0 && tokens == nullptr) return JK_ERR_BAD_ARG;
+  const int dtype = q->dtype == JK_F32 || q->dtype == JK_BF16 || q->dtype == JK_F16 ? static_cast<int>(q->dtype) : -1;
+  if (dtype < 0) return JK_ERR_BAD_DTYPE;
+  if (batch > 0 && (q->target == nullptr || q->uniform == nullptr || q->out_tokens == nullptr || q->accepted == nullptr)) return JK_ERR_BAD_ARG;
+  if (batch > 0 && drafted > 0 && q->tokens == nullptr) return JK_ERR_BAD_ARG;
   if (int st = check_device()) return st;
   if (batch == 0) return JK_OK;
-  const Args g{target,  draft,  target_stride_b, target_stride_t, draft_stride_b, draft_stride_t, tokens,
-               uniform, counts, static_cast<int32_t>(drafted), static_cast<int32_t>(vocab), out_tokens, accepted};
+  const Args g{q->target, q->draft, q->target_stride[0], q->target_stride[1], q->draft_stride[0], q->draft_stride[1], q->tokens, q->uniform,
+               q->counts, static_cast<int32_t>(drafted), static_cast<int32_t>(vocab), q->out_tokens, q->accepted};
   auto s = reinterpret_cast<cudaStream_t>(stream);
   JK_WITH_TYPE(dtype, T, return launch<T>(g, batch, s));
 }

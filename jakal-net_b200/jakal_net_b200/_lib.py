@@ -39,13 +39,6 @@ class JkHeads(ctypes.Structure):
                 ("head_bias", ctypes.c_void_p)]
 
 
-class JkPools(ctypes.Structure):
-    """jk_pools_t: host arrays that name a cache's pools."""
-
-    _fields_ = [("data", ctypes.c_void_p), ("page_bytes", ctypes.c_void_p), ("stride_bytes", ctypes.c_void_p),
-                ("count", ctypes.c_int64)]
-
-
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
@@ -165,43 +158,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _p, _p, _p, _i64, _i32, _i32,  # grads, outs, numels, dtypes, out_dtypes, count, norm_kind, clip
          _f32, _f32, _p, _p, _p],               # max_norm, eps, total, workspace, stream
     ),
-    "jk_cached_propagation_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
-    "jk_cached_propagation": (
-        _i32,
-        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64,    # query, strides, keys, strides
-         _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,    # values, strides, states, strides
-         _p, _i64, _p, _p,                              # table, table_stride, lengths, counts
-         _i64, _i64, _i64, _i64, _i64, _i64,            # batch, new_nodes, heads, kv_heads, rank, dim
-         _i64, _i64, _i64, _i32, _i64, _i32,            # pages, page_size, columns, dtype, window, compress
-         _f32, _f32, _p, _p, _p, _p],                   # scale, score_bias, out_value, out_state, workspace, stream
-    ),
+    "jk_cached_propagation_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    # jk_cache_t, jk_nodes_t, jk_pools_t, jk_rows_t and jk_draft_t have 8-byte fields only: arrays of them go in their place
+    "jk_cached_propagation": (_i32, [_p, _p, _f32, _f32, _p]),  # cache, nodes, scale, score_bias, stream
     "jk_cache_reserve_workspace": (_i64, [_i64, _i64]),
-    "jk_cache_reserve": (
-        _i32,
-        [_p, _p, _i64, _p, _p, _p,                      # pools, table, table_stride, lengths, refs, counts
-         _i64, _i64, _i64, _i64, _p, _p, _p],           # batch, columns, pages, page_size, added, workspace, stream
-    ),
-    "jk_cache_write": (
-        _i32,
-        [_p, _p, _p, _p, _p, _p, _i64,                  # pages, strides, rows, strides, widths, element_bytes, count
-         _p, _i64, _p, _p,                              # table, table_stride, lengths, counts
-         _i64, _i64, _i64, _i64, _i64, _i64, _p],       # batch, new_nodes, heads, pages, page_size, columns, stream
-    ),
+    "jk_cache_reserve": (_i32, [_p, _p, _p, _p, _p, _p]),       # pools, cache, counts, added, workspace, stream
+    "jk_cache_write": (_i32, [_p, _p, _p, _p]),                 # rows, cache, counts, stream
     "jk_cache_fork_workspace": (_i64, [_i64, _i64]),
-    "jk_cache_fork": (
-        _i32,
-        [_p, _i64, _p, _p, _p, _p,                      # table, table_stride, lengths, refs, parents, children
-         _i64, _i64, _i64, _i64, _p, _p, _p],           # forks, batch, columns, pages, done, workspace, stream
-    ),
-    "jk_cache_release": (_i32, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "jk_cache_fork": (_i32, [_p, _p, _p, _i64, _p, _p, _p]),    # cache, parents, children, forks, done, workspace, stream
+    "jk_cache_release": (_i32, [_p, _p, _p]),                   # cache, new_lengths, stream
     "jk_cache_compact_workspace": (_i64, [_i64]),
-    "jk_cache_compact": (_i32, [_p, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p]),
-    "jk_cache_copy": (_i32, [_p, _p, _p, _i64, _i64, _p]),
-    "jk_verify_draft": (
-        _i32,
-        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p,    # target, strides, draft, strides, tokens, uniform, counts
-         _i64, _i64, _i64, _i32, _p, _p, _p],           # batch, drafted, vocab, dtype, out_tokens, accepted, stream
-    ),
+    "jk_cache_compact": (_i32, [_p, _p, _p, _p, _p]),           # pools, cache, live, workspace, stream
+    "jk_cache_copy": (_i32, [_p, _p, _p, _i64, _i64, _p]),      # pools, src, dst, n, pages, stream
+    "jk_verify_draft": (_i32, [_p, _p]),                        # draft, stream
     "jk_debug_window_stalled_producer": (
         _i32,
         [_p, _p, _i64, _i64, _i64, _i64, _i32,  # row_proj, col_proj, B, n_rows, n_cols, rp, proj_dtype

@@ -25,7 +25,7 @@ The operators have no backward pass and refuse inputs that ask for one.
 from __future__ import annotations
 
 import array
-import ctypes
+import functools
 from typing import Optional, Sequence, Union
 
 import torch
@@ -52,11 +52,20 @@ _COMPRESS = {
     "signed_abs_softmax": _lib.JK_SIGNED_ABS_SOFTMAX,
 }
 _MAX_WRITE = 64  # pairs of one jk_cache_write
+_INT32 = torch.int32
+# bytes by sizes, which a loop asks for again and again
+_propagation_workspace = functools.lru_cache(maxsize=4096)(_LIBRARY.jk_cached_propagation_workspace)
+_reserve_workspace = functools.lru_cache(maxsize=4096)(_LIBRARY.jk_cache_reserve_workspace)
+_fork_workspace = functools.lru_cache(maxsize=4096)(_LIBRARY.jk_cache_fork_workspace)
+_compact_workspace = functools.lru_cache(maxsize=4096)(_LIBRARY.jk_cache_compact_workspace)
 
 
 # ----------------------------------------------------------------------------- checks
 def _ints(name: str, t: Tensor, shape: Optional[tuple], device: int) -> None:
     """t is an int32 tensor on the device, of the shape (None: of one dim), contiguous."""
+    if (isinstance(t, Tensor) and t.dtype is _INT32 and t.get_device() == device and (t.dim() == 1 if shape is None else t.shape == shape)
+            and t.is_contiguous()):
+        return
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a tensor")
     if not t.is_cuda:
@@ -77,15 +86,28 @@ def _table(table: Tensor) -> tuple[int, int, int, int]:
         raise TypeError("table must be a tensor")
     if not table.is_cuda:
         raise RuntimeError(f"table must be a CUDA tensor in the b200_sm100a backend (got {table.device}).")
-    if table.dtype != torch.int32:
+    if table.dtype is not _INT32:
         raise RuntimeError(f"table: unsupported dtype {table.dtype} (int32)")
     if table.dim() != 2:
         raise ValueError(f"table has shape {tuple(table.shape)}, expected [batch, columns]")
     batch, columns = table.shape
+    if table.is_contiguous():
+        return table.get_device(), batch, columns, columns
     row, step = table.stride()
     if (columns > 1 and step != 1) or (batch > 1 and row < columns):
         raise ValueError("table must have rows that are contiguous inside and apart")
     return table.get_device(), batch, columns, max(row, columns)
+
+
+def _cache(table: Tensor, stride: int, lengths: Optional[Tensor], refs: Optional[Tensor], batch: int, columns: int, pages: int,
+           page_size: int) -> array.array:
+    """jk_cache_t"""
+    return array.array("q", (table.data_ptr(), stride, 0 if lengths is None else lengths.data_ptr(), 0 if refs is None else refs.data_ptr(),
+                             batch, columns, pages, page_size))
+
+
+def _at(words: array.array) -> int:
+    return words.buffer_info()[0]
 
 
 def _no_grad(**tensors: Optional[Tensor]) -> None:
@@ -106,34 +128,40 @@ def _one_block(shape, strides) -> bool:
 
 
 class _Pools:
-    """A call's pools as jk_pools_t; `arrays` keeps what it points to alive."""
+    """A call's pools as jk_pools_t (`words`), which points into `arrays`."""
 
     def __init__(self, pools: Union[Tensor, Sequence[Tensor]], pages: int, device: int):
         tensors = [pools] if isinstance(pools, Tensor) else list(pools)
-        data, sizes, strides = array.array("Q"), array.array("q"), array.array("q")
+        data, sizes, strides = [], [], []
         for i, p in enumerate(tensors):
             if not isinstance(p, Tensor):
                 raise TypeError(f"pool {i} must be a tensor")
             if p.get_device() != device:
                 raise RuntimeError(f"pool {i} is on {p.device}, expected cuda:{device}")
-            shape, stride, size = p.shape, p.stride(), p.element_size()
+            shape, size = p.shape, p.element_size()
             if not shape or shape[0] != pages:
                 raise ValueError(f"pool {i} has shape {tuple(shape)}, expected {pages} pages in its first dim")
-            block = 1
-            for n in shape[1:]:
-                block *= n
-            if not (p.is_contiguous() or _one_block(shape[1:], stride[1:])) or (pages > 1 and stride[0] < block):
-                raise ValueError(f"pool {i}: a page must be one block of memory, apart from the other pages")
+            if p.is_contiguous():
+                block = step = p.numel() // pages if pages else 0
+            else:
+                stride, block = p.stride(), 1
+                for n in shape[1:]:
+                    block *= n
+                if not _one_block(shape[1:], stride[1:]) or (pages > 1 and stride[0] < block):
+                    raise ValueError(f"pool {i}: a page must be one block of memory, apart from the other pages")
+                step = max(stride[0], block)
             data.append(p.data_ptr())
             sizes.append(block * size)
-            strides.append(max(stride[0], block) * size)
+            strides.append(step * size)
         if len(set(data)) != len(data) and any(p.numel() for p in tensors):
             raise ValueError("a pool is given twice")
-        self.tensors, self.arrays = tensors, (data, sizes, strides)
-        self.struct = _lib.JkPools(data.buffer_info()[0], sizes.buffer_info()[0], strides.buffer_info()[0], len(tensors))
+        n = len(data)
+        self.tensors, self.arrays = tensors, array.array("q", data + sizes + strides)
+        at = _at(self.arrays)
+        self.words = array.array("q", (at, at + 8 * n, at + 16 * n, n))
 
-    def pointer(self):
-        return ctypes.addressof(self.struct)
+    def pointer(self) -> int:
+        return _at(self.words)
 
 
 def _page_size(page_size: int) -> int:
@@ -149,7 +177,7 @@ def _cache_pages(name: str, t: Tensor, query: Tensor, dims: int) -> None:
         raise TypeError(f"{name} must be a tensor")
     if t.get_device() != query.get_device():
         raise RuntimeError(f"{name} is on {t.device}, expected {query.device}")
-    if t.dtype != query.dtype:
+    if t.dtype is not query.dtype:
         raise RuntimeError(f"{name} has dtype {t.dtype}, expected {query.dtype}")
     if t.dim() != dims:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {dims} dims")
@@ -202,25 +230,33 @@ def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, ta
     _ints("lengths", lengths, (batch,), device)
     if counts is not None:
         _ints("counts", counts, (batch,), device)
-    if window is not None and window < 0:
+    if window is None:
+        window = -1
+    elif window < 0:
         raise ValueError(f"window is {window}")
-    state_at, state_strides, state = None, (0, 0, 0), None
+    else:
+        window = min(int(window), 0x7fffffff)
+    state_at, state_strides, state, out_state = 0, (0, 0, 0), None, 0
     if state_pages is not None:
         _cache_pages("state_pages", state_pages, query, 3)
         if state_pages.shape != (pages, kv_heads, page_size):
             raise ValueError(f"state_pages has shape {tuple(state_pages.shape)}, expected {(pages, kv_heads, page_size)}")
-        state = torch.empty((batch, new, heads), dtype=query.dtype, device=query.device)
-        state_at, state_strides = state_pages.data_ptr(), state_pages.stride()
-    if rank > 1 and query.stride(3) != 1:
+        state = query.new_empty((batch, new, heads))
+        state_at, state_strides, out_state = state_pages.data_ptr(), state_pages.stride(), state.data_ptr()
+    query_strides = query.stride()
+    if rank > 1 and query_strides[3] != 1:
         query = query.contiguous()
-    value = torch.empty((batch, new, heads, dim), dtype=query.dtype, device=query.device)
-    work = _empty((_LIBRARY.jk_cached_propagation_workspace(batch, new, heads, kv_heads, dim, page_size, columns, code) // 4,),
-                  torch.float32, query.device)
-    _call(_LIBRARY.jk_cached_propagation, "jk_cached_propagation", device, query.data_ptr(), *query.stride()[:3],
-          key_pages.data_ptr(), *key_pages.stride()[:3], value_pages.data_ptr(), *value_pages.stride()[:3], state_at, *state_strides,
-          table.data_ptr(), table_stride, lengths.data_ptr(), _ptr(counts), batch, new, heads, kv_heads, rank, dim, pages, page_size,
-          columns, code, -1 if window is None else min(int(window), 0x7fffffff), kind, float(scale), float(score_bias), value.data_ptr(),
-          _ptr(state), work.data_ptr())
+        query_strides = query.stride()
+    value = query.new_empty((batch, new, heads, dim))
+    size = _propagation_workspace(batch, new, heads, kv_heads, rank, dim, page_size, columns, window, code)
+    work = _empty((size // 4,), torch.float32, query.device) if size else None
+    key_strides, value_strides = key_pages.stride(), value_pages.stride()
+    cache = _cache(table, table_stride, lengths, None, batch, columns, pages, page_size)
+    nodes = array.array("q", (
+        query.data_ptr(), *query_strides[:3], key_pages.data_ptr(), *key_strides[:3], value_pages.data_ptr(), *value_strides[:3], state_at,
+        *state_strides, 0 if counts is None else counts.data_ptr(), new, heads, kv_heads, rank, dim, code, window, kind, value.data_ptr(),
+        out_state, 0 if work is None else work.data_ptr()))
+    _call(_LIBRARY.jk_cached_propagation, "jk_cached_propagation", device, _at(cache), _at(nodes), scale, score_bias)
     return value if state is None else (state, value)
 
 
@@ -244,9 +280,9 @@ def cache_reserve_(pools: Union[Tensor, Sequence[Tensor]], table: Tensor, length
     pages = refs.numel()
     named = _Pools(pools, pages, device)
     added = torch.empty_like(counts)
-    work = _empty((_LIBRARY.jk_cache_reserve_workspace(batch, pages) // 8,), torch.int64, table.device)
-    _call(_LIBRARY.jk_cache_reserve, "jk_cache_reserve", device, named.pointer(), table.data_ptr(), stride, lengths.data_ptr(),
-          refs.data_ptr(), counts.data_ptr(), batch, columns, pages, page_size, added.data_ptr(), work.data_ptr())
+    work = _empty((_reserve_workspace(batch, pages) // 4,), _INT32, table.device)
+    cache = _cache(table, stride, lengths, refs, batch, columns, pages, page_size)
+    _call(_LIBRARY.jk_cache_reserve, "jk_cache_reserve", device, named.pointer(), _at(cache), counts.data_ptr(), added.data_ptr(), work.data_ptr())
     _written([table, lengths, refs, *named.tensors])
     return added
 
@@ -268,47 +304,51 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
     if len(pages) != len(rows) or not pages:
         raise ValueError(f"{len(rows)} tensors of rows for {len(pages)} of pages")
     count = new = heads = page_size = None
-    at, from_ = array.array("Q"), array.array("Q")
-    page_strides, row_strides, widths, sizes = (array.array("q") for _ in range(4))
+    at, from_, page_strides, row_strides, widths, sizes = [], [], [], [], [], []
     kept = []  # copies of rows, until the launch
     for i, (p, r) in enumerate(zip(pages, rows)):
         if not isinstance(p, Tensor) or not isinstance(r, Tensor):
             raise TypeError(f"pages {i} and rows {i} must be tensors")
         if p.get_device() != device or r.get_device() != device:
             raise RuntimeError(f"pages {i} and rows {i} are on {p.device} and {r.device}, expected cuda:{device}")
-        if p.dtype != r.dtype:
+        if p.dtype is not r.dtype:
             raise RuntimeError(f"rows {i} has dtype {r.dtype}, expected {p.dtype}")
-        if p.dim() not in (3, 4) or r.dim() != p.dim():
-            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(p.shape)} and {tuple(r.shape)}")
+        shape, dims = p.shape, p.dim()
+        if dims not in (3, 4) or r.dim() != dims:
+            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(shape)} and {tuple(r.shape)}")
         if i == 0:
-            (count, heads, page_size), new = p.shape[:3], r.shape[1]
-        if p.shape[:3] != (count, heads, page_size) or r.shape != (batch, new, heads, *p.shape[3:]):
-            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(p.shape)} and {tuple(r.shape)}, which do not fit "
+            (count, heads, page_size), new = shape[:3], r.shape[1]
+        if shape[:3] != (count, heads, page_size) or r.shape != (batch, new, heads, *shape[3:]):
+            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(shape)} and {tuple(r.shape)}, which do not fit "
                              f"{batch} sequences, {new} nodes, {heads} heads and {count} pages of {page_size}")
         _no_grad(pages=p, rows=r)
-        width = p.shape[3] if p.dim() == 4 else 1
-        page_stride = p.stride()
-        if p.dim() == 4 and width > 1 and page_stride[3] != 1:
-            raise ValueError(f"pages {i} must be contiguous in their last dim")
-        if not (p.is_contiguous() or _one_block(p.shape[1:], page_stride[1:])) or (count > 1 and page_stride[0] < heads * page_size * width):
-            raise ValueError(f"pages {i}: a page must be one block of memory, apart from the other pages")
-        if r.dim() == 4 and width > 1 and r.stride(3) != 1:
+        width = shape[3] if dims == 4 else 1
+        page_stride, row_stride = p.stride(), r.stride()
+        if not p.is_contiguous():
+            if dims == 4 and width > 1 and page_stride[3] != 1:
+                raise ValueError(f"pages {i} must be contiguous in their last dim")
+            if not _one_block(shape[1:], page_stride[1:]) or (count > 1 and page_stride[0] < heads * page_size * width):
+                raise ValueError(f"pages {i}: a page must be one block of memory, apart from the other pages")
+        if dims == 4 and width > 1 and row_stride[3] != 1:
             r = r.contiguous()
             kept.append(r)
+            row_stride = r.stride()
         at.append(p.data_ptr())
         from_.append(r.data_ptr())
-        page_strides.extend(page_stride[:3])
-        row_strides.extend(r.stride()[:3])
+        page_strides += page_stride[:3]
+        row_strides += row_stride[:3]
         widths.append(width)
         sizes.append(p.element_size())
     if not page_size:
         raise ValueError("page_size is 0")
-    for i in range(0, len(pages), _MAX_WRITE):
-        n = min(_MAX_WRITE, len(pages) - i)
-        _call(_LIBRARY.jk_cache_write, "jk_cache_write", device, at.buffer_info()[0] + 8 * i, page_strides.buffer_info()[0] + 24 * i,
-              from_.buffer_info()[0] + 8 * i, row_strides.buffer_info()[0] + 24 * i, widths.buffer_info()[0] + 8 * i,
-              sizes.buffer_info()[0] + 8 * i, n, table.data_ptr(), stride, lengths.data_ptr(), _ptr(counts), batch, new, heads, count,
-              page_size, columns)
+    cache = _cache(table, stride, lengths, None, batch, columns, count, page_size)
+    n = len(pages)
+    words = array.array("q", at + from_ + widths + sizes + page_strides + row_strides)
+    base = _at(words)
+    for i in range(0, n, _MAX_WRITE):
+        call = array.array("q", (base + 8 * i, base + 8 * (4 * n + 3 * i), base + 8 * (n + i), base + 8 * (7 * n + 3 * i), base + 8 * (2 * n + i),
+                                 base + 8 * (3 * n + i), min(_MAX_WRITE, n - i), new, heads))
+        _call(_LIBRARY.jk_cache_write, "jk_cache_write", device, _at(call), _at(cache), _ptr(counts))
     _written(pages)
 
 
@@ -326,9 +366,10 @@ def cache_fork_(table: Tensor, lengths: Tensor, refs: Tensor, parents: Tensor, c
     _ints("children", children, parents.shape, device)
     forks = parents.numel()
     done = torch.empty_like(parents, dtype=torch.bool)
-    work = _empty((_LIBRARY.jk_cache_fork_workspace(batch, forks) // 4,), torch.int32, table.device)
-    _call(_LIBRARY.jk_cache_fork, "jk_cache_fork", device, table.data_ptr(), stride, lengths.data_ptr(), refs.data_ptr(), parents.data_ptr(),
-          children.data_ptr(), forks, batch, columns, refs.numel(), done.data_ptr(), work.data_ptr())
+    work = _empty((_fork_workspace(batch, forks) // 4,), _INT32, table.device)
+    cache = _cache(table, stride, lengths, refs, batch, columns, refs.numel(), 1)
+    _call(_LIBRARY.jk_cache_fork, "jk_cache_fork", device, _at(cache), parents.data_ptr(), children.data_ptr(), forks, done.data_ptr(),
+          work.data_ptr())
     _written([table, lengths, refs])
     return done
 
@@ -341,8 +382,8 @@ def cache_release_(table: Tensor, lengths: Tensor, refs: Tensor, new_lengths: Te
     _ints("lengths", lengths, (batch,), device)
     _ints("refs", refs, None, device)
     _ints("new_lengths", new_lengths, (batch,), device)
-    _call(_LIBRARY.jk_cache_release, "jk_cache_release", device, table.data_ptr(), stride, lengths.data_ptr(), refs.data_ptr(),
-          new_lengths.data_ptr(), batch, columns, refs.numel(), _page_size(page_size))
+    cache = _cache(table, stride, lengths, refs, batch, columns, refs.numel(), _page_size(page_size))
+    _call(_LIBRARY.jk_cache_release, "jk_cache_release", device, _at(cache), new_lengths.data_ptr())
     _written([table, lengths, refs])
 
 
@@ -357,10 +398,10 @@ def cache_compact_(pools: Union[Tensor, Sequence[Tensor]], table: Tensor, refs: 
     _ints("refs", refs, None, device)
     pages = refs.numel()
     named = _Pools(pools, pages, device)
-    live = _empty((), torch.int32, table.device)
-    work = _empty((_LIBRARY.jk_cache_compact_workspace(pages) // 4,), torch.int32, table.device)
-    _call(_LIBRARY.jk_cache_compact, "jk_cache_compact", device, named.pointer(), table.data_ptr(), stride, refs.data_ptr(), batch, columns,
-          pages, live.data_ptr(), work.data_ptr())
+    live = _empty((), _INT32, table.device)
+    work = _empty((_compact_workspace(pages) // 4,), _INT32, table.device)
+    cache = _cache(table, stride, None, refs, batch, columns, pages, 1)
+    _call(_LIBRARY.jk_cache_compact, "jk_cache_compact", device, named.pointer(), _at(cache), live.data_ptr(), work.data_ptr())
     _written([table, refs, *named.tensors])
     return live
 
@@ -386,6 +427,18 @@ def cache_copy_(pools: Union[Tensor, Sequence[Tensor]], src: Tensor, dst: Tensor
 
 
 # ----------------------------------------------------------------------------- drafted tokens
+def _given(name: str, t: Tensor, like: Tensor, shape: tuple, dtypes: tuple) -> None:
+    """t has the shape, one of the dtypes and like's device."""
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.get_device() != like.get_device():
+        raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name}: unsupported dtype {t.dtype} ({' or '.join(str(d) for d in dtypes)})")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+
+
 def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, uniform: Tensor, counts: Optional[Tensor] = None):
     """Holds drafted tokens against the target's probabilities, so that what is kept is distributed
     as the target's own tokens are.
@@ -419,26 +472,20 @@ def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, unifor
             raise ValueError(f"draft has shape {tuple(draft.shape)}, expected {(batch, drafted, vocab)}")
         if draft.stride(2) != 1 and vocab > 1:
             draft = draft.detach().contiguous()
-    for name, t, shape, dtypes in (("tokens", tokens, (batch, drafted), (torch.int64, torch.int32)),
-                                   ("uniform", uniform, (batch, drafted + 1), (torch.float32,))):
-        if not isinstance(t, Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if t.get_device() != device:
-            raise RuntimeError(f"{name} is on {t.device}, expected {target.device}")
-        if t.dtype not in dtypes:
-            raise RuntimeError(f"{name}: unsupported dtype {t.dtype} ({' or '.join(str(d) for d in dtypes)})")
-        if t.shape != shape:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    _given("tokens", tokens, target, (batch, drafted), (torch.int64, _INT32))
+    _given("uniform", uniform, target, (batch, drafted + 1), (torch.float32,))
     if counts is not None:
         _ints("counts", counts, (batch,), device)
     if target.stride(2) != 1 and vocab > 1:
         target = target.detach().contiguous()
-    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
         tokens = tokens.to(torch.int64).contiguous()
-    uniform = uniform.detach().contiguous()
-    out = torch.empty((batch, drafted + 1), dtype=torch.int64, device=target.device)
-    accepted = _empty((batch,), torch.int32, target.device)
-    draft_strides = (0, 0) if draft is None else draft.stride()[:2]
-    _call(_LIBRARY.jk_verify_draft, "jk_verify_draft", device, target.data_ptr(), *target.stride()[:2], _ptr(draft), *draft_strides,
-          tokens.data_ptr(), uniform.data_ptr(), _ptr(counts), batch, drafted, vocab, code, out.data_ptr(), accepted.data_ptr())
+    if not uniform.is_contiguous():
+        uniform = uniform.detach().contiguous()
+    out = tokens.new_empty((batch, drafted + 1))
+    accepted = _empty((batch,), _INT32, target.device)
+    words = array.array("q", (
+        target.data_ptr(), *target.stride()[:2], *((0, 0, 0) if draft is None else (draft.data_ptr(), *draft.stride()[:2])), tokens.data_ptr(),
+        uniform.data_ptr(), 0 if counts is None else counts.data_ptr(), batch, drafted, vocab, code, out.data_ptr(), accepted.data_ptr()))
+    _call(_LIBRARY.jk_verify_draft, "jk_verify_draft", device, _at(words))
     return out, accepted

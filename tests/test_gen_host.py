@@ -32,32 +32,46 @@ def test_generation_step_operators_refuse_cpu_tensors():
         jk.cache_reserve_([pool], None, n, refs, n, 4)
 
 
+def _words(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _cache(p, **changed):
+    c = dict(dict(table=p, stride=4, lengths=p, refs=p, batch=2, columns=4, pages=4, page=4), **changed)
+    return _words(*(0 if v is None else v for v in c.values()))
+
+
 def test_propagation_entry_point_checks_its_arguments_before_the_device():
     import jakal_net_b200 as jk
 
     buf, p = _pointer()
-    good = dict(q=p, k=p, v=p, st=None, table=p, stride=4, lengths=p, counts=None, batch=2, new=1, heads=4, kv=2, rank=8, dim=8, pages=4, page=4,
-                columns=4, dtype=1, window=-1, compress=3, out=p, out_state=None, work=p)
+    good = dict(q=p, k=p, v=p, st=None, counts=None, new=1, heads=4, kv=2, rank=8, dim=8, dtype=1, window=-1, compress=3, out=p, out_state=None,
+                work=p)
 
-    def status(**changed):
-        a = dict(good, **changed)
+    def status(cache=None, **changed):
+        a = {k: 0 if v is None else v for k, v in dict(good, **changed).items()}
         three = (1, 1, 1)
-        return jk._LIBRARY.jk_cached_propagation(
-            a["q"], *three, a["k"], *three, a["v"], *three, a["st"], *three, a["table"], a["stride"], a["lengths"], a["counts"], a["batch"],
-            a["new"], a["heads"], a["kv"], a["rank"], a["dim"], a["pages"], a["page"], a["columns"], a["dtype"], a["window"], a["compress"], 1.0,
-            0.0, a["out"], a["out_state"], a["work"], None)
+        nodes = _words(a["q"], *three, a["k"], *three, a["v"], *three, a["st"], *three, a["counts"], a["new"], a["heads"], a["kv"], a["rank"],
+                       a["dim"], a["dtype"], a["window"], a["compress"], a["out"], a["out_state"], a["work"])
+        return jk._LIBRARY.jk_cached_propagation(_cache(p, **(cache or {})), nodes, 1.0, 0.0, None)
 
-    for name, value in (("batch", -1), ("new", -1), ("new", 65), ("heads", 0), ("heads", 5), ("kv", 0), ("rank", 0), ("rank", 257), ("dim", 0),
-                        ("dim", 513), ("pages", -1), ("page", 0), ("columns", -1), ("stride", -1)):
+    for name, value in (("new", -1), ("new", 65), ("heads", 0), ("heads", 5), ("kv", 0), ("rank", 0), ("rank", 257), ("dim", 0), ("dim", 513)):
         assert status(**{name: value}) == -1, (name, value)
-    assert status(dtype=3) == -2
+    for name, value in (("batch", -1), ("pages", -1), ("page", 0), ("columns", -1), ("stride", -1), ("pages", 1 << 31), ("columns", 1 << 40)):
+        assert status(cache={name: value}) == -1, (name, value)
+    assert status(dtype=3) == -2 and status(dtype=1 << 40) == -2
     assert status(compress=2) == -3 and status(compress=9) == -3
-    for name in ("q", "k", "v", "table", "lengths", "out", "work"):
+    for name in ("q", "k", "v", "out"):
         assert status(**{name: None}) == -7, name
+    for name in ("table", "lengths"):
+        assert status(cache={name: None}) == -7, name
+    # a workspace is needed where a sequence can be split
+    assert status(cache=dict(columns=1000, stride=1000), work=None) == -7
     assert status(st=p) == -7 and status(out_state=p) == -7
     assert status(work=p + 4) == -8
+    assert jk._LIBRARY.jk_cached_propagation(None, None, 1.0, 0.0, None) == -7
     if not torch.cuda.is_available():
-        assert status() == -4
+        assert status() == -4 and status(work=None) == -4 and status(cache=dict(columns=1000, stride=1000)) == -4
 
 
 def test_page_entry_points_check_their_arguments_before_the_device():
@@ -65,47 +79,45 @@ def test_page_entry_points_check_their_arguments_before_the_device():
 
     lib = jk._LIBRARY
     buf, p = _pointer()
-    pools = (ctypes.c_int64 * 4)(ctypes.addressof(ctypes.c_uint64(0)), p, p, 0)
-    none = ctypes.addressof(pools)
-    data, size, stride = (ctypes.c_uint64 * 1)(p), (ctypes.c_int64 * 1)(64), (ctypes.c_int64 * 1)(32)
-
-    def made(data_, size_, stride_, n=1):
-        s = (ctypes.c_uint64 * 4)(ctypes.addressof(data_) if data_ is not None else 0, ctypes.addressof(size_), ctypes.addressof(stride_), n)
-        kept.append(s)
-        return ctypes.addressof(s)
-
     kept = []
-    reserve = lambda q, *a: lib.jk_cache_reserve(q, *a, None)  # noqa: E731
-    ok = (p, 4, p, p, p, 2, 4, 4, 4, p, p)
-    assert reserve(None, *ok) == -7
-    assert reserve(made(data, size, stride), *ok) == -1  # pages that overlap
-    assert reserve(made(None, size, size), *ok) == -7
-    assert reserve(made((ctypes.c_uint64 * 1)(0), size, size), *ok) == -7
-    assert reserve(made(data, size, size, 513), *ok) == -1
-    assert reserve(none, p, 3, p, p, p, 2, 4, 4, 4, p, p) == -1  # rows that overlap
-    assert reserve(none, p, 4, p, p, p, -1, 4, 4, 4, p, p) == -1
-    assert reserve(none, p, 4, p, p, p, 2, 4, 4, 0, p, p) == -1
-    assert reserve(none, p, 4, None, p, p, 2, 4, 4, 4, p, p) == -7
-    assert reserve(none, p, 4, p, None, p, 2, 4, 4, 4, p, p) == -7
-    assert reserve(none, p, 4, p, p, p, 2, 4, 4, 4, p, p + 8) == -8
-    three = (ctypes.c_int64 * 3)(1, 1, 1)
-    at, width, bytes_ = ctypes.addressof(three), (ctypes.c_int64 * 1)(8), (ctypes.c_int64 * 1)(2)
 
-    def write(count=1, pages=data, rows=data, w=width, b=bytes_, batch=2, new=1, heads=1, n_pages=4, page=4):
-        return lib.jk_cache_write(ctypes.addressof(pages), at, ctypes.addressof(rows), at, ctypes.addressof(w), ctypes.addressof(b), count, p, 4, p,
-                                  p, batch, new, heads, n_pages, page, 4, None)
+    def pools(data=p, size=64, stride=64, n=1, null=False):
+        arrays = _words(data), _words(size), _words(stride)
+        s = _words(0 if null else ctypes.addressof(arrays[0]), ctypes.addressof(arrays[1]), ctypes.addressof(arrays[2]), n)
+        kept.append(arrays)
+        return s
 
-    assert write(count=65) == -1 and write(count=-1) == -1 and write(new=-1) == -1 and write(page=0) == -1
-    assert write(heads=1 << 30, new=4) == -1
-    assert write(b=(ctypes.c_int64 * 1)(3)) == -2
-    assert write(rows=(ctypes.c_uint64 * 1)(0)) == -7 and write(pages=(ctypes.c_uint64 * 1)(0)) == -7
-    assert lib.jk_cache_fork(p, 4, p, p, p, p, -1, 2, 4, 4, p, p, None) == -1
-    assert lib.jk_cache_fork(p, 4, p, p, None, p, 1, 2, 4, 4, p, p, None) == -7
-    assert lib.jk_cache_fork(p, 4, p, p, p, p, 1, 2, 4, 4, p, p + 4, None) == -8
-    assert lib.jk_cache_release(p, 4, p, p, None, 2, 4, 4, 4, None) == -7
-    assert lib.jk_cache_release(p, 2, p, p, p, 2, 4, 4, 4, None) == -1
-    assert lib.jk_cache_compact(none, p, 4, p, 2, 4, 4, None, p, None) == -7
-    assert lib.jk_cache_compact(none, p, 4, p, 2, 4, 4, p, p + 4, None) == -8
+    def reserve(q, counts=p, added=p, work=p, **changed):
+        return lib.jk_cache_reserve(q, _cache(p, **changed), counts, added, work, None)
+
+    none = _words(0, 0, 0, 0)
+    assert reserve(None) == -7 and lib.jk_cache_reserve(none, None, p, p, p, None) == -7
+    assert reserve(pools(stride=32)) == -1  # pages that overlap
+    assert reserve(pools(null=True)) == -7 and reserve(pools(data=0)) == -7
+    assert reserve(pools(n=513)) == -1 and reserve(pools(n=-1)) == -1
+    assert reserve(none, stride=3) == -1  # rows that overlap
+    assert reserve(none, batch=-1) == -1 and reserve(none, page=0) == -1
+    for name in ("lengths", "refs", "table"):
+        assert reserve(none, **{name: None}) == -7, name
+    assert reserve(none, counts=None) == -7 and reserve(none, added=None) == -7 and reserve(none, work=None) == -7
+    assert reserve(none, work=p + 8) == -8
+    three = _words(1, 1, 1)
+
+    def write(count=1, pages=p, rows=p, width=8, size=2, new=1, heads=1, **changed):
+        arrays = _words(pages), _words(rows), _words(width), _words(size)
+        at = [ctypes.addressof(x) for x in arrays]
+        q = _words(at[0], ctypes.addressof(three), at[1], ctypes.addressof(three), at[2], at[3], count, new, heads)
+        return lib.jk_cache_write(q, _cache(p, **changed), p, None)
+
+    assert write(count=65) == -1 and write(count=-1) == -1 and write(new=-1) == -1 and write(page=0) == -1 and write(width=-1) == -1
+    assert write(heads=1 << 30, new=4) == -1 and write(heads=1 << 40) == -1
+    assert write(size=3) == -2
+    assert write(rows=0) == -7 and write(pages=0) == -7 and write(lengths=None) == -7 and lib.jk_cache_write(None, _cache(p), p, None) == -7
+    fork = lambda n, parents=p, children=p, done=p, work=p, **c: lib.jk_cache_fork(_cache(p, **c), parents, children, n, done, work, None)  # noqa: E731
+    assert fork(-1) == -1 and fork(1, parents=None) == -7 and fork(1, done=None) == -7 and fork(1, work=p + 4) == -8 and fork(1, refs=None) == -7
+    assert lib.jk_cache_release(_cache(p), None, None) == -7 and lib.jk_cache_release(_cache(p, stride=2), p, None) == -1
+    assert lib.jk_cache_compact(none, _cache(p), None, p, None) == -7
+    assert lib.jk_cache_compact(none, _cache(p), p, p + 4, None) == -8
     assert lib.jk_cache_copy(none, None, p, 1, 4, None) == -7 and lib.jk_cache_copy(none, p, p, -1, 4, None) == -1
 
 
@@ -113,15 +125,19 @@ def test_verification_checks_its_arguments_before_the_device():
     import jakal_net_b200 as jk
 
     buf, p = _pointer()
-    f = jk._LIBRARY.jk_verify_draft
-    assert f(p, 8, 8, p, 8, 8, p, p, None, -1, 1, 8, 0, p, p, None) == -1
-    assert f(p, 8, 8, p, 8, 8, p, p, None, 1, -1, 8, 0, p, p, None) == -1
-    assert f(p, 8, 8, p, 8, 8, p, p, None, 1, 1, 0, 0, p, p, None) == -1
-    assert f(p, 8, 8, p, 8, 8, p, p, None, 1, 1, 8, 3, p, p, None) == -2
+
+    def status(i=None, value=0):
+        a = [p, 8, 8, p, 8, 8, p, p, 0, 1, 1, 8, 0, p, p]
+        if i is not None:
+            a[i] = value
+        return jk._LIBRARY.jk_verify_draft(_words(*a), None)
+
+    for i, value in ((9, -1), (10, -1), (11, 0), (11, (1 << 30) + 1), (9, 1 << 30)):
+        assert status(i, value) == -1, i
+    assert status(12, 3) == -2 and status(12, 1 << 32) == -2
     for i in (0, 6, 7, 13, 14):
-        args = [p, 8, 8, p, 8, 8, p, p, None, 1, 1, 8, 0, p, p, None]
-        args[i] = None
-        assert f(*args) == -7, i
+        assert status(i) == -7, i
+    assert jk._LIBRARY.jk_verify_draft(None, None) == -7
 
 
 def test_workspaces():
@@ -130,11 +146,13 @@ def test_workspaces():
     lib = jk._LIBRARY
     assert lib.jk_cache_reserve_workspace(-1, 5) == 0 and lib.jk_cache_reserve_workspace(3, 5) >= 3 * 24 + 5 * 4
     assert lib.jk_cache_compact_workspace(7) >= 16 + 7 * 12 and lib.jk_cache_fork_workspace(3, 5) >= 32
+    size = lib.jk_cached_propagation_workspace
     for dtype in (0, 1, 2):
-        assert lib.jk_cached_propagation_workspace(0, 1, 1, 1, 8, 4, 4, dtype) % 16 == 0
-        # two rows' sums at least of every block that the GPU holds
-        assert lib.jk_cached_propagation_workspace(5, 1, 1, 1, 512, 4, 4, dtype) >= 296 * 2 * 512 * 4
-        assert lib.jk_cached_propagation_workspace(5000, 1, 1, 1, 8, 4, 4, dtype) % 16 == 0
+        assert size(0, 1, 1, 1, 8, 8, 4, 4, -1, dtype) == 0 and size(5, 1, 1, 1, 8, 8, 16, 32, -1, dtype) == 0
+        assert size(5, 1, 1, 1, 8, 8, 16, 33, 100, dtype) == 0
+        # sums and words of a row at least of every block of the GPU
+        assert size(5, 1, 1, 1, 8, 512, 16, 33, -1, dtype) >= 148 * 2 * 516 * 4
+        assert size(5000, 1, 1, 1, 8, 8, 16, 33, -1, dtype) % 16 == 0
 
 
 def test_inputs_that_ask_for_gradients_are_refused():
