@@ -11,17 +11,30 @@ int64_t part_row(int64_t dim) { return (dim + 3) / 4 * 4 + 4; }
 // Tiles that a unit can have: the places of a table's row, as far as they are seen.
 int64_t tiles_at_most(int64_t page_size, int64_t columns, int64_t window, int64_t new_nodes) {
   const int64_t room = columns > (int64_t(1) << 31) / page_size ? int64_t(1) << 31 : columns * page_size;
-  const int64_t reach = window < 0 || window + new_nodes > room ? room : window + new_nodes;
+  // (with a window tiles may begin up to 15 places before what is seen)
+  const int64_t reach = window < 0 || window + new_nodes + kKeys - 1 > room ? room : window + new_nodes + kKeys - 1;
   return reach < 1 ? 1 : (reach + kTile - 1) / kTile;
 }
 
 int32_t window_of(int64_t window) { return window < 0 ? -1 : window > 0x7fffffff ? 0x7fffffff : static_cast<int32_t>(window); }
 
 // Bytes of one asynchronous copy: the most that addresses, strides and the row's length allow.
-int chunk_of(const void* base, const int64_t (&stride)[3], int64_t row_bytes) {
+int piece_of(const void* base, const int64_t (&stride)[3], int64_t row_bytes) {
   uint64_t odd = reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(row_bytes);
   for (int64_t s : stride) odd |= static_cast<uint64_t>(s);
   return (odd & 15) == 0 ? 16 : (odd & 7) == 0 ? 8 : (odd & 3) == 0 ? 4 : 0;
+}
+
+// The map of [pages][heads][places][columns], of which a copy fetches 16 places x 128 bytes.
+bool make_map(CUtensorMap* map, const void* base, int64_t columns, const int64_t (&stride)[3], int64_t pages, int64_t heads, int64_t page_size,
+              int dtype) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(columns), static_cast<uint64_t>(page_size), static_cast<uint64_t>(heads), static_cast<uint64_t>(pages)};
+  uint64_t strides[3] = {static_cast<uint64_t>(stride[2]), static_cast<uint64_t>(stride[1]), static_cast<uint64_t>(stride[0])};
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i + 1] == 1 && strides[i] == 0) strides[i] = 16;  // of a dim of one, any
+    if (strides[i] == 0 || strides[i] >= (uint64_t(1) << 40)) return false;
+  }
+  return make_tmap_4d(map, base, dims, strides, static_cast<uint32_t>(128 / dtype_bytes(dtype)), kKeys, dtype) == JK_OK;
 }
 
 }  // namespace
@@ -37,8 +50,8 @@ int64_t jk_cached_propagation_workspace(int64_t batch, int64_t new_nodes, int64_
   if (batch < 1 || new_nodes < 1 || heads < 1 || kv_heads < 1 || rank < 1 || dim < 1 || page_size < 1 || columns < 1) return 0;
   if (tiles_at_most(page_size, columns, window_of(window), new_nodes) <= kUnitTiles) return 0;
   int64_t most = 0;
-  for (const bool blocks16 : {false, true}) {
-    const Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, blocks16);
+  for (const bool tiled : {false, true}) {
+    const Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, tiled);
     const int64_t bytes = int64_t(kSms) * s.per_sm * 2 * s.rows * part_row(dim) * 4;
     most = bytes > most ? bytes : most;
   }
@@ -86,16 +99,17 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
   // the softmax's scores are compared and subtracted in units of log 2, and a bias moves them all
   a.scale = a.compress == JK_SOFTMAX ? static_cast<float>(double(scale) * 1.4426950408889634) : scale;
   a.bias = score_bias;
-  a.key_chunk = chunk_of(q->keys, a.key_stride, rank * size), a.value_chunk = chunk_of(q->values, a.value_stride, dim * size);
-  a.blocks16 = a.key_chunk == 16 && a.value_chunk == 16;
-  Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, a.blocks16);
-  if (a.blocks16 && s.stages == 1) {  // a row copied by one instruction needs a second stage
-    a.blocks16 = false;
-    s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, false);
-  }
+  a.key_piece = piece_of(q->keys, a.key_stride, rank * size), a.value_piece = piece_of(q->values, a.value_stride, dim * size);
+  Maps maps{};
+  Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, true);
+  // tiled copies: pages of a multiple of 16 places, rows in 16-byte blocks, strides that a map can hold, and a second stage
+  a.tiled = a.key_piece == 16 && a.value_piece == 16 && page_size % kKeys == 0 && s.stages > 1 && pages > 0 && a.columns > 0 &&
+            make_map(&maps.keys, q->keys, rank, a.key_stride, pages, kv_heads, page_size, dtype) &&
+            make_map(&maps.values, q->values, dim, a.value_stride, pages, kv_heads, page_size, dtype);
+  if (!a.tiled) s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, false);
   a.rows = s.rows, a.row_blocks = s.row_blocks;
-  a.key_row = s.key_row, a.value_row = s.value_row, a.key_cols = s.key_cols;
-  a.stages = s.stages, a.stage_bytes = s.stage_bytes;
+  a.key_cols = s.key_cols, a.query_row = s.query_row, a.key_bytes = s.key_bytes;
+  a.stages = s.stages, a.stage_bytes = s.stage_bytes, a.ring_bytes = s.ring_bytes;
   a.part_row = static_cast<int32_t>(part_row(dim));
   a.parts = static_cast<float*>(q->workspace);
   a.split = split;
@@ -114,9 +128,9 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
     const int64_t slots = int64_t(kSms) * s.per_sm;
     a.blocks = static_cast<int32_t>(units > slots / unit_tiles ? slots : units * unit_tiles);
     int status;
-    if (dtype == JK_F32) status = launch_f32(a, s, units, st);
-    else if (dtype == JK_BF16) status = launch_bf16(a, s, units, st);
-    else status = launch_f16(a, s, units, st);
+    if (dtype == JK_F32) status = launch_f32(a, maps, s, units, st);
+    else if (dtype == JK_BF16) status = launch_bf16(a, maps, s, units, st);
+    else status = launch_f16(a, maps, s, units, st);
     if (status != JK_OK) return status;
   }
   return JK_OK;

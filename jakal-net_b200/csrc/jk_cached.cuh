@@ -11,10 +11,14 @@
 //     adds them up for itself). A unit that several blocks have parts of is joined by a second kernel
 //     from what they leave: reference, sum and unnormalised values. Few tiles a unit: a block each, and
 //     no second kernel.
-//   * A warp has every fourth 16 places of the run to itself: its own ring of shared memory fed by
-//     asynchronous copies, its own reference and sums, no barrier between warps until the run's end,
-//     where the four are joined in shared memory. Its turn is short of instructions, as few warps fit an
-//     SM beside their rings: 16 places that all rows see, of one page, need no masks and one address.
+//   * A warp has every fourth 16 places of the run to itself: its own ring of shared memory, its own
+//     reference and sums, no barrier between warps until the run's end, where the four are joined in
+//     shared memory. Where pages hold a multiple of 16 places in 16-byte rows, one lane fetches the 16 by
+//     tiled copies of 128-byte columns (4 for rank and dim 128 in 16 bits); else all lanes copy pieces.
+//     (One bulk copy a row takes as long as the rest of the turn: 32 of them are issued one by one.)
+//   * Few warps fit an SM beside their rings, so a turn is short of instructions: places that all rows see
+//     need no masks, and a reference that follows the maximum only once that is 8 (a factor of 256)
+//     above it needs a vote a turn in place of a maximum over the warp.
 // 16-bit types: both products are warp matrix instructions with the places (scores) and the value's
 // columns (sums) as their 16 rows, and the unit's rows as their 8 columns, of which one node of one head
 // fills one: S^T = K Q^T, O^T = V^T W^T. W^T leaves the first product with places across the wrong
@@ -22,8 +26,7 @@
 // high + low, so their rounding (2^-16 and less) is far below that of the result.
 // f32: the same walk with fused multiply-adds, which keep f32's rounding.
 // Exponentials are base 2 on a reference that is itself rounded, so partial sums with different
-// references join without a rounding of their own. The reference follows the maximum only once that is
-// 8 (a factor of 256) above it: a vote a turn, in place of a maximum over the warp.
+// references join without a rounding of their own.
 //
 // What is not seen has no part in a result, whatever it holds: places past the last node and places
 // without a page arrive as zeros, and a tile of which rows see different parts (the newest nodes of a
@@ -42,10 +45,12 @@ namespace cached {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kKeys = 16;               // places of a warp's turn
+constexpr int kColumn = 2048;           // bytes of 16 places x 128 bytes of their rows: what a tiled copy fetches
 constexpr int kTile = kWarps * kKeys;   // places of a block's turn
 constexpr int kSms = 148;
 constexpr int kMaxPerSm = 3;            // blocks of an SM
-constexpr int kMaxBatch = 1024;         // sequences of a launch
+constexpr int kMaxBatch = 256;          // sequences of a launch
+constexpr int kMaxStages = 3;           // of a warp's ring
 constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
 constexpr int kUnitTiles = 8;           // units of at most so many tiles get a block each
 constexpr float kLog2e = 1.4426950408889634f;
@@ -64,14 +69,14 @@ struct Args {
   char *out_value, *out_state;
   // layout
   int32_t blocks, row_blocks, rows;       // blocks of the grid; row blocks of a unit's rows, and rows of one
-  int32_t key_chunk, value_chunk;         // bytes of one asynchronous copy (16, 8, 4), 0: element by element
-  int32_t key_row, value_row;             // elements of a row in shared memory
+  int32_t key_piece, value_piece;         // bytes of one asynchronous copy (16, 8, 4), 0: element by element
   int32_t key_cols;                       // of a key's row read: rank rounded up to the product's steps
-  int32_t stages, stage_bytes;
-  bool blocks16;                          // rows of keys and values are in 16-byte blocks
+  int32_t query_row;                      // elements from one query to the next in shared memory
+  int32_t key_bytes, stage_bytes, stages; // of a ring: keys of a stage, a stage, their number
+  int32_t ring_bytes;                     // of all rings (and of what is joined in their place)
   int32_t part_row;                       // floats of a row that a block leaves: dim rounded up to 4, reference, sum, state
   float* parts;                           // [blocks][2][rows][part_row]
-  bool split;
+  bool split, tiled;
 };
 
 // ---- a sequence's places
@@ -80,8 +85,10 @@ struct Span {
   int32_t n;         // new nodes that count
   int32_t first;     // place of the first of them (may be negative)
   int32_t low, end;  // places that any of them sees: [low, end)
+  int32_t base;      // where the tiles begin
 };
 
+template <bool TILED>
 __device__ __forceinline__ Span span_of(const Args& a, int32_t b) {
   Span s;
   const int32_t length = a.lengths[b];
@@ -93,10 +100,13 @@ __device__ __forceinline__ Span span_of(const Args& a, int32_t b) {
   s.end = s.n == 0 || length < 0 ? 0 : length < most ? length : most;
   const int64_t low = a.window < 0 ? 0 : int64_t(s.first) - a.window;
   s.low = low < 0 ? 0 : low < s.end ? static_cast<int32_t>(low) : s.end;
+  s.base = TILED ? s.low & ~(kKeys - 1) : s.low;  // a tiled copy's places are of one page
   return s;
 }
 
-__device__ __forceinline__ int32_t tiles_of(const Span& s) { return (s.end - s.low + kTile - 1) / kTile; }
+__device__ __forceinline__ int32_t tiles_of(const Span& s) { return s.low < s.end ? (s.end - s.base + kTile - 1) / kTile : 0; }
+
+__device__ __forceinline__ Span span_as(const Args& a, int32_t b) { return a.tiled ? span_of<true>(a, b) : span_of<false>(a, b); }
 
 // ---- small pieces
 
@@ -172,16 +182,15 @@ template <int COMPRESS>
 __device__ __forceinline__ float score_of(float dot, float scale, float bias) {
   return COMPRESS == JK_SOFTMAX ? dot : fmaf(dot, scale, bias);
 }
-// Its level, which is held against the reference (units of log 2).
+// Its level above the reference, in units of log 2.
 template <int COMPRESS>
-__device__ __forceinline__ float level_of(float s, float scale) {
-  return COMPRESS == JK_SOFTMAX ? s * scale : fabsf(s) * kLog2e;
+__device__ __forceinline__ float level_of(float s, float scale, float ref) {
+  return COMPRESS == JK_SOFTMAX ? fmaf(s, scale, -ref) : fmaf(fabsf(s), kLog2e, -ref);
 }
-// Its part of the sum, on the reference (softsign: the weight itself).
+// Its part of the sum (softsign: the weight itself).
 template <int COMPRESS>
-__device__ __forceinline__ float mass_of(float s, float scale, float ref) {
-  if (COMPRESS == JK_SOFTSIGN) return s / (1.0f + fabsf(s));
-  return power2(COMPRESS == JK_SOFTMAX ? fmaf(s, scale, -ref) : fmaf(fabsf(s), kLog2e, -ref));
+__device__ __forceinline__ float mass_of(float s, float level) {
+  return COMPRESS == JK_SOFTSIGN ? s / (1.0f + fabsf(s)) : power2(level);
 }
 // Its weight.
 template <int COMPRESS>
@@ -190,34 +199,47 @@ __device__ __forceinline__ float weight_of(float s, float mass) {
   return s == 0.0f ? 0.0f : copysignf(mass, s);
 }
 
-template <typename T, int BYTES>
-__device__ __forceinline__ void load_chunks(char* dst, int32_t dst_row, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
-  const uint32_t to = shared_at(dst);
+// A stage holds columns of 128 bytes of its 16 rows, 2048 bytes each, in which the 16-byte block c of row r lies at
+// 128 r + 16 (c ^ (r mod 8)): eight rows' blocks c are in different banks. (Tiled copies write it so.)
+__device__ __forceinline__ int block_at(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
+
+template <int BYTES>
+__device__ __forceinline__ void load_pieces(uint32_t to, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {  // 8 lanes a row
     const int row = 4 * q + (lane >> 3);
     const char* from = src + __shfl_sync(0xffffffffu, offset, row);
     const bool ok = (there >> row) & 1;
-    for (int c = (lane & 7) * BYTES; c < row_bytes; c += 8 * BYTES) copy_async<BYTES>(to + row * dst_row + c, from + c, ok);
+    for (int c = (lane & 7) * BYTES; c < row_bytes; c += 8 * BYTES)
+      copy_async<BYTES>(to + (c >> 7) * kColumn + block_at(row, (c >> 4) & 7) + (c & 15), from + c, ok);
   }
 }
 
+// Rows of the 16 lanes' places; rows that are not `there` arrive as zeros.
 template <typename T>
-__device__ __forceinline__ void load_rows(char* dst, int32_t dst_row, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int chunk,
-                                          int lane) {
-  if (chunk == 16) return load_chunks<T, 16>(dst, dst_row, src, offset, there, row_bytes, lane);
-  if (chunk == 8) return load_chunks<T, 8>(dst, dst_row, src, offset, there, row_bytes, lane);
-  if (chunk == 4) return load_chunks<T, 4>(dst, dst_row, src, offset, there, row_bytes, lane);
+__device__ __forceinline__ void load_rows(char* dst, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int piece, int lane) {
+  const uint32_t to = shared_at(dst);
+  if (piece == 16) return load_pieces<16>(to, src, offset, there, row_bytes, lane);
+  if (piece == 8) return load_pieces<8>(to, src, offset, there, row_bytes, lane);
+  if (piece == 4) return load_pieces<4>(to, src, offset, there, row_bytes, lane);
   if constexpr (sizeof(T) == 2) {  // 16-bit rows of an odd width, or that begin anywhere
-    const int n = row_bytes / 2;
 #pragma unroll 4
     for (int row = 0; row < kKeys; ++row) {
       const char* from = src + __shfl_sync(0xffffffffu, offset, row);
       const bool ok = (there >> row) & 1;
-      for (int c = lane; c < n; c += 32)
-        reinterpret_cast<uint16_t*>(dst + row * dst_row)[c] = ok ? reinterpret_cast<const uint16_t*>(from)[c] : uint16_t(0);
+      for (int c = 2 * lane; c < row_bytes; c += 64)
+        *reinterpret_cast<uint16_t*>(dst + (c >> 7) * kColumn + block_at(row, (c >> 4) & 7) + (c & 15)) =
+            ok ? *reinterpret_cast<const uint16_t*>(from + c) : uint16_t(0);
     }
   }
+}
+
+// One column of 128 bytes of the 16 places from `place` on of a page: a tiled copy, counted on `bar`.
+__device__ __forceinline__ void load_column(char* dst, const CUtensorMap* map, uint64_t* bar, int element, int place, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(shared_at(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(shared_at(bar)), "r"(element), "r"(place), "r"(head), "r"(page)
+      : "memory");
 }
 
 // ---- the kernel
@@ -228,11 +250,16 @@ struct Turn {
   float state;
 };
 
+// The tensor maps of the tiled copies: dims (columns of a row, places, heads, pages).
+struct Maps {
+  CUtensorMap keys, values;
+};
+
 // ROWS: rows of a unit that a block takes (a multiple of 8 for 16-bit types); DIM: columns of the value at most.
-// BULK: rows of keys and values are in 16-byte blocks, so each lane copies one row by one instruction (lanes 0-15 the keys,
-// the others the values). Else rows are copied in pieces of the size that their alignment allows.
-template <typename T, int ROWS, int DIM, int COMPRESS, bool BULK>
-__global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) cached_kernel(const __grid_constant__ Args a) {
+// TILED: pages hold a multiple of 16 places, and the maps fetch them.
+template <typename T, int ROWS, int DIM, int COMPRESS, bool TILED>
+__global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) cached_kernel(const __grid_constant__ Args a,
+                                                                                             const __grid_constant__ Maps maps) {
   constexpr bool kWide = std::is_same_v<T, float>;
   constexpr int NT = kWide ? 1 : ROWS / 8;             // 8-row tiles of the matrix instructions
   constexpr int MT = kWide ? 1 : DIM / 16;             // 16-column tiles of the value
@@ -240,17 +267,19 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   // rows whose reference and sum a thread keeps (f32: half of them, lanes 16.. the other half)
   constexpr int OWN = kWide ? (ROWS + 1) / 2 : 2 * NT;
   constexpr int SIZE = sizeof(T);
-  extern __shared__ __align__(16) char memory[];
+  constexpr int COLUMN = 128 / SIZE;                   // elements of a 128-byte column
+  extern __shared__ char memory_[];
   __shared__ int64_t before[kMaxBatch + 1];
   __shared__ int64_t scan[kWarps];
   __shared__ float ref_s[kWarps][ROWS], sum_s[kWarps][ROWS], state_s[kWarps][ROWS];
-  __shared__ uint64_t landed[kWarps][2];
+  __shared__ uint64_t landed[kWarps][kMaxStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint32_t issued = 0, taken = 0;  // BULK: this warp's turns that copied something, of all units
+  int fill = 0, take = 0;          // TILED: the stage that the next turn fills, and the one that is taken next, of all units
+  uint32_t phase = 0, issued = 0;  // and the phase of the latter; turns that copied something
   bool late = false;               // a wait gave up
-  if (BULK && lane == 0) {
-    mbar_init(&landed[warp][0], 1);
-    mbar_init(&landed[warp][1], 1);
+  if (TILED && lane == 0) {
+    if (warp == 0) prefetch_tmap(&maps.keys), prefetch_tmap(&maps.values);
+    for (int i = 0; i < kMaxStages; ++i) mbar_init(&landed[warp][i], 1);
     fence_barrier_init();
   }
   __syncwarp();
@@ -262,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     if (tid == 0) before[0] = 0;
     for (int32_t base = 0; base < a.batch; base += kThreads) {
       const int32_t b = base + tid;
-      int64_t v = b < a.batch ? int64_t(tiles_of(span_of(a, b))) * a.kv_heads * a.row_blocks : 0;
+      int64_t v = b < a.batch ? int64_t(tiles_of(span_of<TILED>(a, b))) * a.kv_heads * a.row_blocks : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
@@ -286,15 +315,14 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     until = at + chunk < carry ? at + chunk : carry;
   }
 
-  // shared memory: queries, the weights of a tile that is added up row by row, then the rings
-  const int query_row = a.key_row;
-  T* query = reinterpret_cast<T*>(memory);
+  // shared memory: the rings (whose columns begin at multiples of 1024 bytes), queries, and the weights of a tile that is
+  // added up row by row
+  char* const memory = memory_ + ((1024u - (shared_at(memory_) & 1023u)) & 1023u);
+  char* const ring = memory + warp * a.stages * a.stage_bytes;
+  float* const joined = reinterpret_cast<float*>(memory);  // [kWarps][ROWS][DIM + 4], once the rings are drained
+  T* const query = reinterpret_cast<T*>(memory + a.ring_bytes);
   constexpr int kWeightRow = kWide ? kKeys : kKeys + 1;
-  float* weights = reinterpret_cast<float*>(memory + ((ROWS * query_row * SIZE + 15) & ~15)) + warp * (ROWS * kWeightRow);
-  char* rings = memory + ((ROWS * query_row * SIZE + 15) & ~15) + ((kWarps * ROWS * kWeightRow * 4 + 15) & ~15);
-  const int key_bytes = kKeys * a.key_row * SIZE;
-  char* const ring = rings + warp * a.stages * a.stage_bytes;
-  float* joined = reinterpret_cast<float*>(rings);  // [kWarps][ROWS][DIM + 4], once the rings are drained
+  float* const weights = reinterpret_cast<float*>(memory + a.ring_bytes + ROWS * a.query_row * SIZE) + warp * (ROWS * kWeightRow);
 
   while (at < until) {
     // ---- the unit and the run of its tiles
@@ -311,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     } else {
       b = blockIdx.x / (a.kv_heads * a.row_blocks);
     }
-    const Span span = span_of(a, b);
+    const Span span = span_of<TILED>(a, b);
     unit_tiles = tiles_of(span);
     if (a.split) {
       const int64_t in = at - before[b];
@@ -340,10 +368,10 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     const char* values = a.values + kv * a.value_stride[1];
     const char* states = a.states == nullptr ? nullptr : a.states + kv * a.state_stride[1];
     const int32_t* table = a.table + b * a.table_stride;
-    const int32_t key0 = span.low + tile * kTile + warp * kKeys;
-    // the page and offset of this lane's place, turn after turn
-    const uint32_t first_place = static_cast<uint32_t>(key0) + (lane & 15);
-    uint32_t column = first_place / a.page_size, offset = first_place - column * a.page_size;
+    const int32_t key0 = span.base + tile * kTile + warp * kKeys;
+    // page and offset of a place, turn after turn: of the turn's first where one page has them all, else of this lane's
+    const int own_place = lane & 15, looked_up = TILED ? 0 : own_place;
+    uint32_t column = static_cast<uint32_t>(key0 + looked_up) / a.page_size, offset = static_cast<uint32_t>(key0 + looked_up) - column * a.page_size;
     const uint32_t column_step = kTile / a.page_size, offset_step = kTile - column_step * a.page_size;
     struct Place {
       int32_t page;  // -1: none
@@ -352,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     auto next_place = [&](int32_t i) {
       Place p{-1, offset};
       // (64 bits: the turn after the last may lie past 2^31)
-      if (i < tiles && int64_t(key0) + int64_t(i) * kTile + (lane & 15) < span.end) {
+      if (i < tiles && int64_t(key0) + int64_t(i) * kTile + looked_up < span.end) {
         const int32_t page = table[column];
         if (static_cast<uint32_t>(page) < static_cast<uint64_t>(a.pages)) p.page = page;
       }
@@ -364,45 +392,46 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     auto issue = [&](int32_t i, Place p) {
       Turn made{0, 0.0f};
       if (i < tiles && !late) {
-        const int place = lane & 15;
-        const bool mine = p.page >= 0;
-        made.there = __ballot_sync(0xffffffffu, mine) & 0xffffu;
-        if (BULK) {
-          if (made.there != 0) {
-            char* stage = ring + (issued & 1) * a.stage_bytes;
-            uint64_t* bar = &landed[warp][issued & 1];
-            ++issued;
-            const int key_row = a.rank * SIZE, value_row = a.dim * SIZE;
-            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(made.there) * (key_row + value_row));
-            char* to = lane < 16 ? stage + place * a.key_row * SIZE : stage + key_bytes + place * a.value_row * SIZE;
-            if (mine) {
-              const char* from = lane < 16 ? keys + p.page * a.key_stride[0] + p.offset * a.key_stride[2]
-                                           : values + p.page * a.value_stride[0] + p.offset * a.value_stride[2];
-              bulk_load(to, from, lane < 16 ? key_row : value_row, bar);
-            } else if (lane >= 16) {  // a weight of 0 is no help against a value of NaN
-              for (int c = 0; c < value_row; c += 16) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
-              fence_proxy_async_smem();
+        if (TILED) {
+          const int32_t k0 = key0 + i * kTile;
+          const int low = span.low - k0, high = span.end - k0;  // places of this turn that count: [low, high), low < 16
+          if (p.page >= 0 && high > 0) {
+            made.there = (high >= kKeys ? 0xffffu : (1u << high) - 1) & (low <= 0 ? 0xffffu : 0xffffu << low);
+            if (lane == 0) {
+              char* stage = ring + fill * a.stage_bytes;
+              uint64_t* bar = &landed[warp][fill];
+              mbar_arrive_expect_tx(bar, a.stage_bytes);
+              for (int c = 0; c < a.rank; c += COLUMN, stage += kColumn) load_column(stage, &maps.keys, bar, c, p.offset, kv, p.page);
+              for (int c = 0; c < a.dim; c += COLUMN, stage += kColumn) load_column(stage, &maps.values, bar, c, p.offset, kv, p.page);
             }
+            fill = fill + 1 == a.stages ? 0 : fill + 1;
+            ++issued;
           }
+          p.offset += own_place;
         } else {
+          made.there = __ballot_sync(0xffffffffu, p.page >= 0) & 0xffffu;
           char* stage = ring + (a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
-          const int64_t page = mine ? p.page : 0, off = mine ? p.offset : 0;
-          load_rows<T>(stage, a.key_row * SIZE, keys, page * a.key_stride[0] + off * a.key_stride[2], made.there, a.rank * SIZE, a.key_chunk, lane);
-          load_rows<T>(stage + key_bytes, a.value_row * SIZE, values, page * a.value_stride[0] + off * a.value_stride[2], made.there, a.dim * SIZE,
-                       a.value_chunk, lane);
+          const int64_t page = p.page >= 0 ? p.page : 0, off = p.page >= 0 ? p.offset : 0;
+          load_rows<T>(stage, keys, page * a.key_stride[0] + off * a.key_stride[2], made.there, a.rank * SIZE, a.key_piece, lane);
+          load_rows<T>(stage + a.key_bytes, values, page * a.value_stride[0] + off * a.value_stride[2], made.there, a.dim * SIZE, a.value_piece, lane);
         }
-        if (states != nullptr && mine)
+        if (states != nullptr && ((made.there >> own_place) & 1))
           made.state = to_f32(*reinterpret_cast<const T*>(states + p.page * a.state_stride[0] + p.offset * a.state_stride[2]));
       }
-      if (!BULK) copy_commit();
+      if (!TILED) copy_commit();
       return made;
     };
-    const int lead = BULK ? 1 : a.stages - 1;  // turns on their way while one is worked on
+    const int lead = TILED && a.stages == kMaxStages ? 2 : a.stages > 1 ? 1 : 0;  // turns on their way while one is worked on
     Place todo = next_place(0);
-    Turn turn{0, 0.0f};
+    Turn first{0, 0.0f}, second{0, 0.0f};
     if (lead) {
       const Place after = next_place(1);
-      turn = issue(0, todo);
+      first = issue(0, todo);
+      todo = after;
+    }
+    if (lead == 2) {
+      const Place after = next_place(2);
+      second = issue(1, todo);
       todo = after;
     }
 
@@ -411,19 +440,20 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
       const bool counts = r < rows && t < span.n;
       const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
-      for (int c = lane; c < a.key_cols; c += 32) query[r * query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
+      for (int c = lane; c < a.key_cols; c += 32) query[r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
     }
-    if (a.key_cols > a.rank) {
+    if (!TILED && a.key_cols > a.rank) {
       for (int i = lane; i < a.stages * kKeys; i += 32) {
-        T* k = reinterpret_cast<T*>(ring + i / kKeys * a.stage_bytes) + i % kKeys * a.key_row;
-        for (int c = a.rank; c < a.key_cols; ++c) k[c] = from_f32<T>(0.0f);
+        char* k = ring + i / kKeys * a.stage_bytes;
+        for (int c = a.rank; c < a.key_cols; ++c)
+          *reinterpret_cast<T*>(k + c / COLUMN * kColumn + block_at(i % kKeys, c % COLUMN * SIZE / 16) + c * SIZE % 16) = from_f32<T>(0.0f);
       }
     }
 
     // ---- this thread's rows: the places they see, [row_low, row_end)
     const int own_row = kWide && ROWS > 1 && lane >= 16 ? OWN : 0;
     int32_t row_low[OWN], row_end[OWN];
-    float ref[OWN], sum[OWN], state[OWN];
+    float ref[OWN], base[OWN], sum[OWN], state[OWN];  // base: the reference, 0 while there is none
     bool any[OWN];
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
@@ -433,10 +463,11 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       const int32_t place = span.first + t;
       row_end[i] = !counts ? 0 : place + 1 < span.end ? place + 1 : span.end;
       row_low[i] = a.window < 0 || place < a.window ? 0 : place - a.window;
-      ref[i] = COMPRESS == JK_SOFTSIGN ? 0.0f : -INFINITY;
-      sum[i] = state[i] = 0.0f;
+      ref[i] = COMPRESS == JK_SOFTSIGN || !counts ? 0.0f : -INFINITY;
+      base[i] = sum[i] = state[i] = 0.0f;
       any[i] = false;
     }
+    bool unset = true;  // a row that counts has no reference yet
     float out[MT][NT * 4];
     uint64_t pairs[kWide ? ROWS : 1][CP];  // f32's sums
 #pragma unroll
@@ -453,28 +484,36 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       __syncwarp();  // the stage to fill has been read by all lanes
       const Place after = next_place(i + lead + 1);
       const Turn made = issue(i + lead, todo);
-      const Turn now = lead ? turn : made;
-      turn = made;
+      const Turn now = lead ? first : made;
+      first = lead == 2 ? second : made;
+      second = made;
       todo = after;
       const uint32_t there = now.there;
-      if (!BULK) copy_wait(lead);
+      if (!TILED) copy_wait(lead);
       if (there == 0) continue;
-      const char* stage = ring + (BULK ? taken & 1 : a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
-      if (BULK) {
-        if (!late && !mbar_wait(&landed[warp][taken & 1], (taken >> 1) & 1)) {
+      char* const stage = ring + (TILED ? take : a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
+      if (TILED) {
+        if (!late && !mbar_wait(&landed[warp][take], phase)) {
           late = true;
           g_device_error = JK_ERR_DEVICE_TIMEOUT;
         }
         late = __any_sync(0xffffffffu, late);
-        ++taken;
+        if (++take == a.stages) take = 0, phase ^= 1;
       }
       __syncwarp();
-      const T* const stage_keys = reinterpret_cast<const T*>(stage);
-      const T* const stage_values = reinterpret_cast<const T*>(stage + key_bytes);
+      char* const stage_values = stage + a.key_bytes;
       const int32_t k0 = key0 + i * kTile;
       // rows see different parts of it
-      const bool mixed = (k0 + kKeys < span.end ? k0 + kKeys : span.end) > all_end || k0 < all_low;
+      const bool mixed = (k0 + kKeys < span.end ? k0 + kKeys : span.end) > all_end || (k0 > span.low ? k0 : span.low) < all_low;
       const bool full = there == 0xffffu && !mixed;
+      if (TILED && there != 0xffffu) {  // rows of values that do not count: 0, as a weight of 0 is no help against NaN
+        for (int r = lane >> 3; r < kKeys; r += 4)
+          if (!((there >> r) & 1))
+            for (int c = lane & 7; c < (a.stage_bytes - a.key_bytes) / kColumn * 8; c += 8)
+              *reinterpret_cast<uint4*>(stage_values + (c >> 3) * kColumn + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // before the next copy into them
+        __syncwarp();
+      }
 
       if constexpr (!kWide) {
         float c[NT][4], c2[NT][4];
@@ -483,22 +522,23 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[n][e] = c2[n][e] = 0.0f;
         {
-          // K: matrices (places 0-7 | 8-15) x (columns 0-7 | 8-15); Q: rows 0-7 x four times 8 columns; two steps at a time
-          uint32_t k_at = shared_at(stage_keys + (lane & 15) * a.key_row + (lane >> 4) * 8);
-          uint32_t q_at = shared_at(query + (lane & 7) * query_row + (lane >> 3) * 8);
+          // K: matrices (places 0-7 | 8-15) x (columns 0-7 | 8-15); Q: rows 0-7 x four times 8 columns; two steps at a time,
+          // four in a column of 128 bytes
+          uint32_t k_at = shared_at(stage) + block_at(lane & 15, lane >> 4);
+          uint32_t q_at = shared_at(query + (lane & 7) * a.query_row + (lane >> 3) * 8);
 #pragma unroll 2
           for (int k = 0; k < a.key_cols; k += 32) {
             uint32_t ka[4], kb[4];
             ldmatrix4(ka, k_at);
-            ldmatrix4(kb, k_at + 32);
+            ldmatrix4(kb, k_at ^ 32);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               uint32_t q[4];
-              ldmatrix4(q, q_at + n * 16 * query_row);
+              ldmatrix4(q, q_at + n * 16 * a.query_row);
               mma<T>(c[n], ka, q[0], q[1]);
               mma<T>(c2[n], kb, q[2], q[3]);
             }
-            k_at += 64;
+            k_at = (k & 32) ? (k_at ^ 64) + kColumn : k_at ^ 64;
             q_at += 64;
           }
         }
@@ -513,7 +553,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         auto weigh = [&](auto whole) {
           constexpr bool FULL = decltype(whole)::value;
           bool sees[NT][4];
-          bool higher = false;
+          float level[NT][4];
+          bool higher = unset;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -522,31 +563,38 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               c[n][e] = score_of<COMPRESS>(c[n][e] + c2[n][e], a.scale, a.bias);
               sees[n][e] = FULL || (((there >> p) & 1) && k0 + p < row_end[i2] && k0 + p >= row_low[i2]);
               any[i2] |= sees[n][e];
-              if (COMPRESS != JK_SOFTSIGN) higher |= sees[n][e] && level_of<COMPRESS>(c[n][e], a.scale) > ref[i2] + kSlack;
+              level[n][e] = level_of<COMPRESS>(c[n][e], a.scale, base[i2]);
+              higher |= sees[n][e] && level[n][e] > kSlack;
             }
           if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
+            unset = false;
 #pragma unroll
             for (int i2 = 0; i2 < OWN; ++i2) {
               const int n = i2 >> 1, e = i2 & 1;
-              float top = sees[n][e] ? level_of<COMPRESS>(c[n][e], a.scale) : -INFINITY;
-              if (sees[n][e + 2]) top = fmaxf(top, level_of<COMPRESS>(c[n][e + 2], a.scale));
+              float top = sees[n][e] ? level[n][e] + base[i2] : -INFINITY;
+              if (sees[n][e + 2]) top = fmaxf(top, level[n][e + 2] + base[i2]);
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               top = fmaxf(top, ref[i2]);
               const float factor = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
               ref[i2] = top;
+              base[i2] = top == -INFINITY ? 0.0f : top;
+              unset |= top == -INFINITY;
               sum[i2] *= factor;
               state[i2] *= factor;
+              level[n][e] = level_of<COMPRESS>(c[n][e], a.scale, base[i2]);
+              level[n][e + 2] = level_of<COMPRESS>(c[n][e + 2], a.scale, base[i2]);
 #pragma unroll
               for (int m = 0; m < MT; ++m) out[m][4 * n + e] *= factor, out[m][4 * n + e + 2] *= factor;
             }
+            unset = __any_sync(0xffffffffu, unset);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int i2 = 2 * n + (e & 1);
-              float w = mass_of<COMPRESS>(c[n][e], a.scale, COMPRESS == JK_SOFTSIGN || ref[i2] == -INFINITY ? 0.0f : ref[i2]);
+              float w = mass_of<COMPRESS>(c[n][e], level[n][e]);
               if (!FULL && !sees[n][e]) w = 0.0f;
               if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
               w = weight_of<COMPRESS>(c[n][e], w);
@@ -571,14 +619,14 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               low[n][h] = transpose8(*reinterpret_cast<const uint32_t*>(&lo));
             }
           // V^T: matrices (columns 0-7 | 8-15) x (places 0-7 | 8-15), read transposed
-          const uint32_t v_at = shared_at(stage_values + ((lane & 7) + ((lane >> 4) & 1) * 8) * a.value_row + ((lane >> 3) & 1) * 8);
+          const uint32_t v_at = shared_at(stage_values) + block_at((lane & 7) + ((lane >> 4) & 1) * 8, (lane >> 3) & 1);
 #pragma unroll
           for (int m4 = 0; m4 < MT; m4 += 4) {
             if (m4 * 16 < a.dim) {  // (columns past the value's are read and added up for nothing)
 #pragma unroll
               for (int m = m4; m < m4 + 4; ++m) {
                 uint32_t va[4];
-                ldmatrix4_trans(va, v_at + m * 32);
+                ldmatrix4_trans(va, (v_at ^ (32 * (m & 3))) + (m >> 2) * kColumn);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   float(&o)[4] = *reinterpret_cast<float(*)[4]>(&out[m][4 * n]);
@@ -594,7 +642,6 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) weights[(8 * n + 2 * (lane & 3) + (e & 1)) * kWeightRow + place + 8 * (e >> 1)] = c[n][e];
           __syncwarp();
-          const T* v = stage_values + place;
 #pragma unroll 1
           for (int k = 0; k < kKeys; ++k) {
             if (!((there >> k) & 1)) continue;
@@ -607,8 +654,11 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                   if (m * 16 < a.dim) {
-                    out[m][4 * n + e] = fmaf(w, to_f32(v[k * a.value_row + m * 16]), out[m][4 * n + e]);
-                    out[m][4 * n + e + 2] = fmaf(w, to_f32(v[k * a.value_row + m * 16 + 8]), out[m][4 * n + e + 2]);
+                    const uint32_t at0 = static_cast<uint32_t>(32 * (m & 3)), column0 = (m >> 2) * kColumn;
+                    const T x0 = *reinterpret_cast<const T*>(stage_values + column0 + k * 128 + ((at0 ^ ((k & 7) << 4)) + 2 * place));
+                    const T x1 = *reinterpret_cast<const T*>(stage_values + column0 + k * 128 + (((at0 + 16) ^ ((k & 7) << 4)) + 2 * place));
+                    out[m][4 * n + e] = fmaf(w, to_f32(x0), out[m][4 * n + e]);
+                    out[m][4 * n + e + 2] = fmaf(w, to_f32(x1), out[m][4 * n + e + 2]);
                   }
                 }
               }
@@ -616,57 +666,58 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         }
       } else {
         // f32: a lane has half of a place's columns, lanes 16.. the other half
-        const int place = lane & 15;
-        const int half = a.key_cols / 2;
-        const float* k = stage_keys + place * a.key_row + (lane < 16 ? 0 : half);
-        const float* q = reinterpret_cast<const float*>(query) + (lane < 16 ? 0 : half);
+        const int place = own_place, half = a.key_cols / 2, x0 = lane < 16 ? 0 : half;
+        const float* q = reinterpret_cast<const float*>(query) + x0;
         uint64_t dots[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) dots[r] = 0;
 #pragma unroll 2
         for (int x = 0; x < half; x += 4) {
-          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(k + x);
+          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(stage + ((x0 + x) >> 5) * kColumn + block_at(place, ((x0 + x) >> 2) & 7));
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
-            const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(q + r * query_row + x);
+            const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(q + r * a.query_row + x);
             dots[r] = fma2(k4.y, q4.y, fma2(k4.x, q4.x, dots[r]));
           }
         }
-        float score[OWN];
+        float score[OWN], level[OWN];
+        bool sees[OWN];
+        bool higher = unset;
 #pragma unroll
         for (int i2 = 0; i2 < OWN; ++i2) {
           float2 v = unpair(dots[i2]);
-          const float first = v.x + v.y;
+          const float mine = v.x + v.y;
           if (ROWS == 1) {
-            score[i2] = first + __shfl_xor_sync(0xffffffffu, first, 16);
+            score[i2] = mine + __shfl_xor_sync(0xffffffffu, mine, 16);
           } else {  // each half of the warp gives the other half the sums of its rows
             v = unpair(dots[i2 + ROWS - OWN]);
-            const float second = v.x + v.y;
-            score[i2] = (lane < 16 ? first : second) + __shfl_xor_sync(0xffffffffu, lane < 16 ? second : first, 16);
+            const float other = v.x + v.y;
+            score[i2] = (lane < 16 ? mine : other) + __shfl_xor_sync(0xffffffffu, lane < 16 ? other : mine, 16);
           }
           score[i2] = score_of<COMPRESS>(score[i2], a.scale, a.bias);
-        }
-        bool sees[OWN];
-        bool higher = false;
-#pragma unroll
-        for (int i2 = 0; i2 < OWN; ++i2) {
           sees[i2] = full || (((there >> place) & 1) && k0 + place < row_end[i2] && k0 + place >= row_low[i2]);
           any[i2] |= sees[i2];
-          if (COMPRESS != JK_SOFTSIGN) higher |= sees[i2] && level_of<COMPRESS>(score[i2], a.scale) > ref[i2] + kSlack;
+          level[i2] = level_of<COMPRESS>(score[i2], a.scale, base[i2]);
+          higher |= sees[i2] && level[i2] > kSlack;
         }
         if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
           float factor[OWN];
+          unset = false;
 #pragma unroll
           for (int i2 = 0; i2 < OWN; ++i2) {
-            float top = sees[i2] ? level_of<COMPRESS>(score[i2], a.scale) : -INFINITY;
+            float top = sees[i2] ? level[i2] + base[i2] : -INFINITY;
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             top = fmaxf(top, ref[i2]);
             factor[i2] = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
             ref[i2] = top;
+            base[i2] = top == -INFINITY ? 0.0f : top;
+            unset |= top == -INFINITY;
             sum[i2] *= factor[i2];
             state[i2] *= factor[i2];
+            level[i2] = level_of<COMPRESS>(score[i2], a.scale, base[i2]);
           }
+          unset = __any_sync(0xffffffffu, unset);
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
             const float f = __shfl_sync(0xffffffffu, factor[r % OWN], r < OWN ? 0 : 16);
@@ -676,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         }
 #pragma unroll
         for (int i2 = 0; i2 < OWN; ++i2) {
-          float w = mass_of<COMPRESS>(score[i2], a.scale, COMPRESS == JK_SOFTSIGN || ref[i2] == -INFINITY ? 0.0f : ref[i2]);
+          float w = mass_of<COMPRESS>(score[i2], level[i2]);
           w = sees[i2] ? w : 0.0f;
           if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
           w = sees[i2] ? weight_of<COMPRESS>(score[i2], w) : 0.0f;
@@ -684,7 +735,9 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           weights[(own_row + i2) * kWeightRow + place] = w;
         }
         __syncwarp();
-        const float* v = stage_values + 2 * lane;
+        // a lane's columns 2 lane and 2 lane + 1 of every 64
+        const char* v = stage_values + (lane >> 4) * kColumn + (lane & 1) * 8;
+        const int block = (lane & 15) >> 1;
         constexpr int AT_ONCE = DIM == 512 ? 2 : 4;  // places whose values are in registers together
 #pragma unroll 1
         for (int k4 = 0; k4 < kKeys; k4 += AT_ONCE) {
@@ -692,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
           for (int k1 = 0; k1 < AT_ONCE; ++k1)
 #pragma unroll
-            for (int y = 0; y < CP; ++y) x[k1][y] = *reinterpret_cast<const uint64_t*>(v + (k4 + k1) * a.value_row + 64 * y);
+            for (int y = 0; y < CP; ++y) x[k1][y] = *reinterpret_cast<const uint64_t*>(v + 2 * y * kColumn + block_at(k4 + k1, block));
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
             float w[AT_ONCE];
@@ -719,9 +772,10 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         }
       }
     }
-    if (!BULK) copy_wait(0);
+    if (!TILED) copy_wait(0);
     // what gave up waiting still lets its copies land
-    for (uint32_t q = issued < 2 ? 0 : issued - 2; BULK && late && q != issued; ++q) mbar_wait(&landed[warp][q & 1], (q >> 1) & 1);
+    for (uint32_t q = issued < uint32_t(a.stages) ? 0 : issued - a.stages; TILED && late && q != issued; ++q)
+      mbar_wait(&landed[warp][q % a.stages], (q / a.stages) & 1);
 
     // ---- the warps' sums, then the block's
 #pragma unroll
@@ -803,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         }
       }
     }
-    if (BULK) fence_proxy_async_smem();
+    if (TILED) fence_proxy_async_smem();
     __syncthreads();  // before the next unit's queries, and before the rings are filled again
     if (a.split) at += tiles;
     else at = until;
@@ -826,11 +880,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   const int32_t t = row_of / a.group, g = row_of - t * a.group;
   const int64_t row = (int64_t(b) * a.new_nodes + t) * a.heads + kv * a.group + g;
   // the blocks' runs, as the first kernel has them (while it runs)
-  const Span span = span_of(a, b);
+  const Span span = span_as(a, b);
   const int32_t tiles = tiles_of(span);
   int64_t mine = 0, all_tiles = 0;
   for (int32_t i = tid; i < a.batch; i += 256) {
-    const int64_t n = int64_t(tiles_of(span_of(a, i))) * a.kv_heads * a.row_blocks;
+    const int64_t n = int64_t(tiles_of(span_as(a, i))) * a.kv_heads * a.row_blocks;
     all_tiles += n;
     if (i < b) mine += n;
   }
@@ -915,115 +969,116 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 struct Shape {
   int rows, dim;     // template arguments
   int row_blocks;
-  int key_cols, key_row, value_row;
+  int key_cols, query_row, key_bytes, stage_bytes, stages, ring_bytes;
   size_t shared;
-  int stages, stage_bytes, per_sm;
+  int per_sm;        // blocks of an SM
 };
 
 // Rows of a block and its shared memory, from sizes alone (the workspace's size depends on them).
-inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, bool blocks16) {
+inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, bool tiled) {
   Shape s;
   const bool wide = dtype == JK_F32;
-  const int size = wide ? 4 : 2;
+  const int size = wide ? 4 : 2, column = 128 / size;
   s.dim = dim <= 64 && !wide ? 64 : dim <= 128 ? 128 : dim <= 256 ? 256 : 512;
-  // 128 registers of sums a thread at most (f32: 64, as it keeps a tile's values too); rows that are copied in smaller
-  // pieces take what time that takes, so they have one size of a block
-  if (wide) s.rows = !blocks16 ? 4 : unit_rows == 1 ? 1 : unit_rows <= 4 || s.dim == 512 ? 4 : 8;
-  else s.rows = !blocks16 || unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
+  // 128 registers of sums a thread at most (f32: 64, as it keeps a tile's values too); where rows are copied in pieces the
+  // copies are what takes time, so blocks have one size
+  if (wide) s.rows = !tiled ? 4 : unit_rows == 1 ? 1 : unit_rows <= 4 || s.dim == 512 ? 4 : 8;
+  else s.rows = !tiled || unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
   s.row_blocks = static_cast<int>((unit_rows + s.rows - 1) / s.rows);
-  // columns in the products' steps (two of 16, or two halves of 4), and rows an odd number of 16-byte blocks apart, so that
+  // columns in the products' steps (two of 16, or two halves of 4); queries an odd number of 16-byte blocks apart, so that
   // eight of them lie in different banks
   s.key_cols = static_cast<int>(wide ? (rank + 7) / 8 * 8 : (rank + 31) / 32 * 32);
-  s.key_row = s.key_cols + 16 / size;
-  s.value_row = static_cast<int>(wide ? (dim + 3) / 4 * 4 : (dim + 15) / 16 * 16 + 8);
-  s.stage_bytes = kKeys * (s.key_row + s.value_row) * size;
-  const size_t fixed = ((s.rows * s.key_row * size + 15) & ~15) + ((kWarps * s.rows * (wide ? kKeys : kKeys + 1) * 4 + 15) & ~15);
-  const size_t join = size_t(kWarps) * s.rows * (s.dim + 4) * 4;
-  auto bytes = [&](int stages) {
-    const size_t rings = size_t(kWarps) * stages * s.stage_bytes;
-    // (the last row is read up to DIM columns)
-    return fixed + (rings + s.dim * size > join ? rings + s.dim * size : join);
+  s.query_row = s.key_cols + 16 / size;
+  s.key_bytes = static_cast<int>((rank + column - 1) / column) * kColumn;
+  s.stage_bytes = s.key_bytes + static_cast<int>((dim + column - 1) / column) * kColumn;
+  const int join = kWarps * s.rows * (s.dim + 4) * 4;
+  // f32 reads a value's row up to DIM columns
+  const int past = wide ? s.dim / column * kColumn - (s.stage_bytes - s.key_bytes) : 0;
+  auto ring = [&](int stages) {
+    const int bytes = kWarps * stages * s.stage_bytes + past;
+    return bytes > join ? bytes : join;
   };
-  // Two stages a warp, in as many blocks as an SM holds (three at most: registers); where not even one block has room for
-  // them, one stage. (32 sequences of 10240 f16 nodes, rank and dim 128: see the figures above.)
-  const size_t sm = 227 * 1024, fixed_block = 10 * 1024 + 512;
-  s.stages = bytes(2) + fixed_block <= sm ? 2 : 1;
-  s.per_sm = static_cast<int>(sm / (bytes(s.stages) + fixed_block));
+  const int rest = s.rows * s.query_row * size + kWarps * s.rows * (wide ? kKeys : kKeys + 1) * 4;
+  auto blocks = [&](int stages) { return static_cast<int>(227 * 1024 / (1024 + ring(stages) + rest + 4 * 1024)); };
   const int most = s.rows * s.dim <= 1024 ? kMaxPerSm : 2;
-  if (s.per_sm > most) s.per_sm = most;
-  s.shared = bytes(s.stages);
+  // Two stages a warp in as many blocks of an SM as fit, a third where that costs none; where not even one block has room for
+  // two, one stage. (32 sequences of 10240 f16 nodes, rank and dim 128: see the figures above.)
+  s.stages = blocks(2) < 1 ? 1 : tiled && blocks(3) >= (blocks(2) < most ? blocks(2) : most) ? 3 : 2;
+  s.per_sm = blocks(s.stages) < most ? blocks(s.stages) : most;
+  s.ring_bytes = ring(s.stages);
+  s.shared = 1024 + s.ring_bytes + rest;
   return s;
 }
 
-template <typename T, int ROWS, int DIM, int COMPRESS, bool BULK>
-int launch_kernel(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(cached_kernel<T, ROWS, DIM, COMPRESS, BULK>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(s.shared)) != cudaSuccess) {
+template <typename T, int ROWS, int DIM, int COMPRESS, bool TILED>
+int launch_kernel(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) {
+  if (cudaFuncSetAttribute(cached_kernel<T, ROWS, DIM, COMPRESS, TILED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(s.shared)) != cudaSuccess) {
     cudaGetLastError();
     return JK_ERR_LAUNCH;
   }
-  cached_kernel<T, ROWS, DIM, COMPRESS, BULK><<<static_cast<unsigned>(a.split ? a.blocks : units), kThreads, s.shared, stream>>>(a);
+  cached_kernel<T, ROWS, DIM, COMPRESS, TILED><<<static_cast<unsigned>(a.split ? a.blocks : units), kThreads, s.shared, stream>>>(a, maps);
   if (int st = launch_status()) return st;
   if (!a.split) return JK_OK;
   launch_dependent(join_kernel<T>, static_cast<unsigned>(int64_t(a.batch) * a.heads * a.new_nodes * ((a.dim + 127) / 128)), 256, 0, stream, a);
   return launch_status();
 }
 
-template <typename T, int ROWS, int DIM, bool BULK = true>
-int launch_one(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
-  if (a.compress == JK_SOFTMAX) return launch_kernel<T, ROWS, DIM, JK_SOFTMAX, BULK>(a, s, units, stream);
-  if (a.compress == JK_SOFTSIGN) return launch_kernel<T, ROWS, DIM, JK_SOFTSIGN, BULK>(a, s, units, stream);
-  return launch_kernel<T, ROWS, DIM, JK_SIGNED_ABS_SOFTMAX, BULK>(a, s, units, stream);
+template <typename T, int ROWS, int DIM, bool TILED = true>
+int launch_one(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) {
+  if (a.compress == JK_SOFTMAX) return launch_kernel<T, ROWS, DIM, JK_SOFTMAX, TILED>(a, maps, s, units, stream);
+  if (a.compress == JK_SOFTSIGN) return launch_kernel<T, ROWS, DIM, JK_SOFTSIGN, TILED>(a, maps, s, units, stream);
+  return launch_kernel<T, ROWS, DIM, JK_SIGNED_ABS_SOFTMAX, TILED>(a, maps, s, units, stream);
 }
 
 // One launch, for at most kMaxBatch sequences; instantiated for each type in a unit of its own.
 template <typename T>
-int launch(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) {
+int launch(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) {
   if constexpr (std::is_same_v<T, float>) {
-    if (!a.blocks16) {
-      if (s.dim == 128) return launch_one<T, 4, 128, false>(a, s, units, stream);
-      if (s.dim == 256) return launch_one<T, 4, 256, false>(a, s, units, stream);
-      return launch_one<T, 4, 512, false>(a, s, units, stream);
+    if (!a.tiled) {
+      if (s.dim == 128) return launch_one<T, 4, 128, false>(a, maps, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 4, 256, false>(a, maps, s, units, stream);
+      return launch_one<T, 4, 512, false>(a, maps, s, units, stream);
     }
     if (s.rows == 1) {
-      if (s.dim == 128) return launch_one<T, 1, 128>(a, s, units, stream);
-      if (s.dim == 256) return launch_one<T, 1, 256>(a, s, units, stream);
-      return launch_one<T, 1, 512>(a, s, units, stream);
+      if (s.dim == 128) return launch_one<T, 1, 128>(a, maps, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 1, 256>(a, maps, s, units, stream);
+      return launch_one<T, 1, 512>(a, maps, s, units, stream);
     }
     if (s.rows == 4) {
-      if (s.dim == 128) return launch_one<T, 4, 128>(a, s, units, stream);
-      if (s.dim == 256) return launch_one<T, 4, 256>(a, s, units, stream);
-      return launch_one<T, 4, 512>(a, s, units, stream);
+      if (s.dim == 128) return launch_one<T, 4, 128>(a, maps, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 4, 256>(a, maps, s, units, stream);
+      return launch_one<T, 4, 512>(a, maps, s, units, stream);
     }
-    if (s.dim == 128) return launch_one<T, 8, 128>(a, s, units, stream);
-    return launch_one<T, 8, 256>(a, s, units, stream);
+    if (s.dim == 128) return launch_one<T, 8, 128>(a, maps, s, units, stream);
+    return launch_one<T, 8, 256>(a, maps, s, units, stream);
   } else {
-    if (!a.blocks16) {
-      if (s.dim == 64) return launch_one<T, 8, 64, false>(a, s, units, stream);
-      if (s.dim == 128) return launch_one<T, 8, 128, false>(a, s, units, stream);
-      if (s.dim == 256) return launch_one<T, 8, 256, false>(a, s, units, stream);
-      return launch_one<T, 8, 512, false>(a, s, units, stream);
+    if (!a.tiled) {
+      if (s.dim == 64) return launch_one<T, 8, 64, false>(a, maps, s, units, stream);
+      if (s.dim == 128) return launch_one<T, 8, 128, false>(a, maps, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 8, 256, false>(a, maps, s, units, stream);
+      return launch_one<T, 8, 512, false>(a, maps, s, units, stream);
     }
     if (s.dim == 64) {
-      if (s.rows == 8) return launch_one<T, 8, 64>(a, s, units, stream);
-      if (s.rows == 16) return launch_one<T, 16, 64>(a, s, units, stream);
-      return launch_one<T, 32, 64>(a, s, units, stream);
+      if (s.rows == 8) return launch_one<T, 8, 64>(a, maps, s, units, stream);
+      if (s.rows == 16) return launch_one<T, 16, 64>(a, maps, s, units, stream);
+      return launch_one<T, 32, 64>(a, maps, s, units, stream);
     }
     if (s.dim == 128) {
-      if (s.rows == 8) return launch_one<T, 8, 128>(a, s, units, stream);
-      if (s.rows == 16) return launch_one<T, 16, 128>(a, s, units, stream);
-      return launch_one<T, 32, 128>(a, s, units, stream);
+      if (s.rows == 8) return launch_one<T, 8, 128>(a, maps, s, units, stream);
+      if (s.rows == 16) return launch_one<T, 16, 128>(a, maps, s, units, stream);
+      return launch_one<T, 32, 128>(a, maps, s, units, stream);
     }
     if (s.dim == 256) {
-      if (s.rows == 8) return launch_one<T, 8, 256>(a, s, units, stream);
-      return launch_one<T, 16, 256>(a, s, units, stream);
+      if (s.rows == 8) return launch_one<T, 8, 256>(a, maps, s, units, stream);
+      return launch_one<T, 16, 256>(a, maps, s, units, stream);
     }
-    return launch_one<T, 8, 512>(a, s, units, stream);
+    return launch_one<T, 8, 512>(a, maps, s, units, stream);
   }
 }
 
-int launch_f32(const Args& a, const Shape& s, int64_t units, cudaStream_t stream);
-int launch_bf16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream);
-int launch_f16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream);
+int launch_f32(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream);
+int launch_bf16(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream);
+int launch_f16(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream);
 
 }  // namespace cached
 }  // namespace jk

@@ -4,7 +4,7 @@
 namespace jk {
 namespace cached {
 
-int launch_bf16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__nv_bfloat16>(a, s, units, stream); }
+int launch_bf16(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__nv_bfloat16>(a, maps, s, units, stream); }
 
 }  // namespace cached
 

@@ -4,7 +4,7 @@
 namespace jk {
 namespace cached {
 
-int launch_f16(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__half>(a, s, units, stream); }
+int launch_f16(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) { return launch<__half>(a, maps, s, units, stream); }
 
 }  // namespace cached
 

@@ -4,7 +4,7 @@
 namespace jk {
 namespace cached {
 
-int launch_f32(const Args& a, const Shape& s, int64_t units, cudaStream_t stream) { return launch<float>(a, s, units, stream); }
+int launch_f32(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) { return launch<float>(a, maps, s, units, stream); }
 
 }  // namespace cached
 

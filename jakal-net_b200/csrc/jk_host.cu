@@ -67,6 +67,24 @@ int make_tmap_3d_16bit(CUtensorMap* map, const void* base, uint64_t d0, uint64_t
   return r == CUDA_SUCCESS ? JK_OK : JK_ERR_BAD_SHAPE;
 }
 
+int make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], uint32_t box0, uint32_t box1,
+                 int dtype) {
+  auto encode = get_encode_fn();
+  if (encode == nullptr) return JK_ERR_UNSUPPORTED_DEVICE;
+  if (!aligned16(base)) return JK_ERR_ALIGNMENT;
+  cuuint64_t d[4], st[3];
+  for (int i = 0; i < 4; ++i) d[i] = dims[i];
+  for (int i = 0; i < 3; ++i) st[i] = strides[i];
+  cuuint32_t box[4] = {box0, box1, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = dtype == JK_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == JK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = encode(map, type, 4, const_cast<void*>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? JK_OK : JK_ERR_BAD_SHAPE;
+}
+
 }  // namespace jk
 
 extern "C" {

@@ -54,6 +54,11 @@ int launch_status();
 int make_tmap_3d_16bit(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
                        uint32_t box0, uint32_t box1, bool bf16, bool swizzle128 = true);
 
+// Encodes a 4-D tiled tensor map (dtype code JK_F32, JK_BF16 or JK_F16) with a {box0, box1, 1, 1} box, 128-byte
+// swizzled; strides of dims 1..3 in bytes, multiples of 16. Returns JK_OK or an error status.
+int make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], uint32_t box0, uint32_t box1,
+                 int dtype);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Scorer heads of a call: 1 (single low-rank scorer) when h is null, else h checked
