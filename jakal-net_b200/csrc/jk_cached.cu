@@ -115,8 +115,12 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
   a.split = split;
   const int64_t row_bytes = new_nodes * heads * size;
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  for (int64_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
-    a.batch = static_cast<int32_t>(batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch);
+  // sequences of a launch: their tiles are counted in 32 bits
+  const int64_t of_one = kv_heads * s.row_blocks * unit_tiles;
+  if (of_one > (1 << 30)) return JK_ERR_BAD_SHAPE;
+  const int64_t together = (1 << 30) / of_one < kMaxBatch ? (1 << 30) / of_one : kMaxBatch;
+  for (int64_t b0 = 0; b0 < batch; b0 += together) {
+    a.batch = static_cast<int32_t>(batch - b0 < together ? batch - b0 : together);
     a.query = static_cast<const char*>(q->query) + b0 * a.query_stride[0];
     a.table = cache->table == nullptr ? nullptr : cache->table + b0 * a.table_stride;
     a.lengths = cache->lengths + b0;

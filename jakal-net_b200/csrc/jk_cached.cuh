@@ -203,15 +203,22 @@ __device__ __forceinline__ float weight_of(float s, float mass) {
 // 128 r + 16 (c ^ (r mod 8)): eight rows' blocks c are in different banks. (Tiled copies write it so.)
 __device__ __forceinline__ int block_at(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
 
+// (as many lanes a row as have 128 bytes of it, so that a lane keeps its place in a column)
 template <int BYTES>
 __device__ __forceinline__ void load_pieces(uint32_t to, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
+  constexpr int kLanes = 128 / BYTES, kStep = 32 / kLanes;
+  const int byte = lane % kLanes * BYTES;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {  // 8 lanes a row
-    const int row = 4 * q + (lane >> 3);
-    const char* from = src + __shfl_sync(0xffffffffu, offset, row);
+  for (int row0 = 0; row0 < kKeys; row0 += kStep) {
+    const int row = row0 + lane / kLanes;
+    const char* from = src + __shfl_sync(0xffffffffu, offset, row) + byte;
+    uint32_t dst = to + block_at(row, byte >> 4) + (byte & 15);
     const bool ok = (there >> row) & 1;
-    for (int c = (lane & 7) * BYTES; c < row_bytes; c += 8 * BYTES)
-      copy_async<BYTES>(to + (c >> 7) * kColumn + block_at(row, (c >> 4) & 7) + (c & 15), from + c, ok);
+    for (int c = byte; c < row_bytes; c += 128) {
+      copy_async<BYTES>(dst, from, ok);
+      dst += kColumn;
+      from += 128;
+    }
   }
 }
 
@@ -269,8 +276,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   constexpr int SIZE = sizeof(T);
   constexpr int COLUMN = 128 / SIZE;                   // elements of a 128-byte column
   extern __shared__ char memory_[];
-  __shared__ int64_t before[kMaxBatch + 1];
-  __shared__ int64_t scan[kWarps];
+  __shared__ int32_t before[kMaxBatch + 1];
+  __shared__ int32_t scan[kWarps];
   __shared__ float ref_s[kWarps][ROWS], sum_s[kWarps][ROWS], state_s[kWarps][ROWS];
   __shared__ uint64_t landed[kWarps][kMaxStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -284,23 +291,23 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   }
   __syncwarp();
 
-  int64_t chunk = 1, at = 0, until = 1;
+  int32_t chunk = 1, at = 0, until = 1;  // (the host sees to it that all tiles are fewer than 2^30)
   if (a.split) {
     // tiles before each sequence
-    int64_t carry = 0;
+    int32_t carry = 0;
     if (tid == 0) before[0] = 0;
     for (int32_t base = 0; base < a.batch; base += kThreads) {
       const int32_t b = base + tid;
-      int64_t v = b < a.batch ? int64_t(tiles_of(span_of<TILED>(a, b))) * a.kv_heads * a.row_blocks : 0;
+      int32_t v = b < a.batch ? tiles_of(span_of<TILED>(a, b)) * (a.kv_heads * a.row_blocks) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+        const int32_t up = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += up;
       }
       __syncthreads();
       if (lane == 31) scan[warp] = v;
       __syncthreads();
-      int64_t add = carry;
+      int32_t add = carry;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w < warp) add += scan[w];
@@ -311,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     __syncthreads();
     grid_dependency_launch();
     chunk = (carry + a.blocks - 1) / a.blocks;
-    at = chunk * blockIdx.x < carry ? chunk * blockIdx.x : carry;
+    at = chunk * int32_t(blockIdx.x) < carry ? chunk * int32_t(blockIdx.x) : carry;
     until = at + chunk < carry ? at + chunk : carry;
   }
 
@@ -327,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   while (at < until) {
     // ---- the unit and the run of its tiles
     int32_t b, inner, tile = 0, tiles, unit_tiles;
-    int64_t unit_begin = 0;
+    int32_t unit_begin = 0;
     if (a.split) {
       int32_t low = 0, high = a.batch - 1;
       while (low < high) {  // the sequence that tile `at` is of: the first that ends after it
@@ -342,12 +349,11 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     const Span span = span_of<TILED>(a, b);
     unit_tiles = tiles_of(span);
     if (a.split) {
-      const int64_t in = at - before[b];
-      inner = static_cast<int32_t>(in / unit_tiles);
-      tile = static_cast<int32_t>(in - int64_t(inner) * unit_tiles);
+      const uint32_t in = at - before[b];
+      inner = in / static_cast<uint32_t>(unit_tiles);
+      tile = in - inner * unit_tiles;
       unit_begin = at - tile;
-      const int64_t left = until - at;
-      tiles = unit_tiles - tile < left ? unit_tiles - tile : static_cast<int32_t>(left);
+      tiles = unit_tiles - tile < until - at ? unit_tiles - tile : until - at;
     } else {
       inner = blockIdx.x - b * (a.kv_heads * a.row_blocks);
       tiles = unit_tiles;
@@ -369,28 +375,34 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     const char* states = a.states == nullptr ? nullptr : a.states + kv * a.state_stride[1];
     const int32_t* table = a.table + b * a.table_stride;
     const int32_t key0 = span.base + tile * kTile + warp * kKeys;
-    // page and offset of a place, turn after turn: of the turn's first where one page has them all, else of this lane's
-    const int own_place = lane & 15, looked_up = TILED ? 0 : own_place;
-    uint32_t column = static_cast<uint32_t>(key0 + looked_up) / a.page_size, offset = static_cast<uint32_t>(key0 + looked_up) - column * a.page_size;
-    const uint32_t column_step = kTile / a.page_size, offset_step = kTile - column_step * a.page_size;
+    const int own_place = lane & 15;
     struct Place {
       int32_t page;  // -1: none
       uint32_t offset;
     };
-    auto next_place = [&](int32_t i) {
-      Place p{-1, offset};
-      // (64 bits: the turn after the last may lie past 2^31)
-      if (i < tiles && int64_t(key0) + int64_t(i) * kTile + looked_up < span.end) {
+    auto page_of = [&](int64_t j, Place& p) {  // of place j (64 bits: turns after the last may lie past 2^31)
+      p.page = -1;
+      if (j < span.end) {
+        const uint32_t column = static_cast<uint32_t>(j) / a.page_size;
+        p.offset = static_cast<uint32_t>(j) - column * a.page_size;
         const int32_t page = table[column];
         if (static_cast<uint32_t>(page) < static_cast<uint64_t>(a.pages)) p.page = page;
       }
-      column += column_step;
-      offset += offset_step;
-      if (offset >= a.page_size) offset -= a.page_size, ++column;
-      return p;
     };
-    auto issue = [&](int32_t i, Place p) {
+    // TILED: lane l has turn l's of the 32 turns at hand, looked up together; else a lane has that of its place of the next turn
+    Place looked_up{-1, 0};
+    if (TILED) page_of(int64_t(key0) + lane * kTile, looked_up);
+    else page_of(int64_t(key0) + own_place, looked_up);
+    auto issue = [&](int32_t i) {
       Turn made{0, 0.0f};
+      Place p = looked_up;
+      if (TILED) {
+        p.page = __shfl_sync(0xffffffffu, looked_up.page, i & 31);
+        p.offset = __shfl_sync(0xffffffffu, looked_up.offset, i & 31);
+        if ((i & 31) == 31) page_of(int64_t(key0) + (int64_t(i) + 1 + lane) * kTile, looked_up);
+      } else {
+        page_of(int64_t(key0) + (int64_t(i) + 1) * kTile + own_place, looked_up);
+      }
       if (i < tiles && !late) {
         if (TILED) {
           const int32_t k0 = key0 + i * kTile;
@@ -422,34 +434,6 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       return made;
     };
     const int lead = TILED && a.stages == kMaxStages ? 2 : a.stages > 1 ? 1 : 0;  // turns on their way while one is worked on
-    Place todo = next_place(0);
-    Turn first{0, 0.0f}, second{0, 0.0f};
-    if (lead) {
-      const Place after = next_place(1);
-      first = issue(0, todo);
-      todo = after;
-    }
-    if (lead == 2) {
-      const Place after = next_place(2);
-      second = issue(1, todo);
-      todo = after;
-    }
-
-    // ---- queries, and the keys' columns that no copy fills: 0
-    for (int r = warp; r < ROWS; r += kWarps) {
-      const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
-      const bool counts = r < rows && t < span.n;
-      const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
-      for (int c = lane; c < a.key_cols; c += 32) query[r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
-    }
-    if (!TILED && a.key_cols > a.rank) {
-      for (int i = lane; i < a.stages * kKeys; i += 32) {
-        char* k = ring + i / kKeys * a.stage_bytes;
-        for (int c = a.rank; c < a.key_cols; ++c)
-          *reinterpret_cast<T*>(k + c / COLUMN * kColumn + block_at(i % kKeys, c % COLUMN * SIZE / 16) + c * SIZE % 16) = from_f32<T>(0.0f);
-      }
-    }
-
     // ---- this thread's rows: the places they see, [row_low, row_end)
     const int own_row = kWide && ROWS > 1 && lane >= 16 ? OWN : 0;
     int32_t row_low[OWN], row_end[OWN];
@@ -478,16 +462,31 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     for (int i = 0; i < (kWide ? ROWS : 1); ++i)
 #pragma unroll
       for (int j = 0; j < CP; ++j) pairs[i][j] = 0;
-    __syncthreads();
-
-    for (int32_t i = 0; i < tiles; ++i) {
+    Turn first{0, 0.0f}, second{0, 0.0f};
+    for (int32_t i = -lead; i < tiles; ++i) {
       __syncwarp();  // the stage to fill has been read by all lanes
-      const Place after = next_place(i + lead + 1);
-      const Turn made = issue(i + lead, todo);
+      const Turn made = issue(i + lead);
       const Turn now = lead ? first : made;
       first = lead == 2 ? second : made;
       second = made;
-      todo = after;
+      if (i < 0) continue;
+      if (i == 0) {
+        // ---- queries, and the keys' columns that no copy fills: 0
+        for (int r = warp; r < ROWS; r += kWarps) {
+          const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
+          const bool counts = r < rows && t < span.n;
+          const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
+          for (int c = lane; c < a.key_cols; c += 32) query[r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
+        }
+        if (!TILED && a.key_cols > a.rank) {
+          for (int i = lane; i < a.stages * kKeys; i += 32) {
+            char* k = ring + i / kKeys * a.stage_bytes;
+            for (int c = a.rank; c < a.key_cols; ++c)
+              *reinterpret_cast<T*>(k + c / COLUMN * kColumn + block_at(i % kKeys, c % COLUMN * SIZE / 16) + c * SIZE % 16) = from_f32<T>(0.0f);
+          }
+        }
+        __syncthreads();
+      }
       const uint32_t there = now.there;
       if (!TILED) copy_wait(lead);
       if (there == 0) continue;
@@ -822,10 +821,12 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     const bool whole = tiles == unit_tiles;
     float* part = nullptr;
     if (!whole) {
-      const int slot = unit_begin < chunk * blockIdx.x ? 0 : 1;  // a unit that began before this block's run, or one that goes on after it
+      const int slot = unit_begin < chunk * int32_t(blockIdx.x) ? 0 : 1;  // a unit that began before this block's run, or one that goes on after it
       part = a.parts + (int64_t(blockIdx.x) * 2 + slot) * ROWS * a.part_row;
     }
-    for (int r = warp; r < rows; r += kWarps) {
+    // a warp a row, or where there are few rows all warps
+    const int step = rows < kWarps ? kThreads : 32, lane_of = rows < kWarps ? tid : lane;
+    for (int r = rows < kWarps ? 0 : warp; r < rows; r += rows < kWarps ? 1 : kWarps) {
       float top = ref_s[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ref_s[w][r]);
@@ -841,14 +842,14 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
       const int64_t row = (int64_t(b) * a.new_nodes + t) * a.heads + kv * a.group + g;
       const bool zero = whole && (t >= span.n || (top == -INFINITY && norm == 0.0f));
-      for (int d = lane; d < a.dim; d += 32) {
+      for (int d = lane_of; d < a.dim; d += step) {
         float x = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) x = fmaf(f[w], joined[(w * ROWS + r) * kJoinRow + d], x);
         if (whole) reinterpret_cast<T*>(a.out_value)[row * a.dim + d] = from_f32<T>(zero ? 0.0f : x * norm);
         else part[r * a.part_row + d] = x;
       }
-      if (lane == 0) {
+      if (lane_of == 0) {
         if (!whole) {
           float* words = part + r * a.part_row + a.part_row - 4;
           words[0] = top, words[1] = all, words[2] = st;
@@ -867,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 // Joins the parts of a unit's row that several blocks left, 128 columns a block; a unit without tiles has zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
-  __shared__ int64_t counted[8][2];
+  __shared__ int32_t counted[8][2];
   __shared__ float words_s[8][3];
   __shared__ __align__(16) float columns[8][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -882,9 +883,9 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   // the blocks' runs, as the first kernel has them (while it runs)
   const Span span = span_as(a, b);
   const int32_t tiles = tiles_of(span);
-  int64_t mine = 0, all_tiles = 0;
+  int32_t mine = 0, all_tiles = 0;
   for (int32_t i = tid; i < a.batch; i += 256) {
-    const int64_t n = int64_t(tiles_of(span_as(a, i))) * a.kv_heads * a.row_blocks;
+    const int32_t n = tiles_of(span_as(a, i)) * (a.kv_heads * a.row_blocks);
     all_tiles += n;
     if (i < b) mine += n;
   }
@@ -906,10 +907,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     grid_dependency_wait();
     return;
   }
-  const int64_t chunk = (all_tiles + a.blocks - 1) / a.blocks;
+  const int32_t chunk = (all_tiles + a.blocks - 1) / a.blocks;
   const int32_t row_block = row_of / a.rows, r = row_of - row_block * a.rows;
-  const int64_t begin = mine + (int64_t(kv) * a.row_blocks + row_block) * tiles;
-  const int32_t first = static_cast<int32_t>(begin / chunk), last = static_cast<int32_t>((begin + tiles - 1) / chunk);
+  const int32_t begin = mine + (kv * a.row_blocks + row_block) * tiles;
+  const int32_t first = begin / chunk, last = (begin + tiles - 1) / chunk;
   grid_dependency_wait();
   if (first == last) return;  // one block had all of it
   // a warp has every eighth part, a lane four columns
@@ -981,8 +982,8 @@ inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, b
   const int size = wide ? 4 : 2, column = 128 / size;
   s.dim = dim <= 64 && !wide ? 64 : dim <= 128 ? 128 : dim <= 256 ? 256 : 512;
   // 128 registers of sums a thread at most (f32: 64, as it keeps a tile's values too); where rows are copied in pieces the
-  // copies are what takes time, so blocks have one size
-  if (wide) s.rows = !tiled ? 4 : unit_rows == 1 ? 1 : unit_rows <= 4 || s.dim == 512 ? 4 : 8;
+  // copies are what takes time, so blocks have fewer sizes
+  if (wide) s.rows = unit_rows == 1 ? 1 : (tiled && unit_rows <= 4) || s.dim == 512 ? 4 : 8;
   else s.rows = !tiled || unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
   s.row_blocks = static_cast<int>((unit_rows + s.rows - 1) / s.rows);
   // columns in the products' steps (two of 16, or two halves of 4); queries an odd number of 16-byte blocks apart, so that
@@ -1035,8 +1036,13 @@ template <typename T>
 int launch(const Args& a, const Maps& maps, const Shape& s, int64_t units, cudaStream_t stream) {
   if constexpr (std::is_same_v<T, float>) {
     if (!a.tiled) {
-      if (s.dim == 128) return launch_one<T, 4, 128, false>(a, maps, s, units, stream);
-      if (s.dim == 256) return launch_one<T, 4, 256, false>(a, maps, s, units, stream);
+      if (s.rows == 1) {
+        if (s.dim == 128) return launch_one<T, 1, 128, false>(a, maps, s, units, stream);
+        if (s.dim == 256) return launch_one<T, 1, 256, false>(a, maps, s, units, stream);
+        return launch_one<T, 1, 512, false>(a, maps, s, units, stream);
+      }
+      if (s.dim == 128) return launch_one<T, 8, 128, false>(a, maps, s, units, stream);
+      if (s.dim == 256) return launch_one<T, 8, 256, false>(a, maps, s, units, stream);
       return launch_one<T, 4, 512, false>(a, maps, s, units, stream);
     }
     if (s.rows == 1) {
