@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   char* const ring = memory + warp * a.stages * a.stage_bytes;
   float* const joined = reinterpret_cast<float*>(memory);  // [kWarps][ROWS][DIM + 4], once the rings are drained
   T* const query = reinterpret_cast<T*>(memory + a.ring_bytes);
-  constexpr int kWeightRow = kWide ? kKeys : kKeys + 1;
+  constexpr int kWeightRow = kWide ? 2 * kKeys : kKeys + 1;  // f32: each weight twice, as its product is with two columns
   float* const weights = reinterpret_cast<float*>(memory + a.ring_bytes + ROWS * a.query_row * SIZE) + warp * (ROWS * kWeightRow);
 
   while (at < until) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     const int32_t key0 = span.base + tile * kTile + warp * kKeys;
     const int own_place = lane & 15;
     struct Place {
-      int32_t page;  // -1: none
+      int32_t page;  // what the table says, -1: past the end
       uint32_t offset;
     };
     auto page_of = [&](int64_t j, Place& p) {  // of place j (64 bits: turns after the last may lie past 2^31)
@@ -385,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       if (j < span.end) {
         const uint32_t column = static_cast<uint32_t>(j) / a.page_size;
         p.offset = static_cast<uint32_t>(j) - column * a.page_size;
-        const int32_t page = table[column];
-        if (static_cast<uint32_t>(page) < static_cast<uint64_t>(a.pages)) p.page = page;
+        p.page = table[column];
       }
     };
     // TILED: lane l has turn l's of the 32 turns at hand, looked up together; else a lane has that of its place of the next turn
@@ -403,11 +402,12 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       } else {
         page_of(int64_t(key0) + (int64_t(i) + 1) * kTile + own_place, looked_up);
       }
+      const bool there = static_cast<uint32_t>(p.page) < static_cast<uint64_t>(a.pages);
       if (i < tiles && !late) {
         if (TILED) {
           const int32_t k0 = key0 + i * kTile;
           const int low = span.low - k0, high = span.end - k0;  // places of this turn that count: [low, high), low < 16
-          if (p.page >= 0 && high > 0) {
+          if (there && high > 0) {
             made.there = (high >= kKeys ? 0xffffu : (1u << high) - 1) & (low <= 0 ? 0xffffu : 0xffffu << low);
             if (lane == 0) {
               char* stage = ring + fill * a.stage_bytes;
@@ -421,9 +421,9 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           }
           p.offset += own_place;
         } else {
-          made.there = __ballot_sync(0xffffffffu, p.page >= 0) & 0xffffu;
+          made.there = __ballot_sync(0xffffffffu, there) & 0xffffu;
           char* stage = ring + (a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
-          const int64_t page = p.page >= 0 ? p.page : 0, off = p.page >= 0 ? p.offset : 0;
+          const int64_t page = there ? p.page : 0, off = there ? p.offset : 0;
           load_rows<T>(stage, keys, page * a.key_stride[0] + off * a.key_stride[2], made.there, a.rank * SIZE, a.key_piece, lane);
           load_rows<T>(stage + a.key_bytes, values, page * a.value_stride[0] + off * a.value_stride[2], made.there, a.dim * SIZE, a.value_piece, lane);
         }
@@ -731,40 +731,43 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
           w = sees[i2] ? weight_of<COMPRESS>(score[i2], w) : 0.0f;
           if (states != nullptr && sees[i2]) state[i2] = fmaf(w, now.state, state[i2]);
-          weights[(own_row + i2) * kWeightRow + place] = w;
+          *reinterpret_cast<float2*>(weights + (own_row + i2) * kWeightRow + 2 * place) = make_float2(w, w);
         }
         __syncwarp();
         // a lane's columns 2 lane and 2 lane + 1 of every 64
         const char* v = stage_values + (lane >> 4) * kColumn + (lane & 1) * 8;
         const int block = (lane & 15) >> 1;
-        constexpr int AT_ONCE = DIM == 512 ? 2 : 4;  // places whose values are in registers together
+        if (!mixed) {
+          constexpr int AT_ONCE = DIM == 512 ? 2 : 4;  // places whose values are in registers together
 #pragma unroll 1
-        for (int k4 = 0; k4 < kKeys; k4 += AT_ONCE) {
-          uint64_t x[AT_ONCE][CP];
+          for (int k4 = 0; k4 < kKeys; k4 += AT_ONCE) {
+            uint64_t x[AT_ONCE][CP];
 #pragma unroll
-          for (int k1 = 0; k1 < AT_ONCE; ++k1)
+            for (int k1 = 0; k1 < AT_ONCE; ++k1)
 #pragma unroll
-            for (int y = 0; y < CP; ++y) x[k1][y] = *reinterpret_cast<const uint64_t*>(v + 2 * y * kColumn + block_at(k4 + k1, block));
+              for (int y = 0; y < CP; ++y) x[k1][y] = *reinterpret_cast<const uint64_t*>(v + 2 * y * kColumn + block_at(k4 + k1, block));
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            float w[AT_ONCE];
-            if constexpr (AT_ONCE == 4) {
-              const float4 w4 = *reinterpret_cast<const float4*>(weights + r * kWeightRow + k4);
-              w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
-            } else {
-              const float2 w2 = *reinterpret_cast<const float2*>(weights + r * kWeightRow + k4);
-              w[0] = w2.x, w[1] = w2.y;
-            }
-            int from = 0, to = kKeys;
-            if (mixed) {
-              from = __shfl_sync(0xffffffffu, row_low[r % OWN], r < OWN ? 0 : 16) - k0;
-              to = __shfl_sync(0xffffffffu, row_end[r % OWN], r < OWN ? 0 : 16) - k0;
-            }
+            for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-            for (int k1 = 0; k1 < AT_ONCE; ++k1) {
-              if (k4 + k1 >= from && k4 + k1 < to) {
+              for (int k1 = 0; k1 < AT_ONCE; k1 += 2) {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(weights + r * kWeightRow + 2 * (k4 + k1));
 #pragma unroll
-                for (int y = 0; y < CP; ++y) pairs[r][y] = fma2(x[k1][y], pair(w[k1], w[k1]), pairs[r][y]);
+                for (int y = 0; y < CP; ++y) pairs[r][y] = fma2(x[k1 + 1][y], w.y, fma2(x[k1][y], w.x, pairs[r][y]));
+              }
+          }
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < kKeys; ++k) {
+            uint64_t x[CP];
+#pragma unroll
+            for (int y = 0; y < CP; ++y) x[y] = *reinterpret_cast<const uint64_t*>(v + 2 * y * kColumn + block_at(k, block));
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+              const int from = __shfl_sync(0xffffffffu, row_low[r % OWN], r < OWN ? 0 : 16), to = __shfl_sync(0xffffffffu, row_end[r % OWN], r < OWN ? 0 : 16);
+              if (k0 + k >= from && k0 + k < to) {
+                const uint64_t w = *reinterpret_cast<const uint64_t*>(weights + r * kWeightRow + 2 * k);
+#pragma unroll
+                for (int y = 0; y < CP; ++y) pairs[r][y] = fma2(x[y], w, pairs[r][y]);
               }
             }
           }
@@ -999,7 +1002,7 @@ inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, b
     const int bytes = kWarps * stages * s.stage_bytes + past;
     return bytes > join ? bytes : join;
   };
-  const int rest = s.rows * s.query_row * size + kWarps * s.rows * (wide ? kKeys : kKeys + 1) * 4;
+  const int rest = s.rows * s.query_row * size + kWarps * s.rows * (wide ? 2 * kKeys : kKeys + 1) * 4;
   auto blocks = [&](int stages) { return static_cast<int>(227 * 1024 / (1024 + ring(stages) + rest + 4 * 1024)); };
   const int most = s.rows * s.dim <= 1024 ? kMaxPerSm : 2;
   // Two stages a warp in as many blocks of an SM as fit, a third where that costs none; where not even one block has room for
