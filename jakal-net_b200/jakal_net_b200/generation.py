@@ -32,7 +32,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .training import _call, _check_input, _empty, _ptr, _written
+from .training import _DTYPE_CODE, _call, _check_input, _empty, _ptr, _written
 
 __all__ = [
     "cached_propagation",
@@ -110,11 +110,11 @@ def _at(words: array.array) -> int:
     return words.buffer_info()[0]
 
 
-def _no_grad(**tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} requires grad: the generation-step operators have no backward pass (use torch.no_grad())")
+def _no_grad(*tensors: tuple) -> None:
+    """Refuses (name, tensor) pairs that ask for a gradient (where gradients are recorded)."""
+    for name, t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{name} requires grad: the generation-step operators have no backward pass (use torch.no_grad())")
 
 
 def _one_block(shape, strides) -> bool:
@@ -132,33 +132,44 @@ class _Pools:
 
     def __init__(self, pools: Union[Tensor, Sequence[Tensor]], pages: int, device: int):
         tensors = [pools] if isinstance(pools, Tensor) else list(pools)
+        # one look at all of them (a model has dozens); which one is wrong is sought only if one is
+        try:
+            plain = (pages > 0 and set(map(Tensor.get_device, tensors)) <= {device} and all(map(Tensor.is_contiguous, tensors))
+                     and all([t.dim() and t.size(0) == pages for t in tensors]))
+        except TypeError:  # not a tensor
+            plain = False
+        if plain:
+            data = list(map(Tensor.data_ptr, tensors))
+            sizes = strides = [t.numel() // pages * t.element_size() for t in tensors]
+        else:
+            data, sizes, strides = self._others(tensors, pages, device)
+        if len(set(data)) != len(data) and any(t.numel() for t in tensors):
+            raise ValueError("a pool is given twice")
+        n = len(data)
+        self.tensors, self.arrays = tensors, array.array("q", data + sizes + strides)
+        at = _at(self.arrays)
+        self.words = array.array("q", (at, at + 8 * n, at + 16 * n, n))
+
+    @staticmethod
+    def _others(tensors, pages: int, device: int):
         data, sizes, strides = [], [], []
         for i, p in enumerate(tensors):
             if not isinstance(p, Tensor):
                 raise TypeError(f"pool {i} must be a tensor")
             if p.get_device() != device:
                 raise RuntimeError(f"pool {i} is on {p.device}, expected cuda:{device}")
-            shape, size = p.shape, p.element_size()
+            shape, stride = p.shape, p.stride()
             if not shape or shape[0] != pages:
                 raise ValueError(f"pool {i} has shape {tuple(shape)}, expected {pages} pages in its first dim")
-            if p.is_contiguous():
-                block = step = p.numel() // pages if pages else 0
-            else:
-                stride, block = p.stride(), 1
-                for n in shape[1:]:
-                    block *= n
-                if not _one_block(shape[1:], stride[1:]) or (pages > 1 and stride[0] < block):
-                    raise ValueError(f"pool {i}: a page must be one block of memory, apart from the other pages")
-                step = max(stride[0], block)
+            block = 1
+            for n in shape[1:]:
+                block *= n
+            if not (p.is_contiguous() or _one_block(shape[1:], stride[1:])) or (pages > 1 and stride[0] < block):
+                raise ValueError(f"pool {i}: a page must be one block of memory, apart from the other pages")
             data.append(p.data_ptr())
-            sizes.append(block * size)
-            strides.append(step * size)
-        if len(set(data)) != len(data) and any(p.numel() for p in tensors):
-            raise ValueError("a pool is given twice")
-        n = len(data)
-        self.tensors, self.arrays = tensors, array.array("q", data + sizes + strides)
-        at = _at(self.arrays)
-        self.words = array.array("q", (at, at + 8 * n, at + 16 * n, n))
+            sizes.append(block * p.element_size())
+            strides.append(max(stride[0], block) * p.element_size())
+        return data, sizes, strides
 
     def pointer(self) -> int:
         return _at(self.words)
@@ -173,16 +184,15 @@ def _page_size(page_size: int) -> int:
 
 # ----------------------------------------------------------------------------- propagation
 def _cache_pages(name: str, t: Tensor, query: Tensor, dims: int) -> None:
+    if isinstance(t, Tensor) and t.dtype is query.dtype and t.get_device() == query.get_device() and t.dim() == dims:
+        return
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.get_device() != query.get_device():
         raise RuntimeError(f"{name} is on {t.device}, expected {query.device}")
     if t.dtype is not query.dtype:
         raise RuntimeError(f"{name} has dtype {t.dtype}, expected {query.dtype}")
-    if t.dim() != dims:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {dims} dims")
-    if dims == 4 and t.shape[3] > 1 and t.stride(3) != 1:
-        raise ValueError(f"{name} must be contiguous in its last dim")
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {dims} dims")
 
 
 def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, table: Tensor, lengths: Tensor,
@@ -206,15 +216,19 @@ def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, ta
     Returns value [batch, new, heads, dim], or (state [batch, new, heads], value), in query's dtype.
     Nodes that see nothing (an empty sequence, pages that are missing) and rows past counts are zeros.
     Places that are not seen have no part in a result, whatever they hold. rank <= 256, dim <= 512, new <= 64."""
-    code = _check_input("query", query)
-    if query.dim() != 4:
-        raise ValueError(f"query has shape {tuple(query.shape)}, expected [batch, new, heads, rank]")
+    code = _DTYPE_CODE.get(query.dtype) if isinstance(query, Tensor) and query.is_cuda else None
+    if code is None:
+        _check_input("query", query)
     kind = _COMPRESS.get(compress)
     if kind is None:
         raise ValueError(f"unknown compress {compress!r} (softmax, softsign or signed_abs_softmax)")
+    dtype = query.dtype
+    if query.dim() != 4:
+        raise ValueError(f"query has shape {tuple(query.shape)}, expected [batch, new, heads, rank]")
     _cache_pages("key_pages", key_pages, query, 4)
     _cache_pages("value_pages", value_pages, query, 4)
-    _no_grad(query=query, key_pages=key_pages, value_pages=value_pages, state_pages=state_pages)
+    if torch.is_grad_enabled():
+        _no_grad(("query", query), ("key_pages", key_pages), ("value_pages", value_pages), ("state_pages", state_pages))
     batch, new, heads, rank = query.shape
     pages, kv_heads, page_size, dim = value_pages.shape
     if key_pages.shape != (pages, kv_heads, page_size, rank):
@@ -224,6 +238,9 @@ def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, ta
     if page_size < 1 or not 1 <= rank <= 256 or not 1 <= dim <= 512 or new > 64:
         raise ValueError(f"page_size {page_size}, rank {rank}, dim {dim} or {new} new nodes outside the supported range "
                          "(rank <= 256, dim <= 512, new <= 64)")
+    key_strides, value_strides, query_strides = key_pages.stride(), value_pages.stride(), query.stride()
+    if (rank > 1 and key_strides[3] != 1) or (dim > 1 and value_strides[3] != 1):
+        raise ValueError("key_pages and value_pages must be contiguous in their last dim")
     device, rows, columns, table_stride = _table(table)
     if rows != batch or device != query.get_device():
         raise ValueError(f"table has {rows} rows on {table.device}, expected {batch} on {query.device}")
@@ -241,16 +258,14 @@ def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, ta
         _cache_pages("state_pages", state_pages, query, 3)
         if state_pages.shape != (pages, kv_heads, page_size):
             raise ValueError(f"state_pages has shape {tuple(state_pages.shape)}, expected {(pages, kv_heads, page_size)}")
-        state = query.new_empty((batch, new, heads))
+        state = torch.empty_strided((batch, new, heads), (new * heads, heads, 1), dtype=dtype, device=query.device)
         state_at, state_strides, out_state = state_pages.data_ptr(), state_pages.stride(), state.data_ptr()
-    query_strides = query.stride()
     if rank > 1 and query_strides[3] != 1:
         query = query.contiguous()
         query_strides = query.stride()
-    value = query.new_empty((batch, new, heads, dim))
+    value = torch.empty_strided((batch, new, heads, dim), (new * heads * dim, heads * dim, dim, 1), dtype=dtype, device=query.device)
     size = _propagation_workspace(batch, new, heads, kv_heads, rank, dim, page_size, columns, window, code)
     work = _empty((size // 4,), torch.float32, query.device) if size else None
-    key_strides, value_strides = key_pages.stride(), value_pages.stride()
     cache = _cache(table, table_stride, lengths, None, batch, columns, pages, page_size)
     nodes = array.array("q", (
         query.data_ptr(), *query_strides[:3], key_pages.data_ptr(), *key_strides[:3], value_pages.data_ptr(), *value_strides[:3], state_at,
@@ -303,6 +318,7 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
         _ints("counts", counts, (batch,), device)
     if len(pages) != len(rows) or not pages:
         raise ValueError(f"{len(rows)} tensors of rows for {len(pages)} of pages")
+    recording = torch.is_grad_enabled()
     count = new = heads = page_size = None
     at, from_, page_strides, row_strides, widths, sizes = [], [], [], [], [], []
     kept = []  # copies of rows, until the launch
@@ -313,23 +329,31 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
             raise RuntimeError(f"pages {i} and rows {i} are on {p.device} and {r.device}, expected cuda:{device}")
         if p.dtype is not r.dtype:
             raise RuntimeError(f"rows {i} has dtype {r.dtype}, expected {p.dtype}")
-        shape, dims = p.shape, p.dim()
-        if dims not in (3, 4) or r.dim() != dims:
-            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(shape)} and {tuple(r.shape)}")
+        if recording:
+            _no_grad(("pages", p), ("rows", r))
+        shape, row_shape, page_stride, row_stride = p.shape, r.shape, p.stride(), r.stride()
+        dims = len(shape)
+        if dims == 4 and len(row_shape) == 4:
+            n_pages, n_heads, n_places, width = shape
+            n_batch, n_new, r_heads, r_width = row_shape
+        elif dims == 3 and len(row_shape) == 3:
+            n_pages, n_heads, n_places = shape
+            n_batch, n_new, r_heads = row_shape
+            width = r_width = 1
+        else:
+            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(shape)} and {tuple(row_shape)}")
         if i == 0:
-            (count, heads, page_size), new = shape[:3], r.shape[1]
-        if shape[:3] != (count, heads, page_size) or r.shape != (batch, new, heads, *shape[3:]):
-            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(shape)} and {tuple(r.shape)}, which do not fit "
+            count, heads, page_size, new = n_pages, n_heads, n_places, n_new
+        if (n_pages != count or n_heads != heads or n_places != page_size or n_batch != batch or n_new != new or r_heads != heads
+                or r_width != width):
+            raise ValueError(f"pages {i} and rows {i} have shapes {tuple(shape)} and {tuple(row_shape)}, which do not fit "
                              f"{batch} sequences, {new} nodes, {heads} heads and {count} pages of {page_size}")
-        _no_grad(pages=p, rows=r)
-        width = shape[3] if dims == 4 else 1
-        page_stride, row_stride = p.stride(), r.stride()
         if not p.is_contiguous():
-            if dims == 4 and width > 1 and page_stride[3] != 1:
+            if width > 1 and page_stride[3] != 1:
                 raise ValueError(f"pages {i} must be contiguous in their last dim")
             if not _one_block(shape[1:], page_stride[1:]) or (count > 1 and page_stride[0] < heads * page_size * width):
                 raise ValueError(f"pages {i}: a page must be one block of memory, apart from the other pages")
-        if dims == 4 and width > 1 and row_stride[3] != 1:
+        if width > 1 and row_stride[3] != 1:
             r = r.contiguous()
             kept.append(r)
             row_stride = r.stride()
@@ -456,17 +480,20 @@ def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, unifor
 
     Returns (out int64 [batch, drafted + 1]: the accepted tokens, the new one, -1 behind it (and in its
     place where there is nothing to draw from); accepted int32 [batch]: a)."""
-    code = _check_input("target", target)
+    code = _DTYPE_CODE.get(target.dtype) if isinstance(target, Tensor) and target.is_cuda else None
+    if code is None:
+        _check_input("target", target)
     if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
         raise ValueError(f"target has shape {tuple(target.shape)}, expected [batch, drafted + 1, vocab]")
-    batch, drafted, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    batch, drafted, vocab = target.shape
+    drafted -= 1
     device = target.get_device()
     if draft is not None:
         if not isinstance(draft, Tensor):
             raise TypeError("draft must be a tensor")
         if draft.get_device() != device:
             raise RuntimeError(f"draft is on {draft.device}, expected {target.device}")
-        if draft.dtype != target.dtype:
+        if draft.dtype is not target.dtype:
             raise RuntimeError(f"draft has dtype {draft.dtype}, expected {target.dtype}")
         if draft.shape != (batch, drafted, vocab):
             raise ValueError(f"draft has shape {tuple(draft.shape)}, expected {(batch, drafted, vocab)}")
@@ -482,7 +509,7 @@ def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, unifor
         tokens = tokens.to(torch.int64).contiguous()
     if not uniform.is_contiguous():
         uniform = uniform.detach().contiguous()
-    out = tokens.new_empty((batch, drafted + 1))
+    out = torch.empty_strided((batch, drafted + 1), (drafted + 1, 1), dtype=torch.int64, device=target.device)
     accepted = _empty((batch,), _INT32, target.device)
     words = array.array("q", (
         target.data_ptr(), *target.stride()[:2], *((0, 0, 0) if draft is None else (draft.data_ptr(), *draft.stride()[:2])), tokens.data_ptr(),

@@ -160,10 +160,8 @@ def test_inputs_that_ask_for_gradients_are_refused():
 
     x = torch.ones(2, requires_grad=True)
     with pytest.raises(RuntimeError, match="backward"):
-        generation._no_grad(query=x)
-    generation._no_grad(query=x.detach(), states=None)
-    with torch.no_grad():
-        generation._no_grad(query=x)
+        generation._no_grad(("states", None), ("query", x))
+    generation._no_grad(("query", x.detach()), ("states", None))
     assert generation._one_block((3, 4), (4, 1)) and generation._one_block((3, 4), (1, 3)) and generation._one_block((), ())
     assert not generation._one_block((3, 4), (5, 1)) and not generation._one_block((3, 4), (0, 1))
 
