@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
   char* to = w.pages[i] + page * w.page_stride[i][0] + h * w.page_stride[i][1] + off * w.page_stride[i][2];
   const char* from = w.rows[i] + b * w.row_stride[i][0] + t * w.row_stride[i][1] + h * w.row_stride[i][2];
   const int64_t bytes = w.bytes[i], blocks = blocks16(to, bytes);
-  for (int64_t k = threadIdx.x & (lanes - 1); k < blocks; k += 2 * lanes) copy_blocks<2>(to, from, bytes, w.unit[i], k, lanes);
+  for (int64_t k = threadIdx.x & (lanes - 1); k < blocks; k += 4 * lanes) copy_blocks<4>(to, from, bytes, w.unit[i], k, lanes);
 }
 
 // ---- sequences that branch, and that are cut back
@@ -555,8 +555,10 @@ int jk_cache_write(const jk_rows_t* q, const jk_cache_t* cache, const int32_t* c
       w.row_stride[i][j] = q->rows_strides[3 * i + j] * size;
     }
     w.unit[i] = static_cast<uint8_t>(size);
-    // as many lanes as a row has blocks (one more where it begins inside a block), a power of 2
-    const int64_t blocks = (w.bytes[i] + 15) / 16 + (w.bytes[i] % 16 != 0 && w.bytes[i] > 16 ? 1 : 0);
+    // lanes of a row: as many as it has blocks (one more where it begins inside a block), a power of 2, but four blocks a lane
+    // in rows of 512 bytes and more, so that each table entry that is waited for is followed by that many loads
+    int64_t blocks = (w.bytes[i] + 15) / 16 + (w.bytes[i] % 16 != 0 && w.bytes[i] > 16 ? 1 : 0);
+    if (blocks >= 32) blocks = (blocks + 3) / 4;
     int log2 = 0;
     while (log2 < 5 && (int64_t(1) << log2) < blocks) ++log2;
     w.lanes_log2[i] = static_cast<uint8_t>(log2);

@@ -6,8 +6,10 @@
 // Where all are accepted r is the target's next distribution.
 //
 // A comparison of a product or of a running sum decides a token, so both are in f64: products of two
-// f32 are exact there, and a running sum is off by less than 2^-50 of the total, where f32 would give
-// another token in one of some thousand draws over a vocabulary of 100,000.
+// f32 are exact there, and a running sum is off by less than 2^-44 of the total, where f32 would give
+// another token in one of some thousand draws over a vocabulary of 100,000. Conversions to f64 are the
+// slowest part (16 a cycle and SM), so a difference takes one: d = x - y in f32, whose rounding error
+// (x - d) - y is exact there for x >= y >= 0, and errors are added up on their own.
 //
 // Of the draft's and the target's rows only place a's are read, once: a cluster of blocks per
 // sequence adds them up by warps, each a run of 16-byte packs; the run that holds the draw is cut
@@ -18,11 +20,14 @@
 #include "jk_host.h"
 #include "jk_rows.cuh"
 
+#include <type_traits>
+
 namespace jk {
 namespace verify {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kFew = 512, kMany = 128;  // threads of a block, for few sequences and for many
+constexpr int kManyPerSm = 7;
+constexpr int kLoads = 2;               // packs of a lane whose loads are on their way together
 constexpr int kMaxCluster = 8;
 constexpr int kSms = 148;
 
@@ -44,7 +49,28 @@ __device__ __forceinline__ double warp_sum64(double v) {
 }
 
 // NaN and negative values count as 0.
-__device__ __forceinline__ float mass(float v) { return v > 0.0f ? v : 0.0f; }
+__device__ __forceinline__ float mass(float v) { return fmaxf(v, 0.0f); }
+
+// Packs of both as 0 <= y <= x: 16-bit types two at a time.
+template <typename T>
+__device__ __forceinline__ void bounded(const uint4& u, const uint4& v, float (&x)[kPack<T>], float (&y)[kPack<T>]) {
+  if constexpr (sizeof(T) == 4) {
+    unpack<T>(u, x);
+    unpack<T>(v, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = mass(x[e]), y[e] = fminf(mass(y[e]), x[e]);
+  } else {
+    using P = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    uint4 a = u, b = v;
+    P *pa = reinterpret_cast<P*>(&a), *pb = reinterpret_cast<P*>(&b);
+    const uint32_t none = 0;
+    const P zero = *reinterpret_cast<const P*>(&none);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pa[i] = __hmax2(pa[i], zero), pb[i] = __hmin2(__hmax2(pb[i], zero), pa[i]);
+    unpack<T>(a, x);
+    unpack<T>(b, y);
+  }
+}
 
 // One place's r: packs of E entries on the 16-byte blocks of the target's row.
 template <typename T>
@@ -62,44 +88,89 @@ struct Rest {
     apart = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q_) - reinterpret_cast<uintptr_t>(p_)) & 15u;
   }
 
-  // Entries [E k - head, E k - head + E); those outside the row are 0.
-  __device__ __forceinline__ void load(int32_t k, double (&r)[E]) const {
+  // Entries [E k - head, E k - head + E) of both, as 0 <= y <= x; those outside the row, and `without`, are 0.
+  __device__ __forceinline__ void load(int32_t k, float (&x)[E], float (&y)[E]) const {
     const int32_t j = k * E - head;
-    float a[E], b[E];
-    if (j >= 0 && j + E <= vocab) {
-      unpack<T>(*reinterpret_cast<const uint4*>(p + j), a);
-      if (q == nullptr) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) b[e] = 0.0f;
-      } else {
-        unpack<T>(load16(q + j, apart), b);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const bool in = j + e >= 0 && j + e < vocab;
-        a[e] = in ? to_f32(p[j + e]) : 0.0f;
-        b[e] = in && q != nullptr ? to_f32(q[j + e]) : 0.0f;
-      }
-    }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float x = mass(a[e]), y = mass(b[e]);
-      r[e] = x > y && j + e != without ? static_cast<double>(x) - static_cast<double>(y) : 0.0;
+      const bool in = j + e >= 0 && j + e < vocab && j + e != without;
+      x[e] = mass(in ? to_f32(p[j + e]) : 0.0f);
+      y[e] = fminf(mass(in && q != nullptr ? to_f32(q[j + e]) : 0.0f), x[e]);
     }
+  }
+
+  static __device__ __forceinline__ void add(const float (&x)[E], const float (&y)[E], double& s, float& lost) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = x[e] - y[e];
+      lost += (x[e] - d) - y[e];
+      s += static_cast<double>(d);
+    }
+  }
+
+  // Over packs [from, to), a warp. WORDS: apart / 4, known where the loop is compiled, as selecting words would take most of
+  // its time; 4: there is no draft.
+  template <int WORDS>
+  __device__ __forceinline__ double sum_of(int32_t from, int32_t to) const {
+    const int lane = threadIdx.x & 31;
+    double s = 0.0;
+    float lost = 0.0f;
+    // packs that lie in the row as a whole, [low, high): their loads go out kLoads at a time
+    const int32_t first = head > 0 ? 1 : 0, past = (head + vocab) / E;
+    const int32_t low = from > first ? from : first, high = to < past ? to : past;
+    const int32_t odd = without >= 0 ? (without + head) / E : -1;
+    for (int32_t k = low + lane; k < high; k += 32 * kLoads) {
+      uint4 u[kLoads], v[kLoads], n[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        u[i] = v[i] = n[i] = make_uint4(0, 0, 0, 0);
+        if (k + 32 * i < high) {
+          const int32_t j = (k + 32 * i) * E - head;
+          u[i] = *reinterpret_cast<const uint4*>(p + j);
+          if (WORDS < 4) {
+            const uint4* block = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(q + j) - apart);
+            v[i] = block[0];
+            if (WORDS > 0 || apart != 0) n[i] = block[1];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (WORDS < 4) {
+          const uint32_t w[8] = {v[i].x, v[i].y, v[i].z, v[i].w, n[i].x, n[i].y, n[i].z, n[i].w}, bits = (apart & 3) * 8;
+          constexpr int W = WORDS & 3;
+          v[i] = make_uint4(__funnelshift_r(w[W], w[W + 1], bits), __funnelshift_r(w[W + 1], w[W + 2], bits),
+                            __funnelshift_r(w[W + 2], w[W + 3], bits), __funnelshift_r(w[W + 3], w[W + 4], bits));
+        }
+        float x[E], y[E];
+        bounded<T>(u[i], v[i], x, y);
+        if (WORDS == 4 && k + 32 * i == odd) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (odd * E - head + e == without) x[e] = 0.0f;
+        }
+        add(x, y, s, lost);
+      }
+    }
+    // the row's first and last pack, where other data share them
+    const int32_t edge = lane == 0 ? 0 : packs - 1;
+    if (lane < 2 && edge >= from && edge < to && (edge < first || edge >= past) && (lane == 0 || packs > 1)) {
+      float x[E], y[E];
+      load(edge, x, y);
+      add(x, y, s, lost);
+    }
+    return warp_sum64(s + static_cast<double>(lost));
   }
 
   // Over packs [from, to), a warp.
   __device__ __forceinline__ double sum(int32_t from, int32_t to) const {
-    double s = 0.0;
-#pragma unroll 4
-    for (int32_t k = from + (threadIdx.x & 31); k < to; k += 32) {
-      double r[E];
-      load(k, r);
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += r[e];
+    if (q == nullptr) return sum_of<4>(from, to);
+    switch (apart >> 2) {
+      case 0: return sum_of<0>(from, to);
+      case 1: return sum_of<1>(from, to);
+      case 2: return sum_of<2>(from, to);
+      default: return sum_of<3>(from, to);
     }
-    return warp_sum64(s);
   }
 };
 
@@ -120,8 +191,9 @@ __device__ __forceinline__ int part_of(const double* sums, int n, double draw, d
   return best;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const Args g) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == kMany ? kManyPerSm : 1) verify_kernel(const Args g) {
+  constexpr int kWarps = THREADS / 32;
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
   __shared__ double sums[kWarps];
@@ -139,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args g) {
   const float* uniform = g.uniform + b * (g.drafted + 1);
   if (tid == 0) first = n;
   __syncthreads();
-  for (int32_t i = tid; i < n; i += kThreads) {
+  for (int32_t i = tid; i < n; i += THREADS) {
     const int64_t x = tokens[i];
     bool ok = false;
     if (x >= 0 && x < g.vocab) {
@@ -202,8 +274,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args g) {
     if (warp == 0) {
       int32_t found = -1, last = -1;
       for (int32_t k0 = from; k0 < to && found < 0; k0 += 32) {
-        double r[Rest<T>::E] = {};
-        if (k0 + lane < to) rest.load(k0 + lane, r);
+        float x[Rest<T>::E] = {}, y[Rest<T>::E] = {};
+        if (k0 + lane < to) rest.load(k0 + lane, x, y);
+        double r[Rest<T>::E];
+#pragma unroll
+        for (int e = 0; e < Rest<T>::E; ++e) r[e] = static_cast<double>(x[e]) - static_cast<double>(y[e]);
         double own = 0.0;
 #pragma unroll
         for (int e = 0; e < Rest<T>::E; ++e) own += r[e];
@@ -237,20 +312,16 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args g) {
   __syncthreads();
   if (owner == rank || (owner < 0 && rank == 0)) {
     int64_t* out = g.out + b * (g.drafted + 1);
-    for (int32_t i = tid; i <= g.drafted; i += kThreads) out[i] = i < a ? tokens[i] : i == a ? token : -1;
+    for (int32_t i = tid; i <= g.drafted; i += THREADS) out[i] = i < a ? tokens[i] : i == a ? token : -1;
     if (tid == 0) g.accepted[b] = a;
   }
 }
 
-template <typename T>
-int launch(const Args& g, int64_t batch, cudaStream_t s) {
-  // Blocks of a sequence: as many as leave each SM two blocks at most, none for less than 2048
-  // entries. (One sequence of 131072 entries in f32: see the figures below.)
-  int size = 1;
-  while (size < kMaxCluster && batch * size * 2 <= 2 * kSms && g.vocab / (size * 2) >= 2048) size *= 2;
+template <typename T, int THREADS>
+int launch_one(const Args& g, int64_t batch, int size, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * size));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -258,8 +329,20 @@ int launch(const Args& g, int64_t batch, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, verify_kernel<T>, g);
+  cudaLaunchKernelEx(&cfg, verify_kernel<T, THREADS>, g);
   return launch_status();
+}
+
+template <typename T>
+int launch(const Args& g, int64_t batch, cudaStream_t s) {
+  // Blocks of a sequence: a power of 2, as many as the SMs hold together, none for less than 2048 entries. Few sequences: large
+  // blocks, one to an SM; many: small ones, whose number the SMs share out more evenly (256 sequences of 100003 entries: four
+  // blocks each, 1024 blocks where 1036 fit).
+  const bool few = batch * kMaxCluster <= kSms;
+  const int64_t slots = few ? kSms : kSms * kManyPerSm;
+  int size = 1;
+  while (size < kMaxCluster && batch * size * 2 <= slots && g.vocab / (size * 2) >= 2048) size *= 2;
+  return few ? launch_one<T, kFew>(g, batch, size, s) : launch_one<T, kMany>(g, batch, size, s);
 }
 
 }  // namespace verify
