@@ -476,7 +476,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
           const bool counts = r < rows && t < span.n;
           const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
-          for (int c = lane; c < a.key_cols; c += 32) query[r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
+          // (f32: columns first)
+      for (int c = lane; c < a.key_cols; c += 32) query[kWide ? c * ROWS + r : r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
         }
         if (!TILED && a.key_cols > a.rank) {
           for (int i = lane; i < a.stages * kKeys; i += 32) {
@@ -664,19 +665,31 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           }
         }
       } else {
-        // f32: a lane has half of a place's columns, lanes 16.. the other half
-        const int place = own_place, half = a.key_cols / 2, x0 = lane < 16 ? 0 : half;
-        const float* q = reinterpret_cast<const float*>(query) + x0;
-        uint64_t dots[ROWS];
+        // f32: a lane has a place and half of the rows, lanes 16.. the other half; columns in order, one sum a row
+        const int place = own_place;
+        const float* q = reinterpret_cast<const float*>(query) + own_row;
+        uint64_t dots[(OWN + 1) / 2];  // rows in pairs
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) dots[r] = 0;
+        for (int j = 0; j < (OWN + 1) / 2; ++j) dots[j] = 0;
 #pragma unroll 2
-        for (int x = 0; x < half; x += 4) {
-          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(stage + ((x0 + x) >> 5) * kColumn + block_at(place, ((x0 + x) >> 2) & 7));
+        for (int x = 0; x < a.key_cols; x += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(stage + (x >> 5) * kColumn + block_at(place, (x >> 2) & 7));
+          const float k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(q + r * a.query_row + x);
-            dots[r] = fma2(k4.y, q4.y, fma2(k4.x, q4.x, dots[r]));
+          for (int x1 = 0; x1 < 4; ++x1) {
+            const float* at_x = q + (x + x1) * ROWS;
+            if constexpr (OWN == 1) {
+              dots[0] = pair(fmaf(k[x1], *at_x, unpair(dots[0]).x), 0.0f);
+            } else {
+              const uint64_t kk = pair(k[x1], k[x1]);
+              if constexpr (OWN == 4) {
+                const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(at_x);
+                dots[0] = fma2(kk, two.x, dots[0]);
+                dots[1] = fma2(kk, two.y, dots[1]);
+              } else {
+                dots[0] = fma2(kk, *reinterpret_cast<const uint64_t*>(at_x), dots[0]);
+              }
+            }
           }
         }
         float score[OWN], level[OWN];
@@ -684,16 +697,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         bool higher = unset;
 #pragma unroll
         for (int i2 = 0; i2 < OWN; ++i2) {
-          float2 v = unpair(dots[i2]);
-          const float mine = v.x + v.y;
-          if (ROWS == 1) {
-            score[i2] = mine + __shfl_xor_sync(0xffffffffu, mine, 16);
-          } else {  // each half of the warp gives the other half the sums of its rows
-            v = unpair(dots[i2 + ROWS - OWN]);
-            const float other = v.x + v.y;
-            score[i2] = (lane < 16 ? mine : other) + __shfl_xor_sync(0xffffffffu, lane < 16 ? other : mine, 16);
-          }
-          score[i2] = score_of<COMPRESS>(score[i2], a.scale, a.bias);
+          const float2 two = unpair(dots[i2 / 2]);
+          score[i2] = score_of<COMPRESS>(i2 % 2 == 0 ? two.x : two.y, a.scale, a.bias);
           sees[i2] = full || (((there >> place) & 1) && k0 + place < row_end[i2] && k0 + place >= row_low[i2]);
           any[i2] |= sees[i2];
           level[i2] = level_of<COMPRESS>(score[i2], a.scale, base[i2]);
@@ -989,9 +994,9 @@ inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, b
   if (wide) s.rows = unit_rows == 1 ? 1 : (tiled && unit_rows <= 4) || s.dim == 512 ? 4 : 8;
   else s.rows = !tiled || unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
   s.row_blocks = static_cast<int>((unit_rows + s.rows - 1) / s.rows);
-  // columns in the products' steps (two of 16, or two halves of 4); queries an odd number of 16-byte blocks apart, so that
+  // columns in the products' steps (two of 16, or 4); queries of 16-bit types an odd number of 16-byte blocks apart, so that
   // eight of them lie in different banks
-  s.key_cols = static_cast<int>(wide ? (rank + 7) / 8 * 8 : (rank + 31) / 32 * 32);
+  s.key_cols = static_cast<int>(wide ? (rank + 3) / 4 * 4 : (rank + 31) / 32 * 32);
   s.query_row = s.key_cols + 16 / size;
   s.key_bytes = static_cast<int>((rank + column - 1) / column) * kColumn;
   s.stage_bytes = s.key_bytes + static_cast<int>((dim + column - 1) / column) * kColumn;
