@@ -76,7 +76,9 @@ struct Args {
   int32_t ring_bytes;                     // of all rings (and of what is joined in their place)
   int32_t part_row;                       // floats of a row that a block leaves: dim rounded up to 4, reference, sum, state
   float* parts;                           // [blocks][2][rows][part_row]
+  int32_t units;
   bool split, tiled;
+  bool whole_runs;                        // a block's run is of one unit: units are few, so that what is left empty is little
 };
 
 // ---- a sequence's places
@@ -107,6 +109,14 @@ __device__ __forceinline__ Span span_of(const Args& a, int32_t b) {
 __device__ __forceinline__ int32_t tiles_of(const Span& s) { return s.low < s.end ? (s.end - s.base + kTile - 1) / kTile : 0; }
 
 __device__ __forceinline__ Span span_as(const Args& a, int32_t b) { return a.tiled ? span_of<true>(a, b) : span_of<false>(a, b); }
+
+// Tiles of a block's run, of `total` tiles.
+__device__ __forceinline__ int32_t run_of(const Args& a, int32_t total) {
+  const int32_t runs = a.whole_runs ? a.blocks - a.units : a.blocks;
+  return total <= runs ? 1 : (total + runs - 1) / runs;
+}
+
+__device__ __forceinline__ int32_t filled_up(int32_t tiles, int32_t run) { return run == 1 ? tiles : (tiles + run - 1) / run * run; }
 
 // ---- small pieces
 
@@ -293,31 +303,34 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 
   int32_t chunk = 1, at = 0, until = 1;  // (the host sees to it that all tiles are fewer than 2^30)
   if (a.split) {
-    // tiles before each sequence
+    // tiles before each sequence; where runs end with a unit, of units that are filled up to whole runs
     int32_t carry = 0;
-    if (tid == 0) before[0] = 0;
-    for (int32_t base = 0; base < a.batch; base += kThreads) {
-      const int32_t b = base + tid;
-      int32_t v = b < a.batch ? tiles_of(span_of<TILED>(a, b)) * (a.kv_heads * a.row_blocks) : 0;
+    for (int turn = 0; turn < (a.whole_runs ? 2 : 1); ++turn) {
+      if (turn == 1) chunk = run_of(a, carry), carry = 0;
+      if (tid == 0) before[0] = 0;
+      for (int32_t base = 0; base < a.batch; base += kThreads) {
+        const int32_t b = base + tid;
+        int32_t v = b < a.batch ? filled_up(tiles_of(span_of<TILED>(a, b)), chunk) * (a.kv_heads * a.row_blocks) : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int32_t up = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += up;
-      }
-      __syncthreads();
-      if (lane == 31) scan[warp] = v;
-      __syncthreads();
-      int32_t add = carry;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int32_t up = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += up;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = v;
+        __syncthreads();
+        int32_t add = carry;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) add += scan[w];
-        carry += scan[w];
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) add += scan[w];
+          carry += scan[w];
+        }
+        if (b < a.batch) before[b + 1] = v + add;
       }
-      if (b < a.batch) before[b + 1] = v + add;
     }
     __syncthreads();
     grid_dependency_launch();
-    chunk = (carry + a.blocks - 1) / a.blocks;
+    if (!a.whole_runs) chunk = run_of(a, carry);
     at = chunk * int32_t(blockIdx.x) < carry ? chunk * int32_t(blockIdx.x) : carry;
     until = at + chunk < carry ? at + chunk : carry;
   }
@@ -349,9 +362,9 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     const Span span = span_of<TILED>(a, b);
     unit_tiles = tiles_of(span);
     if (a.split) {
-      const uint32_t in = at - before[b];
-      inner = in / static_cast<uint32_t>(unit_tiles);
-      tile = in - inner * unit_tiles;
+      const uint32_t in = at - before[b], room = a.whole_runs ? filled_up(unit_tiles, chunk) : unit_tiles;
+      inner = in / room;
+      tile = in - inner * room;
       unit_begin = at - tile;
       tiles = unit_tiles - tile < until - at ? unit_tiles - tile : until - at;
     } else {
@@ -868,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     }
     if (TILED) fence_proxy_async_smem();
     __syncthreads();  // before the next unit's queries, and before the rings are filled again
-    if (a.split) at += tiles;
+    if (a.split && !a.whole_runs) at += tiles;
     else at = until;
   }
 }
@@ -891,22 +904,30 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   // the blocks' runs, as the first kernel has them (while it runs)
   const Span span = span_as(a, b);
   const int32_t tiles = tiles_of(span);
-  int32_t mine = 0, all_tiles = 0;
-  for (int32_t i = tid; i < a.batch; i += 256) {
-    const int32_t n = tiles_of(span_as(a, i)) * (a.kv_heads * a.row_blocks);
-    all_tiles += n;
-    if (i < b) mine += n;
-  }
+  int32_t mine = 0, all_tiles = 0, chunk = 1;
+  for (int turn = 0; turn < (a.whole_runs ? 2 : 1); ++turn) {
+    if (turn == 1) {
+      chunk = run_of(a, all_tiles);
+      __syncthreads();  // the counts have been read
+    }
+    mine = all_tiles = 0;
+    for (int32_t i = tid; i < a.batch; i += 256) {
+      const int32_t n = filled_up(tiles_of(span_as(a, i)), chunk) * (a.kv_heads * a.row_blocks);
+      all_tiles += n;
+      if (i < b) mine += n;
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    all_tiles += __shfl_xor_sync(0xffffffffu, all_tiles, o);
-  }
-  if (lane == 0) counted[warp][0] = mine, counted[warp][1] = all_tiles;
-  __syncthreads();
-  mine = all_tiles = 0;
+    for (int o = 16; o > 0; o >>= 1) {
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      all_tiles += __shfl_xor_sync(0xffffffffu, all_tiles, o);
+    }
+    if (lane == 0) counted[warp][0] = mine, counted[warp][1] = all_tiles;
+    __syncthreads();
+    mine = all_tiles = 0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) mine += counted[w][0], all_tiles += counted[w][1];
+    for (int w = 0; w < 8; ++w) mine += counted[w][0], all_tiles += counted[w][1];
+  }
+  if (!a.whole_runs) chunk = run_of(a, all_tiles);
   T* out = reinterpret_cast<T*>(a.out_value) + row * a.dim + d0;
   const bool first_slice = tid == 0 && d0 == 0 && a.out_state != nullptr;
   if (tiles == 0) {
@@ -915,9 +936,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     grid_dependency_wait();
     return;
   }
-  const int32_t chunk = (all_tiles + a.blocks - 1) / a.blocks;
   const int32_t row_block = row_of / a.rows, r = row_of - row_block * a.rows;
-  const int32_t begin = mine + (kv * a.row_blocks + row_block) * tiles;
+  const int32_t begin = mine + (kv * a.row_blocks + row_block) * (a.whole_runs ? filled_up(tiles, chunk) : tiles);
   const int32_t first = begin / chunk, last = (begin + tiles - 1) / chunk;
   grid_dependency_wait();
   if (first == last) return;  // one block had all of it
