@@ -52,6 +52,15 @@ __device__ __forceinline__ void copy_blocks(char* dst, const char* src, int64_t 
   const uint32_t head = address16(dst), a = (address16(src) - head) & 15u;
   const int64_t at = first * 16 - head;
   uint4 v[N];
+  if (((head | a | static_cast<uint32_t>(bytes)) & 15u) == 0) {  // 16-byte blocks on both sides: what caches mostly have
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (at + j * step * 16 < bytes) v[j] = *reinterpret_cast<const uint4*>(src + at + j * step * 16);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (at + j * step * 16 < bytes) *reinterpret_cast<uint4*>(dst + at + j * step * 16) = v[j];
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int64_t off = at + int64_t(j) * step * 16;

@@ -99,12 +99,17 @@ struct Rest {
     }
   }
 
-  static __device__ __forceinline__ void add(const float (&x)[E], const float (&y)[E], double& s, float& lost) {
+  // s + lost: the sum of x - y; two differences at a time.
+  static __device__ __forceinline__ void add(const float (&x)[E], const float (&y)[E], double& s, uint64_t& lost) {
+    const uint64_t minus = pair(-1.0f, -1.0f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = x[e] - y[e];
-      lost += (x[e] - d) - y[e];
-      s += static_cast<double>(d);
+    for (int e = 0; e < E; e += 2) {
+      const uint64_t x2 = pair(x[e], x[e + 1]), y2 = pair(y[e], y[e + 1]);
+      const uint64_t d = fma2(y2, minus, x2);
+      lost = add2(lost, fma2(y2, minus, fma2(d, minus, x2)));
+      const float2 f = unpair(d);
+      s += static_cast<double>(f.x);
+      s += static_cast<double>(f.y);
     }
   }
 
@@ -114,43 +119,50 @@ struct Rest {
   __device__ __forceinline__ double sum_of(int32_t from, int32_t to) const {
     const int lane = threadIdx.x & 31;
     double s = 0.0;
-    float lost = 0.0f;
+    uint64_t lost = 0;
     // packs that lie in the row as a whole, [low, high): their loads go out kLoads at a time
     const int32_t first = head > 0 ? 1 : 0, past = (head + vocab) / E;
     const int32_t low = from > first ? from : first, high = to < past ? to : past;
     const int32_t odd = without >= 0 ? (without + head) / E : -1;
-    for (int32_t k = low + lane; k < high; k += 32 * kLoads) {
+    auto fetch = [&](int32_t k, uint4& u, uint4& v, uint4& n) {
+      const int32_t j = k * E - head;
+      u = *reinterpret_cast<const uint4*>(p + j);
+      v = n = make_uint4(0, 0, 0, 0);
+      if (WORDS < 4) {
+        const uint4* block = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(q + j) - apart);
+        v = block[0];
+        if (WORDS > 0 || apart != 0) n = block[1];
+      }
+    };
+    auto take = [&](int32_t k, const uint4& u, uint4 v, const uint4& n) {
+      if (WORDS < 4) {
+        const uint32_t w[8] = {v.x, v.y, v.z, v.w, n.x, n.y, n.z, n.w}, bits = (apart & 3) * 8;
+        constexpr int W = WORDS & 3;
+        v = make_uint4(__funnelshift_r(w[W], w[W + 1], bits), __funnelshift_r(w[W + 1], w[W + 2], bits),
+                       __funnelshift_r(w[W + 2], w[W + 3], bits), __funnelshift_r(w[W + 3], w[W + 4], bits));
+      }
+      float x[E], y[E];
+      bounded<T>(u, v, x, y);
+      if (WORDS == 4 && k == odd) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (odd * E - head + e == without) x[e] = 0.0f;
+      }
+      add(x, y, s, lost);
+    };
+    int32_t k = low + lane;
+    for (; k + 32 * (kLoads - 1) < high; k += 32 * kLoads) {
       uint4 u[kLoads], v[kLoads], n[kLoads];
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        u[i] = v[i] = n[i] = make_uint4(0, 0, 0, 0);
-        if (k + 32 * i < high) {
-          const int32_t j = (k + 32 * i) * E - head;
-          u[i] = *reinterpret_cast<const uint4*>(p + j);
-          if (WORDS < 4) {
-            const uint4* block = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(q + j) - apart);
-            v[i] = block[0];
-            if (WORDS > 0 || apart != 0) n[i] = block[1];
-          }
-        }
-      }
+      for (int i = 0; i < kLoads; ++i) fetch(k + 32 * i, u[i], v[i], n[i]);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        if (WORDS < 4) {
-          const uint32_t w[8] = {v[i].x, v[i].y, v[i].z, v[i].w, n[i].x, n[i].y, n[i].z, n[i].w}, bits = (apart & 3) * 8;
-          constexpr int W = WORDS & 3;
-          v[i] = make_uint4(__funnelshift_r(w[W], w[W + 1], bits), __funnelshift_r(w[W + 1], w[W + 2], bits),
-                            __funnelshift_r(w[W + 2], w[W + 3], bits), __funnelshift_r(w[W + 3], w[W + 4], bits));
-        }
-        float x[E], y[E];
-        bounded<T>(u[i], v[i], x, y);
-        if (WORDS == 4 && k + 32 * i == odd) {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (odd * E - head + e == without) x[e] = 0.0f;
-        }
-        add(x, y, s, lost);
-      }
+      for (int i = 0; i < kLoads; ++i) take(k + 32 * i, u[i], v[i], n[i]);
+    }
+#pragma unroll 1
+    for (; k < high; k += 32) {
+      uint4 u, v, n;
+      fetch(k, u, v, n);
+      take(k, u, v, n);
     }
     // the row's first and last pack, where other data share them
     const int32_t edge = lane == 0 ? 0 : packs - 1;
@@ -159,7 +171,8 @@ struct Rest {
       load(edge, x, y);
       add(x, y, s, lost);
     }
-    return warp_sum64(s + static_cast<double>(lost));
+    const float2 rest = unpair(lost);
+    return warp_sum64(s + (static_cast<double>(rest.x) + static_cast<double>(rest.y)));
   }
 
   // Over packs [from, to), a warp.
