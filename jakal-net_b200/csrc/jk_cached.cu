@@ -18,11 +18,11 @@ int64_t tiles_at_most(int64_t page_size, int64_t columns, int64_t window, int64_
 
 int32_t window_of(int64_t window) { return window < 0 ? -1 : window > 0x7fffffff ? 0x7fffffff : static_cast<int32_t>(window); }
 
-// Bytes of one asynchronous copy: the most that addresses, strides and the row's length allow.
+// Bytes of the pieces that rows can be copied in: what addresses, strides and the row's length allow.
 int piece_of(const void* base, const int64_t (&stride)[3], int64_t row_bytes) {
   uint64_t odd = reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(row_bytes);
   for (int64_t s : stride) odd |= static_cast<uint64_t>(s);
-  return (odd & 15) == 0 ? 16 : (odd & 7) == 0 ? 8 : (odd & 3) == 0 ? 4 : 0;
+  return (odd & 15) == 0 ? 16 : (odd & 7) == 0 ? 8 : (odd & 3) == 0 ? 4 : 2;
 }
 
 // The map of [pages][heads][places][columns], of which a copy fetches 16 places x 128 bytes.

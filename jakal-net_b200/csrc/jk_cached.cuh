@@ -14,8 +14,10 @@
 //   * A warp has every fourth 16 places of the run to itself: its own ring of shared memory, its own
 //     reference and sums, no barrier between warps until the run's end, where the four are joined in
 //     shared memory. Where pages hold a multiple of 16 places in 16-byte rows, one lane fetches the 16 by
-//     tiled copies of 128-byte columns (4 for rank and dim 128 in 16 bits); else all lanes copy pieces.
-//     (One bulk copy a row takes as long as the rest of the turn: 32 of them are issued one by one.)
+//     tiled copies of 128-byte columns (4 for rank and dim 128 in 16 bits); else all lanes copy pieces
+//     of 16, 8 or 4 bytes (7.0 and 8.8 us for 256 places of 8 heads of rank and dim 64, 13.3 and 14.4 for 4 x
+//     4097 of dim 512, 222 and 225 for 32 x 10240 of 8 heads of 128, on the device). One bulk copy a row took
+//     326 for the latter: 32 of them are issued one by one.
 //   * Few warps fit an SM beside their rings, so a turn is short of instructions: places that all rows see
 //     need no masks, and a reference that follows the maximum only once that is 8 (a factor of 256)
 //     above it needs a vote a turn in place of a maximum over the warp.
@@ -50,7 +52,7 @@ constexpr int kTile = kWarps * kKeys;   // places of a block's turn
 constexpr int kSms = 148;
 constexpr int kMaxPerSm = 3;            // blocks of an SM
 constexpr int kMaxBatch = 256;          // sequences of a launch
-constexpr int kMaxStages = 3;           // of a warp's ring
+constexpr int kMaxStages = 2;           // of a warp's ring
 constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
 constexpr int kUnitTiles = 8;           // units of at most so many tiles get a block each
 constexpr float kLog2e = 1.4426950408889634f;
@@ -69,7 +71,7 @@ struct Args {
   char *out_value, *out_state;
   // layout
   int32_t blocks, row_blocks, rows;       // blocks of the grid; row blocks of a unit's rows, and rows of one
-  int32_t key_piece, value_piece;         // bytes of one asynchronous copy (16, 8, 4), 0: element by element
+  int32_t key_piece, value_piece;         // bytes of a piece that rows are copied in (16, 8, 4, 2)
   int32_t key_cols;                       // of a key's row read: rank rounded up to the product's steps
   int32_t query_row;                      // elements from one query to the next in shared memory
   int32_t key_bytes, stage_bytes, stages; // of a ring: keys of a stage, a stage, their number
@@ -161,22 +163,19 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// `bytes` of src, or zeros.
+// `BYTES` of src, or zeros.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const char* src, bool there) {
-  const int n = there ? BYTES : 0;
   if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until at most `pending` of this thread's groups are on their way.
 __device__ __forceinline__ void copy_wait(int pending) {
   if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else asm volatile("cp.async.wait_group 1;" ::: "memory");
 }
 
 // ---- compressors
@@ -213,42 +212,64 @@ __device__ __forceinline__ float weight_of(float s, float mass) {
 // 128 r + 16 (c ^ (r mod 8)): eight rows' blocks c are in different banks. (Tiled copies write it so.)
 __device__ __forceinline__ int block_at(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
 
-// (as many lanes a row as have 128 bytes of it, so that a lane keeps its place in a column)
+// Rows of the 16 lanes' places in pieces of 16, 8 or 4 bytes, as their alignment allows, with as many lanes a row as have 128
+// bytes of it; rows that are not `there` arrive as zeros.
 template <int BYTES>
-__device__ __forceinline__ void load_pieces(uint32_t to, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
+__device__ __forceinline__ void load_pieces(char* stage, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
   constexpr int kLanes = 128 / BYTES, kStep = 32 / kLanes;
   const int byte = lane % kLanes * BYTES;
 #pragma unroll
   for (int row0 = 0; row0 < kKeys; row0 += kStep) {
     const int row = row0 + lane / kLanes;
     const char* from = src + __shfl_sync(0xffffffffu, offset, row) + byte;
-    uint32_t dst = to + block_at(row, byte >> 4) + (byte & 15);
+    uint32_t to = shared_at(stage) + block_at(row, byte >> 4) + (byte & 15);
     const bool ok = (there >> row) & 1;
     for (int c = byte; c < row_bytes; c += 128) {
-      copy_async<BYTES>(dst, from, ok);
-      dst += kColumn;
+      copy_async<BYTES>(to, from, ok);
+      to += kColumn;
       from += 128;
     }
   }
 }
 
-// Rows of the 16 lanes' places; rows that are not `there` arrive as zeros.
+// The same for 16-bit rows that begin at any element: 16-byte blocks are put together from the two that hold their bytes, through
+// registers. (These loads are waited for. 32 sequences of 10240 f16 nodes, rank 128: 222 us with a dim of 128, 306 with 124 in
+// pieces of 8, 404 with 126 in pieces of 4, 801 with 127 so, 1355 element by element; 126 so would take 762.)
 template <typename T>
-__device__ __forceinline__ void load_rows(char* dst, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int piece, int lane) {
-  const uint32_t to = shared_at(dst);
-  if (piece == 16) return load_pieces<16>(to, src, offset, there, row_bytes, lane);
-  if (piece == 8) return load_pieces<8>(to, src, offset, there, row_bytes, lane);
-  if (piece == 4) return load_pieces<4>(to, src, offset, there, row_bytes, lane);
-  if constexpr (sizeof(T) == 2) {  // 16-bit rows of an odd width, or that begin anywhere
-#pragma unroll 4
-    for (int row = 0; row < kKeys; ++row) {
-      const char* from = src + __shfl_sync(0xffffffffu, offset, row);
-      const bool ok = (there >> row) & 1;
-      for (int c = 2 * lane; c < row_bytes; c += 64)
-        *reinterpret_cast<uint16_t*>(dst + (c >> 7) * kColumn + block_at(row, (c >> 4) & 7) + (c & 15)) =
-            ok ? *reinterpret_cast<const uint16_t*>(from + c) : uint16_t(0);
+__device__ __forceinline__ void load_odd_rows(char* dst, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
+  const char* from[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) from[q] = src + __shfl_sync(0xffffffffu, offset, 4 * q + (lane >> 3));
+#pragma unroll 1
+  for (int c = (lane & 7) * 16; c < row_bytes; c += 128) {
+    char* to = dst + (c >> 7) * kColumn;
+    if (c + 16 <= row_bytes) {
+      uint4 v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[q] = make_uint4(0, 0, 0, 0);
+        if ((there >> (4 * q + (lane >> 3))) & 1) v[q] = load16(from[q] + c, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from[q])) & 15u);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(to + block_at(4 * q + (lane >> 3), lane & 7)) = v[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = 4 * q + (lane >> 3);
+#pragma unroll 1
+        for (int e = c; e < row_bytes; e += sizeof(T))
+          *reinterpret_cast<T*>(to + block_at(row, lane & 7) + (e & 15)) = (there >> row) & 1 ? *reinterpret_cast<const T*>(from[q] + e) : from_f32<T>(0.0f);
+      }
     }
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_rows(char* stage, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int piece, int lane) {
+  if (piece == 16) return load_pieces<16>(stage, src, offset, there, row_bytes, lane);
+  if (piece == 8) return load_pieces<8>(stage, src, offset, there, row_bytes, lane);
+  if (piece == 4) return load_pieces<4>(stage, src, offset, there, row_bytes, lane);
+  if constexpr (sizeof(T) == 2) load_odd_rows<T>(stage, src, offset, there, row_bytes, lane);
 }
 
 // One column of 128 bytes of the 16 places from `place` on of a page: a tiled copy, counted on `bar`.
@@ -429,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               for (int c = 0; c < a.rank; c += COLUMN, stage += kColumn) load_column(stage, &maps.keys, bar, c, p.offset, kv, p.page);
               for (int c = 0; c < a.dim; c += COLUMN, stage += kColumn) load_column(stage, &maps.values, bar, c, p.offset, kv, p.page);
             }
-            fill = fill + 1 == a.stages ? 0 : fill + 1;
+            fill ^= 1;
             ++issued;
           }
           p.offset += own_place;
@@ -437,8 +458,9 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           made.there = __ballot_sync(0xffffffffu, there) & 0xffffu;
           char* stage = ring + (a.stages == 1 ? 0 : i & 1) * a.stage_bytes;
           const int64_t page = there ? p.page : 0, off = there ? p.offset : 0;
-          load_rows<T>(stage, keys, page * a.key_stride[0] + off * a.key_stride[2], made.there, a.rank * SIZE, a.key_piece, lane);
-          load_rows<T>(stage + a.key_bytes, values, page * a.value_stride[0] + off * a.value_stride[2], made.there, a.dim * SIZE, a.value_piece, lane);
+          const int64_t key_at = page * a.key_stride[0] + off * a.key_stride[2], value_at = page * a.value_stride[0] + off * a.value_stride[2];
+          load_rows<T>(stage, keys, key_at, made.there, a.rank * SIZE, a.key_piece, lane);
+          load_rows<T>(stage + a.key_bytes, values, value_at, made.there, a.dim * SIZE, a.value_piece, lane);
         }
         if (states != nullptr && ((made.there >> own_place) & 1))
           made.state = to_f32(*reinterpret_cast<const T*>(states + p.page * a.state_stride[0] + p.offset * a.state_stride[2]));
@@ -446,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       if (!TILED) copy_commit();
       return made;
     };
-    const int lead = TILED && a.stages == kMaxStages ? 2 : a.stages > 1 ? 1 : 0;  // turns on their way while one is worked on
+    const int lead = TILED || a.stages > 1 ? 1 : 0;  // turns on their way while one is worked on
     // ---- this thread's rows: the places they see, [row_low, row_end)
     const int own_row = kWide && ROWS > 1 && lane >= 16 ? OWN : 0;
     int32_t row_low[OWN], row_end[OWN];
@@ -475,13 +497,12 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     for (int i = 0; i < (kWide ? ROWS : 1); ++i)
 #pragma unroll
       for (int j = 0; j < CP; ++j) pairs[i][j] = 0;
-    Turn first{0, 0.0f}, second{0, 0.0f};
+    Turn first{0, 0.0f};
     for (int32_t i = -lead; i < tiles; ++i) {
       __syncwarp();  // the stage to fill has been read by all lanes
       const Turn made = issue(i + lead);
       const Turn now = lead ? first : made;
-      first = lead == 2 ? second : made;
-      second = made;
+      first = made;
       if (i < 0) continue;
       if (i == 0) {
         // ---- queries, and the keys' columns that no copy fills: 0
@@ -511,7 +532,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           g_device_error = JK_ERR_DEVICE_TIMEOUT;
         }
         late = __any_sync(0xffffffffu, late);
-        if (++take == a.stages) take = 0, phase ^= 1;
+        take ^= 1;
+        if (take == 0) phase ^= 1;
       }
       __syncwarp();
       char* const stage_values = stage + a.key_bytes;
@@ -794,8 +816,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     }
     if (!TILED) copy_wait(0);
     // what gave up waiting still lets its copies land
-    for (uint32_t q = issued < uint32_t(a.stages) ? 0 : issued - a.stages; TILED && late && q != issued; ++q)
-      mbar_wait(&landed[warp][q % a.stages], (q / a.stages) & 1);
+    for (uint32_t q = issued < 2 ? 0 : issued - 2; TILED && late && q != issued; ++q) mbar_wait(&landed[warp][q & 1], (q >> 1) & 1);
 
     // ---- the warps' sums, then the block's
 #pragma unroll
@@ -1030,9 +1051,9 @@ inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, b
   const int rest = s.rows * s.query_row * size + kWarps * s.rows * (wide ? 2 * kKeys : kKeys + 1) * 4;
   auto blocks = [&](int stages) { return static_cast<int>(227 * 1024 / (1024 + ring(stages) + rest + 4 * 1024)); };
   const int most = s.rows * s.dim <= 1024 ? kMaxPerSm : 2;
-  // Two stages a warp in as many blocks of an SM as fit, a third where that costs none; where not even one block has room for
-  // two, one stage. (32 sequences of 10240 f16 nodes, rank and dim 128: see the figures above.)
-  s.stages = blocks(2) < 1 ? 1 : tiled && blocks(3) >= (blocks(2) < most ? blocks(2) : most) ? 3 : 2;
+  // Two stages a warp in as many blocks of an SM as fit (a third stage gained nothing in any of the cases that are measured);
+  // where not even one block has room for two, one stage.
+  s.stages = blocks(2) < 1 ? 1 : 2;
   s.per_sm = blocks(s.stages) < most ? blocks(s.stages) : most;
   s.ring_bytes = ring(s.stages);
   s.shared = 1024 + s.ring_bytes + rest;
