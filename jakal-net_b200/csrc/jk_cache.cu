@@ -8,7 +8,9 @@
 // fills the GPU. Whole numbers throughout: results do not depend on the order in which blocks run
 // (references are added to, never read, where blocks share them).
 //
-// Bound: bookkeeping by the latency of a few dependent reads and a launch or two, copies by memory.
+// Bound: bookkeeping by the latency of a few dependent reads and a launch or two (room for a node in each of 32 sequences,
+// its rows written and given back: 9.8 us on the device, 45 as calls), copies by memory (the 70 us of 460 MB moved
+// together are what they take at the measured copy rate; 76 MB of new rows 16 us, of which 12 for the memory).
 // A copy has 16-byte stores to aligned blocks whatever the alignment of its two sides: where they
 // differ, a block is put together from the two aligned blocks of the source that hold its bytes
 // (so rows of 65 bf16 cost two loads a block instead of eight).
@@ -565,7 +567,8 @@ int jk_cache_write(const jk_rows_t* q, const jk_cache_t* cache, const int32_t* c
     }
     w.unit[i] = static_cast<uint8_t>(size);
     // lanes of a row: as many as it has blocks (one more where it begins inside a block), a power of 2, but four blocks a lane
-    // in rows of 512 bytes and more, so that each table entry that is waited for is followed by that many loads
+    // in rows of 512 bytes and more, so that each table entry that is waited for is followed by that many loads (32 x 1024 nodes of 64 + 512 + 1 bf16, with room and
+    // release: 24.4 us with two blocks a lane in all rows, 21.7 with four)
     int64_t blocks = (w.bytes[i] + 15) / 16 + (w.bytes[i] % 16 != 0 && w.bytes[i] > 16 ? 1 : 0);
     if (blocks >= 32) blocks = (blocks + 3) / 4;
     int log2 = 0;
@@ -606,8 +609,10 @@ int jk_cache_fork(const jk_cache_t* cache, const int32_t* parents, const int32_t
   auto* taken = static_cast<int32_t*>(workspace);
   auto* copied = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + round16(batch * 4));
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  // few table entries: the block that decides copies them as well, which saves a launch
-  const bool rows_too = columns == 0 || forks <= 32768 / columns;
+  // few table entries: the block that decides copies them as well, which saves a launch (forks and entries each, together with
+  // the release that undoes them, a call and on the device: 63 x 128 19.0 and 6.2 us so, 20.9 and 5.7 with a launch for the
+  // rows; 63 x 512 18.7 and 12.0, 21.0 and 6.3)
+  const bool rows_too = columns == 0 || forks <= 8192 / columns;
   fork_kernel<<<1, kOne, 0, s>>>(t, lengths, refs, parents, children, forks, done, taken, copied, rows_too);
   if (!rows_too)
     launch_dependent(fork_rows_kernel, static_cast<unsigned>(forks < kMaxBlocks ? forks : kMaxBlocks), kThreads, 0, s, t, refs, parents, children,

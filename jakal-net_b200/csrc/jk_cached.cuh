@@ -54,7 +54,9 @@ constexpr int kMaxPerSm = 3;            // blocks of an SM
 constexpr int kMaxBatch = 256;          // sequences of a launch
 constexpr int kMaxStages = 2;           // of a warp's ring
 constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
-constexpr int kUnitTiles = 8;           // units of at most so many tiles get a block each
+// Units of at most so many tiles get a block each, which saves a launch (8 heads of 512 places: 13.4 us a call and 11.4 on the
+// device so, 17.7 and 8.4 split; of 1024 places 21.2 and 18.3, 17.6 and 8.5).
+constexpr int kUnitTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;          // by which a score may pass its row's reference, in units of log 2
 
