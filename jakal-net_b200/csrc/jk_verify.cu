@@ -15,7 +15,7 @@
 // sequence adds them up by warps, each a run of 16-byte packs; the run that holds the draw is cut
 // into runs again, one for each warp of its block, until one warp finds the token (the second look
 // at a run comes from L2). Bound: for a batch the issue of instructions (about ten an entry) and, in the end, the steps that
-// find the token: 29 us on the device for 256 sequences of 100003 bf16 entries, of which 14 for the memory; for a few sequences
+// find the token: 24 us on the device for 256 sequences of 100003 bf16 entries, of which 14 for the memory; for a few sequences
 // the latency of these steps (8.6 us for one of 131072 f32 entries, 5.6 for one of 1000).
 #include <cooperative_groups.h>
 
@@ -207,7 +207,7 @@ __device__ __forceinline__ int part_of(const double* sums, int n, double draw, d
 }
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == kMany ? kManyPerSm : 1) verify_kernel(const Args g) {
+__global__ void __launch_bounds__(THREADS, THREADS == kMany ? kManyPerSm : 2) verify_kernel(const Args g) {
   constexpr int kWarps = THREADS / 32;
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
@@ -350,12 +350,11 @@ int launch_one(const Args& g, int64_t batch, int size, cudaStream_t s) {
 
 template <typename T>
 int launch(const Args& g, int64_t batch, cudaStream_t s) {
-  // Blocks of a sequence: a power of 2, none for less than 2048 entries. Up to a sequence an SM: large blocks, 128 at most, as
-  // clusters of 8 do not fill every SM. More: small ones, whose number the SMs share out more evenly (four each of 256
-  // sequences, 1024 blocks where 1036 fit). On the device, large and small: 8.6 and 11.1 us for 1 x 131072 f32, 8.3 and 8.0
-  // for 32 x 32000 f32, 15.8 and 20.4 for 128 x 100003 bf16; 18 x 100003 13.9 with clusters of 8 large blocks (which run one
-  // part after the other), 10.5 with 8 small ones.
-  const bool few = batch <= kSms;
+  // Blocks of a sequence: a power of 2, none for less than 2048 entries. Up to two sequences an SM: large blocks, of which an SM
+  // holds two, 128 at most in clusters, as clusters of 8 do not fill every SM. More sequences: small ones, whose number the SMs
+  // share out more evenly. On the device, large and small: 8.6 and 11.1 us for 1 x 131072 f32, 16 and 20 for 128 x 100003 bf16,
+  // 24 and 29 for 256 x 100003, 41 and 37 for 320 x 100003, 53 and 33 for 1000 x 20000 f32, 39 and 14 for 2000 x 1000.
+  const bool few = batch <= 2 * kSms;
   const int64_t slots = few ? 128 : kSms * kManyPerSm;
   int size = 1;
   while (size < kMaxCluster && batch * size * 2 <= slots && g.vocab / (size * 2) >= 2048) size *= 2;
