@@ -52,6 +52,7 @@ _COMPRESS = {
     "signed_abs_softmax": _lib.JK_SIGNED_ABS_SOFTMAX,
 }
 _MAX_WRITE = 64  # pairs of one jk_cache_write
+_MAX_POOLS = 512
 _INT32 = torch.int32
 # bytes by sizes, which a loop asks for again and again
 _propagation_workspace = functools.lru_cache(maxsize=4096)(_LIBRARY.jk_cached_propagation_workspace)
@@ -146,6 +147,8 @@ class _Pools:
         if len(set(data)) != len(data) and any(t.numel() for t in tensors):
             raise ValueError("a pool is given twice")
         n = len(data)
+        if n > _MAX_POOLS:
+            raise ValueError(f"{n} pools, at most {_MAX_POOLS} are supported")
         self.tensors, self.arrays = tensors, array.array("q", data + sizes + strides)
         at = _at(self.arrays)
         self.words = array.array("q", (at, at + 8 * n, at + 16 * n, n))
@@ -281,7 +284,7 @@ def cache_reserve_(pools: Union[Tensor, Sequence[Tensor]], table: Tensor, length
     """Makes room for counts[b] more nodes in every sequence, in the order of the sequences: free
     pages, lowest first, enter the table, and lengths grow. A sequence that grows inside a page that
     others hold too first gets a copy of it in every pool (all pools whose pages the table names: keys,
-    values and states of every layer).
+    values and states of every layer, 512 at most).
 
     counts int32 [batch]. Returns added int32 [batch]: counts[b], or 0 for a sequence that is left
     as it is because its count is negative, its row of the table is too short, or the pages ran out (from
