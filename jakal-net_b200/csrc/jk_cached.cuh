@@ -27,8 +27,9 @@
 // lanes; a matrix transpose within the warp turns it. Weights go into the second product as two planes,
 // high + low, so their rounding (2^-16 and less) is far below that of the result.
 // f32: the same walk with fused multiply-adds, which keep f32's rounding.
-// Exponentials are base 2 on a reference that is itself rounded, so partial sums with different
-// references join without a rounding of their own.
+// Exponentials are base 2. A reference is one of the scores seen, in their own units, and what is taken
+// from a score is exact for scores near it: the largest has a weight of 1 at any magnitude (a product
+// of score and scale would be rounded by more than an exponent has range from scores of 1e9 on).
 //
 // What is not seen has no part in a result, whatever it holds: places past the last node and places
 // without a page arrive as zeros, and a tile of which rows see different parts (the newest nodes of a
@@ -58,7 +59,7 @@ constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
 // device so, 17.7 and 8.4 split; of 1024 places 21.2 and 18.3, 17.6 and 8.5).
 constexpr int kUnitTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.0f;          // by which a score may pass its row's reference, in units of log 2
+constexpr float kSlack = 8.0f;          // by which a score may pass its row's reference, as a power of 2
 
 struct Args {
   const char *query, *keys, *values, *states;  // states null: none
@@ -69,7 +70,7 @@ struct Args {
   int32_t batch, new_nodes, heads, kv_heads, group, rank, dim;
   uint32_t page_size;
   int32_t window, compress;
-  float scale, bias;
+  float scale, bias;                           // softmax: the unit of a score's distance from its reference, above 0
   char *out_value, *out_state;
   // layout
   int32_t blocks, row_blocks, rows;       // blocks of the grid; row blocks of a unit's rows, and rows of one
@@ -82,6 +83,7 @@ struct Args {
   float* parts;                           // [blocks][2][rows][part_row]
   int32_t units;
   bool split, tiled;
+  bool negate;                            // the query, so that the softmax's unit is above 0
   bool whole_runs;                        // a block's run is of one unit: units are few, so that what is left empty is little
 };
 
@@ -188,15 +190,24 @@ __device__ __forceinline__ float power2(float x) {
   return r;
 }
 
-// What a product becomes: for the softmax nothing yet (its scale has log2(e) in it), else the score.
+// What a product becomes: for the softmax nothing yet (its scale is in the unit), else the score.
 template <int COMPRESS>
 __device__ __forceinline__ float score_of(float dot, float scale, float bias) {
   return COMPRESS == JK_SOFTMAX ? dot : fmaf(dot, scale, bias);
 }
-// Its level above the reference, in units of log 2.
+// What is compared with the reference.
 template <int COMPRESS>
-__device__ __forceinline__ float level_of(float s, float scale, float ref) {
-  return COMPRESS == JK_SOFTMAX ? fmaf(s, scale, -ref) : fmaf(fabsf(s), kLog2e, -ref);
+__device__ __forceinline__ float height_of(float s) {
+  return COMPRESS == JK_SOFTMAX ? s : fabsf(s);
+}
+// Its level above the reference, as a power of 2.
+template <int COMPRESS>
+__device__ __forceinline__ float level_of(float s, float unit, float ref) {
+  return (height_of<COMPRESS>(s) - ref) * unit;
+}
+// What sums on the reference `from` have to be multiplied by to be on `to`, the higher of the two and not -inf.
+__device__ __forceinline__ float factor_of(float from, float to, float unit) {
+  return power2((from - to) * unit);
 }
 // Its part of the sum (softsign: the weight itself).
 template <int COMPRESS>
@@ -308,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   constexpr int OWN = kWide ? (ROWS + 1) / 2 : 2 * NT;
   constexpr int SIZE = sizeof(T);
   constexpr int COLUMN = 128 / SIZE;                   // elements of a 128-byte column
+  const float rate = COMPRESS == JK_SOFTMAX ? a.scale : kLog2e;
   extern __shared__ char memory_[];
   __shared__ int32_t before[kMaxBatch + 1];
   __shared__ int32_t scan[kWarps];
@@ -508,12 +520,16 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       if (i < 0) continue;
       if (i == 0) {
         // ---- queries, and the keys' columns that no copy fills: 0
+        using Bits = std::conditional_t<kWide, uint32_t, uint16_t>;
+        Bits* const query = reinterpret_cast<Bits*>(memory + a.ring_bytes);
+        const Bits flip = a.negate ? Bits(1) << (8 * SIZE - 1) : 0;
         for (int r = warp; r < ROWS; r += kWarps) {
           const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
           const bool counts = r < rows && t < span.n;
-          const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
+          const Bits* from = reinterpret_cast<const Bits*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
           // (f32: columns first)
-      for (int c = lane; c < a.key_cols; c += 32) query[kWide ? c * ROWS + r : r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
+          for (int c = lane; c < a.key_cols; c += 32)
+            query[kWide ? c * ROWS + r : r * a.query_row + c] = (counts && c < a.rank ? from[c] : Bits(0)) ^ flip;
         }
         if (!TILED && a.key_cols > a.rank) {
           for (int i = lane; i < a.stages * kKeys; i += 32) {
@@ -602,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               c[n][e] = score_of<COMPRESS>(NT == 1 ? c[n][e] + c2[e] : c[n][e], a.scale, a.bias);
               sees[n][e] = FULL || (((there >> p) & 1) && k0 + p < row_end[i2] && k0 + p >= row_low[i2]);
               any[i2] |= sees[n][e];
-              level[n][e] = level_of<COMPRESS>(c[n][e], a.scale, base[i2]);
+              level[n][e] = level_of<COMPRESS>(c[n][e], rate, base[i2]);
               highest = fmaxf(highest, sees[n][e] ? level[n][e] : -INFINITY);
             }
           if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, unset || highest > kSlack)) {
@@ -610,19 +626,19 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
             for (int i2 = 0; i2 < OWN; ++i2) {
               const int n = i2 >> 1, e = i2 & 1;
-              float top = sees[n][e] ? level[n][e] + base[i2] : -INFINITY;
-              if (sees[n][e + 2]) top = fmaxf(top, level[n][e + 2] + base[i2]);
+              float top = sees[n][e] ? height_of<COMPRESS>(c[n][e]) : -INFINITY;
+              if (sees[n][e + 2]) top = fmaxf(top, height_of<COMPRESS>(c[n][e + 2]));
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               top = fmaxf(top, ref[i2]);
-              const float factor = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
+              const float factor = top == -INFINITY ? 1.0f : factor_of(ref[i2], top, rate);
               ref[i2] = top;
               base[i2] = top == -INFINITY ? 0.0f : top;
               unset |= top == -INFINITY;
               sum[i2] *= factor;
               state[i2] *= factor;
-              level[n][e] = level_of<COMPRESS>(c[n][e], a.scale, base[i2]);
-              level[n][e + 2] = level_of<COMPRESS>(c[n][e + 2], a.scale, base[i2]);
+              level[n][e] = level_of<COMPRESS>(c[n][e], rate, base[i2]);
+              level[n][e + 2] = level_of<COMPRESS>(c[n][e + 2], rate, base[i2]);
 #pragma unroll
               for (int m = 0; m < MT; ++m) out[m][4 * n + e] *= factor, out[m][4 * n + e + 2] *= factor;
             }
@@ -740,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           score[i2] = score_of<COMPRESS>(i2 % 2 == 0 ? two.x : two.y, a.scale, a.bias);
           sees[i2] = full || (((there >> place) & 1) && k0 + place < row_end[i2] && k0 + place >= row_low[i2]);
           any[i2] |= sees[i2];
-          level[i2] = level_of<COMPRESS>(score[i2], a.scale, base[i2]);
+          level[i2] = level_of<COMPRESS>(score[i2], rate, base[i2]);
           higher |= sees[i2] && level[i2] > kSlack;
         }
         if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
@@ -748,17 +764,17 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           unset = false;
 #pragma unroll
           for (int i2 = 0; i2 < OWN; ++i2) {
-            float top = sees[i2] ? level[i2] + base[i2] : -INFINITY;
+            float top = sees[i2] ? height_of<COMPRESS>(score[i2]) : -INFINITY;
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             top = fmaxf(top, ref[i2]);
-            factor[i2] = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
+            factor[i2] = top == -INFINITY ? 1.0f : factor_of(ref[i2], top, rate);
             ref[i2] = top;
             base[i2] = top == -INFINITY ? 0.0f : top;
             unset |= top == -INFINITY;
             sum[i2] *= factor[i2];
             state[i2] *= factor[i2];
-            level[i2] = level_of<COMPRESS>(score[i2], a.scale, base[i2]);
+            level[i2] = level_of<COMPRESS>(score[i2], rate, base[i2]);
           }
           unset = __any_sync(0xffffffffu, unset);
 #pragma unroll
@@ -880,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const bool none = top != -INFINITY && ref_s[w][r] == -INFINITY;  // a warp that saw nothing, or only -inf
-        f[w] = top == -INFINITY ? 1.0f : power2(ref_s[w][r] - top);
+        f[w] = top == -INFINITY ? 1.0f : factor_of(ref_s[w][r], top, rate);
         if (!none) all = fmaf(sum_s[w][r], f[w], all), st = fmaf(state_s[w][r], f[w], st);
       }
       float norm = 1.0f;
@@ -914,6 +930,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 // Joins the parts of a unit's row that several blocks left, 128 columns a block; a unit without tiles has zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
+  const float rate = a.compress == JK_SOFTMAX ? a.scale : kLog2e;
   __shared__ int32_t counted[8][2];
   __shared__ float words_s[8][3];
   __shared__ __align__(16) float columns[8][128];
@@ -988,7 +1005,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     for (int i = 0; i < 4; ++i) {
       const float higher = fmaxf(top, w[i].x);
       const bool none = higher == -INFINITY;
-      const float f = none ? 1.0f : power2(top - higher), h = none ? 1.0f : power2(w[i].x - higher);
+      const float f = none ? 1.0f : factor_of(top, higher, rate), h = none ? 1.0f : factor_of(w[i].x, higher, rate);
       // a part of scores of -inf alone has a NaN for its sum, which counts only where there is nothing else
       const float s0 = !none && top == -INFINITY ? 0.0f : all * f, s1 = !none && w[i].x == -INFINITY ? 0.0f : w[i].y * h;
       all = s0 + s1;
@@ -1007,7 +1024,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   all = st = 0.0f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
-    const float ref = words_s[w][0], f = top == -INFINITY ? 1.0f : power2(ref - top);
+    const float ref = words_s[w][0], f = top == -INFINITY ? 1.0f : factor_of(ref, top, rate);
     if (top == -INFINITY || ref != -INFINITY) all = fmaf(words_s[w][1], f, all), st = fmaf(words_s[w][2], f, st);
     if (tid < 128) y = fmaf(columns[w][tid], f, y);
   }
