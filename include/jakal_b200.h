@@ -557,8 +557,9 @@ int64_t jk_cached_propagation_workspace(int64_t batch, int64_t new_nodes, int64_
  *   out_value[b, t, h] = sum_j w_j values[j],  out_state[b, t, h] = sum_j w_j states[j]
  * with compress JK_SOFTMAX, JK_SOFTSIGN or JK_SIGNED_ABS_SOFTMAX. A node that sees none, and nodes
  * t >= n, have zeros; a softmax over scores that are all -inf is NaN. What places that are not
- * seen hold (NaN, infinities) has no part in a result. Sums are f32; 16-bit weights go into the value
- * product as two planes (16 significant bits and more).
+ * seen hold (NaN, infinities) has no part in a result. Sums are f32, before they are divided by the
+ * weights' sum. 16-bit weights go into the value product as two planes, rounded by at most 2^-16 of a
+ * weight, in f16 at least 2^-32 of the largest (softsign: 2^-40).
  * rank <= 256, dim <= 512, new_nodes <= 64, heads a multiple of kv_heads. */
 int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* nodes, float scale, float score_bias,
                           jk_stream_t stream);

@@ -25,7 +25,9 @@
 // columns (sums) as their 16 rows, and the unit's rows as their 8 columns, of which one node of one head
 // fills one: S^T = K Q^T, O^T = V^T W^T. W^T leaves the first product with places across the wrong
 // lanes; a matrix transpose within the warp turns it. Weights go into the second product as two planes,
-// high + low, so their rounding (2^-16 and less) is far below that of the result.
+// high + low, so their rounding (2^-16 and less) is far below that of the result. f16 has few exponents
+// for that, so its weights are 2^7 times as large (softmaxes, whose weights are 2^8 at most then 2^15) or 2^15
+// (softsign, below 1), and what they leave is below 2^-32 of a weight of 1 on the reference, or 2^-40.
 // f32: the same walk with fused multiply-adds, which keep f32's rounding.
 // Exponentials are base 2. A reference is one of the scores seen, in their own units, and what is taken
 // from a score is exact for scores near it: the largest has a weight of 1 at any magnitude (a product
@@ -200,19 +202,26 @@ template <int COMPRESS>
 __device__ __forceinline__ float height_of(float s) {
   return COMPRESS == JK_SOFTMAX ? s : fabsf(s);
 }
+// The power of 2 that all weights are multiplied by, in the sums too.
+template <typename T, int COMPRESS>
+constexpr float kUp = !std::is_same_v<T, __half> ? 0.0f : COMPRESS == JK_SOFTSIGN ? 15.0f : 7.0f;
+constexpr float kSoftsignDown = 1.0f / 32768.0f;  // f16: what takes it out of the softsign's (the softmaxes' sum has it too)
+
 // Its level above the reference, as a power of 2.
-template <int COMPRESS>
+template <typename T, int COMPRESS>
 __device__ __forceinline__ float level_of(float s, float unit, float ref) {
-  return (height_of<COMPRESS>(s) - ref) * unit;
+  return kUp<T, COMPRESS> == 0.0f ? (height_of<COMPRESS>(s) - ref) * unit : fmaf(height_of<COMPRESS>(s) - ref, unit, kUp<T, COMPRESS>);
 }
 // What sums on the reference `from` have to be multiplied by to be on `to`, the higher of the two and not -inf.
 __device__ __forceinline__ float factor_of(float from, float to, float unit) {
   return power2((from - to) * unit);
 }
 // Its part of the sum (softsign: the weight itself).
-template <int COMPRESS>
+template <typename T, int COMPRESS>
 __device__ __forceinline__ float mass_of(float s, float level) {
-  return COMPRESS == JK_SOFTSIGN ? s / (1.0f + fabsf(s)) : power2(level);
+  if (COMPRESS != JK_SOFTSIGN) return power2(level);
+  const float w = s / (1.0f + fabsf(s));
+  return kUp<T, COMPRESS> == 0.0f ? w : w * (1.0f / kSoftsignDown);
 }
 // Its weight.
 template <int COMPRESS>
@@ -618,10 +627,10 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               c[n][e] = score_of<COMPRESS>(NT == 1 ? c[n][e] + c2[e] : c[n][e], a.scale, a.bias);
               sees[n][e] = FULL || (((there >> p) & 1) && k0 + p < row_end[i2] && k0 + p >= row_low[i2]);
               any[i2] |= sees[n][e];
-              level[n][e] = level_of<COMPRESS>(c[n][e], rate, base[i2]);
+              level[n][e] = level_of<T, COMPRESS>(c[n][e], rate, base[i2]);
               highest = fmaxf(highest, sees[n][e] ? level[n][e] : -INFINITY);
             }
-          if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, unset || highest > kSlack)) {
+          if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, unset || highest > kSlack + kUp<T, COMPRESS>)) {
             unset = false;
 #pragma unroll
             for (int i2 = 0; i2 < OWN; ++i2) {
@@ -637,8 +646,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               unset |= top == -INFINITY;
               sum[i2] *= factor;
               state[i2] *= factor;
-              level[n][e] = level_of<COMPRESS>(c[n][e], rate, base[i2]);
-              level[n][e + 2] = level_of<COMPRESS>(c[n][e + 2], rate, base[i2]);
+              level[n][e] = level_of<T, COMPRESS>(c[n][e], rate, base[i2]);
+              level[n][e + 2] = level_of<T, COMPRESS>(c[n][e + 2], rate, base[i2]);
 #pragma unroll
               for (int m = 0; m < MT; ++m) out[m][4 * n + e] *= factor, out[m][4 * n + e + 2] *= factor;
             }
@@ -649,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int i2 = 2 * n + (e & 1);
-              float w = mass_of<COMPRESS>(c[n][e], level[n][e]);
+              float w = mass_of<T, COMPRESS>(c[n][e], level[n][e]);
               if (!FULL && !sees[n][e]) w = 0.0f;
               if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
               w = weight_of<COMPRESS>(c[n][e], w);
@@ -756,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           score[i2] = score_of<COMPRESS>(i2 % 2 == 0 ? two.x : two.y, a.scale, a.bias);
           sees[i2] = full || (((there >> place) & 1) && k0 + place < row_end[i2] && k0 + place >= row_low[i2]);
           any[i2] |= sees[i2];
-          level[i2] = level_of<COMPRESS>(score[i2], rate, base[i2]);
-          higher |= sees[i2] && level[i2] > kSlack;
+          level[i2] = level_of<T, COMPRESS>(score[i2], rate, base[i2]);
+          higher |= sees[i2] && level[i2] > kSlack;  // (kUp is 0)
         }
         if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
           float factor[OWN];
@@ -774,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
             unset |= top == -INFINITY;
             sum[i2] *= factor[i2];
             state[i2] *= factor[i2];
-            level[i2] = level_of<COMPRESS>(score[i2], rate, base[i2]);
+            level[i2] = level_of<T, COMPRESS>(score[i2], rate, base[i2]);
           }
           unset = __any_sync(0xffffffffu, unset);
 #pragma unroll
@@ -786,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         }
 #pragma unroll
         for (int i2 = 0; i2 < OWN; ++i2) {
-          float w = mass_of<COMPRESS>(score[i2], level[i2]);
+          float w = mass_of<T, COMPRESS>(score[i2], level[i2]);
           w = sees[i2] ? w : 0.0f;
           if (COMPRESS != JK_SOFTSIGN) sum[i2] += w;
           w = sees[i2] ? weight_of<COMPRESS>(score[i2], w) : 0.0f;
@@ -899,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         f[w] = top == -INFINITY ? 1.0f : factor_of(ref_s[w][r], top, rate);
         if (!none) all = fmaf(sum_s[w][r], f[w], all), st = fmaf(state_s[w][r], f[w], st);
       }
-      float norm = 1.0f;
+      float norm = std::is_same_v<T, __half> ? kSoftsignDown : 1.0f;
       if (whole && COMPRESS != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
       const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
       const int64_t row = (int64_t(b) * a.new_nodes + t) * a.heads + kv * a.group + g;
@@ -1028,7 +1037,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     if (top == -INFINITY || ref != -INFINITY) all = fmaf(words_s[w][1], f, all), st = fmaf(words_s[w][2], f, st);
     if (tid < 128) y = fmaf(columns[w][tid], f, y);
   }
-  float norm = 1.0f;
+  float norm = std::is_same_v<T, __half> ? kSoftsignDown : 1.0f;
   if (a.compress != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
   const bool zero = t >= span.n || (top == -INFINITY && norm == 0.0f);
   if (tid < 128 && d0 + tid < a.dim) out[tid] = from_f32<T>(zero ? 0.0f : y * norm);

@@ -62,3 +62,79 @@ def test_scores_of_any_magnitude(jk, dtype, page, heads, compress, scale):
         state, value = jk.cached_propagation(**p, compress=compress, scale=scale)
         for got, w in ((value, torch.stack(want)[:, None, None]), (state, torch.stack(want_state)[:, None, None])):
             assert ((got.double() - w).abs() <= ROUND[dtype] * w.abs() + 2.0 ** -25).all()
+
+
+def one_sequence(dtype, keys, values, query, page, new=1, lengths=None):
+    """A cache of one sequence, its pages in order: keys [n, rank], values [n, dim], whose first column is the states'."""
+    n, columns = keys.shape[0], -(-keys.shape[0] // page)
+
+    def paged(x):
+        out = torch.full((columns * page, *x.shape[1:]), math.nan, dtype=dtype, device="cuda")
+        out[:n] = x.to(dtype)
+        return out.view(columns, 1, page, *x.shape[1:])
+
+    return dict(query=query.to(dtype).cuda().view(1, new, 1, -1), key_pages=paged(keys), value_pages=paged(values), state_pages=paged(values[:, 0]),
+                table=torch.arange(columns, dtype=torch.int32, device="cuda")[None], lengths=torch.tensor([n], dtype=torch.int32, device="cuda"))
+
+
+def additions(n):
+    """Of a sum's chain at most: a block's run of 64 places' turns of two planes of 16 (148 SMs and more share the places
+    from 513 on), the join of four warps, and that of eight times 56 parts."""
+    return (-(-n // 64) if n <= 512 else -(-n // (64 * 148)) + 1) * 32 + 4 + 56 + 8
+
+
+def close(got, weights, slack, values):
+    """got [dim] is sum_j weights[j] values[j], each weight off by `slack` [n] and by the sum's rounding."""
+    n, dtype = weights.numel(), got.dtype
+    want = (weights[:, None] * values).sum(0)
+    off = ((slack + additions(n) * 2.0 ** -23 * weights.abs())[:, None] * values.abs()).sum(0)
+    off = off + ROUND[dtype] * (want.abs() + off) + (2.0 ** -25 if dtype == F16 else 2.0 ** -140)
+    d = (got.double().cpu() - want).abs()
+    assert (d <= off).all(), f"off by {(d / off).max():.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("n", [64, 500, 5000])
+@pytest.mark.parametrize("scale", [1e-4, 1e-5, 1e-6, 1e-7, 1e-8])
+def test_softsign_of_small_scores(jk, dtype, page, n, scale):
+    """Scores of one size, so that the roundings of their weights have one sign. A score's sum errs by 2^-24 a term
+    and a product's rounding, the softsign by three more, the two planes by 2^-16, and in f16 by 2^-40."""
+    g = torch.Generator().manual_seed(n)
+    keys = torch.full((n, 4), 0.25)
+    keys[::7] = 0.5
+    values = 64 * (1 + torch.rand(n, 24, generator=g))
+    p = one_sequence(dtype, keys, values, torch.full((4,), 1.0), page)
+    state, value = jk.cached_propagation(**p, compress="softsign", scale=scale)
+    s = keys.double().sum(1) * float(torch.tensor(scale, dtype=torch.float32))
+    w = s / (1 + s)
+    slack = w * (8 * 2.0 ** -24 + (0.0 if dtype == torch.float32 else 2.0 ** -16)) + (2.0 ** -40 if dtype == F16 else 0.0)
+    v = values.to(dtype).double()
+    close(value[0, 0, 0], w, slack, v)
+    close(state[0, 0, 0, None], w, slack, v[:, :1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("n", [400, 32768, 262144])
+@pytest.mark.parametrize("compress", ["softmax", "signed_abs_softmax"])
+@pytest.mark.parametrize("above", [9.25, 17.375, 18.5])
+def test_one_high_score_and_a_long_tail(jk, dtype, page, n, compress, above):
+    """One node far above all others, which are alike and have a large part of the result together. Scores are exact; a
+    distance from the reference is rounded twice (2^-24 of 27 powers of 2), an exponential by 2^-22, factors of joins the same,
+    the two planes by 2^-16, and in f16 by 2^-32 of the weight on the reference, which is the highest node's."""
+    for top in (0, n // 2, n - 1):
+        keys = torch.zeros(n, 4)
+        keys[:, 0] = -above if compress == "softmax" else 0.5
+        keys[top, 0] = 0.0 if compress == "softmax" else above + 0.5
+        g = torch.Generator().manual_seed(n)
+        values = 1 + torch.rand(n, 24, generator=g)
+        values[top] = 0.5
+        p = one_sequence(dtype, keys, values, torch.tensor([1.0, 0.0, 0.0, 0.0]), page)
+        state, value = jk.cached_propagation(**p, compress=compress)
+        w = keys[:, 0].double().softmax(0)
+        slack = w * (2 * (2 * 27 * 2.0 ** -24 * 0.7 + 4 * 2.0 ** -22) + (0.0 if dtype == torch.float32 else 2.0 ** -16))
+        slack = slack + (2.0 ** -32 if dtype == F16 else 0.0)
+        v = values.to(dtype).double()
+        close(value[0, 0, 0], w, slack, v)
+        close(state[0, 0, 0, None], w, slack, v[:, :1])
