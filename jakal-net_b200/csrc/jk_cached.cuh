@@ -81,7 +81,7 @@ struct Args {
   int32_t query_row;                      // elements from one query to the next in shared memory
   int32_t key_bytes, stage_bytes, stages; // of a ring: keys of a stage, a stage, their number
   int32_t ring_bytes;                     // of all rings (and of what is joined in their place)
-  int32_t part_row;                       // floats of a row that a block leaves: dim rounded up to 4, reference, sum, state
+  int32_t part_row;                       // floats of a row that a block leaves: dim rounded up to 4, reference, sum, state, whether it saw any
   float* parts;                           // [blocks][2][rows][part_row]
   int32_t units;
   bool split, tiled;
@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   __shared__ int32_t before[kMaxBatch + 1];
   __shared__ int32_t scan[kWarps];
   __shared__ float ref_s[kWarps][ROWS], sum_s[kWarps][ROWS], state_s[kWarps][ROWS];
+  __shared__ bool seen_s[kWarps][ROWS];
   __shared__ uint64_t landed[kWarps][kMaxStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int fill = 0, take = 0;          // TILED: the stage that the next turn fills, and the one that is taken next, of all units
@@ -850,15 +851,12 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     // ---- the warps' sums, then the block's
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      bool seen = any[i];
 #pragma unroll
       for (int o = kWide ? 1 : 4; o < (kWide ? 16 : 32); o <<= 1) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
         state[i] += __shfl_xor_sync(0xffffffffu, state[i], o);
-        seen |= __shfl_xor_sync(0xffffffffu, int(seen), o) != 0;
+        any[i] |= __shfl_xor_sync(0xffffffffu, int(any[i]), o) != 0;
       }
-      // scores that are all -inf: their softmax is NaN, unlike that of no score at all
-      if (seen && ref[i] == -INFINITY) sum[i] = NAN;
     }
     __syncthreads();  // the rings are drained
     constexpr int kJoinRow = DIM + 4;
@@ -866,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
         const int r = (i >> 1) * 8 + 2 * (lane & 3) + (i & 1);
-        if (lane < 4) ref_s[warp][r] = ref[i], sum_s[warp][r] = sum[i], state_s[warp][r] = state[i];
+        if (lane < 4) ref_s[warp][r] = ref[i], sum_s[warp][r] = sum[i], state_s[warp][r] = state[i], seen_s[warp][r] = any[i];
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -882,7 +880,10 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     } else {
 #pragma unroll
       for (int i = 0; i < OWN; ++i)
-        if ((lane & 15) == 0) ref_s[warp][own_row + i] = ref[i], sum_s[warp][own_row + i] = sum[i], state_s[warp][own_row + i] = state[i];
+        if ((lane & 15) == 0) {
+          const int r = own_row + i;
+          ref_s[warp][r] = ref[i], sum_s[warp][r] = sum[i], state_s[warp][r] = state[i], seen_s[warp][r] = any[i];
+        }
 #pragma unroll
       for (int r = 0; r < ROWS; ++r)
 #pragma unroll
@@ -901,18 +902,22 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       float top = ref_s[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ref_s[w][r]);
+      // A reference of -inf: nothing seen, or scores of -inf and NaN alone. Its factor is 0, which leaves a sum of 0 out and keeps NaN.
       float f[kWarps], all = 0.0f, st = 0.0f;
+      bool seen = false;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const bool none = top != -INFINITY && ref_s[w][r] == -INFINITY;  // a warp that saw nothing, or only -inf
         f[w] = top == -INFINITY ? 1.0f : factor_of(ref_s[w][r], top, rate);
-        if (!none) all = fmaf(sum_s[w][r], f[w], all), st = fmaf(state_s[w][r], f[w], st);
+        all = fmaf(sum_s[w][r], f[w], all), st = fmaf(state_s[w][r], f[w], st);
+        seen |= seen_s[w][r];
       }
+      // a softmax of scores that are all -inf is NaN, unlike that of no score at all
+      const bool none = top == -INFINITY && !seen;
       float norm = std::is_same_v<T, __half> ? kSoftsignDown : 1.0f;
-      if (whole && COMPRESS != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
+      if (whole && COMPRESS != JK_SOFTSIGN) norm = top == -INFINITY ? NAN : 1.0f / all;
       const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
       const int64_t row = (int64_t(b) * a.new_nodes + t) * a.heads + kv * a.group + g;
-      const bool zero = whole && (t >= span.n || (top == -INFINITY && norm == 0.0f));
+      const bool zero = whole && (t >= span.n || none);
       for (int d = lane_of; d < a.dim; d += step) {
         float x = 0.0f;
 #pragma unroll
@@ -923,7 +928,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       if (lane_of == 0) {
         if (!whole) {
           float* words = part + r * a.part_row + a.part_row - 4;
-          words[0] = top, words[1] = all, words[2] = st;
+          words[0] = top, words[1] = all, words[2] = st, words[3] = none ? 0.0f : 1.0f;
         } else if (a.out_state != nullptr) {
           reinterpret_cast<T*>(a.out_state)[row] = from_f32<T>(zero ? 0.0f : st * norm);
         }
@@ -941,7 +946,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
   const float rate = a.compress == JK_SOFTMAX ? a.scale : kLog2e;
   __shared__ int32_t counted[8][2];
-  __shared__ float words_s[8][3];
+  __shared__ float words_s[8][4];
   __shared__ __align__(16) float columns[8][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t unit_rows = a.group * a.new_nodes, slices = (a.dim + 127) / 128;
@@ -995,7 +1000,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   // a warp has every eighth part, a lane four columns
   const int32_t words = a.part_row - 4;
   const bool has = d0 + 4 * lane < words;
-  float top = -INFINITY, all = 0.0f, st = 0.0f;
+  float top = -INFINITY, all = 0.0f, st = 0.0f, seen = 0.0f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int32_t block = first + warp; block <= last; block += 4 * 8) {
     float4 v[4], w[4];
@@ -1015,15 +1020,14 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
       const float higher = fmaxf(top, w[i].x);
       const bool none = higher == -INFINITY;
       const float f = none ? 1.0f : factor_of(top, higher, rate), h = none ? 1.0f : factor_of(w[i].x, higher, rate);
-      // a part of scores of -inf alone has a NaN for its sum, which counts only where there is nothing else
-      const float s0 = !none && top == -INFINITY ? 0.0f : all * f, s1 = !none && w[i].x == -INFINITY ? 0.0f : w[i].y * h;
-      all = s0 + s1;
+      all = fmaf(w[i].y, h, all * f);
       st = fmaf(w[i].z, h, st * f);
+      seen = fmaxf(seen, w[i].w);
       x.x = fmaf(v[i].x, h, x.x * f), x.y = fmaf(v[i].y, h, x.y * f), x.z = fmaf(v[i].z, h, x.z * f), x.w = fmaf(v[i].w, h, x.w * f);
       top = higher;
     }
   }
-  if (lane == 0) words_s[warp][0] = top, words_s[warp][1] = all, words_s[warp][2] = st;
+  if (lane == 0) words_s[warp][0] = top, words_s[warp][1] = all, words_s[warp][2] = st, words_s[warp][3] = seen;
   *reinterpret_cast<float4*>(&columns[warp][4 * lane]) = x;
   __syncthreads();
   top = -INFINITY;
@@ -1034,12 +1038,13 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
     const float ref = words_s[w][0], f = top == -INFINITY ? 1.0f : factor_of(ref, top, rate);
-    if (top == -INFINITY || ref != -INFINITY) all = fmaf(words_s[w][1], f, all), st = fmaf(words_s[w][2], f, st);
+    all = fmaf(words_s[w][1], f, all), st = fmaf(words_s[w][2], f, st);
+    seen = fmaxf(seen, words_s[w][3]);
     if (tid < 128) y = fmaf(columns[w][tid], f, y);
   }
   float norm = std::is_same_v<T, __half> ? kSoftsignDown : 1.0f;
-  if (a.compress != JK_SOFTSIGN) norm = top == -INFINITY ? (all != all ? NAN : 0.0f) : 1.0f / all;
-  const bool zero = t >= span.n || (top == -INFINITY && norm == 0.0f);
+  if (a.compress != JK_SOFTSIGN) norm = top == -INFINITY ? NAN : 1.0f / all;
+  const bool zero = t >= span.n || (top == -INFINITY && seen == 0.0f);
   if (tid < 128 && d0 + tid < a.dim) out[tid] = from_f32<T>(zero ? 0.0f : y * norm);
   if (first_slice) reinterpret_cast<T*>(a.out_state)[row] = from_f32<T>(zero ? 0.0f : st * norm);
 }

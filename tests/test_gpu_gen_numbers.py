@@ -138,3 +138,43 @@ def test_one_high_score_and_a_long_tail(jk, dtype, page, n, compress, above):
         v = values.to(dtype).double()
         close(value[0, 0, 0], w, slack, v)
         close(state[0, 0, 0, None], w, slack, v[:, :1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("heads", [1, 9])
+@pytest.mark.parametrize("compress", ["softmax", "softsign", "signed_abs_softmax"])
+@pytest.mark.parametrize("n,some,split", [(17, [16], False), (17, [0], False), (300, [299], False), (1, [0], False), (17, [16], True), (3000, [2999], True),
+                                          (3000, range(2944, 3000), True), (3000, range(0, 64), True), (3000, range(0, 3000), True), (100, range(64, 80), True)])
+def test_scores_that_are_none(jk, dtype, page, heads, compress, n, some, split):
+    """A score that is NaN makes value and state NaN, whoever sees it beside what else."""
+    p = problem(dtype, [n, 40], heads=heads, rank=16, dim=24, page=page, columns=-(-3000 // page) if split else None, states=True)
+    at, off = places(p, 0, n)
+    keep = p["key_pages"].clone()
+    p["key_pages"][at[list(some)], :, off[list(some)]] = math.nan
+    state, value = jk.cached_propagation(**p, compress=compress, scale=0.3)
+    assert value[0].isnan().all() and state[0].isnan().all()
+    assert value[1].isfinite().all() and state[1].isfinite().all()
+    # scores of -inf count for nothing beside others, and alone they make NaN too (softsign: everywhere, as -inf / inf)
+    p["key_pages"] = keep
+    p["query"][0] = 1.0
+    p["key_pages"][at[list(some)], :, off[list(some)]] = -math.inf
+    state, value = jk.cached_propagation(**p, compress=compress, scale=0.3)
+    if compress == "softmax" and len(some) < n:
+        assert value[0].isfinite().all() and state[0].isfinite().all()
+    else:
+        assert value[0].isnan().all() and state[0].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("group", [1, 9])
+def test_a_later_node_that_is_none_and_the_states(jk, dtype, page, group):
+    for lengths in ([5, 70, 130], [900, 64, 17]):
+        p = problem(dtype, lengths, new=5, heads=group, rank=16, dim=24, page=page, states=True)
+        for b, n in enumerate(lengths):
+            at, off = places(p, b, n)
+            p["key_pages"][at[-1], :, off[-1]] = math.nan
+        state, value = jk.cached_propagation(**p, scale=0.3)
+        assert value[:, :4].isfinite().all() and state[:, :4].isfinite().all()
+        assert value[:, 4].isnan().all() and state[:, 4].isnan().all()
