@@ -2,8 +2,6 @@
 // jk_cached.cuh, instantiated by type in jk_cached_{f32,bf16,f16}.cu.
 #include "jk_cached.cuh"
 
-#include <limits>
-
 namespace jk {
 namespace cached {
 namespace {
@@ -98,14 +96,8 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
   a.page_size = static_cast<uint32_t>(page_size);
   a.window = window;
   a.compress = static_cast<int32_t>(q->compress);
-  a.scale = scale, a.bias = score_bias;
-  if (a.compress == JK_SOFTMAX) {
-    // products are compared and subtracted, which a bias moves together; a scale below 0 is one above 0 of -query, and one of 0
-    // the least above it (of which a distance of -inf is -inf)
-    a.negate = scale < 0.0f;
-    a.scale = static_cast<float>((a.negate ? -double(scale) : double(scale)) * 1.4426950408889634);
-    if (a.scale == 0.0f) a.scale = std::numeric_limits<float>::denorm_min();
-  }
+  a.scale = a.compress == JK_SOFTMAX ? static_cast<float>(double(scale) * 1.4426950408889634) : scale;
+  a.bias = score_bias;
   a.key_piece = piece_of(q->keys, a.key_stride, rank * size), a.value_piece = piece_of(q->values, a.value_stride, dim * size);
   Maps maps{};
   Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, true);

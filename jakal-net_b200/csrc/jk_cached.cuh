@@ -29,9 +29,9 @@
 // for that, so its weights are 2^7 times as large (softmaxes, whose weights are 2^8 at most then 2^15) or 2^15
 // (softsign, below 1), and what they leave is below 2^-32 of a weight of 1 on the reference, or 2^-40.
 // f32: the same walk with fused multiply-adds, which keep f32's rounding.
-// Exponentials are base 2. A reference is one of the scores seen, in their own units, and what is taken
-// from a score is exact for scores near it: the largest has a weight of 1 at any magnitude (a product
-// of score and scale would be rounded by more than an exponent has range from scores of 1e9 on).
+// Exponentials are base 2, of one fused multiply-add: a score times a rate less a reference, which is such a
+// product rounded. From references of 2^24 on that rounding is a power of 2 and more (an exponent's whole range from 2^31 on), so
+// the product is rounded before the difference too, as the score itself has been.
 //
 // What is not seen has no part in a result, whatever it holds: places past the last node and places
 // without a page arrive as zeros, and a tile of which rows see different parts (the newest nodes of a
@@ -62,6 +62,7 @@ constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
 constexpr int kUnitTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;          // by which a score may pass its row's reference, as a power of 2
+constexpr float kFar = 16777216.0f;     // references from which a product with the rate is rounded before they are subtracted
 
 struct Args {
   const char *query, *keys, *values, *states;  // states null: none
@@ -72,7 +73,7 @@ struct Args {
   int32_t batch, new_nodes, heads, kv_heads, group, rank, dim;
   uint32_t page_size;
   int32_t window, compress;
-  float scale, bias;                           // softmax: the unit of a score's distance from its reference, above 0
+  float scale, bias;                           // softmax: the rate (its scale and log2(e)), which the bias has no part in
   char *out_value, *out_state;
   // layout
   int32_t blocks, row_blocks, rows;       // blocks of the grid; row blocks of a unit's rows, and rows of one
@@ -85,7 +86,6 @@ struct Args {
   float* parts;                           // [blocks][2][rows][part_row]
   int32_t units;
   bool split, tiled;
-  bool negate;                            // the query, so that the softmax's unit is above 0
   bool whole_runs;                        // a block's run is of one unit: units are few, so that what is left empty is little
 };
 
@@ -192,7 +192,7 @@ __device__ __forceinline__ float power2(float x) {
   return r;
 }
 
-// What a product becomes: for the softmax nothing yet (its scale is in the unit), else the score.
+// What a product becomes: for the softmax nothing yet (its scale is in the rate), else the score.
 template <int COMPRESS>
 __device__ __forceinline__ float score_of(float dot, float scale, float bias) {
   return COMPRESS == JK_SOFTMAX ? dot : fmaf(dot, scale, bias);
@@ -208,13 +208,13 @@ constexpr float kUp = !std::is_same_v<T, __half> ? 0.0f : COMPRESS == JK_SOFTSIG
 constexpr float kSoftsignDown = 1.0f / 32768.0f;  // f16: what takes it out of the softsign's (the softmaxes' sum has it too)
 
 // Its level above the reference, as a power of 2.
-template <typename T, int COMPRESS>
-__device__ __forceinline__ float level_of(float s, float unit, float ref) {
-  return kUp<T, COMPRESS> == 0.0f ? (height_of<COMPRESS>(s) - ref) * unit : fmaf(height_of<COMPRESS>(s) - ref, unit, kUp<T, COMPRESS>);
+template <int COMPRESS>
+__device__ __forceinline__ float level_of(float s, float rate, float ref) {
+  return fmaf(height_of<COMPRESS>(s), rate, -ref);
 }
-// What sums on the reference `from` have to be multiplied by to be on `to`, the higher of the two and not -inf.
-__device__ __forceinline__ float factor_of(float from, float to, float unit) {
-  return power2((from - to) * unit);
+template <int COMPRESS>
+__device__ __forceinline__ float far_level_of(float s, float rate, float ref) {
+  return __fsub_rn(__fmul_rn(height_of<COMPRESS>(s), rate), ref);
 }
 // Its part of the sum (softsign: the weight itself).
 template <typename T, int COMPRESS>
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       base[i] = sum[i] = state[i] = 0.0f;
       any[i] = false;
     }
-    bool unset = true;  // a row that counts has no reference yet
+    bool unset = true;  // a row that counts has no reference yet, or one of kFar and more, and is looked at in every turn
     float out[MT][NT * 4];
     uint64_t pairs[kWide ? ROWS : 1][CP];  // f32's sums
 #pragma unroll
@@ -530,16 +530,12 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       if (i < 0) continue;
       if (i == 0) {
         // ---- queries, and the keys' columns that no copy fills: 0
-        using Bits = std::conditional_t<kWide, uint32_t, uint16_t>;
-        Bits* const query = reinterpret_cast<Bits*>(memory + a.ring_bytes);
-        const Bits flip = a.negate ? Bits(1) << (8 * SIZE - 1) : 0;
         for (int r = warp; r < ROWS; r += kWarps) {
           const int t = (row0 + r) / a.group, g = (row0 + r) - t * a.group;
           const bool counts = r < rows && t < span.n;
-          const Bits* from = reinterpret_cast<const Bits*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
+          const T* from = reinterpret_cast<const T*>(a.query + b * a.query_stride[0] + t * a.query_stride[1] + (kv * a.group + g) * a.query_stride[2]);
           // (f32: columns first)
-          for (int c = lane; c < a.key_cols; c += 32)
-            query[kWide ? c * ROWS + r : r * a.query_row + c] = (counts && c < a.rank ? from[c] : Bits(0)) ^ flip;
+          for (int c = lane; c < a.key_cols; c += 32) query[kWide ? c * ROWS + r : r * a.query_row + c] = counts && c < a.rank ? from[c] : from_f32<T>(0.0f);
         }
         if (!TILED && a.key_cols > a.rank) {
           for (int i = lane; i < a.stages * kKeys; i += 32) {
@@ -628,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
               c[n][e] = score_of<COMPRESS>(NT == 1 ? c[n][e] + c2[e] : c[n][e], a.scale, a.bias);
               sees[n][e] = FULL || (((there >> p) & 1) && k0 + p < row_end[i2] && k0 + p >= row_low[i2]);
               any[i2] |= sees[n][e];
-              level[n][e] = level_of<T, COMPRESS>(c[n][e], rate, base[i2]);
+              level[n][e] = level_of<COMPRESS>(c[n][e], rate, base[i2]);
               highest = fmaxf(highest, sees[n][e] ? level[n][e] : -INFINITY);
             }
           if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, unset || highest > kSlack + kUp<T, COMPRESS>)) {
@@ -636,19 +632,21 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
             for (int i2 = 0; i2 < OWN; ++i2) {
               const int n = i2 >> 1, e = i2 & 1;
-              float top = sees[n][e] ? height_of<COMPRESS>(c[n][e]) : -INFINITY;
-              if (sees[n][e + 2]) top = fmaxf(top, height_of<COMPRESS>(c[n][e + 2]));
+              float top = sees[n][e] ? far_level_of<COMPRESS>(c[n][e], rate, kUp<T, COMPRESS>) : -INFINITY;
+              if (sees[n][e + 2]) top = fmaxf(top, far_level_of<COMPRESS>(c[n][e + 2], rate, kUp<T, COMPRESS>));
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               top = fmaxf(top, ref[i2]);
-              const float factor = top == -INFINITY ? 1.0f : factor_of(ref[i2], top, rate);
+              const float factor = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
               ref[i2] = top;
               base[i2] = top == -INFINITY ? 0.0f : top;
               unset |= top == -INFINITY;
               sum[i2] *= factor;
               state[i2] *= factor;
-              level[n][e] = level_of<T, COMPRESS>(c[n][e], rate, base[i2]);
-              level[n][e + 2] = level_of<T, COMPRESS>(c[n][e + 2], rate, base[i2]);
+              const bool away = fabsf(base[i2]) >= kFar;
+              unset |= away;
+              level[n][e] = away ? far_level_of<COMPRESS>(c[n][e], rate, base[i2]) : level_of<COMPRESS>(c[n][e], rate, base[i2]);
+              level[n][e + 2] = away ? far_level_of<COMPRESS>(c[n][e + 2], rate, base[i2]) : level_of<COMPRESS>(c[n][e + 2], rate, base[i2]);
 #pragma unroll
               for (int m = 0; m < MT; ++m) out[m][4 * n + e] *= factor, out[m][4 * n + e + 2] *= factor;
             }
@@ -766,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           score[i2] = score_of<COMPRESS>(i2 % 2 == 0 ? two.x : two.y, a.scale, a.bias);
           sees[i2] = full || (((there >> place) & 1) && k0 + place < row_end[i2] && k0 + place >= row_low[i2]);
           any[i2] |= sees[i2];
-          level[i2] = level_of<T, COMPRESS>(score[i2], rate, base[i2]);
+          level[i2] = level_of<COMPRESS>(score[i2], rate, base[i2]);
           higher |= sees[i2] && level[i2] > kSlack;  // (kUp is 0)
         }
         if (COMPRESS != JK_SOFTSIGN && __any_sync(0xffffffffu, higher)) {
@@ -774,17 +772,19 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           unset = false;
 #pragma unroll
           for (int i2 = 0; i2 < OWN; ++i2) {
-            float top = sees[i2] ? height_of<COMPRESS>(score[i2]) : -INFINITY;
+            float top = sees[i2] ? far_level_of<COMPRESS>(score[i2], rate, 0.0f) : -INFINITY;
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             top = fmaxf(top, ref[i2]);
-            factor[i2] = top == -INFINITY ? 1.0f : factor_of(ref[i2], top, rate);
+            factor[i2] = top == -INFINITY ? 1.0f : power2(ref[i2] - top);
             ref[i2] = top;
             base[i2] = top == -INFINITY ? 0.0f : top;
             unset |= top == -INFINITY;
             sum[i2] *= factor[i2];
             state[i2] *= factor[i2];
-            level[i2] = level_of<T, COMPRESS>(score[i2], rate, base[i2]);
+            const bool away = fabsf(base[i2]) >= kFar;
+            unset |= away;
+            level[i2] = away ? far_level_of<COMPRESS>(score[i2], rate, base[i2]) : level_of<COMPRESS>(score[i2], rate, base[i2]);
           }
           unset = __any_sync(0xffffffffu, unset);
 #pragma unroll
@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       bool seen = false;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        f[w] = top == -INFINITY ? 1.0f : factor_of(ref_s[w][r], top, rate);
+        f[w] = top == -INFINITY ? 1.0f : power2(ref_s[w][r] - top);
         all = fmaf(sum_s[w][r], f[w], all), st = fmaf(state_s[w][r], f[w], st);
         seen |= seen_s[w][r];
       }
@@ -944,7 +944,6 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 // Joins the parts of a unit's row that several blocks left, 128 columns a block; a unit without tiles has zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
-  const float rate = a.compress == JK_SOFTMAX ? a.scale : kLog2e;
   __shared__ int32_t counted[8][2];
   __shared__ float words_s[8][4];
   __shared__ __align__(16) float columns[8][128];
@@ -1019,7 +1018,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     for (int i = 0; i < 4; ++i) {
       const float higher = fmaxf(top, w[i].x);
       const bool none = higher == -INFINITY;
-      const float f = none ? 1.0f : factor_of(top, higher, rate), h = none ? 1.0f : factor_of(w[i].x, higher, rate);
+      const float f = none ? 1.0f : power2(top - higher), h = none ? 1.0f : power2(w[i].x - higher);
       all = fmaf(w[i].y, h, all * f);
       st = fmaf(w[i].z, h, st * f);
       seen = fmaxf(seen, w[i].w);
@@ -1037,7 +1036,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   all = st = 0.0f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
-    const float ref = words_s[w][0], f = top == -INFINITY ? 1.0f : factor_of(ref, top, rate);
+    const float ref = words_s[w][0], f = top == -INFINITY ? 1.0f : power2(ref - top);
     all = fmaf(words_s[w][1], f, all), st = fmaf(words_s[w][2], f, st);
     seen = fmaxf(seen, words_s[w][3]);
     if (tid < 128) y = fmaf(columns[w][tid], f, y);
