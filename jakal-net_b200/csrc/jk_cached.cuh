@@ -315,6 +315,43 @@ struct Maps {
   CUtensorMap keys, values;
 };
 
+// 16-bit types: an infinite value times a low plane that is 0 or of the other sign is NaN. A warp whose sums `joined` (a row every
+// `join_row` floats) have NaN adds up those rows again, place after place, with their weights in one piece; what is NaN then is so
+// by the formula. This is slow, and a function of its own, whose registers the loop does not pay for.
+template <typename T, int COMPRESS, bool TILED>
+__device__ __noinline__ void add_again(const Args& a, const T* query, const float* refs, float* joined, int join_row, int32_t b, int32_t kv,
+                                       int32_t row0, int32_t rows, int32_t key0, int32_t tiles) {
+  const int lane = threadIdx.x & 31;
+  const float rate = COMPRESS == JK_SOFTMAX ? a.scale : kLog2e;
+  const Span span = span_of<TILED>(a, b);
+  const int32_t* table = a.table + b * a.table_stride;
+  for (int32_t r = 0; r < rows; ++r, query += a.query_row, joined += join_row) {
+    const int32_t place = span.first + (row0 + r) / a.group;
+    bool none = false;
+    for (int d = lane; d < a.dim; d += 32) none |= joined[d] != joined[d];
+    if ((row0 + r) / a.group >= span.n || !__any_sync(0xffffffffu, none)) continue;
+    const float ref = refs[r] == -INFINITY ? 0.0f : refs[r];
+    const int32_t low = a.window < 0 || place < a.window || place - a.window < span.low ? span.low : place - a.window;
+    const int32_t end = place + 1 < span.end ? place + 1 : span.end;
+    for (int d = lane; d < a.dim; d += 32) joined[d] = 0.0f;
+    for (int32_t i = 0; i < tiles * kKeys; ++i) {
+      const int32_t j = key0 + i / kKeys * kTile + i % kKeys;
+      if (j < low || j >= end) continue;
+      const uint32_t column = static_cast<uint32_t>(j) / a.page_size, off = static_cast<uint32_t>(j) - column * a.page_size;
+      const int32_t page = table[column];
+      if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(a.pages)) continue;
+      const T* key = reinterpret_cast<const T*>(a.keys + kv * a.key_stride[1] + page * a.key_stride[0] + off * a.key_stride[2]);
+      const T* value = reinterpret_cast<const T*>(a.values + kv * a.value_stride[1] + page * a.value_stride[0] + off * a.value_stride[2]);
+      float dot = 0.0f;
+      for (int c = lane; c < a.rank; c += 32) dot = fmaf(to_f32(query[c]), to_f32(key[c]), dot);
+      const float score = score_of<COMPRESS>(warp_sum32(dot), a.scale, a.bias);
+      const float level = fabsf(ref) >= kFar ? far_level_of<COMPRESS>(score, rate, ref) : level_of<COMPRESS>(score, rate, ref);
+      const float w = weight_of<COMPRESS>(score, mass_of<T, COMPRESS>(score, level));
+      for (int d = lane; d < a.dim; d += 32) joined[d] = fmaf(w, to_f32(value[d]), joined[d]);
+    }
+  }
+}
+
 // ROWS: rows of a unit that a block takes (a multiple of 8 for 16-bit types); DIM: columns of the value at most.
 // TILED: pages hold a multiple of 16 places, and the maps fetch them.
 template <typename T, int ROWS, int DIM, int COMPRESS, bool TILED>
@@ -866,6 +903,7 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         const int r = (i >> 1) * 8 + 2 * (lane & 3) + (i & 1);
         if (lane < 4) ref_s[warp][r] = ref[i], sum_s[warp][r] = sum[i], state_s[warp][r] = state[i], seen_s[warp][r] = any[i];
       }
+      bool none = false;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
         if (m * 16 < a.dim) {
@@ -875,8 +913,13 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
             for (int e = 0; e < 4; ++e) {
               const int r = 8 * n + 2 * (lane & 3) + (e & 1), d = m * 16 + (lane >> 2) + 8 * (e >> 1);
               joined[(warp * ROWS + r) * kJoinRow + d] = out[m][4 * n + e];
+              none |= out[m][4 * n + e] != out[m][4 * n + e] && d < a.dim;
             }
         }
+      if (__any_sync(0xffffffffu, none)) {
+        __syncwarp();
+        add_again<T, COMPRESS, TILED>(a, query, ref_s[warp], joined + warp * ROWS * kJoinRow, kJoinRow, b, kv, row0, rows, key0, tiles);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < OWN; ++i)

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import cache_oracle
 from cache_oracle import ROUND
 from test_gpu_gen_propagation import F16, TYPES, problem
 
@@ -178,3 +179,38 @@ def test_a_later_node_that_is_none_and_the_states(jk, dtype, page, group):
         state, value = jk.cached_propagation(**p, scale=0.3)
         assert value[:, :4].isfinite().all() and state[:, :4].isfinite().all()
         assert value[:, 4].isnan().all() and state[:, 4].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("new,group", [(1, 1), (1, 9), (3, 1), (3, 8)])
+@pytest.mark.parametrize("compress", ["softmax", "softsign", "signed_abs_softmax"])
+@pytest.mark.parametrize("window", [None, 30])
+def test_infinite_values(jk, dtype, page, new, group, compress, window):
+    """An infinite value that is seen gives an infinity of its weight's sign, in its own column alone."""
+    lengths = [20, 90, 1500, 3]
+    for columns in (None, 1500):
+        p = problem(dtype, lengths, new=new, heads=group, rank=16, dim=43, page=page, columns=columns and -(-columns // page))
+        finite = {k: v.clone() for k, v in p.items()}
+        finite["value_pages"][..., 3:6] = 0.0
+        p["value_pages"][..., 3:6] = 0.0
+        for b, n in enumerate(lengths):
+            at, off = places(p, b, n)
+            j, k = max(0, n - new - 12), max(0, n - new - 1)  # seen by all new nodes
+            finite["value_pages"][at[j], 0, off[j], 3] = 1.0  # the weights of the infinities
+            finite["value_pages"][at[j], 0, off[j], 4] = -1.0
+            p["value_pages"][at[j], 0, off[j], 3] = math.inf
+            p["value_pages"][at[j], 0, off[j], 4] = -math.inf
+            p["value_pages"][at[j], 0, off[j], 5] = math.inf
+            p["value_pages"][at[k], 0, off[k], 5] = -math.inf if j != k else math.nan
+        options = dict(compress=compress, scale=0.3, window=window)
+        got = jk.cached_propagation(**p, **options).cpu().double()
+        args = {k.replace("_pages", "s"): v for k, v in finite.items()}
+        want, _, off, _ = cache_oracle.propagate(**args, **options)
+        assert (want[..., 3].abs() > 1e-12).all()
+        want[..., 3:5] = want[..., 3:5].sign() * math.inf
+        assert torch.equal(got[..., 3:5], want[..., 3:5])
+        if compress == "softmax":
+            assert got[..., 5].isnan().all()
+        for some in (slice(0, 3), slice(6, None)):
+            assert ((got - want).abs() <= off)[..., some].all()
