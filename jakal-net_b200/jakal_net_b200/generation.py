@@ -20,7 +20,8 @@ An empty cache has a table of -1 and zeros. All of it stays on the device: nothi
 a step (``cache_reserve_``, for every layer ``cache_write_`` and ``cached_propagation``, then
 ``verify_draft`` and ``cache_release_``) can be captured into a CUDA graph. Everything runs on the
 current stream; calls on one cache have to be ordered. Results are the same from run to run.
-The operators have no backward pass and refuse inputs that ask for one.
+The operators have no derivatives and refuse inputs that ask for them: tensors that require grad while
+gradients are recorded, and those with forward-mode tangents.
 """
 from __future__ import annotations
 
@@ -30,6 +31,7 @@ from typing import Optional, Sequence, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .training import _DTYPE_CODE, _call, _check_input, _empty, _ptr, _written
@@ -118,6 +120,16 @@ def _no_grad(*tensors: tuple) -> None:
             raise RuntimeError(f"{name} requires grad: the generation-step operators have no backward pass (use torch.no_grad())")
 
 
+def _no_derivatives(*tensors: tuple) -> None:
+    """Refuses (name, tensor) pairs that take part in a derivative at hand, backward or forward."""
+    if torch.is_grad_enabled():
+        _no_grad(*tensors)
+    if forward_ad._current_level >= 0:
+        for name, t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has a tangent: the generation-step operators have no forward-mode derivative")
+
+
 def _one_block(shape, strides) -> bool:
     """Whether these dims fill one block of memory, in whatever order."""
     expected = 1
@@ -149,6 +161,8 @@ class _Pools:
         n = len(data)
         if n > _MAX_POOLS:
             raise ValueError(f"{n} pools, at most {_MAX_POOLS} are supported")
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+            _no_derivatives(*[(f"pool {i}", t) for i, t in enumerate(tensors)])
         self.tensors, self.arrays = tensors, array.array("q", data + sizes + strides)
         at = _at(self.arrays)
         self.words = array.array("q", (at, at + 8 * n, at + 16 * n, n))
@@ -230,8 +244,8 @@ def cached_propagation(query: Tensor, key_pages: Tensor, value_pages: Tensor, ta
         raise ValueError(f"query has shape {tuple(query.shape)}, expected [batch, new, heads, rank]")
     _cache_pages("key_pages", key_pages, query, 4)
     _cache_pages("value_pages", value_pages, query, 4)
-    if torch.is_grad_enabled():
-        _no_grad(("query", query), ("key_pages", key_pages), ("value_pages", value_pages), ("state_pages", state_pages))
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        _no_derivatives(("query", query), ("key_pages", key_pages), ("value_pages", value_pages), ("state_pages", state_pages))
     batch, new, heads, rank = query.shape
     pages, kv_heads, page_size, dim = value_pages.shape
     if key_pages.shape != (pages, kv_heads, page_size, rank):
@@ -321,7 +335,7 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
         _ints("counts", counts, (batch,), device)
     if len(pages) != len(rows) or not pages:
         raise ValueError(f"{len(rows)} tensors of rows for {len(pages)} of pages")
-    recording = torch.is_grad_enabled()
+    derivatives = torch.is_grad_enabled() or forward_ad._current_level >= 0
     count = new = heads = page_size = None
     at, from_, page_strides, row_strides, widths, sizes = [], [], [], [], [], []
     kept = []  # copies of rows, until the launch
@@ -332,8 +346,8 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
             raise RuntimeError(f"pages {i} and rows {i} are on {p.device} and {r.device}, expected cuda:{device}")
         if p.dtype is not r.dtype:
             raise RuntimeError(f"rows {i} has dtype {r.dtype}, expected {p.dtype}")
-        if recording:
-            _no_grad(("pages", p), ("rows", r))
+        if derivatives:
+            _no_derivatives(("pages", p), ("rows", r))
         shape, row_shape, page_stride, row_stride = p.shape, r.shape, p.stride(), r.stride()
         dims = len(shape)
         if dims == 4 and len(row_shape) == 4:
@@ -506,6 +520,8 @@ def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, unifor
     _given("uniform", uniform, target, (batch, drafted + 1), (torch.float32,))
     if counts is not None:
         _ints("counts", counts, (batch,), device)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        _no_derivatives(("target", target), ("draft", draft), ("uniform", uniform))
     if target.stride(2) != 1 and vocab > 1:
         target = target.detach().contiguous()
     if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
