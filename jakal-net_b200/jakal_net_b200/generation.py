@@ -130,6 +130,14 @@ def _no_derivatives(*tensors: tuple) -> None:
                 raise RuntimeError(f"{name} has a tangent: the generation-step operators have no forward-mode derivative")
 
 
+def _given_twice(tensors: Sequence[Tensor], data: Sequence[int]) -> bool:
+    """Whether two of the tensors, at these addresses, begin at the same one; those without elements have none."""
+    if len(set(data)) == len(data):
+        return False
+    filled = [at for at, t in zip(data, tensors) if t.numel()]
+    return len(set(filled)) != len(filled)
+
+
 def _one_block(shape, strides) -> bool:
     """Whether these dims fill one block of memory, in whatever order."""
     expected = 1
@@ -156,7 +164,7 @@ class _Pools:
             sizes = strides = [t.numel() // pages * t.element_size() for t in tensors]
         else:
             data, sizes, strides = self._others(tensors, pages, device)
-        if len(set(data)) != len(data) and any(t.numel() for t in tensors):
+        if _given_twice(tensors, data):
             raise ValueError("a pool is given twice")
         n = len(data)
         if n > _MAX_POOLS:

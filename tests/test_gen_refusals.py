@@ -37,3 +37,16 @@ def test_tensors_with_tangents_are_refused():
     generation._no_derivatives(("keys", x), ("none", None))
     with pytest.raises(RuntimeError, match="keys.*backward"):
         generation._no_derivatives(("keys", x.clone().requires_grad_(True)))
+
+
+def test_pools_given_twice_are_refused_and_empty_ones_are_not():
+    from jakal_net_b200 import generation
+
+    some, none = torch.zeros(4, 2), [torch.zeros(4, 0), torch.zeros(4, 1, 0), torch.zeros(4, 3, 0)]
+    generation._Pools([none[0], some, none[1], none[2]], 4, CPU)
+    generation._Pools(none, 4, CPU)
+    wide = torch.zeros(4, 6)
+    generation._Pools([wide[:, :2], wide[:, 2:]], 4, CPU)
+    for pools in ([some, some], [some, none[0], some], [wide[:, :2], wide[:, :3]], [wide, wide[:, :0], wide[:, :1]]):
+        with pytest.raises(ValueError, match="twice"):
+            generation._Pools(pools, 4, CPU)
