@@ -334,7 +334,7 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
     pages: one tensor [pages, kv_heads, page_size, width] or [pages, kv_heads, page_size], or several
     (a layer's keys, values and states); rows: for each [batch, new, kv_heads, width] or [batch, new,
     kv_heads] of its dtype. Node t of the counts[b] (None: `new`) that a sequence has goes to place
-    lengths[b] - counts[b] + t; places without a page are left out."""
+    lengths[b] - counts[b] + t; places without a page are left out. A tensor of pages is given once."""
     pages = [pages] if isinstance(pages, Tensor) else list(pages)
     rows = [rows] if isinstance(rows, Tensor) else list(rows)
     device, batch, columns, stride = _table(table)
@@ -390,6 +390,8 @@ def cache_write_(pages: Union[Tensor, Sequence[Tensor]], rows: Union[Tensor, Seq
         sizes.append(p.element_size())
     if not page_size:
         raise ValueError("page_size is 0")
+    if _given_twice(pages, at):
+        raise ValueError("pages are given twice")
     cache = _cache(table, stride, lengths, None, batch, columns, count, page_size)
     n = len(pages)
     words = array.array("q", at + from_ + widths + sizes + page_strides + row_strides)

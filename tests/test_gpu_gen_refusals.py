@@ -52,3 +52,19 @@ def test_inputs_that_take_part_in_derivatives(jk):
                 call()
         for call in calls(jk, pool, target, draft, uniform):
             call()
+
+
+def test_pages_given_twice(jk):
+    """Two sets of rows for the same places: which stays would depend on which is written last."""
+    pool, other = torch.zeros(5, 1, 4, 8, device="cuda"), torch.zeros(5, 1, 4, 8, device="cuda")
+    table, lengths = ints([0, 1]), ints(6)
+    rows = [torch.full((1, 2, 1, 8), float(i), device="cuda") for i in range(3)]
+    for pages in ([pool, pool], [pool, other, pool]):
+        with pytest.raises(ValueError, match="twice"):
+            jk.cache_write_(pages, rows[:len(pages)], table, lengths)
+    with pytest.raises(ValueError, match="twice"):
+        jk.cache_write_([pool, pool[..., :3]], [rows[0], rows[1][..., :3]], table, lengths)
+    assert not pool.any() and not other.any()
+    empty = [torch.zeros(5, 1, 4, 0, device="cuda") for _ in range(2)]
+    jk.cache_write_([empty[0], pool, empty[1]], [r[..., :0] if i != 1 else r for i, r in enumerate(rows)], table, lengths)
+    assert pool[1, 0].tolist() == [[1.0] * 8] * 2 + [[0.0] * 8] * 2
