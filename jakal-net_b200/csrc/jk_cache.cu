@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(Table t, int32_t* len
 
 // ---- pages moved together
 
-// sum over the workspace: moves[0] pages, from[i] -> to[i], map[page]: where a page that moved went.
+// sum over the workspace: moves[0] pages, from[i] -> to[i], map[page]: where a page past the first `live` went, -1: it is free.
 struct Compact {
   int32_t *moves, *from, *to, *map;
 };
@@ -395,6 +395,7 @@ __global__ void __launch_bounds__(kOne) compact_kernel(int32_t* refs, int64_t pa
     for (int j = 0; j < 4; ++j) {
       if (hole[j]) w.to[h++] = static_cast<int32_t>(at + j);
       if (move[j]) w.from[m++] = static_cast<int32_t>(at + j);
+      else if (at + j >= live && at + j < pages) w.map[at + j] = -1;
     }
     holes += total & 0xffff;
     moves += total >> 16;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
   for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < entries; i += int64_t(gridDim.x) * kThreads) {
     int32_t* at = t.at + (i / t.columns) * t.stride + i % t.columns;
     const int32_t page = *at;
-    // an entry past the pages in use names one that moved, if the references are right: the map holds only those
+    // an entry past the pages in use names one that moved, if the references are right; one that has none stays as it is
     if (page >= live && in_cache(page, t.pages)) {
       const int32_t to = w.map[page];
       if (in_cache(to, live)) *at = to;

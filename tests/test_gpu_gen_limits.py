@@ -1,0 +1,39 @@
+"""Generation-step operators at the ends of what they take: lengths and vocabularies, references that do not fit the table."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def jk():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    import jakal_net_b200
+
+    return jakal_net_b200
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("before", [0, 1, -1, 7])
+def test_entries_without_a_reference_stay_where_they_are(jk, before):
+    """Compaction of a table that names pages whose reference count is 0, past the pages in use; the workspace holds numbers
+    of an earlier call, which must not be taken for pages."""
+    pages = 12
+    table, refs = ints([9, 10, -1], [11, 2, 40]), ints(0, 0, 1, 0, 0, 0, 0, 0, 0, 0, 1, 0)
+    size = jk._LIBRARY.jk_cache_compact_workspace(pages)
+    work = torch.full((size // 4,), before, dtype=torch.int32, device="cuda")
+    live = ints(0)
+    words = lambda *v: (ctypes.c_int64 * len(v))(*v)  # noqa: E731
+    cache = words(table.data_ptr(), 3, 0, refs.data_ptr(), 2, 3, pages, 1)
+    status = jk._LIBRARY.jk_cache_compact(words(0, 0, 0, 0), cache, live.data_ptr(), work.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert status == 0 and live.item() == 2
+    # pages 2 and 10 are in use and go to the first two; 9 and 11 have no reference, 40 is no page
+    assert table.tolist() == [[9, 1, -1], [11, 0, 40]] and refs.tolist() == [1, 1] + [0] * 10
