@@ -580,8 +580,8 @@ int64_t jk_cache_reserve_workspace(int64_t batch, int64_t pages);
  * free when the call begins, lowest first, enter the table with one reference; lengths grow. A
  * sequence that grows inside a page that others hold too (refs > 1) first gets a copy of that page
  * in every pool and gives up its reference. added[b] (int32 [batch]) is counts[b], or 0 where the
- * sequence is left as it is: a negative count, more nodes than the table's row has room for, or
- * pages that ran out (from the first sequence that could not be served on, none that needs a page
+ * sequence is left as it is: a negative count, more nodes than the table's row has room for or than
+ * 2^31 - 65, or pages that ran out (from the first sequence that could not be served on, none that needs a page
  * is). Needs refs. workspace: jk_cache_reserve_workspace(...) bytes, 16-byte aligned. */
 int jk_cache_reserve(const jk_pools_t* pools, const jk_cache_t* cache, const int32_t* counts, int32_t* added,
                      void* workspace, jk_stream_t stream);

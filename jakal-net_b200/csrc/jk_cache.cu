@@ -27,6 +27,7 @@ constexpr int kPiece = 32 * kLoads; // 16-byte blocks of a piece: a warp's turn
 constexpr int kMaxBlocks = 148 * 8;
 constexpr int kSmall = 8, kLarge = 512;  // pools of a launch: its parameters are copied, so few take the small table
 constexpr int kMaxWrite = 64;
+constexpr int64_t kMaxLength = 0x7fffffff - 64;  // nodes of a sequence: what the propagation sees
 
 // ---- copies of any alignment
 
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kOne) reserve_kernel(Table t, int32_t* lengths
     bool fits = false;
     if (b < t.batch) {
       const int64_t n = lengths[b], c = counts[b];
-      fits = n >= 0 && c >= 0 && n + c <= t.columns * page_size;
+      fits = n >= 0 && c >= 0 && n + c <= t.columns * page_size && n + c <= kMaxLength;
       if (fits && c > 0) {
         have = (n + page_size - 1) / page_size;
         need = static_cast<int32_t>((n + c + page_size - 1) / page_size - have);

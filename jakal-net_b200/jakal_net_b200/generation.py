@@ -309,8 +309,8 @@ def cache_reserve_(pools: Union[Tensor, Sequence[Tensor]], table: Tensor, length
     values and states of every layer, 512 at most).
 
     counts int32 [batch]. Returns added int32 [batch]: counts[b], or 0 for a sequence that is left
-    as it is because its count is negative, its row of the table is too short, or the pages ran out (from
-    the first sequence that could not be served on, none that needs a page is). Give `added` to
+    as it is because its count is negative, its row of the table is too short (or its length would pass
+    2^31 - 65), or the pages ran out (from the first sequence that could not be served on, none that needs a page is). Give `added` to
     ``cache_write_`` and ``cached_propagation`` as their counts."""
     device, batch, columns, stride = _table(table)
     _ints("lengths", lengths, (batch,), device)

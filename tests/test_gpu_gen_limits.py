@@ -37,3 +37,13 @@ def test_entries_without_a_reference_stay_where_they_are(jk, before):
     assert status == 0 and live.item() == 2
     # pages 2 and 10 are in use and go to the first two; 9 and 11 have no reference, 40 is no page
     assert table.tolist() == [[9, 1, -1], [11, 0, 40]] and refs.tolist() == [1, 1] + [0] * 10
+
+
+def test_lengths_end_before_2_31(jk):
+    """Tables with room for more nodes than a length can count."""
+    page = 1 << 30
+    most = 2 ** 31 - 65
+    table, lengths, refs = ints([0, 1, -1, -1], [2, 3, -1, -1], [4, 5, -1, -1]), ints(most - 5, most - 5, 2 ** 31 - 7), ints(1, 1, 1, 1, 1, 1, 0, 0)
+    added = jk.cache_reserve_([], table, lengths, refs, ints(5, 6, 100), page)
+    assert added.tolist() == [5, 0, 0] and lengths.tolist() == [most, most - 5, 2 ** 31 - 7]
+    assert refs.tolist() == [1] * 6 + [0, 0] and table[:, 2:].eq(-1).all()
