@@ -2,6 +2,9 @@
 // jk_cached.cuh, instantiated by type in jk_cached_{f32,bf16,f16}.cu.
 #include "jk_cached.cuh"
 
+#include <cmath>
+#include <limits>
+
 namespace jk {
 namespace cached {
 namespace {
@@ -98,6 +101,8 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
   a.compress = static_cast<int32_t>(q->compress);
   a.scale = a.compress == JK_SOFTMAX ? static_cast<float>(double(scale) * 1.4426950408889634) : scale;
   a.bias = score_bias;
+  // (the softmax leaves a bias out, as it moves all scores together; with one that is no number or infinite they are not apart)
+  if (a.compress == JK_SOFTMAX && !std::isfinite(score_bias)) a.scale = std::numeric_limits<float>::quiet_NaN();
   a.key_piece = piece_of(q->keys, a.key_stride, rank * size), a.value_piece = piece_of(q->values, a.value_stride, dim * size);
   Maps maps{};
   Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, true);

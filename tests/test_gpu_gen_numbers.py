@@ -214,3 +214,14 @@ def test_infinite_values(jk, dtype, page, new, group, compress, window):
             assert got[..., 5].isnan().all()
         for some in (slice(0, 3), slice(6, None)):
             assert ((got - want).abs() <= off)[..., some].all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("compress", ["softmax", "signed_abs_softmax"])
+@pytest.mark.parametrize("columns", [None, 100])
+@pytest.mark.parametrize("bias", [math.inf, -math.inf, math.nan])
+def test_biases_that_are_no_numbers(jk, dtype, compress, columns, bias):
+    """Scores that are all NaN or infinite have no softmax; a node that sees nothing still has zeros."""
+    p = problem(dtype, [20, 0, 700], heads=2, page=16, columns=columns, states=True)
+    state, value = jk.cached_propagation(**p, compress=compress, score_bias=bias)
+    assert value[::2].isnan().all() and state[::2].isnan().all() and not value[1].any() and not state[1].any()
