@@ -6,10 +6,11 @@
 // Where all are accepted r is the target's next distribution.
 //
 // A comparison of a product or of a running sum decides a token, so both are in f64: products of two
-// f32 are exact there, and a running sum is off by less than 2^-44 of the total, where f32 would give
+// f32 are exact there, and a running sum is off by less than 2^-40 + m 2^-53 of the total (m: entries that a lane adds up,
+// at most 2^18 for a few sequences and 2^23 for many), where f32 would give
 // another token in one of some thousand draws over a vocabulary of 100,000. Conversions to f64 are the
 // slowest part (16 a cycle and SM), so a difference takes one: d = x - y in f32, whose rounding error
-// (x - d) - y is exact there for x >= y >= 0, and errors are added up on their own.
+// (x - d) - y is exact there for x >= y >= 0, and errors are added up on their own, in f32 up to 128 of them.
 //
 // Of the draft's and the target's rows only place a's are read, once: a cluster of blocks per
 // sequence adds them up by warps, each a run of 16-byte packs; the run that holds the draw is cut
@@ -153,7 +154,15 @@ struct Rest {
       add(x, y, s, lost);
     };
     int32_t k = low + lane;
+    // errors go over into the sum after at most 128 of them, so that their own rounding does not grow with the vocabulary
+    auto over = [&] {
+      const float2 some = unpair(lost);
+      s += static_cast<double>(some.x) + static_cast<double>(some.y);
+      lost = 0;
+    };
+    int pending = 0;
     for (; k + 32 * (kLoads - 1) < high; k += 32 * kLoads) {
+      if (++pending > 128 / (kLoads * E / 2)) over(), pending = 1;
       uint4 u[kLoads], v[kLoads], n[kLoads];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) fetch(k + 32 * i, u[i], v[i], n[i]);
@@ -173,8 +182,8 @@ struct Rest {
       load(edge, x, y);
       add(x, y, s, lost);
     }
-    const float2 rest = unpair(lost);
-    return warp_sum64(s + (static_cast<double>(rest.x) + static_cast<double>(rest.y)));
+    over();
+    return warp_sum64(s);
   }
 
   // Over packs [from, to), a warp.

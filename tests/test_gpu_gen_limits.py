@@ -47,3 +47,19 @@ def test_lengths_end_before_2_31(jk):
     added = jk.cache_reserve_([], table, lengths, refs, ints(5, 6, 100), page)
     assert added.tolist() == [5, 0, 0] and lengths.tolist() == [most, most - 5, 2 ** 31 - 7]
     assert refs.tolist() == [1] * 6 + [0, 0] and table[:, 2:].eq(-1).all()
+
+
+@pytest.mark.parametrize("k", [60979, 54809, 49873, 58511])
+def test_sums_over_a_large_vocabulary_keep_their_small_parts(jk, k):
+    """Every entry is 1 - k 2^-42, which f32 rounds to 1 with an error of k 2^-42. With u a multiple of 2^-11 the draw lies on
+    a border between two entries, and all sums up to there are exact in f64 (42 bits), as are 128 errors of 16 bits in f32: the
+    token is the first entry past the border. (An f32 sum of 8192 errors rounds by up to 2^-27.)"""
+    vocab = 1 << 26
+    if torch.cuda.mem_get_info()[0] < 2 << 30:
+        pytest.skip("needs 2 GB")
+    target = torch.ones(1, 2, 1, device="cuda").expand(1, 2, vocab).contiguous()
+    draft = torch.full((1, 1, vocab), k * 2.0 ** -42, device="cuda")
+    tokens = torch.full((1, 1), -1, dtype=torch.int64, device="cuda")  # not accepted
+    for part in (5, 77, 200, 999, 1029, 1535, 2047):
+        out, accepted = jk.verify_draft(target, draft, tokens, torch.tensor([[0.5, part / 2048]], device="cuda"))
+        assert accepted.tolist() == [0] and out.tolist() == [[part * (vocab // 2048), -1]]
