@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(Table t, int32_t* len
 
 // ---- pages moved together
 
-// sum over the workspace: moves[0] pages, from[i] -> to[i], map[page]: where a page past the first `live` went, -1: it is free.
+// sum over the workspace: moves[0] pages, from[i] -> to[i], map[page]: the i of a page that moved (of the others, any number).
 struct Compact {
   int32_t *moves, *from, *to, *map;
 };
@@ -396,7 +396,6 @@ __global__ void __launch_bounds__(kOne) compact_kernel(int32_t* refs, int64_t pa
     for (int j = 0; j < 4; ++j) {
       if (hole[j]) w.to[h++] = static_cast<int32_t>(at + j);
       if (move[j]) w.from[m++] = static_cast<int32_t>(at + j);
-      else if (at + j >= live && at + j < pages) w.map[at + j] = -1;
     }
     holes += total & 0xffff;
     moves += total >> 16;
@@ -404,7 +403,7 @@ __global__ void __launch_bounds__(kOne) compact_kernel(int32_t* refs, int64_t pa
   __syncthreads();
   for (int32_t i = tid; i < moves; i += kOne) {
     const int32_t from = w.from[i], to = w.to[i];
-    w.map[from] = to;
+    w.map[from] = i;
     refs[to] = refs[from];
     refs[from] = 0;
   }
@@ -417,15 +416,15 @@ __global__ void __launch_bounds__(kOne) compact_kernel(int32_t* refs, int64_t pa
 template <int N>
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ Pools<N> pools, Table t, const int32_t* live_at, Compact w) {
   grid_dependency_wait();
-  const int32_t live = *live_at;
+  const int32_t live = *live_at, moves = *w.moves;
   const int64_t entries = t.batch * t.columns;
   for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < entries; i += int64_t(gridDim.x) * kThreads) {
     int32_t* at = t.at + (i / t.columns) * t.stride + i % t.columns;
     const int32_t page = *at;
     // an entry past the pages in use names one that moved, if the references are right; one that has none stays as it is
     if (page >= live && in_cache(page, t.pages)) {
-      const int32_t to = w.map[page];
-      if (in_cache(to, live)) *at = to;
+      const int32_t k = w.map[page];
+      if (static_cast<uint32_t>(k) < static_cast<uint32_t>(moves) && w.from[k] == page) *at = w.to[k];
     }
   }
   copy_pairs(pools, Pairs{w.from, w.to, 1, 0, w.moves}, t.pages);
