@@ -225,3 +225,37 @@ def test_biases_that_are_no_numbers(jk, dtype, compress, columns, bias):
     p = problem(dtype, [20, 0, 700], heads=2, page=16, columns=columns, states=True)
     state, value = jk.cached_propagation(**p, compress=compress, score_bias=bias)
     assert value[::2].isnan().all() and state[::2].isnan().all() and not value[1].any() and not state[1].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("new,group,dim", [(40, 1, 500), (9, 8, 250), (17, 4, 120)])
+@pytest.mark.parametrize("columns", [None, 60])
+def test_infinite_values_with_many_rows(jk, dtype, page, new, group, dim, columns):
+    """Several blocks to a unit's rows, of which those after the infinite value alone see it, in graphs too."""
+    lengths = [300, new]
+    p = problem(dtype, lengths, new=new, heads=2 * group, kv_heads=2, rank=32, dim=dim, page=page, columns=columns, states=True)
+    counts = torch.tensor([new, new - 3], dtype=torch.int32, device="cuda")
+    first = [n - c for n, c in zip(lengths, counts.tolist())]
+    at = [places(p, b, n) for b, n in enumerate(lengths)]
+    third = [f + new // 3 for f in first]  # seen by the nodes from the (new / 3)-th on
+    finite = {k: v.clone() for k, v in p.items()}
+    for b, j in enumerate(third):
+        p["value_pages"][at[b][0][j], :, at[b][1][j], 7] = math.inf
+        finite["value_pages"][at[b][0][j], :, at[b][1][j], 7] = 0.0
+    options = dict(compress="softmax", scale=0.2, counts=counts)
+    state, value = jk.cached_propagation(**p, **options)
+    want_state, want = jk.cached_propagation(**finite, **options)
+    assert torch.equal(state, want_state)
+    for b in range(2):
+        assert value[b, new // 3:int(counts[b]), :, 7].isposinf().all() and value[b, :new // 3, :, 7].isfinite().all()
+    args = {"states" if k == "state_pages" else k.replace("_pages", "s"): v for k, v in finite.items()}
+    exact, _, off, _ = cache_oracle.propagate(**args, **options)
+    others = [c for c in range(dim) if c != 7]
+    assert ((value.cpu().double() - exact).abs() <= off)[..., others].all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = jk.cached_propagation(**p, **options)
+    for _ in range(2):
+        graph.replay()
+        assert torch.equal(again[0], state) and torch.equal(again[1].nan_to_num(), value.nan_to_num())
