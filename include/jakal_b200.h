@@ -557,7 +557,8 @@ int64_t jk_cached_propagation_workspace(int64_t batch, int64_t new_nodes, int64_
  *   out_value[b, t, h] = sum_j w_j values[j],  out_state[b, t, h] = sum_j w_j states[j]
  * with compress JK_SOFTMAX, JK_SOFTSIGN or JK_SIGNED_ABS_SOFTMAX. A node that sees none, and nodes
  * t >= n, have zeros; a softmax over scores that are all -inf is NaN. What places that are not
- * seen hold (NaN, infinities) has no part in a result. Sums are f32, before they are divided by the
+ * seen hold (NaN, infinities) has no part in a result; a NaN score or an infinite value that is seen has the
+ * part that the formula gives it. Sums are f32, before they are divided by the
  * weights' sum. 16-bit weights go into the value product as two planes, rounded by at most 2^-16 of a
  * weight, in f16 at least 2^-32 of the largest (softsign: 2^-40).
  * rank <= 256, dim <= 512, new_nodes <= 64, heads a multiple of kv_heads. */
@@ -658,7 +659,7 @@ typedef struct jk_draft {
  * NULL: probability 1); with the first a that is not (a = n: all are), out_tokens[b, a] is the least j with
  *   sum_{j' <= j} r_j' > uniform[b, drafted] * sum r,
  * r = max(target[b, a] - draft[b, a], 0) for a < n (target[b, a] where that is 0 throughout), target[b, n]
- * for a = n, in f64. NaN and negative values count as 0; a token outside the vocabulary is not
+ * for a = n, in f64. NaN and negative values count as 0 (infinite ones leave the new token open); a token outside the vocabulary is not
  * accepted; where r has no positive entry out_tokens[b, a] is -1. Before it stand the accepted tokens,
  * behind it -1; accepted[b] is a. vocab <= 2^30. */
 int jk_verify_draft(const jk_draft_t* draft, jk_stream_t stream);

@@ -8,12 +8,13 @@
 // fills the GPU. Whole numbers throughout: results do not depend on the order in which blocks run
 // (references are added to, never read, where blocks share them).
 //
-// Bound: bookkeeping by the latency of a few dependent reads and a launch or two (room for a node in each of 32 sequences,
-// its rows written and given back: 9.8 us on the device, 45 as calls), copies by memory (the 70 us of 460 MB moved
-// together are what they take at the measured copy rate; 76 MB of new rows 16 us, of which 12 for the memory).
-// A copy has 16-byte stores to aligned blocks whatever the alignment of its two sides: where they
-// differ, a block is put together from the two aligned blocks of the source that hold its bytes
-// (so rows of 65 bf16 cost two loads a block instead of eight).
+// Bound: bookkeeping by the latency of a few dependent reads and a launch or two (room for a node
+// in each of 32 sequences, its rows written and given back: 9.8 us on the device, 45 as calls),
+// copies by memory (the 70 us of 460 MB moved together are what they take at the measured copy
+// rate; 76 MB of new rows 16 us, of which 12 for the memory). A copy has 16-byte stores to aligned
+// blocks whatever the alignment of its two sides: where they differ, a block is put together from
+// the two aligned blocks of the source that hold its bytes (so rows of 65 bf16 cost two loads a
+// block instead of eight).
 #include "jk_host.h"
 #include "jk_rows.cuh"
 
@@ -308,7 +309,8 @@ __device__ __forceinline__ void fork_row(const Table& t, int32_t* refs, int32_t 
   }
 }
 
-// taken: [batch], of which only the children's entries are used; copied: [forks] the parent's length, -1: not done.
+// taken: [batch], of which only the children's entries are used; copied: [forks] the parent's
+// length, -1: not done.
 __global__ void __launch_bounds__(kOne) fork_kernel(Table t, int32_t* lengths, int32_t* refs, const int32_t* parents, const int32_t* children,
                                                     int64_t forks, uint8_t* done, int32_t* taken, int32_t* copied, bool rows_too) {
   auto inside = [&](int64_t i) {
@@ -360,7 +362,8 @@ __global__ void __launch_bounds__(kThreads) release_kernel(Table t, int32_t* len
 
 // ---- pages moved together
 
-// sum over the workspace: moves[0] pages, from[i] -> to[i], map[page]: the i of a page that moved (of the others, any number).
+// sum over the workspace: moves[0] pages, from[i] -> to[i], map[page]: the i of a page that moved
+// (of the others, any number).
 struct Compact {
   int32_t *moves, *from, *to, *map;
 };
@@ -421,7 +424,8 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
   for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < entries; i += int64_t(gridDim.x) * kThreads) {
     int32_t* at = t.at + (i / t.columns) * t.stride + i % t.columns;
     const int32_t page = *at;
-    // an entry past the pages in use names one that moved, if the references are right; one that has none stays as it is
+    // an entry past the pages in use names one that moved, if the references are right; one that
+    // has none stays as it is
     if (page >= live && in_cache(page, t.pages)) {
       const int32_t k = w.map[page];
       if (static_cast<uint32_t>(k) < static_cast<uint32_t>(moves) && w.from[k] == page) *at = w.to[k];
@@ -567,9 +571,10 @@ int jk_cache_write(const jk_rows_t* q, const jk_cache_t* cache, const int32_t* c
       w.row_stride[i][j] = q->rows_strides[3 * i + j] * size;
     }
     w.unit[i] = static_cast<uint8_t>(size);
-    // lanes of a row: as many as it has blocks (one more where it begins inside a block), a power of 2, but four blocks a lane
-    // in rows of 512 bytes and more, so that each table entry that is waited for is followed by that many loads (32 x 1024 nodes of 64 + 512 + 1 bf16, with room and
-    // release: 24.4 us with two blocks a lane in all rows, 21.7 with four)
+    // lanes of a row: as many as it has blocks (one more where it begins inside a block), a power
+    // of 2, but four blocks a lane in rows of 512 bytes and more, so that each table entry that is
+    // waited for is followed by that many loads (32 x 1024 nodes of 64 + 512 + 1 bf16, with room
+    // and release: 24.4 us with two blocks a lane in all rows, 21.7 with four)
     int64_t blocks = (w.bytes[i] + 15) / 16 + (w.bytes[i] % 16 != 0 && w.bytes[i] > 16 ? 1 : 0);
     if (blocks >= 32) blocks = (blocks + 3) / 4;
     int log2 = 0;
@@ -610,9 +615,10 @@ int jk_cache_fork(const jk_cache_t* cache, const int32_t* parents, const int32_t
   auto* taken = static_cast<int32_t*>(workspace);
   auto* copied = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + round16(batch * 4));
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  // few table entries: the block that decides copies them as well, which saves a launch (forks and entries each, together with
-  // the release that undoes them, a call and on the device: 63 x 128 19.0 and 6.2 us so, 20.9 and 5.7 with a launch for the
-  // rows; 63 x 512 18.7 and 12.0, 21.0 and 6.3)
+  // few table entries: the block that decides copies them as well, which saves a launch (forks and
+  // entries each, together with the release that undoes them, a call and on the device: 63 x 128
+  // 19.0 and 6.2 us so, 20.9 and 5.7 with a launch for the rows; 63 x 512 18.7 and 12.0, 21.0 and
+  // 6.3)
   const bool rows_too = columns == 0 || forks <= 8192 / columns;
   fork_kernel<<<1, kOne, 0, s>>>(t, lengths, refs, parents, children, forks, done, taken, copied, rows_too);
   if (!rows_too)

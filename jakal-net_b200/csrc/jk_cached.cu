@@ -101,12 +101,14 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
   a.compress = static_cast<int32_t>(q->compress);
   a.scale = a.compress == JK_SOFTMAX ? static_cast<float>(double(scale) * 1.4426950408889634) : scale;
   a.bias = score_bias;
-  // (the softmax leaves a bias out, as it moves all scores together; with one that is no number or infinite they are not apart)
+  // (the softmax leaves a bias out, as it moves all scores together; with one that is no number or
+  // infinite they are not apart)
   if (a.compress == JK_SOFTMAX && !std::isfinite(score_bias)) a.scale = std::numeric_limits<float>::quiet_NaN();
   a.key_piece = piece_of(q->keys, a.key_stride, rank * size), a.value_piece = piece_of(q->values, a.value_stride, dim * size);
   Maps maps{};
   Shape s = shape_of(heads / kv_heads * new_nodes, rank, dim, dtype, true);
-  // tiled copies: pages of a multiple of 16 places, rows in 16-byte blocks, strides that a map can hold, and a second stage
+  // tiled copies: pages of a multiple of 16 places, rows in 16-byte blocks, strides that a map can
+  // hold, and a second stage
   a.tiled = a.key_piece == 16 && a.value_piece == 16 && page_size % kKeys == 0 && s.stages > 1 && pages > 0 && a.columns > 0 &&
             make_map(&maps.keys, q->keys, rank, a.key_stride, pages, kv_heads, page_size, dtype) &&
             make_map(&maps.values, q->values, dim, a.value_stride, pages, kv_heads, page_size, dtype);
@@ -135,9 +137,10 @@ int jk_cached_propagation(const jk_cache_t* cache, const jk_nodes_t* q, float sc
     if (units > most || int64_t(a.batch) * heads * new_nodes * ((dim + 127) / 128) > most) return JK_ERR_BAD_SHAPE;
     const int64_t slots = int64_t(kSms) * s.per_sm;
     a.blocks = static_cast<int32_t>(units > slots / unit_tiles ? slots : units * unit_tiles);
-    // A block whose run is of two units begins and ends twice, which takes as long as two or three tiles; runs that end with
-    // their unit leave up to a run a unit empty, a quarter at most so. (On the device: 4 units of 4097 places, dim 512, 13.4 us,
-    // 15.6 with runs of any; 32 units of 2250 places in f32 27.0 and 29.8.)
+    // A block whose run is of two units begins and ends twice, which takes as long as two or three
+    // tiles; runs that end with their unit leave up to a run a unit empty, a quarter at most so.
+    // (On the device: 4 units of 4097 places, dim 512, 13.4 us, 15.6 with runs of any; 32 units of
+    // 2250 places in f32 27.0 and 29.8.)
     a.units = static_cast<int32_t>(units);
     a.whole_runs = a.blocks > 4 * units;
     int status;

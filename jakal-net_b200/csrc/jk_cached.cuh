@@ -30,8 +30,9 @@
 // (softsign, below 1), and what they leave is below 2^-32 of a weight of 1 on the reference, or 2^-40.
 // f32: the same walk with fused multiply-adds, which keep f32's rounding.
 // Exponentials are base 2, of one fused multiply-add: a score times a rate less a reference, which is such a
-// product rounded. From references of 2^24 on that rounding is a power of 2 and more (an exponent's whole range from 2^31 on), so
-// the product is rounded before the difference too, as the score itself has been.
+// product rounded. From references of 2^24 on that rounding is a power of 2 and more (an exponent's
+// whole range from 2^31 on), so the product is rounded before the difference too, as the score
+// itself has been.
 //
 // What is not seen has no part in a result, whatever it holds: places past the last node and places
 // without a page arrive as zeros, and a tile of which rows see different parts (the newest nodes of a
@@ -57,8 +58,9 @@ constexpr int kMaxPerSm = 3;            // blocks of an SM
 constexpr int kMaxBatch = 256;          // sequences of a launch
 constexpr int kMaxStages = 2;           // of a warp's ring
 constexpr int kMaxRank = 256, kMaxDim = 512, kMaxNew = 64;
-// Units of at most so many tiles get a block each, which saves a launch (8 heads of 512 places: 13.4 us a call and 11.4 on the
-// device so, 17.7 and 8.4 split; of 1024 places 21.2 and 18.3, 17.6 and 8.5).
+// Units of at most so many tiles get a block each, which saves a launch (8 heads of 512 places:
+// 13.4 us a call and 11.4 on the device so, 17.7 and 8.4 split; of 1024 places 21.2 and 18.3, 17.6
+// and 8.5).
 constexpr int kUnitTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;          // by which a score may pass its row's reference, as a power of 2
@@ -230,12 +232,13 @@ __device__ __forceinline__ float weight_of(float s, float mass) {
   return s == 0.0f ? 0.0f : copysignf(mass, s);
 }
 
-// A stage holds columns of 128 bytes of its 16 rows, 2048 bytes each, in which the 16-byte block c of row r lies at
-// 128 r + 16 (c ^ (r mod 8)): eight rows' blocks c are in different banks. (Tiled copies write it so.)
+// A stage holds columns of 128 bytes of its 16 rows, 2048 bytes each, in which the 16-byte block c
+// of row r lies at 128 r + 16 (c ^ (r mod 8)): eight rows' blocks c are in different banks. (Tiled
+// copies write it so.)
 __device__ __forceinline__ int block_at(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
 
-// Rows of the 16 lanes' places in pieces of 16, 8 or 4 bytes, as their alignment allows, with as many lanes a row as have 128
-// bytes of it; rows that are not `there` arrive as zeros.
+// Rows of the 16 lanes' places in pieces of 16, 8 or 4 bytes, as their alignment allows, with as
+// many lanes a row as have 128 bytes of it; rows that are not `there` arrive as zeros.
 template <int BYTES>
 __device__ __forceinline__ void load_pieces(char* stage, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
   constexpr int kLanes = 128 / BYTES, kStep = 32 / kLanes;
@@ -254,9 +257,10 @@ __device__ __forceinline__ void load_pieces(char* stage, const char* src, int64_
   }
 }
 
-// The same for 16-bit rows that begin at any element: 16-byte blocks are put together from the two that hold their bytes, through
-// registers. (These loads are waited for. 32 sequences of 10240 f16 nodes, rank 128: 222 us with a dim of 128, 306 with 124 in
-// pieces of 8, 404 with 126 in pieces of 4, 801 with 127 so, 1355 element by element; 126 so would take 762.)
+// The same for 16-bit rows that begin at any element: 16-byte blocks are put together from the two
+// that hold their bytes, through registers. (These loads are waited for. 32 sequences of 10240 f16
+// nodes, rank 128: 222 us with a dim of 128, 306 with 124 in pieces of 8, 404 with 126 in pieces of
+// 4, 801 with 127 so, 1355 element by element; 126 so would take 762.)
 template <typename T>
 __device__ __forceinline__ void load_odd_rows(char* dst, const char* src, int64_t offset, uint32_t there, int32_t row_bytes, int lane) {
   const char* from[4];
@@ -315,9 +319,10 @@ struct Maps {
   CUtensorMap keys, values;
 };
 
-// 16-bit types: an infinite value times a low plane that is 0 or of the other sign is NaN. A warp whose sums `joined` (a row every
-// `join_row` floats) have NaN adds up those rows again, place after place, with their weights in one piece; what is NaN then is so
-// by the formula. This is slow, and a function of its own, whose registers the loop does not pay for.
+// 16-bit types: an infinite value times a low plane that is 0 or of the other sign is NaN. A warp
+// whose sums `joined` (a row every `join_row` floats) have NaN adds up those rows again, place
+// after place, with their weights in one piece; what is NaN then is so by the formula. This is
+// slow, and a function of its own, whose registers the loop does not pay for.
 template <typename T, int COMPRESS, bool TILED>
 __device__ __noinline__ void add_again(const Args& a, const T* query, const float* refs, float* joined, int join_row, int32_t b, int32_t kv,
                                        int32_t row0, int32_t rows, int32_t key0, int32_t tiles) {
@@ -352,8 +357,8 @@ __device__ __noinline__ void add_again(const Args& a, const T* query, const floa
   }
 }
 
-// ROWS: rows of a unit that a block takes (a multiple of 8 for 16-bit types); DIM: columns of the value at most.
-// TILED: pages hold a multiple of 16 places, and the maps fetch them.
+// ROWS: rows of a unit that a block takes (a multiple of 8 for 16-bit types); DIM: columns of the
+// value at most. TILED: pages hold a multiple of 16 places, and the maps fetch them.
 template <typename T, int ROWS, int DIM, int COMPRESS, bool TILED>
 __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) cached_kernel(const __grid_constant__ Args a,
                                                                                              const __grid_constant__ Maps maps) {
@@ -417,8 +422,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
     until = at + chunk < carry ? at + chunk : carry;
   }
 
-  // shared memory: the rings (whose columns begin at multiples of 1024 bytes), queries, and the weights of a tile that is
-  // added up row by row
+  // shared memory: the rings (whose columns begin at multiples of 1024 bytes), queries, and the
+  // weights of a tile that is added up row by row
   char* const memory = memory_ + ((1024u - (shared_at(memory_) & 1023u)) & 1023u);
   char* const ring = memory + warp * a.stages * a.stage_bytes;
   float* const joined = reinterpret_cast<float*>(memory);  // [kWarps][ROWS][DIM + 4], once the rings are drained
@@ -483,7 +488,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
         p.page = table[column];
       }
     };
-    // TILED: lane l has turn l's of the 32 turns at hand, looked up together; else a lane has that of its place of the next turn
+    // TILED: lane l has turn l's of the 32 turns at hand, looked up together; else a lane has that
+    // of its place of the next turn
     Place looked_up{-1, 0};
     if (TILED) page_of(int64_t(key0) + lane * kTile, looked_up);
     else page_of(int64_t(key0) + own_place, looked_up);
@@ -621,8 +627,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
 #pragma unroll
         for (int e = 0; e < 4; ++e) c2[e] = 0.0f;
         {
-          // K: matrices (places 0-7 | 8-15) x (columns 0-7 | 8-15); Q: rows 0-7 x four times 8 columns; two steps at a time,
-          // four in a column of 128 bytes
+          // K: matrices (places 0-7 | 8-15) x (columns 0-7 | 8-15); Q: rows 0-7 x four times 8
+          // columns; two steps at a time, four in a column of 128 bytes
           uint32_t k_at = shared_at(stage) + block_at(lane & 15, lane >> 4);
           uint32_t q_at = shared_at(query + (lane & 7) * a.query_row + (lane >> 3) * 8);
 #pragma unroll 2
@@ -765,7 +771,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
           }
         }
       } else {
-        // f32: a lane has a place and half of the rows, lanes 16.. the other half; columns in order, one sum a row
+        // f32: a lane has a place and half of the rows, lanes 16.. the other half; columns in
+        // order, one sum a row
         const int place = own_place;
         const float* q = reinterpret_cast<const float*>(query) + own_row;
         uint64_t dots[(OWN + 1) / 2];  // rows in pairs
@@ -945,7 +952,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
       float top = ref_s[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ref_s[w][r]);
-      // A reference of -inf: nothing seen, or scores of -inf and NaN alone. Its factor is 0, which leaves a sum of 0 out and keeps NaN.
+      // A reference of -inf: nothing seen, or scores of -inf and NaN alone. Its factor is 0, which
+      // leaves a sum of 0 out and keeps NaN.
       float f[kWarps], all = 0.0f, st = 0.0f;
       bool seen = false;
 #pragma unroll
@@ -984,7 +992,8 @@ __global__ void __launch_bounds__(kThreads, ROWS * DIM <= 1024 ? kMaxPerSm : 2) 
   }
 }
 
-// Joins the parts of a unit's row that several blocks left, 128 columns a block; a unit without tiles has zeros.
+// Joins the parts of a unit's row that several blocks left, 128 columns a block; a unit without
+// tiles has zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
   __shared__ int32_t counted[8][2];
@@ -1107,15 +1116,15 @@ inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, b
   const bool wide = dtype == JK_F32;
   const int size = wide ? 4 : 2, column = 128 / size;
   s.dim = dim <= 64 && !wide ? 64 : dim <= 128 ? 128 : dim <= 256 ? 256 : 512;
-  // (On the device, 32 sequences of 10240 f16 nodes, rank and dim 128, 32 heads on 8: 16 rows a unit in blocks of 16 285 us, of
-  // 8 420; 32 rows in blocks of 32 432, of 16 554, of 8 830.)
-  // 128 registers of sums a thread at most (f32: 64, as it keeps a tile's values too); where rows are copied in pieces the
-  // copies are what takes time, so blocks have fewer sizes
+  // (On the device, 32 sequences of 10240 f16 nodes, rank and dim 128, 32 heads on 8: 16 rows a
+  // unit in blocks of 16 285 us, of 8 420; 32 rows in blocks of 32 432, of 16 554, of 8 830.) 128
+  // registers of sums a thread at most (f32: 64, as it keeps a tile's values too); where rows are
+  // copied in pieces the copies are what takes time, so blocks have fewer sizes
   if (wide) s.rows = unit_rows == 1 ? 1 : (tiled && unit_rows <= 4) || s.dim == 512 ? 4 : 8;
   else s.rows = !tiled || unit_rows <= 8 || s.dim == 512 ? 8 : unit_rows <= 16 || s.dim == 256 ? 16 : 32;
   s.row_blocks = static_cast<int>((unit_rows + s.rows - 1) / s.rows);
-  // columns in the products' steps (two of 16, or 4); queries of 16-bit types an odd number of 16-byte blocks apart, so that
-  // eight of them lie in different banks
+  // columns in the products' steps (two of 16, or 4); queries of 16-bit types an odd number of
+  // 16-byte blocks apart, so that eight of them lie in different banks
   s.key_cols = static_cast<int>(wide ? (rank + 3) / 4 * 4 : (rank + 31) / 32 * 32);
   s.query_row = s.key_cols + 16 / size;
   s.key_bytes = static_cast<int>((rank + column - 1) / column) * kColumn;
@@ -1130,8 +1139,8 @@ inline Shape shape_of(int64_t unit_rows, int64_t rank, int64_t dim, int dtype, b
   const int rest = s.rows * s.query_row * size + kWarps * s.rows * (wide ? 2 * kKeys : kKeys + 1) * 4;
   auto blocks = [&](int stages) { return static_cast<int>(227 * 1024 / (1024 + ring(stages) + rest + 4 * 1024)); };
   const int most = s.rows * s.dim <= 1024 ? kMaxPerSm : 2;
-  // Two stages a warp in as many blocks of an SM as fit (a third stage gained nothing in any of the cases that are measured);
-  // where not even one block has room for two, one stage.
+  // Two stages a warp in as many blocks of an SM as fit (a third stage gained nothing in any of the
+  // cases that are measured); where not even one block has room for two, one stage.
   s.stages = blocks(2) < 1 ? 1 : 2;
   s.per_sm = blocks(s.stages) < most ? blocks(s.stages) : most;
   s.ring_bytes = ring(s.stages);

@@ -1,5 +1,6 @@
-// Element types, 16-byte packs and reductions of the row kernels (layer norm, cross entropy,
-// gradient clipping). Every kernel computes in f32 or wider and rounds a result once.
+// Element types, 16-byte packs and reductions of the row kernels (layer norm, cross entropy, gradient
+// clipping) and of the generation-step kernels (propagation over a cache, its pages, verification).
+// Every kernel computes in f32 or wider and rounds a result once.
 #pragma once
 
 #include <cstdint>

@@ -6,18 +6,20 @@
 // Where all are accepted r is the target's next distribution.
 //
 // A comparison of a product or of a running sum decides a token, so both are in f64: products of two
-// f32 are exact there, and a running sum is off by less than 2^-40 + m 2^-53 of the total (m: entries that a lane adds up,
-// at most 2^18 for a few sequences and 2^23 for many), where f32 would give
-// another token in one of some thousand draws over a vocabulary of 100,000. Conversions to f64 are the
-// slowest part (16 a cycle and SM), so a difference takes one: d = x - y in f32, whose rounding error
-// (x - d) - y is exact there for x >= y >= 0, and errors are added up on their own, in f32 up to 128 of them.
+// f32 are exact there, and a running sum is off by less than 2^-40 + m 2^-53 of the total (m:
+// entries that a lane adds up, at most 2^18 for a few sequences and 2^23 for many), where f32 would
+// give another token in one of some thousand draws over a vocabulary of 100,000. Conversions to f64
+// are the slowest part (16 a cycle and SM), so a difference takes one: d = x - y in f32, whose
+// rounding error (x - d) - y is exact there for x >= y >= 0, and errors are added up on their own,
+// in f32 up to 128 of them.
 //
 // Of the draft's and the target's rows only place a's are read, once: a cluster of blocks per
 // sequence adds them up by warps, each a run of 16-byte packs; the run that holds the draw is cut
 // into runs again, one for each warp of its block, until one warp finds the token (the second look
-// at a run comes from L2). Bound: for a batch the issue of instructions (about ten an entry) and, in the end, the steps that
-// find the token: 24 us on the device for 256 sequences of 100003 bf16 entries, of which 14 for the memory; for a few sequences
-// the latency of these steps (8.6 us for one of 131072 f32 entries, 5.6 for one of 1000).
+// at a run comes from L2). Bound: for a batch the issue of instructions (14.5 an entry) and, in the end,
+// the steps that find the token: 25 us on the device for 256 sequences of 100003 bf16 entries, of which
+// 14 for the memory; for a few sequences the latency of these steps (8.6 us for one of 131072 f32
+// entries, 5.6 for one of 1000).
 #include <cooperative_groups.h>
 
 #include "jk_host.h"
@@ -116,8 +118,8 @@ struct Rest {
     }
   }
 
-  // Over packs [from, to), a warp. WORDS: apart / 4, known where the loop is compiled, as selecting words would take most of
-  // its time; 4: there is no draft.
+  // Over packs [from, to), a warp. WORDS: apart / 4, known where the loop is compiled, as selecting
+  // words would take most of its time; 4: there is no draft.
   template <int WORDS>
   __device__ __forceinline__ double sum_of(int32_t from, int32_t to) const {
     const int lane = threadIdx.x & 31;
@@ -154,7 +156,8 @@ struct Rest {
       add(x, y, s, lost);
     };
     int32_t k = low + lane;
-    // errors go over into the sum after at most 128 of them, so that their own rounding does not grow with the vocabulary
+    // errors go over into the sum after at most 128 of them, so that their own rounding does not
+    // grow with the vocabulary
     auto over = [&] {
       const float2 some = unpair(lost);
       s += static_cast<double>(some.x) + static_cast<double>(some.y);
@@ -359,10 +362,12 @@ int launch_one(const Args& g, int64_t batch, int size, cudaStream_t s) {
 
 template <typename T>
 int launch(const Args& g, int64_t batch, cudaStream_t s) {
-  // Blocks of a sequence: a power of 2, none for less than 2048 entries. Up to two sequences an SM: large blocks, of which an SM
-  // holds two, 128 at most in clusters, as clusters of 8 do not fill every SM. More sequences: small ones, whose number the SMs
-  // share out more evenly. On the device, large and small: 8.6 and 11.1 us for 1 x 131072 f32, 16 and 20 for 128 x 100003 bf16,
-  // 24 and 29 for 256 x 100003, 41 and 37 for 320 x 100003, 53 and 33 for 1000 x 20000 f32, 39 and 14 for 2000 x 1000.
+  // Blocks of a sequence: a power of 2, none for less than 2048 entries. Up to two sequences an SM:
+  // large blocks, of which an SM holds two, 128 at most in clusters, as clusters of 8 do not fill
+  // every SM. More sequences: small ones, whose number the SMs share out more evenly. On the
+  // device, large and small: 8.6 and 11.1 us for 1 x 131072 f32, 16 and 20 for 128 x 100003 bf16,
+  // 25 and 29 for 256 x 100003, 41 and 37 for 320 x 100003, 53 and 33 for 1000 x 20000 f32, 39 and
+  // 14 for 2000 x 1000.
   const bool few = batch <= 2 * kSms;
   const int64_t slots = few ? 128 : kSms * kManyPerSm;
   int size = 1;

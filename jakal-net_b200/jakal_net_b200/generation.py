@@ -503,7 +503,7 @@ def verify_draft(target: Tensor, draft: Optional[Tensor], tokens: Tensor, unifor
     Token i is accepted while uniform[i] * draft[i, token] < target[i, token]. At the first place a
     that is not accepted the new token is drawn from max(target[a] - draft[a], 0) (where that is 0
     throughout, from target[a]), after the last from target[counts]: the least whose running sum passes
-    uniform[drafted] of the total, in f64. NaN and negative values count as 0.
+    uniform[drafted] of the total, in f64. NaN and negative values count as 0 (infinite ones leave the new token open).
 
     Returns (out int64 [batch, drafted + 1]: the accepted tokens, the new one, -1 behind it (and in its
     place where there is nothing to draw from); accepted int32 [batch]: a)."""
