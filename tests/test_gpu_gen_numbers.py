@@ -259,3 +259,20 @@ def test_infinite_values_with_many_rows(jk, dtype, page, new, group, dim, column
     for _ in range(2):
         graph.replay()
         assert torch.equal(again[0], state) and torch.equal(again[1].nan_to_num(), value.nan_to_num())
+
+
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("group", [1, 9])
+def test_sums_that_pass_the_range_are_not_taken_for_numbers(jk, page, group):
+    """Values of both signs next to the end of bf16's range, whose sums pass it before they are divided: what comes out is
+    right (an f32 sum's rounding of 256 terms and the result's) or not finite."""
+    n, dtype = 256, torch.bfloat16
+    p = problem(dtype, [n], heads=group, rank=16, dim=24, page=page)
+    p["query"].zero_()
+    at, off = places(p, 0, n)
+    big = torch.where(torch.arange(n, device="cuda") < 160, 3e38, -3e38).to(dtype)
+    p["value_pages"][at, 0, off, 5] = big
+    want = big.double().mean()
+    got = jk.cached_propagation(**p)[0, 0, :, 5].double()
+    assert (~got.isfinite() | ((got - want).abs() <= (2.0 ** -8 + 256 * 2.0 ** -23) * 3e38)).all()
+    assert jk.cached_propagation(**p)[..., :5].isfinite().all()
